@@ -21,6 +21,7 @@ DIAG_HEADER_PATH = os.path.join(os.path.dirname(PKG_DIR), "include", "fuselse_am
 _vp = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _int = ctypes.c_int
+_float = ctypes.c_float
 
 # name -> (restype, argtypes); must match include/fuselse_amd.h
 SIGNATURES = {
@@ -63,6 +64,20 @@ SIGNATURES = {
                                      _i64, _vp, _vp, _vp, _vp]),
     "fl_sparse_blocked_grad": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _int, _int, _int, _vp,
                                       _vp, _i64, _vp, _vp, _vp, _vp]),
+    "fl_linear_ce_workspace_bytes": (ctypes.c_size_t, [_i64, _i64, _i64, _int, _int]),
+    "fl_linear_ce_fwd": (_int, [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _int, _i64, _float, _int, _vp, _vp, _vp,
+                                ctypes.c_size_t, _vp]),
+    "fl_linear_ce_bwd": (_int, [_vp, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _int, _i64, _float, _int, _vp,
+                                _vp, _vp, ctypes.c_size_t, _vp]),
+    "fl_distill_workspace_bytes": (ctypes.c_size_t, [_i64, _i64, _int]),
+    "fl_distill_fwd": (_int, [_vp, _i64, _i64, _i64, _i64, _i64, _int, _vp, _int, _vp, _i64, _float, _int, _vp, _vp,
+                              _vp, _vp, _vp, ctypes.c_size_t, _vp]),
+    "fl_distill_bwd": (_int, [_vp, _int, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _int, _vp, _int, _vp, _i64, _float,
+                              _vp, _vp, _vp, _vp]),
+    "fl_router_workspace_bytes": (ctypes.c_size_t, [_i64, _i64, _int]),
+    "fl_router_balance_fwd": (_int, [_vp, _i64, _i64, _i64, _int, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+                                     ctypes.c_size_t, _vp]),
+    "fl_router_balance_bwd": (_int, [_vp, _vp, _vp, _i64, _i64, _i64, _int, _vp, _vp, _vp, _vp, _vp]),
 }
 
 # the measurement library (include/fuselse_amd_diag.h)

@@ -1,0 +1,431 @@
+// Distillation from a teacher's top logits on gfx950.
+//
+//   p_k = softmax over the K teacher logits t_k / T of a row,
+//   q_v = softmax over the V student logits s_v / T,
+//   loss = T^2 sum_k p_k (log p_k - log q_{i_k}),
+//   ds_v = g T (q_v - sum_{k: i_k = v} p_k).
+//
+// Forward: one pass over the student's row (running maximum and sum), K
+// gathers.  Backward: one read and one write of the row.  Both are bound by
+// memory; no product, no matrix cores.  Entries whose teacher logit is -inf
+// are unused, whatever their index; a row without any other has loss and
+// gradient 0.  A used index outside [0, V) makes the row's loss and gradient
+// NaN.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "../../include/fuselse_amd.h"
+#include "fl_status.hpp"
+#include "row_stream.hpp"
+
+namespace fl {
+namespace distill {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMaxTop = 1024;
+
+// ---------------------------------------------------------------------------
+// Forward
+// ---------------------------------------------------------------------------
+struct FwdArgs {
+    const void* x;
+    RowMap map;
+    const void* t;
+    const int64_t* index;
+    int64_t rows, v;
+    int k;
+    float inv_t, t2;
+    int segs;
+    int64_t seg_len;   // a multiple of the vector's elements
+    float2* part;      // [row][segs] when segs > 1
+    float* loss;
+    float* lse;
+    float* tlse;
+};
+
+// Joins the teacher's side of a row, in one wave: its log-sum-exp over
+// t_k / T and the loss.  Returns tlse: -inf for a row without a used entry,
+// NaN where a used index is out of range.
+template <typename T, typename TT>
+__device__ __forceinline__ void finish_row(const FwdArgs& p, int64_t r, float lse) {
+    const int lane = lane_id();
+    const TT* t = static_cast<const TT*>(p.t) + r * p.k;
+    const int64_t* index = p.index + r * p.k;
+    const T* x = static_cast<const T*>(p.x) + p.map.offset(r);
+    float m = -kInf, s = 0.0f;
+    for (int k = lane; k < p.k; k += 64) {
+        float v[1] = {Elem<TT>::scalar(t + k) * p.inv_t};
+        lse_fold<true>(m, s, v);
+    }
+    group_merge<64>(m, s);
+    float tlse = lse_finish<true>(m, s);
+    if (tlse == kInf) tlse = __builtin_nanf("");  // a softmax of +inf
+    float loss = 0.0f;
+    if (m != -kInf || s != 0.0f) {  // a NaN never enters m, but makes s NaN
+        bool bad = false;
+        for (int k = lane; k < p.k; k += 64) {
+            const float tv = Elem<TT>::scalar(t + k) * p.inv_t;
+            if (tv == -kInf) continue;
+            const int64_t i = index[k];
+            if (i < 0 || i >= p.v) {
+                bad = true;
+                continue;
+            }
+            const float logp = tv - tlse;
+            const float prob = fexp2(logp * kLog2e);
+            // a probability that underflows to 0 contributes 0
+            if (prob != 0.0f) loss += prob * (logp - (Elem<T>::scalar(x + i) * p.inv_t - lse));
+        }
+        loss += reduce_partner<1>(loss);
+        loss += reduce_partner<2>(loss);
+        loss += reduce_partner<4>(loss);
+        loss += reduce_partner<8>(loss);
+        loss += reduce_partner<16>(loss);
+        loss += reduce_partner<32>(loss);
+        loss *= p.t2;
+        if (__ballot(bad)) loss = tlse = __builtin_nanf("");
+    }
+    if (lane == 0) {
+        p.loss[r] = loss;
+        p.lse[r] = lse;
+        p.tlse[r] = tlse;
+    }
+}
+
+template <typename T, typename TT>
+__global__ __launch_bounds__(kThreads) void fwd_rows(FwdArgs p) {
+    constexpr int VE = Elem<T>::kVec, U = 4;
+    const int64_t r = blockIdx.x / p.segs;
+    const int seg = blockIdx.x % p.segs;
+    const T* x = static_cast<const T*>(p.x) + p.map.offset(r);
+    const int64_t e0 = seg * p.seg_len;
+    const int64_t e1 = e0 + p.seg_len < p.v ? e0 + p.seg_len : p.v;
+    float m = -kInf, s = 0.0f;
+    int64_t e = e0 + (int64_t)threadIdx.x * VE;
+    constexpr int64_t step = (int64_t)kThreads * VE;
+    for (; e + (U - 1) * step + VE <= e1; e += U * step) {
+        u32x4 raw[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) __builtin_memcpy(&raw[u], x + e + u * step, 16);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            float v[VE];
+            Elem<T>::cvt(raw[u], v);
+#pragma unroll
+            for (int k = 0; k < VE; ++k) v[k] *= p.inv_t;
+            lse_fold<true>(m, s, v);
+        }
+    }
+    for (; e < e1; e += step) {
+        float v[VE];
+        load_vec_part<T>(x + e, e1 - e, -kInf, v);
+#pragma unroll
+        for (int k = 0; k < VE; ++k) v[k] *= p.inv_t;
+        lse_fold<true>(m, s, v);
+    }
+    group_merge<64>(m, s);
+    __shared__ float sm[kThreads / 64], ss[kThreads / 64];
+    if (lane_id() == 0) {
+        sm[threadIdx.x >> 6] = m;
+        ss[threadIdx.x >> 6] = s;
+    }
+    __syncthreads();
+    if (threadIdx.x >= 64) return;
+    m = sm[0];
+    s = ss[0];
+#pragma unroll
+    for (int w = 1; w < kThreads / 64; ++w) lse_merge(m, s, sm[w], ss[w]);
+    if (p.segs == 1) {
+        finish_row<T, TT>(p, r, lse_finish<true>(m, s));
+    } else if (threadIdx.x == 0) {
+        p.part[r * p.segs + seg] = make_float2(m, s);
+    }
+}
+
+template <typename T, typename TT>
+__global__ __launch_bounds__(64) void fwd_finish(FwdArgs p) {
+    const int64_t r = blockIdx.x;
+    float m = -kInf, s = 0.0f;
+    for (int k = threadIdx.x; k < p.segs; k += 64) {
+        const float2 q = p.part[r * p.segs + k];
+        lse_merge(m, s, q.x, q.y);
+    }
+    group_merge<64>(m, s);
+    finish_row<T, TT>(p, r, lse_finish<true>(m, s));
+}
+
+// Sum of the rows' losses in a fixed order; the mean is over the rows that
+// have a teacher.  norm receives what the backward multiplies by.
+__global__ __launch_bounds__(1024) void reduce_rows(const float* rows, const float* tlse, int64_t n, int mean,
+                                                    float* out, float* norm) {
+    __shared__ double sh[1024];
+    __shared__ int shn[1024];
+    double s = 0.0;
+    int live = 0;
+    for (int64_t r = threadIdx.x; r < n; r += 1024) {
+        s += rows[r];
+        live += tlse[r] != -kInf;
+    }
+    sh[threadIdx.x] = s;
+    shn[threadIdx.x] = live;
+    __syncthreads();
+    for (int d = 512; d > 0; d >>= 1) {
+        if ((int)threadIdx.x < d) {
+            sh[threadIdx.x] += sh[threadIdx.x + d];
+            shn[threadIdx.x] += shn[threadIdx.x + d];
+        }
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) {
+        const double by = mean ? 1.0 / (shn[0] > 0 ? shn[0] : 1) : 1.0;
+        *out = (float)(sh[0] * by);
+        *norm = (float)by;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Backward: a block per chunk of a row.
+// ---------------------------------------------------------------------------
+struct BwdArgs {
+    const float* grad;
+    int grad_stride;
+    const float* norm;
+    const void* x;
+    RowMap map;
+    const void* t;
+    const int64_t* index;
+    const float* lse;
+    const float* tlse;
+    int64_t rows, v;
+    int k;
+    float inv_t, temp;
+    int chunks;
+    int64_t block0;
+    void* dx;
+};
+
+constexpr int kBwdVecs = 8;  // vectors a thread
+
+template <typename T, typename TT>
+__global__ __launch_bounds__(kThreads) void bwd_rows(BwdArgs p) {
+    constexpr int VE = Elem<T>::kVec;
+    constexpr int64_t chunk = (int64_t)kThreads * VE * kBwdVecs;
+    __shared__ int li[kMaxTop];
+    __shared__ float lp[kMaxTop];
+    __shared__ int ln;
+    const int64_t block = p.block0 + blockIdx.x;
+    const int64_t r = block / p.chunks;
+    const int c = (int)(block % p.chunks);
+    const T* x = static_cast<const T*>(p.x) + p.map.offset(r);
+    T* dx = static_cast<T*>(p.dx) + r * p.v;
+    const int64_t e0 = c * chunk;
+    const int len = (int)(p.v - e0 < chunk ? p.v - e0 : chunk);
+    const float tlse = p.tlse[r];
+    const bool dead = tlse == -kInf;
+    const float g = dead ? 0.0f : p.grad[r * p.grad_stride] * p.temp * (p.norm ? *p.norm : 1.0f);
+    const float lse = p.lse[r];
+    // the teacher's entries of this chunk, in order, found by one wave
+    if (threadIdx.x < 64) {
+        int n = 0;
+        for (int k0 = 0; !dead && k0 < p.k; k0 += 64) {
+            const int k = k0 + (int)threadIdx.x;
+            int64_t i = -1;
+            float tv = -kInf;
+            if (k < p.k) {
+                i = p.index[r * p.k + k] - e0;
+                tv = Elem<TT>::scalar(static_cast<const TT*>(p.t) + r * p.k + k) * p.inv_t;
+            }
+            const bool mine = tv != -kInf && i >= 0 && i < len;
+            const uint64_t b = __ballot(mine);
+            if (mine) {
+                const int at = n + __popcll(b & ((1ull << threadIdx.x) - 1));
+                li[at] = (int)i;
+                lp[at] = g * fexp2((tv - tlse) * kLog2e);
+            }
+            n += __popcll(b);
+        }
+        if (threadIdx.x == 0) ln = n;
+    }
+    __syncthreads();
+    const float gq = tlse != tlse ? __builtin_nanf("") : g;
+#pragma unroll
+    for (int u = 0; u < kBwdVecs; ++u) {
+        const int e = (u * kThreads + (int)threadIdx.x) * VE;
+        if (e >= len) continue;
+        float v[VE];
+        if (!dead) {
+            load_vec_part<T>(x + e0 + e, len - e, 0.0f, v);
+#pragma unroll
+            for (int k = 0; k < VE; ++k) v[k] = gq * fexp2((v[k] * p.inv_t - lse) * kLog2e);
+        } else {
+#pragma unroll
+            for (int k = 0; k < VE; ++k) v[k] = 0.0f;
+        }
+#pragma unroll
+        for (int k = 0; k < VE; ++k)
+            if (e + k < len) Elem<T>::put(dx + e0 + e + k, v[k]);
+    }
+    // An entry's element is written again by the thread that wrote its vector
+    // (one thread's stores to an address keep their order), with the sum of
+    // all entries of that index.
+    for (int j = 0; j < ln; ++j) {
+        const int i = li[j];
+        if ((i / VE) % kThreads != (int)threadIdx.x) continue;
+        float take = 0.0f;
+        for (int k = 0; k < ln; ++k) take += li[k] == i ? lp[k] : 0.0f;
+        const float q = gq * fexp2((Elem<T>::scalar(x + e0 + i) * p.inv_t - lse) * kLog2e);
+        Elem<T>::put(dx + e0 + i, q - take);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+int elem_size(int dtype) { return dtype == 0 ? 4 : 2; }
+
+// Segments a row is cut into in the forward: enough blocks for the chip, none
+// shorter than 16 KB.
+int segments(int64_t rows, int64_t v, int dtype) {
+    const int64_t most = v * elem_size(dtype) / 16384;
+    int64_t want = rows > 0 ? (1024 + rows - 1) / rows : 1;
+    if (want > most) want = most;
+    if (want > 64) want = 64;
+    return want < 1 ? 1 : (int)want;
+}
+
+struct Ws {
+    int64_t part, rows, bytes;
+};
+Ws ws_layout(int64_t rows, int64_t v, int dtype) {
+    Ws w{};
+    const int segs = segments(rows, v, dtype);
+    w.part = 0;
+    w.rows = segs > 1 ? (rows * segs * 8 + 255) / 256 * 256 : 0;
+    w.bytes = w.rows + rows * 4;
+    return w;
+}
+
+template <typename T, typename TT>
+void launch_fwd(const FwdArgs& a, hipStream_t s) {
+    fwd_rows<T, TT><<<dim3((unsigned)(a.rows * a.segs)), kThreads, 0, s>>>(a);
+    if (a.segs > 1) fwd_finish<T, TT><<<dim3((unsigned)a.rows), 64, 0, s>>>(a);
+}
+
+template <typename T, typename TT>
+void launch_bwd(const BwdArgs& a, hipStream_t s) {
+    BwdArgs b = a;
+    constexpr int64_t chunk = (int64_t)kThreads * Elem<T>::kVec * kBwdVecs;
+    b.chunks = (int)((a.v + chunk - 1) / chunk);
+    for_grid_chunks(a.rows * b.chunks, kThreads, [&](int64_t first, int64_t count) {
+        b.block0 = first;
+        bwd_rows<T, TT><<<dim3((unsigned)count), kThreads, 0, s>>>(b);
+    });
+}
+
+// Calls f(T{}, TT{}) for the student's and the teacher's element types.
+template <typename F>
+void by_types(int dtype, int tdtype, F f) {
+    auto inner = [&](auto t) {
+        if (tdtype == 0) f(t, float{});
+        else if (tdtype == 1) f(t, _Float16{});
+        else f(t, bf16_t{});
+    };
+    if (dtype == 0) inner(float{});
+    else if (dtype == 1) inner(_Float16{});
+    else inner(bf16_t{});
+}
+
+int check(const char* name, int64_t rows, int64_t n1, int64_t v, int64_t k, int dtype, int tdtype, float temp) {
+    FL_CHECK(rows >= 0 && v >= 1 && k >= 0 && n1 >= 1, "%s: bad shape (rows=%lld, V=%lld, K=%lld)", name,
+             (long long)rows, (long long)v, (long long)k);
+    FL_CHECK(dtype >= 0 && dtype <= 2 && tdtype >= 0 && tdtype <= 2, "%s: dtype %d, %d", name, dtype, tdtype);
+    FL_CHECK(temp > 0.0f && __builtin_isfinite(temp), "%s: temperature must be positive and finite", name);
+    if (k > kMaxTop) return set_error(FL_ERANGE, "%s: at most %d teacher logits a row", name, kMaxTop);
+    if (rows > (1 << 22) || v > (1 << 28)) return set_error(FL_ERANGE, "%s: at most 2^22 rows of 2^28 columns", name);
+    return ok();
+}
+
+}  // namespace
+}  // namespace distill
+}  // namespace fl
+
+using namespace fl;
+using namespace fl::distill;
+
+extern "C" size_t fl_distill_workspace_bytes(int64_t rows, int64_t V, int dtype) {
+    if (rows < 1 || V < 1) return 0;
+    return (size_t)ws_layout(rows, V, dtype).bytes;
+}
+
+extern "C" int fl_distill_fwd(const void* logits, int64_t rows, int64_t slice_rows, int64_t slice_stride,
+                              int64_t row_stride, int64_t V, int dtype, const void* teacher, int teacher_dtype,
+                              const int64_t* index, int64_t K, float temperature, int reduction, float* loss,
+                              float* lse, float* teacher_lse, float* norm, void* workspace, size_t workspace_bytes,
+                              void* stream) {
+    const char* name = "fl_distill_fwd";
+    const int rc = check(name, rows, slice_rows, V, K, dtype, teacher_dtype, temperature);
+    if (rc != FL_OK || rows == 0) return rc;
+    FL_CHECK(reduction >= 0 && reduction <= 2, "%s: reduction %d", name, reduction);
+    FL_CHECK(logits && loss && lse && teacher_lse && (K == 0 || (teacher && index)) && (reduction == 0 || norm),
+             "%s: NULL pointer argument", name);
+    const Ws w = ws_layout(rows, V, dtype);
+    FL_CHECK((int64_t)workspace_bytes >= w.bytes, "%s: workspace of %llu bytes, %lld needed", name,
+             (unsigned long long)workspace_bytes, (long long)w.bytes);
+    FL_CHECK(workspace && (reinterpret_cast<uintptr_t>(workspace) & 7u) == 0, "%s: workspace is not 8-byte aligned",
+             name);
+    char* ws = static_cast<char*>(workspace);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    FwdArgs a{};
+    a.x = logits;
+    a.map = RowMap{slice_rows, slice_stride, row_stride};
+    a.t = teacher;
+    a.index = index;
+    a.rows = rows;
+    a.v = V;
+    a.k = (int)K;
+    a.inv_t = 1.0f / temperature;
+    a.t2 = temperature * temperature;
+    a.segs = segments(rows, V, dtype);
+    const int64_t ve = 16 / elem_size(dtype);
+    a.seg_len = ((V + a.segs - 1) / a.segs + ve - 1) / ve * ve;
+    a.part = reinterpret_cast<float2*>(ws + w.part);
+    a.loss = reduction == 0 ? loss : reinterpret_cast<float*>(ws + w.rows);
+    a.lse = lse;
+    a.tlse = teacher_lse;
+    by_types(dtype, teacher_dtype, [&](auto t, auto tt) { launch_fwd<decltype(t), decltype(tt)>(a, s); });
+    if (reduction != 0) reduce_rows<<<1, 1024, 0, s>>>(a.loss, teacher_lse, rows, reduction == 2, loss, norm);
+    return launch_status(name);
+}
+
+extern "C" int fl_distill_bwd(const float* grad, int grad_stride, const float* norm, const void* logits, int64_t rows,
+                              int64_t slice_rows, int64_t slice_stride, int64_t row_stride, int64_t V, int dtype,
+                              const void* teacher, int teacher_dtype, const int64_t* index, int64_t K,
+                              float temperature, const float* lse, const float* teacher_lse, void* grad_logits,
+                              void* stream) {
+    const char* name = "fl_distill_bwd";
+    const int rc = check(name, rows, slice_rows, V, K, dtype, teacher_dtype, temperature);
+    if (rc != FL_OK || rows == 0) return rc;
+    FL_CHECK(grad_stride == 0 || grad_stride == 1, "%s: grad_stride %d", name, grad_stride);
+    FL_CHECK(grad && logits && lse && teacher_lse && grad_logits && (K == 0 || (teacher && index)),
+             "%s: NULL pointer argument", name);
+    BwdArgs a{};
+    a.grad = grad;
+    a.grad_stride = grad_stride;
+    a.norm = norm;
+    a.x = logits;
+    a.map = RowMap{slice_rows, slice_stride, row_stride};
+    a.t = teacher;
+    a.index = index;
+    a.lse = lse;
+    a.tlse = teacher_lse;
+    a.rows = rows;
+    a.v = V;
+    a.k = (int)K;
+    a.inv_t = 1.0f / temperature;
+    a.temp = temperature;
+    a.dx = grad_logits;
+    by_types(dtype, teacher_dtype,
+             [&](auto t, auto tt) { launch_bwd<decltype(t), decltype(tt)>(a, static_cast<hipStream_t>(stream)); });
+    return launch_status(name);
+}

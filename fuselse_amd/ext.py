@@ -857,3 +857,240 @@ def _launch_csr_bwd(child, out, grad_out, logparams, csc_off, csc_edge, csc_node
             _lib.call("fl_sparse_csr_bwd", *args, batch, _stream(child))
         else:
             _lib.call("fl_sparse_csr_bwd_ws", *args, nnz, batch, ws.data_ptr(), nbytes, _stream(child))
+
+
+# ---------------------------------------------------------------------------
+# Training losses (no reference counterpart)
+# ---------------------------------------------------------------------------
+_DTYPE_CODE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_REDUCTION_CODE = {"none": 0, "sum": 1, "mean": 2}
+
+
+def _reduction(name: str) -> int:
+    code = _REDUCTION_CODE.get(name)
+    _check(code is not None, "reduction must be 'none', 'sum' or 'mean'")
+    return code
+
+
+def _check_linear(x, weight, target):
+    _check(x.is_cuda, "x must be CUDA")
+    _check(weight.is_cuda, "weight must be CUDA")
+    _check(target.is_cuda, "target must be CUDA")
+    _check(x.dtype in _DTYPE_CODE, "x must be float32, float16 or bfloat16")
+    _check(weight.dtype == x.dtype, "weight must have x's dtype")
+    _check(target.dtype == torch.int64, "target must be int64")
+    _check(x.dim() == 2, "x must be 2D (N, D)")
+    _check(weight.dim() == 2 and weight.shape[1] == x.shape[1], "weight must be 2D (V, D)")
+    _check(weight.shape[0] >= 1 and weight.shape[1] >= 1, "weight must not be empty")
+    _check(target.dim() == 1 and target.shape[0] == x.shape[0], "target must be 1D (N)")
+    _check(target.is_contiguous(), "target must be contiguous")
+    # a tensor of one row may carry any row stride
+    for t, nm in ((x, "x"), (weight, "weight")):
+        _check((t.stride(1) == 1 or t.shape[1] == 1) and (t.stride(0) >= t.shape[1] or t.shape[0] <= 1),
+               f"{nm} must have contiguous rows that do not overlap")
+    _check_device(x, "x", weight=weight, target=target)
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    return max(t.stride(0), t.shape[1])
+
+
+def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, ignore_index: int = -100,
+                         reduction: str = "mean", z_loss: float = 0.0):
+    """Softmax cross entropy of the logits x @ weight.T, which are never
+    stored: (loss, lse) in fp32, with lse [N] for the backward.  x (N, D) and
+    weight (V, D) fp32, fp16 or bf16 with contiguous rows, target int64 (N,).
+    loss[n] = lse[n] - x[n] . weight[target[n]] + z_loss * lse[n]^2; rows whose
+    target is ignore_index have loss 0 and are not read."""
+    _check_linear(x, weight, target)
+    red = _reduction(reduction)
+    N, D = x.shape
+    V = weight.shape[0]
+    lse = torch.empty((N,), dtype=torch.float32, device=x.device)
+    loss = torch.empty((N,) if red == 0 else (), dtype=torch.float32, device=x.device)
+    if N == 0:
+        return loss.zero_(), lse
+    dt = _DTYPE_CODE[x.dtype]
+    with _on_device(x):
+        nbytes = _lib.load().fl_linear_ce_workspace_bytes(N, V, D, dt, 0)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        _lib.call("fl_linear_ce_fwd", x.data_ptr(), _row_stride(x), weight.data_ptr(), _row_stride(weight),
+                  target.data_ptr(), N, V, D, dt, ignore_index, z_loss, red, loss.data_ptr(), lse.data_ptr(),
+                  ws.data_ptr(), nbytes, _stream(x))
+    return loss, lse
+
+
+def linear_cross_entropy_backward(grad_output: torch.Tensor, x: torch.Tensor, weight: torch.Tensor,
+                                  target: torch.Tensor, lse: torch.Tensor, ignore_index: int = -100,
+                                  reduction: str = "mean", z_loss: float = 0.0, need_x: bool = True,
+                                  need_weight: bool = True):
+    """Gradients (of x, of weight) of linear_cross_entropy, None for one that
+    is not needed; grad_output fp32, (N,) with reduction "none" and a scalar
+    otherwise."""
+    _check_linear(x, weight, target)
+    red = _reduction(reduction)
+    N, D = x.shape
+    V = weight.shape[0]
+    for t, nm in ((grad_output, "grad_output"), (lse, "lse")):
+        _check(t.is_cuda and t.dtype == torch.float32 and t.is_contiguous(), f"{nm} must be contiguous CUDA float32")
+    _check(lse.dim() == 1 and lse.shape[0] == N, "lse must be 1D (N)")
+    _check(grad_output.numel() == (N if red == 0 else 1), "grad_output must have the loss's shape")
+    _check_device(x, "x", grad_output=grad_output, lse=lse)
+    dx = torch.empty((N, D), dtype=x.dtype, device=x.device) if need_x else None
+    dw = torch.empty((V, D), dtype=x.dtype, device=x.device) if need_weight else None
+    if N == 0:
+        return dx, dw.zero_() if need_weight else None
+    if not (need_x or need_weight):
+        return None, None
+    dt = _DTYPE_CODE[x.dtype]
+    with _on_device(x):
+        nbytes = _lib.load().fl_linear_ce_workspace_bytes(N, V, D, dt, 1)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        _lib.call("fl_linear_ce_bwd", grad_output.data_ptr(), x.data_ptr(), _row_stride(x), weight.data_ptr(),
+                  _row_stride(weight), target.data_ptr(), lse.data_ptr(), N, V, D, dt, ignore_index, z_loss, red,
+                  dx.data_ptr() if need_x else None, dw.data_ptr() if need_weight else None, ws.data_ptr(), nbytes,
+                  _stream(x))
+    return dx, dw
+
+
+def _distill_rows(logits: torch.Tensor):
+    """(rows, rows per slice, elements between slices, elements between rows)
+    of 2-D or 3-D logits whose last dimension is contiguous."""
+    V = logits.shape[-1]
+    if logits.dim() == 2:
+        return logits.shape[0], max(1, logits.shape[0]), 0, logits.stride(0)
+    n0, n1, _ = logits.shape
+    return n0 * n1, max(1, n1), logits.stride(0), logits.stride(1)
+
+
+def _check_distill(logits, teacher, index):
+    _check(logits.is_cuda, "logits must be CUDA")
+    _check(teacher.is_cuda, "teacher must be CUDA")
+    _check(index.is_cuda, "index must be CUDA")
+    _check(logits.dtype in _DTYPE_CODE, "logits must be float32, float16 or bfloat16")
+    _check(teacher.dtype in _DTYPE_CODE, "teacher must be float32, float16 or bfloat16")
+    _check(index.dtype == torch.int64, "index must be int64")
+    _check(logits.dim() in (2, 3), "logits must be 2D (rows, V) or 3D (batch, rows, V)")
+    _check(logits.shape[-1] >= 1, "logits must have at least one column")
+    _check(logits.stride(-1) == 1 or logits.shape[-1] == 1, "logits must hold contiguous rows")
+    _check(teacher.dim() == logits.dim() and teacher.shape[:-1] == logits.shape[:-1],
+           "teacher must be (..., K) with the rows of logits")
+    _check(index.shape == teacher.shape, "index must have teacher's shape")
+    _check(teacher.is_contiguous() and index.is_contiguous(), "teacher and index must be contiguous")
+    _check_device(logits, "logits", teacher=teacher, index=index)
+
+
+def topk_distillation(logits: torch.Tensor, teacher: torch.Tensor, index: torch.Tensor, temperature: float = 1.0,
+                      reduction: str = "mean"):
+    """Distillation from a teacher's top-K logits: (loss, lse, teacher_lse,
+    norm), the last three for the backward.  logits (rows, V) or
+    (batch, rows, V) fp32, fp16 or bf16 with contiguous rows, teacher (.., K)
+    of any of these types, index int64 (.., K).
+    loss = temperature^2 * KL(softmax(teacher / temperature) over the K entries
+    || softmax(logits / temperature)); teacher entries of -inf are unused, a row
+    without any other has loss 0 and is left out of the mean."""
+    _check_distill(logits, teacher, index)
+    red = _reduction(reduction)
+    rows, slice_rows, s0, s1 = _distill_rows(logits)
+    V, K = logits.shape[-1], teacher.shape[-1]
+    dev = logits.device
+    loss = torch.empty(logits.shape[:-1] if red == 0 else (), dtype=torch.float32, device=dev)
+    stats = torch.empty((2 * rows + 1,), dtype=torch.float32, device=dev)
+    lse, tlse, norm = stats[:rows], stats[rows:2 * rows], (stats[2 * rows:] if red else None)
+    if rows == 0:
+        return loss.zero_(), lse, tlse, norm
+    dt = _DTYPE_CODE[logits.dtype]
+    with _on_device(logits):
+        nbytes = _lib.load().fl_distill_workspace_bytes(rows, V, dt)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        _lib.call("fl_distill_fwd", logits.data_ptr(), rows, slice_rows, s0, s1, V, dt, teacher.data_ptr(),
+                  _DTYPE_CODE[teacher.dtype], index.data_ptr(), K, temperature, red, loss.data_ptr(), lse.data_ptr(),
+                  tlse.data_ptr(), norm.data_ptr() if red else None, ws.data_ptr(), nbytes, _stream(logits))
+    return loss, lse, tlse, norm
+
+
+def topk_distillation_backward(grad_output: torch.Tensor, logits: torch.Tensor, teacher: torch.Tensor,
+                               index: torch.Tensor, lse: torch.Tensor, teacher_lse: torch.Tensor, norm,
+                               temperature: float = 1.0) -> torch.Tensor:
+    """Gradient of the logits, contiguous and of their type; grad_output fp32
+    with one element per row, or one in all."""
+    _check_distill(logits, teacher, index)
+    rows, slice_rows, s0, s1 = _distill_rows(logits)
+    V, K = logits.shape[-1], teacher.shape[-1]
+    _check(grad_output.is_cuda and grad_output.dtype == torch.float32 and grad_output.is_contiguous(),
+           "grad_output must be contiguous CUDA float32")
+    _check(grad_output.numel() in (1, rows), "grad_output must have one element, or one per row")
+    for t, nm, n in ((lse, "lse", rows), (teacher_lse, "teacher_lse", rows), (norm, "norm", 1)):
+        _check(t is None and nm == "norm" or (t.is_cuda and t.dtype == torch.float32 and t.is_contiguous()
+                                              and t.numel() == n), f"{nm} must be contiguous CUDA float32 of {n}")
+    _check_device(logits, "logits", grad_output=grad_output, lse=lse, teacher_lse=teacher_lse, norm=norm)
+    grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    if rows == 0:
+        return grad
+    with _on_device(logits):
+        _lib.call("fl_distill_bwd", grad_output.data_ptr(), 0 if grad_output.numel() == 1 else 1,
+                  norm.data_ptr() if norm is not None else None, logits.data_ptr(), rows, slice_rows, s0, s1, V,
+                  _DTYPE_CODE[logits.dtype], teacher.data_ptr(), _DTYPE_CODE[teacher.dtype], index.data_ptr(), K,
+                  temperature, lse.data_ptr(), teacher_lse.data_ptr(), grad.data_ptr(), _stream(logits))
+    return grad
+
+
+def _check_router(logits, mask):
+    _check(logits.is_cuda, "logits must be CUDA")
+    _check(logits.dtype in _DTYPE_CODE, "logits must be float32, float16 or bfloat16")
+    _check(logits.dim() == 2 and logits.shape[1] >= 1, "logits must be 2D (tokens, experts)")
+    _check((logits.stride(1) == 1 or logits.shape[1] == 1)
+           and (logits.stride(0) >= logits.shape[1] or logits.shape[0] <= 1),
+           "logits must have contiguous rows that do not overlap")
+    if mask is not None:
+        _check(mask.is_cuda and mask.dtype == torch.bool and mask.is_contiguous() and mask.dim() == 1
+               and mask.shape[0] == logits.shape[0], "mask must be a contiguous CUDA bool tensor (tokens,)")
+        _check_device(logits, "logits", mask=mask)
+
+
+def router_balance(logits: torch.Tensor, index: torch.Tensor, mask: Optional[torch.Tensor] = None):
+    """Balance loss, z loss and per-expert counts of a router: (balance, z,
+    counts, lse, coef), the last two for the backward.  logits
+    (tokens, experts) fp32, fp16 or bf16 with contiguous rows, index int64
+    (tokens, top) the chosen experts, mask bool (tokens,) the tokens that take
+    part (None: all)."""
+    _check_router(logits, mask)
+    T, E = logits.shape
+    _check(index.is_cuda and index.dtype == torch.int64 and index.is_contiguous() and index.dim() == 2
+           and index.shape[0] == T, "index must be a contiguous CUDA int64 tensor (tokens, top)")
+    _check_device(logits, "logits", index=index)
+    dev = logits.device
+    balance = torch.empty((), dtype=torch.float32, device=dev)
+    z = torch.empty((), dtype=torch.float32, device=dev)
+    counts = torch.empty((E,), dtype=torch.int64, device=dev)
+    stats = torch.empty((T + E + 1,), dtype=torch.float32, device=dev)
+    lse, coef = stats[:T], stats[T:]
+    dt = _DTYPE_CODE[logits.dtype]
+    with _on_device(logits):
+        nbytes = _lib.load().fl_router_workspace_bytes(T, E, dt)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        _lib.call("fl_router_balance_fwd", logits.data_ptr(), _row_stride(logits), T, E, dt, index.data_ptr(),
+                  index.shape[1], mask.data_ptr() if mask is not None else None, balance.data_ptr(), z.data_ptr(),
+                  counts.data_ptr(), lse.data_ptr(), coef.data_ptr(), ws.data_ptr(), nbytes, _stream(logits))
+    return balance, z, counts, lse, coef
+
+
+def router_balance_backward(grad_balance, grad_z, logits: torch.Tensor, mask, lse: torch.Tensor,
+                            coef: torch.Tensor) -> torch.Tensor:
+    """Gradient of the router's logits, contiguous and of their type;
+    grad_balance and grad_z fp32 scalars or None."""
+    _check_router(logits, mask)
+    T, E = logits.shape
+    for t, nm, n in ((grad_balance, "grad_balance", 1), (grad_z, "grad_z", 1), (lse, "lse", T), (coef, "coef", E + 1)):
+        _check(t is None and nm in ("grad_balance", "grad_z") or (t.is_cuda and t.dtype == torch.float32
+               and t.is_contiguous() and t.numel() == n), f"{nm} must be contiguous CUDA float32 of {n}")
+    _check_device(logits, "logits", grad_balance=grad_balance, grad_z=grad_z, lse=lse, coef=coef)
+    grad = torch.empty((T, E), dtype=logits.dtype, device=logits.device)
+    if T == 0:
+        return grad
+    with _on_device(logits):
+        _lib.call("fl_router_balance_bwd", grad_balance.data_ptr() if grad_balance is not None else None,
+                  grad_z.data_ptr() if grad_z is not None else None, logits.data_ptr(), _row_stride(logits), T, E,
+                  _DTYPE_CODE[logits.dtype], mask.data_ptr() if mask is not None else None, lse.data_ptr(),
+                  coef.data_ptr(), grad.data_ptr(), _stream(logits))
+    return grad

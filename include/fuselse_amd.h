@@ -328,6 +328,105 @@ int fl_sparse_blocked_grad(const float* node_flows, const float* node_mars, cons
                            const int32_t* csc_edges, int64_t num_elements, float* edge_flows, float* element_flows,
                            float* param_flows, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Losses of a language model's training, each a function of row
+ * log-sum-exps.  No counterpart in the reference.  dtype: 0 fp32, 1 fp16,
+ * 2 bf16.  reduction: 0 none (a loss per row), 1 sum, 2 mean.  A workspace
+ * holds a call's intermediate results (any contents before, nothing of use
+ * after): device memory of at least the queried size, for calls that may run
+ * concurrently one each.
+ * ------------------------------------------------------------------------- */
+
+/* ---------------------------------------------------------------------------
+ * Linear cross entropy: softmax cross entropy of logits x w^T that are never
+ * stored.  x [N, D], rows ldx elements apart; w [V, D], rows ldw apart;
+ * target int64 [N].
+ *   lse_n = log sum_v exp(x_n . w_v)
+ *   loss_n = lse_n - x_n . w_{target_n} + z_loss * lse_n^2
+ * Rows whose target is ignore_index have loss, lse and gradient 0, do not
+ * count in the mean, and their x is not read (it may hold anything).  Any
+ * other target outside [0, V) makes the row's loss NaN, and with it the
+ * gradients it takes part in.  Products of fp16 and bf16 are exact, of fp32
+ * to about 2^-21; sums are fp32.
+ *
+ * fl_linear_ce_fwd: loss fp32 [N] (reduction 0) or [1]; lse fp32 [N], for the
+ *   backward.  A mean over no rows is 0.
+ * fl_linear_ce_bwd: grad fp32 [N] (reduction 0) or [1]; lse as the forward
+ *   wrote it.  dx [N, D] and dw [V, D] contiguous, of x's type; either may be
+ *   NULL.  The softmax gradient enters the products rounded once to x's type
+ *   (fp32: exactly).
+ * fl_linear_ce_workspace_bytes: workspace of either call, which has to be
+ *   256-byte aligned; 0 for arguments that the calls refuse.
+ * At most 2^23 rows, 2^28 vocabulary entries and 2^20 columns (FL_ERANGE).
+ * With N == 0 nothing is written.
+ * ------------------------------------------------------------------------- */
+size_t fl_linear_ce_workspace_bytes(int64_t N, int64_t V, int64_t D, int dtype, int backward);
+int fl_linear_ce_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const int64_t* target, int64_t N,
+                     int64_t V, int64_t D, int dtype, int64_t ignore_index, float z_loss, int reduction, float* loss,
+                     float* lse, void* workspace, size_t workspace_bytes, void* stream);
+int fl_linear_ce_bwd(const float* grad, const void* x, int64_t ldx, const void* w, int64_t ldw, const int64_t* target,
+                     const float* lse, int64_t N, int64_t V, int64_t D, int dtype, int64_t ignore_index, float z_loss,
+                     int reduction, void* dx, void* dw, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Distillation from a teacher's top K logits.  Row r of the student's logits
+ * (V elements, contiguous) starts at
+ *   logits + (r / slice_rows) * slice_stride + (r % slice_rows) * row_stride
+ * elements (logits[:, :-1] of a batch of sequences without a copy); teacher
+ * [rows, K] of teacher_dtype and index int64 [rows, K] are contiguous.
+ *   p = softmax_K(teacher / T), q = softmax_V(logits / T)
+ *   loss_r = T^2 sum_k p_k (log p_k - log q[index_k])
+ *   grad_logits = grad T (q - scatter_add(p))
+ * Teacher entries of -inf are unused, whatever their index; a row without any
+ * other has loss and gradient 0 and does not count in the mean.  A used index
+ * outside [0, V) makes the row's loss and gradient NaN.  An index that comes
+ * several times takes the sum of its probabilities.
+ *
+ * fl_distill_fwd: loss fp32 [rows] or [1]; lse and teacher_lse fp32 [rows]
+ *   and norm fp32 [1] (NULL with reduction 0) for the backward.
+ * fl_distill_bwd: grad fp32, element r * grad_stride (0 or 1) for row r;
+ *   norm as the forward wrote it or NULL; grad_logits [rows, V] contiguous, of
+ *   the logits' type.
+ * At most 2^22 rows of 2^28 columns, K <= 1024 (FL_ERANGE).  With rows == 0
+ * nothing is written.
+ * ------------------------------------------------------------------------- */
+size_t fl_distill_workspace_bytes(int64_t rows, int64_t V, int dtype);
+int fl_distill_fwd(const void* logits, int64_t rows, int64_t slice_rows, int64_t slice_stride, int64_t row_stride,
+                   int64_t V, int dtype, const void* teacher, int teacher_dtype, const int64_t* index, int64_t K,
+                   float temperature, int reduction, float* loss, float* lse, float* teacher_lse, float* norm,
+                   void* workspace, size_t workspace_bytes, void* stream);
+int fl_distill_bwd(const float* grad, int grad_stride, const float* norm, const void* logits, int64_t rows,
+                   int64_t slice_rows, int64_t slice_stride, int64_t row_stride, int64_t V, int dtype,
+                   const void* teacher, int teacher_dtype, const int64_t* index, int64_t K, float temperature,
+                   const float* lse, const float* teacher_lse, void* grad_logits, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Balance loss, z loss and per-expert counts of a mixture-of-experts router.
+ * logits [tokens, experts], rows row_stride elements apart; index int64
+ * [tokens, top] contiguous, the experts each token chose; mask (NULL: all)
+ * one byte a token, 0 for tokens that do not take part (their logits may hold
+ * anything).  Over the n tokens that do, p = softmax(logits):
+ *   counts_e = number of their choices that are e (choices outside
+ *     [0, experts) count for none)
+ *   balance = experts * sum_e counts_e / (n top) * mean_t p_te
+ *   z = mean_t logsumexp(logits_t)^2
+ * The counts are constants in the gradient.  All are 0 when n is 0.
+ *
+ * fl_router_balance_fwd: balance, z fp32 [1], counts int64 [experts]; lse fp32
+ *   [tokens] and coef fp32 [experts + 1] for the backward.
+ * fl_router_balance_bwd: grad_balance, grad_z fp32 [1] (NULL: 0); grad_logits
+ *   [tokens, experts] contiguous, of the logits' type, 0 in masked rows.
+ * At most 1024 experts, 1024 choices a token and 2^31 - 1 choices (FL_ERANGE).
+ * ------------------------------------------------------------------------- */
+size_t fl_router_workspace_bytes(int64_t tokens, int64_t experts, int dtype);
+int fl_router_balance_fwd(const void* logits, int64_t row_stride, int64_t tokens, int64_t experts, int dtype,
+                          const int64_t* index, int64_t top, const uint8_t* mask, float* balance, float* z,
+                          int64_t* counts, float* lse, float* coef, void* workspace, size_t workspace_bytes,
+                          void* stream);
+int fl_router_balance_bwd(const float* grad_balance, const float* grad_z, const void* logits, int64_t row_stride,
+                          int64_t tokens, int64_t experts, int dtype, const uint8_t* mask, const float* lse,
+                          const float* coef, void* grad_logits, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

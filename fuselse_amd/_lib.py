@@ -64,7 +64,7 @@ SIGNATURES = {
                                      _i64, _vp, _vp, _vp, _vp]),
     "fl_sparse_blocked_grad": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _int, _int, _int, _vp,
                                       _vp, _i64, _vp, _vp, _vp, _vp]),
-    "fl_linear_ce_workspace_bytes": (ctypes.c_size_t, [_i64, _i64, _i64, _int, _int]),
+    "fl_linear_ce_workspace_bytes": (ctypes.c_size_t, [_i64, _i64, _i64, _int, _int, _vp, _i64]),
     "fl_linear_ce_fwd": (_int, [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _int, _i64, _float, _int, _vp, _vp, _vp,
                                 ctypes.c_size_t, _vp]),
     "fl_linear_ce_bwd": (_int, [_vp, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _int, _i64, _float, _int, _vp,

@@ -13,6 +13,8 @@
 #include "../../include/fuselse_amd.h"
 #include "fl_status.hpp"
 #include "linear_ce.hpp"
+#include "linear_ce_tile.hpp"
+#include "row_stream.hpp"
 
 namespace fl {
 namespace lce {
@@ -38,24 +40,19 @@ template <> struct Io<kBF16> {
     static constexpr bool kHalf = false;
 };
 
+template <int DT>
+__device__ __forceinline__ uint16_t half_bits(float v) {
+    if constexpr (DT == kF16) return __builtin_bit_cast(uint16_t, (_Float16)v);
+    else return __builtin_bit_cast(uint16_t, (__bf16)v);
+}
+
 // A value as its 16-bit matrix operands: exact for x and w; G, computed in
 // fp32, is rounded to nearest even in fp16 and bf16 (its share of the error of
 // dx and dw is that of one rounding of a term of their sums) and exact in fp32.
 template <int DT>
 __device__ __forceinline__ void to_parts(float v, uint16_t (&o)[Io<DT>::kParts]) {
     if constexpr (DT == kF32) split3(v, o);
-    else if constexpr (DT == kF16) o[0] = __builtin_bit_cast(uint16_t, (_Float16)v);
-    else o[0] = __builtin_bit_cast(uint16_t, (__bf16)v);
-}
-
-template <bool HALF>
-__device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
-    if constexpr (HALF)
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0,
-                                                      0, 0);
-    else
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b),
-                                                       c, 0, 0, 0);
+    else o[0] = half_bits<DT>(v);
 }
 
 // ---------------------------------------------------------------------------
@@ -177,151 +174,105 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs p) {
 }
 
 // ---------------------------------------------------------------------------
-// Packing: rows of x (the live ones) or w as 16-bit operands of ldp elements,
-// zero beyond D, and transposed with rows up to a multiple of 64 (zero beyond
-// the last).
+// Packing: rows of x (the live ones) or w as 16-bit operands of ldp elements (a
+// multiple of 64), zero beyond D; 8 elements a thread.
 // ---------------------------------------------------------------------------
-template <int DT>
-__device__ __forceinline__ float load1(const typename Io<DT>::T* p) {
-    return Elem<typename Io<DT>::T>::scalar(p);
-}
-
 template <int DT>
 __global__ __launch_bounds__(256) void pack_rows(const typename Io<DT>::T* src, int64_t lds_, int64_t d, const int* rows,
                                                  const int* live, int64_t n, uint16_t* dst, int64_t ldp,
                                                  int64_t part) {
-    const int64_t total = live ? *live : n;
-    const int64_t r = blockIdx.x;
-    if (r >= total) return;
-    const typename Io<DT>::T* s = src + (rows ? (int64_t)rows[r] : r) * lds_;
-    for (int64_t c = threadIdx.x; c < ldp; c += 256) {
-        uint16_t o[Io<DT>::kParts];
-        to_parts<DT>(c < d ? load1<DT>(s + c) : 0.0f, o);
+    typedef typename Io<DT>::T T;
+    constexpr int P = Io<DT>::kParts, VE = Elem<T>::kVec;
+    const int64_t chunks = ldp / 8;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t r = i / chunks, c = i % chunks * 8;
+    if (r >= (live ? *live : n)) return;
+    const T* s = src + (rows ? (int64_t)rows[r] : r) * lds_ + c;
+    uint16_t o[8][P];
 #pragma unroll
-        for (int k = 0; k < Io<DT>::kParts; ++k) dst[k * part + r * ldp + c] = o[k];
-    }
-}
-
-// dst[c][r] for rows r of src, r up to ldp (zero past the last row)
-template <int DT>
-__global__ __launch_bounds__(256) void pack_cols(const typename Io<DT>::T* src, int64_t lds_, int64_t d, const int* rows,
-                                                 const int* live, int64_t n, uint16_t* dst, int64_t ldp,
-                                                 int64_t part) {
-    __shared__ float tile[64][65];
-    const int64_t total = live ? *live : n;
-    const int64_t rb = (int64_t)blockIdx.x * 64, cb = (int64_t)blockIdx.y * 64;
-    if (rb >= ((total + 63) & ~(int64_t)63)) return;
-    const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
-    for (int i = ty; i < 64; i += 4) {
-        const int64_t r = rb + i, c = cb + tx;
-        tile[i][tx] = r < total && c < d ? load1<DT>(src + (rows ? (int64_t)rows[r] : r) * lds_ + c) : 0.0f;
-    }
-    __syncthreads();
-    for (int i = ty; i < 64; i += 4) {
-        const int64_t c = cb + i, r = rb + tx;
-        if (c < d && r < ldp) {
-            uint16_t o[Io<DT>::kParts];
-            to_parts<DT>(tile[tx][i], o);
+    for (int h = 0; h < 8; h += VE) {
+        float v[VE];
+        load_vec_part<T>(s + h, d - c - h, 0.0f, v);
 #pragma unroll
-            for (int k = 0; k < Io<DT>::kParts; ++k) dst[k * part + c * ldp + r] = o[k];
-        }
+        for (int k = 0; k < VE; ++k) to_parts<DT>(v[k], o[h + k]);
+    }
+#pragma unroll
+    for (int k = 0; k < P; ++k) {
+        u32x4 w;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) w[q] = o[2 * q][k] | (uint32_t)o[2 * q + 1][k] << 16;
+        *reinterpret_cast<u32x4*>(dst + k * part + r * ldp + c) = w;
     }
 }
 
 // ---------------------------------------------------------------------------
-// The product: C[m][n] = sum_k A[m][k] B[n][k] for a 128 x 128 tile in four
-// waves of 64 x 64, K in steps of 32 through LDS.
+// The products.  Tiles of 256 x 256 in eight waves of 128 x 64: two waves a
+// SIMD, so that one's LDS reads run beside the other's matrix instructions.
 // ---------------------------------------------------------------------------
-constexpr int kTile = 128;
-constexpr int kStep = 32;
-constexpr int kThreads = 256;
-constexpr int kLdsRow = kStep + 8;  // 16-bit elements a row, off the banks' period
+typedef Shape<2, 4, 8, 4> Big;
 
-struct Tile {
-    f32x4 acc[4][4];
+#define FL_LCE_BUFFERS(S)                                     \
+    __shared__ __attribute__((aligned(1024))) char buf0[kBufferBytes<S>]; \
+    __shared__ __attribute__((aligned(1024))) char buf1[kBufferBytes<S>]
+
+// A lane's place in the tile's results.
+template <class S>
+struct Place {
+    int64_t m, n;  // of acc[0][0][0]
+    __device__ __forceinline__ Place(int64_t m0, int64_t n0) {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        m = m0 + wave % S::WM * (S::FM * 16) + (lane >> 4) * 4;
+        n = n0 + wave / S::WM * (S::FN * 16) + (lane & 15);
+    }
 };
-
-template <bool HALF, int PARTS>
-__device__ __forceinline__ void tile_product(const Operand& A, const Operand& B, int64_t m0, int64_t n0, int64_t k0,
-                                             int64_t k1, Tile& t, uint16_t (*sa)[kLdsRow], uint16_t (*sb)[kLdsRow]) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int wm = (wave & 1) * 64, wn = (wave >> 1) * 64;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) t.acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    const int lr = threadIdx.x >> 2, lc = (threadIdx.x & 3) * 8;
-    for (int term = 0; term < (PARTS == 3 ? kTerms : 1); ++term) {
-        const uint16_t* pa = A.p + (PARTS == 3 ? kTermA[term] * A.part : 0);
-        const uint16_t* pb = B.p + (PARTS == 3 ? kTermB[term] * B.part : 0);
-        for (int64_t k = k0; k < k1; k += kStep) {
-            __syncthreads();
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int r = lr + h * 64;
-                const int64_t ra = m0 + r < A.rows ? m0 + r : A.rows - 1;
-                const int64_t rb = n0 + r < B.rows ? n0 + r : B.rows - 1;
-                *reinterpret_cast<u32x4*>(&sa[r][lc]) = *reinterpret_cast<const u32x4*>(pa + ra * A.ld + k + lc);
-                *reinterpret_cast<u32x4*>(&sb[r][lc]) = *reinterpret_cast<const u32x4*>(pb + rb * B.ld + k + lc);
-            }
-            __syncthreads();
-            u32x4 fa[4], fb[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                fa[i] = *reinterpret_cast<const u32x4*>(&sa[wm + i * 16 + (lane & 15)][(lane >> 4) * 8]);
-                fb[i] = *reinterpret_cast<const u32x4*>(&sb[wn + i * 16 + (lane & 15)][(lane >> 4) * 8]);
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) t.acc[i][j] = mfma<HALF>(fa[i], fb[j], t.acc[i][j]);
-        }
-    }
-}
-
-// acc[i][j][q] of a lane is C[m0 + wm + 16 i + 4 (lane / 16) + q][n0 + wn + 16 j + lane % 16].
 
 struct StatArgs {
     Operand w, x;      // M: vocabulary rows, N: live rows
-    int64_t k;
+    int64_t steps;
     const Head* head;
     const int* tgt;
     int64_t v0, v;     // the piece's first row, and its rows
-    int64_t tiles_n;
+    int64_t tiles_m;
     float2* part;      // [live row][parts]: (max, sum)
     int64_t parts;
     float* at_target;  // [live row]
 };
 
-template <int DT>
-__global__ __launch_bounds__(kThreads) void logits_stats(StatArgs p) {
-    __shared__ uint16_t sa[kTile][kLdsRow], sb[kTile][kLdsRow];
+template <int DT, class S>
+__global__ __launch_bounds__(S::kThreads, 2) void logits_stats(StatArgs p) {
+    FL_LCE_BUFFERS(S);
     const int live = p.head->live;
-    const int64_t n0 = (blockIdx.x % p.tiles_n) * kTile, m0 = (blockIdx.x / p.tiles_n) * kTile;
-    if (n0 >= live) return;
+    const int64_t tiles_n = (live + S::TN - 1) / S::TN;
+    if (blockIdx.x >= p.tiles_m * tiles_n) return;
+    int64_t tm, tn;
+    tile_at(xcd_tile(blockIdx.x, p.tiles_m * tiles_n), p.tiles_m, tiles_n, tm, tn);
     p.x.rows = live;
-    Tile t;
-    tile_product<Io<DT>::kHalf, Io<DT>::kParts>(p.w, p.x, m0, n0, 0, p.k, t, sa, sb);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t mw = m0 + (wave & 1) * 64, nw = n0 + (wave >> 1) * 64;
+    Side<S, S::TM, true> A;
+    Side<S, S::TN, true> B;
+    A.init(p.w, tm * S::TM);
+    B.init(p.x, tn * S::TN);
+    f32x4 acc[S::FM][S::FN];
+    tile_product<S, true, true, Io<DT>::kHalf, Io<DT>::kParts>(A, B, 0, p.steps, acc, (lds_char*)buf0, (lds_char*)buf1);
+    const Place<S> at(tm * S::TM, tn * S::TN);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const int64_t n = nw + j * 16 + (lane & 15);
+    for (int j = 0; j < S::FN; ++j) {
+        const int64_t n = at.n + j * 16;
         const int target = n < live ? p.tgt[n] : -1;
-        float v[16];
+        float v[S::FM * 4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < S::FM; ++i)
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                const int64_t m = mw + i * 16 + (lane >> 4) * 4 + q;
-                v[i * 4 + q] = m < p.v ? t.acc[i][j][q] : -kInf;
-                if (p.v0 + m == target && m < p.v) p.at_target[n] = t.acc[i][j][q];
+                const int64_t m = at.m + i * 16 + q;
+                v[i * 4 + q] = m < p.v ? acc[i][j][q] : -kInf;
+                if (p.v0 + m == target && m < p.v) p.at_target[n] = acc[i][j][q];
             }
         float m = -kInf, s = 0.0f;
         lse_fold<true>(m, s, v);
         lse_merge(m, s, exact_xor<16>(m), exact_xor<16>(s));
         lse_merge(m, s, exact_xor<32>(m), exact_xor<32>(s));
-        if (lane < 16 && n < live && mw < p.v) p.part[n * p.parts + mw / 64] = make_float2(m, s);
+        const int64_t mw = at.m / (S::FM * 16);
+        if ((threadIdx.x & 63) < 16 && n < live && mw * (S::FM * 16) < p.v) p.part[n * p.parts + mw] = make_float2(m, s);
     }
 }
 
@@ -363,53 +314,55 @@ __global__ __launch_bounds__(1024) void reduce_rows(const Head* head, const floa
 
 struct GradArgs {
     Operand w, x;
-    int64_t k;
+    int64_t steps;
     const Head* head;
     const int* tgt;
     const float *a, *b, *lse;
     int64_t v0, v;       // the piece: vocabulary rows v0 .. v - 1 are w's rows 0 ..
-    int64_t tiles_n;
+    int64_t tiles_m;
     uint16_t* g;         // [live row][ldg]
     int64_t ldg, g_part;
-    uint16_t* gt;        // [piece row][ldt]
-    int64_t ldt, gt_part;
 };
 
-template <int DT>
-__global__ __launch_bounds__(kThreads) void logits_grad(GradArgs p) {
-    __shared__ uint16_t sa[kTile][kLdsRow], sb[kTile][kLdsRow];
+// G of a piece.  Rows from the live ones up to a multiple of 64 are zero, and so
+// are columns up to the tiles' end: the products' K runs over whole steps.
+template <int DT, class S>
+__global__ __launch_bounds__(S::kThreads, 2) void logits_grad(GradArgs p) {
+    FL_LCE_BUFFERS(S);
     constexpr int P = Io<DT>::kParts;
     const int live = p.head->live;
-    const int64_t n0 = (blockIdx.x % p.tiles_n) * kTile, m0 = (blockIdx.x / p.tiles_n) * kTile;
-    if (n0 >= live) return;
+    const int64_t tiles_n = (live + S::TN - 1) / S::TN;
+    if (blockIdx.x >= p.tiles_m * tiles_n) return;
+    int64_t tm, tn;
+    tile_at(xcd_tile(blockIdx.x, p.tiles_m * tiles_n), p.tiles_m, tiles_n, tm, tn);
     p.x.rows = live;
-    Tile t;
-    tile_product<Io<DT>::kHalf, P>(p.w, p.x, m0, n0, 0, p.k, t, sa, sb);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t mw = m0 + (wave & 1) * 64, nw = n0 + (wave >> 1) * 64;
+    Side<S, S::TM, true> A;
+    Side<S, S::TN, true> B;
+    A.init(p.w, tm * S::TM);
+    B.init(p.x, tn * S::TN);
+    f32x4 acc[S::FM][S::FN];
+    tile_product<S, true, true, Io<DT>::kHalf, P>(A, B, 0, p.steps, acc, (lds_char*)buf0, (lds_char*)buf1);
+    const Place<S> at(tm * S::TM, tn * S::TN);
+    const int64_t n_end = (live + kStep - 1) / kStep * kStep;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const int64_t n = nw + j * 16 + (lane & 15);
+    for (int j = 0; j < S::FN; ++j) {
+        const int64_t n = at.n + j * 16;
         const bool in = n < live;
         const int target = in ? p.tgt[n] : -1;
         const float a = in ? p.a[n] : 0.0f, b = in ? p.b[n] : 0.0f, lse = in ? p.lse[n] : 0.0f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int64_t m = mw + i * 16 + (lane >> 4) * 4;
+        for (int i = 0; i < S::FM; ++i) {
+            const int64_t m = at.m + i * 16;
             uint16_t o[4][P];
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                float g = a * fexp2((t.acc[i][j][q] - lse) * kLog2e);
+                float g = a * fexp2((acc[i][j][q] - lse) * kLog2e);
                 if (p.v0 + m + q == target) g += b;
                 to_parts<DT>(in && p.v0 + m + q < p.v ? g : 0.0f, o[q]);
             }
+            if (n < n_end) {
 #pragma unroll
-            for (int k = 0; k < P; ++k) {
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    if (n < p.ldt && m + q < p.v - p.v0) p.gt[k * p.gt_part + (m + q) * p.ldt + n] = o[q][k];
-                }
-                if (in && m < p.ldg) {
+                for (int k = 0; k < P; ++k) {
                     uint2 u;
                     u.x = o[0][k] | (uint32_t)o[1][k] << 16;
                     u.y = o[2][k] | (uint32_t)o[3][k] << 16;
@@ -423,53 +376,91 @@ __global__ __launch_bounds__(kThreads) void logits_grad(GradArgs p) {
 struct ProductArgs {
     Operand a, b;       // M and N rows
     const Head* head;
-    int64_t k;          // depth; with `live_k`, the live rows up to a multiple of 32
-    int live_k, live_n;
-    int64_t m, n, tiles_m;
+    int64_t steps;      // of K; dw: the live rows'
+    int64_t m, n;       // results
+    int64_t tiles_m;
     int splits;
-    float* acc;         // [split][n][ldc] fp32 sums, added to when `add`
+    float* acc;         // dx: [split][n][ldc] fp32 sums, added to when `add`
     int64_t ldc, split_stride;
     int add;
-    void* out;          // [n][ldc] results
+    void* out;          // dw: [n][ldc] results
 };
 
-template <int DT, bool FINAL>
-__global__ __launch_bounds__(kThreads) void product(ProductArgs p) {
-    __shared__ uint16_t sa[kTile][kLdsRow], sb[kTile][kLdsRow];
-    const int live = p.head->live;
-    const int64_t m0 = (blockIdx.x % p.tiles_m) * kTile, n0 = (blockIdx.x / p.tiles_m) * kTile;
-    const int split = blockIdx.y;
-    const int64_t n_end = p.live_n ? live : p.n;
-    if (n0 >= n_end) return;
-    if (p.live_n) p.b.rows = live;
-    const int64_t depth = p.live_k ? (int64_t)((live + kStep - 1) & ~(kStep - 1)) : p.k;
-    const int64_t per = ((depth + p.splits - 1) / p.splits + kStep - 1) & ~(int64_t)(kStep - 1);
-    const int64_t k0 = split * per;
-    const int64_t k1 = k0 + per < depth ? k0 + per : depth;
-    Tile t;
-    tile_product<Io<DT>::kHalf, Io<DT>::kParts>(p.a, p.b, m0, n0, k0, k1, t, sa, sb);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t mw = m0 + (wave & 1) * 64, nw = n0 + (wave >> 1) * 64;
+// dx (DX): C[n][d] = sum_v G[n][v] w[v][d] over a piece, added to the splits'
+// sums.  dw: C[v][d] = sum_n G[n][v] x[n][d], the piece's rows of the result.
+template <int DT, class S, bool DX>
+__global__ __launch_bounds__(S::kThreads, 2) void product(ProductArgs p) {
+    FL_LCE_BUFFERS(S);
     typedef typename Io<DT>::T T;
+    const int live = p.head->live;
+    const int64_t n_end = DX ? live : p.n;
+    const int64_t tiles_n = (n_end + S::TN - 1) / S::TN;
+    const int64_t tiles = p.tiles_m * tiles_n;
+    if (blockIdx.x >= tiles * p.splits) return;
+    const int64_t t = xcd_tile(blockIdx.x, tiles * p.splits);
+    const int split = (int)(t / tiles);
+    int64_t tm, tn;
+    tile_at(t % tiles, p.tiles_m, tiles_n, tm, tn);
+    int64_t k0 = 0, k1;
+    if constexpr (DX) {
+        p.b.rows = live;
+        const int64_t per = (p.steps + p.splits - 1) / p.splits;
+        k0 = split * per;
+        k1 = k0 + per < p.steps ? k0 + per : p.steps;
+    } else {
+        k1 = (live + kStep - 1) / kStep;
+        p.a.rows = live;
+        p.b.rows = (int)(k1 * kStep);
+    }
+    Side<S, S::TM, false> A;
+    Side<S, S::TN, DX> B;
+    A.init(p.a, tm * S::TM);
+    B.init(p.b, tn * S::TN);
+    f32x4 acc[S::FM][S::FN];
+    tile_product<S, false, DX, Io<DT>::kHalf, Io<DT>::kParts>(A, B, k0, k1, acc, (lds_char*)buf0, (lds_char*)buf1);
+    const Place<S> at(tm * S::TM, tn * S::TN);
     const float inv = p.head->inv_scale;
+    const bool whole = (p.ldc & 3) == 0;  // four results of a lane are one store
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int j = 0; j < S::FN; ++j) {
+        const int64_t n = at.n + j * 16;
+        if (n >= n_end) continue;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int64_t n = nw + j * 16 + (lane & 15);
+        for (int i = 0; i < S::FM; ++i) {
+            const int64_t m = at.m + i * 16;
+            if (m >= p.m) continue;
+            f32x4 v = acc[i][j];
+            if constexpr (DX) {
+                float* c = p.acc + split * p.split_stride + n * p.ldc + m;
+                if (whole) {
+                    if (p.add) v += *reinterpret_cast<const f32x4*>(c);
+                    *reinterpret_cast<f32x4*>(c) = v;
+                } else {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int64_t m = mw + i * 16 + (lane >> 4) * 4 + q;
-                if (m < p.m && n < n_end) {
-                    if constexpr (FINAL) {
-                        Elem<T>::put(static_cast<T*>(p.out) + n * p.ldc + m, t.acc[i][j][q] * inv);
-                    } else {
-                        float* c = p.acc + split * p.split_stride + n * p.ldc + m;
-                        *c = p.add ? *c + t.acc[i][j][q] : t.acc[i][j][q];
-                    }
+                    for (int q = 0; q < 4; ++q)
+                        if (m + q < p.m) c[q] = p.add ? c[q] + v[q] : v[q];
+                }
+            } else {
+                T* c = static_cast<T*>(p.out) + n * p.ldc + m;
+                v *= inv;
+                if (whole && sizeof(T) == 4) {
+                    *reinterpret_cast<f32x4*>(c) = v;
+                } else if (whole) {
+                    uint16_t o[4];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) o[q] = half_bits<DT>(v[q]);
+                    uint2 u;
+                    u.x = o[0] | (uint32_t)o[1] << 16;
+                    u.y = o[2] | (uint32_t)o[3] << 16;
+                    *reinterpret_cast<uint2*>(c) = u;
+                } else {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        if (m + q < p.m) Elem<T>::put(c + q, v[q]);
                 }
             }
         }
+    }
 }
 
 // dx rows from the splits' sums; ignored rows are zero.
@@ -496,18 +487,37 @@ __global__ __launch_bounds__(256) void finish_dx(const Head* head, const int* po
 constexpr int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 constexpr int64_t div_up(int64_t v, int64_t by) { return (v + by - 1) / by; }
 
+// G of a piece takes at most this many bytes: enough vocabulary rows for the
+// products to fill the chip, and a workspace that stays small beside w.
+constexpr int64_t kPieceBytes = 256 << 20;
+
 struct Layout {
-    int64_t piece;       // vocabulary rows of a piece
-    int64_t ldx;         // packed row of x and w
-    int64_t ldn;         // transposed rows: live rows
-    int64_t ldv;         // transposed rows: piece rows
-    int splits;
-    int64_t head, rows, pos, tgt, at_target, loss_rows, part, parts, a, b, lse, xp, xt, wp, wt, g, gt, acc, bytes;
+    int64_t piece;       // vocabulary rows of a piece, a multiple of 256
+    int64_t ldx;         // a packed row of x and w
+    bool pack_w;         // w is packed a piece at a time
+    int splits;          // of K in dx
+    int64_t head, rows, pos, tgt, at_target, loss_rows, part, parts, a, b, lse, xp, wp, g, acc, bytes;
 };
 
 int parts_of(int dtype) { return dtype == kF32 ? 3 : 1; }
 
-Layout layout(int64_t N, int64_t V, int64_t D, int dtype, bool bwd) {
+// Splits of K in dx: as few as fill the chip's 256 places evenly; a split costs
+// about 8 steps for its start and its sums.
+int dx_splits(int64_t tiles, int64_t steps) {
+    int best = 1;
+    int64_t cost = 0;
+    for (int s = 1; s <= 32 && s <= steps; ++s) {
+        const int64_t c = div_up(tiles * s, 256) * (div_up(steps, s) + 8);
+        if (s == 1 || c < cost) {
+            best = s;
+            cost = c;
+        }
+    }
+    return best;
+}
+
+// aligned: w's rows can be read as matrix operands where they are.
+Layout layout(int64_t N, int64_t V, int64_t D, int dtype, bool bwd, bool aligned) {
     Layout l{};
     int64_t at = 0;
     auto take = [&](int64_t bytes) {
@@ -516,18 +526,27 @@ Layout layout(int64_t N, int64_t V, int64_t D, int dtype, bool bwd) {
         return here;
     };
     const int64_t parts = parts_of(dtype);
-    l.piece = V < 16384 ? round_up(V, 64) : 16384;
+    int64_t most = kPieceBytes / (2 * parts * round_up(N, 64)) / 256 * 256;
+    if (most < 2048) most = 2048;
     l.ldx = round_up(D, 64);
-    l.ldn = round_up(N, 64);
-    l.ldv = l.piece;
+    l.pack_w = dtype == kF32 || !aligned || D % 64 != 0;
+    if (l.pack_w) {
+        const int64_t fit = kPieceBytes / (2 * parts * l.ldx) / 256 * 256;
+        if (most > fit) most = fit < 2048 ? 2048 : fit;
+    } else if (!bwd) {
+        // nothing of the workspace grows with a forward's piece; one launch holds
+        // 2^22 tiles easily
+        most = ((int64_t)1 << 22) / div_up(N, Big::TN) * 256;
+    }
+    l.piece = round_up(div_up(V, div_up(V, most)), 256);
     l.head = take(sizeof(Head));
     l.rows = take(4 * N);
     l.pos = take(4 * N);
     l.tgt = take(4 * N);
     l.xp = take(2 * parts * N * l.ldx);
-    l.wp = take(2 * parts * l.piece * l.ldx);
+    l.wp = take(l.pack_w ? 2 * parts * l.piece * l.ldx : 0);
     if (!bwd) {
-        l.parts = div_up(V, 64);
+        l.parts = div_up(V, 128);
         l.at_target = take(4 * N);
         l.loss_rows = take(4 * N);
         l.part = take(8 * N * l.parts);
@@ -535,11 +554,8 @@ Layout layout(int64_t N, int64_t V, int64_t D, int dtype, bool bwd) {
         l.a = take(4 * N);
         l.b = take(4 * N);
         l.lse = take(4 * N);
-        l.splits = 4;
-        l.xt = take(2 * parts * D * l.ldn);
-        l.wt = take(2 * parts * D * l.ldv);
-        l.g = take(2 * parts * N * l.ldv);
-        l.gt = take(2 * parts * l.piece * l.ldn);
+        l.splits = dx_splits(div_up(N, Big::TN) * div_up(D, Big::TM), l.piece / kStep);
+        l.g = take(2 * parts * round_up(N, 64) * l.piece);
         l.acc = take(4 * l.splits * N * D);
     }
     l.bytes = at;
@@ -565,23 +581,27 @@ P* at(const Call& c, int64_t off) {
     return reinterpret_cast<P*>(c.ws + off);
 }
 
+// Rows v0 .. of w as a product's operand.
 template <int DT>
-Operand pack_w(const Call& c, const Layout& l, int64_t v0, int64_t rows) {
+Operand operand_w(const Call& c, const Layout& l, int64_t v0, int64_t rows) {
     typedef typename Io<DT>::T T;
+    const T* w = static_cast<const T*>(c.w) + v0 * c.ldw;
+    if (!l.pack_w) return Operand{reinterpret_cast<const uint16_t*>(w), c.ldw, 0, (int)rows, l.ldx};
     const int64_t part = l.piece * l.ldx;
-    pack_rows<DT><<<dim3((unsigned)rows), 256, 0, c.s>>>(static_cast<const T*>(c.w) + v0 * c.ldw, c.ldw, c.D, nullptr,
-                                                         nullptr, rows, at<uint16_t>(c, l.wp), l.ldx, part);
-    return Operand{at<uint16_t>(c, l.wp), l.ldx, part, (int)rows};
+    pack_rows<DT><<<dim3((unsigned)div_up(rows * (l.ldx / 8), 256)), 256, 0, c.s>>>(
+        w, c.ldw, c.D, nullptr, nullptr, rows, at<uint16_t>(c, l.wp), l.ldx, part);
+    return Operand{at<uint16_t>(c, l.wp), l.ldx, part, (int)rows, l.ldx};
 }
 
 template <int DT>
-Operand pack_x(const Call& c, const Layout& l) {
+Operand operand_x(const Call& c, const Layout& l) {
     typedef typename Io<DT>::T T;
     const Head* head = at<Head>(c, l.head);
     const int64_t part = c.N * l.ldx;
-    pack_rows<DT><<<dim3((unsigned)c.N), 256, 0, c.s>>>(static_cast<const T*>(c.x), c.ldx, c.D, at<int>(c, l.rows),
-                                                        &head->live, c.N, at<uint16_t>(c, l.xp), l.ldx, part);
-    return Operand{at<uint16_t>(c, l.xp), l.ldx, part, (int)c.N};
+    pack_rows<DT><<<dim3((unsigned)div_up(c.N * (l.ldx / 8), 256)), 256, 0, c.s>>>(
+        static_cast<const T*>(c.x), c.ldx, c.D, at<int>(c, l.rows), &head->live, c.N, at<uint16_t>(c, l.xp), l.ldx,
+        part);
+    return Operand{at<uint16_t>(c, l.xp), l.ldx, part, (int)c.N, l.ldx};
 }
 
 PlanArgs plan_args(const Call& c, const Layout& l) {
@@ -600,29 +620,28 @@ PlanArgs plan_args(const Call& c, const Layout& l) {
 }
 
 template <int DT>
-void run_fwd(const Call& c, float* loss, float* lse) {
-    const Layout l = layout(c.N, c.V, c.D, DT, false);
+void run_fwd(const Call& c, const Layout& l, float* loss, float* lse) {
+    typedef Big S;
     PlanArgs p = plan_args(c, l);
     p.loss_rows = c.reduction == 0 ? loss : at<float>(c, l.loss_rows);
     p.lse_out = lse;
     plan_kernel<false><<<1, kPlanThreads, 0, c.s>>>(p);
-    const Operand x = pack_x<DT>(c, l);
-    const int64_t tiles_n = div_up(c.N, kTile);
+    const Operand x = operand_x<DT>(c, l);
     for (int64_t v0 = 0; v0 < c.V; v0 += l.piece) {
         const int64_t rows = c.V - v0 < l.piece ? c.V - v0 : l.piece;
         StatArgs a{};
-        a.w = pack_w<DT>(c, l, v0, rows);
+        a.w = operand_w<DT>(c, l, v0, rows);
         a.x = x;
-        a.k = l.ldx;
+        a.steps = l.ldx / kStep;
         a.head = p.head;
         a.tgt = p.tgt;
         a.v0 = v0;
         a.v = rows;
-        a.tiles_n = tiles_n;
-        a.part = at<float2>(c, l.part) + v0 / 64;
+        a.tiles_m = div_up(rows, S::TM);
+        a.part = at<float2>(c, l.part) + v0 / 128;
         a.parts = l.parts;
         a.at_target = at<float>(c, l.at_target);
-        logits_stats<DT><<<dim3((unsigned)(tiles_n * div_up(rows, kTile))), kThreads, 0, c.s>>>(a);
+        logits_stats<DT, S><<<dim3((unsigned)(div_up(c.N, S::TN) * a.tiles_m)), S::kThreads, 0, c.s>>>(a);
     }
     finish_rows<<<dim3((unsigned)div_up(c.N, 4)), 256, 0, c.s>>>(p.head, p.rows, p.tgt, at<float2>(c, l.part), l.parts,
                                                                  at<float>(c, l.at_target), c.z, p.loss_rows, lse);
@@ -630,9 +649,9 @@ void run_fwd(const Call& c, float* loss, float* lse) {
 }
 
 template <int DT>
-void run_bwd(const Call& c, const float* grad, const float* lse, void* dx, void* dw) {
+void run_bwd(const Call& c, const Layout& l, const float* grad, const float* lse, void* dx, void* dw) {
     typedef typename Io<DT>::T T;
-    const Layout l = layout(c.N, c.V, c.D, DT, true);
+    typedef Big S;
     PlanArgs p = plan_args(c, l);
     p.grad = grad;
     p.grad_stride = c.reduction == 0 ? 1 : 0;
@@ -641,20 +660,15 @@ void run_bwd(const Call& c, const float* grad, const float* lse, void* dx, void*
     p.b = at<float>(c, l.b);
     p.lse = at<float>(c, l.lse);
     plan_kernel<true><<<1, kPlanThreads, 0, c.s>>>(p);
-    const Operand x = pack_x<DT>(c, l);
-    Operand xt{at<uint16_t>(c, l.xt), l.ldn, c.D * l.ldn, (int)c.D};
-    pack_cols<DT><<<dim3((unsigned)(l.ldn / 64), (unsigned)div_up(c.D, 64)), 256, 0, c.s>>>(
-        static_cast<const T*>(c.x), c.ldx, c.D, p.rows, &p.head->live, c.N, at<uint16_t>(c, l.xt), l.ldn,
-        c.D * l.ldn);
-    const int64_t tiles_n = div_up(c.N, kTile), tiles_d = div_up(c.D, kTile);
+    const Operand x = operand_x<DT>(c, l);
+    const int64_t tiles_n = div_up(c.N, S::TN), tiles_d = div_up(c.D, S::TM);
+    const int64_t g_part = round_up(c.N, 64) * l.piece;
     for (int64_t v0 = 0; v0 < c.V; v0 += l.piece) {
         const int64_t rows = c.V - v0 < l.piece ? c.V - v0 : l.piece;
-        const int64_t depth = round_up(rows, 64);
-        const T* w = static_cast<const T*>(c.w) + v0 * c.ldw;
         GradArgs g{};
-        g.w = pack_w<DT>(c, l, v0, rows);
+        g.w = operand_w<DT>(c, l, v0, rows);
         g.x = x;
-        g.k = l.ldx;
+        g.steps = l.ldx / kStep;
         g.head = p.head;
         g.tgt = p.tgt;
         g.a = p.a;
@@ -662,51 +676,45 @@ void run_bwd(const Call& c, const float* grad, const float* lse, void* dx, void*
         g.lse = p.lse;
         g.v0 = v0;
         g.v = v0 + rows;
-        g.tiles_n = tiles_n;
+        g.tiles_m = div_up(rows, S::TM);
         g.g = at<uint16_t>(c, l.g);
-        g.ldg = l.ldv;
-        g.g_part = c.N * l.ldv;
-        g.gt = at<uint16_t>(c, l.gt);
-        g.ldt = l.ldn;
-        g.gt_part = l.piece * l.ldn;
-        logits_grad<DT><<<dim3((unsigned)(tiles_n * div_up(depth, kTile))), kThreads, 0, c.s>>>(g);
+        g.ldg = l.piece;
+        g.g_part = g_part;
+        logits_grad<DT, S><<<dim3((unsigned)(tiles_n * g.tiles_m)), S::kThreads, 0, c.s>>>(g);
+        ProductArgs a{};
+        a.head = p.head;
+        a.m = c.D;
+        a.tiles_m = tiles_d;
+        a.ldc = c.D;
         if (dx) {
-            pack_cols<DT><<<dim3((unsigned)(depth / 64), (unsigned)div_up(c.D, 64)), 256, 0, c.s>>>(
-                w, c.ldw, c.D, nullptr, nullptr, rows, at<uint16_t>(c, l.wt), l.ldv, c.D * l.ldv);
-            ProductArgs a{};
-            a.a = Operand{at<uint16_t>(c, l.wt), l.ldv, c.D * l.ldv, (int)c.D};
-            a.b = Operand{g.g, l.ldv, g.g_part, (int)c.N};
-            a.head = p.head;
-            a.k = depth;
-            a.live_n = 1;
-            a.m = c.D;
+            a.a = g.w;
+            a.b = Operand{g.g, l.piece, g_part, (int)c.N, l.piece};
+            a.steps = div_up(rows, kStep);
             a.n = c.N;
-            a.tiles_m = tiles_d;
             a.splits = l.splits;
             a.acc = at<float>(c, l.acc);
-            a.ldc = c.D;
             a.split_stride = c.N * c.D;
             a.add = v0 > 0;
-            product<DT, false><<<dim3((unsigned)(tiles_d * tiles_n), (unsigned)l.splits), kThreads, 0, c.s>>>(a);
+            product<DT, S, true><<<dim3((unsigned)(tiles_d * tiles_n * l.splits)), S::kThreads, 0, c.s>>>(a);
         }
         if (dw) {
-            ProductArgs a{};
-            a.a = xt;
-            a.b = Operand{g.gt, l.ldn, g.gt_part, (int)rows};
-            a.head = p.head;
-            a.live_k = 1;
-            a.m = c.D;
+            a.a = x;
+            a.b = Operand{g.g, l.piece, g_part, 0, l.piece};
             a.n = rows;
-            a.tiles_m = tiles_d;
             a.splits = 1;
-            a.ldc = c.D;
             a.out = static_cast<T*>(dw) + v0 * c.D;
-            product<DT, true><<<dim3((unsigned)(tiles_d * div_up(rows, kTile)), 1), kThreads, 0, c.s>>>(a);
+            product<DT, S, false><<<dim3((unsigned)(tiles_d * div_up(rows, S::TN))), S::kThreads, 0, c.s>>>(a);
         }
     }
     if (dx)
         finish_dx<DT><<<dim3((unsigned)c.N), 256, 0, c.s>>>(p.head, p.pos, at<float>(c, l.acc), l.splits, c.N * c.D, c.D,
                                                             dx);
+}
+
+// w's rows can be read as operands where they are: 16-byte loads at 16-byte
+// addresses, and a tile's rows within 32-bit offsets.
+bool is_aligned(const void* w, int64_t ldw, int dtype) {
+    return dtype != kF32 && (reinterpret_cast<uintptr_t>(w) & 15u) == 0 && ldw % 8 == 0 && ldw <= (1 << 22);
 }
 
 int check(const char* name, const Call& c, int dtype, size_t ws_bytes, bool bwd) {
@@ -722,7 +730,7 @@ int check(const char* name, const Call& c, int dtype, size_t ws_bytes, bool bwd)
     FL_CHECK(c.x && c.w && c.target, "%s: NULL pointer argument", name);
     FL_CHECK(reinterpret_cast<uintptr_t>(c.x) % size == 0 && reinterpret_cast<uintptr_t>(c.w) % size == 0,
              "%s: x or w is not element-aligned", name);
-    const int64_t need = layout(c.N, c.V, c.D, dtype, bwd).bytes;
+    const int64_t need = layout(c.N, c.V, c.D, dtype, bwd, is_aligned(c.w, c.ldw, dtype)).bytes;
     FL_CHECK((int64_t)ws_bytes >= need, "%s: workspace of %llu bytes, %lld needed", name, (unsigned long long)ws_bytes,
              (long long)need);
     FL_CHECK(c.ws && (reinterpret_cast<uintptr_t>(c.ws) & 255u) == 0, "%s: workspace is not 256-byte aligned", name);
@@ -735,9 +743,10 @@ int check(const char* name, const Call& c, int dtype, size_t ws_bytes, bool bwd)
 
 using namespace fl::lce;
 
-extern "C" size_t fl_linear_ce_workspace_bytes(int64_t N, int64_t V, int64_t D, int dtype, int backward) {
+extern "C" size_t fl_linear_ce_workspace_bytes(int64_t N, int64_t V, int64_t D, int dtype, int backward,
+                                               const void* w, int64_t ldw) {
     if (N < 1 || V < 1 || D < 1 || dtype < 0 || dtype > 2 || N > (1 << 23) || V > (1 << 28) || D > (1 << 20)) return 0;
-    return (size_t)layout(N, V, D, dtype, backward != 0).bytes;
+    return (size_t)layout(N, V, D, dtype, backward != 0, is_aligned(w, ldw, dtype)).bytes;
 }
 
 extern "C" int fl_linear_ce_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const int64_t* target,
@@ -749,9 +758,10 @@ extern "C" int fl_linear_ce_fwd(const void* x, int64_t ldx, const void* w, int64
     const int rc = check("fl_linear_ce_fwd", c, dtype, workspace_bytes, false);
     if (rc != FL_OK || N == 0) return rc;
     FL_CHECK(loss && lse, "fl_linear_ce_fwd: NULL pointer argument");
-    if (dtype == kF32) run_fwd<kF32>(c, loss, lse);
-    else if (dtype == kF16) run_fwd<kF16>(c, loss, lse);
-    else run_fwd<kBF16>(c, loss, lse);
+    const Layout l = layout(N, V, D, dtype, false, is_aligned(c.w, c.ldw, dtype));
+    if (dtype == kF32) run_fwd<kF32>(c, l, loss, lse);
+    else if (dtype == kF16) run_fwd<kF16>(c, l, loss, lse);
+    else run_fwd<kBF16>(c, l, loss, lse);
     return fl::launch_status("fl_linear_ce_fwd");
 }
 
@@ -765,8 +775,9 @@ extern "C" int fl_linear_ce_bwd(const float* grad, const void* x, int64_t ldx, c
     if (rc != FL_OK || N == 0) return rc;
     FL_CHECK(grad && lse, "fl_linear_ce_bwd: NULL pointer argument");
     if (!dx && !dw) return fl::ok();
-    if (dtype == kF32) run_bwd<kF32>(c, grad, lse, dx, dw);
-    else if (dtype == kF16) run_bwd<kF16>(c, grad, lse, dx, dw);
-    else run_bwd<kBF16>(c, grad, lse, dx, dw);
+    const Layout l = layout(N, V, D, dtype, true, is_aligned(c.w, c.ldw, dtype));
+    if (dtype == kF32) run_bwd<kF32>(c, l, grad, lse, dx, dw);
+    else if (dtype == kF16) run_bwd<kF16>(c, l, grad, lse, dx, dw);
+    else run_bwd<kBF16>(c, l, grad, lse, dx, dw);
     return fl::launch_status("fl_linear_ce_bwd");
 }

@@ -44,13 +44,16 @@ __device__ __forceinline__ void split3(float v, uint16_t (&o)[3]) {
     o[2] = (uint16_t)(__builtin_bit_cast(uint32_t, r2) >> 16);
 }
 
-// One product's operand: 16-bit rows of K elements, `ld` apart, in `parts`
-// copies `part` elements apart.  Rows past rows - 1 are read as the last row.
+// One product's operand: 16-bit rows `ld` elements apart, in `parts` copies
+// `part` elements apart, `cols` (a multiple of 8) of a row's elements readable.
+// What a tile reaches beyond the rows and columns is read as the last row and
+// the last 8 columns.
 struct Operand {
     const uint16_t* p;
     int64_t ld;
     int64_t part;
     int rows;
+    int64_t cols;
 };
 
 }  // namespace lce

@@ -912,7 +912,8 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
         return loss.zero_(), lse
     dt = _DTYPE_CODE[x.dtype]
     with _on_device(x):
-        nbytes = _lib.load().fl_linear_ce_workspace_bytes(N, V, D, dt, 0)
+        nbytes = _lib.load().fl_linear_ce_workspace_bytes(N, V, D, dt, 0, weight.data_ptr(),
+                                                         _row_stride(weight))
         ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
         _lib.call("fl_linear_ce_fwd", x.data_ptr(), _row_stride(x), weight.data_ptr(), _row_stride(weight),
                   target.data_ptr(), N, V, D, dt, ignore_index, z_loss, red, loss.data_ptr(), lse.data_ptr(),
@@ -944,7 +945,8 @@ def linear_cross_entropy_backward(grad_output: torch.Tensor, x: torch.Tensor, we
         return None, None
     dt = _DTYPE_CODE[x.dtype]
     with _on_device(x):
-        nbytes = _lib.load().fl_linear_ce_workspace_bytes(N, V, D, dt, 1)
+        nbytes = _lib.load().fl_linear_ce_workspace_bytes(N, V, D, dt, 1, weight.data_ptr(),
+                                                         _row_stride(weight))
         ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
         _lib.call("fl_linear_ce_bwd", grad_output.data_ptr(), x.data_ptr(), _row_stride(x), weight.data_ptr(),
                   _row_stride(weight), target.data_ptr(), lse.data_ptr(), N, V, D, dt, ignore_index, z_loss, red,

@@ -356,11 +356,13 @@ int fl_sparse_blocked_grad(const float* node_flows, const float* node_mars, cons
  *   NULL.  The softmax gradient enters the products rounded once to x's type
  *   (fp32: exactly).
  * fl_linear_ce_workspace_bytes: workspace of either call, which has to be
- *   256-byte aligned; 0 for arguments that the calls refuse.
+ *   256-byte aligned, with w and ldw as that call gets them; 0 for sizes that
+ *   the calls refuse.
  * At most 2^23 rows, 2^28 vocabulary entries and 2^20 columns (FL_ERANGE).
  * With N == 0 nothing is written.
  * ------------------------------------------------------------------------- */
-size_t fl_linear_ce_workspace_bytes(int64_t N, int64_t V, int64_t D, int dtype, int backward);
+size_t fl_linear_ce_workspace_bytes(int64_t N, int64_t V, int64_t D, int dtype, int backward, const void* w,
+                                    int64_t ldw);
 int fl_linear_ce_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const int64_t* target, int64_t N,
                      int64_t V, int64_t D, int dtype, int64_t ignore_index, float z_loss, int reduction, float* loss,
                      float* lse, void* workspace, size_t workspace_bytes, void* stream);

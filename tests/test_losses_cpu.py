@@ -71,8 +71,8 @@ def test_backward_and_other_entry_refusals():
     assert lib.fl_linear_ce_bwd(None, VP, 8, VP, 8, VP, VP, 4, 16, 8, 0, -100, 0.0, 2, VP, VP, VP, big, None) == 1
     assert "NULL" in _message(lib)
     assert lib.fl_linear_ce_bwd(VP, VP, 8, VP, 8, VP, VP, 4, 16, 8, 0, -100, 0.0, 2, None, None, VP, big, None) == 0
-    assert lib.fl_linear_ce_workspace_bytes(0, 4, 4, 0, 0) == 0
-    assert lib.fl_linear_ce_workspace_bytes(4, 4, 4, 5, 0) == 0
+    assert lib.fl_linear_ce_workspace_bytes(0, 4, 4, 0, 0, VP, 4) == 0
+    assert lib.fl_linear_ce_workspace_bytes(4, 4, 4, 5, 0, VP, 4) == 0
 
     def distill(rows=2, n1=2, v=8, dt=0, t=VP, tdt=0, k=2, temp=1.0, red=0, loss=VP, norm=None, ws=VP, nbytes=big):
         return lib.fl_distill_fwd(VP, rows, n1, 8, 8, v, dt, t, tdt, VP, k, temp, red, loss, VP, VP, norm, ws, nbytes,

@@ -24,20 +24,18 @@ namespace {
 // Element types
 // ---------------------------------------------------------------------------
 template <int DT> struct Io;
-template <> struct Io<kF32> {
-    typedef float T;
-    static constexpr int kParts = 3;
-    static constexpr bool kHalf = false;
+template <> struct Io<kF32> { typedef float T; };
+template <> struct Io<kF16> { typedef _Float16 T; };
+template <> struct Io<kBF16> { typedef bf16_t T; };
+
+// How a product takes its operands: the number of parts and their type.
+template <int DT> struct Logits {  // x and w in the logits
+    static constexpr int kParts = DT == kF32 ? 2 : 1;
+    static constexpr bool kHalf = DT != kBF16;
 };
-template <> struct Io<kF16> {
-    typedef _Float16 T;
-    static constexpr int kParts = 1;
-    static constexpr bool kHalf = true;
-};
-template <> struct Io<kBF16> {
-    typedef bf16_t T;
-    static constexpr int kParts = 1;
-    static constexpr bool kHalf = false;
+template <int DT> struct Grads {   // G, w and x in dx and dw
+    static constexpr int kParts = DT == kF32 ? 3 : 1;
+    static constexpr bool kHalf = DT == kF16;
 };
 
 template <int DT>
@@ -46,12 +44,13 @@ __device__ __forceinline__ uint16_t half_bits(float v) {
     else return __builtin_bit_cast(uint16_t, (__bf16)v);
 }
 
-// A value as its 16-bit matrix operands: exact for x and w; G, computed in
-// fp32, is rounded to nearest even in fp16 and bf16 (its share of the error of
-// dx and dw is that of one rounding of a term of their sums) and exact in fp32.
-template <int DT>
-__device__ __forceinline__ void to_parts(float v, uint16_t (&o)[Io<DT>::kParts]) {
-    if constexpr (DT == kF32) split3(v, o);
+// A value as its matrix operands.  x and w are exact in fp16 and bf16; G,
+// computed in fp32, is rounded to nearest even there (its share of the error
+// of dx and dw is that of one rounding of a term of their sums).
+template <int DT, int PARTS>
+__device__ __forceinline__ void to_parts(float v, uint16_t (&o)[PARTS]) {
+    if constexpr (PARTS == 3) split3(v, o);
+    else if constexpr (PARTS == 2) split2(v, o);
     else o[0] = half_bits<DT>(v);
 }
 
@@ -60,16 +59,16 @@ __device__ __forceinline__ void to_parts(float v, uint16_t (&o)[Io<DT>::kParts])
 // ---------------------------------------------------------------------------
 struct Head {          // at the workspace's start, written by the plan kernel
     int live;          // rows whose target is not ignore_index
-    int pad;
     float inv_scale;   // undoes the power of two that a and b carry
-    float pad2;
+    uint32_t big_x;    // fp32: bits of the largest finite magnitude in the live
+    uint32_t big_w;    //   rows of x, and in w
 };
 
 // ---------------------------------------------------------------------------
 // Plan: one block lists the live rows in order, and for the backward their
 // coefficients a and b, scaled by a power of two that brings the largest to
-// [2^9, 2^10): G in fp16 then loses nothing to its smallest values that a sum
-// of its row would show.
+// [2^13, 2^14): G in fp16 then loses 2^-39 of the largest at most to the type's
+// smallest values.
 // ---------------------------------------------------------------------------
 constexpr int kPlanThreads = 1024;
 
@@ -157,11 +156,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs p) {
             __syncthreads();
         }
         big = shf[0];
-        int e = 0;
-        if (big > 0.0f && __builtin_isfinite(big)) {
-            e = 10 - (__builtin_amdgcn_frexp_expf(big));
-            e = e < -100 ? -100 : e > 100 ? 100 : e;
-        }
+        const int e = scale_exp(big, 14);
         const float scale = __builtin_ldexpf(1.0f, e);
         if (threadIdx.x == 0) p.head->inv_scale = __builtin_ldexpf(1.0f, -e);
         at = at - mine;
@@ -170,23 +165,85 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs p) {
             p.b[at + k] *= scale;
         }
     }
-    if (threadIdx.x == 0) p.head->live = live;
+    if (threadIdx.x == 0) {
+        p.head->live = live;
+        p.head->big_x = p.head->big_w = 0;
+    }
+}
+
+// fp32: the largest finite magnitudes of the live rows of x (blocks before
+// `split`) and of w.  A maximum does not depend on the atomics' order.
+struct BigArgs {
+    const float* x;
+    int64_t ldx;
+    const int* rows;
+    const float* w;
+    int64_t ldw, v, d;
+    Head* head;
+    int split;
+};
+__global__ __launch_bounds__(256) void magnitudes(BigArgs p) {
+    const bool is_x = (int)blockIdx.x < p.split;
+    const int64_t n = is_x ? p.head->live : p.v;
+    const int64_t b = is_x ? blockIdx.x : blockIdx.x - p.split;
+    const int64_t blocks = is_x ? p.split : gridDim.x - p.split;
+    float big = 0.0f;
+    // 64 lanes a row, 4 rows at a time a block
+    for (int64_t r = b * 4 + (threadIdx.x >> 6); r < n; r += blocks * 4) {
+        const float* s = is_x ? p.x + (int64_t)p.rows[r] * p.ldx : p.w + r * p.ldw;
+        for (int64_t c = (int64_t)lane_id() * 4; c < p.d; c += 256) {
+            float v[4];
+            load_vec_part<float>(s + c, p.d - c, 0.0f, v);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float m = __builtin_fabsf(v[k]);
+                big = m < kInf ? fmaxf(big, m) : big;
+            }
+        }
+    }
+    big = fmaxf(big, reduce_partner<1>(big));
+    big = fmaxf(big, reduce_partner<2>(big));
+    big = fmaxf(big, reduce_partner<4>(big));
+    big = fmaxf(big, reduce_partner<8>(big));
+    big = fmaxf(big, reduce_partner<16>(big));
+    big = fmaxf(big, reduce_partner<32>(big));
+    if (lane_id() == 0 && big > 0.0f)
+        atomicMax(is_x ? &p.head->big_x : &p.head->big_w, __builtin_bit_cast(uint32_t, big));
+}
+
+// The scale of fp32 logits' operands, and what undoes both in a logit.
+__device__ __forceinline__ float operand_scale(uint32_t bits) {
+    return __builtin_ldexpf(1.0f, scale_exp(__builtin_bit_cast(float, bits), 15));
+}
+template <int DT>
+__device__ __forceinline__ float logit(float acc, float inv_x, float inv_w) {
+    return DT == kF32 ? acc * inv_x * inv_w : acc;
+}
+template <int DT>
+__device__ __forceinline__ void logit_scales(const Head* h, float& inv_x, float& inv_w) {
+    inv_x = inv_w = 1.0f;
+    if constexpr (DT == kF32) {
+        inv_x = 1.0f / operand_scale(h->big_x);
+        inv_w = 1.0f / operand_scale(h->big_w);
+    }
 }
 
 // ---------------------------------------------------------------------------
 // Packing: rows of x (the live ones) or w as 16-bit operands of ldp elements (a
 // multiple of 64), zero beyond D; 8 elements a thread.
 // ---------------------------------------------------------------------------
-template <int DT>
+// `big`: fp32 logits' operands, scaled by its power of two.
+template <int DT, int P>
 __global__ __launch_bounds__(256) void pack_rows(const typename Io<DT>::T* src, int64_t lds_, int64_t d, const int* rows,
-                                                 const int* live, int64_t n, uint16_t* dst, int64_t ldp,
-                                                 int64_t part) {
+                                                 const int* live, int64_t n, uint16_t* dst, int64_t ldp, int64_t part,
+                                                 const uint32_t* big) {
     typedef typename Io<DT>::T T;
-    constexpr int P = Io<DT>::kParts, VE = Elem<T>::kVec;
+    constexpr int VE = Elem<T>::kVec;
     const int64_t chunks = ldp / 8;
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     const int64_t r = i / chunks, c = i % chunks * 8;
     if (r >= (live ? *live : n)) return;
+    const float scale = P == 2 ? operand_scale(*big) : 1.0f;
     const T* s = src + (rows ? (int64_t)rows[r] : r) * lds_ + c;
     uint16_t o[8][P];
 #pragma unroll
@@ -194,7 +251,7 @@ __global__ __launch_bounds__(256) void pack_rows(const typename Io<DT>::T* src, 
         float v[VE];
         load_vec_part<T>(s + h, d - c - h, 0.0f, v);
 #pragma unroll
-        for (int k = 0; k < VE; ++k) to_parts<DT>(v[k], o[h + k]);
+        for (int k = 0; k < VE; ++k) to_parts<DT>(P == 2 ? v[k] * scale : v[k], o[h + k]);
     }
 #pragma unroll
     for (int k = 0; k < P; ++k) {
@@ -206,10 +263,16 @@ __global__ __launch_bounds__(256) void pack_rows(const typename Io<DT>::T* src, 
 }
 
 // ---------------------------------------------------------------------------
-// The products.  Tiles of 256 x 256 in eight waves of 128 x 64: two waves a
-// SIMD, so that one's LDS reads run beside the other's matrix instructions.
+// The products.  Large ones take tiles of 256 x 256 in eight waves of 128 x 64:
+// two waves a SIMD, so that one's LDS reads run beside the other's matrix
+// instructions.  Ones with too few such tiles take 128 x 128 (two blocks a CU)
+// or 64 x 64 in four waves.  Measured, bf16, K-major, us: 8192^3 897 / 957 /
+// 1452; (4096, 2048, K 1024) 29.2 / 21.7 / 29.1; (4096, 512, 768) 22.5 / 10.0 /
+// 8.6; (1024, 128, 256) 10.4 / 6.2 / 4.0.
 // ---------------------------------------------------------------------------
 typedef Shape<2, 4, 8, 4> Big;
+typedef Shape<2, 2, 4, 4> Mid;
+typedef Shape<2, 2, 2, 2> Small;
 
 #define FL_LCE_BUFFERS(S)                                     \
     __shared__ __attribute__((aligned(1024))) char buf0[kBufferBytes<S>]; \
@@ -252,8 +315,11 @@ __global__ __launch_bounds__(S::kThreads, 2) void logits_stats(StatArgs p) {
     A.init(p.w, tm * S::TM);
     B.init(p.x, tn * S::TN);
     f32x4 acc[S::FM][S::FN];
-    tile_product<S, true, true, Io<DT>::kHalf, Io<DT>::kParts>(A, B, 0, p.steps, acc, (lds_char*)buf0, (lds_char*)buf1);
+    tile_product<S, true, true, Logits<DT>::kHalf, Logits<DT>::kParts>(A, B, 0, p.steps, acc, (lds_char*)buf0,
+                                                                       (lds_char*)buf1);
     const Place<S> at(tm * S::TM, tn * S::TN);
+    float inv_x, inv_w;
+    logit_scales<DT>(p.head, inv_x, inv_w);
 #pragma unroll
     for (int j = 0; j < S::FN; ++j) {
         const int64_t n = at.n + j * 16;
@@ -264,8 +330,9 @@ __global__ __launch_bounds__(S::kThreads, 2) void logits_stats(StatArgs p) {
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 const int64_t m = at.m + i * 16 + q;
-                v[i * 4 + q] = m < p.v ? acc[i][j][q] : -kInf;
-                if (p.v0 + m == target && m < p.v) p.at_target[n] = acc[i][j][q];
+                const float l = logit<DT>(acc[i][j][q], inv_x, inv_w);
+                v[i * 4 + q] = m < p.v ? l : -kInf;
+                if (p.v0 + m == target && m < p.v) p.at_target[n] = l;
             }
         float m = -kInf, s = 0.0f;
         lse_fold<true>(m, s, v);
@@ -329,7 +396,7 @@ struct GradArgs {
 template <int DT, class S>
 __global__ __launch_bounds__(S::kThreads, 2) void logits_grad(GradArgs p) {
     FL_LCE_BUFFERS(S);
-    constexpr int P = Io<DT>::kParts;
+    constexpr int P = Grads<DT>::kParts;
     const int live = p.head->live;
     const int64_t tiles_n = (live + S::TN - 1) / S::TN;
     if (blockIdx.x >= p.tiles_m * tiles_n) return;
@@ -341,8 +408,11 @@ __global__ __launch_bounds__(S::kThreads, 2) void logits_grad(GradArgs p) {
     A.init(p.w, tm * S::TM);
     B.init(p.x, tn * S::TN);
     f32x4 acc[S::FM][S::FN];
-    tile_product<S, true, true, Io<DT>::kHalf, P>(A, B, 0, p.steps, acc, (lds_char*)buf0, (lds_char*)buf1);
+    tile_product<S, true, true, Logits<DT>::kHalf, Logits<DT>::kParts>(A, B, 0, p.steps, acc, (lds_char*)buf0,
+                                                                       (lds_char*)buf1);
     const Place<S> at(tm * S::TM, tn * S::TN);
+    float inv_x, inv_w;
+    logit_scales<DT>(p.head, inv_x, inv_w);
     const int64_t n_end = (live + kStep - 1) / kStep * kStep;
 #pragma unroll
     for (int j = 0; j < S::FN; ++j) {
@@ -356,7 +426,7 @@ __global__ __launch_bounds__(S::kThreads, 2) void logits_grad(GradArgs p) {
             uint16_t o[4][P];
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                float g = a * fexp2((acc[i][j][q] - lse) * kLog2e);
+                float g = a * fexp2((logit<DT>(acc[i][j][q], inv_x, inv_w) - lse) * kLog2e);
                 if (p.v0 + m + q == target) g += b;
                 to_parts<DT>(in && p.v0 + m + q < p.v ? g : 0.0f, o[q]);
             }
@@ -417,7 +487,7 @@ __global__ __launch_bounds__(S::kThreads, 2) void product(ProductArgs p) {
     A.init(p.a, tm * S::TM);
     B.init(p.b, tn * S::TN);
     f32x4 acc[S::FM][S::FN];
-    tile_product<S, false, DX, Io<DT>::kHalf, Io<DT>::kParts>(A, B, k0, k1, acc, (lds_char*)buf0, (lds_char*)buf1);
+    tile_product<S, false, DX, Grads<DT>::kHalf, Grads<DT>::kParts>(A, B, k0, k1, acc, (lds_char*)buf0, (lds_char*)buf1);
     const Place<S> at(tm * S::TM, tn * S::TN);
     const float inv = p.head->inv_scale;
     const bool whole = (p.ldc & 3) == 0;  // four results of a lane are one store
@@ -496,24 +566,34 @@ struct Layout {
     int64_t ldx;         // a packed row of x and w
     bool pack_w;         // w is packed a piece at a time
     int splits;          // of K in dx
-    int64_t head, rows, pos, tgt, at_target, loss_rows, part, parts, a, b, lse, xp, wp, g, acc, bytes;
+    int logits, dx, dw;  // the products' tiles: 256, 128 or 64
+    int64_t head, rows, pos, tgt, at_target, loss_rows, part, parts, a, b, lse, xp, xg, wp, wg, g, acc, bytes;
 };
 
-int parts_of(int dtype) { return dtype == kF32 ? 3 : 1; }
+// A product's tiles: the largest that fill most of the chip.
+int tile_size(int64_t m, int64_t n, int64_t copies) {
+    if (n > 128 && div_up(m, 256) * div_up(n, 256) * copies >= 192) return 256;
+    return div_up(m, 128) * div_up(n, 128) * copies >= 200 ? 128 : 64;
+}
 
-// Splits of K in dx: as few as fill the chip's 256 places evenly; a split costs
-// about 8 steps for its start and its sums.
-int dx_splits(int64_t tiles, int64_t steps) {
-    int best = 1;
-    int64_t cost = 0;
-    for (int s = 1; s <= 32 && s <= steps; ++s) {
-        const int64_t c = div_up(tiles * s, 256) * (div_up(steps, s) + 8);
-        if (s == 1 || c < cost) {
-            best = s;
-            cost = c;
+// Tiles and splits of K of dx, m x n results of `steps` of K.  A split costs
+// about 8 steps of a 256-tile for its start and its sums, and a chip holds 256
+// blocks of the largest tiles, 512 of the middle ones and 1024 of the smallest,
+// which take 0.5 and 0.25 of the step's time then.
+void dx_plan(int64_t m, int64_t n, int64_t steps, int& tile, int& splits) {
+    double best = 0.0;
+    for (int t = 256; t >= 64; t /= 2) {
+        const int64_t tiles = div_up(m, t) * div_up(n, t), slots = 256 * (256 / t);
+        const double cost_step = t / 256.0 * (t == 256 ? 1.0 : t == 128 ? 1.1 : 1.6);
+        for (int s = 1; s <= 32 && s <= steps; ++s) {
+            const double c = div_up(tiles * s, slots) * cost_step * (div_up(steps, s) + 8.0);
+            if (best == 0.0 || c < best) {
+                best = c;
+                tile = t;
+                splits = s;
+            }
         }
     }
-    return best;
 }
 
 // aligned: w's rows can be read as matrix operands where they are.
@@ -525,7 +605,7 @@ Layout layout(int64_t N, int64_t V, int64_t D, int dtype, bool bwd, bool aligned
         at += round_up(bytes, 256);
         return here;
     };
-    const int64_t parts = parts_of(dtype);
+    const int64_t lparts = dtype == kF32 ? 2 : 1, parts = dtype == kF32 ? 3 : 1;
     int64_t most = kPieceBytes / (2 * parts * round_up(N, 64)) / 256 * 256;
     if (most < 2048) most = 2048;
     l.ldx = round_up(D, 64);
@@ -535,18 +615,20 @@ Layout layout(int64_t N, int64_t V, int64_t D, int dtype, bool bwd, bool aligned
         if (most > fit) most = fit < 2048 ? 2048 : fit;
     } else if (!bwd) {
         // nothing of the workspace grows with a forward's piece; one launch holds
-        // 2^22 tiles easily
-        most = ((int64_t)1 << 22) / div_up(N, Big::TN) * 256;
+        // 2^22 tiles of any size easily
+        most = ((int64_t)1 << 22) / div_up(N, 64) * 64 / 256 * 256;
+        if (most < 2048) most = 2048;
     }
     l.piece = round_up(div_up(V, div_up(V, most)), 256);
     l.head = take(sizeof(Head));
     l.rows = take(4 * N);
     l.pos = take(4 * N);
     l.tgt = take(4 * N);
-    l.xp = take(2 * parts * N * l.ldx);
-    l.wp = take(l.pack_w ? 2 * parts * l.piece * l.ldx : 0);
+    l.xp = take(2 * lparts * N * l.ldx);
+    l.wp = take(l.pack_w ? 2 * lparts * l.piece * l.ldx : 0);
+    l.logits = tile_size(l.piece, N, 1);
     if (!bwd) {
-        l.parts = div_up(V, 128);
+        l.parts = div_up(V, l.logits / 2);
         l.at_target = take(4 * N);
         l.loss_rows = take(4 * N);
         l.part = take(8 * N * l.parts);
@@ -554,7 +636,11 @@ Layout layout(int64_t N, int64_t V, int64_t D, int dtype, bool bwd, bool aligned
         l.a = take(4 * N);
         l.b = take(4 * N);
         l.lse = take(4 * N);
-        l.splits = dx_splits(div_up(N, Big::TN) * div_up(D, Big::TM), l.piece / kStep);
+        dx_plan(D, N, l.piece / kStep, l.dx, l.splits);
+        l.dw = tile_size(D, l.piece, 1);
+        // fp32: x and w again in the gradients' parts
+        l.xg = dtype == kF32 ? take(2 * parts * N * l.ldx) : l.xp;
+        l.wg = dtype == kF32 ? take(2 * parts * l.piece * l.ldx) : l.wp;
         l.g = take(2 * parts * round_up(N, 64) * l.piece);
         l.acc = take(4 * l.splits * N * D);
     }
@@ -581,27 +667,55 @@ P* at(const Call& c, int64_t off) {
     return reinterpret_cast<P*>(c.ws + off);
 }
 
-// Rows v0 .. of w as a product's operand.
-template <int DT>
-Operand operand_w(const Call& c, const Layout& l, int64_t v0, int64_t rows) {
+// Rows v0 .. of w as an operand of P parts, packed at `to` where they have to be.
+template <int DT, int P>
+Operand operand_w(const Call& c, const Layout& l, int64_t v0, int64_t rows, int64_t to) {
     typedef typename Io<DT>::T T;
     const T* w = static_cast<const T*>(c.w) + v0 * c.ldw;
     if (!l.pack_w) return Operand{reinterpret_cast<const uint16_t*>(w), c.ldw, 0, (int)rows, l.ldx};
     const int64_t part = l.piece * l.ldx;
-    pack_rows<DT><<<dim3((unsigned)div_up(rows * (l.ldx / 8), 256)), 256, 0, c.s>>>(
-        w, c.ldw, c.D, nullptr, nullptr, rows, at<uint16_t>(c, l.wp), l.ldx, part);
-    return Operand{at<uint16_t>(c, l.wp), l.ldx, part, (int)rows, l.ldx};
+    pack_rows<DT, P><<<dim3((unsigned)div_up(rows * (l.ldx / 8), 256)), 256, 0, c.s>>>(
+        w, c.ldw, c.D, nullptr, nullptr, rows, at<uint16_t>(c, to), l.ldx, part, &at<Head>(c, l.head)->big_w);
+    return Operand{at<uint16_t>(c, to), l.ldx, part, (int)rows, l.ldx};
 }
 
-template <int DT>
-Operand operand_x(const Call& c, const Layout& l) {
+// The live rows of x, packed at `to`.
+template <int DT, int P>
+Operand operand_x(const Call& c, const Layout& l, int64_t to) {
     typedef typename Io<DT>::T T;
     const Head* head = at<Head>(c, l.head);
     const int64_t part = c.N * l.ldx;
-    pack_rows<DT><<<dim3((unsigned)div_up(c.N * (l.ldx / 8), 256)), 256, 0, c.s>>>(
-        static_cast<const T*>(c.x), c.ldx, c.D, at<int>(c, l.rows), &head->live, c.N, at<uint16_t>(c, l.xp), l.ldx,
-        part);
-    return Operand{at<uint16_t>(c, l.xp), l.ldx, part, (int)c.N, l.ldx};
+    pack_rows<DT, P><<<dim3((unsigned)div_up(c.N * (l.ldx / 8), 256)), 256, 0, c.s>>>(
+        static_cast<const T*>(c.x), c.ldx, c.D, at<int>(c, l.rows), &head->live, c.N, at<uint16_t>(c, to), l.ldx, part,
+        &head->big_x);
+    return Operand{at<uint16_t>(c, to), l.ldx, part, (int)c.N, l.ldx};
+}
+
+// fp32: the magnitudes that the logits' operands are scaled by.
+template <int DT>
+void run_magnitudes(const Call& c, const Layout& l) {
+    if constexpr (DT == kF32) {
+        auto blocks = [](int64_t rows) { return (int)(div_up(rows, 4) < 1024 ? div_up(rows, 4) : 1024); };
+        BigArgs b{};
+        b.x = static_cast<const float*>(c.x);
+        b.ldx = c.ldx;
+        b.rows = at<int>(c, l.rows);
+        b.w = static_cast<const float*>(c.w);
+        b.ldw = c.ldw;
+        b.v = c.V;
+        b.d = c.D;
+        b.head = at<Head>(c, l.head);
+        b.split = blocks(c.N);
+        magnitudes<<<dim3((unsigned)(b.split + blocks(c.V))), 256, 0, c.s>>>(b);
+    }
+}
+
+// Calls f with the shape of `tile`.
+template <typename F>
+void by_shape(int tile, F f) {
+    if (tile == 256) f(Big{});
+    else if (tile == 128) f(Mid{});
+    else f(Small{});
 }
 
 PlanArgs plan_args(const Call& c, const Layout& l) {
@@ -621,27 +735,30 @@ PlanArgs plan_args(const Call& c, const Layout& l) {
 
 template <int DT>
 void run_fwd(const Call& c, const Layout& l, float* loss, float* lse) {
-    typedef Big S;
     PlanArgs p = plan_args(c, l);
     p.loss_rows = c.reduction == 0 ? loss : at<float>(c, l.loss_rows);
     p.lse_out = lse;
     plan_kernel<false><<<1, kPlanThreads, 0, c.s>>>(p);
-    const Operand x = operand_x<DT>(c, l);
+    run_magnitudes<DT>(c, l);
+    const Operand x = operand_x<DT, Logits<DT>::kParts>(c, l, l.xp);
     for (int64_t v0 = 0; v0 < c.V; v0 += l.piece) {
         const int64_t rows = c.V - v0 < l.piece ? c.V - v0 : l.piece;
         StatArgs a{};
-        a.w = operand_w<DT>(c, l, v0, rows);
+        a.w = operand_w<DT, Logits<DT>::kParts>(c, l, v0, rows, l.wp);
         a.x = x;
         a.steps = l.ldx / kStep;
         a.head = p.head;
         a.tgt = p.tgt;
         a.v0 = v0;
         a.v = rows;
-        a.tiles_m = div_up(rows, S::TM);
-        a.part = at<float2>(c, l.part) + v0 / 128;
+        a.part = at<float2>(c, l.part) + v0 / (l.logits / 2);
         a.parts = l.parts;
         a.at_target = at<float>(c, l.at_target);
-        logits_stats<DT, S><<<dim3((unsigned)(div_up(c.N, S::TN) * a.tiles_m)), S::kThreads, 0, c.s>>>(a);
+        by_shape(l.logits, [&](auto shape) {
+            typedef decltype(shape) S;
+            a.tiles_m = div_up(rows, S::TM);
+            logits_stats<DT, S><<<dim3((unsigned)(div_up(c.N, S::TN) * a.tiles_m)), S::kThreads, 0, c.s>>>(a);
+        });
     }
     finish_rows<<<dim3((unsigned)div_up(c.N, 4)), 256, 0, c.s>>>(p.head, p.rows, p.tgt, at<float2>(c, l.part), l.parts,
                                                                  at<float>(c, l.at_target), c.z, p.loss_rows, lse);
@@ -651,7 +768,6 @@ void run_fwd(const Call& c, const Layout& l, float* loss, float* lse) {
 template <int DT>
 void run_bwd(const Call& c, const Layout& l, const float* grad, const float* lse, void* dx, void* dw) {
     typedef typename Io<DT>::T T;
-    typedef Big S;
     PlanArgs p = plan_args(c, l);
     p.grad = grad;
     p.grad_stride = c.reduction == 0 ? 1 : 0;
@@ -660,13 +776,15 @@ void run_bwd(const Call& c, const Layout& l, const float* grad, const float* lse
     p.b = at<float>(c, l.b);
     p.lse = at<float>(c, l.lse);
     plan_kernel<true><<<1, kPlanThreads, 0, c.s>>>(p);
-    const Operand x = operand_x<DT>(c, l);
-    const int64_t tiles_n = div_up(c.N, S::TN), tiles_d = div_up(c.D, S::TM);
+    run_magnitudes<DT>(c, l);
+    constexpr int LP = Logits<DT>::kParts, GP = Grads<DT>::kParts;
+    const Operand x = operand_x<DT, LP>(c, l, l.xp);
+    const Operand xg = DT == kF32 && dw ? operand_x<DT, GP>(c, l, l.xg) : x;
     const int64_t g_part = round_up(c.N, 64) * l.piece;
     for (int64_t v0 = 0; v0 < c.V; v0 += l.piece) {
         const int64_t rows = c.V - v0 < l.piece ? c.V - v0 : l.piece;
         GradArgs g{};
-        g.w = operand_w<DT>(c, l, v0, rows);
+        g.w = operand_w<DT, LP>(c, l, v0, rows, l.wp);
         g.x = x;
         g.steps = l.ldx / kStep;
         g.head = p.head;
@@ -676,18 +794,20 @@ void run_bwd(const Call& c, const Layout& l, const float* grad, const float* lse
         g.lse = p.lse;
         g.v0 = v0;
         g.v = v0 + rows;
-        g.tiles_m = div_up(rows, S::TM);
         g.g = at<uint16_t>(c, l.g);
         g.ldg = l.piece;
         g.g_part = g_part;
-        logits_grad<DT, S><<<dim3((unsigned)(tiles_n * g.tiles_m)), S::kThreads, 0, c.s>>>(g);
+        by_shape(l.logits, [&](auto shape) {
+            typedef decltype(shape) S;
+            g.tiles_m = div_up(rows, S::TM);
+            logits_grad<DT, S><<<dim3((unsigned)(div_up(c.N, S::TN) * g.tiles_m)), S::kThreads, 0, c.s>>>(g);
+        });
         ProductArgs a{};
         a.head = p.head;
         a.m = c.D;
-        a.tiles_m = tiles_d;
         a.ldc = c.D;
         if (dx) {
-            a.a = g.w;
+            a.a = DT == kF32 ? operand_w<DT, GP>(c, l, v0, rows, l.wg) : g.w;
             a.b = Operand{g.g, l.piece, g_part, (int)c.N, l.piece};
             a.steps = div_up(rows, kStep);
             a.n = c.N;
@@ -695,15 +815,23 @@ void run_bwd(const Call& c, const Layout& l, const float* grad, const float* lse
             a.acc = at<float>(c, l.acc);
             a.split_stride = c.N * c.D;
             a.add = v0 > 0;
-            product<DT, S, true><<<dim3((unsigned)(tiles_d * tiles_n * l.splits)), S::kThreads, 0, c.s>>>(a);
+            by_shape(l.dx, [&](auto shape) {
+                typedef decltype(shape) S;
+                a.tiles_m = div_up(c.D, S::TM);
+                product<DT, S, true><<<dim3((unsigned)(a.tiles_m * div_up(c.N, S::TN) * l.splits)), S::kThreads, 0, c.s>>>(a);
+            });
         }
         if (dw) {
-            a.a = x;
+            a.a = xg;
             a.b = Operand{g.g, l.piece, g_part, 0, l.piece};
             a.n = rows;
             a.splits = 1;
             a.out = static_cast<T*>(dw) + v0 * c.D;
-            product<DT, S, false><<<dim3((unsigned)(tiles_d * div_up(rows, S::TN))), S::kThreads, 0, c.s>>>(a);
+            by_shape(l.dw, [&](auto shape) {
+                typedef decltype(shape) S;
+                a.tiles_m = div_up(c.D, S::TM);
+                product<DT, S, false><<<dim3((unsigned)(a.tiles_m * div_up(rows, S::TN))), S::kThreads, 0, c.s>>>(a);
+            });
         }
     }
     if (dx)

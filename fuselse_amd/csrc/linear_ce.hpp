@@ -21,27 +21,52 @@ enum DType { kF32 = 0, kF16 = 1, kBF16 = 2 };
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
-// The matrix cores take 16-bit operands.  fp16 and bf16 go in as they are.  An
-// fp32 value is the sum of three bf16 parts of 8 bits each (truncated, so
-// that the first part of a large value does not overflow), and a product of
-// two is the six partial products whose parts' indices add up to at most 2;
-// the ones left out are below 2^-21 of the product together.  The bf16 matrix
-// rate is 16 times the fp32 one, so six products cost 0.375 of one fp32
-// product.
-constexpr int kTerms = 6;
-__device__ constexpr int kTermA[kTerms] = {0, 0, 1, 1, 0, 2};
-__device__ constexpr int kTermB[kTerms] = {0, 1, 0, 1, 2, 0};
+// The matrix cores take 16-bit operands.  fp16 and bf16 go in as they are; fp32
+// goes in as parts, whose products' parts' indices add up to less than their
+// number.
+//
+// Logits: two fp16 parts of 11 bits, taken after a power of two that brings the
+// tensor's largest finite magnitude to [2^14, 2^15).  An element is then exact
+// to 2^-23 of itself or 2^-39 of the largest, whichever is more; three partial
+// products, the one left out below 2^-22 of the product.
+//
+// dx and dw: three bf16 parts of 8 bits, truncated, so that the first part of a
+// large value does not overflow: exact at any magnitude, which G, whose
+// entries reach from 1 down to nothing, needs and fp16's exponents do not
+// give.  Six partial products; those left out are below 2^-21 of the product
+// together.
+//
+// The 16-bit matrix rate is 16 times the fp32 one, so three products cost 0.19
+// and six 0.375 of one fp32 product.
+__device__ constexpr int terms(int parts) { return parts == 1 ? 1 : parts == 2 ? 3 : 6; }
+// parts of term t: 00 01 10 | 11 02 20
+__device__ constexpr int term_a(int t) { return t == 2 || t == 3 ? 1 : t == 5 ? 2 : 0; }
+__device__ constexpr int term_b(int t) { return t == 1 || t == 3 ? 1 : t == 4 ? 2 : 0; }
 
+__device__ __forceinline__ void split2(float v, uint16_t (&o)[2]) {
+    const _Float16 hi = (_Float16)v;
+    // an infinite part has no rest
+    const _Float16 lo = __builtin_isfinite(v) ? (_Float16)(v - (float)hi) : (_Float16)0.0f;
+    o[0] = __builtin_bit_cast(uint16_t, hi);
+    o[1] = __builtin_bit_cast(uint16_t, lo);
+}
 __device__ __forceinline__ void split3(float v, uint16_t (&o)[3]) {
     const uint32_t u = __builtin_bit_cast(uint32_t, v);
     o[0] = (uint16_t)(u >> 16);
-    const float r1 = v - __builtin_bit_cast(float, u & 0xFFFF0000u);
     // a part that is inf or NaN has no rest
-    const bool fin = __builtin_isfinite(v);
-    const uint32_t u1 = fin ? __builtin_bit_cast(uint32_t, r1) : 0u;
+    const float r1 = __builtin_isfinite(v) ? v - __builtin_bit_cast(float, u & 0xFFFF0000u) : 0.0f;
+    const uint32_t u1 = __builtin_bit_cast(uint32_t, r1);
     o[1] = (uint16_t)(u1 >> 16);
-    const float r2 = __builtin_bit_cast(float, u1) - __builtin_bit_cast(float, u1 & 0xFFFF0000u);
+    const float r2 = r1 - __builtin_bit_cast(float, u1 & 0xFFFF0000u);
     o[2] = (uint16_t)(__builtin_bit_cast(uint32_t, r2) >> 16);
+}
+
+// Exponent e of the power of two that brings a magnitude m to [2^(to - 1),
+// 2^to), within what fp32 holds; 0 for nothing, inf and NaN.
+__device__ __forceinline__ int scale_exp(float m, int to) {
+    if (!(m > 0.0f) || !__builtin_isfinite(m)) return 0;
+    const int e = to - __builtin_amdgcn_frexp_expf(m);
+    return e < -114 ? -114 : e > 114 ? 114 : e;
 }
 
 // One product's operand: 16-bit rows `ld` elements apart, in `parts` copies

@@ -5,14 +5,30 @@
 // matrix is transposed in HBM: K-major (rows of K, as x and w in the logits) or
 // row-major across K (K rows of the tile's M or N entries, as w in dx = G w).
 // Both are copied to LDS as they lie by 16-byte direct-to-LDS loads, 64 of K a
-// step, two steps' buffers in turn: while a step's products run, the next
-// step's loads are in flight, and one barrier a step orders them.  K-major
-// fragments are 16-byte LDS reads; the others come through ds_read_b64_tr_b16,
-// which hands each lane four consecutive K entries of its column.  The 16-byte
-// chunks of an LDS row are permuted by an exclusive or with the row number, so
-// that the lanes of one read meet different banks; the loads' lane addresses
-// apply it, since a direct-to-LDS load writes its lanes' data in lane order.
+// step, into two buffers in turn.  K-major fragments are 16-byte LDS reads; the
+// others come through ds_read_b64_tr_b16, which hands each lane four
+// consecutive K entries of its column.  The 16-byte chunks of an LDS row are
+// permuted by an exclusive or with bits of the row number, so that the lanes
+// that one cycle of a read serves meet different banks (measured: no bank
+// conflicts in either kind of read); the loads' lane addresses apply the
+// permutation, since a direct-to-LDS load writes its lanes' data in lane order.
+//
+// A step is four phases of a quarter of its products each (one half of K, one
+// half of the wave's rows).  A phase's fragments are read during the phase
+// before, and the loads for the step after next are spread over two phases,
+// one behind every few matrix instructions: issued together they stall a wave
+// for as long as half a step's products take.  One barrier a step, before the
+// phase that first reads the next buffer.
+//
+// Measured at 8192^3 in bf16: 830 us, 1324 TFLOP/s (the library's product:
+// 849 us), the matrix pipe busy 73% of cycles at the 1.73 GHz the card then
+// holds; with all of a step's loads issued at its start 870 us at 1.96 GHz and
+// 62%.  v_mfma 32x32x16 in place of 16x16x32 took 3% fewer cycles and 7% more
+// time: the clock falls further.
 #pragma once
+
+#include <type_traits>
+#include <utility>
 
 #include "linear_ce.hpp"
 
@@ -60,6 +76,16 @@ __device__ __forceinline__ const char* uniform(const char* p) {
 }
 __device__ __forceinline__ void wait_copies() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
+template <int N, typename F, int... I>
+__device__ __forceinline__ void unrolled_(F&& f, std::integer_sequence<int, I...>) {
+    (f(std::integral_constant<int, I>{}), ...);
+}
+// f(integral_constant 0), .., f(integral_constant N - 1)
+template <int N, typename F>
+__device__ __forceinline__ void unrolled(F&& f) {
+    unrolled_<N>(f, std::make_integer_sequence<int, N>{});
+}
+
 // WM x WN waves of FM x FN results of 16 x 16 each.
 template <int WM_, int WN_, int FM_, int FN_>
 struct Shape {
@@ -106,30 +132,38 @@ struct Side {
             for (int j = 0; j < kLoads; ++j) off[j] = (uint32_t)(krow(j) * ld) + col(j, first, o.cols);
         }
     }
+    // across: the permutation of K row k's chunks.  The 32 lanes that a cycle of
+    // a transposing read serves hold 2 chunks each of K rows 0 .. 3 and of those
+    // 8 or 16 further; their 16 chunks have to differ in the 256 bytes that the
+    // banks span, in which a row of 64 has a half of its own.
+    __device__ __forceinline__ static int swz(int k) {
+        const int far = ((k >> 3) ^ (k >> 4)) & 1;
+        if constexpr (T == 64) return (k & 2) | (far << 2);
+        else return ((k & 3) << 1) | (far << 3);
+    }
     // across: the K row and the column's byte of this lane's chunk in load j
     __device__ __forceinline__ static int krow(int j) {
         return ((j * S::kWaves + (int)(threadIdx.x >> 6)) * 1024 + (int)(threadIdx.x & 63) * 16) / kRowBytes;
     }
     __device__ __forceinline__ static uint32_t col(int j, int64_t first, int64_t cols) {
         const int slot = (int)(threadIdx.x & 63) * 16 % kRowBytes / 16;
-        int64_t c = (slot ^ ((krow(j) & 3) << 1)) * 8;
+        int64_t c = (slot ^ swz(krow(j))) * 8;
         if (first + c > cols - 8) c = cols - 8 - first;
         return (uint32_t)(c * 2);  // never before the row: first < cols
     }
 
-    // Starts the loads of step k (and part p) into buf.  `ragged`: the K rows
-    // end inside this step; those past the last are read as the last.
+    // Starts load J of step k (of part p) into buf.  Where the K rows end inside
+    // the step, those past the last are read as the last.
+    template <int J>
     __device__ __forceinline__ void load(lds_char* buf, int64_t k, int p) const {
         const char* b = uniform(base + k * step + p * part);
         const uint32_t lds = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)buf + (threadIdx.x >> 6) * 1024);
-        const bool ragged = !KMAJOR && (k + 1) * kStep > rows;
-        const int last = rows - 1 - (int)(k * kStep);
-#pragma unroll
-        for (int j = 0; j < kLoads; ++j) {
-            uint32_t o = off[j];
-            if (ragged) o -= krow(j) > last ? (uint32_t)((krow(j) - last) * ld) : 0u;
-            load_to_lds(b, o, lds + j * S::kWaves * 1024);
+        uint32_t o = off[J];
+        if (!KMAJOR && (k + 1) * kStep > rows) {
+            const int last = rows - 1 - (int)(k * kStep);
+            o -= krow(J) > last ? (uint32_t)((krow(J) - last) * ld) : 0u;
         }
+        load_to_lds(b, o, lds + J * S::kWaves * 1024);
     }
 
     // Fragment of 16 rows from row0 (a multiple of 16) and K half kk.
@@ -143,7 +177,7 @@ struct Side {
             const int i = lane & 15;
             const int k = kk * 32 + (lane >> 4) * 8 + (i >> 2);
             const int m = row0 + (i & 3) * 4;
-            const int at = k * kRowBytes + ((m >> 3) ^ ((i >> 2) << 1)) * 16 + (m & 7) * 2;
+            const int at = k * kRowBytes + ((m >> 3) ^ swz(k)) * 16 + (m & 7) * 2;
             const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(buf + at));
             const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                 (__attribute__((address_space(3))) s16x4*)(buf + at + 4 * kRowBytes));
@@ -188,46 +222,90 @@ __device__ __forceinline__ void tile_product(const Side<S, S::TM, AK>& A, const 
     for (int i = 0; i < S::FM; ++i)
 #pragma unroll
         for (int j = 0; j < S::FN; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    constexpr int TERMS = PARTS == 3 ? kTerms : 1;
+    constexpr int TERMS = terms(PARTS);
     const int64_t steps = (k1 - k0) * TERMS;
-    auto load = [&](lds_char* buf, int64_t s) {
-        if constexpr (PARTS == 3) {
-            const int64_t k = k0 + s / kTerms;
-            const int t = (int)(s % kTerms);
-            A.load(buf, k, kTermA[t]);
-            B.load(buf + SA::kBytes, k, kTermB[t]);
-        } else {
-            A.load(buf, k0 + s, 0);
-            B.load(buf + SA::kBytes, k0 + s, 0);
-        }
-    };
-    auto compute = [&](const lds_char* buf) {
-#pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-            u32x4 fa[S::FM], fb[S::FN];
-#pragma unroll
-            for (int j = 0; j < S::FN; ++j) fb[j] = SB::frag(buf + SA::kBytes, wn + j * 16, kk);
-#pragma unroll
-            for (int i = 0; i < S::FM; ++i) fa[i] = SA::frag(buf, wm + i * 16, kk);
-#pragma unroll
-            for (int i = 0; i < S::FM; ++i)
-#pragma unroll
-                for (int j = 0; j < S::FN; ++j) acc[i][j] = mfma<HALF>(fa[i], fb[j], acc[i][j]);
-        }
-    };
     if (steps <= 0) return;
-    load(buf0, 0);
+    constexpr int kLoads = SA::kLoads + SB::kLoads, kHalf = kLoads / 2;
+    // loads J0 .. J0 + N - 1 of step s
+    auto load = [&](auto j0, auto n, lds_char* buf, int64_t s) {
+        int64_t k = k0 + s;
+        int ta = 0, tb = 0;
+        if constexpr (TERMS > 1) {
+            k = k0 + s / TERMS;
+            const int t = (int)(s % TERMS);
+            ta = term_a(t);
+            tb = term_b(t);
+        }
+        unrolled<decltype(n)::value>([&](auto i) {
+            constexpr int J = decltype(j0)::value + decltype(i)::value;
+            if constexpr (J < SA::kLoads) A.template load<J>(buf, k, ta);
+            else B.template load<J - SA::kLoads>(buf + SA::kBytes, k, tb);
+        });
+    };
+    constexpr int H = S::FM / 2;
+    static_assert(S::FM % 2 == 0 && kLoads >= 2, "phases take half of a wave's rows");
+    u32x4 fa[2][H], fb[2][S::FN];
+    auto read_a = [&](const lds_char* buf, auto p, int i) {
+        constexpr int P = decltype(p)::value;
+        fa[P & 1][i] = SA::frag(buf, wm + ((P & 1) * H + i) * 16, P >> 1);
+    };
+    auto read_b = [&](const lds_char* buf, auto p, int j) {
+        constexpr int P = decltype(p)::value;
+        fb[P >> 1][j] = SB::frag(buf + SA::kBytes, wn + j * 16, P >> 1);
+    };
+    typedef std::integral_constant<int, 0> C0;
+    typedef std::integral_constant<int, kHalf> CHalf;
+    typedef std::integral_constant<int, kLoads - kHalf> CRest;
+    load(C0{}, std::integral_constant<int, kLoads>{}, buf0, 0);
+    load(C0{}, CHalf{}, buf1, steps > 1 ? 1 : 0);
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kHalf) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < H; ++i) read_a(buf0, C0{}, i);
+#pragma unroll
+    for (int j = 0; j < S::FN; ++j) read_b(buf0, C0{}, j);
+    // Phase P: its products, with the reads of the phase after it (from rd) and
+    // loads J0 .. J0 + N - 1 of step ls (to ld) between them, in this order.
+    auto phase = [&](auto p, const lds_char* rd, auto j0, auto n, lds_char* ld, int64_t ls) {
+        constexpr int P = decltype(p)::value, Q = (P + 1) & 3;
+        typedef std::integral_constant<int, Q> CQ;
+        unrolled<H>([&](auto ic) {
+            constexpr int i = decltype(ic)::value, N = decltype(n)::value;
+            read_a(rd, CQ{}, i);
+            if constexpr ((Q & 1) == 0) {
+#pragma unroll
+                for (int j = i * S::FN / H; j < (i + 1) * S::FN / H; ++j) read_b(rd, CQ{}, j);
+            }
+#pragma unroll
+            for (int j = 0; j < S::FN; ++j)
+                acc[(P & 1) * H + i][j] = mfma<HALF>(fa[P & 1][i], fb[P >> 1][j], acc[(P & 1) * H + i][j]);
+            constexpr int first = i * N / H, count = (i + 1) * N / H - first;
+            if constexpr (count > 0)
+                load(std::integral_constant<int, decltype(j0)::value + first>{}, std::integral_constant<int, count>{}, ld,
+                     ls);
+            __builtin_amdgcn_sched_barrier(0);
+        });
+    };
+    // Step s in cur.  The first half of step s + 2's loads go to cur in phase 3,
+    // when every wave has read it, the others in phase 0 of the next step.  Past
+    // the last step the last one is loaded again, and not used.
+    const int64_t last = steps - 1;
+    auto step = [&](lds_char* cur, lds_char* nxt, int64_t s) {
+        phase(C0{}, cur, CHalf{}, CRest{}, nxt, s + 1 < last ? s + 1 : last);
+        phase(std::integral_constant<int, 1>{}, cur, C0{}, C0{}, nxt, 0);
+        phase(std::integral_constant<int, 2>{}, cur, C0{}, C0{}, nxt, 0);
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        phase(std::integral_constant<int, 3>{}, nxt, C0{}, CHalf{}, cur, s + 2 < last ? s + 2 : last);
+    };
     for (int64_t s = 0; s < steps; s += 2) {
-        wait_copies();
-        __syncthreads();
-        if (s + 1 < steps) load(buf1, s + 1);
-        compute(buf0);
+        step(buf0, buf1, s);
         if (s + 1 >= steps) break;
-        wait_copies();
-        __syncthreads();
-        if (s + 2 < steps) load(buf0, s + 2);
-        compute(buf1);
+        step(buf1, buf0, s + 1);
     }
+    wait_copies();
     __syncthreads();
 }
 

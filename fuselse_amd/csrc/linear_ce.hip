@@ -60,6 +60,7 @@ __device__ __forceinline__ void to_parts(float v, uint16_t (&o)[PARTS]) {
 struct Head {          // at the workspace's start, written by the plan kernel
     int live;          // rows whose target is not ignore_index
     float inv_scale;   // undoes the power of two that a and b carry
+    int splits;        // of K in dx
     uint32_t big_x;    // fp32: bits of the largest finite magnitude in the live
     uint32_t big_w;    //   rows of x, and in w
 };
@@ -72,20 +73,24 @@ struct Head {          // at the workspace's start, written by the plan kernel
 // ---------------------------------------------------------------------------
 constexpr int kPlanThreads = 1024;
 
+// Sum of v over the threads before this one, and over all.
 __device__ __forceinline__ int block_scan_excl(int v, int* sh, int* total) {
-    const int t = threadIdx.x;
-    sh[t] = v;
-    __syncthreads();
-    for (int d = 1; d < kPlanThreads; d <<= 1) {
-        const int add = t >= d ? sh[t - d] : 0;
-        __syncthreads();
-        sh[t] += add;
-        __syncthreads();
+    const int lane = lane_id(), wave = threadIdx.x >> 6;
+    int inc = v;
+    for (int d = 1; d < 64; d *= 2) {
+        const int up = __shfl_up(inc, d, 64);
+        inc += lane >= d ? up : 0;
     }
-    *total = sh[kPlanThreads - 1];
-    const int r = sh[t] - v;
+    if (lane == 63) sh[wave] = inc;
     __syncthreads();
-    return r;
+    int before = 0, all = 0;
+    for (int w = 0; w < kPlanThreads / 64; ++w) {
+        const int t = sh[w];
+        before += w < wave ? t : 0;
+        all += t;
+    }
+    *total = all;
+    return before + inc - v;
 }
 
 struct PlanArgs {
@@ -107,11 +112,37 @@ struct PlanArgs {
     float* a;
     float* b;
     float* lse;
+    int tile, tiles_m, steps;  // dx: its tiles, and products of a step's depth of the first piece
+    int most_splits;
+    int64_t room;              // rows of sums there is room for
+    float sum_cost;            // what a split's sums of a row cost at the end, in steps
 };
+
+// What a split's start and its sums of a tile cost: a tile is written and read
+// at the card's memory rate in about 16 steps.
+constexpr int kSplitSteps = 16;
+
+// Splits of K in dx over tiles that fill the chip's places unevenly: the
+// number with the least rounds of blocks times steps a block takes, and sums at
+// the end.  All lanes of a wave call it.
+__device__ __forceinline__ int dx_splits(const PlanArgs& p, int live) {
+    const int s = lane_id() + 1;
+    const int tiles = p.tiles_m * ((live + p.tile - 1) / p.tile), slots = 256 * (256 / p.tile);
+    const bool fits = s <= p.most_splits && (int64_t)s * live <= p.room;
+    const float cost = (float)((tiles * s + slots - 1) / slots) * (float)((p.steps + s - 1) / s + kSplitSteps) +
+                       p.sum_cost * (float)s * (float)live;
+    // the least cost, and the least s of those: positive floats order as their bits
+    uint64_t best = fits || s == 1 ? (uint64_t)__builtin_bit_cast(uint32_t, cost) << 32 | (uint32_t)s : ~0ull;
+    for (int d = 1; d < 64; d *= 2) {
+        const uint64_t other = __shfl_xor(best, d, 64);
+        best = other < best ? other : best;
+    }
+    return (int)(best & 127);
+}
 
 template <bool BWD>
 __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs p) {
-    __shared__ int sh[kPlanThreads];
+    __shared__ int sh[kPlanThreads / 64];
     const int64_t per = (p.n + kPlanThreads - 1) / kPlanThreads;
     const int64_t r0 = (int64_t)threadIdx.x * per;
     const int64_t r1 = r0 + per < p.n ? r0 + per : p.n;
@@ -148,17 +179,19 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs p) {
         ++at;
     }
     if constexpr (BWD) {
-        float* shf = reinterpret_cast<float*>(sh);
-        shf[threadIdx.x] = big;
+        for (int d = 1; d < 64; d *= 2) big = fmaxf(big, __shfl_xor(big, d, 64));
+        __shared__ float shf[kPlanThreads / 64];
+        if (lane_id() == 0) shf[threadIdx.x >> 6] = big;
         __syncthreads();
-        for (int d = kPlanThreads / 2; d > 0; d >>= 1) {
-            if ((int)threadIdx.x < d) shf[threadIdx.x] = fmaxf(shf[threadIdx.x], shf[threadIdx.x + d]);
-            __syncthreads();
-        }
         big = shf[0];
+        for (int w = 1; w < kPlanThreads / 64; ++w) big = fmaxf(big, shf[w]);
         const int e = scale_exp(big, 14);
         const float scale = __builtin_ldexpf(1.0f, e);
         if (threadIdx.x == 0) p.head->inv_scale = __builtin_ldexpf(1.0f, -e);
+        if (threadIdx.x < 64) {
+            const int splits = dx_splits(p, live);
+            if (threadIdx.x == 0) p.head->splits = splits;
+        }
         at = at - mine;
         for (int k = 0; k < mine; ++k) {
             p.a[at + k] *= scale;
@@ -188,17 +221,28 @@ __global__ __launch_bounds__(256) void magnitudes(BigArgs p) {
     const int64_t b = is_x ? blockIdx.x : blockIdx.x - p.split;
     const int64_t blocks = is_x ? p.split : gridDim.x - p.split;
     float big = 0.0f;
-    // 64 lanes a row, 4 rows at a time a block
+    auto take = [&](const float (&v)[4]) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float m = __builtin_fabsf(v[k]);
+            big = m < kInf ? fmaxf(big, m) : big;
+        }
+    };
+    // a wave a row, four vectors a lane in flight
     for (int64_t r = b * 4 + (threadIdx.x >> 6); r < n; r += blocks * 4) {
         const float* s = is_x ? p.x + (int64_t)p.rows[r] * p.ldx : p.w + r * p.ldw;
-        for (int64_t c = (int64_t)lane_id() * 4; c < p.d; c += 256) {
+        int64_t c = (int64_t)lane_id() * 4;
+        for (; c + 3 * 256 + 4 <= p.d; c += 4 * 256) {
+            float v[4][4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) load_vec_any<float>(s + c + k * 256, v[k]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) take(v[k]);
+        }
+        for (; c < p.d; c += 256) {
             float v[4];
             load_vec_part<float>(s + c, p.d - c, 0.0f, v);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const float m = __builtin_fabsf(v[k]);
-                big = m < kInf ? fmaxf(big, m) : big;
-            }
+            take(v);
         }
     }
     big = fmaxf(big, reduce_partner<1>(big));
@@ -207,7 +251,12 @@ __global__ __launch_bounds__(256) void magnitudes(BigArgs p) {
     big = fmaxf(big, reduce_partner<8>(big));
     big = fmaxf(big, reduce_partner<16>(big));
     big = fmaxf(big, reduce_partner<32>(big));
-    if (lane_id() == 0 && big > 0.0f)
+    __shared__ float sh[4];
+    if (lane_id() == 0) sh[threadIdx.x >> 6] = big;
+    __syncthreads();
+    big = fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3]));
+    // one atomic a block: they take turns at about 10 ns each
+    if (threadIdx.x == 0 && big > 0.0f)
         atomicMax(is_x ? &p.head->big_x : &p.head->big_w, __builtin_bit_cast(uint32_t, big));
 }
 
@@ -278,69 +327,95 @@ typedef Shape<2, 2, 2, 2> Small;
     __shared__ __attribute__((aligned(1024))) char buf0[kBufferBytes<S>]; \
     __shared__ __attribute__((aligned(1024))) char buf1[kBufferBytes<S>]
 
-// A lane's place in the tile's results.
-template <class S>
+// A lane's place in the results: that of acc[0][0][0].  PERM: A's rows are
+// permuted (acc[i][j][q] is then perm_at(i, q) rows further).
+template <class S, bool PERM = false>
 struct Place {
-    int64_t m, n;  // of acc[0][0][0]
-    __device__ __forceinline__ Place(int64_t m0, int64_t n0) {
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-        m = m0 + wave % S::WM * (S::FM * 16) + (lane >> 4) * 4;
+    int m, n;
+    __device__ __forceinline__ Place(int m0, int n0) {
+        const int lane = threadIdx.x & 63, wave = scalar(threadIdx.x >> 6);
+        m = m0 + wave % S::WM * (S::FM * 16) + (lane >> 4) * (PERM ? 8 : 4);
         n = n0 + wave / S::WM * (S::FN * 16) + (lane & 15);
     }
 };
 
+constexpr int perm_at(int i, int q) { return i / 2 * 32 + i % 2 * 4 + q; }
+
 struct StatArgs {
     Operand w, x;      // M: vocabulary rows, N: live rows
-    int64_t steps;
+    int steps;
     const Head* head;
     const int* tgt;
-    int64_t v0, v;     // the piece's first row, and its rows
-    int64_t tiles_m;
+    int v0, v;         // the piece's first row, and its rows
+    int tiles_m;
     float2* part;      // [live row][parts]: (max, sum)
     int64_t parts;
     float* at_target;  // [live row]
 };
 
 template <int DT, class S>
+struct StatJob {
+    StatArgs p;
+    int live;
+    int tiles_n;
+    float inv_x, inv_w;
+
+    typedef Side<S, S::TM, true> SA;
+    typedef Side<S, S::TN, true> SB;
+    struct Rows {
+        int target[S::FN];
+    };
+    __device__ __forceinline__ void place(int t, SA& A, SB& B) const {
+        const TileAt tile = tile_at(t, p.tiles_m, tiles_n);
+        A.template init<true>(p.w, tile.m * S::TM);
+        B.init(p.x, tile.n * S::TN);
+    }
+    __device__ __forceinline__ int first(int) const { return 0; }
+    __device__ __forceinline__ int steps(int) const { return p.steps; }
+    __device__ __forceinline__ Rows rows(int t) const {
+        const Place<S> at(0, tile_at(t, p.tiles_m, tiles_n).n * S::TN);
+        Rows r;
+#pragma unroll
+        for (int j = 0; j < S::FN; ++j) r.target[j] = at.n + j * 16 < live ? p.tgt[at.n + j * 16] : -1;
+        return r;
+    }
+    __device__ __forceinline__ void finish(int t, const Rows& r, const f32x4 (&acc)[S::FM][S::FN]) const {
+        const TileAt tile = tile_at(t, p.tiles_m, tiles_n);
+        const Place<S, true> at(tile.m * S::TM, tile.n * S::TN);
+        const int mw = at.m / (S::FM * 16);
+        const int left = p.v - at.m;  // the piece's rows from this lane's first
+#pragma unroll
+        for (int j = 0; j < S::FN; ++j) {
+            const int64_t n = at.n + j * 16;
+            const int hit = r.target[j] >= 0 && r.target[j] < p.v0 + p.v ? r.target[j] - p.v0 - at.m : -1;
+            float v[S::FM * 4];
+#pragma unroll
+            for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const float l = logit<DT>(acc[i][j][q], inv_x, inv_w);
+                    v[i * 4 + q] = perm_at(i, q) < left ? l : -kInf;
+                    if (perm_at(i, q) == hit) p.at_target[n] = l;
+                }
+            float m = -kInf, s = 0.0f;
+            lse_fold<true>(m, s, v);
+            lse_merge(m, s, exact_xor<16>(m), exact_xor<16>(s));
+            lse_merge(m, s, exact_xor<32>(m), exact_xor<32>(s));
+            if ((threadIdx.x & 63) < 16 && n < live && mw * (S::FM * 16) < p.v)
+                p.part[n * p.parts + mw] = make_float2(m, s);
+        }
+    }
+};
+
+template <int DT, class S>
 __global__ __launch_bounds__(S::kThreads, 2) void logits_stats(StatArgs p) {
     FL_LCE_BUFFERS(S);
-    const int live = p.head->live;
-    const int64_t tiles_n = (live + S::TN - 1) / S::TN;
-    if (blockIdx.x >= p.tiles_m * tiles_n) return;
-    int64_t tm, tn;
-    tile_at(xcd_tile(blockIdx.x, p.tiles_m * tiles_n), p.tiles_m, tiles_n, tm, tn);
-    p.x.rows = live;
-    Side<S, S::TM, true> A;
-    Side<S, S::TN, true> B;
-    A.init(p.w, tm * S::TM);
-    B.init(p.x, tn * S::TN);
-    f32x4 acc[S::FM][S::FN];
-    tile_product<S, true, true, Logits<DT>::kHalf, Logits<DT>::kParts>(A, B, 0, p.steps, acc, (lds_char*)buf0,
-                                                                       (lds_char*)buf1);
-    const Place<S> at(tm * S::TM, tn * S::TN);
-    float inv_x, inv_w;
-    logit_scales<DT>(p.head, inv_x, inv_w);
-#pragma unroll
-    for (int j = 0; j < S::FN; ++j) {
-        const int64_t n = at.n + j * 16;
-        const int target = n < live ? p.tgt[n] : -1;
-        float v[S::FM * 4];
-#pragma unroll
-        for (int i = 0; i < S::FM; ++i)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int64_t m = at.m + i * 16 + q;
-                const float l = logit<DT>(acc[i][j][q], inv_x, inv_w);
-                v[i * 4 + q] = m < p.v ? l : -kInf;
-                if (p.v0 + m == target && m < p.v) p.at_target[n] = l;
-            }
-        float m = -kInf, s = 0.0f;
-        lse_fold<true>(m, s, v);
-        lse_merge(m, s, exact_xor<16>(m), exact_xor<16>(s));
-        lse_merge(m, s, exact_xor<32>(m), exact_xor<32>(s));
-        const int64_t mw = at.m / (S::FM * 16);
-        if ((threadIdx.x & 63) < 16 && n < live && mw * (S::FM * 16) < p.v) p.part[n * p.parts + mw] = make_float2(m, s);
-    }
+    StatJob<DT, S> job{p, p.head->live};
+    job.p.x.rows = job.live;
+    job.tiles_n = (job.live + S::TN - 1) / S::TN;
+    logit_scales<DT>(p.head, job.inv_x, job.inv_w);
+    run_tiles<S, true, true, Logits<DT>::kHalf, Logits<DT>::kParts>(job, p.tiles_m * job.tiles_n, (lds_char*)buf0,
+                                                                    (lds_char*)buf1);
 }
 
 // Joins a live row's pairs; one wave a row.
@@ -381,12 +456,12 @@ __global__ __launch_bounds__(1024) void reduce_rows(const Head* head, const floa
 
 struct GradArgs {
     Operand w, x;
-    int64_t steps;
+    int steps;
     const Head* head;
     const int* tgt;
     const float *a, *b, *lse;
-    int64_t v0, v;       // the piece: vocabulary rows v0 .. v - 1 are w's rows 0 ..
-    int64_t tiles_m;
+    int v0, v;           // the piece: vocabulary rows v0 .. v - 1 are w's rows 0 ..
+    int tiles_m;
     uint16_t* g;         // [live row][ldg]
     int64_t ldg, g_part;
 };
@@ -394,64 +469,94 @@ struct GradArgs {
 // G of a piece.  Rows from the live ones up to a multiple of 64 are zero, and so
 // are columns up to the tiles' end: the products' K runs over whole steps.
 template <int DT, class S>
-__global__ __launch_bounds__(S::kThreads, 2) void logits_grad(GradArgs p) {
-    FL_LCE_BUFFERS(S);
-    constexpr int P = Grads<DT>::kParts;
-    const int live = p.head->live;
-    const int64_t tiles_n = (live + S::TN - 1) / S::TN;
-    if (blockIdx.x >= p.tiles_m * tiles_n) return;
-    int64_t tm, tn;
-    tile_at(xcd_tile(blockIdx.x, p.tiles_m * tiles_n), p.tiles_m, tiles_n, tm, tn);
-    p.x.rows = live;
-    Side<S, S::TM, true> A;
-    Side<S, S::TN, true> B;
-    A.init(p.w, tm * S::TM);
-    B.init(p.x, tn * S::TN);
-    f32x4 acc[S::FM][S::FN];
-    tile_product<S, true, true, Logits<DT>::kHalf, Logits<DT>::kParts>(A, B, 0, p.steps, acc, (lds_char*)buf0,
-                                                                       (lds_char*)buf1);
-    const Place<S> at(tm * S::TM, tn * S::TN);
+struct GradJob {
+    GradArgs p;
+    int live;
+    int tiles_n;
     float inv_x, inv_w;
-    logit_scales<DT>(p.head, inv_x, inv_w);
-    const int64_t n_end = (live + kStep - 1) / kStep * kStep;
+
+    typedef Side<S, S::TM, true> SA;
+    typedef Side<S, S::TN, true> SB;
+    struct Rows {
+        int target[S::FN];
+        float a[S::FN], b[S::FN], lse[S::FN];
+    };
+    __device__ __forceinline__ void place(int t, SA& A, SB& B) const {
+        const TileAt tile = tile_at(t, p.tiles_m, tiles_n);
+        A.template init<true>(p.w, tile.m * S::TM);
+        B.init(p.x, tile.n * S::TN);
+    }
+    __device__ __forceinline__ int first(int) const { return 0; }
+    __device__ __forceinline__ int steps(int) const { return p.steps; }
+    __device__ __forceinline__ Rows rows(int t) const {
+        const Place<S> at(0, tile_at(t, p.tiles_m, tiles_n).n * S::TN);
+        Rows r;
 #pragma unroll
-    for (int j = 0; j < S::FN; ++j) {
-        const int64_t n = at.n + j * 16;
-        const bool in = n < live;
-        const int target = in ? p.tgt[n] : -1;
-        const float a = in ? p.a[n] : 0.0f, b = in ? p.b[n] : 0.0f, lse = in ? p.lse[n] : 0.0f;
+        for (int j = 0; j < S::FN; ++j) {
+            const int64_t n = at.n + j * 16;
+            const bool in = n < live;
+            r.target[j] = in ? p.tgt[n] : -1;
+            r.a[j] = in ? p.a[n] : 0.0f;
+            r.b[j] = in ? p.b[n] : 0.0f;
+            r.lse[j] = in ? p.lse[n] : 0.0f;
+        }
+        return r;
+    }
+    __device__ __forceinline__ void finish(int t, const Rows& r, const f32x4 (&acc)[S::FM][S::FN]) const {
+        constexpr int P = Grads<DT>::kParts;
+        const TileAt tile = tile_at(t, p.tiles_m, tiles_n);
+        const Place<S, true> at(tile.m * S::TM, tile.n * S::TN);
+        const int n_end = (live + kStep - 1) / kStep * kStep;
+        const int left = p.v - p.v0 - at.m;  // the piece's rows from this lane's first
 #pragma unroll
-        for (int i = 0; i < S::FM; ++i) {
-            const int64_t m = at.m + i * 16;
-            uint16_t o[4][P];
+        for (int j = 0; j < S::FN; ++j) {
+            const int64_t n = at.n + j * 16;
+            const int hit = r.target[j] >= 0 ? r.target[j] - p.v0 - at.m : -1;
+            // rows past the live ones have a = 0, but an exponential of anything
+            const int cols = n < live ? left : 0;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                float g = a * fexp2((logit<DT>(acc[i][j][q], inv_x, inv_w) - lse) * kLog2e);
-                if (p.v0 + m + q == target) g += b;
-                to_parts<DT>(in && p.v0 + m + q < p.v ? g : 0.0f, o[q]);
-            }
-            if (n < n_end) {
+            for (int i = 0; i < S::FM; i += 2) {
+                uint16_t o[8][P];
 #pragma unroll
-                for (int k = 0; k < P; ++k) {
-                    uint2 u;
-                    u.x = o[0][k] | (uint32_t)o[1][k] << 16;
-                    u.y = o[2][k] | (uint32_t)o[3][k] << 16;
-                    *reinterpret_cast<uint2*>(p.g + k * p.g_part + n * p.ldg + m) = u;
+                for (int q = 0; q < 8; ++q) {
+                    const int m = perm_at(i, q);  // q runs over both fragments
+                    float g = r.a[j] * fexp2((logit<DT>(acc[i + q / 4][j][q % 4], inv_x, inv_w) - r.lse[j]) * kLog2e);
+                    if (m == hit) g += r.b[j];
+                    to_parts<DT>(m < cols ? g : 0.0f, o[q]);
+                }
+                if (n < n_end) {
+#pragma unroll
+                    for (int k = 0; k < P; ++k) {
+                        u32x4 u;
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) u[q] = o[2 * q][k] | (uint32_t)o[2 * q + 1][k] << 16;
+                        *reinterpret_cast<u32x4*>(p.g + k * p.g_part + n * p.ldg + at.m + i * 16) = u;
+                    }
                 }
             }
         }
     }
+};
+
+template <int DT, class S>
+__global__ __launch_bounds__(S::kThreads, 2) void logits_grad(GradArgs p) {
+    FL_LCE_BUFFERS(S);
+    GradJob<DT, S> job{p, p.head->live};
+    job.p.x.rows = job.live;
+    job.tiles_n = (job.live + S::TN - 1) / S::TN;
+    logit_scales<DT>(p.head, job.inv_x, job.inv_w);
+    run_tiles<S, true, true, Logits<DT>::kHalf, Logits<DT>::kParts>(job, p.tiles_m * job.tiles_n, (lds_char*)buf0,
+                                                                    (lds_char*)buf1);
 }
 
 struct ProductArgs {
     Operand a, b;       // M and N rows
     const Head* head;
-    int64_t steps;      // of K; dw: the live rows'
-    int64_t m, n;       // results
-    int64_t tiles_m;
-    int splits;
-    float* acc;         // dx: [split][n][ldc] fp32 sums, added to when `add`
-    int64_t ldc, split_stride;
+    int steps;          // of K; dw: the live rows'
+    int m, n;           // results
+    int tiles_m;
+    float* acc;         // dx: [split][live row][ldc] fp32 sums, added to when `add`
+    int64_t ldc;
     int add;
     void* out;          // dw: [n][ldc] results
 };
@@ -459,92 +564,120 @@ struct ProductArgs {
 // dx (DX): C[n][d] = sum_v G[n][v] w[v][d] over a piece, added to the splits'
 // sums.  dw: C[v][d] = sum_n G[n][v] x[n][d], the piece's rows of the result.
 template <int DT, class S, bool DX>
-__global__ __launch_bounds__(S::kThreads, 2) void product(ProductArgs p) {
-    FL_LCE_BUFFERS(S);
+struct ProductJob {
+    ProductArgs p;
+    int n_end, tiles_n, tiles, splits;
+    float inv;
+    bool whole;  // four results of a lane are one store
+
     typedef typename Io<DT>::T T;
-    const int live = p.head->live;
-    const int64_t n_end = DX ? live : p.n;
-    const int64_t tiles_n = (n_end + S::TN - 1) / S::TN;
-    const int64_t tiles = p.tiles_m * tiles_n;
-    if (blockIdx.x >= tiles * p.splits) return;
-    const int64_t t = xcd_tile(blockIdx.x, tiles * p.splits);
-    const int split = (int)(t / tiles);
-    int64_t tm, tn;
-    tile_at(t % tiles, p.tiles_m, tiles_n, tm, tn);
-    int64_t k0 = 0, k1;
-    if constexpr (DX) {
-        p.b.rows = live;
-        const int64_t per = (p.steps + p.splits - 1) / p.splits;
-        k0 = split * per;
-        k1 = k0 + per < p.steps ? k0 + per : p.steps;
-    } else {
-        k1 = (live + kStep - 1) / kStep;
-        p.a.rows = live;
-        p.b.rows = (int)(k1 * kStep);
+    typedef Side<S, S::TM, false> SA;
+    typedef Side<S, S::TN, DX> SB;
+    struct Rows {};
+    __device__ __forceinline__ int split(int t) const { return DX ? scalar((unsigned)t / (unsigned)tiles) : 0; }
+    __device__ __forceinline__ TileAt at(int t) const { return tile_at(t - split(t) * tiles, p.tiles_m, tiles_n); }
+    // K's steps are cut evenly
+    __device__ __forceinline__ int first(int t) const {
+        return DX ? scalar((unsigned)(p.steps * split(t)) / (unsigned)splits) : 0;
     }
-    Side<S, S::TM, false> A;
-    Side<S, S::TN, DX> B;
-    A.init(p.a, tm * S::TM);
-    B.init(p.b, tn * S::TN);
-    f32x4 acc[S::FM][S::FN];
-    tile_product<S, false, DX, Grads<DT>::kHalf, Grads<DT>::kParts>(A, B, k0, k1, acc, (lds_char*)buf0, (lds_char*)buf1);
-    const Place<S> at(tm * S::TM, tn * S::TN);
-    const float inv = p.head->inv_scale;
-    const bool whole = (p.ldc & 3) == 0;  // four results of a lane are one store
+    __device__ __forceinline__ int steps(int t) const {
+        return DX ? scalar((unsigned)(p.steps * (split(t) + 1)) / (unsigned)splits) - first(t) : p.steps;
+    }
+    __device__ __forceinline__ void place(int t, SA& A, SB& B) const {
+        const TileAt tile = at(t);
+        A.init(p.a, tile.m * S::TM);
+        B.init(p.b, tile.n * S::TN);
+    }
+    __device__ __forceinline__ Rows rows(int) const { return Rows{}; }
+    __device__ __forceinline__ void finish(int t, const Rows&, const f32x4 (&acc)[S::FM][S::FN]) const {
+        const TileAt tile = at(t);
+        const Place<S> at(tile.m * S::TM, tile.n * S::TN);
+        float* sums = DX ? p.acc + (int64_t)split(t) * n_end * p.ldc : nullptr;
 #pragma unroll
-    for (int j = 0; j < S::FN; ++j) {
-        const int64_t n = at.n + j * 16;
-        if (n >= n_end) continue;
+        for (int j = 0; j < S::FN; ++j) {
+            const int64_t n = at.n + j * 16;
+            if (n >= n_end) continue;
 #pragma unroll
-        for (int i = 0; i < S::FM; ++i) {
-            const int64_t m = at.m + i * 16;
-            if (m >= p.m) continue;
-            f32x4 v = acc[i][j];
-            if constexpr (DX) {
-                float* c = p.acc + split * p.split_stride + n * p.ldc + m;
-                if (whole) {
-                    if (p.add) v += *reinterpret_cast<const f32x4*>(c);
-                    *reinterpret_cast<f32x4*>(c) = v;
+            for (int i = 0; i < S::FM; ++i) {
+                const int64_t m = at.m + i * 16;
+                if (m >= p.m) continue;
+                f32x4 v = acc[i][j];
+                if constexpr (DX) {
+                    float* c = sums + n * p.ldc + m;
+                    if (whole) {
+                        if (p.add) v += *reinterpret_cast<const f32x4*>(c);
+                        *reinterpret_cast<f32x4*>(c) = v;
+                    } else {
+#pragma unroll
+                        for (int q = 0; q < 4; ++q)
+                            if (m + q < p.m) c[q] = p.add ? c[q] + v[q] : v[q];
+                    }
                 } else {
+                    T* c = static_cast<T*>(p.out) + n * p.ldc + m;
+                    v *= inv;
+                    if (whole && sizeof(T) == 4) {
+                        *reinterpret_cast<f32x4*>(c) = v;
+                    } else if (whole) {
+                        uint16_t o[4];
 #pragma unroll
-                    for (int q = 0; q < 4; ++q)
-                        if (m + q < p.m) c[q] = p.add ? c[q] + v[q] : v[q];
-                }
-            } else {
-                T* c = static_cast<T*>(p.out) + n * p.ldc + m;
-                v *= inv;
-                if (whole && sizeof(T) == 4) {
-                    *reinterpret_cast<f32x4*>(c) = v;
-                } else if (whole) {
-                    uint16_t o[4];
+                        for (int q = 0; q < 4; ++q) o[q] = half_bits<DT>(v[q]);
+                        uint2 u;
+                        u.x = o[0] | (uint32_t)o[1] << 16;
+                        u.y = o[2] | (uint32_t)o[3] << 16;
+                        *reinterpret_cast<uint2*>(c) = u;
+                    } else {
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) o[q] = half_bits<DT>(v[q]);
-                    uint2 u;
-                    u.x = o[0] | (uint32_t)o[1] << 16;
-                    u.y = o[2] | (uint32_t)o[3] << 16;
-                    *reinterpret_cast<uint2*>(c) = u;
-                } else {
-#pragma unroll
-                    for (int q = 0; q < 4; ++q)
-                        if (m + q < p.m) Elem<T>::put(c + q, v[q]);
+                        for (int q = 0; q < 4; ++q)
+                            if (m + q < p.m) Elem<T>::put(c + q, v[q]);
+                    }
                 }
             }
         }
     }
+};
+
+template <int DT, class S, bool DX>
+__global__ __launch_bounds__(S::kThreads, 2) void product(ProductArgs p) {
+    FL_LCE_BUFFERS(S);
+    const int live = p.head->live;
+    ProductJob<DT, S, DX> job{p};
+    if constexpr (DX) {
+        job.p.b.rows = live;
+        job.n_end = live;
+        job.splits = p.head->splits < p.steps ? p.head->splits : p.steps;  // a short last piece adds to the first ones
+    } else {
+        job.p.steps = (live + kStep - 1) / kStep;
+        job.p.a.rows = live;
+        job.p.b.rows = job.p.steps * kStep;
+        job.n_end = p.n;
+        job.splits = 1;
+    }
+    job.tiles_n = (job.n_end + S::TN - 1) / S::TN;
+    job.tiles = p.tiles_m * job.tiles_n;
+    job.inv = p.head->inv_scale;
+    job.whole = (p.ldc & 3) == 0;
+    if (!DX && live == 0) {  // no step of K: dw is zero
+        f32x4 none[S::FM][S::FN] = {};
+        for (Walk w(job.tiles); w.t < w.end; w.t += w.stride) job.finish(w.t, {}, none);
+        return;
+    }
+    run_tiles<S, false, DX, Grads<DT>::kHalf, Grads<DT>::kParts>(job, job.tiles * job.splits, (lds_char*)buf0,
+                                                                 (lds_char*)buf1);
 }
 
 // dx rows from the splits' sums; ignored rows are zero.
 template <int DT>
-__global__ __launch_bounds__(256) void finish_dx(const Head* head, const int* pos, const float* acc, int splits,
-                                                 int64_t split_stride, int64_t d, void* dx) {
+__global__ __launch_bounds__(256) void finish_dx(const Head* head, const int* pos, const float* acc, int64_t d, void* dx) {
     typedef typename Io<DT>::T T;
     const int64_t r = blockIdx.x;
     const int at = pos[r];
     const float inv = head->inv_scale;
+    const int splits = head->splits;
+    const int64_t stride = head->live * d;
     for (int64_t c = threadIdx.x; c < d; c += 256) {
         float s = 0.0f;
         if (at >= 0) {
-            for (int k = 0; k < splits; ++k) s += acc[k * split_stride + at * d + c];
+            for (int k = 0; k < splits; ++k) s += acc[k * stride + at * d + c];
             s *= inv;
         }
         Elem<T>::put(static_cast<T*>(dx) + r * d + c, s);
@@ -565,7 +698,8 @@ struct Layout {
     int64_t piece;       // vocabulary rows of a piece, a multiple of 256
     int64_t ldx;         // a packed row of x and w
     bool pack_w;         // w is packed a piece at a time
-    int splits;          // of K in dx
+    int splits;          // of K in dx, with every row live
+    int64_t room;        // rows of its sums
     int logits, dx, dw;  // the products' tiles: 256, 128 or 64
     int64_t head, rows, pos, tgt, at_target, loss_rows, part, parts, a, b, lse, xp, xg, wp, wg, g, acc, bytes;
 };
@@ -576,17 +710,16 @@ int tile_size(int64_t m, int64_t n, int64_t copies) {
     return div_up(m, 128) * div_up(n, 128) * copies >= 200 ? 128 : 64;
 }
 
-// Tiles and splits of K of dx, m x n results of `steps` of K.  A split costs
-// about 8 steps of a 256-tile for its start and its sums, and a chip holds 256
-// blocks of the largest tiles, 512 of the middle ones and 1024 of the smallest,
-// which take 0.5 and 0.25 of the step's time then.
-void dx_plan(int64_t m, int64_t n, int64_t steps, int& tile, int& splits) {
+// Tiles of dx, m x n results of `steps` of K, and the splits that it has room
+// for, as dx_splits chooses them with every row live.
+void dx_plan(int64_t m, int64_t n, int64_t steps, int terms, int& tile, int& splits) {
     double best = 0.0;
     for (int t = 256; t >= 64; t /= 2) {
         const int64_t tiles = div_up(m, t) * div_up(n, t), slots = 256 * (256 / t);
-        const double cost_step = t / 256.0 * (t == 256 ? 1.0 : t == 128 ? 1.1 : 1.6);
-        for (int s = 1; s <= 32 && s <= steps; ++s) {
-            const double c = div_up(tiles * s, slots) * cost_step * (div_up(steps, s) + 8.0);
+        // a step of a tile in 1/256 of the chip, by the times beside the shapes
+        const double step = t == 256 ? 1.0 : t == 128 ? 0.55 : 0.4;
+        for (int s = 1; s <= 64 && s <= steps; ++s) {
+            const double c = div_up(tiles * s, slots) * step * (div_up(steps * terms, s) + kSplitSteps);
             if (best == 0.0 || c < best) {
                 best = c;
                 tile = t;
@@ -614,10 +747,7 @@ Layout layout(int64_t N, int64_t V, int64_t D, int dtype, bool bwd, bool aligned
         const int64_t fit = kPieceBytes / (2 * parts * l.ldx) / 256 * 256;
         if (most > fit) most = fit < 2048 ? 2048 : fit;
     } else if (!bwd) {
-        // nothing of the workspace grows with a forward's piece; one launch holds
-        // 2^22 tiles of any size easily
-        most = ((int64_t)1 << 22) / div_up(N, 64) * 64 / 256 * 256;
-        if (most < 2048) most = 2048;
+        most = V;  // nothing of the workspace grows with a forward's piece
     }
     l.piece = round_up(div_up(V, div_up(V, most)), 256);
     l.head = take(sizeof(Head));
@@ -636,13 +766,16 @@ Layout layout(int64_t N, int64_t V, int64_t D, int dtype, bool bwd, bool aligned
         l.a = take(4 * N);
         l.b = take(4 * N);
         l.lse = take(4 * N);
-        dx_plan(D, N, l.piece / kStep, l.dx, l.splits);
+        dx_plan(D, N, l.piece / kStep, terms((int)parts), l.dx, l.splits);
         l.dw = tile_size(D, l.piece, 1);
         // fp32: x and w again in the gradients' parts
         l.xg = dtype == kF32 ? take(2 * parts * N * l.ldx) : l.xp;
         l.wg = dtype == kF32 ? take(2 * parts * l.piece * l.ldx) : l.wp;
         l.g = take(2 * parts * round_up(N, 64) * l.piece);
-        l.acc = take(4 * l.splits * N * D);
+        // room for more splits where fewer rows are live
+        const int64_t rows = kPieceBytes / (4 * D);
+        l.room = l.splits * N > rows ? l.splits * N : rows > 64 * N ? 64 * N : rows;
+        l.acc = take(4 * l.room * D);
     }
     l.bytes = at;
     return l;
@@ -695,7 +828,7 @@ Operand operand_x(const Call& c, const Layout& l, int64_t to) {
 template <int DT>
 void run_magnitudes(const Call& c, const Layout& l) {
     if constexpr (DT == kF32) {
-        auto blocks = [](int64_t rows) { return (int)(div_up(rows, 4) < 1024 ? div_up(rows, 4) : 1024); };
+        auto blocks = [](int64_t rows, int64_t most) { return (int)(div_up(rows, 4) < most ? div_up(rows, 4) : most); };
         BigArgs b{};
         b.x = static_cast<const float*>(c.x);
         b.ldx = c.ldx;
@@ -705,9 +838,16 @@ void run_magnitudes(const Call& c, const Layout& l) {
         b.v = c.V;
         b.d = c.D;
         b.head = at<Head>(c, l.head);
-        b.split = blocks(c.N);
-        magnitudes<<<dim3((unsigned)(b.split + blocks(c.V))), 256, 0, c.s>>>(b);
+        b.split = blocks(c.N, 128);
+        magnitudes<<<dim3((unsigned)(b.split + blocks(c.V, 512))), 256, 0, c.s>>>(b);
     }
+}
+
+// Blocks for `tiles` tiles: no more than run at a time, in multiples of 8.
+template <class S>
+dim3 grid_of(int64_t tiles) {
+    constexpr int64_t most = 256 * (S::TM == 256 ? 1 : S::TM == 128 ? 2 : 4);
+    return dim3((unsigned)(tiles < most ? round_up(tiles, 8) : most));
 }
 
 // Calls f with the shape of `tile`.
@@ -746,18 +886,18 @@ void run_fwd(const Call& c, const Layout& l, float* loss, float* lse) {
         StatArgs a{};
         a.w = operand_w<DT, Logits<DT>::kParts>(c, l, v0, rows, l.wp);
         a.x = x;
-        a.steps = l.ldx / kStep;
+        a.steps = (int)(l.ldx / kStep);
         a.head = p.head;
         a.tgt = p.tgt;
-        a.v0 = v0;
-        a.v = rows;
+        a.v0 = (int)v0;
+        a.v = (int)rows;
         a.part = at<float2>(c, l.part) + v0 / (l.logits / 2);
         a.parts = l.parts;
         a.at_target = at<float>(c, l.at_target);
         by_shape(l.logits, [&](auto shape) {
             typedef decltype(shape) S;
-            a.tiles_m = div_up(rows, S::TM);
-            logits_stats<DT, S><<<dim3((unsigned)(div_up(c.N, S::TN) * a.tiles_m)), S::kThreads, 0, c.s>>>(a);
+            a.tiles_m = (int)div_up(rows, S::TM);
+            logits_stats<DT, S><<<grid_of<S>(div_up(c.N, S::TN) * a.tiles_m), S::kThreads, 0, c.s>>>(a);
         });
     }
     finish_rows<<<dim3((unsigned)div_up(c.N, 4)), 256, 0, c.s>>>(p.head, p.rows, p.tgt, at<float2>(c, l.part), l.parts,
@@ -775,6 +915,14 @@ void run_bwd(const Call& c, const Layout& l, const float* grad, const float* lse
     p.a = at<float>(c, l.a);
     p.b = at<float>(c, l.b);
     p.lse = at<float>(c, l.lse);
+    p.tile = l.dx;
+    p.tiles_m = (int)div_up(c.D, l.dx);
+    p.most_splits = (int)div_up(c.V < l.piece ? c.V : l.piece, kStep);
+    p.steps = p.most_splits * terms(Grads<DT>::kParts);
+    // a row's sums, 4 D bytes, at about 5 TB/s, once for all pieces; a step takes
+    // about 1.35 us
+    p.sum_cost = (float)((double)c.D * 4 / (5e12 * 1.35e-6) / (double)div_up(c.V, l.piece));
+    p.room = l.room;
     plan_kernel<true><<<1, kPlanThreads, 0, c.s>>>(p);
     run_magnitudes<DT>(c, l);
     constexpr int LP = Logits<DT>::kParts, GP = Grads<DT>::kParts;
@@ -786,57 +934,53 @@ void run_bwd(const Call& c, const Layout& l, const float* grad, const float* lse
         GradArgs g{};
         g.w = operand_w<DT, LP>(c, l, v0, rows, l.wp);
         g.x = x;
-        g.steps = l.ldx / kStep;
+        g.steps = (int)(l.ldx / kStep);
         g.head = p.head;
         g.tgt = p.tgt;
         g.a = p.a;
         g.b = p.b;
         g.lse = p.lse;
-        g.v0 = v0;
-        g.v = v0 + rows;
+        g.v0 = (int)v0;
+        g.v = (int)(v0 + rows);
         g.g = at<uint16_t>(c, l.g);
         g.ldg = l.piece;
         g.g_part = g_part;
         by_shape(l.logits, [&](auto shape) {
             typedef decltype(shape) S;
-            g.tiles_m = div_up(rows, S::TM);
-            logits_grad<DT, S><<<dim3((unsigned)(div_up(c.N, S::TN) * g.tiles_m)), S::kThreads, 0, c.s>>>(g);
+            g.tiles_m = (int)div_up(rows, S::TM);
+            logits_grad<DT, S><<<grid_of<S>(div_up(c.N, S::TN) * g.tiles_m), S::kThreads, 0, c.s>>>(g);
         });
         ProductArgs a{};
         a.head = p.head;
-        a.m = c.D;
+        a.m = (int)c.D;
         a.ldc = c.D;
         if (dx) {
             a.a = DT == kF32 ? operand_w<DT, GP>(c, l, v0, rows, l.wg) : g.w;
             a.b = Operand{g.g, l.piece, g_part, (int)c.N, l.piece};
-            a.steps = div_up(rows, kStep);
-            a.n = c.N;
-            a.splits = l.splits;
+            a.steps = (int)div_up(rows, kStep);
+            a.n = (int)c.N;
             a.acc = at<float>(c, l.acc);
-            a.split_stride = c.N * c.D;
             a.add = v0 > 0;
             by_shape(l.dx, [&](auto shape) {
                 typedef decltype(shape) S;
-                a.tiles_m = div_up(c.D, S::TM);
-                product<DT, S, true><<<dim3((unsigned)(a.tiles_m * div_up(c.N, S::TN) * l.splits)), S::kThreads, 0, c.s>>>(a);
+                a.tiles_m = (int)div_up(c.D, S::TM);
+                product<DT, S, true><<<grid_of<S>((int64_t)a.tiles_m * (div_up(c.N, S::TN) * l.splits + 64)), S::kThreads, 0, c.s>>>(a);
             });
         }
         if (dw) {
             a.a = xg;
             a.b = Operand{g.g, l.piece, g_part, 0, l.piece};
-            a.n = rows;
-            a.splits = 1;
+            a.n = (int)rows;
             a.out = static_cast<T*>(dw) + v0 * c.D;
             by_shape(l.dw, [&](auto shape) {
                 typedef decltype(shape) S;
-                a.tiles_m = div_up(c.D, S::TM);
-                product<DT, S, false><<<dim3((unsigned)(a.tiles_m * div_up(rows, S::TN))), S::kThreads, 0, c.s>>>(a);
+                a.tiles_m = (int)div_up(c.D, S::TM);
+                product<DT, S, false><<<grid_of<S>((int64_t)a.tiles_m * div_up(rows, S::TN)), S::kThreads, 0, c.s>>>(a);
             });
         }
     }
     if (dx)
-        finish_dx<DT><<<dim3((unsigned)c.N), 256, 0, c.s>>>(p.head, p.pos, at<float>(c, l.acc), l.splits, c.N * c.D, c.D,
-                                                            dx);
+        finish_dx<DT><<<dim3((unsigned)c.N), 256, 0, c.s>>>(p.head, p.pos, at<float>(c, l.acc), c.D, dx);
 }
 
 // w's rows can be read as operands where they are: 16-byte loads at 16-byte

@@ -38,7 +38,7 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 //
 // The 16-bit matrix rate is 16 times the fp32 one, so three products cost 0.19
 // and six 0.375 of one fp32 product.
-__device__ constexpr int terms(int parts) { return parts == 1 ? 1 : parts == 2 ? 3 : 6; }
+__host__ __device__ constexpr int terms(int parts) { return parts == 1 ? 1 : parts == 2 ? 3 : 6; }
 // parts of term t: 00 01 10 | 11 02 20
 __device__ constexpr int term_a(int t) { return t == 2 || t == 3 ? 1 : t == 5 ? 2 : 0; }
 __device__ constexpr int term_b(int t) { return t == 1 || t == 3 ? 1 : t == 4 ? 2 : 0; }

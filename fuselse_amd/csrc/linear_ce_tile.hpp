@@ -13,7 +13,9 @@
 // conflicts in either kind of read); the loads' lane addresses apply the
 // permutation, since a direct-to-LDS load writes its lanes' data in lane order.
 //
-// A step is four phases of a quarter of its products each (one half of K, one
+// A block takes one tile after another, and its loads run ahead of its products
+// across tiles: while a tile's results are written, the next tile's first steps
+// arrive.  A step is four phases of a quarter of its products each (one half of K, one
 // half of the wave's rows).  A phase's fragments are read during the phase
 // before, and the loads for the step after next are spread over two phases,
 // one behind every few matrix instructions: issued together they stall a wave
@@ -69,6 +71,7 @@ __device__ __forceinline__ void load_to_lds(const char* base, uint32_t off, uint
         : "memory");
 }
 // A value all lanes share, in scalar registers.
+__device__ __forceinline__ int scalar(int v) { return __builtin_amdgcn_readfirstlane(v); }
 __device__ __forceinline__ const char* uniform(const char* p) {
     const uint64_t u = (uint64_t)p;
     const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)u), hi = __builtin_amdgcn_readfirstlane((uint32_t)(u >> 32));
@@ -108,8 +111,10 @@ struct Side {
     int rows;           // across: K rows there are
     uint32_t off[kLoads];
 
-    // K-major: rows of the operand past its last are read as the last.
-    // Across: columns past the last whole chunk are read as that chunk.
+    // K-major: rows of the operand past its last are read as the last.  With
+    // PERM the side's fragments hold its rows in another order, that of
+    // perm_row.  Across: columns past the last whole chunk are read as that chunk.
+    template <bool PERM = false>
     __device__ __forceinline__ void init(const Operand& o, int64_t first) {
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
         part = o.part * 2;
@@ -121,6 +126,7 @@ struct Side {
 #pragma unroll
             for (int j = 0; j < kLoads; ++j) {
                 int64_t r = (j * S::kWaves + wave) * 8 + (lane >> 3);
+                if (PERM) r = perm_row((int)r);
                 if (first + r >= o.rows) r = o.rows - 1 - first;
                 off[j] = (uint32_t)(r * ld) + ((lane & 7) ^ (lane >> 3)) * 16;
             }
@@ -131,6 +137,14 @@ struct Side {
 #pragma unroll
             for (int j = 0; j < kLoads; ++j) off[j] = (uint32_t)(krow(j) * ld) + col(j, first, o.cols);
         }
+    }
+    // Row r of LDS, of fragment i of a wave's, is row
+    // 32 (i / 2) + 8 (r % 16 / 4) + 4 (i % 2) + r % 4 of the wave's: two fragments'
+    // results of a lane are 8 consecutive rows of C, and the four lanes that
+    // share a column hold 32: whole 64-byte stores of 16-bit results.
+    __device__ __forceinline__ static int perm_row(int r) {
+        const int w = r % (S::FM * 16), i = w / 16;
+        return r - w + i / 2 * 32 + w % 16 / 4 * 8 + i % 2 * 4 + w % 4;
     }
     // across: the permutation of K row k's chunks.  The 32 lanes that a cycle of
     // a transposing read serves hold 2 chunks each of K rows 0 .. 3 and of those
@@ -155,12 +169,12 @@ struct Side {
     // Starts load J of step k (of part p) into buf.  Where the K rows end inside
     // the step, those past the last are read as the last.
     template <int J>
-    __device__ __forceinline__ void load(lds_char* buf, int64_t k, int p) const {
+    __device__ __forceinline__ void load(lds_char* buf, int k, int p) const {
         const char* b = uniform(base + k * step + p * part);
         const uint32_t lds = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)buf + (threadIdx.x >> 6) * 1024);
         uint32_t o = off[J];
         if (!KMAJOR && (k + 1) * kStep > rows) {
-            const int last = rows - 1 - (int)(k * kStep);
+            const int last = rows - 1 - k * kStep;
             o -= krow(J) > last ? (uint32_t)((krow(J) - last) * ld) : 0u;
         }
         load_to_lds(b, o, lds + J * S::kWaves * 1024);
@@ -187,63 +201,90 @@ struct Side {
     }
 };
 
-// Tile t of tiles_m x tiles_n, counted so that blocks that run together share
-// operands: the dispatcher deals blocks to the 8 XCDs in turn, so block b
-// takes tile (b mod 8) total / 8 + b / 8, consecutive tiles of one XCD; and tiles
-// go down columns of 4 in M before they step in N, so that the 32 tiles an XCD
-// runs at a time read 4 row strips and 8 column strips.
-__device__ __forceinline__ int64_t xcd_tile(int64_t b, int64_t total) {
-    const int64_t per = total / 8;
-    return b < per * 8 ? (b & 7) * per + (b >> 3) : b;
-}
-__device__ __forceinline__ void tile_at(int64_t t, int64_t tiles_m, int64_t tiles_n, int64_t& m, int64_t& n) {
-    constexpr int64_t kGroup = 4;
-    const int64_t group = t / (kGroup * tiles_n), first = group * kGroup;
-    const int64_t gm = tiles_m - first < kGroup ? tiles_m - first : kGroup;
-    const int64_t r = t - group * kGroup * tiles_n;
-    m = first + r % gm;
-    n = r / gm;
+// The tiles a block takes, of `total` in the order of tile_at.  The dispatcher
+// deals blocks to the 8 XCDs in turn; each XCD has an eighth of the tiles, in
+// one run, and its blocks take consecutive ones at a time.
+struct Walk {
+    int t, end, stride;
+    __device__ __forceinline__ explicit Walk(int total) {
+        const int xcd = blockIdx.x & 7;
+        end = (int)((xcd + 1) * (int64_t)total / 8);
+        stride = (int)(gridDim.x / 8);
+        t = (int)(xcd * (int64_t)total / 8) + (int)(blockIdx.x >> 3);
+    }
+};
+// Tile t's place among tiles_m x tiles_n: down columns of 4 in M before a step in
+// N, so that the 32 tiles an XCD runs at a time read 4 row strips and 8 column
+// strips.  In scalar registers, which the compiler's division does not keep to.
+struct TileAt {
+    int m, n;
+};
+__device__ __forceinline__ TileAt tile_at(int t, int tiles_m, int tiles_n) {
+    constexpr int kGroup = 4;
+    const int group = scalar((int)((unsigned)t / (unsigned)(kGroup * tiles_n))), first = group * kGroup;
+    const int gm = tiles_m - first < kGroup ? tiles_m - first : kGroup;
+    const int r = t - group * kGroup * tiles_n;
+    const int n = scalar((int)((unsigned)r / (unsigned)gm));
+    return {first + r - n * gm, n};
 }
 
 // Bytes of one step's buffer.
 template <class S>
 constexpr int kBufferBytes = (S::TM + S::TN) * kStep * 2;
 
-// acc[i][j][q] of a lane is C[wm + 16 i + 4 (lane / 16) + q][wn + 16 j + lane % 16]
-// of the tile, with (wm, wn) the wave's corner.
-template <class S, bool AK, bool BK, bool HALF, int PARTS>
-__device__ __forceinline__ void tile_product(const Side<S, S::TM, AK>& A, const Side<S, S::TN, BK>& B, int64_t k0,
-                                             int64_t k1, f32x4 (&acc)[S::FM][S::FN], lds_char* buf0, lds_char* buf1) {
+// Runs a block's tiles.  job.place(t, A, B) sets up tile t's sides; job.first(t)
+// and job.steps(t), at least one, are its steps of K; job.rows(t) loads what its results need;
+// job.finish(t, rows, acc) takes them.  acc[i][j][q] of a lane is
+// C[wm + 16 i + 4 (lane / 16) + q][wn + 16 j + lane % 16] of the tile, or, where A
+// was set up with PERM, C[wm + 32 (i / 2) + 8 (lane / 16) + 4 (i % 2) + q][..], with
+// (wm, wn) the wave's corner.
+template <class S, bool AK, bool BK, bool HALF, int PARTS, class Job>
+__device__ __forceinline__ void run_tiles(const Job& job, int total, lds_char* buf0, lds_char* buf1) {
     typedef Side<S, S::TM, AK> SA;
     typedef Side<S, S::TN, BK> SB;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wm = wave % S::WM * (S::FM * 16), wn = wave / S::WM * (S::FN * 16);
-#pragma unroll
-    for (int i = 0; i < S::FM; ++i)
-#pragma unroll
-        for (int j = 0; j < S::FN; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     constexpr int TERMS = terms(PARTS);
-    const int64_t steps = (k1 - k0) * TERMS;
-    if (steps <= 0) return;
     constexpr int kLoads = SA::kLoads + SB::kLoads, kHalf = kLoads / 2;
-    // loads J0 .. J0 + N - 1 of step s
-    auto load = [&](auto j0, auto n, lds_char* buf, int64_t s) {
-        int64_t k = k0 + s;
-        int ta = 0, tb = 0;
-        if constexpr (TERMS > 1) {
-            k = k0 + s / TERMS;
-            const int t = (int)(s % TERMS);
-            ta = term_a(t);
-            tb = term_b(t);
-        }
-        unrolled<decltype(n)::value>([&](auto i) {
-            constexpr int J = decltype(j0)::value + decltype(i)::value;
-            if constexpr (J < SA::kLoads) A.template load<J>(buf, k, ta);
-            else B.template load<J - SA::kLoads>(buf + SA::kBytes, k, tb);
-        });
-    };
     constexpr int H = S::FM / 2;
     static_assert(S::FM % 2 == 0 && kLoads >= 2, "phases take half of a wave's rows");
+    typedef std::integral_constant<int, 0> C0;
+    typedef std::integral_constant<int, kHalf> CHalf;
+    typedef std::integral_constant<int, kLoads - kHalf> CRest;
+
+    Walk walk(total);
+    if (walk.t >= walk.end) return;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave % S::WM * (S::FM * 16), wn = wave / S::WM * (S::FN * 16);
+
+    // where the loads are: step ls of tile lt
+    SA A;
+    SB B;
+    int lt = walk.t, ls = 0;
+    int lk0 = job.first(lt), ln = job.steps(lt) * TERMS;
+    job.place(lt, A, B);
+    // loads J0 .. J0 + N - 1 of that step
+    auto load = [&](auto j0, auto n, lds_char* buf) {
+        const int k = lk0 + (TERMS > 1 ? scalar((unsigned)ls / TERMS) : ls);
+        const int t = TERMS > 1 ? ls - (k - lk0) * TERMS : 0;
+        unrolled<decltype(n)::value>([&](auto i) {
+            constexpr int J = decltype(j0)::value + decltype(i)::value;
+            if constexpr (J < SA::kLoads) A.template load<J>(buf, k, term_a(t));
+            else B.template load<J - SA::kLoads>(buf + SA::kBytes, k, term_b(t));
+        });
+    };
+    // to the next step; past the last one it is loaded again, and not used
+    auto advance = [&]() {
+        if (ls + 1 < ln) {
+            ++ls;
+        } else if (lt + walk.stride < walk.end) {
+            lt += walk.stride;
+            ls = 0;
+            lk0 = job.first(lt);
+            ln = job.steps(lt) * TERMS;
+            job.place(lt, A, B);
+        }
+    };
+
+    f32x4 acc[S::FM][S::FN];
     u32x4 fa[2][H], fb[2][S::FN];
     auto read_a = [&](const lds_char* buf, auto p, int i) {
         constexpr int P = decltype(p)::value;
@@ -253,21 +294,9 @@ __device__ __forceinline__ void tile_product(const Side<S, S::TM, AK>& A, const 
         constexpr int P = decltype(p)::value;
         fb[P >> 1][j] = SB::frag(buf + SA::kBytes, wn + j * 16, P >> 1);
     };
-    typedef std::integral_constant<int, 0> C0;
-    typedef std::integral_constant<int, kHalf> CHalf;
-    typedef std::integral_constant<int, kLoads - kHalf> CRest;
-    load(C0{}, std::integral_constant<int, kLoads>{}, buf0, 0);
-    load(C0{}, CHalf{}, buf1, steps > 1 ? 1 : 0);
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kHalf) : "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-#pragma unroll
-    for (int i = 0; i < H; ++i) read_a(buf0, C0{}, i);
-#pragma unroll
-    for (int j = 0; j < S::FN; ++j) read_b(buf0, C0{}, j);
     // Phase P: its products, with the reads of the phase after it (from rd) and
-    // loads J0 .. J0 + N - 1 of step ls (to ld) between them, in this order.
-    auto phase = [&](auto p, const lds_char* rd, auto j0, auto n, lds_char* ld, int64_t ls) {
+    // loads J0 .. J0 + N - 1 (to ld) between them, in this order.
+    auto phase = [&](auto p, const lds_char* rd, auto j0, auto n, lds_char* ld) {
         constexpr int P = decltype(p)::value, Q = (P + 1) & 3;
         typedef std::integral_constant<int, Q> CQ;
         unrolled<H>([&](auto ic) {
@@ -282,31 +311,52 @@ __device__ __forceinline__ void tile_product(const Side<S, S::TM, AK>& A, const 
                 acc[(P & 1) * H + i][j] = mfma<HALF>(fa[P & 1][i], fb[P >> 1][j], acc[(P & 1) * H + i][j]);
             constexpr int first = i * N / H, count = (i + 1) * N / H - first;
             if constexpr (count > 0)
-                load(std::integral_constant<int, decltype(j0)::value + first>{}, std::integral_constant<int, count>{}, ld,
-                     ls);
+                load(std::integral_constant<int, decltype(j0)::value + first>{}, std::integral_constant<int, count>{}, ld);
             __builtin_amdgcn_sched_barrier(0);
         });
     };
-    // Step s in cur.  The first half of step s + 2's loads go to cur in phase 3,
-    // when every wave has read it, the others in phase 0 of the next step.  Past
-    // the last step the last one is loaded again, and not used.
-    const int64_t last = steps - 1;
-    auto step = [&](lds_char* cur, lds_char* nxt, int64_t s) {
-        phase(C0{}, cur, CHalf{}, CRest{}, nxt, s + 1 < last ? s + 1 : last);
-        phase(std::integral_constant<int, 1>{}, cur, C0{}, C0{}, nxt, 0);
-        phase(std::integral_constant<int, 2>{}, cur, C0{}, C0{}, nxt, 0);
+    // A step in cur.  The loads of the step after next begin in phase 3, when
+    // every wave has read cur, and end in phase 0 of the next step.
+    auto step = [&](lds_char* cur, lds_char* nxt) {
+        phase(C0{}, cur, CHalf{}, CRest{}, nxt);
+        advance();
+        phase(std::integral_constant<int, 1>{}, cur, C0{}, C0{}, nxt);
+        phase(std::integral_constant<int, 2>{}, cur, C0{}, C0{}, nxt);
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        phase(std::integral_constant<int, 3>{}, nxt, C0{}, CHalf{}, cur, s + 2 < last ? s + 2 : last);
+        phase(std::integral_constant<int, 3>{}, nxt, C0{}, CHalf{}, cur);
     };
-    for (int64_t s = 0; s < steps; s += 2) {
-        step(buf0, buf1, s);
-        if (s + 1 >= steps) break;
-        step(buf1, buf0, s + 1);
+
+    load(C0{}, std::integral_constant<int, kLoads>{}, buf0);
+    advance();
+    load(C0{}, CHalf{}, buf1);
+    wait_copies();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < H; ++i) read_a(buf0, C0{}, i);
+#pragma unroll
+    for (int j = 0; j < S::FN; ++j) read_b(buf0, C0{}, j);
+    // one copy of the step for both buffers: with one for each, the compiler kept
+    // two sets of accumulators
+    lds_char *cur = buf0, *nxt = buf1;
+    for (; walk.t < walk.end; walk.t += walk.stride) {
+        const auto rows = job.rows(walk.t);
+        const int steps = job.steps(walk.t) * TERMS;
+#pragma unroll
+        for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+            for (int j = 0; j < S::FN; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int s = 0; s < steps; ++s) {
+            step(cur, nxt);
+            lds_char* const done = cur;
+            cur = nxt;
+            nxt = done;
+        }
+        job.finish(walk.t, rows, acc);
     }
     wait_copies();
-    __syncthreads();
 }
 
 }  // namespace lce

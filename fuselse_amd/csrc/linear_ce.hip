@@ -61,8 +61,6 @@ struct Head {          // at the workspace's start, written by the plan kernel
     int live;          // rows whose target is not ignore_index
     float inv_scale;   // undoes the power of two that a and b carry
     int splits;        // of K in dx
-    uint32_t big_x;    // fp32: bits of the largest finite magnitude in the live
-    uint32_t big_w;    //   rows of x, and in w
 };
 
 // ---------------------------------------------------------------------------
@@ -140,8 +138,79 @@ __device__ __forceinline__ int dx_splits(const PlanArgs& p, int live) {
     return (int)(best & 127);
 }
 
+// fp32: the largest finite magnitudes of the live rows of x and of w, from which
+// the logits' operands are scaled: a block's of its share of the rows, in mag.
+struct MagArgs {
+    const float* x;
+    int64_t ldx;
+    const float* w;
+    int64_t ldw, d;
+    float* mag;             // [x_blocks + w_blocks]
+    int x_blocks, w_blocks;
+};
+
+__device__ __forceinline__ float wave_max(float v) {
+    v = fmaxf(v, reduce_partner<1>(v));
+    v = fmaxf(v, reduce_partner<2>(v));
+    v = fmaxf(v, reduce_partner<4>(v));
+    v = fmaxf(v, reduce_partner<8>(v));
+    v = fmaxf(v, reduce_partner<16>(v));
+    return fmaxf(v, reduce_partner<32>(v));
+}
+// Maximum over the block's waves of each wave's v; all threads get it.
+template <int THREADS>
+__device__ __forceinline__ float block_max(float v, float* sh) {
+    v = wave_max(v);
+    if (lane_id() == 0) sh[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = sh[0];
+    for (int w = 1; w < THREADS / 64; ++w) v = fmaxf(v, sh[w]);
+    return v;
+}
+
+__device__ __forceinline__ void magnitudes(const PlanArgs& p, const MagArgs& m, int block) {
+    const bool is_x = block < m.x_blocks;
+    const int64_t n = is_x ? p.n : p.v;
+    const int64_t b = is_x ? block : block - m.x_blocks, blocks = is_x ? m.x_blocks : m.w_blocks;
+    float big = 0.0f;
+    auto take = [&](const float (&v)[4]) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float a = __builtin_fabsf(v[k]);
+            big = a < kInf ? fmaxf(big, a) : big;
+        }
+    };
+    // a wave a row, four vectors a lane in flight
+    constexpr int kWaves = kPlanThreads / 64;
+    for (int64_t r = b * kWaves + (threadIdx.x >> 6); r < n; r += blocks * kWaves) {
+        if (is_x && p.target[r] == p.ignore) continue;
+        const float* s = is_x ? m.x + r * m.ldx : m.w + r * m.ldw;
+        int64_t c = (int64_t)lane_id() * 4;
+        for (; c + 3 * 256 + 4 <= m.d; c += 4 * 256) {
+            float v[4][4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) load_vec_any<float>(s + c + k * 256, v[k]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) take(v[k]);
+        }
+        for (; c < m.d; c += 256) {
+            float v[4];
+            load_vec_part<float>(s + c, m.d - c, 0.0f, v);
+            take(v);
+        }
+    }
+    __shared__ float sh[kWaves];
+    big = block_max<kPlanThreads>(big, sh);
+    if (threadIdx.x == 0) m.mag[block] = big;
+}
+
+// Block 0 makes the plan; blocks after it take the magnitudes.
 template <bool BWD>
-__global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs p) {
+__global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs p, MagArgs m) {
+    if (blockIdx.x > 0) {
+        if constexpr (!BWD) magnitudes(p, m, (int)blockIdx.x - 1);
+        return;
+    }
     __shared__ int sh[kPlanThreads / 64];
     const int64_t per = (p.n + kPlanThreads - 1) / kPlanThreads;
     const int64_t r0 = (int64_t)threadIdx.x * per;
@@ -179,12 +248,8 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs p) {
         ++at;
     }
     if constexpr (BWD) {
-        for (int d = 1; d < 64; d *= 2) big = fmaxf(big, __shfl_xor(big, d, 64));
         __shared__ float shf[kPlanThreads / 64];
-        if (lane_id() == 0) shf[threadIdx.x >> 6] = big;
-        __syncthreads();
-        big = shf[0];
-        for (int w = 1; w < kPlanThreads / 64; ++w) big = fmaxf(big, shf[w]);
+        big = block_max<kPlanThreads>(big, shf);
         const int e = scale_exp(big, 14);
         const float scale = __builtin_ldexpf(1.0f, e);
         if (threadIdx.x == 0) p.head->inv_scale = __builtin_ldexpf(1.0f, -e);
@@ -198,116 +263,102 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs p) {
             p.b[at + k] *= scale;
         }
     }
-    if (threadIdx.x == 0) {
-        p.head->live = live;
-        p.head->big_x = p.head->big_w = 0;
-    }
+    if (threadIdx.x == 0) p.head->live = live;
 }
 
-// fp32: the largest finite magnitudes of the live rows of x (blocks before
-// `split`) and of w.  A maximum does not depend on the atomics' order.
-struct BigArgs {
-    const float* x;
-    int64_t ldx;
-    const int* rows;
-    const float* w;
-    int64_t ldw, v, d;
-    Head* head;
-    int split;
-};
-__global__ __launch_bounds__(256) void magnitudes(BigArgs p) {
-    const bool is_x = (int)blockIdx.x < p.split;
-    const int64_t n = is_x ? p.head->live : p.v;
-    const int64_t b = is_x ? blockIdx.x : blockIdx.x - p.split;
-    const int64_t blocks = is_x ? p.split : gridDim.x - p.split;
-    float big = 0.0f;
-    auto take = [&](const float (&v)[4]) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const float m = __builtin_fabsf(v[k]);
-            big = m < kInf ? fmaxf(big, m) : big;
-        }
-    };
-    // a wave a row, four vectors a lane in flight
-    for (int64_t r = b * 4 + (threadIdx.x >> 6); r < n; r += blocks * 4) {
-        const float* s = is_x ? p.x + (int64_t)p.rows[r] * p.ldx : p.w + r * p.ldw;
-        int64_t c = (int64_t)lane_id() * 4;
-        for (; c + 3 * 256 + 4 <= p.d; c += 4 * 256) {
-            float v[4][4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) load_vec_any<float>(s + c + k * 256, v[k]);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) take(v[k]);
-        }
-        for (; c < p.d; c += 256) {
-            float v[4];
-            load_vec_part<float>(s + c, p.d - c, 0.0f, v);
-            take(v);
-        }
-    }
-    big = fmaxf(big, reduce_partner<1>(big));
-    big = fmaxf(big, reduce_partner<2>(big));
-    big = fmaxf(big, reduce_partner<4>(big));
-    big = fmaxf(big, reduce_partner<8>(big));
-    big = fmaxf(big, reduce_partner<16>(big));
-    big = fmaxf(big, reduce_partner<32>(big));
-    __shared__ float sh[4];
-    if (lane_id() == 0) sh[threadIdx.x >> 6] = big;
-    __syncthreads();
-    big = fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3]));
-    // one atomic a block: they take turns at about 10 ns each
-    if (threadIdx.x == 0 && big > 0.0f)
-        atomicMax(is_x ? &p.head->big_x : &p.head->big_w, __builtin_bit_cast(uint32_t, big));
-}
-
-// The scale of fp32 logits' operands, and what undoes both in a logit.
-__device__ __forceinline__ float operand_scale(uint32_t bits) {
-    return __builtin_ldexpf(1.0f, scale_exp(__builtin_bit_cast(float, bits), 15));
-}
+// The scale of fp32 logits' operands, and what undoes both in a logit; big holds
+// the magnitudes of x and of w.
+__device__ __forceinline__ float operand_scale(float big) { return __builtin_ldexpf(1.0f, scale_exp(big, 15)); }
 template <int DT>
 __device__ __forceinline__ float logit(float acc, float inv_x, float inv_w) {
     return DT == kF32 ? acc * inv_x * inv_w : acc;
 }
 template <int DT>
-__device__ __forceinline__ void logit_scales(const Head* h, float& inv_x, float& inv_w) {
+__device__ __forceinline__ void logit_scales(const float* big, float& inv_x, float& inv_w) {
     inv_x = inv_w = 1.0f;
     if constexpr (DT == kF32) {
-        inv_x = 1.0f / operand_scale(h->big_x);
-        inv_w = 1.0f / operand_scale(h->big_w);
+        inv_x = 1.0f / operand_scale(big[0]);
+        inv_w = 1.0f / operand_scale(big[1]);
     }
 }
 
 // ---------------------------------------------------------------------------
-// Packing: rows of x (the live ones) or w as 16-bit operands of ldp elements (a
-// multiple of 64), zero beyond D; 8 elements a thread.
+// Packing: the live rows of x and a piece's rows of w as 16-bit operands of ldp
+// elements (a multiple of 64), zero beyond D; 8 elements a thread.  fp32 rows
+// are written for the logits and, where `grads` is not NULL, for dx and dw.
 // ---------------------------------------------------------------------------
-// `big`: fp32 logits' operands, scaled by its power of two.
+struct PackSide {
+    const void* src;   // NULL: nothing to pack
+    int64_t ld, n;     // rows there are, or may be
+    const int* rows;   // x: the live rows
+    uint16_t* logits;
+    int64_t logits_part;
+    uint16_t* grads;
+    int64_t grads_part;
+};
+struct PackArgs {
+    PackSide x, w;
+    const Head* head;
+    int64_t d, ldp;
+    float* big;        // fp32: magnitudes of x and w; from mag when there is one
+    const float* mag;
+    int x_blocks, w_blocks;
+};
+
 template <int DT, int P>
-__global__ __launch_bounds__(256) void pack_rows(const typename Io<DT>::T* src, int64_t lds_, int64_t d, const int* rows,
-                                                 const int* live, int64_t n, uint16_t* dst, int64_t ldp, int64_t part,
-                                                 const uint32_t* big) {
-    typedef typename Io<DT>::T T;
-    constexpr int VE = Elem<T>::kVec;
-    const int64_t chunks = ldp / 8;
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int64_t r = i / chunks, c = i % chunks * 8;
-    if (r >= (live ? *live : n)) return;
-    const float scale = P == 2 ? operand_scale(*big) : 1.0f;
-    const T* s = src + (rows ? (int64_t)rows[r] : r) * lds_ + c;
+__device__ __forceinline__ void store_parts(const float (&v)[8], float scale, uint16_t* dst, int64_t part) {
     uint16_t o[8][P];
 #pragma unroll
-    for (int h = 0; h < 8; h += VE) {
-        float v[VE];
-        load_vec_part<T>(s + h, d - c - h, 0.0f, v);
-#pragma unroll
-        for (int k = 0; k < VE; ++k) to_parts<DT>(P == 2 ? v[k] * scale : v[k], o[h + k]);
-    }
+    for (int k = 0; k < 8; ++k) to_parts<DT>(P == 2 ? v[k] * scale : v[k], o[k]);
 #pragma unroll
     for (int k = 0; k < P; ++k) {
         u32x4 w;
 #pragma unroll
         for (int q = 0; q < 4; ++q) w[q] = o[2 * q][k] | (uint32_t)o[2 * q + 1][k] << 16;
-        *reinterpret_cast<u32x4*>(dst + k * part + r * ldp + c) = w;
+        *reinterpret_cast<u32x4*>(dst + k * part) = w;
+    }
+}
+
+template <int DT>
+__global__ __launch_bounds__(256) void pack(PackArgs p) {
+    typedef typename Io<DT>::T T;
+    constexpr int VE = Elem<T>::kVec;
+    float big_x = 0.0f, big_w = 0.0f;
+    if constexpr (DT == kF32) {
+        if (p.mag) {
+            __shared__ float sh[2][4];
+            for (int k = threadIdx.x; k < p.x_blocks; k += 256) big_x = fmaxf(big_x, p.mag[k]);
+            for (int k = threadIdx.x; k < p.w_blocks; k += 256) big_w = fmaxf(big_w, p.mag[p.x_blocks + k]);
+            big_x = block_max<256>(big_x, sh[0]);
+            big_w = block_max<256>(big_w, sh[1]);
+            if (blockIdx.x == 0 && threadIdx.x == 0) {
+                p.big[0] = big_x;
+                p.big[1] = big_w;
+            }
+        } else {
+            big_x = p.big[0];
+            big_w = p.big[1];
+        }
+    }
+    const int64_t chunks = p.ldp / 8;
+    int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const bool is_x = i < p.x.n * chunks;
+    const PackSide& s = is_x ? p.x : p.w;
+    if (!is_x) i -= p.x.n * chunks;
+    const int64_t r = i / chunks, c = i % chunks * 8;
+    if (r >= (is_x ? (int64_t)p.head->live : s.n)) return;
+    const T* src = static_cast<const T*>(s.src) + (s.rows ? (int64_t)s.rows[r] : r) * s.ld + c;
+    float v[8];
+#pragma unroll
+    for (int h = 0; h < 8; h += VE) {
+        float t[VE];
+        load_vec_part<T>(src + h, p.d - c - h, 0.0f, t);
+#pragma unroll
+        for (int k = 0; k < VE; ++k) v[h + k] = t[k];
+    }
+    store_parts<DT, Logits<DT>::kParts>(v, operand_scale(is_x ? big_x : big_w), s.logits + r * p.ldp + c, s.logits_part);
+    if constexpr (DT == kF32) {
+        if (s.grads) store_parts<DT, Grads<DT>::kParts>(v, 1.0f, s.grads + r * p.ldp + c, s.grads_part);
     }
 }
 
@@ -351,6 +402,7 @@ struct StatArgs {
     float2* part;      // [live row][parts]: (max, sum)
     int64_t parts;
     float* at_target;  // [live row]
+    const float* big;
 };
 
 template <int DT, class S>
@@ -413,7 +465,7 @@ __global__ __launch_bounds__(S::kThreads, 2) void logits_stats(StatArgs p) {
     StatJob<DT, S> job{p, p.head->live};
     job.p.x.rows = job.live;
     job.tiles_n = (job.live + S::TN - 1) / S::TN;
-    logit_scales<DT>(p.head, job.inv_x, job.inv_w);
+    logit_scales<DT>(p.big, job.inv_x, job.inv_w);
     run_tiles<S, true, true, Logits<DT>::kHalf, Logits<DT>::kParts>(job, p.tiles_m * job.tiles_n, (lds_char*)buf0,
                                                                     (lds_char*)buf1);
 }
@@ -464,6 +516,7 @@ struct GradArgs {
     int tiles_m;
     uint16_t* g;         // [live row][ldg]
     int64_t ldg, g_part;
+    const float* big;
 };
 
 // G of a piece.  Rows from the live ones up to a multiple of 64 are zero, and so
@@ -544,7 +597,7 @@ __global__ __launch_bounds__(S::kThreads, 2) void logits_grad(GradArgs p) {
     GradJob<DT, S> job{p, p.head->live};
     job.p.x.rows = job.live;
     job.tiles_n = (job.live + S::TN - 1) / S::TN;
-    logit_scales<DT>(p.head, job.inv_x, job.inv_w);
+    logit_scales<DT>(p.big, job.inv_x, job.inv_w);
     run_tiles<S, true, true, Logits<DT>::kHalf, Logits<DT>::kParts>(job, p.tiles_m * job.tiles_n, (lds_char*)buf0,
                                                                     (lds_char*)buf1);
 }
@@ -700,8 +753,9 @@ struct Layout {
     bool pack_w;         // w is packed a piece at a time
     int splits;          // of K in dx, with every row live
     int64_t room;        // rows of its sums
+    int x_blocks, w_blocks;  // fp32 forward: blocks that take the magnitudes
     int logits, dx, dw;  // the products' tiles: 256, 128 or 64
-    int64_t head, rows, pos, tgt, at_target, loss_rows, part, parts, a, b, lse, xp, xg, wp, wg, g, acc, bytes;
+    int64_t head, rows, pos, tgt, at_target, loss_rows, part, parts, a, b, lse, xp, xg, wp, wg, mag, g, acc, bytes;
 };
 
 // A product's tiles: the largest that fill most of the chip.
@@ -756,6 +810,9 @@ Layout layout(int64_t N, int64_t V, int64_t D, int dtype, bool bwd, bool aligned
     l.tgt = take(4 * N);
     l.xp = take(2 * lparts * N * l.ldx);
     l.wp = take(l.pack_w ? 2 * lparts * l.piece * l.ldx : 0);
+    l.x_blocks = dtype == kF32 && !bwd ? (int)(div_up(N, 16) < 32 ? div_up(N, 16) : 32) : 0;
+    l.w_blocks = dtype == kF32 && !bwd ? (int)(div_up(V, 16) < 256 ? div_up(V, 16) : 256) : 0;
+    l.mag = take(4 * (l.x_blocks + l.w_blocks));
     l.logits = tile_size(l.piece, N, 1);
     if (!bwd) {
         l.parts = div_up(V, l.logits / 2);
@@ -800,47 +857,46 @@ P* at(const Call& c, int64_t off) {
     return reinterpret_cast<P*>(c.ws + off);
 }
 
-// Rows v0 .. of w as an operand of P parts, packed at `to` where they have to be.
-template <int DT, int P>
-Operand operand_w(const Call& c, const Layout& l, int64_t v0, int64_t rows, int64_t to) {
+// Operands of x and of rows v0 .. of w: for the logits, and for dw and dx.
+struct Operands {
+    Operand x, xg, w, wg;
+};
+
+// Packs what has to be packed for the piece at v0 (x with the first piece) and
+// sets up its operands.
+template <int DT>
+void operands(const Call& c, const Layout& l, int64_t v0, int64_t rows, bool dx, bool dw, bool fwd, float* big,
+              Operands& o) {
     typedef typename Io<DT>::T T;
     const T* w = static_cast<const T*>(c.w) + v0 * c.ldw;
-    if (!l.pack_w) return Operand{reinterpret_cast<const uint16_t*>(w), c.ldw, 0, (int)rows, l.ldx};
-    const int64_t part = l.piece * l.ldx;
-    pack_rows<DT, P><<<dim3((unsigned)div_up(rows * (l.ldx / 8), 256)), 256, 0, c.s>>>(
-        w, c.ldw, c.D, nullptr, nullptr, rows, at<uint16_t>(c, to), l.ldx, part, &at<Head>(c, l.head)->big_w);
-    return Operand{at<uint16_t>(c, to), l.ldx, part, (int)rows, l.ldx};
-}
-
-// The live rows of x, packed at `to`.
-template <int DT, int P>
-Operand operand_x(const Call& c, const Layout& l, int64_t to) {
-    typedef typename Io<DT>::T T;
-    const Head* head = at<Head>(c, l.head);
-    const int64_t part = c.N * l.ldx;
-    pack_rows<DT, P><<<dim3((unsigned)div_up(c.N * (l.ldx / 8), 256)), 256, 0, c.s>>>(
-        static_cast<const T*>(c.x), c.ldx, c.D, at<int>(c, l.rows), &head->live, c.N, at<uint16_t>(c, to), l.ldx, part,
-        &head->big_x);
-    return Operand{at<uint16_t>(c, to), l.ldx, part, (int)c.N, l.ldx};
-}
-
-// fp32: the magnitudes that the logits' operands are scaled by.
-template <int DT>
-void run_magnitudes(const Call& c, const Layout& l) {
-    if constexpr (DT == kF32) {
-        auto blocks = [](int64_t rows, int64_t most) { return (int)(div_up(rows, 4) < most ? div_up(rows, 4) : most); };
-        BigArgs b{};
-        b.x = static_cast<const float*>(c.x);
-        b.ldx = c.ldx;
-        b.rows = at<int>(c, l.rows);
-        b.w = static_cast<const float*>(c.w);
-        b.ldw = c.ldw;
-        b.v = c.V;
-        b.d = c.D;
-        b.head = at<Head>(c, l.head);
-        b.split = blocks(c.N, 128);
-        magnitudes<<<dim3((unsigned)(b.split + blocks(c.V, 512))), 256, 0, c.s>>>(b);
+    PackArgs p{};
+    p.head = at<Head>(c, l.head);
+    p.d = c.D;
+    p.ldp = l.ldx;
+    p.big = big;
+    if (fwd && v0 == 0) p.mag = at<float>(c, l.mag);
+    p.x_blocks = l.x_blocks;
+    p.w_blocks = l.w_blocks;
+    if (v0 == 0) {
+        const int64_t part = c.N * l.ldx;
+        uint16_t* to = at<uint16_t>(c, l.xp);
+        o.x = o.xg = Operand{to, l.ldx, part, (int)c.N, l.ldx};
+        p.x = PackSide{c.x, c.ldx, c.N, at<int>(c, l.rows), to, part, nullptr, part};
+        if (DT == kF32 && dw) p.x.grads = at<uint16_t>(c, l.xg);
+        if (DT == kF32) o.xg.p = p.x.grads;
     }
+    if (l.pack_w) {
+        const int64_t part = l.piece * l.ldx;
+        uint16_t* to = at<uint16_t>(c, l.wp);
+        o.w = o.wg = Operand{to, l.ldx, part, (int)rows, l.ldx};
+        p.w = PackSide{w, c.ldw, rows, nullptr, to, part, nullptr, part};
+        if (DT == kF32 && dx) p.w.grads = at<uint16_t>(c, l.wg);
+        if (DT == kF32) o.wg.p = p.w.grads;
+    } else {
+        o.w = o.wg = Operand{reinterpret_cast<const uint16_t*>(w), c.ldw, 0, (int)rows, l.ldx};
+    }
+    const int64_t threads = (p.x.n + p.w.n) * (l.ldx / 8);
+    if (threads > 0) pack<DT><<<dim3((unsigned)div_up(threads, 256)), 256, 0, c.s>>>(p);
 }
 
 // Blocks for `tiles` tiles: no more than run at a time, in multiples of 8.
@@ -878,14 +934,20 @@ void run_fwd(const Call& c, const Layout& l, float* loss, float* lse) {
     PlanArgs p = plan_args(c, l);
     p.loss_rows = c.reduction == 0 ? loss : at<float>(c, l.loss_rows);
     p.lse_out = lse;
-    plan_kernel<false><<<1, kPlanThreads, 0, c.s>>>(p);
-    run_magnitudes<DT>(c, l);
-    const Operand x = operand_x<DT, Logits<DT>::kParts>(c, l, l.xp);
+    MagArgs m{};
+    if constexpr (DT == kF32)
+        m = MagArgs{static_cast<const float*>(c.x), c.ldx,      static_cast<const float*>(c.w), c.ldw, c.D,
+                    at<float>(c, l.mag),            l.x_blocks, l.w_blocks};
+    plan_kernel<false><<<dim3((unsigned)(1 + l.x_blocks + l.w_blocks)), kPlanThreads, 0, c.s>>>(p, m);
+    Operands o{};
+    float* big = lse + c.N;
     for (int64_t v0 = 0; v0 < c.V; v0 += l.piece) {
         const int64_t rows = c.V - v0 < l.piece ? c.V - v0 : l.piece;
+        operands<DT>(c, l, v0, rows, false, false, true, big, o);
         StatArgs a{};
-        a.w = operand_w<DT, Logits<DT>::kParts>(c, l, v0, rows, l.wp);
-        a.x = x;
+        a.w = o.w;
+        a.x = o.x;
+        a.big = big;
         a.steps = (int)(l.ldx / kStep);
         a.head = p.head;
         a.tgt = p.tgt;
@@ -923,17 +985,17 @@ void run_bwd(const Call& c, const Layout& l, const float* grad, const float* lse
     // about 1.35 us
     p.sum_cost = (float)((double)c.D * 4 / (5e12 * 1.35e-6) / (double)div_up(c.V, l.piece));
     p.room = l.room;
-    plan_kernel<true><<<1, kPlanThreads, 0, c.s>>>(p);
-    run_magnitudes<DT>(c, l);
-    constexpr int LP = Logits<DT>::kParts, GP = Grads<DT>::kParts;
-    const Operand x = operand_x<DT, LP>(c, l, l.xp);
-    const Operand xg = DT == kF32 && dw ? operand_x<DT, GP>(c, l, l.xg) : x;
+    plan_kernel<true><<<1, kPlanThreads, 0, c.s>>>(p, MagArgs{});
+    Operands o{};
+    float* big = const_cast<float*>(lse) + c.N;  // read, not written, here
     const int64_t g_part = round_up(c.N, 64) * l.piece;
     for (int64_t v0 = 0; v0 < c.V; v0 += l.piece) {
         const int64_t rows = c.V - v0 < l.piece ? c.V - v0 : l.piece;
+        operands<DT>(c, l, v0, rows, dx != nullptr, dw != nullptr, false, big, o);
         GradArgs g{};
-        g.w = operand_w<DT, LP>(c, l, v0, rows, l.wp);
-        g.x = x;
+        g.w = o.w;
+        g.x = o.x;
+        g.big = big;
         g.steps = (int)(l.ldx / kStep);
         g.head = p.head;
         g.tgt = p.tgt;
@@ -955,7 +1017,7 @@ void run_bwd(const Call& c, const Layout& l, const float* grad, const float* lse
         a.m = (int)c.D;
         a.ldc = c.D;
         if (dx) {
-            a.a = DT == kF32 ? operand_w<DT, GP>(c, l, v0, rows, l.wg) : g.w;
+            a.a = o.wg;
             a.b = Operand{g.g, l.piece, g_part, (int)c.N, l.piece};
             a.steps = (int)div_up(rows, kStep);
             a.n = (int)c.N;
@@ -968,7 +1030,7 @@ void run_bwd(const Call& c, const Layout& l, const float* grad, const float* lse
             });
         }
         if (dw) {
-            a.a = xg;
+            a.a = o.xg;
             a.b = Operand{g.g, l.piece, g_part, 0, l.piece};
             a.n = (int)rows;
             a.out = static_cast<T*>(dw) + v0 * c.D;

@@ -898,7 +898,8 @@ def _row_stride(t: torch.Tensor) -> int:
 def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, ignore_index: int = -100,
                          reduction: str = "mean", z_loss: float = 0.0):
     """Softmax cross entropy of the logits x @ weight.T, which are never
-    stored: (loss, lse) in fp32, with lse [N] for the backward.  x (N, D) and
+    stored: (loss, lse) in fp32; lse (N + 2,) holds the rows' log-sum-exps and
+    two values more for the backward.  x (N, D) and
     weight (V, D) fp32, fp16 or bf16 with contiguous rows, target int64 (N,).
     loss[n] = lse[n] - x[n] . weight[target[n]] + z_loss * lse[n]^2; rows whose
     target is ignore_index have loss 0 and are not read."""
@@ -906,7 +907,7 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     red = _reduction(reduction)
     N, D = x.shape
     V = weight.shape[0]
-    lse = torch.empty((N,), dtype=torch.float32, device=x.device)
+    lse = torch.empty((N + 2,), dtype=torch.float32, device=x.device)
     loss = torch.empty((N,) if red == 0 else (), dtype=torch.float32, device=x.device)
     if N == 0:
         return loss.zero_(), lse
@@ -934,7 +935,7 @@ def linear_cross_entropy_backward(grad_output: torch.Tensor, x: torch.Tensor, we
     V = weight.shape[0]
     for t, nm in ((grad_output, "grad_output"), (lse, "lse")):
         _check(t.is_cuda and t.dtype == torch.float32 and t.is_contiguous(), f"{nm} must be contiguous CUDA float32")
-    _check(lse.dim() == 1 and lse.shape[0] == N, "lse must be 1D (N)")
+    _check(lse.dim() == 1 and lse.shape[0] == N + 2, "lse must be 1D (N + 2)")
     _check(grad_output.numel() == (N if red == 0 else 1), "grad_output must have the loss's shape")
     _check_device(x, "x", grad_output=grad_output, lse=lse)
     dx = torch.empty((N, D), dtype=x.dtype, device=x.device) if need_x else None

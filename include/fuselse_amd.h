@@ -347,10 +347,12 @@ int fl_sparse_blocked_grad(const float* node_flows, const float* node_mars, cons
  * count in the mean, and their x is not read (it may hold anything).  Any
  * other target outside [0, V) makes the row's loss NaN, and with it the
  * gradients it takes part in.  Products of fp16 and bf16 are exact, of fp32
- * to about 2^-21; sums are fp32.
+ * to about 2^-21 (an element's digits below 2^-39 of the largest magnitude
+ * in its tensor do not enter the logits); sums are fp32.
  *
- * fl_linear_ce_fwd: loss fp32 [N] (reduction 0) or [1]; lse fp32 [N], for the
- *   backward.  A mean over no rows is 0.
+ * fl_linear_ce_fwd: loss fp32 [N] (reduction 0) or [1]; lse fp32
+ *   [N + 2], the rows' log-sum-exps (0 for ignored ones) and two values more
+ *   for the backward.  A mean over no rows is 0.
  * fl_linear_ce_bwd: grad fp32 [N] (reduction 0) or [1]; lse as the forward
  *   wrote it.  dx [N, D] and dw [V, D] contiguous, of x's type; either may be
  *   NULL.  The softmax gradient enters the products rounded once to x's type

@@ -58,17 +58,26 @@ __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
 // bytes first waits for vmcnt and a barrier.  Written as assembly because the
 // compiler, which cannot tell the two step buffers apart at every read, put a
 // wait for all copies in flight before reads of the other buffer.
+template <bool NT = false>
 __device__ __forceinline__ void load_to_lds(const char* base, uint32_t off, uint32_t lds) {
     // The compiler does not see what the assembly is, so the wait states it would
     // put in are written out: one from m0's write, and five from a vector
     // instruction's write of base's registers (readfirstlane) to their use as
     // an address.
-    asm volatile(
-        "s_nop 4\n\t"
-        "global_load_lds_dwordx4 %1, %2"
-        :
-        : "{m0}"(lds), "v"(off), "s"(base)
-        : "memory");
+    if constexpr (NT)  // nontemporal: data that is read once
+        asm volatile(
+            "s_nop 4\n\t"
+            "global_load_lds_dwordx4 %1, %2 nt"
+            :
+            : "{m0}"(lds), "v"(off), "s"(base)
+            : "memory");
+    else
+        asm volatile(
+            "s_nop 4\n\t"
+            "global_load_lds_dwordx4 %1, %2"
+            :
+            : "{m0}"(lds), "v"(off), "s"(base)
+            : "memory");
 }
 // A value all lanes share, in scalar registers.
 __device__ __forceinline__ int scalar(int v) { return __builtin_amdgcn_readfirstlane(v); }

@@ -5,8 +5,8 @@ backward, at the sizes and masks where the kernels change path.
 Tolerances.  A rounding to type t is off by at most half a step, eps_t / 2
 relative (u(t) below).  An fp32 sum of n terms is off by at most n 2^-23 of the
 sum of their magnitudes (2^-23 a step covers an accumulator that truncates).
-fp32 operands' products are 2^-21 off (six of nine partial products of three
-bf16 parts)."""
+fp32 operands' products are 2^-21 off (three of four partial products of two
+fp16 parts, six of nine of three bf16 parts)."""
 
 import math
 
@@ -158,6 +158,29 @@ def test_linear_several_pieces(cuda, n, d, v, dtype):
     x, w, t = linear_inputs(cuda, n, d, v, dtype, ignored=0.1, seed=4)
     t[0] = v - 1
     check_linear(x, w, t, "sum")
+
+
+@pytest.mark.parametrize("n", [1, 3, 16, 17])
+@pytest.mark.parametrize("d,v", [(64, 1), (64, 33), (192, 4097), (320, 70001), (1088, 32003)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_linear_few_rows(cuda, n, d, v, dtype):
+    """Rows that one pass over the projection serves, K ending inside a stage,
+    vocabularies of less and more than a row group a wave."""
+    print(f"case linear few {n} {d} {v} {dtype}", flush=True)
+    x, w, t = linear_inputs(cuda, n, d, v, dtype, ignored=0.3, seed=n)
+    t[-1] = v - 1
+    check_linear(x, w, t, "none", z=1e-3)
+
+
+@pytest.mark.parametrize("n,d,v", [(700, 130, 5000), (1500, 320, 9000), (130, 500, 20000), (1100, 64, 300),
+                                   (260, 2048, 520)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_linear_tile_sizes(cuda, n, d, v, dtype):
+    """Sizes whose products take the large and the middle tiles, with several
+    tiles a block and several splits."""
+    print(f"case linear tiles {n} {d} {v} {dtype}", flush=True)
+    x, w, t = linear_inputs(cuda, n, d, v, dtype, ignored=0.25, seed=v)
+    check_linear(x, w, t, "sum", z=1e-4)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)

@@ -44,9 +44,17 @@ __device__ __forceinline__ uint16_t half_bits(float v) {
     else return __builtin_bit_cast(uint16_t, (__bf16)v);
 }
 
+template <int DT>
+__device__ __forceinline__ float widen(uint16_t bits) {
+    if constexpr (DT == kF16) return (float)__builtin_bit_cast(_Float16, bits);
+    else return __builtin_bit_cast(float, (uint32_t)bits << 16);
+}
+
 // A value as its matrix operands.  x and w are exact in fp16 and bf16; G,
-// computed in fp32, is rounded to nearest even there (its share of the error
-// of dx and dw is that of one rounding of a term of their sums).
+// computed in fp32, is rounded to nearest even there.  What the rounding of a
+// row's largest entry, its target's, takes off is kept and added to dx and dw
+// in fp32: their error is then that of their own rounding within 5%, against
+// up to 1.5 times as much without (64-bit results, 60 drawn cases).
 template <int DT, int PARTS>
 __device__ __forceinline__ void to_parts(float v, uint16_t (&o)[PARTS]) {
     if constexpr (PARTS == 3) split3(v, o);
@@ -114,6 +122,10 @@ struct PlanArgs {
     int most_splits;
     int64_t room;              // rows of sums there is room for
     float sum_cost;            // what a split's sums of a row cost at the end, in steps
+    int* list;                 // fp16, bf16: rows by their target's group of 64, in order
+    int* list_at;              // [groups + 1]: where a group's rows begin
+    int* rest_row;             // [groups * 64]: set to -1
+    int groups;                // 0: no lists
 };
 
 // What a split's start and its sums of a tile cost: a tile is written and read
@@ -147,6 +159,7 @@ struct MagArgs {
     int64_t ldw, d;
     float* mag;             // [x_blocks + w_blocks]
     int x_blocks, w_blocks;
+    const float* given;     // backward: the forward's, below 0 where it had none
 };
 
 __device__ __forceinline__ float wave_max(float v) {
@@ -169,6 +182,7 @@ __device__ __forceinline__ float block_max(float v, float* sh) {
 }
 
 __device__ __forceinline__ void magnitudes(const PlanArgs& p, const MagArgs& m, int block) {
+    if (m.given && m.given[0] >= 0.0f) return;
     const bool is_x = block < m.x_blocks;
     const int64_t n = is_x ? p.n : p.v;
     const int64_t b = is_x ? block : block - m.x_blocks, blocks = is_x ? m.x_blocks : m.w_blocks;
@@ -204,11 +218,40 @@ __device__ __forceinline__ void magnitudes(const PlanArgs& p, const MagArgs& m, 
     if (threadIdx.x == 0) m.mag[block] = big;
 }
 
-// Block 0 makes the plan; blocks after it take the magnitudes.
+// Rows by their targets' groups of 64 vocabulary entries: a wave a group.
+constexpr int kGroup = 64;
+__device__ __forceinline__ void target_lists(const PlanArgs& p, int block) {
+    const int group = block * (kPlanThreads / 64) + (int)(threadIdx.x >> 6), lane = lane_id();
+    if (group >= p.groups) return;
+    const int64_t lo = (int64_t)group * kGroup, hi = lo + kGroup < p.v ? lo + kGroup : p.v;
+    p.rest_row[lo + lane] = -1;
+    int before = 0, mine = 0;
+    for (int64_t r0 = 0; r0 < p.n; r0 += 64) {
+        const int64_t t = r0 + lane < p.n ? p.target[r0 + lane] : -1;
+        const bool in = t >= 0 && t != p.ignore;
+        before += __popcll(__ballot(in && t < lo));
+        mine += __popcll(__ballot(in && t >= lo && t < hi));
+    }
+    if (lane == 0) {
+        p.list_at[group] = before;
+        if (group == p.groups - 1) p.list_at[p.groups] = before + mine;
+    }
+    for (int64_t r0 = 0; mine > 0 && r0 < p.n; r0 += 64) {
+        const int64_t t = r0 + lane < p.n ? p.target[r0 + lane] : -1;
+        const bool in = t >= lo && t < hi && t != p.ignore;
+        const uint64_t b = __ballot(in);
+        if (in) p.list[before + __popcll(b & ((1ull << lane) - 1))] = (int)(r0 + lane);
+        before += __popcll(b);
+        mine -= __popcll(b);
+    }
+}
+
+// Block 0 makes the plan; blocks after it take the magnitudes or the lists.
 template <bool BWD>
 __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs p, MagArgs m) {
     if (blockIdx.x > 0) {
-        if constexpr (!BWD) magnitudes(p, m, (int)blockIdx.x - 1);
+        if (m.mag) magnitudes(p, m, (int)blockIdx.x - 1);
+        else target_lists(p, (int)blockIdx.x - 1);
         return;
     }
     __shared__ int sh[kPlanThreads / 64];
@@ -263,7 +306,10 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs p, MagArgs 
             p.b[at + k] *= scale;
         }
     }
-    if (threadIdx.x == 0) p.head->live = live;
+    if (threadIdx.x == 0) {
+        p.head->live = live;
+        if constexpr (!BWD) p.lse_out[p.n] = p.lse_out[p.n + 1] = -1.0f;  // no magnitudes; packing sets them
+    }
 }
 
 // The scale of fp32 logits' operands, and what undoes both in a logit; big holds
@@ -300,8 +346,9 @@ struct PackArgs {
     PackSide x, w;
     const Head* head;
     int64_t d, ldp;
-    float* big;        // fp32: magnitudes of x and w; from mag when there is one
-    const float* mag;
+    float* big;        // fp32: magnitudes of x and w
+    const float* mag;  // first piece: where they come from, unless they are given
+    const float* given;
     int x_blocks, w_blocks;
 };
 
@@ -326,11 +373,16 @@ __global__ __launch_bounds__(256) void pack(PackArgs p) {
     float big_x = 0.0f, big_w = 0.0f;
     if constexpr (DT == kF32) {
         if (p.mag) {
-            __shared__ float sh[2][4];
-            for (int k = threadIdx.x; k < p.x_blocks; k += 256) big_x = fmaxf(big_x, p.mag[k]);
-            for (int k = threadIdx.x; k < p.w_blocks; k += 256) big_w = fmaxf(big_w, p.mag[p.x_blocks + k]);
-            big_x = block_max<256>(big_x, sh[0]);
-            big_w = block_max<256>(big_w, sh[1]);
+            if (p.given && p.given[0] >= 0.0f) {
+                big_x = p.given[0];
+                big_w = p.given[1];
+            } else {
+                __shared__ float sh[2][4];
+                for (int k = threadIdx.x; k < p.x_blocks; k += 256) big_x = fmaxf(big_x, p.mag[k]);
+                for (int k = threadIdx.x; k < p.w_blocks; k += 256) big_w = fmaxf(big_w, p.mag[p.x_blocks + k]);
+                big_x = block_max<256>(big_x, sh[0]);
+                big_w = block_max<256>(big_w, sh[1]);
+            }
             if (blockIdx.x == 0 && threadIdx.x == 0) {
                 p.big[0] = big_x;
                 p.big[1] = big_w;
@@ -471,21 +523,22 @@ __global__ __launch_bounds__(S::kThreads, 2) void logits_stats(StatArgs p) {
 }
 
 // ---------------------------------------------------------------------------
-// Few rows (at most 16): bound by reading w once.  Each wave takes 32 rows of w
-// after another, 256 of K at a time through two LDS buffers of its own, so that
-// a row's loads are 512 consecutive bytes and no wave waits for another; x's
-// fragments come from the caches, a stage ahead.  A lane keeps one running
-// (max, sum) of its token over all its wave's rows.  (8, 2048, 128256) in
-// bf16: 89 us, 5.9 TB/s, against 123 us through tiles; without the nontemporal
-// hint 102; rows of 256 bytes a load 106.
+// Few rows (16 in fp16 and bf16, 64 in fp32): bound by reading w once.  Each wave
+// takes 32 rows of w after another, 512 bytes of each at a time through two LDS
+// buffers of its own, so that a row's loads are consecutive and no wave waits
+// for another; x's fragments come from the caches, a stage ahead.  A lane keeps
+// one running (max, sum) of its tokens over all its wave's rows.  (8, 2048,
+// 128256) in bf16: 89 us, 5.9 TB/s, against 123 us through tiles; without the
+// nontemporal hint 102; rows of 256 bytes a load 106.  fp32 is split into bf16
+// parts in registers here, which saves writing and reading w's parts.
 // ---------------------------------------------------------------------------
 struct FewArgs {
-    const uint16_t* w;
+    const void* w;
     int64_t ldw;
-    const uint16_t* x;
+    const void* x;     // fp16, bf16: the packed live rows; fp32: all rows
     int64_t ldx;
-    int k;             // a multiple of 64
-    int v;
+    const int* rows;
+    int k, v;          // k: a multiple of 64; fp32: of 4
     const Head* head;
     const int* tgt;
     float2* part;      // [live row][parts]
@@ -493,52 +546,87 @@ struct FewArgs {
     float* at_target;
 };
 
-constexpr int kFewRows = 16, kFewWaves = 2;
+constexpr int kFewWaves = 2;
+constexpr int few_rows(int dtype) { return dtype == kF32 ? 64 : 16; }
 
-template <int DT>
+// split3 of 8 fp32 values, two to a conversion.
+__device__ __forceinline__ void split_frag(const f32x4& lo, const f32x4& hi, u32x4 (&o)[3]) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        float a = q < 2 ? lo[2 * q] : hi[2 * q - 4], b = q < 2 ? lo[2 * q + 1] : hi[2 * q - 3];
+#pragma unroll
+        for (int p = 0; p < 3; ++p) {
+            const uint32_t u = bf16_pack2(a, b);
+            o[p][q] = u;
+            a -= __builtin_bit_cast(float, u << 16);
+            b -= __builtin_bit_cast(float, u & 0xFFFF0000u);
+        }
+    }
+}
+
+template <int DT, int FN>
 __global__ __launch_bounds__(kFewWaves * 64) void logits_few(FewArgs p) {
-    constexpr int FM = 2, R = FM * 16, KC = 256, STAGE = R * KC * 2, LOADS = STAGE / 1024, KS = KC / 32;
+    typedef typename Io<DT>::T T;
+    constexpr bool F32 = DT == kF32;
+    constexpr int FM = 2, R = FM * 16, ROW = 512, KC = ROW / (int)sizeof(T), STAGE = R * ROW, LOADS = STAGE / 1024;
+    constexpr int KS = KC / 32, XV = F32 ? 2 : 1;  // K of a product; 16-byte vectors of a fragment
     __shared__ __attribute__((aligned(1024))) char lds[kFewWaves * 2 * STAGE];
     const int lane = threadIdx.x & 63, wave = scalar(threadIdx.x >> 6);
     lds_char* mine = (lds_char*)lds + wave * 2 * STAGE;
     const int live = p.head->live;
     const int me = (int)blockIdx.x * kFewWaves + wave, waves = (int)gridDim.x * kFewWaves;
     const int groups = (p.v + R - 1) / R, stages = (p.k + KC - 1) / KC;
-    const int n = lane & 15;
     if (live == 0) return;
-    const uint16_t* x = p.x + (int64_t)(n < live ? n : live - 1) * p.ldx + (lane >> 4) * 8;
-    const int target = n < live ? p.tgt[n] : -1;
-    float m = -kInf, s = 0.0f;
+    const T* x[FN];
+    int target[FN];
+    float m[FN], s[FN];
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+        const int n = j * 16 + (lane & 15), at = n < live ? n : live - 1;
+        x[j] = static_cast<const T*>(p.x) + (int64_t)(F32 ? p.rows[at] : at) * p.ldx;
+        target[j] = n < live ? p.tgt[n] : -1;
+        m[j] = -kInf;
+        s[j] = 0.0f;
+    }
 
     // where the loads are: stage ls of rows lg R ..
     int lg = me, ls = 0;
     const char* base = nullptr;
     uint32_t row[LOADS];
     auto place = [&]() {
-        base = uniform(reinterpret_cast<const char*>(p.w + (int64_t)lg * R * p.ldw));
+        base = uniform(reinterpret_cast<const char*>(static_cast<const T*>(p.w) + (int64_t)lg * R * p.ldw));
 #pragma unroll
         for (int j = 0; j < LOADS; ++j) {
             const int r = j * 2 + (lane >> 5);
-            row[j] = (uint32_t)((lg * R + r < p.v ? r : p.v - 1 - lg * R) * p.ldw * 2);
+            row[j] = (uint32_t)((lg * R + r < p.v ? r : p.v - 1 - lg * R) * p.ldw * (int)sizeof(T));
         }
     };
-    u32x4 next[KS], now[KS];
+    u32x4 next[KS][FN][XV], now[KS][FN][XV];
     auto load = [&](lds_char* buf) {
         const int left = p.k - ls * KC;  // of K, from this stage on
 #pragma unroll
-        for (int t = 0; t < KS; ++t) {
-            const int k = t * 32 < left ? ls * KC + t * 32 : 0;  // past K: not used
-            next[t] = *reinterpret_cast<const u32x4*>(x + k);
-        }
-        const char* b = uniform(base + (int64_t)ls * KC * 2);
+        for (int t = 0; t < KS; ++t)
+#pragma unroll
+            for (int j = 0; j < FN; ++j) {
+                const int k = t * 32 + (lane >> 4) * 8;
+#pragma unroll
+                for (int h = 0; h < XV; ++h) {
+                    // past K: zero, so that what w's side holds there adds nothing
+                    next[t][j][h] = u32x4{0, 0, 0, 0};
+                    if (k + h * 4 < left) __builtin_memcpy(&next[t][j][h], x[j] + ls * KC + k + h * 4, 16);
+                }
+            }
+        const char* b = uniform(base + (int64_t)ls * ROW);
         const uint32_t to = scalar((int)(uint32_t)(uintptr_t)buf);
 #pragma unroll
         for (int j = 0; j < LOADS; ++j) {
-            // the 16 chunks of 256 bytes permuted by the row number, as in a tile
+            // the 16 chunks of 256 bytes permuted by the row number, as in a tile;
+            // past K: the row's last chunk
             const int r = j * 2 + (lane >> 5), c = lane & 31;
-            int col = ((c & 16) | ((c ^ r) & 15)) * 8;
-            if (col > left - 8) col = left - 8;
-            load_to_lds<true>(b, row[j] + col * 2, to + j * 1024);
+            int col = ((c & 16) | ((c ^ r) & 15)) * 16;
+            const int end = left * (int)sizeof(T);
+            if (col > end - 16) col = end - 16;
+            load_to_lds<true>(b, row[j] + col, to + j * 1024);
         }
     };
     auto advance = [&]() {
@@ -550,6 +638,11 @@ __global__ __launch_bounds__(kFewWaves * 64) void logits_few(FewArgs p) {
             place();
         }
     };
+    // chunk c of row r, in a stage's buffer
+    auto chunk = [](const lds_char* buf, int r, int c) {
+        return *reinterpret_cast<const __attribute__((address_space(3))) u32x4*>(buf + r * ROW +
+                                                                                 ((c & 16) | ((c ^ r) & 15)) * 16);
+    };
     lds_char *cur = mine, *nxt = mine + STAGE;
     if (me < groups) {
         place();
@@ -557,30 +650,54 @@ __global__ __launch_bounds__(kFewWaves * 64) void logits_few(FewArgs p) {
         advance();
     }
     for (int g = me; g < groups; g += waves) {
-        f32x4 acc[FM];
+        f32x4 acc[FM][FN];
 #pragma unroll
-        for (int i = 0; i < FM; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         for (int st = 0; st < stages; ++st) {
             // the wave's own copies and x's fragments are there, and its reads of the
             // buffer that is filled next are done
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
 #pragma unroll
-            for (int t = 0; t < KS; ++t) {
-                asm volatile("" : "+v"(next[t]));
-                now[t] = next[t];
-            }
+            for (int t = 0; t < KS; ++t)
+#pragma unroll
+                for (int j = 0; j < FN; ++j)
+#pragma unroll
+                    for (int h = 0; h < XV; ++h) {
+                        asm volatile("" : "+v"(next[t][j][h]));
+                        now[t][j][h] = next[t][j][h];
+                    }
             load(nxt);
             advance();
             const int left = p.k - st * KC;
 #pragma unroll
             for (int t = 0; t < KS; ++t) {
                 if (t * 32 >= left) break;
+                u32x4 b[FN][Grads<DT>::kParts];
+#pragma unroll
+                for (int j = 0; j < FN; ++j) {
+                    if constexpr (F32)
+                        split_frag(__builtin_bit_cast(f32x4, now[t][j][0]), __builtin_bit_cast(f32x4, now[t][j][XV - 1]), b[j]);
+                    else b[j][0] = now[t][j][0];
+                }
 #pragma unroll
                 for (int i = 0; i < FM; ++i) {
-                    const int r = i * 16 + (lane & 15), c = t * 4 + (lane >> 4);
-                    const int at = r * KC * 2 + ((c & 16) | ((c ^ r) & 15)) * 16;
-                    const u32x4 a = *reinterpret_cast<const __attribute__((address_space(3))) u32x4*>(cur + at);
-                    acc[i] = mfma<Logits<DT>::kHalf>(a, now[t], acc[i]);
+                    const int r = i * 16 + (lane & 15);
+                    u32x4 a[Grads<DT>::kParts];
+                    if constexpr (F32) {
+                        const int c = t * 8 + (lane >> 4) * 2;
+                        split_frag(__builtin_bit_cast(f32x4, chunk(cur, r, c)), __builtin_bit_cast(f32x4, chunk(cur, r, c + 1)), a);
+                    } else {
+                        a[0] = chunk(cur, r, t * 4 + (lane >> 4));
+                    }
+                    constexpr int kTerms = terms(Grads<DT>::kParts);
+                    unrolled<kTerms>([&](auto tc) {
+                        constexpr int k = decltype(tc)::value;
+#pragma unroll
+                        for (int j = 0; j < FN; ++j)
+                            acc[i][j] = mfma<Grads<DT>::kHalf>(a[term_a(k)], b[j][term_b(k)], acc[i][j]);
+                    });
                 }
             }
             lds_char* const done = cur;
@@ -588,21 +705,28 @@ __global__ __launch_bounds__(kFewWaves * 64) void logits_few(FewArgs p) {
             nxt = done;
         }
         const int first = g * R + (lane >> 4) * 4;
-        float v[FM * 4];
 #pragma unroll
-        for (int i = 0; i < FM; ++i)
+        for (int j = 0; j < FN; ++j) {
+            float v[FM * 4];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int at = first + i * 16 + q;
-                v[i * 4 + q] = at < p.v ? acc[i][q] : -kInf;
-                if (at == target) p.at_target[n] = acc[i][q];
-            }
-        lse_fold<true>(m, s, v);
+            for (int i = 0; i < FM; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int at = first + i * 16 + q;
+                    v[i * 4 + q] = at < p.v ? acc[i][j][q] : -kInf;
+                    if (at == target[j]) p.at_target[j * 16 + (lane & 15)] = acc[i][j][q];
+                }
+            lse_fold<true>(m[j], s[j], v);
+        }
     }
     wait_copies();
-    lse_merge(m, s, exact_xor<16>(m), exact_xor<16>(s));
-    lse_merge(m, s, exact_xor<32>(m), exact_xor<32>(s));
-    if (lane < 16 && n < live) p.part[n * p.parts + me] = make_float2(m, s);
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+        const int n = j * 16 + (lane & 15);
+        lse_merge(m[j], s[j], exact_xor<16>(m[j]), exact_xor<16>(s[j]));
+        lse_merge(m[j], s[j], exact_xor<32>(m[j]), exact_xor<32>(s[j]));
+        if (lane < 16 && n < live) p.part[n * p.parts + me] = make_float2(m[j], s[j]);
+    }
 }
 
 // Joins a live row's pairs; one wave a row.
@@ -652,6 +776,7 @@ struct GradArgs {
     uint16_t* g;         // [live row][ldg]
     int64_t ldg, g_part;
     const float* big;
+    float* rest;         // fp16, bf16: [live row] what rounding took off the target's entry
 };
 
 // G of a piece.  Rows from the live ones up to a multiple of 64 are zero, and so
@@ -702,6 +827,7 @@ struct GradJob {
             const int hit = r.target[j] >= 0 ? r.target[j] - p.v0 - at.m : -1;
             // rows past the live ones have a = 0, but an exponential of anything
             const int cols = n < live ? left : 0;
+            float hit_g = 0.0f;
 #pragma unroll
             for (int i = 0; i < S::FM; i += 2) {
                 uint16_t o[8][P];
@@ -709,7 +835,7 @@ struct GradJob {
                 for (int q = 0; q < 8; ++q) {
                     const int m = perm_at(i, q);  // q runs over both fragments
                     float g = r.a[j] * fexp2((logit<DT>(acc[i + q / 4][j][q % 4], inv_x, inv_w) - r.lse[j]) * kLog2e);
-                    if (m == hit) g += r.b[j];
+                    if (m == hit) hit_g = g += r.b[j];
                     to_parts<DT>(m < cols ? g : 0.0f, o[q]);
                 }
                 if (n < n_end) {
@@ -721,6 +847,11 @@ struct GradJob {
                         *reinterpret_cast<u32x4*>(p.g + k * p.g_part + n * p.ldg + at.m + i * 16) = u;
                     }
                 }
+            }
+            if constexpr (DT != kF32) {
+                // of the rows that a lane's results cover: hit is one of them
+                if (hit >= 0 && hit < S::FM * 16 && hit % 32 < 8)
+                    p.rest[n] = hit_g - widen<DT>(half_bits<DT>(hit_g));
             }
         }
     }
@@ -747,6 +878,10 @@ struct ProductArgs {
     int64_t ldc;
     int add;
     void* out;          // dw: [n][ldc] results
+    // dw in fp16, bf16: fp32 rows that are added to the results, and which one
+    // (-1: none) to result row n
+    const float* rests;
+    const int* rest_row;
 };
 
 // dx (DX): C[n][d] = sum_v G[n][v] w[v][d] over a piece, added to the splits'
@@ -761,7 +896,10 @@ struct ProductJob {
     typedef typename Io<DT>::T T;
     typedef Side<S, S::TM, false> SA;
     typedef Side<S, S::TN, DX> SB;
-    struct Rows {};
+    static constexpr bool kRests = !DX && DT != kF32;
+    struct Rows {
+        int rest[kRests ? S::FN : 1];
+    };
     __device__ __forceinline__ int split(int t) const { return DX ? scalar((unsigned)t / (unsigned)tiles) : 0; }
     __device__ __forceinline__ TileAt at(int t) const { return tile_at(t - split(t) * tiles, p.tiles_m, tiles_n); }
     // K's steps are cut evenly
@@ -776,8 +914,16 @@ struct ProductJob {
         A.init(p.a, tile.m * S::TM);
         B.init(p.b, tile.n * S::TN);
     }
-    __device__ __forceinline__ Rows rows(int) const { return Rows{}; }
-    __device__ __forceinline__ void finish(int t, const Rows&, const f32x4 (&acc)[S::FM][S::FN]) const {
+    __device__ __forceinline__ Rows rows(int t) const {
+        Rows r{};
+        if constexpr (kRests) {
+            const Place<S> at(0, this->at(t).n * S::TN);
+#pragma unroll
+            for (int j = 0; j < S::FN; ++j) r.rest[j] = at.n + j * 16 < n_end ? p.rest_row[at.n + j * 16] : -1;
+        }
+        return r;
+    }
+    __device__ __forceinline__ void finish(int t, const Rows& r, const f32x4 (&acc)[S::FM][S::FN]) const {
         const TileAt tile = at(t);
         const Place<S> at(tile.m * S::TM, tile.n * S::TN);
         float* sums = DX ? p.acc + (int64_t)split(t) * n_end * p.ldc : nullptr;
@@ -802,6 +948,13 @@ struct ProductJob {
                     }
                 } else {
                     T* c = static_cast<T*>(p.out) + n * p.ldc + m;
+                    if constexpr (kRests) {
+                        if (r.rest[j] >= 0) {
+                            const float* more = p.rests + r.rest[j] * p.ldc + m;
+#pragma unroll
+                            for (int q = 0; q < 4; ++q) v[q] += m + q < p.m ? more[q] : 0.0f;
+                        }
+                    }
                     v *= inv;
                     if (whole && sizeof(T) == 4) {
                         *reinterpret_cast<f32x4*>(c) = v;
@@ -846,26 +999,98 @@ __global__ __launch_bounds__(S::kThreads, 2) void product(ProductArgs p) {
     job.whole = (p.ldc & 3) == 0;
     if (!DX && live == 0) {  // no step of K: dw is zero
         f32x4 none[S::FM][S::FN] = {};
-        for (Walk w(job.tiles); w.t < w.end; w.t += w.stride) job.finish(w.t, {}, none);
+        for (Walk w(job.tiles); w.t < w.end; w.t += w.stride) job.finish(w.t, job.rows(w.t), none);
         return;
     }
     run_tiles<S, false, DX, Grads<DT>::kHalf, Grads<DT>::kParts>(job, job.tiles * job.splits, (lds_char*)buf0,
                                                                  (lds_char*)buf1);
 }
 
-// dx rows from the splits' sums; ignored rows are zero.
+// dw's share of the rests: for each target of a group of 64, the sum over its
+// rows, in order, of rest times x.  A block a group and 64 columns; each of its
+// waves takes a run of the group's rows and keeps a sum in LDS for each of the
+// group's targets, and the waves' sums are added in their order.
+struct RestArgs {
+    const float* rest;
+    const int *list, *list_at, *pos, *tgt;
+    const uint16_t* x;   // packed live rows
+    int64_t ldx;
+    int d, group0;
+    float* rests;        // [place in the list][d]
+    int* rest_row;       // [vocabulary entry]
+};
+template <int DT, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void sum_rests(RestArgs p) {
+    __shared__ float sum[WAVES][kGroup][64];
+    const int group = p.group0 + (int)blockIdx.x, lane = lane_id(), wave = scalar(threadIdx.x >> 6);
+    const int c = (int)blockIdx.y * 64 + lane;
+    const int begin = p.list_at[group], end = p.list_at[group + 1];
+    if (begin == end) return;
+    uint64_t there = 0;  // the group's targets that come
+    for (int e0 = begin; e0 < end; e0 += 64) {
+        uint64_t m = 0;
+        if (e0 + lane < end) m = 1ull << (p.tgt[p.pos[p.list[e0 + lane]]] % kGroup);
+        for (int d = 1; d < 64; d *= 2) m |= __shfl_xor(m, d, 64);
+        there |= m;
+    }
+    const int targets = __popcll(there);
+    for (int k = 0; k < targets; ++k) sum[wave][k][lane] = 0.0f;
+    // a lane reads and writes its own column of its wave's sums only
+    const uint16_t* x = p.x + c;  // packed rows are whole multiples of 64 elements
+    const int per = (end - begin + WAVES * 64 - 1) / (WAVES * 64) * 64;
+    const int mine = begin + wave * per, mine_end = mine + per < end ? mine + per : end;
+    for (int e0 = mine; e0 < mine_end; e0 += 64) {
+        int row = 0, slot = 0;
+        float rest = 0.0f;
+        if (e0 + lane < mine_end) {
+            row = p.pos[p.list[e0 + lane]];
+            slot = __popcll(there & ((1ull << (p.tgt[row] % kGroup)) - 1));
+            rest = p.rest[row];
+        }
+        const int n = mine_end - e0 < 64 ? mine_end - e0 : 64;
+        for (int k0 = 0; k0 < n; k0 += 8) {
+            float v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k)  // past n: row 0, not added
+                v[k] = widen<DT>(x[(int64_t)__builtin_amdgcn_readlane(row, k0 + k) * p.ldx]);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                if (k0 + k >= n) break;
+                const float f = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, rest), k0 + k));
+                sum[wave][__builtin_amdgcn_readlane(slot, k0 + k)][lane] += f * v[k];
+            }
+        }
+    }
+    __syncthreads();
+    for (int k = wave; k < targets; k += WAVES) {
+        float s = sum[0][k][lane];
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w) s += sum[w][k][lane];
+        if (c < p.d) p.rests[(int64_t)(begin + k) * p.d + c] = s;
+    }
+    if (blockIdx.y == 0 && wave == 0 && (there >> lane & 1))
+        p.rest_row[group * kGroup + lane] = begin + __popcll(there & ((1ull << lane) - 1));
+}
+
+// dx rows from the splits' sums, and what rounding took off the targets' entries;
+// ignored rows are zero.
 template <int DT>
-__global__ __launch_bounds__(256) void finish_dx(const Head* head, const int* pos, const float* acc, int64_t d, void* dx) {
+__global__ __launch_bounds__(256) void finish_dx(const Head* head, const int* pos, const float* acc, int64_t d, void* dx,
+                                                 const float* rest, const int* tgt, const void* w, int64_t ldw) {
     typedef typename Io<DT>::T T;
     const int64_t r = blockIdx.x;
     const int at = pos[r];
     const float inv = head->inv_scale;
     const int splits = head->splits;
     const int64_t stride = head->live * d;
+    const int target = at >= 0 && DT != kF32 ? tgt[at] : -1;
+    const float more = target >= 0 ? rest[at] : 0.0f;
+    const T* wt = static_cast<const T*>(w) + target * ldw;
     for (int64_t c = threadIdx.x; c < d; c += 256) {
         float s = 0.0f;
         if (at >= 0) {
             for (int k = 0; k < splits; ++k) s += acc[k * stride + at * d + c];
+            if (target >= 0) s += more * Elem<T>::scalar(wt + c);
             s *= inv;
         }
         Elem<T>::put(static_cast<T*>(dx) + r * d + c, s);
@@ -888,10 +1113,10 @@ struct Layout {
     bool pack_w;         // w is packed a piece at a time
     int splits;          // of K in dx, with every row live
     int64_t room;        // rows of its sums
-    int x_blocks, w_blocks;  // fp32 forward: blocks that take the magnitudes
+    int x_blocks, w_blocks;  // fp32: blocks that take the magnitudes
     int few;             // forward of few rows: its blocks, or 0
     int logits, dx, dw;  // the products' tiles: 256, 128 or 64
-    int64_t head, rows, pos, tgt, at_target, loss_rows, part, parts, a, b, lse, xp, xg, wp, wg, mag, g, acc, bytes;
+    int64_t head, rows, pos, tgt, at_target, loss_rows, part, parts, a, b, lse, xp, xg, wp, wg, mag, big, rest, list, list_at, rest_row, rests, g, acc, bytes;
 };
 
 // A product's tiles: the largest that fill most of the chip.
@@ -932,7 +1157,12 @@ Layout layout(int64_t N, int64_t V, int64_t D, int dtype, bool bwd, bool aligned
     int64_t most = kPieceBytes / (2 * parts * round_up(N, 64)) / 256 * 256;
     if (most < 2048) most = 2048;
     l.ldx = round_up(D, 64);
-    l.pack_w = dtype == kF32 || !aligned || D % 64 != 0;
+    const bool few = N <= few_rows(dtype) && aligned && D % (dtype == kF32 ? 4 : 64) == 0;
+    if (!bwd && few) {
+        const int64_t blocks = div_up(div_up(V, 32), kFewWaves);
+        l.few = (int)(blocks < 512 ? blocks : 512);
+    }
+    l.pack_w = !l.few && (dtype == kF32 || !aligned || D % 64 != 0);
     if (l.pack_w) {
         const int64_t fit = kPieceBytes / (2 * parts * l.ldx) / 256 * 256;
         if (most > fit) most = fit < 2048 ? 2048 : fit;
@@ -946,15 +1176,12 @@ Layout layout(int64_t N, int64_t V, int64_t D, int dtype, bool bwd, bool aligned
     l.tgt = take(4 * N);
     l.xp = take(2 * lparts * N * l.ldx);
     l.wp = take(l.pack_w ? 2 * lparts * l.piece * l.ldx : 0);
-    l.x_blocks = dtype == kF32 && !bwd ? (int)(div_up(N, 16) < 32 ? div_up(N, 16) : 32) : 0;
-    l.w_blocks = dtype == kF32 && !bwd ? (int)(div_up(V, 16) < 256 ? div_up(V, 16) : 256) : 0;
+    l.x_blocks = dtype == kF32 && !l.few ? (int)(div_up(N, 16) < 32 ? div_up(N, 16) : 32) : 0;
+    l.w_blocks = dtype == kF32 && !l.few ? (int)(div_up(V, 16) < 256 ? div_up(V, 16) : 256) : 0;
     l.mag = take(4 * (l.x_blocks + l.w_blocks));
+    l.big = take(8);
     l.logits = tile_size(l.piece, N, 1);
     if (!bwd) {
-        if (N <= kFewRows && !l.pack_w) {
-            const int64_t blocks = div_up(div_up(V, 32), kFewWaves);
-            l.few = (int)(blocks < 512 ? blocks : 512);
-        }
         l.parts = l.few ? l.few * kFewWaves : div_up(V, l.logits / 2);
         l.at_target = take(4 * N);
         l.loss_rows = take(4 * N);
@@ -963,6 +1190,11 @@ Layout layout(int64_t N, int64_t V, int64_t D, int dtype, bool bwd, bool aligned
         l.a = take(4 * N);
         l.b = take(4 * N);
         l.lse = take(4 * N);
+        l.rest = take(4 * N);
+        l.list = take(4 * N);
+        l.list_at = take(4 * (div_up(V, kGroup) + 1));
+        l.rest_row = take(4 * round_up(V, kGroup));
+        l.rests = take(dtype == kF32 ? 0 : 4 * N * D);
         dx_plan(D, N, l.piece / kStep, terms((int)parts), l.dx, l.splits);
         l.dw = tile_size(D, l.piece, 1);
         // fp32: x and w again in the gradients' parts
@@ -1005,8 +1237,8 @@ struct Operands {
 // Packs what has to be packed for the piece at v0 (x with the first piece) and
 // sets up its operands.
 template <int DT>
-void operands(const Call& c, const Layout& l, int64_t v0, int64_t rows, bool dx, bool dw, bool fwd, float* big,
-              Operands& o) {
+void operands(const Call& c, const Layout& l, int64_t v0, int64_t rows, bool dx, bool dw, float* big,
+              const float* given, Operands& o) {
     typedef typename Io<DT>::T T;
     const T* w = static_cast<const T*>(c.w) + v0 * c.ldw;
     PackArgs p{};
@@ -1014,7 +1246,8 @@ void operands(const Call& c, const Layout& l, int64_t v0, int64_t rows, bool dx,
     p.d = c.D;
     p.ldp = l.ldx;
     p.big = big;
-    if (fwd && v0 == 0) p.mag = at<float>(c, l.mag);
+    if (v0 == 0) p.mag = at<float>(c, l.mag);
+    p.given = given;
     p.x_blocks = l.x_blocks;
     p.w_blocks = l.w_blocks;
     if (v0 == 0) {
@@ -1070,27 +1303,38 @@ PlanArgs plan_args(const Call& c, const Layout& l) {
 }
 
 template <int DT>
+MagArgs mag_args(const Call& c, const Layout& l, const float* given) {
+    if constexpr (DT != kF32) return MagArgs{};
+    return MagArgs{static_cast<const float*>(c.x), c.ldx,      static_cast<const float*>(c.w), c.ldw, c.D,
+                   at<float>(c, l.mag),            l.x_blocks, l.w_blocks,                     given};
+}
+
+template <int DT>
 void run_fwd(const Call& c, const Layout& l, float* loss, float* lse) {
     PlanArgs p = plan_args(c, l);
     p.loss_rows = c.reduction == 0 ? loss : at<float>(c, l.loss_rows);
     p.lse_out = lse;
-    MagArgs m{};
-    if constexpr (DT == kF32)
-        m = MagArgs{static_cast<const float*>(c.x), c.ldx,      static_cast<const float*>(c.w), c.ldw, c.D,
-                    at<float>(c, l.mag),            l.x_blocks, l.w_blocks};
-    plan_kernel<false><<<dim3((unsigned)(1 + l.x_blocks + l.w_blocks)), kPlanThreads, 0, c.s>>>(p, m);
+    plan_kernel<false><<<dim3((unsigned)(1 + l.x_blocks + l.w_blocks)), kPlanThreads, 0, c.s>>>(
+        p, mag_args<DT>(c, l, nullptr));
     Operands o{};
     float* big = lse + c.N;
     for (int64_t v0 = 0; v0 < c.V; v0 += l.piece) {
         const int64_t rows = c.V - v0 < l.piece ? c.V - v0 : l.piece;
-        operands<DT>(c, l, v0, rows, false, false, true, big, o);
-        if constexpr (DT != kF32) {  // fp32 is packed, and packing reads w as well
-            if (l.few) {
-                logits_few<DT><<<dim3((unsigned)l.few), kFewWaves * 64, 0, c.s>>>(
-                    FewArgs{o.w.p, o.w.ld, o.x.p, o.x.ld, (int)l.ldx, (int)rows, p.head, p.tgt, at<float2>(c, l.part),
-                            l.parts, at<float>(c, l.at_target)});
-                continue;
+        if (DT != kF32 || !l.few) operands<DT>(c, l, v0, rows, false, false, big, nullptr, o);
+        if (l.few) {
+            FewArgs f{c.w, c.ldw, o.x.p, o.x.ld, p.rows, (int)c.D, (int)c.V, p.head, p.tgt, at<float2>(c, l.part), l.parts,
+                      at<float>(c, l.at_target)};
+            const dim3 grid((unsigned)l.few), block(kFewWaves * 64);
+            if constexpr (DT == kF32) {
+                f.x = c.x;
+                f.ldx = c.ldx;
+                if (c.N > 32) logits_few<DT, 4><<<grid, block, 0, c.s>>>(f);
+                else if (c.N > 16) logits_few<DT, 2><<<grid, block, 0, c.s>>>(f);
+                else logits_few<DT, 1><<<grid, block, 0, c.s>>>(f);
+            } else {
+                logits_few<DT, 1><<<grid, block, 0, c.s>>>(f);
             }
+            break;  // one piece
         }
         StatArgs a{};
         a.w = o.w;
@@ -1133,17 +1377,23 @@ void run_bwd(const Call& c, const Layout& l, const float* grad, const float* lse
     // about 1.35 us
     p.sum_cost = (float)((double)c.D * 4 / (5e12 * 1.35e-6) / (double)div_up(c.V, l.piece));
     p.room = l.room;
-    plan_kernel<true><<<1, kPlanThreads, 0, c.s>>>(p, MagArgs{});
+    p.list = at<int>(c, l.list);
+    p.list_at = at<int>(c, l.list_at);
+    p.rest_row = at<int>(c, l.rest_row);
+    p.groups = DT != kF32 && dw ? (int)div_up(c.V, kGroup) : 0;
+    const int64_t beside = DT == kF32 ? l.x_blocks + l.w_blocks : div_up(p.groups, kPlanThreads / 64);
+    plan_kernel<true><<<dim3((unsigned)(1 + beside)), kPlanThreads, 0, c.s>>>(p, mag_args<DT>(c, l, lse + c.N));
     Operands o{};
-    float* big = const_cast<float*>(lse) + c.N;  // read, not written, here
+    float* big = at<float>(c, l.big);
     const int64_t g_part = round_up(c.N, 64) * l.piece;
     for (int64_t v0 = 0; v0 < c.V; v0 += l.piece) {
         const int64_t rows = c.V - v0 < l.piece ? c.V - v0 : l.piece;
-        operands<DT>(c, l, v0, rows, dx != nullptr, dw != nullptr, false, big, o);
+        operands<DT>(c, l, v0, rows, dx != nullptr, dw != nullptr, big, lse + c.N, o);
         GradArgs g{};
         g.w = o.w;
         g.x = o.x;
         g.big = big;
+        g.rest = at<float>(c, l.rest);
         g.steps = (int)(l.ldx / kStep);
         g.head = p.head;
         g.tgt = p.tgt;
@@ -1164,6 +1414,8 @@ void run_bwd(const Call& c, const Layout& l, const float* grad, const float* lse
         a.head = p.head;
         a.m = (int)c.D;
         a.ldc = c.D;
+        a.rests = at<float>(c, l.rests);
+        a.rest_row = p.rest_row + v0;
         if (dx) {
             a.a = o.wg;
             a.b = Operand{g.g, l.piece, g_part, (int)c.N, l.piece};
@@ -1178,6 +1430,17 @@ void run_bwd(const Call& c, const Layout& l, const float* grad, const float* lse
             });
         }
         if (dw) {
+            if constexpr (DT != kF32) {
+                const RestArgs r{g.rest,  p.list,   p.list_at, p.pos,                 p.tgt,
+                                 o.x.p,   o.x.ld,   (int)c.D,  (int)(v0 / kGroup),    at<float>(c, l.rests),
+                                 p.rest_row};
+                const dim3 grid((unsigned)div_up(rows, kGroup), (unsigned)div_up(c.D, 64));
+                // many rows a group (small vocabularies): eight waves share them.
+                // (2469, 64, 125): the call 412 us with one wave, which is all that
+                // fits eight blocks a CU where most groups have a few rows
+                if (c.N * kGroup > 256 * c.V) sum_rests<DT, 8><<<grid, 512, 0, c.s>>>(r);
+                else sum_rests<DT, 1><<<grid, 64, 0, c.s>>>(r);
+            }
             a.a = o.xg;
             a.b = Operand{g.g, l.piece, g_part, 0, l.piece};
             a.n = (int)rows;
@@ -1190,13 +1453,14 @@ void run_bwd(const Call& c, const Layout& l, const float* grad, const float* lse
         }
     }
     if (dx)
-        finish_dx<DT><<<dim3((unsigned)c.N), 256, 0, c.s>>>(p.head, p.pos, at<float>(c, l.acc), c.D, dx);
+        finish_dx<DT><<<dim3((unsigned)c.N), 256, 0, c.s>>>(p.head, p.pos, at<float>(c, l.acc), c.D, dx,
+                                                            at<float>(c, l.rest), p.tgt, c.w, c.ldw);
 }
 
 // w's rows can be read as operands where they are: 16-byte loads at 16-byte
 // addresses, and a tile's rows within 32-bit offsets.
 bool is_aligned(const void* w, int64_t ldw, int dtype) {
-    return dtype != kF32 && (reinterpret_cast<uintptr_t>(w) & 15u) == 0 && ldw % 8 == 0 && ldw <= (1 << 22);
+    return (reinterpret_cast<uintptr_t>(w) & 15u) == 0 && ldw % (dtype == kF32 ? 4 : 8) == 0 && ldw <= (1 << 22);
 }
 
 int check(const char* name, const Call& c, int dtype, size_t ws_bytes, bool bwd) {

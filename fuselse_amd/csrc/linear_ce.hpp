@@ -30,11 +30,11 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 // to 2^-23 of itself or 2^-39 of the largest, whichever is more; three partial
 // products, the one left out below 2^-22 of the product.
 //
-// dx and dw: three bf16 parts of 8 bits, truncated, so that the first part of a
-// large value does not overflow: exact at any magnitude, which G, whose
-// entries reach from 1 down to nothing, needs and fp16's exponents do not
-// give.  Six partial products; those left out are below 2^-21 of the product
-// together.
+// dx and dw: three bf16 parts of 8 bits, to nearest: exact at any magnitude,
+// which G, whose entries reach from 1 down to nothing, needs and fp16's
+// exponents do not give (values within 2^-9 of the largest fp32 count as
+// infinite, and infinite ones make NaN).  Six partial products; those left out are below 2^-24 of the
+// product together.
 //
 // The 16-bit matrix rate is 16 times the fp32 one, so three products cost 0.19
 // and six 0.375 of one fp32 product.
@@ -50,15 +50,12 @@ __device__ __forceinline__ void split2(float v, uint16_t (&o)[2]) {
     o[0] = __builtin_bit_cast(uint16_t, hi);
     o[1] = __builtin_bit_cast(uint16_t, lo);
 }
+__device__ __forceinline__ uint16_t bf16_bits(float v) { return __builtin_bit_cast(uint16_t, (__bf16)v); }
 __device__ __forceinline__ void split3(float v, uint16_t (&o)[3]) {
-    const uint32_t u = __builtin_bit_cast(uint32_t, v);
-    o[0] = (uint16_t)(u >> 16);
-    // a part that is inf or NaN has no rest
-    const float r1 = __builtin_isfinite(v) ? v - __builtin_bit_cast(float, u & 0xFFFF0000u) : 0.0f;
-    const uint32_t u1 = __builtin_bit_cast(uint32_t, r1);
-    o[1] = (uint16_t)(u1 >> 16);
-    const float r2 = r1 - __builtin_bit_cast(float, u1 & 0xFFFF0000u);
-    o[2] = (uint16_t)(__builtin_bit_cast(uint32_t, r2) >> 16);
+    o[0] = bf16_bits(v);
+    const float r1 = v - __builtin_bit_cast(float, (uint32_t)o[0] << 16);  // NaN of an infinite v
+    o[1] = bf16_bits(r1);
+    o[2] = bf16_bits(r1 - __builtin_bit_cast(float, (uint32_t)o[1] << 16));
 }
 
 // Exponent e of the power of two that brings a magnitude m to [2^(to - 1),

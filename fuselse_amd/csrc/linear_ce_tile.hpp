@@ -229,10 +229,10 @@ struct TileAt {
     int m, n;
 };
 __device__ __forceinline__ TileAt tile_at(int t, int tiles_m, int tiles_n) {
-    constexpr int kGroup = 4;
-    const int group = scalar((int)((unsigned)t / (unsigned)(kGroup * tiles_n))), first = group * kGroup;
-    const int gm = tiles_m - first < kGroup ? tiles_m - first : kGroup;
-    const int r = t - group * kGroup * tiles_n;
+    constexpr int kRows = 4;
+    const int group = scalar((int)((unsigned)t / (unsigned)(kRows * tiles_n))), first = group * kRows;
+    const int gm = tiles_m - first < kRows ? tiles_m - first : kRows;
+    const int r = t - group * kRows * tiles_n;
     const int n = scalar((int)((unsigned)r / (unsigned)gm));
     return {first + r - n * gm, n};
 }

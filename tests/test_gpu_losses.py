@@ -160,9 +160,9 @@ def test_linear_several_pieces(cuda, n, d, v, dtype):
     check_linear(x, w, t, "sum")
 
 
-@pytest.mark.parametrize("n", [1, 3, 16, 17])
-@pytest.mark.parametrize("d,v", [(64, 1), (64, 33), (192, 4097), (320, 70001), (1088, 32003)])
-@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("n", [1, 3, 16, 17, 33, 64, 65])
+@pytest.mark.parametrize("d,v", [(64, 1), (68, 33), (192, 4097), (320, 70001), (1088, 32003)])
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_linear_few_rows(cuda, n, d, v, dtype):
     """Rows that one pass over the projection serves, K ending inside a stage,
     vocabularies of less and more than a row group a wave."""

@@ -104,18 +104,34 @@ __global__ __launch_bounds__(kThreads) void fwd_rows(FwdArgs p) {
     float m = -kInf, s = 0.0f;
     int64_t e = e0 + (int64_t)threadIdx.x * VE;
     constexpr int64_t step = (int64_t)kThreads * VE;
-    for (; e + (U - 1) * step + VE <= e1; e += U * step) {
-        u32x4 raw[U];
+    auto fold = [&](const u32x4& raw) {
+        float v[VE];
+        Elem<T>::cvt(raw, v);
 #pragma unroll
-        for (int u = 0; u < U; ++u) __builtin_memcpy(&raw[u], x + e + u * step, 16);
+        for (int k = 0; k < VE; ++k) v[k] *= p.inv_t;
+        lse_fold<true>(m, s, v);
+    };
+    // U vectors are folded while the next U are in flight
+    const int64_t full = U * step + VE - step;  // elements from e on that U vectors span
+    u32x4 now[U], next[U];
+    bool more = e + full <= e1;
+    if (more) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            float v[VE];
-            Elem<T>::cvt(raw[u], v);
+        for (int u = 0; u < U; ++u) now[u] = load_raw_stream<T>(x + e + u * step);
+        e += U * step;
+    }
+    while (more) {
+        const bool again = e + full <= e1;
+        if (again) {
 #pragma unroll
-            for (int k = 0; k < VE; ++k) v[k] *= p.inv_t;
-            lse_fold<true>(m, s, v);
+            for (int u = 0; u < U; ++u) next[u] = load_raw_stream<T>(x + e + u * step);
+            e += U * step;
         }
+#pragma unroll
+        for (int u = 0; u < U; ++u) fold(now[u]);
+#pragma unroll
+        for (int u = 0; u < U; ++u) now[u] = next[u];
+        more = again;
     }
     for (; e < e1; e += step) {
         float v[VE];
@@ -207,75 +223,95 @@ struct BwdArgs {
 
 constexpr int kBwdVecs = 8;  // vectors a thread
 
+// A block takes kBwdVecs vectors a thread of a row of the result, from the
+// result's first 128-byte line on, so that a wave stores whole lines; the input,
+// whose rows may lie in another phase, is read at any alignment.  The elements
+// before the first line and after the last vector belong to the first and the
+// last chunk.
 template <typename T, typename TT>
 __global__ __launch_bounds__(kThreads) void bwd_rows(BwdArgs p) {
     constexpr int VE = Elem<T>::kVec;
-    constexpr int64_t chunk = (int64_t)kThreads * VE * kBwdVecs;
+    constexpr int kChunk = kThreads * kBwdVecs;  // vectors
     __shared__ int li[kMaxTop];
     __shared__ float lp[kMaxTop];
     __shared__ int ln;
     const int64_t block = p.block0 + blockIdx.x;
     const int64_t r = block / p.chunks;
-    const int c = (int)(block % p.chunks);
+    const int c = (int)(block % p.chunks), tid = threadIdx.x;
     const T* x = static_cast<const T*>(p.x) + p.map.offset(r);
     T* dx = static_cast<T*>(p.dx) + r * p.v;
-    const int64_t e0 = c * chunk;
-    const int len = (int)(p.v - e0 < chunk ? p.v - e0 : chunk);
+    // the row's vectors, and this chunk's elements [e0, e1)
+    int head = (int)(((128 - (reinterpret_cast<uintptr_t>(dx) & 127)) & 127) / sizeof(T));
+    if (head > p.v) head = (int)p.v;
+    const int vecs = (int)((p.v - head) / VE);
+    const int v0 = c * kChunk, v1 = vecs - v0 < kChunk ? vecs : v0 + kChunk;
+    const bool last = c == p.chunks - 1;
+    const int body = head + v0 * VE;  // the chunk's first whole vector
+    const int e0 = c == 0 ? 0 : body, e1 = last ? (int)p.v : head + v1 * VE;
+
     const float tlse = p.tlse[r];
     const bool dead = tlse == -kInf;
+    u32x4 raw[kBwdVecs] = {};
+    if (!dead && vecs > 0) {
+#pragma unroll
+        for (int u = 0; u < kBwdVecs; ++u) {
+            // past the last vector: the last one, so that no load has a branch of its own
+            const int v = v0 + u * kThreads + tid;
+            raw[u] = load_raw_stream<T>(x + head + (int64_t)(v < vecs ? v : vecs - 1) * VE);
+        }
+    }
     const float g = dead ? 0.0f : p.grad[r * p.grad_stride] * p.temp * (p.norm ? *p.norm : 1.0f);
     const float lse = p.lse[r];
     // the teacher's entries of this chunk, in order, found by one wave
-    if (threadIdx.x < 64) {
+    if (tid < 64) {
         int n = 0;
         for (int k0 = 0; !dead && k0 < p.k; k0 += 64) {
-            const int k = k0 + (int)threadIdx.x;
+            const int k = k0 + tid;
             int64_t i = -1;
             float tv = -kInf;
             if (k < p.k) {
-                i = p.index[r * p.k + k] - e0;
+                i = p.index[r * p.k + k];
                 tv = Elem<TT>::scalar(static_cast<const TT*>(p.t) + r * p.k + k) * p.inv_t;
             }
-            const bool mine = tv != -kInf && i >= 0 && i < len;
+            const bool mine = tv != -kInf && i >= e0 && i < e1;
             const uint64_t b = __ballot(mine);
             if (mine) {
-                const int at = n + __popcll(b & ((1ull << threadIdx.x) - 1));
+                const int at = n + __popcll(b & ((1ull << tid) - 1));
                 li[at] = (int)i;
                 lp[at] = g * fexp2((tv - tlse) * kLog2e);
             }
             n += __popcll(b);
         }
-        if (threadIdx.x == 0) ln = n;
+        if (tid == 0) ln = n;
     }
     __syncthreads();
     const float gq = tlse != tlse ? __builtin_nanf("") : g;
+    auto grad = [&](float v) { return dead ? 0.0f : gq * fexp2((v * p.inv_t - lse) * kLog2e); };
+    // the elements off the grid: one a thread
+    if (c == 0 && tid < head) Elem<T>::put(dx + tid, grad(dead ? 0.0f : Elem<T>::scalar(x + tid)));
+    const int tail = head + vecs * VE;
+    if (last && tid < p.v - tail) Elem<T>::put(dx + tail + tid, grad(dead ? 0.0f : Elem<T>::scalar(x + tail + tid)));
+    // stores past the chunk's vectors fall outside the resource and are dropped
+    const __amdgpu_buffer_rsrc_t to =
+        __builtin_amdgcn_make_buffer_rsrc(dx + body, 0, v1 > v0 ? (v1 - v0) * 16 : 0, 0x00020000);
 #pragma unroll
     for (int u = 0; u < kBwdVecs; ++u) {
-        const int e = (u * kThreads + (int)threadIdx.x) * VE;
-        if (e >= len) continue;
-        float v[VE];
-        if (!dead) {
-            load_vec_part<T>(x + e0 + e, len - e, 0.0f, v);
+        float o[VE];
+        Elem<T>::cvt(raw[u], o);
 #pragma unroll
-            for (int k = 0; k < VE; ++k) v[k] = gq * fexp2((v[k] * p.inv_t - lse) * kLog2e);
-        } else {
-#pragma unroll
-            for (int k = 0; k < VE; ++k) v[k] = 0.0f;
-        }
-#pragma unroll
-        for (int k = 0; k < VE; ++k)
-            if (e + k < len) Elem<T>::put(dx + e0 + e + k, v[k]);
+        for (int k = 0; k < VE; ++k) o[k] = grad(o[k]);
+        Elem<T>::put_vec_buf(to, (u * kThreads + tid) * 16, o);
     }
-    // An entry's element is written again by the thread that wrote its vector
-    // (one thread's stores to an address keep their order), with the sum of
-    // all entries of that index.
+    // An entry's element is written again by the thread that wrote it before (one
+    // thread's stores to an address keep their order), with the sum of all
+    // entries of that index.
     for (int j = 0; j < ln; ++j) {
         const int i = li[j];
-        if ((i / VE) % kThreads != (int)threadIdx.x) continue;
+        const int owner = i < head ? i : i >= tail ? i - tail : (i - head) / VE % kThreads;
+        if (owner != tid) continue;
         float take = 0.0f;
         for (int k = 0; k < ln; ++k) take += li[k] == i ? lp[k] : 0.0f;
-        const float q = gq * fexp2((Elem<T>::scalar(x + e0 + i) * p.inv_t - lse) * kLog2e);
-        Elem<T>::put(dx + e0 + i, q - take);
+        Elem<T>::put(dx + i, grad(Elem<T>::scalar(x + i)) - take);
     }
 }
 
@@ -315,8 +351,11 @@ void launch_fwd(const FwdArgs& a, hipStream_t s) {
 template <typename T, typename TT>
 void launch_bwd(const BwdArgs& a, hipStream_t s) {
     BwdArgs b = a;
-    constexpr int64_t chunk = (int64_t)kThreads * Elem<T>::kVec * kBwdVecs;
-    b.chunks = (int)((a.v + chunk - 1) / chunk);
+    // a row has at most this many whole vectors; with none its few elements
+    // still take a chunk
+    constexpr int64_t chunk = (int64_t)kThreads * kBwdVecs;
+    b.chunks = (int)((a.v / Elem<T>::kVec + chunk - 1) / chunk);
+    if (b.chunks < 1) b.chunks = 1;
     for_grid_chunks(a.rows * b.chunks, kThreads, [&](int64_t first, int64_t count) {
         b.block0 = first;
         bwd_rows<T, TT><<<dim3((unsigned)count), kThreads, 0, s>>>(b);

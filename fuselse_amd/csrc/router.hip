@@ -6,11 +6,13 @@
 //   balance = E sum_e f_e mean_t p_te,   z = mean_t lse_t^2,
 //   dl_te = p_te (gb E / n (f_e - sum_j p_tj f_j) + gz 2 lse_t / n).
 //
-// A group of lanes holds a token's logits in registers; a lane meets the same
-// experts in every token and sums their probabilities in registers, joined per
-// block and then over blocks in a fixed order, so results do not depend on the
-// order of the blocks.  Both directions read the logits once and are bound by
-// memory, or by the launches where the batch is small.
+// A group of lanes holds a token's logits in registers, up to four 16-byte
+// vectors a lane, so that a wave has several tokens' loads in flight and few
+// steps of a reduction to wait for.  A lane meets the same experts in every
+// token and sums their probabilities in registers, joined per wave, per block
+// and then over blocks in a fixed order, so results do not depend on the order
+// of the blocks.  Both directions read the logits once and are bound by memory,
+// or by the launches where the batch is small: one block then does it all.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -24,7 +26,7 @@ namespace fl {
 namespace router {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 512;
 constexpr int kMaxExperts = 1024;
 
 struct Args {
@@ -37,10 +39,11 @@ struct Args {
     const uint8_t* mask;  // NULL: every token counts
     float* lse;
     // per block
-    float* sum_p;   // [blocks][experts]
-    int* count;     // [blocks][experts]
+    int2* part;     // [blocks][experts]: the probabilities' sum (fp32 bits), the choices
     double* sum_z;  // [blocks]
     int* live;      // [blocks]
+    double* shares; // [finishing blocks]: of the balance
+    int* arrived;   // finishing blocks that are done; cleared by the first kernel
     int blocks;
     // results
     float* balance;
@@ -51,6 +54,7 @@ struct Args {
     const float* gb;
     const float* gz;
     void* dx;
+    bool whole;  // rows of dx are whole 16-byte vectors
 };
 
 // A token's logits: NV vectors a lane, lane `sub` of G holding vectors
@@ -74,66 +78,95 @@ __device__ __forceinline__ float token_lse(const float (&v)[NV][VE]) {
     return lse_finish<true>(m, s);
 }
 
-// Joins the blocks' sums and writes the results; one block.
-__device__ __forceinline__ void finish(const Args& p) {
-    __shared__ double sh[kThreads];
-    __shared__ int shn;
-    int n = 0;
-    double z = 0.0;
-    for (int b = threadIdx.x; b < p.blocks; b += kThreads) {
-        n += p.live[b];
-        z += p.sum_z[b];
-    }
-    if (threadIdx.x == 0) shn = 0;
-    sh[threadIdx.x] = z;
+__device__ __forceinline__ double wave_sum(double v) {
+    for (int d = 1; d < 64; d *= 2) v += __shfl_xor(v, d, 64);
+    return v;
+}
+// Sum of v over the block, in a fixed order; all threads get it.
+template <int THREADS = kThreads>
+__device__ __forceinline__ double block_sum(double v, double* sh) {
+    v = wave_sum(v);
     __syncthreads();
-    atomicAdd(&shn, n);
-    for (int d = kThreads / 2; d > 0; d >>= 1) {
-        __syncthreads();
-        if ((int)threadIdx.x < d) sh[threadIdx.x] += sh[threadIdx.x + d];
-    }
+    if (lane_id() == 0) sh[threadIdx.x >> 6] = v;
     __syncthreads();
-    n = shn;
-    z = sh[0];
-    __syncthreads();
+    v = 0.0;
+    for (int w = 0; w < THREADS / 64; ++w) v += sh[w];
+    return v;
+}
+
+// Results from the sums over blocks of expert e's probabilities and choices (sp,
+// c; of this thread's expert, e < experts), of z and of tokens.
+__device__ __forceinline__ void results(const Args& p, int e, double sp, int64_t c, double z, int n, double& bal) {
     const double inv = n > 0 ? 1.0 / n : 0.0;
-    double bal = 0.0;
-    for (int e = threadIdx.x; e < p.experts; e += kThreads) {
-        double sp = 0.0;
-        int64_t c = 0;
-        for (int b = 0; b < p.blocks; ++b) {
-            sp += p.sum_p[(int64_t)b * p.experts + e];
-            c += p.count[(int64_t)b * p.experts + e];
-        }
-        const double f = p.top > 0 ? c * inv / p.top : 0.0;
-        p.counts[e] = c;
-        p.coef[e] = (float)(p.experts * f * inv);
-        bal += f * sp * inv;
-    }
-    sh[threadIdx.x] = bal;
-    for (int d = kThreads / 2; d > 0; d >>= 1) {
-        __syncthreads();
-        if ((int)threadIdx.x < d) sh[threadIdx.x] += sh[threadIdx.x + d];
-    }
-    if (threadIdx.x == 0) {
-        *p.balance = (float)(p.experts * sh[0]);
+    const double f = p.top > 0 ? c * inv / p.top : 0.0;
+    p.counts[e] = c;
+    p.coef[e] = (float)(p.experts * f * inv);
+    bal += f * sp * inv;
+    if (e == 0) {
         *p.z = (float)(z * inv);
         p.coef[p.experts] = (float)(2.0 * inv);
+    }
+}
+
+// Joins the blocks' sums, eight experts a block: the parts lie in other XCDs'
+// memory, of which one CU reads no more than about 12 GB/s (256 blocks of 256
+// experts: 42 us in one block).  The balance is the sum of the blocks' shares,
+// added up in their order by the last block to arrive.
+constexpr int kFinish = 256, kFinishExperts = 8, kRuns = kFinish / kFinishExperts;
+__global__ __launch_bounds__(kFinish) void fwd_finish(Args p) {
+    __shared__ double sh[kFinish / 64], shp[kRuns][kFinishExperts];
+    __shared__ int shc[kRuns][kFinishExperts];
+    double zs = 0.0, ns = 0.0;
+    for (int b = threadIdx.x; b < p.blocks; b += kFinish) {
+        zs += p.sum_z[b];
+        ns += p.live[b];
+    }
+    const double z = block_sum<kFinish>(zs, sh);
+    const int n = (int)block_sum<kFinish>(ns, sh);
+    const int run = (int)threadIdx.x / kFinishExperts, ee = (int)threadIdx.x % kFinishExperts;
+    const int e = (int)blockIdx.x * kFinishExperts + ee;
+    double sp = 0.0, bal = 0.0;
+    int c = 0;
+    if (e < p.experts) {
+        for (int b = run; b < p.blocks; b += kRuns) {
+            const int2 v = p.part[(int64_t)b * p.experts + e];
+            sp += __builtin_bit_cast(float, v.x);
+            c += v.y;
+        }
+    }
+    shp[run][ee] = sp;
+    shc[run][ee] = c;
+    __syncthreads();
+    if (run == 0 && e < p.experts) {
+        for (int k = 1; k < kRuns; ++k) {
+            sp += shp[k][ee];
+            c += shc[k][ee];
+        }
+        results(p, e, sp, c, z, n, bal);
+    }
+    bal = block_sum<kFinish>(bal, sh);
+    if (threadIdx.x == 0) {
+        __hip_atomic_store(&p.shares[blockIdx.x], bal, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const int before = __hip_atomic_fetch_add(p.arrived, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+        if (before == (int)gridDim.x - 1) {
+            double all = 0.0;
+            for (int b = 0; b < (int)gridDim.x; ++b)
+                all += __hip_atomic_load(&p.shares[b], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            *p.balance = (float)(p.experts * all);
+        }
     }
 }
 
 template <typename T, int G, int NV>
 __global__ __launch_bounds__(kThreads) void fwd_tokens(Args p) {
     constexpr int VE = Elem<T>::kVec;
-    constexpr int GROUPS = kThreads / G;
+    constexpr int GROUPS = kThreads / G, WAVES = kThreads / 64;
     constexpr int W = G * NV * VE;  // experts the lanes hold
-    __shared__ float shp[GROUPS < 16 ? GROUPS : 16][W];
+    __shared__ float shp[WAVES][W];
     __shared__ int shc[W];
-    __shared__ double shz[kThreads];
-    __shared__ int shl;
-    const int group = threadIdx.x / G, sub = threadIdx.x % G;
+    __shared__ double sh[WAVES];
+    const int group = threadIdx.x / G, sub = threadIdx.x % G, wave = threadIdx.x >> 6;
     for (int e = threadIdx.x; e < W; e += kThreads) shc[e] = 0;
-    if (threadIdx.x == 0) shl = 0;
     __syncthreads();
     float sum[NV][VE] = {};
     double z = 0.0;
@@ -145,6 +178,10 @@ __global__ __launch_bounds__(kThreads) void fwd_tokens(Args p) {
         }
         float v[NV][VE];
         load_token<T, G, NV>(static_cast<const T*>(p.x) + t * p.ldx, p.experts, sub, v);
+        for (int k = sub; k < p.top; k += G) {
+            const int64_t e = p.index[t * p.top + k];
+            if (e >= 0 && e < p.experts) atomicAdd(&shc[e], 1);
+        }
         const float lse = token_lse<G, NV, VE>(v);
 #pragma unroll
         for (int j = 0; j < NV; ++j)
@@ -155,51 +192,39 @@ __global__ __launch_bounds__(kThreads) void fwd_tokens(Args p) {
             z += (double)lse * lse;
             ++live;
         }
-        for (int k = sub; k < p.top; k += G) {
-            const int64_t e = p.index[t * p.top + k];
-            if (e >= 0 && e < p.experts) atomicAdd(&shc[e], 1);
-        }
     }
-    if (sub == 0 && live) atomicAdd(&shl, live);
-    // sums over the block's groups in order: at most 16 at a time
-    float total[(W + kThreads - 1) / kThreads] = {};
-    for (int g0 = 0; g0 < GROUPS; g0 += 16) {
-        __syncthreads();
-        if (group >= g0 && group < g0 + 16) {
+    // over the wave's groups (lanes of the same sub), then over the waves
 #pragma unroll
-            for (int j = 0; j < NV; ++j)
+    for (int j = 0; j < NV; ++j)
 #pragma unroll
-                for (int k = 0; k < VE; ++k) shp[group - g0][(sub + j * G) * VE + k] = sum[j][k];
+        for (int k = 0; k < VE; ++k) {
+            float s = sum[j][k];
+            for (int d = G; d < 64; d *= 2) s += __shfl_xor(s, d, 64);
+            if ((threadIdx.x & 63) < G) shp[wave][(sub + j * G) * VE + k] = s;
         }
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < (W + kThreads - 1) / kThreads; ++i) {
-            const int e = threadIdx.x + i * kThreads;
-            if (e < W)
-                for (int g = 0; g < (GROUPS < 16 ? GROUPS : 16); ++g) total[i] += shp[g][e];
-        }
-    }
-    shz[threadIdx.x] = sub == 0 ? z : 0.0;
-    for (int d = kThreads / 2; d > 0; d >>= 1) {
-        __syncthreads();
-        if ((int)threadIdx.x < d) shz[threadIdx.x] += shz[threadIdx.x + d];
-    }
+    const double zs = block_sum(z, sh);
+    const int n = (int)block_sum((double)live, sh);
     const int64_t b = blockIdx.x;
+    double bal = 0.0;
+    for (int e = threadIdx.x; e < p.experts; e += kThreads) {
+        float s = shp[0][e];
 #pragma unroll
-    for (int i = 0; i < (W + kThreads - 1) / kThreads; ++i) {
-        const int e = threadIdx.x + i * kThreads;
-        if (e < p.experts) {
-            p.sum_p[b * p.experts + e] = total[i];
-            p.count[b * p.experts + e] = shc[e];
+        for (int w = 1; w < WAVES; ++w) s += shp[w][e];
+        if (p.blocks == 1) {
+            results(p, e, s, shc[e], zs, n, bal);
+        } else {
+            p.part[b * p.experts + e] = make_int2(__builtin_bit_cast(int, s), shc[e]);
         }
     }
-    if (threadIdx.x == 0) {
-        p.sum_z[b] = shz[0];
-        p.live[b] = shl;
+    if (p.blocks == 1) {
+        bal = block_sum(bal, sh);
+        if (threadIdx.x == 0) *p.balance = (float)(p.experts * bal);
+    } else if (threadIdx.x == 0) {
+        p.sum_z[b] = zs;
+        p.live[b] = n;
+        if (b == 0) *p.arrived = 0;
     }
 }
-
-__global__ __launch_bounds__(kThreads) void fwd_finish(Args p) { finish(p); }
 
 template <typename T, int G, int NV>
 __global__ __launch_bounds__(kThreads) void bwd_tokens(Args p) {
@@ -246,12 +271,16 @@ __global__ __launch_bounds__(kThreads) void bwd_tokens(Args p) {
                 for (int k = 0; k < VE; ++k) v[j][k] *= gb * (c[j][k] - dot) + gz * lse;
         }
 #pragma unroll
-        for (int j = 0; j < NV; ++j)
+        for (int j = 0; j < NV; ++j) {
+            const int e = (sub + j * G) * VE;
+            if (p.whole) {
+                if (e < p.experts) Elem<T>::put_vec(dx + e, v[j]);
+            } else {
 #pragma unroll
-            for (int k = 0; k < VE; ++k) {
-                const int e = (sub + j * G) * VE + k;
-                if (e < p.experts) Elem<T>::put(dx + e, v[j][k]);
+                for (int k = 0; k < VE; ++k)
+                    if (e + k < p.experts) Elem<T>::put(dx + e + k, v[j][k]);
             }
+        }
     }
 }
 
@@ -260,54 +289,61 @@ __global__ __launch_bounds__(kThreads) void bwd_tokens(Args p) {
 // ---------------------------------------------------------------------------
 int elem_size(int dtype) { return dtype == 0 ? 4 : 2; }
 
-// Lanes a token: the smallest power of two whose vectors cover the experts.
-int lanes(int experts, int dtype) {
-    const int vecs = (experts * elem_size(dtype) + 15) / 16;
-    int g = 1;
-    while (g < vecs && g < 64) g *= 2;
-    return g;
+// Lanes a token and vectors a lane: as few lanes as hold the experts in four
+// vectors each, and one vector while up to four lanes do.  A wave then works on
+// up to 16 tokens, and reads 4 KB at a time.
+int vectors(int experts, int dtype) { return (experts * elem_size(dtype) + 15) / 16; }
+void shape(int experts, int dtype, int& g, int& nv) {
+    const int vecs = vectors(experts, dtype);
+    nv = vecs <= 4 ? 1 : vecs <= 16 ? 2 : 4;
+    g = 1;
+    while (g * nv < vecs) g *= 2;
 }
 
+// Elements one block takes by itself, results and all, rather than a second
+// launch: about 2 us of work.
+constexpr int64_t kAlone = 16384;
+
 int block_count(int64_t tokens, int experts, int dtype) {
-    const int groups = kThreads / lanes(experts, dtype);
+    int g, nv;
+    shape(experts, dtype, g, nv);
+    const int groups = kThreads / g;
+    if (tokens * experts <= kAlone) return 1;
     const int64_t want = (tokens + groups - 1) / groups;
     return (int)(want < 256 ? (want < 1 ? 1 : want) : 256);
 }
 
 struct Ws {
-    int64_t sum_p, count, sum_z, live, bytes;
+    int64_t sum_z, shares, part, live, arrived, bytes;
 };
 Ws ws_layout(int64_t tokens, int experts, int dtype) {
     const int64_t blocks = block_count(tokens, experts, dtype);
     Ws w{};
     w.sum_z = 0;
-    w.live = blocks * 8;
-    w.sum_p = w.live + blocks * 4;
-    w.count = w.sum_p + blocks * experts * 4;
-    w.bytes = w.count + blocks * experts * 4;
+    w.shares = blocks * 8;
+    w.part = w.shares + (experts + kFinishExperts - 1) / kFinishExperts * 8;
+    w.live = w.part + blocks * experts * 8;
+    w.arrived = w.live + blocks * 4;
+    w.bytes = w.arrived + 4;
     return w;
 }
 
 // Calls f(T{}, lanes, vectors) with the last two as integral constants.
 template <typename T, typename F>
 void by_lanes(int experts, int dtype, F f) {
-    const int g = lanes(experts, dtype);
-    const int vecs = (experts * elem_size(dtype) + 15) / 16;
-#define FL_CASE(G) \
-    case G: f(T{}, std::integral_constant<int, G>{}, std::integral_constant<int, 1>{}); break
-    switch (g) {
-        FL_CASE(1);
-        FL_CASE(2);
-        FL_CASE(4);
-        FL_CASE(8);
-        FL_CASE(16);
-        FL_CASE(32);
-        default:
-            if (vecs <= 64) f(T{}, std::integral_constant<int, 64>{}, std::integral_constant<int, 1>{});
-            else if (vecs <= 128 || sizeof(T) == 2)  // 1024 halves are 128 vectors
-                f(T{}, std::integral_constant<int, 64>{}, std::integral_constant<int, 2>{});
-            else f(T{}, std::integral_constant<int, 64>{}, std::integral_constant<int, sizeof(T) == 2 ? 2 : 4>{});
-    }
+    int g, nv;
+    shape(experts, dtype, g, nv);
+#define FL_CASE(G, NV) \
+    if (g == G && nv == NV) return f(T{}, std::integral_constant<int, G>{}, std::integral_constant<int, NV>{})
+    FL_CASE(1, 1);
+    FL_CASE(2, 1);
+    FL_CASE(4, 1);
+    FL_CASE(4, 2);
+    FL_CASE(8, 2);
+    FL_CASE(8, 4);
+    FL_CASE(16, 4);
+    FL_CASE(32, 4);
+    if constexpr (sizeof(T) == 4) FL_CASE(64, 4);  // 1024 halves are 128 vectors
 #undef FL_CASE
 }
 template <typename F>
@@ -364,8 +400,9 @@ extern "C" int fl_router_balance_fwd(const void* logits, int64_t row_stride, int
     a.top = (int)top;
     a.mask = mask;
     a.lse = lse;
-    a.sum_p = reinterpret_cast<float*>(ws + w.sum_p);
-    a.count = reinterpret_cast<int*>(ws + w.count);
+    a.part = reinterpret_cast<int2*>(ws + w.part);
+    a.shares = reinterpret_cast<double*>(ws + w.shares);
+    a.arrived = reinterpret_cast<int*>(ws + w.arrived);
     a.sum_z = reinterpret_cast<double*>(ws + w.sum_z);
     a.live = reinterpret_cast<int*>(ws + w.live);
     a.blocks = block_count(tokens, (int)experts, dtype);
@@ -377,7 +414,7 @@ extern "C" int fl_router_balance_fwd(const void* logits, int64_t row_stride, int
     by_type((int)experts, dtype, [&](auto t, auto g, auto nv) {
         fwd_tokens<decltype(t), decltype(g)::value, decltype(nv)::value><<<dim3((unsigned)a.blocks), kThreads, 0, s>>>(a);
     });
-    fwd_finish<<<1, kThreads, 0, s>>>(a);
+    if (a.blocks > 1) fwd_finish<<<dim3((unsigned)((experts + kFinishExperts - 1) / kFinishExperts)), kFinish, 0, s>>>(a);
     return launch_status(name);
 }
 
@@ -400,9 +437,12 @@ extern "C" int fl_router_balance_bwd(const float* grad_balance, const float* gra
     a.gb = grad_balance;
     a.gz = grad_z;
     a.dx = grad_logits;
-    const int groups = kThreads / lanes((int)experts, dtype);
+    a.whole = experts * elem_size(dtype) % 16 == 0 && (reinterpret_cast<uintptr_t>(grad_logits) & 15) == 0;
+    int g, nv;
+    shape((int)experts, dtype, g, nv);
+    const int groups = kThreads / g;
     const int64_t want = (tokens + groups - 1) / groups;
-    a.blocks = (int)(want < 4096 ? want : 4096);
+    a.blocks = (int)(want < 2048 ? want : 2048);
     hipStream_t s = static_cast<hipStream_t>(stream);
     by_type((int)experts, dtype, [&](auto t, auto g, auto nv) {
         bwd_tokens<decltype(t), decltype(g)::value, decltype(nv)::value><<<dim3((unsigned)a.blocks), kThreads, 0, s>>>(a);

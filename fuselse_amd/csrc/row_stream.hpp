@@ -7,7 +7,13 @@
 namespace fl {
 
 // One 16-byte vector of row elements at any element alignment (gfx950 takes
-// unaligned global accesses; one load instruction either way).
+// unaligned global accesses; one load instruction either way), as it lies and
+// streamed with the nontemporal hint, or widened.
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+template <typename T>
+__device__ __forceinline__ u32x4 load_raw_stream(const T* p) {
+    return __builtin_nontemporal_load(reinterpret_cast<const u32x4_any*>(p));
+}
 template <typename T>
 __device__ __forceinline__ void load_vec_any(const T* p, float (&o)[Elem<T>::kVec]) {
     u32x4 r;

@@ -904,22 +904,57 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     loss[n] = lse[n] - x[n] . weight[target[n]] + z_loss * lse[n]^2; rows whose
     target is ignore_index have loss 0 and are not read."""
     _check_linear(x, weight, target)
-    red = _reduction(reduction)
+    return _linear_fwd(x, weight, target, ignore_index, _reduction(reduction), z_loss)
+
+
+def _linear_workspace(N, V, D, dt, backward, w_ptr, ldw, device):
+    key = (N, V, D, dt, backward, w_ptr & 15, ldw)
+    nbytes = _ws_cache.get(key)
+    if nbytes is None:
+        if len(_ws_cache) >= 4096:
+            _ws_cache.clear()
+        nbytes = _ws_cache[key] = _lib.load().fl_linear_ce_workspace_bytes(N, V, D, dt, backward, w_ptr, ldw)
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+
+# The calls themselves, on tensors that were checked (the autograd layers' were,
+# in the forward: the host side is most of a small call's time).
+def _linear_fwd(x, weight, target, ignore_index, red, z_loss):
     N, D = x.shape
     V = weight.shape[0]
-    lse = torch.empty((N + 2,), dtype=torch.float32, device=x.device)
-    loss = torch.empty((N,) if red == 0 else (), dtype=torch.float32, device=x.device)
+    dev = x.device
+    lse = torch.empty((N + 2,), dtype=torch.float32, device=dev)
+    loss = torch.empty((N,) if red == 0 else (), dtype=torch.float32, device=dev)
     if N == 0:
         return loss.zero_(), lse
     dt = _DTYPE_CODE[x.dtype]
+    w_ptr, ldw = weight.data_ptr(), _row_stride(weight)
     with _on_device(x):
-        nbytes = _lib.load().fl_linear_ce_workspace_bytes(N, V, D, dt, 0, weight.data_ptr(),
-                                                         _row_stride(weight))
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-        _lib.call("fl_linear_ce_fwd", x.data_ptr(), _row_stride(x), weight.data_ptr(), _row_stride(weight),
-                  target.data_ptr(), N, V, D, dt, ignore_index, z_loss, red, loss.data_ptr(), lse.data_ptr(),
-                  ws.data_ptr(), nbytes, _stream(x))
+        ws = _linear_workspace(N, V, D, dt, 0, w_ptr, ldw, dev)
+        _lib.call("fl_linear_ce_fwd", x.data_ptr(), _row_stride(x), w_ptr, ldw, target.data_ptr(), N, V, D, dt,
+                  ignore_index, z_loss, red, loss.data_ptr(), lse.data_ptr(), ws.data_ptr(), ws.numel(), _stream(x))
     return loss, lse
+
+
+def _linear_bwd(grad_output, x, weight, target, lse, ignore_index, red, z_loss, need_x, need_weight):
+    N, D = x.shape
+    V = weight.shape[0]
+    dev = x.device
+    dx = torch.empty((N, D), dtype=x.dtype, device=dev) if need_x else None
+    dw = torch.empty((V, D), dtype=x.dtype, device=dev) if need_weight else None
+    if N == 0:
+        return dx, dw.zero_() if need_weight else None
+    if not (need_x or need_weight):
+        return None, None
+    dt = _DTYPE_CODE[x.dtype]
+    w_ptr, ldw = weight.data_ptr(), _row_stride(weight)
+    with _on_device(x):
+        ws = _linear_workspace(N, V, D, dt, 1, w_ptr, ldw, dev)
+        _lib.call("fl_linear_ce_bwd", grad_output.data_ptr(), x.data_ptr(), _row_stride(x), w_ptr, ldw,
+                  target.data_ptr(), lse.data_ptr(), N, V, D, dt, ignore_index, z_loss, red,
+                  dx.data_ptr() if need_x else None, dw.data_ptr() if need_weight else None, ws.data_ptr(),
+                  ws.numel(), _stream(x))
+    return dx, dw
 
 
 def linear_cross_entropy_backward(grad_output: torch.Tensor, x: torch.Tensor, weight: torch.Tensor,
@@ -931,29 +966,13 @@ def linear_cross_entropy_backward(grad_output: torch.Tensor, x: torch.Tensor, we
     otherwise."""
     _check_linear(x, weight, target)
     red = _reduction(reduction)
-    N, D = x.shape
-    V = weight.shape[0]
+    N = x.shape[0]
     for t, nm in ((grad_output, "grad_output"), (lse, "lse")):
         _check(t.is_cuda and t.dtype == torch.float32 and t.is_contiguous(), f"{nm} must be contiguous CUDA float32")
     _check(lse.dim() == 1 and lse.shape[0] == N + 2, "lse must be 1D (N + 2)")
     _check(grad_output.numel() == (N if red == 0 else 1), "grad_output must have the loss's shape")
     _check_device(x, "x", grad_output=grad_output, lse=lse)
-    dx = torch.empty((N, D), dtype=x.dtype, device=x.device) if need_x else None
-    dw = torch.empty((V, D), dtype=x.dtype, device=x.device) if need_weight else None
-    if N == 0:
-        return dx, dw.zero_() if need_weight else None
-    if not (need_x or need_weight):
-        return None, None
-    dt = _DTYPE_CODE[x.dtype]
-    with _on_device(x):
-        nbytes = _lib.load().fl_linear_ce_workspace_bytes(N, V, D, dt, 1, weight.data_ptr(),
-                                                         _row_stride(weight))
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-        _lib.call("fl_linear_ce_bwd", grad_output.data_ptr(), x.data_ptr(), _row_stride(x), weight.data_ptr(),
-                  _row_stride(weight), target.data_ptr(), lse.data_ptr(), N, V, D, dt, ignore_index, z_loss, red,
-                  dx.data_ptr() if need_x else None, dw.data_ptr() if need_weight else None, ws.data_ptr(), nbytes,
-                  _stream(x))
-    return dx, dw
+    return _linear_bwd(grad_output, x, weight, target, lse, ignore_index, red, z_loss, need_x, need_weight)
 
 
 def _distill_rows(logits: torch.Tensor):
@@ -993,7 +1012,10 @@ def topk_distillation(logits: torch.Tensor, teacher: torch.Tensor, index: torch.
     || softmax(logits / temperature)); teacher entries of -inf are unused, a row
     without any other has loss 0 and is left out of the mean."""
     _check_distill(logits, teacher, index)
-    red = _reduction(reduction)
+    return _distill_fwd(logits, teacher, index, temperature, _reduction(reduction))
+
+
+def _distill_fwd(logits, teacher, index, temperature, red):
     rows, slice_rows, s0, s1 = _distill_rows(logits)
     V, K = logits.shape[-1], teacher.shape[-1]
     dev = logits.device
@@ -1003,13 +1025,31 @@ def topk_distillation(logits: torch.Tensor, teacher: torch.Tensor, index: torch.
     if rows == 0:
         return loss.zero_(), lse, tlse, norm
     dt = _DTYPE_CODE[logits.dtype]
+    key = (rows, V, dt)
+    nbytes = _ws_cache.get(key + ("distill",))
+    if nbytes is None:
+        nbytes = _ws_cache[key + ("distill",)] = _lib.load().fl_distill_workspace_bytes(rows, V, dt)
+    at = stats.data_ptr()
     with _on_device(logits):
-        nbytes = _lib.load().fl_distill_workspace_bytes(rows, V, dt)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         _lib.call("fl_distill_fwd", logits.data_ptr(), rows, slice_rows, s0, s1, V, dt, teacher.data_ptr(),
-                  _DTYPE_CODE[teacher.dtype], index.data_ptr(), K, temperature, red, loss.data_ptr(), lse.data_ptr(),
-                  tlse.data_ptr(), norm.data_ptr() if red else None, ws.data_ptr(), nbytes, _stream(logits))
+                  _DTYPE_CODE[teacher.dtype], index.data_ptr(), K, temperature, red, loss.data_ptr(), at,
+                  at + 4 * rows, at + 8 * rows if red else None, ws.data_ptr(), nbytes, _stream(logits))
     return loss, lse, tlse, norm
+
+
+def _distill_bwd(grad_output, logits, teacher, index, lse, teacher_lse, norm, temperature):
+    rows, slice_rows, s0, s1 = _distill_rows(logits)
+    grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    if rows == 0:
+        return grad
+    with _on_device(logits):
+        _lib.call("fl_distill_bwd", grad_output.data_ptr(), 0 if grad_output.numel() == 1 else 1,
+                  norm.data_ptr() if norm is not None else None, logits.data_ptr(), rows, slice_rows, s0, s1,
+                  logits.shape[-1], _DTYPE_CODE[logits.dtype], teacher.data_ptr(), _DTYPE_CODE[teacher.dtype],
+                  index.data_ptr(), teacher.shape[-1], temperature, lse.data_ptr(), teacher_lse.data_ptr(),
+                  grad.data_ptr(), _stream(logits))
+    return grad
 
 
 def topk_distillation_backward(grad_output: torch.Tensor, logits: torch.Tensor, teacher: torch.Tensor,
@@ -1018,8 +1058,7 @@ def topk_distillation_backward(grad_output: torch.Tensor, logits: torch.Tensor, 
     """Gradient of the logits, contiguous and of their type; grad_output fp32
     with one element per row, or one in all."""
     _check_distill(logits, teacher, index)
-    rows, slice_rows, s0, s1 = _distill_rows(logits)
-    V, K = logits.shape[-1], teacher.shape[-1]
+    rows = _distill_rows(logits)[0]
     _check(grad_output.is_cuda and grad_output.dtype == torch.float32 and grad_output.is_contiguous(),
            "grad_output must be contiguous CUDA float32")
     _check(grad_output.numel() in (1, rows), "grad_output must have one element, or one per row")
@@ -1027,18 +1066,10 @@ def topk_distillation_backward(grad_output: torch.Tensor, logits: torch.Tensor, 
         _check(t is None and nm == "norm" or (t.is_cuda and t.dtype == torch.float32 and t.is_contiguous()
                                               and t.numel() == n), f"{nm} must be contiguous CUDA float32 of {n}")
     _check_device(logits, "logits", grad_output=grad_output, lse=lse, teacher_lse=teacher_lse, norm=norm)
-    grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    if rows == 0:
-        return grad
-    with _on_device(logits):
-        _lib.call("fl_distill_bwd", grad_output.data_ptr(), 0 if grad_output.numel() == 1 else 1,
-                  norm.data_ptr() if norm is not None else None, logits.data_ptr(), rows, slice_rows, s0, s1, V,
-                  _DTYPE_CODE[logits.dtype], teacher.data_ptr(), _DTYPE_CODE[teacher.dtype], index.data_ptr(), K,
-                  temperature, lse.data_ptr(), teacher_lse.data_ptr(), grad.data_ptr(), _stream(logits))
-    return grad
+    return _distill_bwd(grad_output, logits, teacher, index, lse, teacher_lse, norm, temperature)
 
 
-def _check_router(logits, mask):
+def _check_router(logits, index, mask):
     _check(logits.is_cuda, "logits must be CUDA")
     _check(logits.dtype in _DTYPE_CODE, "logits must be float32, float16 or bfloat16")
     _check(logits.dim() == 2 and logits.shape[1] >= 1, "logits must be 2D (tokens, experts)")
@@ -1048,7 +1079,10 @@ def _check_router(logits, mask):
     if mask is not None:
         _check(mask.is_cuda and mask.dtype == torch.bool and mask.is_contiguous() and mask.dim() == 1
                and mask.shape[0] == logits.shape[0], "mask must be a contiguous CUDA bool tensor (tokens,)")
-        _check_device(logits, "logits", mask=mask)
+    if index is not None:
+        _check(index.is_cuda and index.dtype == torch.int64 and index.is_contiguous() and index.dim() == 2
+               and index.shape[0] == logits.shape[0], "index must be a contiguous CUDA int64 tensor (tokens, top)")
+    _check_device(logits, "logits", mask=mask, index=index)
 
 
 def router_balance(logits: torch.Tensor, index: torch.Tensor, mask: Optional[torch.Tensor] = None):
@@ -1057,37 +1091,33 @@ def router_balance(logits: torch.Tensor, index: torch.Tensor, mask: Optional[tor
     (tokens, experts) fp32, fp16 or bf16 with contiguous rows, index int64
     (tokens, top) the chosen experts, mask bool (tokens,) the tokens that take
     part (None: all)."""
-    _check_router(logits, mask)
+    _check_router(logits, index, mask)
+    return _router_fwd(logits, index, mask)
+
+
+def _router_fwd(logits, index, mask):
     T, E = logits.shape
-    _check(index.is_cuda and index.dtype == torch.int64 and index.is_contiguous() and index.dim() == 2
-           and index.shape[0] == T, "index must be a contiguous CUDA int64 tensor (tokens, top)")
-    _check_device(logits, "logits", index=index)
     dev = logits.device
     balance = torch.empty((), dtype=torch.float32, device=dev)
     z = torch.empty((), dtype=torch.float32, device=dev)
     counts = torch.empty((E,), dtype=torch.int64, device=dev)
     stats = torch.empty((T + E + 1,), dtype=torch.float32, device=dev)
-    lse, coef = stats[:T], stats[T:]
     dt = _DTYPE_CODE[logits.dtype]
+    key = ("router", T, E, dt)
+    nbytes = _ws_cache.get(key)
+    if nbytes is None:
+        nbytes = _ws_cache[key] = _lib.load().fl_router_workspace_bytes(T, E, dt)
+    at = stats.data_ptr()
     with _on_device(logits):
-        nbytes = _lib.load().fl_router_workspace_bytes(T, E, dt)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         _lib.call("fl_router_balance_fwd", logits.data_ptr(), _row_stride(logits), T, E, dt, index.data_ptr(),
                   index.shape[1], mask.data_ptr() if mask is not None else None, balance.data_ptr(), z.data_ptr(),
-                  counts.data_ptr(), lse.data_ptr(), coef.data_ptr(), ws.data_ptr(), nbytes, _stream(logits))
-    return balance, z, counts, lse, coef
+                  counts.data_ptr(), at, at + 4 * T, ws.data_ptr(), nbytes, _stream(logits))
+    return balance, z, counts, stats[:T], stats[T:]
 
 
-def router_balance_backward(grad_balance, grad_z, logits: torch.Tensor, mask, lse: torch.Tensor,
-                            coef: torch.Tensor) -> torch.Tensor:
-    """Gradient of the router's logits, contiguous and of their type;
-    grad_balance and grad_z fp32 scalars or None."""
-    _check_router(logits, mask)
+def _router_bwd(grad_balance, grad_z, logits, mask, lse, coef):
     T, E = logits.shape
-    for t, nm, n in ((grad_balance, "grad_balance", 1), (grad_z, "grad_z", 1), (lse, "lse", T), (coef, "coef", E + 1)):
-        _check(t is None and nm in ("grad_balance", "grad_z") or (t.is_cuda and t.dtype == torch.float32
-               and t.is_contiguous() and t.numel() == n), f"{nm} must be contiguous CUDA float32 of {n}")
-    _check_device(logits, "logits", grad_balance=grad_balance, grad_z=grad_z, lse=lse, coef=coef)
     grad = torch.empty((T, E), dtype=logits.dtype, device=logits.device)
     if T == 0:
         return grad
@@ -1097,3 +1127,16 @@ def router_balance_backward(grad_balance, grad_z, logits: torch.Tensor, mask, ls
                   _DTYPE_CODE[logits.dtype], mask.data_ptr() if mask is not None else None, lse.data_ptr(),
                   coef.data_ptr(), grad.data_ptr(), _stream(logits))
     return grad
+
+
+def router_balance_backward(grad_balance, grad_z, logits: torch.Tensor, mask, lse: torch.Tensor,
+                            coef: torch.Tensor) -> torch.Tensor:
+    """Gradient of the router's logits, contiguous and of their type;
+    grad_balance and grad_z fp32 scalars or None."""
+    _check_router(logits, None, mask)
+    T, E = logits.shape
+    for t, nm, n in ((grad_balance, "grad_balance", 1), (grad_z, "grad_z", 1), (lse, "lse", T), (coef, "coef", E + 1)):
+        _check(t is None and nm in ("grad_balance", "grad_z") or (t.is_cuda and t.dtype == torch.float32
+               and t.is_contiguous() and t.numel() == n), f"{nm} must be contiguous CUDA float32 of {n}")
+    _check_device(logits, "logits", grad_balance=grad_balance, grad_z=grad_z, lse=lse, coef=coef)
+    return _router_bwd(grad_balance, grad_z, logits, mask, lse, coef)

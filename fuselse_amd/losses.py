@@ -39,7 +39,7 @@ def _integers(t: torch.Tensor, name: str) -> torch.Tensor:
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, target, ignore_index, reduction, z_loss):
-        loss, lse = ext.linear_cross_entropy(x, weight, target, ignore_index, reduction, z_loss)
+        loss, lse = ext._linear_fwd(x, weight, target, ignore_index, reduction, z_loss)
         ctx.save_for_backward(x, weight, target, lse)
         ctx.args = (ignore_index, reduction, z_loss)
         return loss
@@ -48,9 +48,9 @@ class _LinearCrossEntropy(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, grad):
         x, weight, target, lse = ctx.saved_tensors
-        dx, dw = ext.linear_cross_entropy_backward(grad.contiguous(), _rows(x), _rows(weight), target, lse, *ctx.args,
-                                                   need_x=ctx.needs_input_grad[0],
-                                                   need_weight=ctx.needs_input_grad[1])
+        need = ctx.needs_input_grad
+        # in rows again, which a saved-tensor hook may have changed
+        dx, dw = ext._linear_bwd(grad.contiguous(), _rows(x), _rows(weight), target, lse, *ctx.args, need[0], need[1])
         return dx, dw, None, None, None, None
 
 
@@ -74,17 +74,19 @@ def linear_cross_entropy(input: torch.Tensor, weight: torch.Tensor, target: torc
                "target must have input's shape without its last dimension")
     x, w = _rows(input), _rows(weight) if weight.dim() == 2 else weight
     t = _integers(target, "target").reshape(-1).contiguous()
+    ext._check_linear(x, w, t)
+    red = ext._reduction(reduction)
     if torch.is_grad_enabled() and (input.requires_grad or weight.requires_grad):
-        loss = _LinearCrossEntropy.apply(x, w, t, ignore_index, reduction, z_loss)
+        loss = _LinearCrossEntropy.apply(x, w, t, ignore_index, red, z_loss)
     else:
-        loss, _ = ext.linear_cross_entropy(x, w, t, ignore_index, reduction, z_loss)
+        loss, _ = ext._linear_fwd(x, w, t, ignore_index, red, z_loss)
     return loss.reshape(target.shape) if reduction == "none" and target.dim() != 1 else loss
 
 
 class _TopkDistillation(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, teacher, index, temperature, reduction):
-        loss, lse, tlse, norm = ext.topk_distillation(logits, teacher, index, temperature, reduction)
+        loss, lse, tlse, norm = ext._distill_fwd(logits, teacher, index, temperature, reduction)
         ctx.save_for_backward(logits, teacher, index, lse, tlse, norm)
         ctx.temperature = temperature
         return loss
@@ -95,8 +97,7 @@ class _TopkDistillation(torch.autograd.Function):
         logits, teacher, index, lse, tlse, norm = ctx.saved_tensors
         if logits.stride(-1) != 1 and logits.shape[-1] != 1:  # as a saved-tensor hook may give it back
             logits = logits.contiguous()
-        g = ext.topk_distillation_backward(grad.contiguous(), logits, teacher, index, lse, tlse, norm,
-                                           ctx.temperature)
+        g = ext._distill_bwd(grad.contiguous(), logits, teacher, index, lse, tlse, norm, ctx.temperature)
         return g, None, None, None, None
 
 
@@ -128,10 +129,12 @@ def topk_distillation(logits: torch.Tensor, teacher_logits: torch.Tensor, teache
     if x.stride(-1) != 1 and x.shape[-1] != 1:
         x = x.contiguous()
     t, i = t.contiguous(), i.contiguous()
+    ext._check_distill(x, t, i)
+    red = ext._reduction(reduction)
     if torch.is_grad_enabled() and logits.requires_grad:
-        loss = _TopkDistillation.apply(x, t, i, temperature, reduction)
+        loss = _TopkDistillation.apply(x, t, i, temperature, red)
     else:
-        loss = ext.topk_distillation(x, t, i, temperature, reduction)[0]
+        loss = ext._distill_fwd(x, t, i, temperature, red)[0]
     return loss.reshape(lead) if reduction == "none" else loss
 
 
@@ -146,7 +149,7 @@ class RouterBalance(NamedTuple):
 class _RouterBalance(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, index, mask):
-        balance, z, counts, lse, coef = ext.router_balance(logits, index, mask)
+        balance, z, counts, lse, coef = ext._router_fwd(logits, index, mask)
         ctx.save_for_backward(logits, mask, lse, coef)
         ctx.mark_non_differentiable(counts)
         ctx.set_materialize_grads(False)
@@ -158,7 +161,7 @@ class _RouterBalance(torch.autograd.Function):
         if grad_balance is None and grad_z is None:
             return None, None, None
         logits, mask, lse, coef = ctx.saved_tensors
-        return ext.router_balance_backward(grad_balance, grad_z, _rows(logits), mask, lse, coef), None, None
+        return ext._router_bwd(grad_balance, grad_z, _rows(logits), mask, lse, coef), None, None
 
 
 def router_balance(logits: torch.Tensor, index: torch.Tensor, mask: Optional[torch.Tensor] = None) -> RouterBalance:
@@ -182,6 +185,7 @@ def router_balance(logits: torch.Tensor, index: torch.Tensor, mask: Optional[tor
     i = _integers(index, "index")
     i = i.reshape(x.shape[0], i.shape[-1]).contiguous() if i.dim() != 2 else i.contiguous()
     m = mask.reshape(-1).contiguous() if mask is not None else None
+    ext._check_router(x, i, m)
     if torch.is_grad_enabled() and logits.requires_grad:
         return RouterBalance(*_RouterBalance.apply(x, i, m))
-    return RouterBalance(*ext.router_balance(x, i, m)[:3])
+    return RouterBalance(*ext._router_fwd(x, i, m)[:3])

@@ -108,7 +108,7 @@ struct PlanArgs {
     int* tgt;     // live row -> target, -1 for one outside [0, v)
     // forward: ignored rows' results
     float* loss_rows;
-    float* lse_out;
+    float* lse_out;    // NULL: no backward follows
     // backward
     const float* grad;
     int grad_stride;
@@ -122,9 +122,9 @@ struct PlanArgs {
     int most_splits;
     int64_t room;              // rows of sums there is room for
     float sum_cost;            // what a split's sums of a row cost at the end, in steps
-    int* list;                 // fp16, bf16: rows by their target's group of 64, in order
+    int* list;                 // fp16, bf16: live rows by their target's group of 64, in order
     int* list_at;              // [groups + 1]: where a group's rows begin
-    int* rest_row;             // [groups * 64]: set to -1
+    int* rest_row;             // [groups * 64]: a target's place among the targets' rows, else -1
     int groups;                // 0: no lists
 };
 
@@ -159,7 +159,6 @@ struct MagArgs {
     int64_t ldw, d;
     float* mag;             // [x_blocks + w_blocks]
     int x_blocks, w_blocks;
-    const float* given;     // backward: the forward's, below 0 where it had none
 };
 
 __device__ __forceinline__ float wave_max(float v) {
@@ -182,7 +181,6 @@ __device__ __forceinline__ float block_max(float v, float* sh) {
 }
 
 __device__ __forceinline__ void magnitudes(const PlanArgs& p, const MagArgs& m, int block) {
-    if (m.given && m.given[0] >= 0.0f) return;
     const bool is_x = block < m.x_blocks;
     const int64_t n = is_x ? p.n : p.v;
     const int64_t b = is_x ? block : block - m.x_blocks, blocks = is_x ? m.x_blocks : m.w_blocks;
@@ -218,32 +216,58 @@ __device__ __forceinline__ void magnitudes(const PlanArgs& p, const MagArgs& m, 
     if (threadIdx.x == 0) m.mag[block] = big;
 }
 
-// Rows by their targets' groups of 64 vocabulary entries: a wave a group.
-constexpr int kGroup = 64;
+// Live rows by their targets' groups of 64 vocabulary entries, a wave a group: an
+// entry is the live row and, from bit 24, the target's place in its group.
+constexpr int kGroup = 64, kSlotShift = 24;
 __device__ __forceinline__ void target_lists(const PlanArgs& p, int block) {
     const int group = block * (kPlanThreads / 64) + (int)(threadIdx.x >> 6), lane = lane_id();
     if (group >= p.groups) return;
     const int64_t lo = (int64_t)group * kGroup, hi = lo + kGroup < p.v ? lo + kGroup : p.v;
-    p.rest_row[lo + lane] = -1;
+    constexpr int U = 8;
+    auto targets = [&](int64_t r0, int64_t (&t)[U]) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) t[u] = r0 + u * 64 + lane < p.n ? p.target[r0 + u * 64 + lane] : p.ignore;
+    };
     int before = 0, mine = 0;
-    for (int64_t r0 = 0; r0 < p.n; r0 += 64) {
-        const int64_t t = r0 + lane < p.n ? p.target[r0 + lane] : -1;
-        const bool in = t >= 0 && t != p.ignore;
-        before += __popcll(__ballot(in && t < lo));
-        mine += __popcll(__ballot(in && t >= lo && t < hi));
+    for (int64_t r0 = 0; r0 < p.n; r0 += 64 * U) {
+        int64_t t[U];
+        targets(r0, t);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const bool in = t[u] != p.ignore && t[u] >= 0;
+            before += __popcll(__ballot(in && t[u] < lo));
+            mine += __popcll(__ballot(in && t[u] >= lo && t[u] < hi));
+        }
     }
     if (lane == 0) {
         p.list_at[group] = before;
         if (group == p.groups - 1) p.list_at[p.groups] = before + mine;
     }
-    for (int64_t r0 = 0; mine > 0 && r0 < p.n; r0 += 64) {
-        const int64_t t = r0 + lane < p.n ? p.target[r0 + lane] : -1;
-        const bool in = t >= lo && t < hi && t != p.ignore;
-        const uint64_t b = __ballot(in);
-        if (in) p.list[before + __popcll(b & ((1ull << lane) - 1))] = (int)(r0 + lane);
-        before += __popcll(b);
-        mine -= __popcll(b);
+    const int begin = before;
+    int live = 0;
+    bool comes = false;  // this lane's entry of the group is a target
+    for (int64_t r0 = 0; mine > 0 && r0 < p.n; r0 += 64 * U) {
+        int64_t t[U];
+        targets(r0, t);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const uint64_t below = (1ull << lane) - 1;
+            const uint64_t any = __ballot(t[u] != p.ignore);
+            const bool in = t[u] != p.ignore && t[u] >= lo && t[u] < hi;
+            uint64_t b = __ballot(in);
+            for (uint64_t left = b; left; left &= left - 1) {
+                const int l = __builtin_ctzll(left);
+                comes |= lane == __builtin_amdgcn_readlane((int)(t[u] - lo), l);
+            }
+            if (in)
+                p.list[before + __popcll(b & below)] = (live + __popcll(any & below)) | (int)(t[u] - lo) << kSlotShift;
+            before += __popcll(b);
+            mine -= __popcll(b);
+            live += __popcll(any);
+        }
     }
+    const uint64_t there = __ballot(comes);
+    p.rest_row[lo + lane] = comes ? begin + __popcll(there & ((1ull << lane) - 1)) : -1;
 }
 
 // Block 0 makes the plan; blocks after it take the magnitudes or the lists.
@@ -270,7 +294,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs p, MagArgs 
             p.pos[r] = -1;
             if constexpr (!BWD) {
                 p.loss_rows[r] = 0.0f;
-                p.lse_out[r] = 0.0f;
+                if (p.lse_out) p.lse_out[r] = 0.0f;
             }
             continue;
         }
@@ -306,10 +330,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs p, MagArgs 
             p.b[at + k] *= scale;
         }
     }
-    if (threadIdx.x == 0) {
-        p.head->live = live;
-        if constexpr (!BWD) p.lse_out[p.n] = p.lse_out[p.n + 1] = -1.0f;  // no magnitudes; packing sets them
-    }
+    if (threadIdx.x == 0) p.head->live = live;
 }
 
 // The scale of fp32 logits' operands, and what undoes both in a logit; big holds
@@ -347,8 +368,7 @@ struct PackArgs {
     const Head* head;
     int64_t d, ldp;
     float* big;        // fp32: magnitudes of x and w
-    const float* mag;  // first piece: where they come from, unless they are given
-    const float* given;
+    const float* mag;  // forward, first piece: where they come from
     int x_blocks, w_blocks;
 };
 
@@ -373,16 +393,11 @@ __global__ __launch_bounds__(256) void pack(PackArgs p) {
     float big_x = 0.0f, big_w = 0.0f;
     if constexpr (DT == kF32) {
         if (p.mag) {
-            if (p.given && p.given[0] >= 0.0f) {
-                big_x = p.given[0];
-                big_w = p.given[1];
-            } else {
-                __shared__ float sh[2][4];
-                for (int k = threadIdx.x; k < p.x_blocks; k += 256) big_x = fmaxf(big_x, p.mag[k]);
-                for (int k = threadIdx.x; k < p.w_blocks; k += 256) big_w = fmaxf(big_w, p.mag[p.x_blocks + k]);
-                big_x = block_max<256>(big_x, sh[0]);
-                big_w = block_max<256>(big_w, sh[1]);
-            }
+            __shared__ float sh[2][4];
+            for (int k = threadIdx.x; k < p.x_blocks; k += 256) big_x = fmaxf(big_x, p.mag[k]);
+            for (int k = threadIdx.x; k < p.w_blocks; k += 256) big_w = fmaxf(big_w, p.mag[p.x_blocks + k]);
+            big_x = block_max<256>(big_x, sh[0]);
+            big_w = block_max<256>(big_w, sh[1]);
             if (blockIdx.x == 0 && threadIdx.x == 0) {
                 p.big[0] = big_x;
                 p.big[1] = big_w;
@@ -745,7 +760,7 @@ __global__ __launch_bounds__(256) void finish_rows(const Head* head, const int* 
     if (lane == 0) {
         const float lse = lse_finish<true>(m, s);
         const int row = rows[r];
-        lse_out[row] = lse;
+        if (lse_out) lse_out[row] = lse;
         loss_rows[row] = tgt[r] >= 0 ? lse - at_target[r] + z * lse * lse : __builtin_nanf("");
     }
 }
@@ -874,20 +889,23 @@ struct ProductArgs {
     int steps;          // of K; dw: the live rows'
     int m, n;           // results
     int tiles_m;
-    float* acc;         // dx: [split][live row][ldc] fp32 sums, added to when `add`
+    float* acc;         // [split][live row, or row of the piece][ldc] fp32 sums
     int64_t ldc;
-    int add;
+    int add;            // dx: the sums are added to
+    int splits;         // dw's
     void* out;          // dw: [n][ldc] results
-    // dw in fp16, bf16: fp32 rows that are added to the results, and which one
-    // (-1: none) to result row n
-    const float* rests;
+    // dw in fp16, bf16: result row n is also wanted in fp32, at this place (-1: not)
+    float* rests;
     const int* rest_row;
 };
 
-// dx (DX): C[n][d] = sum_v G[n][v] w[v][d] over a piece, added to the splits'
-// sums.  dw: C[v][d] = sum_n G[n][v] x[n][d], the piece's rows of the result.
-template <int DT, class S, bool DX>
+// kDx: C[n][d] = sum_v G[n][v] w[v][d] over a piece, added to the splits' sums.
+// kDw: C[v][d] = sum_n G[n][v] x[n][d], the piece's rows of the result; in
+// kDwSplit the splits' sums of them.
+enum Mode { kDx, kDw, kDwSplit };
+template <int DT, class S, int MODE>
 struct ProductJob {
+    static constexpr bool DX = MODE == kDx, SUMS = MODE != kDw;
     ProductArgs p;
     int n_end, tiles_n, tiles, splits;
     float inv;
@@ -896,18 +914,18 @@ struct ProductJob {
     typedef typename Io<DT>::T T;
     typedef Side<S, S::TM, false> SA;
     typedef Side<S, S::TN, DX> SB;
-    static constexpr bool kRests = !DX && DT != kF32;
+    static constexpr bool kRests = MODE == kDw && DT != kF32;
     struct Rows {
         int rest[kRests ? S::FN : 1];
     };
-    __device__ __forceinline__ int split(int t) const { return DX ? scalar((unsigned)t / (unsigned)tiles) : 0; }
+    __device__ __forceinline__ int split(int t) const { return SUMS ? scalar((unsigned)t / (unsigned)tiles) : 0; }
     __device__ __forceinline__ TileAt at(int t) const { return tile_at(t - split(t) * tiles, p.tiles_m, tiles_n); }
     // K's steps are cut evenly
     __device__ __forceinline__ int first(int t) const {
-        return DX ? scalar((unsigned)(p.steps * split(t)) / (unsigned)splits) : 0;
+        return SUMS ? scalar((unsigned)(p.steps * split(t)) / (unsigned)splits) : 0;
     }
     __device__ __forceinline__ int steps(int t) const {
-        return DX ? scalar((unsigned)(p.steps * (split(t) + 1)) / (unsigned)splits) - first(t) : p.steps;
+        return SUMS ? scalar((unsigned)(p.steps * (split(t) + 1)) / (unsigned)splits) - first(t) : p.steps;
     }
     __device__ __forceinline__ void place(int t, SA& A, SB& B) const {
         const TileAt tile = at(t);
@@ -926,7 +944,7 @@ struct ProductJob {
     __device__ __forceinline__ void finish(int t, const Rows& r, const f32x4 (&acc)[S::FM][S::FN]) const {
         const TileAt tile = at(t);
         const Place<S> at(tile.m * S::TM, tile.n * S::TN);
-        float* sums = DX ? p.acc + (int64_t)split(t) * n_end * p.ldc : nullptr;
+        float* sums = SUMS ? p.acc + (int64_t)split(t) * n_end * p.ldc : nullptr;
 #pragma unroll
         for (int j = 0; j < S::FN; ++j) {
             const int64_t n = at.n + j * 16;
@@ -936,23 +954,28 @@ struct ProductJob {
                 const int64_t m = at.m + i * 16;
                 if (m >= p.m) continue;
                 f32x4 v = acc[i][j];
-                if constexpr (DX) {
+                if constexpr (SUMS) {
                     float* c = sums + n * p.ldc + m;
                     if (whole) {
-                        if (p.add) v += *reinterpret_cast<const f32x4*>(c);
+                        if (DX && p.add) v += *reinterpret_cast<const f32x4*>(c);
                         *reinterpret_cast<f32x4*>(c) = v;
                     } else {
 #pragma unroll
                         for (int q = 0; q < 4; ++q)
-                            if (m + q < p.m) c[q] = p.add ? c[q] + v[q] : v[q];
+                            if (m + q < p.m) c[q] = DX && p.add ? c[q] + v[q] : v[q];
                     }
                 } else {
                     T* c = static_cast<T*>(p.out) + n * p.ldc + m;
                     if constexpr (kRests) {
                         if (r.rest[j] >= 0) {
-                            const float* more = p.rests + r.rest[j] * p.ldc + m;
+                            float* f = p.rests + r.rest[j] * p.ldc + m;
+                            if (whole) {
+                                *reinterpret_cast<f32x4*>(f) = v;
+                            } else {
 #pragma unroll
-                            for (int q = 0; q < 4; ++q) v[q] += m + q < p.m ? more[q] : 0.0f;
+                                for (int q = 0; q < 4; ++q)
+                                    if (m + q < p.m) f[q] = v[q];
+                            }
                         }
                     }
                     v *= inv;
@@ -977,107 +1000,131 @@ struct ProductJob {
     }
 };
 
-template <int DT, class S, bool DX>
+template <int DT, class S, int MODE>
 __global__ __launch_bounds__(S::kThreads, 2) void product(ProductArgs p) {
     FL_LCE_BUFFERS(S);
+    constexpr bool DX = MODE == kDx;
     const int live = p.head->live;
-    ProductJob<DT, S, DX> job{p};
+    ProductJob<DT, S, MODE> job{p};
     if constexpr (DX) {
         job.p.b.rows = live;
         job.n_end = live;
-        job.splits = p.head->splits < p.steps ? p.head->splits : p.steps;  // a short last piece adds to the first ones
     } else {
         job.p.steps = (live + kStep - 1) / kStep;
         job.p.a.rows = live;
         job.p.b.rows = job.p.steps * kStep;
         job.n_end = p.n;
-        job.splits = 1;
     }
+    // no split without a step: a short last piece of dx adds to the first ones
+    const int splits = DX ? p.head->splits : MODE == kDwSplit ? p.splits : 1;
+    job.splits = splits < job.p.steps ? splits : job.p.steps;
     job.tiles_n = (job.n_end + S::TN - 1) / S::TN;
     job.tiles = p.tiles_m * job.tiles_n;
     job.inv = p.head->inv_scale;
     job.whole = (p.ldc & 3) == 0;
-    if (!DX && live == 0) {  // no step of K: dw is zero
+    if (MODE == kDw && live == 0) {  // no step of K: dw is zero
         f32x4 none[S::FM][S::FN] = {};
         for (Walk w(job.tiles); w.t < w.end; w.t += w.stride) job.finish(w.t, job.rows(w.t), none);
         return;
     }
-    run_tiles<S, false, DX, Grads<DT>::kHalf, Grads<DT>::kParts>(job, job.tiles * job.splits, (lds_char*)buf0,
-                                                                 (lds_char*)buf1);
+    run_tiles<S, false, DX, Grads<DT>::kHalf, Grads<DT>::kParts>(job, job.tiles * (MODE == kDw ? 1 : job.splits),
+                                                                 (lds_char*)buf0, (lds_char*)buf1);
 }
 
-// dw's share of the rests: for each target of a group of 64, the sum over its
-// rows, in order, of rest times x.  A block a group and 64 columns; each of its
-// waves takes a run of the group's rows and keeps a sum in LDS for each of the
-// group's targets, and the waves' sums are added in their order.
+// dw's rows that are targets: the product's fp32 sums and, for each of the
+// target's rows in order, rest times x.  A wave a group of 64 entries, 256 columns
+// and every `parts`-th of the group's targets.
 struct RestArgs {
+    const Head* head;
     const float* rest;
-    const int *list, *list_at, *pos, *tgt;
+    const int *list, *list_at, *rest_row;
     const uint16_t* x;   // packed live rows
     int64_t ldx;
-    int d, group0;
-    float* rests;        // [place in the list][d]
-    int* rest_row;       // [vocabulary entry]
+    int d, group0, cols, parts;  // cols: blocks of 256 columns
+    const float* rests;  // [place][d]
+    void* dw;            // [vocabulary entry][d]
 };
-template <int DT, int WAVES>
-__global__ __launch_bounds__(WAVES * 64) void sum_rests(RestArgs p) {
-    __shared__ float sum[WAVES][kGroup][64];
-    const int group = p.group0 + (int)blockIdx.x, lane = lane_id(), wave = scalar(threadIdx.x >> 6);
-    const int c = (int)blockIdx.y * 64 + lane;
+template <int DT>
+__global__ __launch_bounds__(64) void finish_targets(RestArgs p) {
+    typedef typename Io<DT>::T T;
+    const int group = p.group0 + (int)blockIdx.x, lane = lane_id();
+    const int part = (int)blockIdx.y / p.cols, c = (int)blockIdx.y % p.cols * 256 + lane * 4;
     const int begin = p.list_at[group], end = p.list_at[group + 1];
     if (begin == end) return;
-    uint64_t there = 0;  // the group's targets that come
-    for (int e0 = begin; e0 < end; e0 += 64) {
-        uint64_t m = 0;
-        if (e0 + lane < end) m = 1ull << (p.tgt[p.pos[p.list[e0 + lane]]] % kGroup);
-        for (int d = 1; d < 64; d *= 2) m |= __shfl_xor(m, d, 64);
-        there |= m;
-    }
-    const int targets = __popcll(there);
-    for (int k = 0; k < targets; ++k) sum[wave][k][lane] = 0.0f;
-    // a lane reads and writes its own column of its wave's sums only
-    const uint16_t* x = p.x + c;  // packed rows are whole multiples of 64 elements
-    const int per = (end - begin + WAVES * 64 - 1) / (WAVES * 64) * 64;
-    const int mine = begin + wave * per, mine_end = mine + per < end ? mine + per : end;
-    for (int e0 = mine; e0 < mine_end; e0 += 64) {
-        int row = 0, slot = 0;
-        float rest = 0.0f;
-        if (e0 + lane < mine_end) {
-            row = p.pos[p.list[e0 + lane]];
-            slot = __popcll(there & ((1ull << (p.tgt[row] % kGroup)) - 1));
-            rest = p.rest[row];
-        }
-        const int n = mine_end - e0 < 64 ? mine_end - e0 : 64;
-        for (int k0 = 0; k0 < n; k0 += 8) {
-            float v[8];
+    const int place = p.rest_row[group * kGroup + lane];
+    const float inv = p.head->inv_scale;
+    // packed rows are whole multiples of 64 elements; past them: not stored
+    const uint16_t* x = p.x + (c < p.ldx ? c : 0);
+    int at = 0;
+    for (uint64_t left = __ballot(place >= 0); left; left &= left - 1, ++at) {
+        if (at % p.parts != part) continue;
+        const int slot = __builtin_ctzll(left);
+        const float* base = p.rests + (int64_t)__builtin_amdgcn_readlane(place, slot) * p.d + c;
+        f32x4 s;
 #pragma unroll
-            for (int k = 0; k < 8; ++k)  // past n: row 0, not added
-                v[k] = widen<DT>(x[(int64_t)__builtin_amdgcn_readlane(row, k0 + k) * p.ldx]);
+        for (int q = 0; q < 4; ++q) s[q] = c + q < p.d ? base[q] : 0.0f;
+        for (int e0 = begin; e0 < end; e0 += 64) {
+            const int e = e0 + lane < end ? p.list[e0 + lane] : -1;
+            const bool mine = e >= 0 && e >> kSlotShift == slot;
+            const int row = e & ((1 << kSlotShift) - 1);
+            const float rest = mine ? p.rest[row] : 0.0f;
+            uint64_t hits = __ballot(mine);
+            while (hits) {  // four rows' loads at a time; past the hits: a rest of 0
+                uint2 u[4];
+                float f[4];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                if (k0 + k >= n) break;
-                const float f = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, rest), k0 + k));
-                sum[wave][__builtin_amdgcn_readlane(slot, k0 + k)][lane] += f * v[k];
+                for (int k = 0; k < 4; ++k) {
+                    const int l = hits ? __builtin_ctzll(hits) : 0;
+                    f[k] = hits ? __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, rest), l)) : 0.0f;
+                    const int r = hits ? __builtin_amdgcn_readlane(row, l) : 0;
+                    hits &= hits - 1;
+                    u[k] = *reinterpret_cast<const uint2*>(x + (int64_t)r * p.ldx);
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    if (f[k] == 0.0f) continue;  // and what row 0 holds adds nothing
+                    s[0] += f[k] * widen<DT>((uint16_t)u[k].x);
+                    s[1] += f[k] * widen<DT>((uint16_t)(u[k].x >> 16));
+                    s[2] += f[k] * widen<DT>((uint16_t)u[k].y);
+                    s[3] += f[k] * widen<DT>((uint16_t)(u[k].y >> 16));
+                }
             }
         }
-    }
-    __syncthreads();
-    for (int k = wave; k < targets; k += WAVES) {
-        float s = sum[0][k][lane];
+        T* to = static_cast<T*>(p.dw) + (int64_t)(group * kGroup + slot) * p.d + c;
 #pragma unroll
-        for (int w = 1; w < WAVES; ++w) s += sum[w][k][lane];
-        if (c < p.d) p.rests[(int64_t)(begin + k) * p.d + c] = s;
+        for (int q = 0; q < 4; ++q)
+            if (c + q < p.d) Elem<T>::put(to + q, s[q] * inv);
     }
-    if (blockIdx.y == 0 && wave == 0 && (there >> lane & 1))
-        p.rest_row[group * kGroup + lane] = begin + __popcll(there & ((1ull << lane) - 1));
+}
+
+// dw rows of a piece from the splits' sums; targets' sums go to `rests` as they
+// are.
+template <int DT>
+__global__ __launch_bounds__(256) void finish_dw(const Head* head, const float* acc, int splits, int64_t rows, int64_t d,
+                                                 void* dw, const int* rest_row, float* rests) {
+    typedef typename Io<DT>::T T;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= rows * d) return;
+    // a split of no step wrote nothing
+    const int steps = (head->live + kStep - 1) / kStep;
+    splits = splits < steps ? splits : steps;
+    float s = 0.0f;
+    for (int k = 0; k < splits; ++k) s += acc[k * rows * d + i];
+    if constexpr (DT != kF32) {
+        const int place = rest_row[i / d];
+        if (place >= 0) rests[place * d + i % d] = s;
+    }
+    Elem<T>::put(static_cast<T*>(dw) + i, s * head->inv_scale);
 }
 
 // dx rows from the splits' sums, and what rounding took off the targets' entries;
-// ignored rows are zero.
-template <int DT>
+// ignored rows are zero.  Q columns a thread: 4 where rows of sums are whole
+// 16-byte vectors.
+template <int DT, int Q>
 __global__ __launch_bounds__(256) void finish_dx(const Head* head, const int* pos, const float* acc, int64_t d, void* dx,
                                                  const float* rest, const int* tgt, const void* w, int64_t ldw) {
     typedef typename Io<DT>::T T;
+    typedef float vec __attribute__((ext_vector_type(Q)));
     const int64_t r = blockIdx.x;
     const int at = pos[r];
     const float inv = head->inv_scale;
@@ -1086,14 +1133,20 @@ __global__ __launch_bounds__(256) void finish_dx(const Head* head, const int* po
     const int target = at >= 0 && DT != kF32 ? tgt[at] : -1;
     const float more = target >= 0 ? rest[at] : 0.0f;
     const T* wt = static_cast<const T*>(w) + target * ldw;
-    for (int64_t c = threadIdx.x; c < d; c += 256) {
-        float s = 0.0f;
+    for (int64_t c = (int64_t)threadIdx.x * Q; c < d; c += 256 * Q) {
+        vec s = (vec)(0.0f);
         if (at >= 0) {
-            for (int k = 0; k < splits; ++k) s += acc[k * stride + at * d + c];
-            if (target >= 0) s += more * Elem<T>::scalar(wt + c);
-            s *= inv;
+            const float* from = acc + at * d + c;
+#pragma unroll 4
+            for (int k = 0; k < splits; ++k) s += *reinterpret_cast<const vec*>(from + k * stride);
+#pragma unroll
+            for (int q = 0; q < Q; ++q) {
+                if (target >= 0) s[q] += more * Elem<T>::scalar(wt + c + q);
+                s[q] *= inv;
+            }
         }
-        Elem<T>::put(static_cast<T*>(dx) + r * d + c, s);
+#pragma unroll
+        for (int q = 0; q < Q; ++q) Elem<T>::put(static_cast<T*>(dx) + r * d + c + q, s[q]);
     }
 }
 
@@ -1116,7 +1169,8 @@ struct Layout {
     int x_blocks, w_blocks;  // fp32: blocks that take the magnitudes
     int few;             // forward of few rows: its blocks, or 0
     int logits, dx, dw;  // the products' tiles: 256, 128 or 64
-    int64_t head, rows, pos, tgt, at_target, loss_rows, part, parts, a, b, lse, xp, xg, wp, wg, mag, big, rest, list, list_at, rest_row, rests, g, acc, bytes;
+    int dw_splits;
+    int64_t head, rows, pos, tgt, at_target, loss_rows, part, parts, a, b, lse, xp, xg, wp, wg, mag, big, rest, list, list_at, rest_row, rests, dw_acc, g, acc, bytes;
 };
 
 // A product's tiles: the largest that fill most of the chip.
@@ -1125,9 +1179,9 @@ int tile_size(int64_t m, int64_t n, int64_t copies) {
     return div_up(m, 128) * div_up(n, 128) * copies >= 200 ? 128 : 64;
 }
 
-// Tiles of dx, m x n results of `steps` of K, and the splits that it has room
-// for, as dx_splits chooses them with every row live.
-void dx_plan(int64_t m, int64_t n, int64_t steps, int terms, int& tile, int& splits) {
+// Tiles and splits of K of dx or dw, m x n results of `steps` of K, as dx_splits
+// chooses them with every row live.
+void split_plan(int64_t m, int64_t n, int64_t steps, int terms, int& tile, int& splits) {
     double best = 0.0;
     for (int t = 256; t >= 64; t /= 2) {
         const int64_t tiles = div_up(m, t) * div_up(n, t), slots = 256 * (256 / t);
@@ -1145,7 +1199,10 @@ void dx_plan(int64_t m, int64_t n, int64_t steps, int terms, int& tile, int& spl
 }
 
 // aligned: w's rows can be read as matrix operands where they are.
-Layout layout(int64_t N, int64_t V, int64_t D, int dtype, bool bwd, bool aligned) {
+// alone: a forward that no backward follows.  One that is followed takes the tiles
+// also for few rows: the backward makes its logits again, and they have to be
+// the ones its lse was taken of, to the bit, where a probability is near 1.
+Layout layout(int64_t N, int64_t V, int64_t D, int dtype, bool bwd, bool alone, bool aligned) {
     Layout l{};
     int64_t at = 0;
     auto take = [&](int64_t bytes) {
@@ -1157,8 +1214,7 @@ Layout layout(int64_t N, int64_t V, int64_t D, int dtype, bool bwd, bool aligned
     int64_t most = kPieceBytes / (2 * parts * round_up(N, 64)) / 256 * 256;
     if (most < 2048) most = 2048;
     l.ldx = round_up(D, 64);
-    const bool few = N <= few_rows(dtype) && aligned && D % (dtype == kF32 ? 4 : 64) == 0;
-    if (!bwd && few) {
+    if (alone && N <= few_rows(dtype) && aligned && D % (dtype == kF32 ? 4 : 64) == 0) {
         const int64_t blocks = div_up(div_up(V, 32), kFewWaves);
         l.few = (int)(blocks < 512 ? blocks : 512);
     }
@@ -1176,8 +1232,8 @@ Layout layout(int64_t N, int64_t V, int64_t D, int dtype, bool bwd, bool aligned
     l.tgt = take(4 * N);
     l.xp = take(2 * lparts * N * l.ldx);
     l.wp = take(l.pack_w ? 2 * lparts * l.piece * l.ldx : 0);
-    l.x_blocks = dtype == kF32 && !l.few ? (int)(div_up(N, 16) < 32 ? div_up(N, 16) : 32) : 0;
-    l.w_blocks = dtype == kF32 && !l.few ? (int)(div_up(V, 16) < 256 ? div_up(V, 16) : 256) : 0;
+    l.x_blocks = dtype == kF32 && !bwd && !l.few ? (int)(div_up(N, 16) < 32 ? div_up(N, 16) : 32) : 0;
+    l.w_blocks = dtype == kF32 && !bwd && !l.few ? (int)(div_up(V, 16) < 256 ? div_up(V, 16) : 256) : 0;
     l.mag = take(4 * (l.x_blocks + l.w_blocks));
     l.big = take(8);
     l.logits = tile_size(l.piece, N, 1);
@@ -1187,6 +1243,9 @@ Layout layout(int64_t N, int64_t V, int64_t D, int dtype, bool bwd, bool aligned
         l.loss_rows = take(4 * N);
         l.part = take(8 * N * l.parts);
     } else {
+        split_plan(D, N, l.piece / kStep, terms((int)parts), l.dx, l.splits);
+        split_plan(D, l.piece, div_up(N, kStep), terms((int)parts), l.dw, l.dw_splits);
+        if (l.dw_splits == 1) l.dw = tile_size(D, l.piece, 1);
         l.a = take(4 * N);
         l.b = take(4 * N);
         l.lse = take(4 * N);
@@ -1195,8 +1254,7 @@ Layout layout(int64_t N, int64_t V, int64_t D, int dtype, bool bwd, bool aligned
         l.list_at = take(4 * (div_up(V, kGroup) + 1));
         l.rest_row = take(4 * round_up(V, kGroup));
         l.rests = take(dtype == kF32 ? 0 : 4 * N * D);
-        dx_plan(D, N, l.piece / kStep, terms((int)parts), l.dx, l.splits);
-        l.dw = tile_size(D, l.piece, 1);
+        l.dw_acc = take(l.dw_splits > 1 ? 4 * l.dw_splits * l.piece * D : 0);
         // fp32: x and w again in the gradients' parts
         l.xg = dtype == kF32 ? take(2 * parts * N * l.ldx) : l.xp;
         l.wg = dtype == kF32 ? take(2 * parts * l.piece * l.ldx) : l.wp;
@@ -1237,8 +1295,8 @@ struct Operands {
 // Packs what has to be packed for the piece at v0 (x with the first piece) and
 // sets up its operands.
 template <int DT>
-void operands(const Call& c, const Layout& l, int64_t v0, int64_t rows, bool dx, bool dw, float* big,
-              const float* given, Operands& o) {
+void operands(const Call& c, const Layout& l, int64_t v0, int64_t rows, bool dx, bool dw, bool fwd, float* big,
+              Operands& o) {
     typedef typename Io<DT>::T T;
     const T* w = static_cast<const T*>(c.w) + v0 * c.ldw;
     PackArgs p{};
@@ -1246,8 +1304,7 @@ void operands(const Call& c, const Layout& l, int64_t v0, int64_t rows, bool dx,
     p.d = c.D;
     p.ldp = l.ldx;
     p.big = big;
-    if (v0 == 0) p.mag = at<float>(c, l.mag);
-    p.given = given;
+    if (fwd && v0 == 0) p.mag = at<float>(c, l.mag);
     p.x_blocks = l.x_blocks;
     p.w_blocks = l.w_blocks;
     if (v0 == 0) {
@@ -1303,10 +1360,10 @@ PlanArgs plan_args(const Call& c, const Layout& l) {
 }
 
 template <int DT>
-MagArgs mag_args(const Call& c, const Layout& l, const float* given) {
+MagArgs mag_args(const Call& c, const Layout& l) {
     if constexpr (DT != kF32) return MagArgs{};
     return MagArgs{static_cast<const float*>(c.x), c.ldx,      static_cast<const float*>(c.w), c.ldw, c.D,
-                   at<float>(c, l.mag),            l.x_blocks, l.w_blocks,                     given};
+                   at<float>(c, l.mag),            l.x_blocks, l.w_blocks};
 }
 
 template <int DT>
@@ -1315,12 +1372,12 @@ void run_fwd(const Call& c, const Layout& l, float* loss, float* lse) {
     p.loss_rows = c.reduction == 0 ? loss : at<float>(c, l.loss_rows);
     p.lse_out = lse;
     plan_kernel<false><<<dim3((unsigned)(1 + l.x_blocks + l.w_blocks)), kPlanThreads, 0, c.s>>>(
-        p, mag_args<DT>(c, l, nullptr));
+        p, mag_args<DT>(c, l));
     Operands o{};
-    float* big = lse + c.N;
+    float* big = lse ? lse + c.N : at<float>(c, l.big);
     for (int64_t v0 = 0; v0 < c.V; v0 += l.piece) {
         const int64_t rows = c.V - v0 < l.piece ? c.V - v0 : l.piece;
-        if (DT != kF32 || !l.few) operands<DT>(c, l, v0, rows, false, false, big, nullptr, o);
+        if (DT != kF32 || !l.few) operands<DT>(c, l, v0, rows, false, false, true, big, o);
         if (l.few) {
             FewArgs f{c.w, c.ldw, o.x.p, o.x.ld, p.rows, (int)c.D, (int)c.V, p.head, p.tgt, at<float2>(c, l.part), l.parts,
                       at<float>(c, l.at_target)};
@@ -1381,14 +1438,14 @@ void run_bwd(const Call& c, const Layout& l, const float* grad, const float* lse
     p.list_at = at<int>(c, l.list_at);
     p.rest_row = at<int>(c, l.rest_row);
     p.groups = DT != kF32 && dw ? (int)div_up(c.V, kGroup) : 0;
-    const int64_t beside = DT == kF32 ? l.x_blocks + l.w_blocks : div_up(p.groups, kPlanThreads / 64);
-    plan_kernel<true><<<dim3((unsigned)(1 + beside)), kPlanThreads, 0, c.s>>>(p, mag_args<DT>(c, l, lse + c.N));
+    const int64_t beside = div_up(p.groups, kPlanThreads / 64);
+    plan_kernel<true><<<dim3((unsigned)(1 + beside)), kPlanThreads, 0, c.s>>>(p, MagArgs{});
     Operands o{};
-    float* big = at<float>(c, l.big);
+    float* big = const_cast<float*>(lse) + c.N;  // the forward's; not written here
     const int64_t g_part = round_up(c.N, 64) * l.piece;
     for (int64_t v0 = 0; v0 < c.V; v0 += l.piece) {
         const int64_t rows = c.V - v0 < l.piece ? c.V - v0 : l.piece;
-        operands<DT>(c, l, v0, rows, dx != nullptr, dw != nullptr, big, lse + c.N, o);
+        operands<DT>(c, l, v0, rows, dx != nullptr, dw != nullptr, false, big, o);
         GradArgs g{};
         g.w = o.w;
         g.x = o.x;
@@ -1426,35 +1483,43 @@ void run_bwd(const Call& c, const Layout& l, const float* grad, const float* lse
             by_shape(l.dx, [&](auto shape) {
                 typedef decltype(shape) S;
                 a.tiles_m = (int)div_up(c.D, S::TM);
-                product<DT, S, true><<<grid_of<S>((int64_t)a.tiles_m * (div_up(c.N, S::TN) * l.splits + 64)), S::kThreads, 0, c.s>>>(a);
+                product<DT, S, kDx><<<grid_of<S>((int64_t)a.tiles_m * (div_up(c.N, S::TN) * l.splits + 64)), S::kThreads, 0, c.s>>>(a);
             });
         }
         if (dw) {
-            if constexpr (DT != kF32) {
-                const RestArgs r{g.rest,  p.list,   p.list_at, p.pos,                 p.tgt,
-                                 o.x.p,   o.x.ld,   (int)c.D,  (int)(v0 / kGroup),    at<float>(c, l.rests),
-                                 p.rest_row};
-                const dim3 grid((unsigned)div_up(rows, kGroup), (unsigned)div_up(c.D, 64));
-                // many rows a group (small vocabularies): eight waves share them.
-                // (2469, 64, 125): the call 412 us with one wave, which is all that
-                // fits eight blocks a CU where most groups have a few rows
-                if (c.N * kGroup > 256 * c.V) sum_rests<DT, 8><<<grid, 512, 0, c.s>>>(r);
-                else sum_rests<DT, 1><<<grid, 64, 0, c.s>>>(r);
-            }
             a.a = o.xg;
             a.b = Operand{g.g, l.piece, g_part, 0, l.piece};
             a.n = (int)rows;
             a.out = static_cast<T*>(dw) + v0 * c.D;
+            a.acc = at<float>(c, l.dw_acc);
+            a.splits = l.dw_splits;
             by_shape(l.dw, [&](auto shape) {
                 typedef decltype(shape) S;
                 a.tiles_m = (int)div_up(c.D, S::TM);
-                product<DT, S, false><<<grid_of<S>((int64_t)a.tiles_m * div_up(rows, S::TN)), S::kThreads, 0, c.s>>>(a);
+                const int64_t tiles = (int64_t)a.tiles_m * div_up(rows, S::TN);
+                if (a.splits > 1) product<DT, S, kDwSplit><<<grid_of<S>(tiles * a.splits), S::kThreads, 0, c.s>>>(a);
+                else product<DT, S, kDw><<<grid_of<S>(tiles), S::kThreads, 0, c.s>>>(a);
             });
+            if (a.splits > 1)
+                finish_dw<DT><<<dim3((unsigned)div_up(rows * c.D, 256)), 256, 0, c.s>>>(
+                    p.head, a.acc, a.splits, rows, c.D, a.out, a.rest_row, a.rests);
+            if constexpr (DT != kF32) {
+                // many rows a group (small vocabularies): its targets in 16 waves
+                const int cols = (int)div_up(c.D, 256), parts = c.N * kGroup > 128 * c.V ? 16 : 1;
+                finish_targets<DT><<<dim3((unsigned)div_up(rows, kGroup), (unsigned)(cols * parts)), 64, 0, c.s>>>(
+                    RestArgs{p.head, g.rest, p.list, p.list_at, p.rest_row, o.x.p, o.x.ld, (int)c.D, (int)(v0 / kGroup),
+                             cols, parts, a.rests, dw});
+            }
         }
     }
-    if (dx)
-        finish_dx<DT><<<dim3((unsigned)c.N), 256, 0, c.s>>>(p.head, p.pos, at<float>(c, l.acc), c.D, dx,
-                                                            at<float>(c, l.rest), p.tgt, c.w, c.ldw);
+    if (dx) {
+        auto finish = [&](auto q) {
+            finish_dx<DT, decltype(q)::value><<<dim3((unsigned)c.N), 256, 0, c.s>>>(
+                p.head, p.pos, at<float>(c, l.acc), c.D, dx, at<float>(c, l.rest), p.tgt, c.w, c.ldw);
+        };
+        if (c.D % 4 == 0) finish(std::integral_constant<int, 4>{});
+        else finish(std::integral_constant<int, 1>{});
+    }
 }
 
 // w's rows can be read as operands where they are: 16-byte loads at 16-byte
@@ -1463,7 +1528,7 @@ bool is_aligned(const void* w, int64_t ldw, int dtype) {
     return (reinterpret_cast<uintptr_t>(w) & 15u) == 0 && ldw % (dtype == kF32 ? 4 : 8) == 0 && ldw <= (1 << 22);
 }
 
-int check(const char* name, const Call& c, int dtype, size_t ws_bytes, bool bwd) {
+int check(const char* name, const Call& c, int dtype, size_t ws_bytes, bool bwd, bool alone) {
     FL_CHECK(c.N >= 0 && c.V >= 1 && c.D >= 1, "%s: bad shape (N=%lld, V=%lld, D=%lld)", name, (long long)c.N,
              (long long)c.V, (long long)c.D);
     FL_CHECK(dtype >= 0 && dtype <= 2, "%s: dtype %d", name, dtype);
@@ -1476,7 +1541,7 @@ int check(const char* name, const Call& c, int dtype, size_t ws_bytes, bool bwd)
     FL_CHECK(c.x && c.w && c.target, "%s: NULL pointer argument", name);
     FL_CHECK(reinterpret_cast<uintptr_t>(c.x) % size == 0 && reinterpret_cast<uintptr_t>(c.w) % size == 0,
              "%s: x or w is not element-aligned", name);
-    const int64_t need = layout(c.N, c.V, c.D, dtype, bwd, is_aligned(c.w, c.ldw, dtype)).bytes;
+    const int64_t need = layout(c.N, c.V, c.D, dtype, bwd, alone, is_aligned(c.w, c.ldw, dtype)).bytes;
     FL_CHECK((int64_t)ws_bytes >= need, "%s: workspace of %llu bytes, %lld needed", name, (unsigned long long)ws_bytes,
              (long long)need);
     FL_CHECK(c.ws && (reinterpret_cast<uintptr_t>(c.ws) & 255u) == 0, "%s: workspace is not 256-byte aligned", name);
@@ -1489,10 +1554,10 @@ int check(const char* name, const Call& c, int dtype, size_t ws_bytes, bool bwd)
 
 using namespace fl::lce;
 
-extern "C" size_t fl_linear_ce_workspace_bytes(int64_t N, int64_t V, int64_t D, int dtype, int backward,
+extern "C" size_t fl_linear_ce_workspace_bytes(int64_t N, int64_t V, int64_t D, int dtype, int pass,
                                                const void* w, int64_t ldw) {
-    if (N < 1 || V < 1 || D < 1 || dtype < 0 || dtype > 2 || N > (1 << 23) || V > (1 << 28) || D > (1 << 20)) return 0;
-    return (size_t)layout(N, V, D, dtype, backward != 0, is_aligned(w, ldw, dtype)).bytes;
+    if (N < 1 || V < 1 || D < 1 || dtype < 0 || dtype > 2 || pass < 0 || pass > 2 || N > (1 << 23) || V > (1 << 28) || D > (1 << 20)) return 0;
+    return (size_t)layout(N, V, D, dtype, pass == 2, pass == 0, is_aligned(w, ldw, dtype)).bytes;
 }
 
 extern "C" int fl_linear_ce_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const int64_t* target,
@@ -1501,10 +1566,10 @@ extern "C" int fl_linear_ce_fwd(const void* x, int64_t ldx, const void* w, int64
                                 void* stream) {
     const Call c{x,      ldx, w, ldw, target, N, V, D, ignore_index, z_loss, reduction, static_cast<char*>(workspace),
                  static_cast<hipStream_t>(stream)};
-    const int rc = check("fl_linear_ce_fwd", c, dtype, workspace_bytes, false);
+    const int rc = check("fl_linear_ce_fwd", c, dtype, workspace_bytes, false, !lse);
     if (rc != FL_OK || N == 0) return rc;
-    FL_CHECK(loss && lse, "fl_linear_ce_fwd: NULL pointer argument");
-    const Layout l = layout(N, V, D, dtype, false, is_aligned(c.w, c.ldw, dtype));
+    FL_CHECK(loss, "fl_linear_ce_fwd: NULL pointer argument");
+    const Layout l = layout(N, V, D, dtype, false, !lse, is_aligned(c.w, c.ldw, dtype));
     if (dtype == kF32) run_fwd<kF32>(c, l, loss, lse);
     else if (dtype == kF16) run_fwd<kF16>(c, l, loss, lse);
     else run_fwd<kBF16>(c, l, loss, lse);
@@ -1517,11 +1582,11 @@ extern "C" int fl_linear_ce_bwd(const float* grad, const void* x, int64_t ldx, c
                                 void* workspace, size_t workspace_bytes, void* stream) {
     const Call c{x,      ldx, w, ldw, target, N, V, D, ignore_index, z_loss, reduction, static_cast<char*>(workspace),
                  static_cast<hipStream_t>(stream)};
-    const int rc = check("fl_linear_ce_bwd", c, dtype, workspace_bytes, true);
+    const int rc = check("fl_linear_ce_bwd", c, dtype, workspace_bytes, true, false);
     if (rc != FL_OK || N == 0) return rc;
     FL_CHECK(grad && lse, "fl_linear_ce_bwd: NULL pointer argument");
     if (!dx && !dw) return fl::ok();
-    const Layout l = layout(N, V, D, dtype, true, is_aligned(c.w, c.ldw, dtype));
+    const Layout l = layout(N, V, D, dtype, true, false, is_aligned(c.w, c.ldw, dtype));
     if (dtype == kF32) run_bwd<kF32>(c, l, grad, lse, dx, dw);
     else if (dtype == kF16) run_bwd<kF16>(c, l, grad, lse, dx, dw);
     else run_bwd<kBF16>(c, l, grad, lse, dx, dw);

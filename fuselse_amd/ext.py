@@ -896,43 +896,45 @@ def _row_stride(t: torch.Tensor) -> int:
 
 
 def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, ignore_index: int = -100,
-                         reduction: str = "mean", z_loss: float = 0.0):
+                         reduction: str = "mean", z_loss: float = 0.0, with_lse: bool = True):
     """Softmax cross entropy of the logits x @ weight.T, which are never
     stored: (loss, lse) in fp32; lse (N + 2,) holds the rows' log-sum-exps and
-    two values more for the backward.  x (N, D) and
+    two values more for the backward, or is None without with_lse, which few
+    rows take less time for.  x (N, D) and
     weight (V, D) fp32, fp16 or bf16 with contiguous rows, target int64 (N,).
     loss[n] = lse[n] - x[n] . weight[target[n]] + z_loss * lse[n]^2; rows whose
     target is ignore_index have loss 0 and are not read."""
     _check_linear(x, weight, target)
-    return _linear_fwd(x, weight, target, ignore_index, _reduction(reduction), z_loss)
+    return _linear_fwd(x, weight, target, ignore_index, _reduction(reduction), z_loss, with_lse)
 
 
-def _linear_workspace(N, V, D, dt, backward, w_ptr, ldw, device):
-    key = (N, V, D, dt, backward, w_ptr & 15, ldw)
+def _linear_workspace(N, V, D, dt, which, w_ptr, ldw, device):
+    key = (N, V, D, dt, which, w_ptr & 15, ldw)
     nbytes = _ws_cache.get(key)
     if nbytes is None:
         if len(_ws_cache) >= 4096:
             _ws_cache.clear()
-        nbytes = _ws_cache[key] = _lib.load().fl_linear_ce_workspace_bytes(N, V, D, dt, backward, w_ptr, ldw)
+        nbytes = _ws_cache[key] = _lib.load().fl_linear_ce_workspace_bytes(N, V, D, dt, which, w_ptr, ldw)
     return torch.empty(nbytes, dtype=torch.uint8, device=device)
 
 
 # The calls themselves, on tensors that were checked (the autograd layers' were,
 # in the forward: the host side is most of a small call's time).
-def _linear_fwd(x, weight, target, ignore_index, red, z_loss):
+def _linear_fwd(x, weight, target, ignore_index, red, z_loss, with_lse):
     N, D = x.shape
     V = weight.shape[0]
     dev = x.device
-    lse = torch.empty((N + 2,), dtype=torch.float32, device=dev)
+    lse = torch.empty((N + 2,), dtype=torch.float32, device=dev) if with_lse else None
     loss = torch.empty((N,) if red == 0 else (), dtype=torch.float32, device=dev)
     if N == 0:
         return loss.zero_(), lse
     dt = _DTYPE_CODE[x.dtype]
     w_ptr, ldw = weight.data_ptr(), _row_stride(weight)
     with _on_device(x):
-        ws = _linear_workspace(N, V, D, dt, 0, w_ptr, ldw, dev)
+        ws = _linear_workspace(N, V, D, dt, 1 if with_lse else 0, w_ptr, ldw, dev)
         _lib.call("fl_linear_ce_fwd", x.data_ptr(), _row_stride(x), w_ptr, ldw, target.data_ptr(), N, V, D, dt,
-                  ignore_index, z_loss, red, loss.data_ptr(), lse.data_ptr(), ws.data_ptr(), ws.numel(), _stream(x))
+                  ignore_index, z_loss, red, loss.data_ptr(), lse.data_ptr() if with_lse else None, ws.data_ptr(),
+                  ws.numel(), _stream(x))
     return loss, lse
 
 
@@ -949,7 +951,7 @@ def _linear_bwd(grad_output, x, weight, target, lse, ignore_index, red, z_loss, 
     dt = _DTYPE_CODE[x.dtype]
     w_ptr, ldw = weight.data_ptr(), _row_stride(weight)
     with _on_device(x):
-        ws = _linear_workspace(N, V, D, dt, 1, w_ptr, ldw, dev)
+        ws = _linear_workspace(N, V, D, dt, 2, w_ptr, ldw, dev)
         _lib.call("fl_linear_ce_bwd", grad_output.data_ptr(), x.data_ptr(), _row_stride(x), w_ptr, ldw,
                   target.data_ptr(), lse.data_ptr(), N, V, D, dt, ignore_index, z_loss, red,
                   dx.data_ptr() if need_x else None, dw.data_ptr() if need_weight else None, ws.data_ptr(),

@@ -39,7 +39,7 @@ def _integers(t: torch.Tensor, name: str) -> torch.Tensor:
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, target, ignore_index, reduction, z_loss):
-        loss, lse = ext._linear_fwd(x, weight, target, ignore_index, reduction, z_loss)
+        loss, lse = ext._linear_fwd(x, weight, target, ignore_index, reduction, z_loss, True)
         ctx.save_for_backward(x, weight, target, lse)
         ctx.args = (ignore_index, reduction, z_loss)
         return loss
@@ -79,7 +79,7 @@ def linear_cross_entropy(input: torch.Tensor, weight: torch.Tensor, target: torc
     if torch.is_grad_enabled() and (input.requires_grad or weight.requires_grad):
         loss = _LinearCrossEntropy.apply(x, w, t, ignore_index, red, z_loss)
     else:
-        loss, _ = ext._linear_fwd(x, w, t, ignore_index, red, z_loss)
+        loss, _ = ext._linear_fwd(x, w, t, ignore_index, red, z_loss, False)
     return loss.reshape(target.shape) if reduction == "none" and target.dim() != 1 else loss
 
 

@@ -352,18 +352,19 @@ int fl_sparse_blocked_grad(const float* node_flows, const float* node_mars, cons
  *
  * fl_linear_ce_fwd: loss fp32 [N] (reduction 0) or [1]; lse fp32
  *   [N + 2], the rows' log-sum-exps (0 for ignored ones) and two values more
- *   for the backward.  A mean over no rows is 0.
+ *   for the backward, or NULL where none follows (few rows then take less
+ *   time).  A mean over no rows is 0.
  * fl_linear_ce_bwd: grad fp32 [N] (reduction 0) or [1]; lse as the forward
  *   wrote it.  dx [N, D] and dw [V, D] contiguous, of x's type; either may be
  *   NULL.  The softmax gradient enters the products rounded once to x's type
  *   (fp32: exactly).
- * fl_linear_ce_workspace_bytes: workspace of either call, which has to be
- *   256-byte aligned, with w and ldw as that call gets them; 0 for sizes that
- *   the calls refuse.
+ * fl_linear_ce_workspace_bytes: workspace of a call, which has to be 256-byte
+ *   aligned: pass 0 a forward without lse, 1 a forward with it, 2 a backward; w
+ *   and ldw as that call gets them.  0 for sizes that the calls refuse.
  * At most 2^23 rows, 2^28 vocabulary entries and 2^20 columns (FL_ERANGE).
  * With N == 0 nothing is written.
  * ------------------------------------------------------------------------- */
-size_t fl_linear_ce_workspace_bytes(int64_t N, int64_t V, int64_t D, int dtype, int backward, const void* w,
+size_t fl_linear_ce_workspace_bytes(int64_t N, int64_t V, int64_t D, int dtype, int pass, const void* w,
                                     int64_t ldw);
 int fl_linear_ce_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const int64_t* target, int64_t N,
                      int64_t V, int64_t D, int dtype, int64_t ignore_index, float z_loss, int reduction, float* loss,

@@ -123,9 +123,10 @@ def check_linear(x, w, t, reduction, z=0.0, ignore=-100):
     within(loss, want, b, "loss")
     within(dx, rx, bx, "dx")
     within(dw, rw, bw, "dw")
+    # without gradients few rows take another path
     plain = fuselse_amd.linear_cross_entropy(x.detach(), w.detach(), t, ignore_index=ignore, reduction=reduction,
                                              z_loss=z)
-    assert torch.equal(plain, loss.detach())
+    within(plain, want, b, "loss without gradients")
 
 
 LINEAR_SHAPES = [(1, 1, 1), (1, 64, 100), (2, 33, 7), (5, 130, 1000), (17, 64, 65), (64, 31, 129), (65, 128, 300),
@@ -173,7 +174,7 @@ def test_linear_few_rows(cuda, n, d, v, dtype):
 
 
 @pytest.mark.parametrize("n,d,v", [(700, 130, 5000), (1500, 320, 9000), (130, 500, 20000), (1100, 64, 300),
-                                   (260, 2048, 520)])
+                                   (260, 2048, 520), (3000, 200, 70), (2000, 66, 3)])
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_linear_tile_sizes(cuda, n, d, v, dtype):
     """Sizes whose products take the large and the middle tiles, with several

@@ -57,7 +57,8 @@ def linear_args(lib, **k):
     (dict(red=3), 1, "reduction"), (dict(ldx=7), 1, "overlap"), (dict(ldw=7), 1, "overlap"),
     (dict(n=(1 << 23) + 1), 3, "2^23 rows"), (dict(v=(1 << 28) + 1), 3, "2^23 rows"), (dict(x=None), 1, "NULL"),
     (dict(t=None), 1, "NULL"), (dict(x=ctypes.c_void_p(4097)), 1, "element-aligned"), (dict(nbytes=8), 1, "needed"),
-    (dict(ws=ctypes.c_void_p(4100)), 1, "256-byte"), (dict(loss=None), 1, "NULL"), (dict(n=0, x=None), 0, ""),
+    (dict(ws=ctypes.c_void_p(4100)), 1, "256-byte"), (dict(loss=None), 1, "NULL"),
+    (dict(lse=None, nbytes=8), 1, "needed"), (dict(n=0, x=None), 0, ""),
 ])
 def test_linear_entry_refusals(change, code, message):
     lib = _lib.load()

@@ -550,9 +550,9 @@ __global__ __launch_bounds__(S::kThreads, 2) void logits_stats(StatArgs p) {
 struct FewArgs {
     const void* w;
     int64_t ldw;
-    const void* x;     // fp16, bf16: the packed live rows; fp32: all rows
+    const void* x;
     int64_t ldx;
-    const int* rows;
+    const int* rows;   // the live ones
     int k, v;          // k: a multiple of 64; fp32: of 4
     const Head* head;
     const int* tgt;
@@ -598,7 +598,7 @@ __global__ __launch_bounds__(kFewWaves * 64) void logits_few(FewArgs p) {
 #pragma unroll
     for (int j = 0; j < FN; ++j) {
         const int n = j * 16 + (lane & 15), at = n < live ? n : live - 1;
-        x[j] = static_cast<const T*>(p.x) + (int64_t)(F32 ? p.rows[at] : at) * p.ldx;
+        x[j] = static_cast<const T*>(p.x) + (int64_t)p.rows[at] * p.ldx;
         target[j] = n < live ? p.tgt[n] : -1;
         m[j] = -kInf;
         s[j] = 0.0f;
@@ -1157,7 +1157,9 @@ constexpr int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * t
 constexpr int64_t div_up(int64_t v, int64_t by) { return (v + by - 1) / by; }
 
 // G of a piece takes at most this many bytes: enough vocabulary rows for the
-// products to fill the chip, and a workspace that stays small beside w.
+// products to fill the chip, and a workspace that stays small beside w.  Training
+// calls with 128 / 256 / 512 / 1024 MB, us: bf16 (4096, 2048, 128256) 5365 / 5263 /
+// 5257 / 5199; fp32 (2048, 1024, 32000) 2542 / 2103 / 2092 / 2100.
 constexpr int64_t kPieceBytes = 256 << 20;
 
 struct Layout {
@@ -1377,14 +1379,11 @@ void run_fwd(const Call& c, const Layout& l, float* loss, float* lse) {
     float* big = lse ? lse + c.N : at<float>(c, l.big);
     for (int64_t v0 = 0; v0 < c.V; v0 += l.piece) {
         const int64_t rows = c.V - v0 < l.piece ? c.V - v0 : l.piece;
-        if (DT != kF32 || !l.few) operands<DT>(c, l, v0, rows, false, false, true, big, o);
         if (l.few) {
-            FewArgs f{c.w, c.ldw, o.x.p, o.x.ld, p.rows, (int)c.D, (int)c.V, p.head, p.tgt, at<float2>(c, l.part), l.parts,
-                      at<float>(c, l.at_target)};
+            const FewArgs f{c.w,    c.ldw,  c.x,   c.ldx, p.rows,  (int)c.D, (int)c.V,
+                            p.head, p.tgt, at<float2>(c, l.part), l.parts, at<float>(c, l.at_target)};
             const dim3 grid((unsigned)l.few), block(kFewWaves * 64);
             if constexpr (DT == kF32) {
-                f.x = c.x;
-                f.ldx = c.ldx;
                 if (c.N > 32) logits_few<DT, 4><<<grid, block, 0, c.s>>>(f);
                 else if (c.N > 16) logits_few<DT, 2><<<grid, block, 0, c.s>>>(f);
                 else logits_few<DT, 1><<<grid, block, 0, c.s>>>(f);
@@ -1393,6 +1392,7 @@ void run_fwd(const Call& c, const Layout& l, float* loss, float* lse) {
             }
             break;  // one piece
         }
+        operands<DT>(c, l, v0, rows, false, false, true, big, o);
         StatArgs a{};
         a.w = o.w;
         a.x = o.x;

@@ -247,7 +247,9 @@ __global__ __launch_bounds__(kThreads) void bwd_rows(BwdArgs p) {
     const int v0 = c * kChunk, v1 = vecs - v0 < kChunk ? vecs : v0 + kChunk;
     const bool last = c == p.chunks - 1;
     const int body = head + v0 * VE;  // the chunk's first whole vector
-    const int e0 = c == 0 ? 0 : body, e1 = last ? (int)p.v : head + v1 * VE;
+    const int tail = head + vecs * VE;
+    // the last chunk may have no vector, and begin behind the tail
+    const int e0 = c == 0 ? 0 : body < tail ? body : tail, e1 = last ? (int)p.v : head + v1 * VE;
 
     const float tlse = p.tlse[r];
     const bool dead = tlse == -kInf;
@@ -289,7 +291,6 @@ __global__ __launch_bounds__(kThreads) void bwd_rows(BwdArgs p) {
     auto grad = [&](float v) { return dead ? 0.0f : gq * fexp2((v * p.inv_t - lse) * kLog2e); };
     // the elements off the grid: one a thread
     if (c == 0 && tid < head) Elem<T>::put(dx + tid, grad(dead ? 0.0f : Elem<T>::scalar(x + tid)));
-    const int tail = head + vecs * VE;
     if (last && tid < p.v - tail) Elem<T>::put(dx + tail + tid, grad(dead ? 0.0f : Elem<T>::scalar(x + tail + tid)));
     // stores past the chunk's vectors fall outside the resource and are dropped
     const __amdgpu_buffer_rsrc_t to =

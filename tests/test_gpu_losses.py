@@ -431,6 +431,17 @@ def test_distill_repeated_index_takes_the_sum(cuda):
         assert torch.equal(first, check_distill(s, t, i, 2.0, "sum"))
 
 
+@pytest.mark.parametrize("v", [8193, 8195, 8197, 8199, 16385, 16393, 16399, 32777])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_distill_teacher_at_a_rows_end(cuda, v, dtype):
+    """Rows a little longer than whole chunks of the backward, at every phase
+    of their first line, with the teacher's entries in the last columns."""
+    print(f"case distill end {v} {dtype}", flush=True)
+    s, t, i = distill_inputs(cuda, (64,), v, 12, dtype, dtype, seed=v)
+    i[:] = v - 1 - torch.arange(12, device=cuda)
+    check_distill(s, t, i, 1.0, "none")
+
+
 def test_distill_masked_student_and_special_values(cuda):
     print("case distill special", flush=True)
     for dtype in DTYPES:

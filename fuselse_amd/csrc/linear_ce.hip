@@ -74,8 +74,9 @@ struct Head {          // at the workspace's start, written by the plan kernel
 // ---------------------------------------------------------------------------
 // Plan: one block lists the live rows in order, and for the backward their
 // coefficients a and b, scaled by a power of two that brings the largest to
-// [2^13, 2^14): G in fp16 then loses 2^-39 of the largest at most to the type's
-// smallest values.
+// [2^13, 2^14) for fp16: G then loses 2^-39 of the largest at most to the type's
+// smallest values.  The others have room below, and need it above, where w or x
+// near the type's largest enter the sums: [2^9, 2^10).
 // ---------------------------------------------------------------------------
 constexpr int kPlanThreads = 1024;
 
@@ -115,6 +116,7 @@ struct PlanArgs {
     const float* lse_in;
     float z;
     int mean;
+    int scale_to;              // the exponent above
     float* a;
     float* b;
     float* lse;
@@ -317,7 +319,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs p, MagArgs 
     if constexpr (BWD) {
         __shared__ float shf[kPlanThreads / 64];
         big = block_max<kPlanThreads>(big, shf);
-        const int e = scale_exp(big, 14);
+        const int e = scale_exp(big, p.scale_to);
         const float scale = __builtin_ldexpf(1.0f, e);
         if (threadIdx.x == 0) p.head->inv_scale = __builtin_ldexpf(1.0f, -e);
         if (threadIdx.x < 64) {
@@ -333,20 +335,17 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs p, MagArgs 
     if (threadIdx.x == 0) p.head->live = live;
 }
 
-// The scale of fp32 logits' operands, and what undoes both in a logit; big holds
-// the magnitudes of x and of w.
+// The scale of fp32 logits' operands, and the exponent that undoes both in a
+// logit (as one step: one of the two may leave the type's range where both
+// together do not); big holds the magnitudes of x and of w.
 __device__ __forceinline__ float operand_scale(float big) { return __builtin_ldexpf(1.0f, scale_exp(big, 15)); }
 template <int DT>
-__device__ __forceinline__ float logit(float acc, float inv_x, float inv_w) {
-    return DT == kF32 ? acc * inv_x * inv_w : acc;
+__device__ __forceinline__ float logit(float acc, int undo) {
+    return DT == kF32 ? __builtin_ldexpf(acc, undo) : acc;
 }
 template <int DT>
-__device__ __forceinline__ void logit_scales(const float* big, float& inv_x, float& inv_w) {
-    inv_x = inv_w = 1.0f;
-    if constexpr (DT == kF32) {
-        inv_x = 1.0f / operand_scale(big[0]);
-        inv_w = 1.0f / operand_scale(big[1]);
-    }
+__device__ __forceinline__ int logit_scale(const float* big) {
+    return DT == kF32 ? -scale_exp(big[0], 15) - scale_exp(big[1], 15) : 0;
 }
 
 // ---------------------------------------------------------------------------
@@ -477,7 +476,7 @@ struct StatJob {
     StatArgs p;
     int live;
     int tiles_n;
-    float inv_x, inv_w;
+    int undo;
 
     typedef Side<S, S::TM, true> SA;
     typedef Side<S, S::TN, true> SB;
@@ -512,7 +511,7 @@ struct StatJob {
             for (int i = 0; i < S::FM; ++i)
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
-                    const float l = logit<DT>(acc[i][j][q], inv_x, inv_w);
+                    const float l = logit<DT>(acc[i][j][q], undo);
                     v[i * 4 + q] = perm_at(i, q) < left ? l : -kInf;
                     if (perm_at(i, q) == hit) p.at_target[n] = l;
                 }
@@ -532,7 +531,7 @@ __global__ __launch_bounds__(S::kThreads, 2) void logits_stats(StatArgs p) {
     StatJob<DT, S> job{p, p.head->live};
     job.p.x.rows = job.live;
     job.tiles_n = (job.live + S::TN - 1) / S::TN;
-    logit_scales<DT>(p.big, job.inv_x, job.inv_w);
+    job.undo = logit_scale<DT>(p.big);
     run_tiles<S, true, true, Logits<DT>::kHalf, Logits<DT>::kParts>(job, p.tiles_m * job.tiles_n, (lds_char*)buf0,
                                                                     (lds_char*)buf1);
 }
@@ -801,7 +800,7 @@ struct GradJob {
     GradArgs p;
     int live;
     int tiles_n;
-    float inv_x, inv_w;
+    int undo;
 
     typedef Side<S, S::TM, true> SA;
     typedef Side<S, S::TN, true> SB;
@@ -849,7 +848,7 @@ struct GradJob {
 #pragma unroll
                 for (int q = 0; q < 8; ++q) {
                     const int m = perm_at(i, q);  // q runs over both fragments
-                    float g = r.a[j] * fexp2((logit<DT>(acc[i + q / 4][j][q % 4], inv_x, inv_w) - r.lse[j]) * kLog2e);
+                    float g = r.a[j] * fexp2((logit<DT>(acc[i + q / 4][j][q % 4], undo) - r.lse[j]) * kLog2e);
                     if (m == hit) hit_g = g += r.b[j];
                     to_parts<DT>(m < cols ? g : 0.0f, o[q]);
                 }
@@ -878,7 +877,7 @@ __global__ __launch_bounds__(S::kThreads, 2) void logits_grad(GradArgs p) {
     GradJob<DT, S> job{p, p.head->live};
     job.p.x.rows = job.live;
     job.tiles_n = (job.live + S::TN - 1) / S::TN;
-    logit_scales<DT>(p.big, job.inv_x, job.inv_w);
+    job.undo = logit_scale<DT>(p.big);
     run_tiles<S, true, true, Logits<DT>::kHalf, Logits<DT>::kParts>(job, p.tiles_m * job.tiles_n, (lds_char*)buf0,
                                                                     (lds_char*)buf1);
 }
@@ -1232,7 +1231,7 @@ Layout layout(int64_t N, int64_t V, int64_t D, int dtype, bool bwd, bool alone, 
     l.rows = take(4 * N);
     l.pos = take(4 * N);
     l.tgt = take(4 * N);
-    l.xp = take(2 * lparts * N * l.ldx);
+    l.xp = take(l.few ? 0 : 2 * lparts * N * l.ldx);
     l.wp = take(l.pack_w ? 2 * lparts * l.piece * l.ldx : 0);
     l.x_blocks = dtype == kF32 && !bwd && !l.few ? (int)(div_up(N, 16) < 32 ? div_up(N, 16) : 32) : 0;
     l.w_blocks = dtype == kF32 && !bwd && !l.few ? (int)(div_up(V, 16) < 256 ? div_up(V, 16) : 256) : 0;
@@ -1423,6 +1422,7 @@ void run_bwd(const Call& c, const Layout& l, const float* grad, const float* lse
     p.grad = grad;
     p.grad_stride = c.reduction == 0 ? 1 : 0;
     p.lse_in = lse;
+    p.scale_to = DT == kF16 ? 14 : 10;
     p.a = at<float>(c, l.a);
     p.b = at<float>(c, l.b);
     p.lse = at<float>(c, l.lse);
@@ -1504,8 +1504,11 @@ void run_bwd(const Call& c, const Layout& l, const float* grad, const float* lse
                 finish_dw<DT><<<dim3((unsigned)div_up(rows * c.D, 256)), 256, 0, c.s>>>(
                     p.head, a.acc, a.splits, rows, c.D, a.out, a.rest_row, a.rests);
             if constexpr (DT != kF32) {
-                // many rows a group (small vocabularies): its targets in 16 waves
-                const int cols = (int)div_up(c.D, 256), parts = c.N * kGroup > 128 * c.V ? 16 : 1;
+                // many rows a group (small vocabularies): its targets in 16 waves.
+                // (2469, 64, 125) in bf16: 162 us for 412 in one; with fewer rows than
+                // that most waves would find no target.  A grid has 65535 rows.
+                const int cols = (int)div_up(c.D, 256);
+                const int parts = c.N * kGroup > 128 * c.V && cols <= 65535 / 16 ? 16 : 1;
                 finish_targets<DT><<<dim3((unsigned)div_up(rows, kGroup), (unsigned)(cols * parts)), 64, 0, c.s>>>(
                     RestArgs{p.head, g.rest, p.list, p.list_at, p.rest_row, o.x.p, o.x.ld, (int)c.D, (int)(v0 / kGroup),
                              cols, parts, a.rests, dw});

@@ -33,8 +33,8 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 // dx and dw: three bf16 parts of 8 bits, to nearest: exact at any magnitude,
 // which G, whose entries reach from 1 down to nothing, needs and fp16's
 // exponents do not give (values within 2^-9 of the largest fp32 count as
-// infinite, and infinite ones make NaN).  Six partial products; those left out are below 2^-24 of the
-// product together.
+// infinite, and infinite ones make NaN).  Six partial products; those left out
+// are below 2^-24 of the product together.
 //
 // The 16-bit matrix rate is 16 times the fp32 one, so three products cost 0.19
 // and six 0.375 of one fp32 product.
@@ -63,7 +63,7 @@ __device__ __forceinline__ void split3(float v, uint16_t (&o)[3]) {
 __device__ __forceinline__ int scale_exp(float m, int to) {
     if (!(m > 0.0f) || !__builtin_isfinite(m)) return 0;
     const int e = to - __builtin_amdgcn_frexp_expf(m);
-    return e < -114 ? -114 : e > 114 ? 114 : e;
+    return e < -126 ? -126 : e > 126 ? 126 : e;
 }
 
 // One product's operand: 16-bit rows `ld` elements apart, in `parts` copies

@@ -348,7 +348,9 @@ int fl_sparse_blocked_grad(const float* node_flows, const float* node_mars, cons
  * other target outside [0, V) makes the row's loss NaN, and with it the
  * gradients it takes part in.  Products of fp16 and bf16 are exact, of fp32
  * to about 2^-21 (an element's digits below 2^-39 of the largest magnitude
- * in its tensor do not enter the logits); sums are fp32.
+ * in its tensor do not enter the logits; one that is not finite, or within
+ * 2^-9 of the type's largest, makes NaN of the gradients it enters); sums are
+ * fp32.
  *
  * fl_linear_ce_fwd: loss fp32 [N] (reduction 0) or [1]; lse fp32
  *   [N + 2], the rows' log-sum-exps (0 for ignored ones) and two values more

@@ -289,6 +289,41 @@ def test_linear_fp16_small_upstream(cuda):
     assert ((a.double() * 2.0 ** 8 - b.double()).abs() <= tiny(torch.float16) * 2.0 ** 8).all()
 
 
+@pytest.mark.parametrize("large", ["weight", "input"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_linear_gradients_near_the_types_largest(cuda, dtype, large):
+    """Gradients of the size of weight (of input) while it is 2^116 times
+    larger and its partner as much smaller: sums on the way stay finite."""
+    print(f"case linear near the largest {dtype} {large}", flush=True)
+    x, w, t = linear_inputs(cuda, 20, 64, 300, dtype, ignored=0.2, seed=12)
+    # no element of the small side is below the type's smallest normal
+    x, w = (torch.where(v.abs() < 2.0 ** -6, 2.0 ** -6, v) for v in (x, w))
+    e = 2.0 ** (116 if large == "weight" else -116)
+    x, w = (x * (1 / e)).requires_grad_(True), (w * e).requires_grad_(True)
+    up = linear_upstream(cuda, 20, "none")
+    loss = fuselse_amd.linear_cross_entropy(x, w, t, reduction="none")
+    want, rx, rw, b, bx, bw = linear_reference(x, w, t, -100, "none", 0.0, up)
+    within(loss, want, b, "loss")
+    dx, dw = torch.autograd.grad(loss, (x, w), up)
+    if large == "weight":
+        within(dx, rx, bx, "dx")
+    else:
+        within(dw, rw, bw, "dw")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_linear_few_rows_at_any_alignment(cuda, dtype):
+    """Rows of x that begin at odd elements, where one pass serves them."""
+    print(f"case linear few unaligned {dtype}", flush=True)
+    x, w, t = linear_inputs(cuda, 7, 192, 4000, dtype, seed=13)
+    for off, stride in ((1, 193), (3, 201), (0, 192)):
+        room = torch.full((7 * stride + off,), float("nan"), device=cuda, dtype=dtype)
+        there = room[off:].as_strided((7, 192), (stride, 1))
+        there.copy_(x)
+        got = fuselse_amd.linear_cross_entropy(there, w, t, reduction="none")
+        assert torch.equal(got, fuselse_amd.linear_cross_entropy(x, w, t, reduction="none")), (off, stride)
+
+
 def test_linear_gradient_against_differences(cuda):
     print("case linear differences", flush=True)
     x, w, t = linear_inputs(cuda, 6, 16, 40, torch.float32, seed=11)

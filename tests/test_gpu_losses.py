@@ -757,3 +757,75 @@ def test_backward_twice_and_saved_hooks(cuda):
     c = torch.autograd.grad(ce, (s["hidden"], s["head"]))
     assert all(torch.equal(x, y) for x, y in zip(a, c))
     torch.autograd.grad(rt.balance_loss, s["router"])
+
+
+# ---------------------------------------------------------------------------
+# Tensors of more than 2^32 bytes, and elements past 2^31
+# ---------------------------------------------------------------------------
+def test_linear_offsets_past_32_bits(cuda):
+    print("case linear large offsets", flush=True)
+    n, d, v, dtype = 40, 2048, 1_100_000, torch.bfloat16
+    g = torch.Generator(device=cuda).manual_seed(20)
+    w = torch.empty(v, d, device=cuda, dtype=dtype).normal_(0.0, 2.0 / math.sqrt(d), generator=g)
+    t = torch.randint(v - 1000, v, (n,), device=cuda, generator=g)
+    t[0], t[1] = 0, -100
+    x = (torch.randn(n, d, device=cuda, generator=g) + 2 * w[t].float()).to(dtype)
+    up = linear_upstream(cuda, n, "none")
+    x.requires_grad_(True)
+    w.requires_grad_(True)
+    loss = fuselse_amd.linear_cross_entropy(x, w, t, reduction="none")
+    dx, dw = torch.autograd.grad(loss, (x, w), up)
+    plain = fuselse_amd.linear_cross_entropy(x.detach()[:12], w.detach(), t[:12], reduction="none")
+    want, rx, rw, b, bx, bw = linear_reference(x, w, t, -100, "none", 0.0, up)
+    within(loss, want, b, "loss")
+    within(plain, want[:12], b[:12], "loss of few rows")
+    within(dx, rx, bx, "dx")
+    for part in (slice(0, 1000), slice(v - 1000, v)):
+        within(dw[part], rw[part], bw[part], "dw")
+
+
+def test_distill_offsets_past_32_bits(cuda):
+    print("case distill large offsets", flush=True)
+    rows, v, k = 17000, 128256, 8
+    g = torch.Generator(device=cuda).manual_seed(21)
+    s = torch.empty(rows, v, device=cuda, dtype=torch.bfloat16).normal_(0.0, 3.0, generator=g).requires_grad_(True)
+    t = torch.randn(rows, k, device=cuda, generator=g)
+    i = torch.arange(k, device=cuda) * 7919 + torch.arange(rows, device=cuda)[:, None]
+    up = torch.randn(rows, device=cuda, generator=g)
+    loss = fuselse_amd.topk_distillation(s, t, i, reduction="none")
+    (ds,) = torch.autograd.grad(loss, s, up)
+    for part in (slice(0, 20), slice(rows - 20, rows)):
+        want, rs, b, bs = distill_reference(s[part], t[part], i[part], 1.0, "none", up[part])
+        within(loss[part], want, b, "loss")
+        within(ds[part], rs, bs, "ds")
+
+
+def test_router_offsets_past_32_bits(cuda):
+    """A batch repeated: the losses of one copy, its counts times the copies,
+    and its gradient over the copies in each."""
+    print("case router large offsets", flush=True)
+    tokens, e, k, copies = 4096, 1024, 2, 520
+    g = torch.Generator(device=cuda).manual_seed(22)
+    base = (torch.randn(tokens, e, device=cuda, generator=g)).to(torch.float16)
+    index = torch.randint(0, e, (tokens, k), device=cuda, generator=g)
+    x = base.repeat(copies, 1).requires_grad_(True)
+    out = fuselse_amd.router_balance(x, index.repeat(copies, 1))
+    xd = base.double()
+    p = torch.softmax(xd, 1)
+    counts = torch.bincount(index.flatten(), minlength=e)
+    f = counts.double() / (tokens * k)
+    balance, z = e * (f * p.mean(0)).sum(), (torch.logsumexp(xd, 1) ** 2).mean()
+    assert torch.equal(out.counts, counts * copies)
+    # a lane adds at most tokens copies / (256 blocks 16 groups) probabilities
+    # one after another, of exponents that are rounded by 2^-21 each
+    rel = tokens * copies / (256 * 16) * E23 + 2.0 ** -20
+    assert abs(float(out.balance_loss) - float(balance)) <= rel * float(balance)
+    assert abs(float(out.z_loss) - float(z)) <= 2.0 ** -18 * float(z)
+    # upstream gradients that bring an element's to the size of p: within fp16
+    scale = float(tokens * copies)
+    (dx,) = torch.autograd.grad(out.balance_loss, x, torch.full((), scale, device=cuda))
+    want = p * (e * f - (p * (e * f)).sum(1, keepdim=True))
+    bound = (2.0 ** -18 * p * (e * f + (p * (e * f)).sum(1, keepdim=True)) + u(torch.float16) * want.abs()
+             + tiny(torch.float16))
+    for c in (0, copies - 1):
+        within(dx[c * tokens:(c + 1) * tokens], want, bound, f"dx of copy {c}")

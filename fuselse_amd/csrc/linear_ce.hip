@@ -751,9 +751,14 @@ __global__ __launch_bounds__(256) void finish_rows(const Head* head, const int* 
     if (r >= head->live) return;
     const int lane = threadIdx.x & 63;
     float m = -kInf, s = 0.0f;
-    for (int64_t k = lane; k < parts; k += 64) {
-        const float2 q = part[r * parts + k];
-        lse_merge(m, s, q.x, q.y);
+    // the pairs lie in other XCDs' memory: eight loads a lane in flight
+    constexpr int U = 8;
+    for (int64_t k0 = lane; k0 < parts; k0 += 64 * U) {
+        float2 q[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) q[u] = k0 + u * 64 < parts ? part[r * parts + k0 + u * 64] : make_float2(-kInf, 0.0f);
+#pragma unroll
+        for (int u = 0; u < U; ++u) lse_merge(m, s, q[u].x, q[u].y);
     }
     group_merge<64>(m, s);
     if (lane == 0) {

@@ -7,10 +7,13 @@
 //
 // Forward: one pass over the student's row (running maximum and sum), K
 // gathers.  Backward: one read and one write of the row.  Both are bound by
-// memory; no product, no matrix cores.  Entries whose teacher logit is -inf
-// are unused, whatever their index; a row without any other has loss and
-// gradient 0.  A used index outside [0, V) makes the row's loss and gradient
-// NaN.
+// memory; no product, no matrix cores.  (4092, 128256) in bf16 with 64 entries:
+// forward 172 us, 6.1 TB/s, backward 303 us, 6.9 TB/s; (1536, 50257) in fp32 with
+// 20: 52 us, 5.9 TB/s, and 96 us, 6.4 TB/s (a copy: 6.8).
+//
+// Entries whose teacher logit is -inf are unused, whatever their index; a row
+// without any other has loss and gradient 0.  A used index outside [0, V) makes
+// the row's loss and gradient NaN.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -43,6 +46,25 @@ struct FwdArgs {
     float* lse;
     float* tlse;
 };
+
+// lse_fold of v * inv_t, the factor taken into the exponent's: c = inv_t log2 e.
+template <int K>
+__device__ __forceinline__ void fold_scaled(float& m, float& s, const float (&v)[K], float inv_t, float c) {
+    float cm = v[0];
+#pragma unroll
+    for (int k = 1; k < K; ++k) cm = fmaxf(cm, v[k]);
+    const float b = lse_rebase<true>(m, s, cm * inv_t);
+    float acc = 0.0f;
+    if (lse_fused_exp_ok(b)) {
+        const float nb = -b * kLog2e;
+#pragma unroll
+        for (int k = 0; k < K; ++k) acc += fexp2(__builtin_fmaf(v[k], c, nb));
+    } else {
+#pragma unroll
+        for (int k = 0; k < K; ++k) acc += lse_exp_exact(v[k] * inv_t, b);
+    }
+    s += acc;
+}
 
 // Joins the teacher's side of a row, in one wave: its log-sum-exp over
 // t_k / T and the loss.  Returns tlse: -inf for a row without a used entry,
@@ -104,14 +126,20 @@ __global__ __launch_bounds__(kThreads) void fwd_rows(FwdArgs p) {
     float m = -kInf, s = 0.0f;
     int64_t e = e0 + (int64_t)threadIdx.x * VE;
     constexpr int64_t step = (int64_t)kThreads * VE;
-    auto fold = [&](const u32x4& raw) {
-        float v[VE];
-        Elem<T>::cvt(raw, v);
+    const float scale = p.inv_t * kLog2e;
+    auto fold = [&](const u32x4 (&raw)[U]) {
+        float v[U * VE];
 #pragma unroll
-        for (int k = 0; k < VE; ++k) v[k] *= p.inv_t;
-        lse_fold<true>(m, s, v);
+        for (int u = 0; u < U; ++u) {
+            float t[VE];
+            Elem<T>::cvt(raw[u], t);
+#pragma unroll
+            for (int k = 0; k < VE; ++k) v[u * VE + k] = t[k];
+        }
+        fold_scaled(m, s, v, p.inv_t, scale);
     };
-    // U vectors are folded while the next U are in flight
+    // U vectors are folded, under one rescale, while the next U are in flight (a
+    // rescale each: 6% more time in bf16, whose vectors hold 8 elements)
     const int64_t full = U * step + VE - step;  // elements from e on that U vectors span
     u32x4 now[U], next[U];
     bool more = e + full <= e1;
@@ -127,8 +155,7 @@ __global__ __launch_bounds__(kThreads) void fwd_rows(FwdArgs p) {
             for (int u = 0; u < U; ++u) next[u] = load_raw_stream<T>(x + e + u * step);
             e += U * step;
         }
-#pragma unroll
-        for (int u = 0; u < U; ++u) fold(now[u]);
+        fold(now);
 #pragma unroll
         for (int u = 0; u < U; ++u) now[u] = next[u];
         more = again;
@@ -136,9 +163,7 @@ __global__ __launch_bounds__(kThreads) void fwd_rows(FwdArgs p) {
     for (; e < e1; e += step) {
         float v[VE];
         load_vec_part<T>(x + e, e1 - e, -kInf, v);
-#pragma unroll
-        for (int k = 0; k < VE; ++k) v[k] *= p.inv_t;
-        lse_fold<true>(m, s, v);
+        fold_scaled(m, s, v, p.inv_t, scale);
     }
     group_merge<64>(m, s);
     __shared__ float sm[kThreads / 64], ss[kThreads / 64];
@@ -221,7 +246,7 @@ struct BwdArgs {
     void* dx;
 };
 
-constexpr int kBwdVecs = 8;  // vectors a thread
+constexpr int kBwdVecs = 2;  // vectors a thread
 
 // A block takes kBwdVecs vectors a thread of a row of the result, from the
 // result's first 128-byte line on, so that a wave stores whole lines; the input,
@@ -322,7 +347,8 @@ __global__ __launch_bounds__(kThreads) void bwd_rows(BwdArgs p) {
 int elem_size(int dtype) { return dtype == 0 ? 4 : 2; }
 
 // Segments a row is cut into in the forward: enough blocks for the chip, none
-// shorter than 16 KB.
+// shorter than 16 KB.  (16, 128256) in bf16: 16 segments 8.8 us, whole rows 22.1,
+// 64 KB at least 13.1; more blocks than 1024 or shorter segments gain nothing.
 int segments(int64_t rows, int64_t v, int dtype) {
     const int64_t most = v * elem_size(dtype) / 16384;
     int64_t want = rows > 0 ? (1024 + rows - 1) / rows : 1;
@@ -380,7 +406,8 @@ int check(const char* name, int64_t rows, int64_t n1, int64_t v, int64_t k, int 
     FL_CHECK(rows >= 0 && v >= 1 && k >= 0 && n1 >= 1, "%s: bad shape (rows=%lld, V=%lld, K=%lld)", name,
              (long long)rows, (long long)v, (long long)k);
     FL_CHECK(dtype >= 0 && dtype <= 2 && tdtype >= 0 && tdtype <= 2, "%s: dtype %d, %d", name, dtype, tdtype);
-    FL_CHECK(temp > 0.0f && __builtin_isfinite(temp), "%s: temperature must be positive and finite", name);
+    FL_CHECK(temp > 0.0f && __builtin_isfinite(temp) && __builtin_isfinite(1.0f / temp),
+             "%s: temperature must be positive and finite, and so its inverse", name);
     if (k > kMaxTop) return set_error(FL_ERANGE, "%s: at most %d teacher logits a row", name, kMaxTop);
     if (rows > (1 << 22) || v > (1 << 28)) return set_error(FL_ERANGE, "%s: at most 2^22 rows of 2^28 columns", name);
     return ok();

@@ -1251,6 +1251,9 @@ Layout layout(int64_t N, int64_t V, int64_t D, int dtype, bool bwd, bool alone, 
     } else {
         split_plan(D, N, l.piece / kStep, terms((int)parts), l.dx, l.splits);
         split_plan(D, l.piece, div_up(N, kStep), terms((int)parts), l.dw, l.dw_splits);
+        // without splits a partly filled round of large tiles is the better one:
+        // (2047, 768, 50257) in fp16, 591 tiles of 256 in three rounds: dw 221 us;
+        // 2358 of 128 in five shorter ones: 258
         if (l.dw_splits == 1) l.dw = tile_size(D, l.piece, 1);
         l.a = take(4 * N);
         l.b = take(4 * N);

@@ -13,6 +13,9 @@
 // and then over blocks in a fixed order, so results do not depend on the order
 // of the blocks.  Both directions read the logits once and are bound by memory,
 // or by the launches where the batch is small: one block then does it all.
+// (131072, 256) in fp32 with 8 choices: forward 30 us (4.8 TB/s) and 9.6 for the
+// join, backward 42 us (6.4 TB/s); (16383, 64) in bf16 with 6: 7.9 + 6.1 and 5.6 us,
+// (512, 8) in fp32 4.5 and 2.9.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -301,7 +304,7 @@ void shape(int experts, int dtype, int& g, int& nv) {
 }
 
 // Elements one block takes by itself, results and all, rather than a second
-// launch: about 2 us of work.
+// launch: (256, 64) 7.5 us for 11.0, but (1024, 64) 14.8 for 11.2.
 constexpr int64_t kAlone = 16384;
 
 int block_count(int64_t tokens, int experts, int dtype) {
@@ -309,6 +312,8 @@ int block_count(int64_t tokens, int experts, int dtype) {
     shape(experts, dtype, g, nv);
     const int groups = kThreads / g;
     if (tokens * experts <= kAlone) return 1;
+    // one block a CU: (131072, 256) 38.2 us in all, with half as many 55.5, with
+    // twice as many, whose parts take longer to join, 39.0
     const int64_t want = (tokens + groups - 1) / groups;
     return (int)(want < 256 ? (want < 1 ? 1 : want) : 256);
 }

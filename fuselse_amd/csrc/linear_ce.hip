@@ -568,6 +568,9 @@ struct FewArgs {
 };
 
 constexpr int kFewWaves = 2;
+// One pass / tiles, us: bf16 (16, 2048, 128256) 99 / 131, 32 rows of it 124 / 123, 64
+// 182 / 125 (x's fragments, read for every 32 rows of w, outweigh w); fp32 (16,
+// 1024, 32000) 39 / 110, 64 rows 79 / 113.
 constexpr int few_rows(int dtype) { return dtype == kF32 ? 64 : 16; }
 
 // split3 of 8 fp32 values, two to a conversion.

@@ -47,21 +47,25 @@ struct FwdArgs {
     float* tlse;
 };
 
-// lse_fold of v * inv_t, the factor taken into the exponent's: c = inv_t log2 e.
+// lse_fold of v / T with the factor in the exponent's, c = log2 e / T: m is the
+// maximum of v itself.  The exponents are c times differences from m, so that c's
+// rounding counts with the differences' size, not with the values'.
 template <int K>
-__device__ __forceinline__ void fold_scaled(float& m, float& s, const float (&v)[K], float inv_t, float c) {
-    float cm = v[0];
+__device__ __forceinline__ void fold_scaled(float& m, float& s, const float (&v)[K], float c) {
+    float mn = m;
 #pragma unroll
-    for (int k = 1; k < K; ++k) cm = fmaxf(cm, v[k]);
-    const float b = lse_rebase<true>(m, s, cm * inv_t);
+    for (int k = 0; k < K; ++k) mn = fmaxf(mn, v[k]);
+    const float b = lse_base(mn);
+    s *= m == -kInf ? 0.0f : fexp2((lse_base(m) - b) * c);
+    m = mn;
+    const float nb = -b * c;
     float acc = 0.0f;
-    if (lse_fused_exp_ok(b)) {
-        const float nb = -b * kLog2e;
+    if (lse_fused_exp_ok(nb)) {
 #pragma unroll
         for (int k = 0; k < K; ++k) acc += fexp2(__builtin_fmaf(v[k], c, nb));
     } else {
 #pragma unroll
-        for (int k = 0; k < K; ++k) acc += lse_exp_exact(v[k] * inv_t, b);
+        for (int k = 0; k < K; ++k) acc += fexp2((v[k] - b) * c);
     }
     s += acc;
 }
@@ -70,8 +74,11 @@ __device__ __forceinline__ void fold_scaled(float& m, float& s, const float (&v)
 // t_k / T and the loss.  Returns tlse: -inf for a row without a used entry,
 // NaN where a used index is out of range.
 template <typename T, typename TT>
-__device__ __forceinline__ void finish_row(const FwdArgs& p, int64_t r, float lse) {
+__device__ __forceinline__ void finish_row(const FwdArgs& p, int64_t r, float sm, float ss) {
     const int lane = lane_id();
+    // log q = (x / T - maximum) - log of the sum: the log-sum-exp's own rounding, of
+    // the maximum's size, stays out
+    const float base = lse_base(sm), rest = flog2(ss) * kLn2, lse = lse_finish<true>(sm, ss);
     const TT* t = static_cast<const TT*>(p.t) + r * p.k;
     const int64_t* index = p.index + r * p.k;
     const T* x = static_cast<const T*>(p.x) + p.map.offset(r);
@@ -83,6 +90,7 @@ __device__ __forceinline__ void finish_row(const FwdArgs& p, int64_t r, float ls
     group_merge<64>(m, s);
     float tlse = lse_finish<true>(m, s);
     if (tlse == kInf) tlse = __builtin_nanf("");  // a softmax of +inf
+    const float tbase = lse_base(m), trest = tlse == tlse ? flog2(s) * kLn2 : tlse;
     float loss = 0.0f;
     if (m != -kInf || s != 0.0f) {  // a NaN never enters m, but makes s NaN
         bool bad = false;
@@ -94,10 +102,10 @@ __device__ __forceinline__ void finish_row(const FwdArgs& p, int64_t r, float ls
                 bad = true;
                 continue;
             }
-            const float logp = tv - tlse;
+            const float logp = (tv - tbase) - trest;
             const float prob = fexp2(logp * kLog2e);
             // a probability that underflows to 0 contributes 0
-            if (prob != 0.0f) loss += prob * (logp - (Elem<T>::scalar(x + i) * p.inv_t - lse));
+            if (prob != 0.0f) loss += prob * (logp - ((Elem<T>::scalar(x + i) * p.inv_t - base) - rest));
         }
         loss += reduce_partner<1>(loss);
         loss += reduce_partner<2>(loss);
@@ -136,7 +144,7 @@ __global__ __launch_bounds__(kThreads) void fwd_rows(FwdArgs p) {
 #pragma unroll
             for (int k = 0; k < VE; ++k) v[u * VE + k] = t[k];
         }
-        fold_scaled(m, s, v, p.inv_t, scale);
+        fold_scaled(m, s, v, scale);
     };
     // U vectors are folded, under one rescale, while the next U are in flight (a
     // rescale each: 6% more time in bf16, whose vectors hold 8 elements)
@@ -163,8 +171,9 @@ __global__ __launch_bounds__(kThreads) void fwd_rows(FwdArgs p) {
     for (; e < e1; e += step) {
         float v[VE];
         load_vec_part<T>(x + e, e1 - e, -kInf, v);
-        fold_scaled(m, s, v, p.inv_t, scale);
+        fold_scaled(m, s, v, scale);
     }
+    m *= p.inv_t;
     group_merge<64>(m, s);
     __shared__ float sm[kThreads / 64], ss[kThreads / 64];
     if (lane_id() == 0) {
@@ -178,7 +187,7 @@ __global__ __launch_bounds__(kThreads) void fwd_rows(FwdArgs p) {
 #pragma unroll
     for (int w = 1; w < kThreads / 64; ++w) lse_merge(m, s, sm[w], ss[w]);
     if (p.segs == 1) {
-        finish_row<T, TT>(p, r, lse_finish<true>(m, s));
+        finish_row<T, TT>(p, r, m, s);
     } else if (threadIdx.x == 0) {
         p.part[r * p.segs + seg] = make_float2(m, s);
     }
@@ -193,7 +202,7 @@ __global__ __launch_bounds__(64) void fwd_finish(FwdArgs p) {
         lse_merge(m, s, q.x, q.y);
     }
     group_merge<64>(m, s);
-    finish_row<T, TT>(p, r, lse_finish<true>(m, s));
+    finish_row<T, TT>(p, r, m, s);
 }
 
 // Sum of the rows' losses in a fixed order; the mean is over the rows that
@@ -258,7 +267,7 @@ __global__ __launch_bounds__(kThreads) void bwd_rows(BwdArgs p) {
     constexpr int VE = Elem<T>::kVec;
     constexpr int kChunk = kThreads * kBwdVecs;  // vectors
     __shared__ int li[kMaxTop];
-    __shared__ float lp[kMaxTop];
+    __shared__ float lp[kMaxTop], lv[kMaxTop];
     __shared__ int ln;
     const int64_t block = p.block0 + blockIdx.x;
     const int64_t r = block / p.chunks;
@@ -292,28 +301,44 @@ __global__ __launch_bounds__(kThreads) void bwd_rows(BwdArgs p) {
     // the teacher's entries of this chunk, in order, found by one wave
     if (tid < 64) {
         int n = 0;
-        for (int k0 = 0; !dead && k0 < p.k; k0 += 64) {
-            const int k = k0 + tid;
-            int64_t i = -1;
-            float tv = -kInf;
-            if (k < p.k) {
-                i = p.index[r * p.k + k];
-                tv = Elem<TT>::scalar(static_cast<const TT*>(p.t) + r * p.k + k) * p.inv_t;
+        constexpr int U = 4;  // entries a lane whose loads are in flight
+        for (int k0 = 0; !dead && k0 < p.k; k0 += 64 * U) {
+            int64_t i[U];
+            float tv[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int k = k0 + u * 64 + tid;
+                i[u] = k < p.k ? p.index[r * p.k + k] : -1;
+                tv[u] = k < p.k ? Elem<TT>::scalar(static_cast<const TT*>(p.t) + r * p.k + k) * p.inv_t : -kInf;
             }
-            const bool mine = tv != -kInf && i >= e0 && i < e1;
-            const uint64_t b = __ballot(mine);
-            if (mine) {
-                const int at = n + __popcll(b & ((1ull << tid) - 1));
-                li[at] = (int)i;
-                lp[at] = g * fexp2((tv - tlse) * kLog2e);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const bool mine = tv[u] != -kInf && i[u] >= e0 && i[u] < e1;
+                const uint64_t b = __ballot(mine);
+                if (mine) {
+                    const int at = n + __popcll(b & ((1ull << tid) - 1));
+                    li[at] = (int)i[u];
+                    lp[at] = g * fexp2((tv[u] - tlse) * kLog2e);
+                }
+                n += __popcll(b);
             }
-            n += __popcll(b);
         }
         if (tid == 0) ln = n;
     }
     __syncthreads();
     const float gq = tlse != tlse ? __builtin_nanf("") : g;
     auto grad = [&](float v) { return dead ? 0.0f : gq * fexp2((v * p.inv_t - lse) * kLog2e); };
+    // The entries' elements, each with the sum of all entries of its index, a thread
+    // an entry: 20 us for 1.2 ms by the elements' own threads one after another at
+    // (9880, 527) with 108 entries.
+    const int n = ln;
+    for (int j = tid; j < n; j += kThreads) {
+        const int i = li[j];
+        const float q = grad(Elem<T>::scalar(x + i));
+        float take = 0.0f;
+        for (int k = 0; k < n; ++k) take += li[k] == i ? lp[k] : 0.0f;
+        lv[j] = q - take;
+    }
     // the elements off the grid: one a thread
     if (c == 0 && tid < head) Elem<T>::put(dx + tid, grad(dead ? 0.0f : Elem<T>::scalar(x + tid)));
     if (last && tid < p.v - tail) Elem<T>::put(dx + tail + tid, grad(dead ? 0.0f : Elem<T>::scalar(x + tail + tid)));
@@ -328,16 +353,14 @@ __global__ __launch_bounds__(kThreads) void bwd_rows(BwdArgs p) {
         for (int k = 0; k < VE; ++k) o[k] = grad(o[k]);
         Elem<T>::put_vec_buf(to, (u * kThreads + tid) * 16, o);
     }
-    // An entry's element is written again by the thread that wrote it before (one
-    // thread's stores to an address keep their order), with the sum of all
-    // entries of that index.
-    for (int j = 0; j < ln; ++j) {
+    // An entry's element is written again by the thread that wrote it before: one
+    // thread's stores to an address keep their order.
+    if (n == 0) return;
+    __syncthreads();
+    for (int j = 0; j < n; ++j) {
         const int i = li[j];
         const int owner = i < head ? i : i >= tail ? i - tail : (i - head) / VE % kThreads;
-        if (owner != tid) continue;
-        float take = 0.0f;
-        for (int k = 0; k < ln; ++k) take += li[k] == i ? lp[k] : 0.0f;
-        Elem<T>::put(dx + i, grad(Elem<T>::scalar(x + i)) - take);
+        if (owner == tid) Elem<T>::put(dx + i, lv[j]);
     }
 }
 

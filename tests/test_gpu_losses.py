@@ -477,6 +477,18 @@ def test_distill_teacher_at_a_rows_end(cuda, v, dtype):
     check_distill(s, t, i, 1.0, "none")
 
 
+@pytest.mark.parametrize("k", [3, 4, 5, 63, 255, 256, 257, 1021, 1022, 1023, 1024])
+def test_distill_many_entries_in_one_chunk(cuda, k):
+    """All of a row's entries in one chunk of the backward, most of them several
+    times, unused ones between them."""
+    print(f"case distill many {k}", flush=True)
+    for dtype in DTYPES:
+        s, t, i = distill_inputs(cuda, (9,), 300, k, dtype, torch.float32, seed=k)
+        i %= 150
+        t[:, 1::7] = -math.inf
+        check_distill(s, t, i, 1.0, "none")
+
+
 def test_distill_masked_student_and_special_values(cuda):
     print("case distill special", flush=True)
     for dtype in DTYPES:

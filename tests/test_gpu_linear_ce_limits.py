@@ -106,3 +106,83 @@ def test_vocabularies_of_several_pieces(cuda, dtype, n, d, v, ignored):
     within(loss[live], want, b, "loss")
     within(dx[live], rx, bx, "dx")
     within(dw, rw, bw, "dw")
+
+
+# ---------------------------------------------------------------------------
+# The rounding of the targets' entries, and of the logits
+# ---------------------------------------------------------------------------
+def dominated_inputs(cuda, n, d, v, dtype, targets, seed=0):
+    """Targets' entries dominate both gradients: all probabilities are about
+    1 / v, only targets' rows of w are large, and logits are exact (x whole
+    multiples of 2^-12 below 2^-4, w quarters from 1 to 1.75, the others +-2^-6)."""
+    g = torch.Generator(device=cuda).manual_seed(seed)
+    sign = lambda *s: torch.randint(0, 2, s, device=cuda, generator=g) * 2.0 - 1.0
+    x = torch.randint(128, 256, (n, d), device=cuda, generator=g) * sign(n, d) * 2.0 ** -12
+    w = sign(v, d) * 2.0 ** -6
+    large = targets.unique()
+    w[large] *= 2.0 ** 6 + 2.0 ** 4 * torch.randint(0, 4, (len(large), d), device=cuda, generator=g)
+    return x.to(dtype), w.to(dtype)
+
+
+def rounded(G, dtype):
+    """G as the products would take it with every entry rounded to dtype."""
+    scale = 2.0 ** (13 - math.frexp(float(G.abs().max()))[1])
+    return (G * scale).to(dtype).double() / scale
+
+
+@pytest.mark.parametrize("n,d,v,kind", [
+    (300, 64, 20000, "few"),        # several rows a target, several targets a group of 64
+    (300, 130, 20000, "one"),       # one target of every row; rows that are no whole vectors
+    (513, 64, 9000, "each"),        # a target of its own for nearly every row
+    (2469, 64, 125, "weighted"),    # many rows a group: its targets in several waves
+    (65536, 64, 16389, "ignored"),  # several pieces
+    (1500, 320, 9000, "few"),       # dw in whole sums
+])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_the_rounding_of_a_targets_entry_is_given_back(cuda, n, d, v, kind, dtype):
+    print(f"case linear target rounding {n} {d} {v} {kind} {dtype}", flush=True)
+    g = torch.Generator(device=cuda).manual_seed(n + d)
+    if kind == "few":
+        t = torch.tensor([64, 65, 66, 127, 700, v - 1], device=cuda)[torch.randint(0, 6, (n,), device=cuda, generator=g)]
+    elif kind == "one":
+        t = torch.full((n,), v - 3, device=cuda)
+    else:
+        t = torch.randint(0, 20 if kind == "weighted" else v, (n,), device=cuda, generator=g) * (5 if kind == "weighted" else 1)
+    if kind == "ignored":
+        t[torch.rand(n, device=cuda, generator=g) < 0.99] = -100
+    x, w = dominated_inputs(cuda, n, d, v, dtype, t[t != -100], seed=v)
+    up = upstream(cuda, n)
+    if kind == "ignored":
+        assert_several_pieces(n, d, v, dtype, w)
+    if kind == "weighted":  # few rows carry the gradients
+        up = torch.where(torch.arange(n, device=cuda) % 157 == 0, up, 2.0 ** -14)
+    live = t != -100
+    xl, tl, ul = x[live], t[live], up[live]
+    loss, dx, dw = own(x, w, t, up)
+    want, rx, rw, b, bx, bw, G = live_reference(xl, w, tl, ul, 0.0)
+    # the bounds tell: without the rounding given back each gradient breaks them
+    wrong = rounded(G, dtype)
+    for name, bad, right, bound in (("dx", (wrong @ w.double()).to(dtype), rx, bx),
+                                    ("dw", (wrong.t() @ xl.double()).to(dtype), rw, bw)):
+        assert ((bad.double() - right).abs() > bound).any(), f"{name}: the bound does not tell"
+    within(loss[live], want, b, "loss")
+    within(dx[live], rx, bx, "dx")
+    within(dw, rw, bw, "dw")
+
+
+@pytest.mark.parametrize("n,d,v", [(300, 2048, 1000), (129, 4096, 300)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_exact_logits_of_many_columns(cuda, n, d, v, dtype):
+    """x and w of -1, 0 and 1 times powers of two: logits have no error, and
+    the results that of the exponentials, G's rounding and the sums alone."""
+    print(f"case linear exact logits {n} {d} {v} {dtype}", flush=True)
+    g = torch.Generator(device=cuda).manual_seed(d)
+    x = (torch.randint(-1, 2, (n, d), device=cuda, generator=g) * 2.0 ** -2).to(dtype)
+    w = (torch.randint(-1, 2, (v, d), device=cuda, generator=g) * 2.0 ** -2).to(dtype)
+    t = torch.randint(0, v, (n,), device=cuda, generator=g)
+    up = upstream(cuda, n)
+    loss, dx, dw = own(x, w, t, up, z=1e-3)
+    want, rx, rw, b, bx, bw, _ = live_reference(x, w, t, up, 0.0, z=1e-3)
+    within(loss, want, b, "loss")
+    within(dx, rx, bx, "dx")
+    within(dw, rw, bw, "dw")

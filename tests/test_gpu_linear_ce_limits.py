@@ -186,3 +186,22 @@ def test_exact_logits_of_many_columns(cuda, n, d, v, dtype):
     within(loss, want, b, "loss")
     within(dx, rx, bx, "dx")
     within(dw, rw, bw, "dw")
+
+
+# ---------------------------------------------------------------------------
+# Rows that are not finite
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_row_that_is_not_finite_stays_alone(cuda, value, dtype):
+    print(f"case linear not finite {value} {dtype}", flush=True)
+    x, w, t = linear_inputs(cuda, 90, 64, 300, dtype, seed=31)
+    up = upstream(cuda, 90)
+    bad_x = x.clone()
+    bad_x[11, 5] = value
+    loss, dx, dw = own(bad_x, w, t, up)
+    rows = torch.arange(90, device=cuda) != 11
+    want, rx, _, b, bx, _, _ = live_reference(x[rows], w, t[rows], up[rows], logit_error(x[rows], w))
+    within(loss[rows], want, b, "loss")
+    within(dx[rows], rx, bx, "dx")
+    assert not torch.isfinite(loss[11]) and dx[11].isnan().all() and not torch.isfinite(dw[:, 5]).any()

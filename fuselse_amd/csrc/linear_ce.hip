@@ -159,17 +159,6 @@ __device__ __forceinline__ int dx_splits(const PlanArgs& p, int live) {
     return (int)(best & 127);
 }
 
-// fp32: the largest finite magnitudes of the live rows of x and of w, from which
-// the logits' operands are scaled: a block's of its share of the rows, in mag.
-struct MagArgs {
-    const float* x;
-    int64_t ldx;
-    const float* w;
-    int64_t ldw, d;
-    float* mag;             // [x_blocks + w_blocks]
-    int x_blocks, w_blocks;
-};
-
 __device__ __forceinline__ float wave_max(float v) {
     v = fmaxf(v, reduce_partner<1>(v));
     v = fmaxf(v, reduce_partner<2>(v));
@@ -187,42 +176,6 @@ __device__ __forceinline__ float block_max(float v, float* sh) {
     v = sh[0];
     for (int w = 1; w < THREADS / 64; ++w) v = fmaxf(v, sh[w]);
     return v;
-}
-
-__device__ __forceinline__ void magnitudes(const PlanArgs& p, const MagArgs& m, int block) {
-    const bool is_x = block < m.x_blocks;
-    const int64_t n = is_x ? p.n : p.v;
-    const int64_t b = is_x ? block : block - m.x_blocks, blocks = is_x ? m.x_blocks : m.w_blocks;
-    float big = 0.0f;
-    auto take = [&](const float (&v)[4]) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const float a = __builtin_fabsf(v[k]);
-            big = a < kInf ? fmaxf(big, a) : big;
-        }
-    };
-    // a wave a row, four vectors a lane in flight
-    constexpr int kWaves = kPlanThreads / 64;
-    for (int64_t r = b * kWaves + (threadIdx.x >> 6); r < n; r += blocks * kWaves) {
-        if (is_x && p.target[r] == p.ignore) continue;
-        const float* s = is_x ? m.x + r * m.ldx : m.w + r * m.ldw;
-        int64_t c = (int64_t)lane_id() * 4;
-        for (; c + 3 * 256 + 4 <= m.d; c += 4 * 256) {
-            float v[4][4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) load_vec_any<float>(s + c + k * 256, v[k]);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) take(v[k]);
-        }
-        for (; c < m.d; c += 256) {
-            float v[4];
-            load_vec_part<float>(s + c, m.d - c, 0.0f, v);
-            take(v);
-        }
-    }
-    __shared__ float sh[kWaves];
-    big = block_max<kPlanThreads>(big, sh);
-    if (threadIdx.x == 0) m.mag[block] = big;
 }
 
 // Live rows by their targets' groups of 64 vocabulary entries, a wave a group: an
@@ -279,12 +232,11 @@ __device__ __forceinline__ void target_lists(const PlanArgs& p, int block) {
     p.rest_row[lo + lane] = comes ? begin + __popcll(there & ((1ull << lane) - 1)) : -1;
 }
 
-// Block 0 makes the plan; blocks after it take the magnitudes or the lists.
+// Block 0 makes the plan; blocks after it take the lists.
 template <bool BWD>
-__global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs p, MagArgs m) {
+__global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs p) {
     if (blockIdx.x > 0) {
-        if (m.mag) magnitudes(p, m, (int)blockIdx.x - 1);
-        else target_lists(p, (int)blockIdx.x - 1);
+        target_lists(p, (int)blockIdx.x - 1);
         return;
     }
     __shared__ int sh[kPlanThreads / 64];
@@ -340,25 +292,21 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs p, MagArgs 
         }
     }
     if (threadIdx.x == 0) p.head->live = live;
+    if constexpr (!BWD) {
+        if (p.lse_out && threadIdx.x < 2) p.lse_out[p.n + threadIdx.x] = 0.0f;
+    }
 }
 
-// The scale of fp32 logits' operands, and the exponent that undoes both in a
-// logit (as one step: one of the two may leave the type's range where both
-// together do not); big holds the magnitudes of x and of w.
-__device__ __forceinline__ float operand_scale(float big) { return __builtin_ldexpf(1.0f, scale_exp(big, 15)); }
+// fp32 logits: `undo` takes back both operands' rows' scales (as one step: one of
+// the two may leave the type's range where both together do not).
 template <int DT>
 __device__ __forceinline__ float logit(float acc, int undo) {
     return DT == kF32 ? __builtin_ldexpf(acc, undo) : acc;
 }
-template <int DT>
-__device__ __forceinline__ int logit_scale(const float* big) {
-    return DT == kF32 ? -scale_exp(big[0], 15) - scale_exp(big[1], 15) : 0;
-}
 
 // ---------------------------------------------------------------------------
 // Packing: the live rows of x and a piece's rows of w as 16-bit operands of ldp
-// elements (a multiple of 64), zero beyond D; 8 elements a thread.  fp32 rows
-// are written for the logits and, where `grads` is not NULL, for dx and dw.
+// elements (a multiple of 64), zero beyond D; 8 elements a thread at a time.
 // ---------------------------------------------------------------------------
 struct PackSide {
     const void* src;   // NULL: nothing to pack
@@ -366,17 +314,29 @@ struct PackSide {
     const int* rows;   // x: the live rows
     uint16_t* logits;
     int64_t logits_part;
+    // fp32: parts for dx and dw (NULL: not wanted), and a row's undoing exponent
     uint16_t* grads;
     int64_t grads_part;
+    int8_t* undo;
 };
 struct PackArgs {
     PackSide x, w;
     const Head* head;
     int64_t d, ldp;
-    float* big;        // fp32: magnitudes of x and w
-    const float* mag;  // forward, first piece: where they come from
-    int x_blocks, w_blocks;
+    int lanes;         // fp32: of a row
 };
+
+template <typename T>
+__device__ __forceinline__ void load8(const T* src, int64_t left, float (&v)[8]) {
+    constexpr int VE = Elem<T>::kVec;
+#pragma unroll
+    for (int h = 0; h < 8; h += VE) {
+        float t[VE];
+        load_vec_part<T>(src + h, left - h, 0.0f, t);
+#pragma unroll
+        for (int k = 0; k < VE; ++k) v[h + k] = t[k];
+    }
+}
 
 template <int DT, int P>
 __device__ __forceinline__ void store_parts(const float (&v)[8], float scale, uint16_t* dst, int64_t part) {
@@ -392,27 +352,10 @@ __device__ __forceinline__ void store_parts(const float (&v)[8], float scale, ui
     }
 }
 
+// fp16 and bf16.
 template <int DT>
 __global__ __launch_bounds__(256) void pack(PackArgs p) {
     typedef typename Io<DT>::T T;
-    constexpr int VE = Elem<T>::kVec;
-    float big_x = 0.0f, big_w = 0.0f;
-    if constexpr (DT == kF32) {
-        if (p.mag) {
-            __shared__ float sh[2][4];
-            for (int k = threadIdx.x; k < p.x_blocks; k += 256) big_x = fmaxf(big_x, p.mag[k]);
-            for (int k = threadIdx.x; k < p.w_blocks; k += 256) big_w = fmaxf(big_w, p.mag[p.x_blocks + k]);
-            big_x = block_max<256>(big_x, sh[0]);
-            big_w = block_max<256>(big_w, sh[1]);
-            if (blockIdx.x == 0 && threadIdx.x == 0) {
-                p.big[0] = big_x;
-                p.big[1] = big_w;
-            }
-        } else {
-            big_x = p.big[0];
-            big_w = p.big[1];
-        }
-    }
     const int64_t chunks = p.ldp / 8;
     int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     const bool is_x = i < p.x.n * chunks;
@@ -420,18 +363,57 @@ __global__ __launch_bounds__(256) void pack(PackArgs p) {
     if (!is_x) i -= p.x.n * chunks;
     const int64_t r = i / chunks, c = i % chunks * 8;
     if (r >= (is_x ? (int64_t)p.head->live : s.n)) return;
-    const T* src = static_cast<const T*>(s.src) + (s.rows ? (int64_t)s.rows[r] : r) * s.ld + c;
     float v[8];
+    load8(static_cast<const T*>(s.src) + (s.rows ? (int64_t)s.rows[r] : r) * s.ld + c, p.d - c, v);
+    store_parts<DT, 1>(v, 1.0f, s.logits + r * p.ldp + c, s.logits_part);
+}
+
+// fp32: a group of lanes takes a row's largest finite magnitude, and with it the
+// row's scale, then writes the row for the logits and, where `grads` is not
+// NULL, for dx and dw.  Up to C of a lane's chunks stay in registers; longer
+// rows are read twice, the second time from the caches.
+template <int C>
+__global__ __launch_bounds__(256) void pack_f32(PackArgs p) {
+    const int sub = (int)threadIdx.x % p.lanes;
+    int64_t r = (int64_t)blockIdx.x * (256 / p.lanes) + (int)threadIdx.x / p.lanes;
+    const bool is_x = r < p.x.n;
+    const PackSide& s = is_x ? p.x : p.w;
+    if (!is_x) r -= p.x.n;
+    if (r >= (is_x ? (int64_t)p.head->live : s.n)) return;  // whole groups
+    const float* src = static_cast<const float*>(s.src) + (s.rows ? (int64_t)s.rows[r] : r) * s.ld;
+    const int64_t first = sub * 8, step = p.lanes * 8;
+    float kept[C][8], big = 0.0f;
+    auto take = [&](const float (&v)[8]) {
 #pragma unroll
-    for (int h = 0; h < 8; h += VE) {
-        float t[VE];
-        load_vec_part<T>(src + h, p.d - c - h, 0.0f, t);
+        for (int k = 0; k < 8; ++k) {
+            const float a = __builtin_fabsf(v[k]);
+            big = a < kInf ? fmaxf(big, a) : big;
+        }
+    };
 #pragma unroll
-        for (int k = 0; k < VE; ++k) v[h + k] = t[k];
+    for (int j = 0; j < C; ++j) load8(src + first + j * step, p.d - first - j * step, kept[j]);
+#pragma unroll
+    for (int j = 0; j < C; ++j) take(kept[j]);
+    for (int64_t c = first + C * step; c < p.ldp; c += step) {
+        float v[8];
+        load8(src + c, p.d - c, v);
+        take(v);
     }
-    store_parts<DT, Logits<DT>::kParts>(v, operand_scale(is_x ? big_x : big_w), s.logits + r * p.ldp + c, s.logits_part);
-    if constexpr (DT == kF32) {
-        if (s.grads) store_parts<DT, Grads<DT>::kParts>(v, 1.0f, s.grads + r * p.ldp + c, s.grads_part);
+    for (int d = 1; d < p.lanes; d *= 2) big = fmaxf(big, __shfl_xor(big, d, 64));
+    const int e = scale_exp(big, 15);
+    const float scale = __builtin_ldexpf(1.0f, e);
+    if (sub == 0) s.undo[r] = (int8_t)-e;
+    auto put = [&](int64_t c, const float (&v)[8]) {
+        store_parts<kF32, 2>(v, scale, s.logits + r * p.ldp + c, s.logits_part);
+        if (s.grads) store_parts<kF32, 3>(v, 1.0f, s.grads + r * p.ldp + c, s.grads_part);
+    };
+#pragma unroll
+    for (int j = 0; j < C; ++j)
+        if (first + j * step < p.ldp) put(first + j * step, kept[j]);
+    for (int64_t c = first + C * step; c < p.ldp; c += step) {
+        float v[8];
+        load8(src + c, p.d - c, v);
+        put(c, v);
     }
 }
 
@@ -465,6 +447,28 @@ struct Place {
 
 constexpr int perm_at(int i, int q) { return i / 2 * 32 + i % 2 * 4 + q; }
 
+// fp32: what undoes the scales of a lane's permuted rows of w, perm_at(i, q) from
+// `from` on, for FM fragments (past the piece: of no meaning, in the buffer).
+// A byte each, since as whole registers they spilled, and loaded before the tile's
+// products: at their end the loads stand behind the next tile's, and G of
+// (2048, 1024, 16128) took 198 us for 180.
+template <int DT, int FM>
+struct Undo {
+    uint2 e[DT == kF32 ? FM / 2 : 1];
+    __device__ __forceinline__ void load(const int8_t* from) {
+        if constexpr (DT == kF32) {
+#pragma unroll
+            for (int i = 0; i < FM; i += 2) e[i / 2] = *reinterpret_cast<const uint2*>(from + perm_at(i, 0));
+        }
+    }
+    // of the lane's result k = 4 i + q
+    __device__ __forceinline__ int at(int k) const {
+        if constexpr (DT != kF32) return 0;
+        const uint32_t word = k & 4 ? e[k / 8].y : e[k / 8].x;
+        return (int8_t)(word >> 8 * (k & 3));
+    }
+};
+
 struct StatArgs {
     Operand w, x;      // M: vocabulary rows, N: live rows
     int steps;
@@ -475,7 +479,7 @@ struct StatArgs {
     float2* part;      // [live row][parts]: (max, sum)
     int64_t parts;
     float* at_target;  // [live row]
-    const float* big;
+    const int8_t *undo_w, *undo_x;  // fp32: of the piece's rows, of the live rows
 };
 
 template <int DT, class S>
@@ -483,12 +487,12 @@ struct StatJob {
     StatArgs p;
     int live;
     int tiles_n;
-    int undo;
 
     typedef Side<S, S::TM, true> SA;
     typedef Side<S, S::TN, true> SB;
     struct Rows {
-        int target[S::FN];
+        int target[S::FN], undo_x[DT == kF32 ? S::FN : 1];
+        Undo<DT, S::FM> undo_w;
     };
     __device__ __forceinline__ void place(int t, SA& A, SB& B) const {
         const TileAt tile = tile_at(t, p.tiles_m, tiles_n);
@@ -498,10 +502,16 @@ struct StatJob {
     __device__ __forceinline__ int first(int) const { return 0; }
     __device__ __forceinline__ int steps(int) const { return p.steps; }
     __device__ __forceinline__ Rows rows(int t) const {
-        const Place<S> at(0, tile_at(t, p.tiles_m, tiles_n).n * S::TN);
+        const TileAt tile = tile_at(t, p.tiles_m, tiles_n);
+        const Place<S, true> at(tile.m * S::TM, tile.n * S::TN);
         Rows r;
+        r.undo_w.load(p.undo_w + at.m);
 #pragma unroll
-        for (int j = 0; j < S::FN; ++j) r.target[j] = at.n + j * 16 < live ? p.tgt[at.n + j * 16] : -1;
+        for (int j = 0; j < S::FN; ++j) {
+            const int n = at.n + j * 16;
+            r.target[j] = n < live ? p.tgt[n] : -1;
+            if constexpr (DT == kF32) r.undo_x[j] = n < live ? p.undo_x[n] : 0;
+        }
         return r;
     }
     __device__ __forceinline__ void finish(int t, const Rows& r, const f32x4 (&acc)[S::FM][S::FN]) const {
@@ -512,13 +522,14 @@ struct StatJob {
 #pragma unroll
         for (int j = 0; j < S::FN; ++j) {
             const int64_t n = at.n + j * 16;
+            const int undo_x = DT == kF32 ? r.undo_x[j] : 0;
             const int hit = r.target[j] >= 0 && r.target[j] < p.v0 + p.v ? r.target[j] - p.v0 - at.m : -1;
             float v[S::FM * 4];
 #pragma unroll
             for (int i = 0; i < S::FM; ++i)
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
-                    const float l = logit<DT>(acc[i][j][q], undo);
+                    const float l = logit<DT>(acc[i][j][q], r.undo_w.at(i * 4 + q) + undo_x);
                     v[i * 4 + q] = perm_at(i, q) < left ? l : -kInf;
                     if (perm_at(i, q) == hit) p.at_target[n] = l;
                 }
@@ -538,7 +549,6 @@ __global__ __launch_bounds__(S::kThreads, 2) void logits_stats(StatArgs p) {
     StatJob<DT, S> job{p, p.head->live};
     job.p.x.rows = job.live;
     job.tiles_n = (job.live + S::TN - 1) / S::TN;
-    job.undo = logit_scale<DT>(p.big);
     run_tiles<S, true, true, Logits<DT>::kHalf, Logits<DT>::kParts>(job, p.tiles_m * job.tiles_n, (lds_char*)buf0,
                                                                     (lds_char*)buf1);
 }
@@ -804,7 +814,7 @@ struct GradArgs {
     int tiles_m;
     uint16_t* g;         // [live row][ldg]
     int64_t ldg, g_part;
-    const float* big;
+    const int8_t *undo_w, *undo_x;  // fp32: of the piece's rows, of the live rows
     float* rest;         // fp16, bf16: [live row] what rounding took off the target's entry
 };
 
@@ -815,12 +825,12 @@ struct GradJob {
     GradArgs p;
     int live;
     int tiles_n;
-    int undo;
 
     typedef Side<S, S::TM, true> SA;
     typedef Side<S, S::TN, true> SB;
     struct Rows {
-        int target[S::FN];
+        int target[S::FN], undo_x[DT == kF32 ? S::FN : 1];
+        Undo<DT, S::FM> undo_w;
         float a[S::FN], b[S::FN], lse[S::FN];
     };
     __device__ __forceinline__ void place(int t, SA& A, SB& B) const {
@@ -831,8 +841,10 @@ struct GradJob {
     __device__ __forceinline__ int first(int) const { return 0; }
     __device__ __forceinline__ int steps(int) const { return p.steps; }
     __device__ __forceinline__ Rows rows(int t) const {
-        const Place<S> at(0, tile_at(t, p.tiles_m, tiles_n).n * S::TN);
+        const TileAt tile = tile_at(t, p.tiles_m, tiles_n);
+        const Place<S, true> at(tile.m * S::TM, tile.n * S::TN);
         Rows r;
+        r.undo_w.load(p.undo_w + at.m);
 #pragma unroll
         for (int j = 0; j < S::FN; ++j) {
             const int64_t n = at.n + j * 16;
@@ -841,6 +853,7 @@ struct GradJob {
             r.a[j] = in ? p.a[n] : 0.0f;
             r.b[j] = in ? p.b[n] : 0.0f;
             r.lse[j] = in ? p.lse[n] : 0.0f;
+            if constexpr (DT == kF32) r.undo_x[j] = in ? p.undo_x[n] : 0;
         }
         return r;
     }
@@ -856,6 +869,7 @@ struct GradJob {
             const int hit = r.target[j] >= 0 ? r.target[j] - p.v0 - at.m : -1;
             // rows past the live ones have a = 0, but an exponential of anything
             const int cols = n < live ? left : 0;
+            const int undo_x = DT == kF32 ? r.undo_x[j] : 0;
             float hit_g = 0.0f;
 #pragma unroll
             for (int i = 0; i < S::FM; i += 2) {
@@ -863,7 +877,7 @@ struct GradJob {
 #pragma unroll
                 for (int q = 0; q < 8; ++q) {
                     const int m = perm_at(i, q);  // q runs over both fragments
-                    float g = r.a[j] * fexp2((logit<DT>(acc[i + q / 4][j][q % 4], undo) - r.lse[j]) * kLog2e);
+                    float g = r.a[j] * fexp2((logit<DT>(acc[i + q / 4][j][q % 4], r.undo_w.at(i * 4 + q) + undo_x) - r.lse[j]) * kLog2e);
                     if (m == hit) hit_g = g += r.b[j];
                     to_parts<DT>(m < cols ? g : 0.0f, o[q]);
                 }
@@ -892,7 +906,6 @@ __global__ __launch_bounds__(S::kThreads, 2) void logits_grad(GradArgs p) {
     GradJob<DT, S> job{p, p.head->live};
     job.p.x.rows = job.live;
     job.tiles_n = (job.live + S::TN - 1) / S::TN;
-    job.undo = logit_scale<DT>(p.big);
     run_tiles<S, true, true, Logits<DT>::kHalf, Logits<DT>::kParts>(job, p.tiles_m * job.tiles_n, (lds_char*)buf0,
                                                                     (lds_char*)buf1);
 }
@@ -1188,11 +1201,10 @@ struct Layout {
     bool pack_w;         // w is packed a piece at a time
     int splits;          // of K in dx, with every row live
     int64_t room;        // rows of its sums
-    int x_blocks, w_blocks;  // fp32: blocks that take the magnitudes
     int few;             // forward of few rows: its blocks, or 0
     int logits, dx, dw;  // the products' tiles: 256, 128 or 64
     int dw_splits;
-    int64_t head, rows, pos, tgt, at_target, loss_rows, part, parts, a, b, lse, xp, xg, wp, wg, mag, big, rest, list,
+    int64_t head, rows, pos, tgt, at_target, loss_rows, part, parts, a, b, lse, xp, xg, wp, wg, undo_x, undo_w, rest, list,
         list_at, rest_row, rests, dw_acc, g, acc, bytes;
 };
 
@@ -1257,10 +1269,8 @@ Layout layout(int64_t N, int64_t V, int64_t D, int dtype, bool bwd, bool alone, 
     l.tgt = take(4 * N);
     l.xp = take(l.few ? 0 : 2 * lparts * N * l.ldx);
     l.wp = take(l.pack_w ? 2 * lparts * l.piece * l.ldx : 0);
-    l.x_blocks = dtype == kF32 && !bwd && !l.few ? (int)(div_up(N, 16) < 32 ? div_up(N, 16) : 32) : 0;
-    l.w_blocks = dtype == kF32 && !bwd && !l.few ? (int)(div_up(V, 16) < 256 ? div_up(V, 16) : 256) : 0;
-    l.mag = take(4 * (l.x_blocks + l.w_blocks));
-    l.big = take(8);
+    l.undo_x = take(dtype == kF32 && !l.few ? N : 0);
+    l.undo_w = take(dtype == kF32 && !l.few ? l.piece : 0);
     l.logits = tile_size(l.piece, N);
     if (!bwd) {
         l.parts = l.few ? l.few * kFewWaves : div_up(V, l.logits / 2);
@@ -1323,23 +1333,18 @@ struct Operands {
 // Packs what has to be packed for the piece at v0 (x with the first piece) and
 // sets up its operands.
 template <int DT>
-void operands(const Call& c, const Layout& l, int64_t v0, int64_t rows, bool dx, bool dw, bool fwd, float* big,
-              Operands& o) {
+void operands(const Call& c, const Layout& l, int64_t v0, int64_t rows, bool dx, bool dw, Operands& o) {
     typedef typename Io<DT>::T T;
     const T* w = static_cast<const T*>(c.w) + v0 * c.ldw;
     PackArgs p{};
     p.head = at<Head>(c, l.head);
     p.d = c.D;
     p.ldp = l.ldx;
-    p.big = big;
-    if (fwd && v0 == 0) p.mag = at<float>(c, l.mag);
-    p.x_blocks = l.x_blocks;
-    p.w_blocks = l.w_blocks;
     if (v0 == 0) {
         const int64_t part = c.N * l.ldx;
         uint16_t* to = at<uint16_t>(c, l.xp);
         o.x = o.xg = Operand{to, l.ldx, part, (int)c.N, l.ldx};
-        p.x = PackSide{c.x, c.ldx, c.N, at<int>(c, l.rows), to, part, nullptr, part};
+        p.x = PackSide{c.x, c.ldx, c.N, at<int>(c, l.rows), to, part, nullptr, part, at<int8_t>(c, l.undo_x)};
         if (DT == kF32 && dw) p.x.grads = at<uint16_t>(c, l.xg);
         if (DT == kF32) o.xg.p = p.x.grads;
     }
@@ -1347,14 +1352,23 @@ void operands(const Call& c, const Layout& l, int64_t v0, int64_t rows, bool dx,
         const int64_t part = l.piece * l.ldx;
         uint16_t* to = at<uint16_t>(c, l.wp);
         o.w = o.wg = Operand{to, l.ldx, part, (int)rows, l.ldx};
-        p.w = PackSide{w, c.ldw, rows, nullptr, to, part, nullptr, part};
+        p.w = PackSide{w, c.ldw, rows, nullptr, to, part, nullptr, part, at<int8_t>(c, l.undo_w)};
         if (DT == kF32 && dx) p.w.grads = at<uint16_t>(c, l.wg);
         if (DT == kF32) o.wg.p = p.w.grads;
     } else {
         o.w = o.wg = Operand{reinterpret_cast<const uint16_t*>(w), c.ldw, 0, (int)rows, l.ldx};
     }
-    const int64_t threads = (p.x.n + p.w.n) * (l.ldx / 8);
-    if (threads > 0) pack<DT><<<dim3((unsigned)div_up(threads, 256)), 256, 0, c.s>>>(p);
+    const int64_t packed = p.x.n + p.w.n;
+    if (packed == 0) return;
+    if constexpr (DT == kF32) {
+        p.lanes = 8;  // a row is 64 elements at least
+        while (p.lanes < 64 && p.lanes * 8 < l.ldx) p.lanes *= 2;
+        const dim3 grid((unsigned)div_up(packed * p.lanes, 256));
+        if (l.ldx <= 512) pack_f32<1><<<grid, 256, 0, c.s>>>(p);
+        else pack_f32<2><<<grid, 256, 0, c.s>>>(p);
+    } else {
+        pack<DT><<<dim3((unsigned)div_up(packed * (l.ldx / 8), 256)), 256, 0, c.s>>>(p);
+    }
 }
 
 // Blocks for `tiles` tiles: no more than run at a time, in multiples of 8.
@@ -1388,21 +1402,12 @@ PlanArgs plan_args(const Call& c, const Layout& l) {
 }
 
 template <int DT>
-MagArgs mag_args(const Call& c, const Layout& l) {
-    if constexpr (DT != kF32) return MagArgs{};
-    return MagArgs{static_cast<const float*>(c.x), c.ldx,      static_cast<const float*>(c.w), c.ldw, c.D,
-                   at<float>(c, l.mag),            l.x_blocks, l.w_blocks};
-}
-
-template <int DT>
 void run_fwd(const Call& c, const Layout& l, float* loss, float* lse) {
     PlanArgs p = plan_args(c, l);
     p.loss_rows = c.reduction == 0 ? loss : at<float>(c, l.loss_rows);
     p.lse_out = lse;
-    plan_kernel<false><<<dim3((unsigned)(1 + l.x_blocks + l.w_blocks)), kPlanThreads, 0, c.s>>>(
-        p, mag_args<DT>(c, l));
+    plan_kernel<false><<<1, kPlanThreads, 0, c.s>>>(p);
     Operands o{};
-    float* big = lse ? lse + c.N : at<float>(c, l.big);
     for (int64_t v0 = 0; v0 < c.V; v0 += l.piece) {
         const int64_t rows = c.V - v0 < l.piece ? c.V - v0 : l.piece;
         if (l.few) {
@@ -1418,11 +1423,12 @@ void run_fwd(const Call& c, const Layout& l, float* loss, float* lse) {
             }
             break;  // one piece
         }
-        operands<DT>(c, l, v0, rows, false, false, true, big, o);
+        operands<DT>(c, l, v0, rows, false, false, o);
         StatArgs a{};
         a.w = o.w;
         a.x = o.x;
-        a.big = big;
+        a.undo_w = at<int8_t>(c, l.undo_w);
+        a.undo_x = at<int8_t>(c, l.undo_x);
         a.steps = (int)(l.ldx / kStep);
         a.head = p.head;
         a.tgt = p.tgt;
@@ -1466,17 +1472,17 @@ void run_bwd(const Call& c, const Layout& l, const float* grad, const float* lse
     p.rest_row = at<int>(c, l.rest_row);
     p.groups = DT != kF32 && dw ? (int)div_up(c.V, kGroup) : 0;
     const int64_t beside = div_up(p.groups, kPlanThreads / 64);
-    plan_kernel<true><<<dim3((unsigned)(1 + beside)), kPlanThreads, 0, c.s>>>(p, MagArgs{});
+    plan_kernel<true><<<dim3((unsigned)(1 + beside)), kPlanThreads, 0, c.s>>>(p);
     Operands o{};
-    float* big = const_cast<float*>(lse) + c.N;  // the forward's; not written here
     const int64_t g_part = round_up(c.N, 64) * l.piece;
     for (int64_t v0 = 0; v0 < c.V; v0 += l.piece) {
         const int64_t rows = c.V - v0 < l.piece ? c.V - v0 : l.piece;
-        operands<DT>(c, l, v0, rows, dx != nullptr, dw != nullptr, false, big, o);
+        operands<DT>(c, l, v0, rows, dx != nullptr, dw != nullptr, o);
         GradArgs g{};
         g.w = o.w;
         g.x = o.x;
-        g.big = big;
+        g.undo_w = at<int8_t>(c, l.undo_w);
+        g.undo_x = at<int8_t>(c, l.undo_x);
         g.rest = at<float>(c, l.rest);
         g.steps = (int)(l.ldx / kStep);
         g.head = p.head;

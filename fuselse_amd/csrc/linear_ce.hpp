@@ -26,9 +26,10 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 // number.
 //
 // Logits: two fp16 parts of 11 bits, taken after a power of two that brings the
-// tensor's largest finite magnitude to [2^14, 2^15).  An element is then exact
-// to 2^-23 of itself or 2^-39 of the largest, whichever is more; three partial
-// products, the one left out below 2^-22 of the product.
+// row's largest finite magnitude to [2^14, 2^15).  An element is then exact to
+// 2^-23 of itself or 2^-39 of its row's largest, whichever is more; three partial
+// products, the one left out below 2^-22 of the product.  A scale a row, so that
+// no row's result depends on another row's size.
 //
 // dx and dw: three bf16 parts of 8 bits, to nearest: exact at any magnitude,
 // which G, whose entries reach from 1 down to nothing, needs and fp16's

@@ -899,8 +899,7 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
                          reduction: str = "mean", z_loss: float = 0.0, with_lse: bool = True):
     """Softmax cross entropy of the logits x @ weight.T, which are never
     stored: (loss, lse) in fp32; lse (N + 2,) holds the rows' log-sum-exps and
-    two values more for the backward, or is None without with_lse, which few
-    rows take less time for.  x (N, D) and
+    two zeros, or is None without with_lse, which few rows take less time for.  x (N, D) and
     weight (V, D) fp32, fp16 or bf16 with contiguous rows, target int64 (N,).
     loss[n] = lse[n] - x[n] . weight[target[n]] + z_loss * lse[n]^2; rows whose
     target is ignore_index have loss 0 and are not read."""

@@ -348,14 +348,14 @@ int fl_sparse_blocked_grad(const float* node_flows, const float* node_mars, cons
  * other target outside [0, V) makes the row's loss NaN, and with it the
  * gradients it takes part in.  Products of fp16 and bf16 are exact, of fp32
  * to about 2^-21 (an element's digits below 2^-39 of the largest magnitude
- * in its tensor do not enter the logits; one that is not finite, or within
+ * in its row do not enter the logits; one that is not finite, or within
  * 2^-9 of the type's largest, makes NaN of the gradients it enters); sums are
  * fp32.
  *
  * fl_linear_ce_fwd: loss fp32 [N] (reduction 0) or [1]; lse fp32
- *   [N + 2], the rows' log-sum-exps (0 for ignored ones) and two values more
- *   for the backward, or NULL where none follows (few rows then take less
- *   time).  A mean over no rows is 0.
+ *   [N + 2], the rows' log-sum-exps (0 for ignored ones) and two zeros, or
+ *   NULL where no backward follows (few rows then take less time).  A mean
+ *   over no rows is 0.
  * fl_linear_ce_bwd: grad fp32 [N] (reduction 0) or [1]; lse as the forward
  *   wrote it.  dx [N, D] and dw [V, D] contiguous, of x's type; either may be
  *   NULL.  The softmax gradient enters the products rounded once to x's type

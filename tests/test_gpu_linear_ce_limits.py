@@ -70,6 +70,39 @@ def upstream(cuda, n, seed=1):
 
 
 # ---------------------------------------------------------------------------
+# Rows of very different magnitudes
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("e", [20, 30, 60])
+@pytest.mark.parametrize("n,d,v", [(80, 64, 300), (140, 200, 1031), (700, 130, 5000)])
+def test_one_large_row_leaves_the_others_their_digits(cuda, n, d, v, e):
+    """fp32: a row of x and a row of w 2^e times the others'.  The large row of
+    w has logits that underflow in every softmax, so that the other rows'
+    losses and gradients are those without either."""
+    print(f"case linear large row {n} {d} {v} {e}", flush=True)
+    x, w, t = linear_inputs(cuda, n, d, v, torch.float32, seed=e)
+    x = x.abs() + 0.25
+    t[t == 5] = 6
+    big_x, big_w = x.clone(), w.clone()
+    big_x[3] *= 2.0 ** e
+    big_w[5] = -(w[5].abs() + 0.25) * 2.0 ** e
+    up = upstream(cuda, n)
+    loss, dx, dw = own(big_x, big_w, t, up)
+    rows = torch.arange(n, device=cuda) != 3
+    others = torch.arange(v, device=cuda) != 5
+    ts = torch.where(t > 5, t - 1, t)
+    want, rx, _, b, bx, _, _ = live_reference(x[rows], w[others], ts[rows], up[rows], logit_error(x[rows], w[others]))
+    within(loss[rows], want, b, "loss")
+    within(dx[rows], rx, bx, "dx")
+    plain = fuselse_amd.linear_cross_entropy(big_x, big_w, t, reduction="none")
+    within(plain[rows], want, b, "loss without gradients")
+    # dw without the large row's part: its upstream gradient is 0
+    up[3] = 0.0
+    _, _, dw = own(big_x, big_w, t, up)
+    _, _, rw, _, _, bw, _ = live_reference(x[rows], w[others], ts[rows], up[rows], logit_error(x[rows], w[others]))
+    within(dw[others], rw, bw, "dw")
+
+
+# ---------------------------------------------------------------------------
 # Several pieces of the vocabulary
 # ---------------------------------------------------------------------------
 def assert_several_pieces(n, d, v, dtype, w):

@@ -763,25 +763,30 @@ __global__ __launch_bounds__(kFewWaves * 64) void logits_few(FewArgs p) {
     }
 }
 
-// Joins a live row's pairs; one wave a row.
-__global__ __launch_bounds__(256) void finish_rows(const Head* head, const int* rows, const int* tgt,
-                                                   const float2* part, int64_t parts, const float* at_target, float z,
-                                                   float* loss_rows, float* lse_out) {
+// Joins a live row's pairs begin .. end - 1; one wave a row.  With `more` pieces to
+// come the joined pair goes to the row's first place.
+__global__ __launch_bounds__(256) void finish_rows(const Head* head, const int* rows, const int* tgt, float2* part,
+                                                   int64_t parts, int64_t begin, int64_t end, bool more,
+                                                   const float* at_target, float z, float* loss_rows, float* lse_out) {
     const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (r >= head->live) return;
     const int lane = threadIdx.x & 63;
     float m = -kInf, s = 0.0f;
     // the pairs lie in other XCDs' memory: eight loads a lane in flight
     constexpr int U = 8;
-    for (int64_t k0 = lane; k0 < parts; k0 += 64 * U) {
+    for (int64_t k0 = begin + lane; k0 < end; k0 += 64 * U) {
         float2 q[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) q[u] = k0 + u * 64 < parts ? part[r * parts + k0 + u * 64] : make_float2(-kInf, 0.0f);
+        for (int u = 0; u < U; ++u) q[u] = k0 + u * 64 < end ? part[r * parts + k0 + u * 64] : make_float2(-kInf, 0.0f);
 #pragma unroll
         for (int u = 0; u < U; ++u) lse_merge(m, s, q[u].x, q[u].y);
     }
     group_merge<64>(m, s);
     if (lane == 0) {
+        if (more) {
+            part[r * parts] = make_float2(m, s);
+            return;
+        }
         const float lse = lse_finish<true>(m, s);
         const int row = rows[r];
         if (lse_out) lse_out[row] = lse;
@@ -1203,6 +1208,7 @@ struct Layout {
     int64_t room;        // rows of its sums
     int few;             // forward of few rows: its blocks, or 0
     int logits, dx, dw;  // the products' tiles: 256, 128 or 64
+    bool join;           // forward: a row's pairs are joined after every piece
     int dw_splits;
     int64_t head, rows, pos, tgt, at_target, loss_rows, part, parts, a, b, lse, xp, xg, wp, wg, undo_x, undo_w, rest, list,
         list_at, rest_row, rests, dw_acc, g, acc, bytes;
@@ -1260,7 +1266,15 @@ Layout layout(int64_t N, int64_t V, int64_t D, int dtype, bool bwd, bool alone, 
         const int64_t fit = kPieceBytes / (2 * parts * l.ldx) / 256 * 256;
         if (most > fit) most = fit < 2048 ? 2048 : fit;
     } else if (!bwd) {
-        most = V;  // nothing of the workspace grows with a forward's piece
+        most = V;
+    }
+    // A forward's pairs, 8 bytes for each row and half tile, cover the vocabulary
+    // where they fit, and else one piece beside the join of those before.  (Tiles of
+    // 64 never have that many.)
+    if (!bwd && !l.few && 8 * N * div_up(V, tile_size(V, N) / 2) > kPieceBytes) {
+        l.join = true;
+        const int64_t fit = kPieceBytes / (8 * N) * (N > 128 ? 128 : 64) / 256 * 256;
+        if (most > fit) most = fit < 2048 ? 2048 : fit;
     }
     l.piece = round_up(div_up(V, div_up(V, most)), 256);
     l.head = take(sizeof(Head));
@@ -1273,7 +1287,7 @@ Layout layout(int64_t N, int64_t V, int64_t D, int dtype, bool bwd, bool alone, 
     l.undo_w = take(dtype == kF32 && !l.few ? l.piece : 0);
     l.logits = tile_size(l.piece, N);
     if (!bwd) {
-        l.parts = l.few ? l.few * kFewWaves : div_up(V, l.logits / 2);
+        l.parts = l.few ? l.few * kFewWaves : l.join ? 1 + l.piece / (l.logits / 2) : div_up(V, l.logits / 2);
         l.at_target = take(4 * N);
         l.loss_rows = take(4 * N);
         l.part = take(8 * N * l.parts);
@@ -1408,6 +1422,12 @@ void run_fwd(const Call& c, const Layout& l, float* loss, float* lse) {
     p.lse_out = lse;
     plan_kernel<false><<<1, kPlanThreads, 0, c.s>>>(p);
     Operands o{};
+    auto finish = [&](int64_t begin, int64_t end, bool more) {
+        finish_rows<<<dim3((unsigned)div_up(c.N, 4)), 256, 0, c.s>>>(p.head, p.rows, p.tgt, at<float2>(c, l.part), l.parts,
+                                                                     begin, end, more, at<float>(c, l.at_target), c.z,
+                                                                     p.loss_rows, lse);
+    };
+    const int64_t half = l.logits / 2;
     for (int64_t v0 = 0; v0 < c.V; v0 += l.piece) {
         const int64_t rows = c.V - v0 < l.piece ? c.V - v0 : l.piece;
         if (l.few) {
@@ -1434,7 +1454,7 @@ void run_fwd(const Call& c, const Layout& l, float* loss, float* lse) {
         a.tgt = p.tgt;
         a.v0 = (int)v0;
         a.v = (int)rows;
-        a.part = at<float2>(c, l.part) + v0 / (l.logits / 2);
+        a.part = at<float2>(c, l.part) + (l.join ? 1 : v0 / half);
         a.parts = l.parts;
         a.at_target = at<float>(c, l.at_target);
         by_shape(l.logits, [&](auto shape) {
@@ -1442,9 +1462,9 @@ void run_fwd(const Call& c, const Layout& l, float* loss, float* lse) {
             a.tiles_m = (int)div_up(rows, S::TM);
             logits_stats<DT, S><<<grid_of<S>(div_up(c.N, S::TN) * a.tiles_m), S::kThreads, 0, c.s>>>(a);
         });
+        if (l.join) finish(v0 == 0, 1 + div_up(rows, half), v0 + rows < c.V);
     }
-    finish_rows<<<dim3((unsigned)div_up(c.N, 4)), 256, 0, c.s>>>(p.head, p.rows, p.tgt, at<float2>(c, l.part), l.parts,
-                                                                 at<float>(c, l.at_target), c.z, p.loss_rows, lse);
+    if (!l.join) finish(0, l.parts, false);
     if (c.reduction != 0) reduce_rows<<<1, 1024, 0, c.s>>>(p.head, p.loss_rows, c.N, p.mean, loss);
 }
 

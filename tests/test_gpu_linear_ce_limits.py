@@ -238,3 +238,31 @@ def test_a_row_that_is_not_finite_stays_alone(cuda, value, dtype):
     within(loss[rows], want, b, "loss")
     within(dx[rows], rx, bx, "dx")
     assert not torch.isfinite(loss[11]) and dx[11].isnan().all() and not torch.isfinite(dw[:, 5]).any()
+
+
+# ---------------------------------------------------------------------------
+# Forwards whose rows' pairs are joined piece by piece
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype,n,d,v", [(torch.bfloat16, 65539, 64, 70001), (torch.float16, 65539, 72, 140003),
+                                         (torch.float32, 65539, 64, 70001), (torch.bfloat16, 100, 32, 44_000_003)])
+def test_pairs_joined_piece_by_piece(cuda, dtype, n, d, v):
+    print(f"case linear join {dtype} {n} {d} {v}", flush=True)
+    x, w, t = linear_inputs(cuda, n, d, v, dtype, ignored=0.1, seed=41)
+    t[0], t[n - 1] = v - 1, 0
+    loss = fuselse_amd.linear_cross_entropy(x, w, t, reduction="none")
+    some = torch.arange(0, n, max(1, n // 99), device=cuda)
+    some[-1] = n - 1
+    xs, ts = x[some].double(), t[some]
+    lse, size = torch.full((len(some),), -math.inf, dtype=torch.float64, device=cuda), 0.0
+    for v0 in range(0, v, 1 << 20):
+        part = w[v0:v0 + (1 << 20)].double()
+        lse = torch.logaddexp(lse, torch.logsumexp(xs @ part.t(), 1))
+        size = torch.maximum((xs.abs() @ part.abs().t()).amax(1), torch.as_tensor(size, device=cuda))
+    live = ts != -100
+    want = torch.where(live, lse - (xs * w[torch.where(live, ts, 0)].double()).sum(1), 0.0)
+    dl = size * ((d / 32 + 96) * E23 + (2.0 ** -21 if dtype == torch.float32 else 0.0))
+    bound = torch.where(live, 2 * dl + 2.0 ** -15 + 2.0 ** -21 * lse.abs(), 0.0)
+    within(loss[some], want, bound, "loss")
+    # a row's loss does not depend on the rows beside it, nor on the pieces
+    few = fuselse_amd.linear_cross_entropy(x[some], w, t[some], reduction="none")
+    within(few, want, bound, "loss of some rows")

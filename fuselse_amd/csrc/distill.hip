@@ -47,22 +47,28 @@ struct FwdArgs {
     float* tlse;
 };
 
-// lse_fold of v / T with the factor in the exponent's, c = log2 e / T: m is the
-// maximum of v itself.  The exponents are c times differences from m, so that c's
-// rounding counts with the differences' size, not with the values'.
+// The state (m, s) of v / T: m is the maximum of v itself and s the sum of exponentials
+// of (v - m) c, c = log2 e / T in the exponent, so that no rounding counts with the
+// values' own size (rows of 4096 around 1000 lost 2e-5 of their sum to it).
+__device__ __forceinline__ float rescale(float from, float to, float c) {
+    return from == -kInf ? 0.0f : fexp2((lse_base(from) - lse_base(to)) * c);
+}
+
 template <int K>
 __device__ __forceinline__ void fold_scaled(float& m, float& s, const float (&v)[K], float c) {
     float mn = m;
 #pragma unroll
     for (int k = 0; k < K; ++k) mn = fmaxf(mn, v[k]);
     const float b = lse_base(mn);
-    s *= m == -kInf ? 0.0f : fexp2((lse_base(m) - b) * c);
+    s *= rescale(m, mn, c);
     m = mn;
     const float nb = -b * c;
     float acc = 0.0f;
     if (lse_fused_exp_ok(nb)) {
 #pragma unroll
         for (int k = 0; k < K; ++k) acc += fexp2(__builtin_fmaf(v[k], c, nb));
+        // nb's rounding is in every exponent, and is taken out again
+        acc *= fexp2(-__builtin_fmaf(b, c, nb));
     } else {
 #pragma unroll
         for (int k = 0; k < K; ++k) acc += fexp2((v[k] - b) * c);
@@ -70,55 +76,86 @@ __device__ __forceinline__ void fold_scaled(float& m, float& s, const float (&v)
     s += acc;
 }
 
+__device__ __forceinline__ void merge_scaled(float& m, float& s, float m2, float s2, float c) {
+    const float mn = fmaxf(m, m2);
+    s = s * rescale(m, mn, c) + s2 * rescale(m2, mn, c);
+    m = mn;
+}
+
+__device__ __forceinline__ float wave_sum(float v) {
+    v += reduce_partner<1>(v);
+    v += reduce_partner<2>(v);
+    v += reduce_partner<4>(v);
+    v += reduce_partner<8>(v);
+    v += reduce_partner<16>(v);
+    return v + reduce_partner<32>(v);
+}
+
+// Over the wave: the maximum, each lane's sum moved to it, the sum.
+__device__ __forceinline__ void wave_merge(float& m, float& s, float c) {
+    float mm = fmaxf(m, reduce_partner<1>(m));
+    mm = fmaxf(mm, reduce_partner<2>(mm));
+    mm = fmaxf(mm, reduce_partner<4>(mm));
+    mm = fmaxf(mm, reduce_partner<8>(mm));
+    mm = fmaxf(mm, reduce_partner<16>(mm));
+    mm = fmaxf(mm, reduce_partner<32>(mm));
+    s = wave_sum(s * rescale(m, mm, c));
+    m = mm;
+}
+
+// A teacher's entry; one that 1 / T takes to -inf counts as that.
+template <typename TT>
+__device__ __forceinline__ float teacher_logit(const TT* t, float inv_t) {
+    const float v = Elem<TT>::scalar(t);
+    return v * inv_t == -kInf ? -kInf : v;
+}
+
 // Joins the teacher's side of a row, in one wave: its log-sum-exp over
-// t_k / T and the loss.  Returns tlse: -inf for a row without a used entry,
+// t_k / T and the loss.  Writes tlse: -inf for a row without a used entry,
 // NaN where a used index is out of range.
 template <typename T, typename TT>
 __device__ __forceinline__ void finish_row(const FwdArgs& p, int64_t r, float sm, float ss) {
     const int lane = lane_id();
-    // log q = (x / T - maximum) - log of the sum: the log-sum-exp's own rounding, of
+    const float c = p.inv_t * kLog2e;
+    // log q = (x - maximum) / T - log of the sum: the log-sum-exp's own rounding, of
     // the maximum's size, stays out
-    const float base = lse_base(sm), rest = flog2(ss) * kLn2, lse = lse_finish<true>(sm, ss);
+    const float base = lse_base(sm), rest = flog2(ss) * kLn2;
     const TT* t = static_cast<const TT*>(p.t) + r * p.k;
     const int64_t* index = p.index + r * p.k;
     const T* x = static_cast<const T*>(p.x) + p.map.offset(r);
     float m = -kInf, s = 0.0f;
     for (int k = lane; k < p.k; k += 64) {
-        float v[1] = {Elem<TT>::scalar(t + k) * p.inv_t};
-        lse_fold<true>(m, s, v);
+        const float v = teacher_logit(t + k, p.inv_t), mn = fmaxf(m, v);
+        s = s * rescale(m, mn, c) + fexp2((v - lse_base(mn)) * c);
+        m = mn;
     }
-    group_merge<64>(m, s);
-    float tlse = lse_finish<true>(m, s);
+    wave_merge(m, s, c);
+    const float tbase = lse_base(m);
+    float trest = flog2(s) * kLn2, tlse = tbase * p.inv_t + trest;
     if (tlse == kInf) tlse = __builtin_nanf("");  // a softmax of +inf
-    const float tbase = lse_base(m), trest = tlse == tlse ? flog2(s) * kLn2 : tlse;
+    if (tlse != tlse) trest = tlse;
     float loss = 0.0f;
     if (m != -kInf || s != 0.0f) {  // a NaN never enters m, but makes s NaN
         bool bad = false;
         for (int k = lane; k < p.k; k += 64) {
-            const float tv = Elem<TT>::scalar(t + k) * p.inv_t;
+            const float tv = teacher_logit(t + k, p.inv_t);
             if (tv == -kInf) continue;
             const int64_t i = index[k];
             if (i < 0 || i >= p.v) {
                 bad = true;
                 continue;
             }
-            const float logp = (tv - tbase) - trest;
+            const float logp = (tv - tbase) * p.inv_t - trest;
             const float prob = fexp2(logp * kLog2e);
             // a probability that underflows to 0 contributes 0
-            if (prob != 0.0f) loss += prob * (logp - ((Elem<T>::scalar(x + i) * p.inv_t - base) - rest));
+            if (prob != 0.0f) loss += prob * (logp - ((Elem<T>::scalar(x + i) - base) * p.inv_t - rest));
         }
-        loss += reduce_partner<1>(loss);
-        loss += reduce_partner<2>(loss);
-        loss += reduce_partner<4>(loss);
-        loss += reduce_partner<8>(loss);
-        loss += reduce_partner<16>(loss);
-        loss += reduce_partner<32>(loss);
-        loss *= p.t2;
+        loss = wave_sum(loss) * p.t2;
         if (__ballot(bad)) loss = tlse = __builtin_nanf("");
     }
     if (lane == 0) {
         p.loss[r] = loss;
-        p.lse[r] = lse;
+        p.lse[r] = base * p.inv_t + rest;
         p.tlse[r] = tlse;
     }
 }
@@ -173,8 +210,7 @@ __global__ __launch_bounds__(kThreads) void fwd_rows(FwdArgs p) {
         load_vec_part<T>(x + e, e1 - e, -kInf, v);
         fold_scaled(m, s, v, scale);
     }
-    m *= p.inv_t;
-    group_merge<64>(m, s);
+    wave_merge(m, s, scale);
     __shared__ float sm[kThreads / 64], ss[kThreads / 64];
     if (lane_id() == 0) {
         sm[threadIdx.x >> 6] = m;
@@ -185,7 +221,7 @@ __global__ __launch_bounds__(kThreads) void fwd_rows(FwdArgs p) {
     m = sm[0];
     s = ss[0];
 #pragma unroll
-    for (int w = 1; w < kThreads / 64; ++w) lse_merge(m, s, sm[w], ss[w]);
+    for (int w = 1; w < kThreads / 64; ++w) merge_scaled(m, s, sm[w], ss[w], scale);
     if (p.segs == 1) {
         finish_row<T, TT>(p, r, m, s);
     } else if (threadIdx.x == 0) {
@@ -196,12 +232,13 @@ __global__ __launch_bounds__(kThreads) void fwd_rows(FwdArgs p) {
 template <typename T, typename TT>
 __global__ __launch_bounds__(64) void fwd_finish(FwdArgs p) {
     const int64_t r = blockIdx.x;
+    const float c = p.inv_t * kLog2e;
     float m = -kInf, s = 0.0f;
     for (int k = threadIdx.x; k < p.segs; k += 64) {
         const float2 q = p.part[r * p.segs + k];
-        lse_merge(m, s, q.x, q.y);
+        merge_scaled(m, s, q.x, q.y, c);
     }
-    group_merge<64>(m, s);
+    wave_merge(m, s, c);
     finish_row<T, TT>(p, r, m, s);
 }
 

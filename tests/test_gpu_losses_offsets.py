@@ -1,0 +1,68 @@
+"""The distillation and the router balance on logits with a large value in
+common: neither depends on it, and neither may lose digits to it.
+
+A difference from the maximum is exact where logits of a few units lie next to
+a multiple of 2^-11 in fp32; what is left is half a step an operation."""
+
+import math
+
+import pytest
+import torch
+
+import fuselse_amd
+from fuselse_amd import ext
+from test_gpu_losses import E23, u, tiny, within
+
+pytestmark = pytest.mark.gpu
+
+
+def spread(cuda, shape, offset, seed, scale=2.0):
+    """Multiples of 2^-11 of standard deviation `scale` around offset: exact in
+    fp32 up to 2^12."""
+    g = torch.Generator(device=cuda).manual_seed(seed)
+    return (torch.randn(*shape, device=cuda, generator=g) * scale * 2 ** 11).round() / 2 ** 11 + offset
+
+
+def distill_exact(s, t, i, temp, up):
+    """(losses, ds, bounds) in 64 bits of rows that all have a teacher."""
+    sd, td = s.detach().double(), t.double()
+    sd, td = sd - sd.amax(-1, keepdim=True), td - td.amax(-1, keepdim=True)
+    lq, lp = torch.log_softmax(sd / temp, -1), torch.log_softmax(td / temp, -1)
+    q, p = lq.exp(), lp.exp()
+    v, k = s.shape[-1], t.shape[-1]
+    terms = p * (lp - lq.gather(-1, i))
+    loss = temp ** 2 * terms.sum(-1)
+    # an exponent d / T is off by three roundings of its size, log2 e's and 1 / T's
+    # among them: sums by the mean of that, and by their additions (v / 256 a
+    # thread one after another, 64 for the merges); the log of a sum, its storing
+    # and its subtraction by half a step of its size each
+    step = 2.0 ** -22
+    log_sum = lambda x: torch.logsumexp(x / temp, -1) * 2.0 ** -21
+    dq = (q * sd.abs() / temp).sum(-1) * step + (v / 256 + 64) * E23 + log_sum(sd)
+    dp = (p * td.abs() / temp).sum(-1) * step + (k / 64 + 64) * E23 + log_sum(td)
+    size = (p * (lp.abs() + lq.gather(-1, i).abs())).sum(-1)
+    # a probability's error counts with the size of its term
+    err = (p * ((td.abs() / temp * step + dp[..., None]) * (1 + (lp - lq.gather(-1, i)).abs()))).sum(-1)
+    loss_b = temp ** 2 * (dq + dp + err + size * (k / 64 + 16) * E23)
+    g = up.double()[..., None] * temp
+    ps = torch.zeros_like(q).scatter_add_(-1, i, p)
+    ds = g * (q - ps)
+    pe = torch.zeros_like(q).scatter_add_(-1, i, p * (td.abs() / temp * step + dp[..., None] + 2.0 ** -21))
+    ds_b = g.abs() * (q * (sd.abs() / temp * step + dq[..., None] + 2.0 ** -21) + pe + (q + ps) * 2.0 ** -22) \
+        + u(s.dtype) * ds.abs() + 2.0 ** -126 * (1 + g.abs())
+    return loss, ds, loss_b, ds_b
+
+
+OFFSETS = [0.0, 100.0, -1000.0, 2000.0]
+
+
+@pytest.mark.parametrize("offset", OFFSETS)
+@pytest.mark.parametrize("rows,v,k,temp", [(5, 4096, 16, 1.0), (3, 50257, 200, 1.0), (33, 1001, 5, 2.0),
+                                           (2000, 300, 8, 0.7), (4, 40000, 64, 3.0)])
+def test_distillation_of_shifted_logits_loss(cuda, rows, v, k, temp, offset):
+    print(f"case distill offset loss {rows} {v} {k} {temp} {offset}", flush=True)
+    s, t = spread(cuda, (rows, v), offset, v), spread(cuda, (rows, k), -offset, k)
+    i = torch.rand(rows, v, device=cuda).argsort(-1)[:, :k].contiguous()
+    up = torch.ones(rows, device=cuda)
+    want, _, b, _ = distill_exact(s, t, i, temp, up)
+    within(fuselse_amd.topk_distillation(s, t, i, temperature=temp, reduction="none"), want, b, "loss")

@@ -74,6 +74,10 @@ SIGNATURES = {
                               _vp, _vp, _vp, ctypes.c_size_t, _vp]),
     "fl_distill_bwd": (_int, [_vp, _int, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _int, _vp, _int, _vp, _i64, _float,
                               _vp, _vp, _vp, _vp]),
+    "fl_distill_fwd_pairs": (_int, [_vp, _i64, _i64, _i64, _i64, _i64, _int, _vp, _int, _vp, _i64, _float, _int, _vp,
+                                    _vp, _vp, _vp, _vp, _vp, ctypes.c_size_t, _vp]),
+    "fl_distill_bwd_pairs": (_int, [_vp, _int, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _int, _vp, _int, _vp, _i64,
+                                    _float, _vp, _vp, _vp]),
     "fl_router_workspace_bytes": (ctypes.c_size_t, [_i64, _i64, _int]),
     "fl_router_balance_fwd": (_int, [_vp, _i64, _i64, _i64, _int, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
                                      ctypes.c_size_t, _vp]),

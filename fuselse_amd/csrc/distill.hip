@@ -45,6 +45,7 @@ struct FwdArgs {
     float* loss;
     float* lse;
     float* tlse;
+    f32x4* pairs;      // NULL: not wanted
 };
 
 // The state (m, s) of v / T: m is the maximum of v itself and s the sum of exponentials
@@ -112,7 +113,8 @@ __device__ __forceinline__ float teacher_logit(const TT* t, float inv_t) {
 
 // Joins the teacher's side of a row, in one wave: its log-sum-exp over
 // t_k / T and the loss.  Writes tlse: -inf for a row without a used entry,
-// NaN where a used index is out of range.
+// NaN where a used index is out of range; and for the backward both sides'
+// maxima and logs of sums, the teacher's with the same marks.
 template <typename T, typename TT>
 __device__ __forceinline__ void finish_row(const FwdArgs& p, int64_t r, float sm, float ss) {
     const int lane = lane_id();
@@ -151,12 +153,13 @@ __device__ __forceinline__ void finish_row(const FwdArgs& p, int64_t r, float sm
             if (prob != 0.0f) loss += prob * (logp - ((Elem<T>::scalar(x + i) - base) * p.inv_t - rest));
         }
         loss = wave_sum(loss) * p.t2;
-        if (__ballot(bad)) loss = tlse = __builtin_nanf("");
+        if (__ballot(bad)) loss = tlse = trest = __builtin_nanf("");
     }
     if (lane == 0) {
         p.loss[r] = loss;
         p.lse[r] = base * p.inv_t + rest;
         p.tlse[r] = tlse;
+        if (p.pairs) p.pairs[r] = f32x4{base, rest, tbase, trest};
     }
 }
 
@@ -284,6 +287,7 @@ struct BwdArgs {
     const int64_t* index;
     const float* lse;
     const float* tlse;
+    const f32x4* pairs;  // NULL: lse and tlse in their place
     int64_t rows, v;
     int k;
     float inv_t, temp;
@@ -324,8 +328,11 @@ __global__ __launch_bounds__(kThreads) void bwd_rows(BwdArgs p) {
     // the last chunk may have no vector, and begin behind the tail
     const int e0 = c == 0 ? 0 : body < tail ? body : tail, e1 = last ? (int)p.v : head + v1 * VE;
 
-    const float tlse = p.tlse[r];
-    const bool dead = tlse == -kInf;
+    // exponents are (x - maximum) / T - log of the sum: with the pairs no rounding
+    // counts with the logits' own size
+    const f32x4 of = p.pairs ? p.pairs[r] : f32x4{0.0f, p.lse[r], 0.0f, p.tlse[r]};
+    const float base = of[0], rest = of[1], tbase = of[2], trest = of[3];
+    const bool dead = trest == -kInf;
     u32x4 raw[kBwdVecs] = {};
     if (!dead && vecs > 0) {
 #pragma unroll
@@ -336,7 +343,6 @@ __global__ __launch_bounds__(kThreads) void bwd_rows(BwdArgs p) {
         }
     }
     const float g = dead ? 0.0f : p.grad[r * p.grad_stride] * p.temp * (p.norm ? *p.norm : 1.0f);
-    const float lse = p.lse[r];
     // the teacher's entries of this chunk, in order, found by one wave
     if (tid < 64) {
         int n = 0;
@@ -348,7 +354,7 @@ __global__ __launch_bounds__(kThreads) void bwd_rows(BwdArgs p) {
             for (int u = 0; u < U; ++u) {
                 const int k = k0 + u * 64 + tid;
                 i[u] = k < p.k ? p.index[r * p.k + k] : -1;
-                tv[u] = k < p.k ? Elem<TT>::scalar(static_cast<const TT*>(p.t) + r * p.k + k) * p.inv_t : -kInf;
+                tv[u] = k < p.k ? teacher_logit(static_cast<const TT*>(p.t) + r * p.k + k, p.inv_t) : -kInf;
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
@@ -357,7 +363,7 @@ __global__ __launch_bounds__(kThreads) void bwd_rows(BwdArgs p) {
                 if (mine) {
                     const int at = n + __popcll(b & ((1ull << tid) - 1));
                     li[at] = (int)i[u];
-                    lp[at] = g * fexp2((tv[u] - tlse) * kLog2e);
+                    lp[at] = g * fexp2(((tv[u] - tbase) * p.inv_t - trest) * kLog2e);
                 }
                 n += __popcll(b);
             }
@@ -369,8 +375,8 @@ __global__ __launch_bounds__(kThreads) void bwd_rows(BwdArgs p) {
         if (tid == 0) ln = n;
     }
     __syncthreads();
-    const float gq = tlse != tlse ? __builtin_nanf("") : g;
-    auto grad = [&](float v) { return dead ? 0.0f : gq * fexp2((v * p.inv_t - lse) * kLog2e); };
+    const float gq = trest != trest ? __builtin_nanf("") : g;
+    auto grad = [&](float v) { return dead ? 0.0f : gq * fexp2(((v - base) * p.inv_t - rest) * kLog2e); };
     // The entries' elements, each with the sum of all entries of its index, a thread
     // an entry.  (9880, 527) in fp32 with 108 entries: 60 us, for 1224 by the elements'
     // own threads one entry after another; with 8 entries 26.
@@ -502,17 +508,18 @@ extern "C" size_t fl_distill_workspace_bytes(int64_t rows, int64_t V, int dtype)
     return (size_t)ws_layout(rows, V, dtype).bytes;
 }
 
-extern "C" int fl_distill_fwd(const void* logits, int64_t rows, int64_t slice_rows, int64_t slice_stride,
-                              int64_t row_stride, int64_t V, int dtype, const void* teacher, int teacher_dtype,
-                              const int64_t* index, int64_t K, float temperature, int reduction, float* loss,
-                              float* lse, float* teacher_lse, float* norm, void* workspace, size_t workspace_bytes,
-                              void* stream) {
-    const char* name = "fl_distill_fwd";
+namespace {
+
+int forward(const char* name, const void* logits, int64_t rows, int64_t slice_rows, int64_t slice_stride,
+            int64_t row_stride, int64_t V, int dtype, const void* teacher, int teacher_dtype, const int64_t* index,
+            int64_t K, float temperature, int reduction, float* loss, float* lse, float* teacher_lse, float* pairs,
+            float* norm, void* workspace, size_t workspace_bytes, void* stream) {
     const int rc = check(name, rows, slice_rows, V, K, dtype, teacher_dtype, temperature);
     if (rc != FL_OK || rows == 0) return rc;
     FL_CHECK(reduction >= 0 && reduction <= 2, "%s: reduction %d", name, reduction);
     FL_CHECK(logits && loss && lse && teacher_lse && (K == 0 || (teacher && index)) && (reduction == 0 || norm),
              "%s: NULL pointer argument", name);
+    FL_CHECK((reinterpret_cast<uintptr_t>(pairs) & 15u) == 0, "%s: pairs is not 16-byte aligned", name);
     const Ws w = ws_layout(rows, V, dtype);
     FL_CHECK((int64_t)workspace_bytes >= w.bytes, "%s: workspace of %llu bytes, %lld needed", name,
              (unsigned long long)workspace_bytes, (long long)w.bytes);
@@ -537,22 +544,24 @@ extern "C" int fl_distill_fwd(const void* logits, int64_t rows, int64_t slice_ro
     a.loss = reduction == 0 ? loss : reinterpret_cast<float*>(ws + w.rows);
     a.lse = lse;
     a.tlse = teacher_lse;
+    a.pairs = reinterpret_cast<f32x4*>(pairs);
     by_types(dtype, teacher_dtype, [&](auto t, auto tt) { launch_fwd<decltype(t), decltype(tt)>(a, s); });
     if (reduction != 0) reduce_rows<<<1, 1024, 0, s>>>(a.loss, teacher_lse, rows, reduction == 2, loss, norm);
     return launch_status(name);
 }
 
-extern "C" int fl_distill_bwd(const float* grad, int grad_stride, const float* norm, const void* logits, int64_t rows,
-                              int64_t slice_rows, int64_t slice_stride, int64_t row_stride, int64_t V, int dtype,
-                              const void* teacher, int teacher_dtype, const int64_t* index, int64_t K,
-                              float temperature, const float* lse, const float* teacher_lse, void* grad_logits,
-                              void* stream) {
-    const char* name = "fl_distill_bwd";
+// The gradient from both sides' pairs, or where there are none from their
+// log-sum-exps.
+int backward(const char* name, const float* grad, int grad_stride, const float* norm, const void* logits, int64_t rows,
+             int64_t slice_rows, int64_t slice_stride, int64_t row_stride, int64_t V, int dtype, const void* teacher,
+             int teacher_dtype, const int64_t* index, int64_t K, float temperature, const float* lse,
+             const float* teacher_lse, const float* pairs, void* grad_logits, void* stream) {
     const int rc = check(name, rows, slice_rows, V, K, dtype, teacher_dtype, temperature);
     if (rc != FL_OK || rows == 0) return rc;
     FL_CHECK(grad_stride == 0 || grad_stride == 1, "%s: grad_stride %d", name, grad_stride);
-    FL_CHECK(grad && logits && lse && teacher_lse && grad_logits && (K == 0 || (teacher && index)),
+    FL_CHECK(grad && logits && (pairs || (lse && teacher_lse)) && grad_logits && (K == 0 || (teacher && index)),
              "%s: NULL pointer argument", name);
+    FL_CHECK((reinterpret_cast<uintptr_t>(pairs) & 15u) == 0, "%s: pairs is not 16-byte aligned", name);
     BwdArgs a{};
     a.grad = grad;
     a.grad_stride = grad_stride;
@@ -563,6 +572,7 @@ extern "C" int fl_distill_bwd(const float* grad, int grad_stride, const float* n
     a.index = index;
     a.lse = lse;
     a.tlse = teacher_lse;
+    a.pairs = reinterpret_cast<const f32x4*>(pairs);
     a.rows = rows;
     a.v = V;
     a.k = (int)K;
@@ -572,4 +582,46 @@ extern "C" int fl_distill_bwd(const float* grad, int grad_stride, const float* n
     by_types(dtype, teacher_dtype,
              [&](auto t, auto tt) { launch_bwd<decltype(t), decltype(tt)>(a, static_cast<hipStream_t>(stream)); });
     return launch_status(name);
+}
+
+}  // namespace
+
+extern "C" int fl_distill_fwd(const void* logits, int64_t rows, int64_t slice_rows, int64_t slice_stride,
+                              int64_t row_stride, int64_t V, int dtype, const void* teacher, int teacher_dtype,
+                              const int64_t* index, int64_t K, float temperature, int reduction, float* loss,
+                              float* lse, float* teacher_lse, float* norm, void* workspace, size_t workspace_bytes,
+                              void* stream) {
+    return forward("fl_distill_fwd", logits, rows, slice_rows, slice_stride, row_stride, V, dtype, teacher,
+                   teacher_dtype, index, K, temperature, reduction, loss, lse, teacher_lse, nullptr, norm, workspace,
+                   workspace_bytes, stream);
+}
+
+extern "C" int fl_distill_fwd_pairs(const void* logits, int64_t rows, int64_t slice_rows, int64_t slice_stride,
+                                    int64_t row_stride, int64_t V, int dtype, const void* teacher, int teacher_dtype,
+                                    const int64_t* index, int64_t K, float temperature, int reduction, float* loss,
+                                    float* lse, float* teacher_lse, float* pairs, float* norm, void* workspace,
+                                    size_t workspace_bytes, void* stream) {
+    if (rows != 0) FL_CHECK(pairs, "fl_distill_fwd_pairs: NULL pointer argument");
+    return forward("fl_distill_fwd_pairs", logits, rows, slice_rows, slice_stride, row_stride, V, dtype, teacher,
+                   teacher_dtype, index, K, temperature, reduction, loss, lse, teacher_lse, pairs, norm, workspace,
+                   workspace_bytes, stream);
+}
+
+extern "C" int fl_distill_bwd(const float* grad, int grad_stride, const float* norm, const void* logits, int64_t rows,
+                              int64_t slice_rows, int64_t slice_stride, int64_t row_stride, int64_t V, int dtype,
+                              const void* teacher, int teacher_dtype, const int64_t* index, int64_t K,
+                              float temperature, const float* lse, const float* teacher_lse, void* grad_logits,
+                              void* stream) {
+    return backward("fl_distill_bwd", grad, grad_stride, norm, logits, rows, slice_rows, slice_stride, row_stride, V,
+                    dtype, teacher, teacher_dtype, index, K, temperature, lse, teacher_lse, nullptr, grad_logits,
+                    stream);
+}
+
+extern "C" int fl_distill_bwd_pairs(const float* grad, int grad_stride, const float* norm, const void* logits,
+                                    int64_t rows, int64_t slice_rows, int64_t slice_stride, int64_t row_stride,
+                                    int64_t V, int dtype, const void* teacher, int teacher_dtype, const int64_t* index,
+                                    int64_t K, float temperature, const float* pairs, void* grad_logits, void* stream) {
+    return backward("fl_distill_bwd_pairs", grad, grad_stride, norm, logits, rows, slice_rows, slice_stride, row_stride,
+                    V, dtype, teacher, teacher_dtype, index, K, temperature, nullptr, nullptr, pairs, grad_logits,
+                    stream);
 }

@@ -1004,27 +1004,31 @@ def _check_distill(logits, teacher, index):
 
 
 def topk_distillation(logits: torch.Tensor, teacher: torch.Tensor, index: torch.Tensor, temperature: float = 1.0,
-                      reduction: str = "mean"):
+                      reduction: str = "mean", with_pairs: bool = False):
     """Distillation from a teacher's top-K logits: (loss, lse, teacher_lse,
-    norm), the last three for the backward.  logits (rows, V) or
+    norm), the last three for the backward, and with_pairs also pairs
+    (rows, 4), from which the backward loses nothing to the logits' size:
+    both sides' maxima and logs of sums.  logits (rows, V) or
     (batch, rows, V) fp32, fp16 or bf16 with contiguous rows, teacher (.., K)
     of any of these types, index int64 (.., K).
     loss = temperature^2 * KL(softmax(teacher / temperature) over the K entries
     || softmax(logits / temperature)); teacher entries of -inf are unused, a row
     without any other has loss 0 and is left out of the mean."""
     _check_distill(logits, teacher, index)
-    return _distill_fwd(logits, teacher, index, temperature, _reduction(reduction))
+    out = _distill_fwd(logits, teacher, index, temperature, _reduction(reduction), with_pairs)
+    return out if with_pairs else out[:4]
 
 
-def _distill_fwd(logits, teacher, index, temperature, red):
+def _distill_fwd(logits, teacher, index, temperature, red, with_pairs):
     rows, slice_rows, s0, s1 = _distill_rows(logits)
     V, K = logits.shape[-1], teacher.shape[-1]
     dev = logits.device
     loss = torch.empty(logits.shape[:-1] if red == 0 else (), dtype=torch.float32, device=dev)
+    pairs = torch.empty((rows, 4), dtype=torch.float32, device=dev) if with_pairs else None
     stats = torch.empty((2 * rows + 1,), dtype=torch.float32, device=dev)
     lse, tlse, norm = stats[:rows], stats[rows:2 * rows], (stats[2 * rows:] if red else None)
     if rows == 0:
-        return loss.zero_(), lse, tlse, norm
+        return loss.zero_(), lse, tlse, norm, pairs
     dt = _DTYPE_CODE[logits.dtype]
     key = (rows, V, dt)
     nbytes = _ws_cache.get(key + ("distill",))
@@ -1033,41 +1037,51 @@ def _distill_fwd(logits, teacher, index, temperature, red):
     at = stats.data_ptr()
     with _on_device(logits):
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        _lib.call("fl_distill_fwd", logits.data_ptr(), rows, slice_rows, s0, s1, V, dt, teacher.data_ptr(),
-                  _DTYPE_CODE[teacher.dtype], index.data_ptr(), K, temperature, red, loss.data_ptr(), at,
-                  at + 4 * rows, at + 8 * rows if red else None, ws.data_ptr(), nbytes, _stream(logits))
-    return loss, lse, tlse, norm
+        of = (logits.data_ptr(), rows, slice_rows, s0, s1, V, dt, teacher.data_ptr(), _DTYPE_CODE[teacher.dtype],
+              index.data_ptr(), K, temperature, red, loss.data_ptr(), at, at + 4 * rows)
+        to = (at + 8 * rows if red else None, ws.data_ptr(), nbytes, _stream(logits))
+        if with_pairs:
+            _lib.call("fl_distill_fwd_pairs", *of, pairs.data_ptr(), *to)
+        else:
+            _lib.call("fl_distill_fwd", *of, *to)
+    return loss, lse, tlse, norm, pairs
 
 
-def _distill_bwd(grad_output, logits, teacher, index, lse, teacher_lse, norm, temperature):
+def _distill_bwd(grad_output, logits, teacher, index, lse, teacher_lse, norm, temperature, pairs=None):
     rows, slice_rows, s0, s1 = _distill_rows(logits)
     grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
     if rows == 0:
         return grad
     with _on_device(logits):
-        _lib.call("fl_distill_bwd", grad_output.data_ptr(), 0 if grad_output.numel() == 1 else 1,
-                  norm.data_ptr() if norm is not None else None, logits.data_ptr(), rows, slice_rows, s0, s1,
-                  logits.shape[-1], _DTYPE_CODE[logits.dtype], teacher.data_ptr(), _DTYPE_CODE[teacher.dtype],
-                  index.data_ptr(), teacher.shape[-1], temperature, lse.data_ptr(), teacher_lse.data_ptr(),
-                  grad.data_ptr(), _stream(logits))
+        of = (grad_output.data_ptr(), 0 if grad_output.numel() == 1 else 1,
+              norm.data_ptr() if norm is not None else None, logits.data_ptr(), rows, slice_rows, s0, s1,
+              logits.shape[-1], _DTYPE_CODE[logits.dtype], teacher.data_ptr(), _DTYPE_CODE[teacher.dtype],
+              index.data_ptr(), teacher.shape[-1], temperature)
+        if pairs is not None:
+            _lib.call("fl_distill_bwd_pairs", *of, pairs.data_ptr(), grad.data_ptr(), _stream(logits))
+        else:
+            _lib.call("fl_distill_bwd", *of, lse.data_ptr(), teacher_lse.data_ptr(), grad.data_ptr(), _stream(logits))
     return grad
 
 
 def topk_distillation_backward(grad_output: torch.Tensor, logits: torch.Tensor, teacher: torch.Tensor,
                                index: torch.Tensor, lse: torch.Tensor, teacher_lse: torch.Tensor, norm,
-                               temperature: float = 1.0) -> torch.Tensor:
+                               temperature: float = 1.0, pairs=None) -> torch.Tensor:
     """Gradient of the logits, contiguous and of their type; grad_output fp32
-    with one element per row, or one in all."""
+    with one element per row, or one in all.  With pairs (as the forward
+    returned them) lse and teacher_lse are not used."""
     _check_distill(logits, teacher, index)
     rows = _distill_rows(logits)[0]
     _check(grad_output.is_cuda and grad_output.dtype == torch.float32 and grad_output.is_contiguous(),
            "grad_output must be contiguous CUDA float32")
     _check(grad_output.numel() in (1, rows), "grad_output must have one element, or one per row")
-    for t, nm, n in ((lse, "lse", rows), (teacher_lse, "teacher_lse", rows), (norm, "norm", 1)):
-        _check(t is None and nm == "norm" or (t.is_cuda and t.dtype == torch.float32 and t.is_contiguous()
+    for t, nm, n in ((lse, "lse", rows), (teacher_lse, "teacher_lse", rows), (norm, "norm", 1),
+                     (pairs, "pairs", 4 * rows)):
+        _check(t is None and nm in ("norm", "pairs") or (t.is_cuda and t.dtype == torch.float32 and t.is_contiguous()
                                               and t.numel() == n), f"{nm} must be contiguous CUDA float32 of {n}")
-    _check_device(logits, "logits", grad_output=grad_output, lse=lse, teacher_lse=teacher_lse, norm=norm)
-    return _distill_bwd(grad_output, logits, teacher, index, lse, teacher_lse, norm, temperature)
+    _check_device(logits, "logits", grad_output=grad_output, lse=lse, teacher_lse=teacher_lse, norm=norm,
+                  pairs=pairs)
+    return _distill_bwd(grad_output, logits, teacher, index, lse, teacher_lse, norm, temperature, pairs)
 
 
 def _check_router(logits, index, mask):

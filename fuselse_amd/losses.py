@@ -86,18 +86,18 @@ def linear_cross_entropy(input: torch.Tensor, weight: torch.Tensor, target: torc
 class _TopkDistillation(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, teacher, index, temperature, reduction):
-        loss, lse, tlse, norm = ext._distill_fwd(logits, teacher, index, temperature, reduction)
-        ctx.save_for_backward(logits, teacher, index, lse, tlse, norm)
+        loss, _, _, norm, pairs = ext._distill_fwd(logits, teacher, index, temperature, reduction, True)
+        ctx.save_for_backward(logits, teacher, index, norm, pairs)
         ctx.temperature = temperature
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        logits, teacher, index, lse, tlse, norm = ctx.saved_tensors
+        logits, teacher, index, norm, pairs = ctx.saved_tensors
         if logits.stride(-1) != 1 and logits.shape[-1] != 1:  # as a saved-tensor hook may give it back
             logits = logits.contiguous()
-        g = ext._distill_bwd(grad.contiguous(), logits, teacher, index, lse, tlse, norm, ctx.temperature)
+        g = ext._distill_bwd(grad.contiguous(), logits, teacher, index, None, None, norm, ctx.temperature, pairs)
         return g, None, None, None, None
 
 
@@ -134,7 +134,7 @@ def topk_distillation(logits: torch.Tensor, teacher_logits: torch.Tensor, teache
     if torch.is_grad_enabled() and logits.requires_grad:
         loss = _TopkDistillation.apply(x, t, i, temperature, red)
     else:
-        loss = ext._distill_fwd(x, t, i, temperature, red)[0]
+        loss = ext._distill_fwd(x, t, i, temperature, red, False)[0]
     return loss.reshape(lead) if reduction == "none" else loss
 
 

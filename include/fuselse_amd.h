@@ -393,7 +393,12 @@ int fl_linear_ce_bwd(const float* grad, const void* x, int64_t ldx, const void* 
  *   and norm fp32 [1] (NULL with reduction 0) for the backward.
  * fl_distill_bwd: grad fp32, element r * grad_stride (0 or 1) for row r;
  *   norm as the forward wrote it or NULL; grad_logits [rows, V] contiguous, of
- *   the logits' type.
+ *   the logits' type.  Its exponents are off by the rounding of lse and
+ *   teacher_lse, half a step of their size.
+ * fl_distill_fwd_pairs, fl_distill_bwd_pairs: the same with pairs fp32
+ *   [rows, 4] (16-byte aligned), both sides' maxima and logs of the sums of
+ *   exponentials of the differences from them over T.  A backward from them
+ *   loses nothing to a value the logits have in common.
  * At most 2^22 rows of 2^28 columns, K <= 1024 (FL_ERANGE).  With rows == 0
  * nothing is written.
  * ------------------------------------------------------------------------- */
@@ -406,6 +411,15 @@ int fl_distill_bwd(const float* grad, int grad_stride, const float* norm, const 
                    int64_t slice_rows, int64_t slice_stride, int64_t row_stride, int64_t V, int dtype,
                    const void* teacher, int teacher_dtype, const int64_t* index, int64_t K, float temperature,
                    const float* lse, const float* teacher_lse, void* grad_logits, void* stream);
+int fl_distill_fwd_pairs(const void* logits, int64_t rows, int64_t slice_rows, int64_t slice_stride,
+                         int64_t row_stride, int64_t V, int dtype, const void* teacher, int teacher_dtype,
+                         const int64_t* index, int64_t K, float temperature, int reduction, float* loss, float* lse,
+                         float* teacher_lse, float* pairs, float* norm, void* workspace, size_t workspace_bytes,
+                         void* stream);
+int fl_distill_bwd_pairs(const float* grad, int grad_stride, const float* norm, const void* logits, int64_t rows,
+                         int64_t slice_rows, int64_t slice_stride, int64_t row_stride, int64_t V, int dtype,
+                         const void* teacher, int teacher_dtype, const int64_t* index, int64_t K, float temperature,
+                         const float* pairs, void* grad_logits, void* stream);
 
 /* ---------------------------------------------------------------------------
  * Balance loss, z loss and per-expert counts of a mixture-of-experts router.

@@ -66,3 +66,38 @@ def test_distillation_of_shifted_logits_loss(cuda, rows, v, k, temp, offset):
     up = torch.ones(rows, device=cuda)
     want, _, b, _ = distill_exact(s, t, i, temp, up)
     within(fuselse_amd.topk_distillation(s, t, i, temperature=temp, reduction="none"), want, b, "loss")
+
+
+@pytest.mark.parametrize("offset", OFFSETS)
+@pytest.mark.parametrize("rows,v,k,temp", [(5, 4096, 16, 1.0), (3, 50257, 200, 1.0), (33, 1001, 5, 2.0),
+                                           (2000, 300, 8, 0.7), (4, 40000, 64, 3.0)])
+def test_distillation_of_shifted_logits_gradient(cuda, rows, v, k, temp, offset):
+    print(f"case distill offset gradient {rows} {v} {k} {temp} {offset}", flush=True)
+    s, t = spread(cuda, (rows, v), offset, v), spread(cuda, (rows, k), -offset, k)
+    i = torch.rand(rows, v, device=cuda).argsort(-1)[:, :k].contiguous()
+    up = torch.randn(rows, device=cuda, generator=torch.Generator(device=cuda).manual_seed(3))
+    _, want, _, b = distill_exact(s, t, i, temp, up)
+    s.requires_grad_(True)
+    loss = fuselse_amd.topk_distillation(s, t, i, temperature=temp, reduction="none")
+    within(torch.autograd.grad(loss, s, up)[0], want, b, "ds")
+
+
+def test_distillation_gradient_without_pairs(cuda):
+    """The checked calls with and without pairs: the same loss, the gradient
+    off by the log-sum-exps' rounding alone."""
+    print("case distill pairs", flush=True)
+    rows, v, k = 6, 3001, 12
+    s, t = spread(cuda, (rows, v), 0.0, 1), spread(cuda, (rows, k), 0.0, 2)
+    i = torch.rand(rows, v, device=cuda).argsort(-1)[:, :k].contiguous()
+    up = torch.ones(rows, device=cuda)
+    loss, lse, tlse, norm = ext.topk_distillation(s, t, i, 2.0, "none")
+    loss2, _, _, _, pairs = ext.topk_distillation(s, t, i, 2.0, "none", with_pairs=True)
+    assert torch.equal(loss, loss2) and pairs.shape == (rows, 4)
+    a = ext.topk_distillation_backward(up, s, t, i, lse, tlse, norm, 2.0)
+    b = ext.topk_distillation_backward(up, s, t, i, lse, tlse, norm, 2.0, pairs=pairs)
+    _, want, _, bound = distill_exact(s, t, i, 2.0, up)
+    within(b, want, bound, "with pairs")
+    # exponents, and with them an element's parts, off by a step of 16 at most
+    within(a, want, bound + 2.0 ** -18 * want.abs().amax(1, keepdim=True), "without")
+    with pytest.raises(RuntimeError, match="pairs must be"):
+        ext.topk_distillation_backward(up, s, t, i, lse, tlse, norm, 2.0, pairs=pairs[:3])

@@ -1,5 +1,7 @@
 """Sizes, ranges and host-side state of the training losses, without a GPU."""
 
+import ctypes
+
 import pytest
 
 from fuselse_amd import _lib
@@ -18,3 +20,20 @@ def test_a_forwards_workspace_does_not_grow_with_the_logits(dtype, alone):
                 rows = n * (2 * (2 if dtype == 0 else 1) * (-(-d // 64) * 64) + 32)
                 # a piece is 2048 vocabulary entries at least: 17 pairs a row
                 assert nbytes <= rows + (1 << 28) * 2 + 17 * 8 * n + (1 << 16), (n, v, d, nbytes)
+
+
+def test_distillation_pairs_refusals():
+    lib = _lib.load()
+    vp = ctypes.c_void_p(4096)
+
+    def fwd(pairs):
+        return lib.fl_distill_fwd_pairs(vp, 2, 2, 8, 8, 8, 0, vp, 0, vp, 2, 1.0, 0, vp, vp, vp, pairs, None, vp, 1 << 30,
+                                        None)
+
+    def bwd(pairs, rows=2):
+        return lib.fl_distill_bwd_pairs(vp, 1, None, vp, rows, 2, 8, 8, 8, 0, vp, 0, vp, 2, 1.0, pairs, vp, None)
+
+    for call in (fwd, bwd):
+        assert call(None) == 1 and "NULL" in lib.fl_last_error().decode()
+        assert call(ctypes.c_void_p(4104)) == 1 and "16-byte" in lib.fl_last_error().decode()
+    assert bwd(None, rows=0) == 0

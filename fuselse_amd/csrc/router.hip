@@ -13,9 +13,8 @@
 // and then over blocks in a fixed order, so results do not depend on the order
 // of the blocks.  Both directions read the logits once and are bound by memory,
 // or by the launches where the batch is small: one block then does it all.
-// (131072, 256) in fp32 with 8 choices: forward 30 us (4.8 TB/s) and 9.6 for the
-// join, backward 42 us (6.4 TB/s); (16383, 64) in bf16 with 6: 7.9 + 6.1 and 5.6 us,
-// (512, 8) in fp32 4.5 and 2.9.
+// (131072, 256) in fp32 with 8 choices: forward 24.6 us (5.8 TB/s) and 9.5 for the
+// join, backward 42 us (6.4 TB/s); (16383, 64) in bf16 with 6: 7.0 + 6.0 and 5.2 us.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -61,7 +60,7 @@ struct Args {
 };
 
 // A token's logits: NV vectors a lane, lane `sub` of G holding vectors
-// sub, sub + G, ..; past the row -inf.  Returns its (max, sum) joined.
+// sub, sub + G, ..; past the row -inf.
 template <typename T, int G, int NV>
 __device__ __forceinline__ void load_token(const T* x, int experts, int sub, float (&v)[NV][Elem<T>::kVec]) {
     constexpr int VE = Elem<T>::kVec;
@@ -72,13 +71,53 @@ __device__ __forceinline__ void load_token(const T* x, int experts, int sub, flo
     }
 }
 
+// Sum over a group's lanes of values that all of them get.
+template <int G>
+__device__ __forceinline__ float group_sum(float v) {
+    if constexpr (G >= 2) v += reduce_partner<1>(v);
+    if constexpr (G >= 4) v += reduce_partner<2>(v);
+    if constexpr (G >= 8) v += reduce_partner<4>(v);
+    if constexpr (G >= 16) v += reduce_partner<8>(v);
+    if constexpr (G >= 32) v += reduce_partner<16>(v);
+    if constexpr (G >= 64) v += reduce_partner<32>(v);
+    return v;
+}
+template <int G>
+__device__ __forceinline__ float group_max(float v) {
+    if constexpr (G >= 2) v = fmaxf(v, reduce_partner<1>(v));
+    if constexpr (G >= 4) v = fmaxf(v, reduce_partner<2>(v));
+    if constexpr (G >= 8) v = fmaxf(v, reduce_partner<4>(v));
+    if constexpr (G >= 16) v = fmaxf(v, reduce_partner<8>(v));
+    if constexpr (G >= 32) v = fmaxf(v, reduce_partner<16>(v));
+    if constexpr (G >= 64) v = fmaxf(v, reduce_partner<32>(v));
+    return v;
+}
+
+// Turns a token's logits into its probabilities and returns its log-sum-exp.  The
+// probabilities come from differences to the maximum, not from the log-sum-exp,
+// whose rounding in fp32 counts with the logits' own size (2e-5 around 1000).
 template <int G, int NV, int VE>
-__device__ __forceinline__ float token_lse(const float (&v)[NV][VE]) {
+__device__ __forceinline__ float token_softmax(float (&v)[NV][VE]) {
     float m = -kInf, s = 0.0f;
 #pragma unroll
-    for (int j = 0; j < NV; ++j) lse_fold<true>(m, s, v[j]);
-    group_merge<G>(m, s);
-    return lse_finish<true>(m, s);
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int k = 0; k < VE; ++k) m = fmaxf(m, v[j][k]);
+    const float b = lse_base(group_max<G>(m));
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int k = 0; k < VE; ++k) {
+            v[j][k] = fexp2((v[j][k] - b) * kLog2e);
+            s += v[j][k];
+        }
+    s = group_sum<G>(s);
+    const float inv = 1.0f / s;
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int k = 0; k < VE; ++k) v[j][k] *= inv;
+    return b + flog2(s) * kLn2;
 }
 
 __device__ __forceinline__ double wave_sum(double v) {
@@ -185,11 +224,11 @@ __global__ __launch_bounds__(kThreads) void fwd_tokens(Args p) {
             const int64_t e = p.index[t * p.top + k];
             if (e >= 0 && e < p.experts) atomicAdd(&shc[e], 1);
         }
-        const float lse = token_lse<G, NV, VE>(v);
+        const float lse = token_softmax<G, NV, VE>(v);
 #pragma unroll
         for (int j = 0; j < NV; ++j)
 #pragma unroll
-            for (int k = 0; k < VE; ++k) sum[j][k] += fexp2((v[j][k] - lse) * kLog2e);
+            for (int k = 0; k < VE; ++k) sum[j][k] += v[j][k];
         if (sub == 0) {
             p.lse[t] = lse;
             z += (double)lse * lse;
@@ -254,20 +293,13 @@ __global__ __launch_bounds__(kThreads) void bwd_tokens(Args p) {
         } else {
             load_token<T, G, NV>(static_cast<const T*>(p.x) + t * p.ldx, p.experts, sub, v);
             const float lse = p.lse[t];
+            token_softmax<G, NV, VE>(v);
             float dot = 0.0f;
 #pragma unroll
             for (int j = 0; j < NV; ++j)
 #pragma unroll
-                for (int k = 0; k < VE; ++k) {
-                    v[j][k] = fexp2((v[j][k] - lse) * kLog2e);
-                    dot += v[j][k] * c[j][k];
-                }
-            if constexpr (G >= 2) dot += reduce_partner<1>(dot);
-            if constexpr (G >= 4) dot += reduce_partner<2>(dot);
-            if constexpr (G >= 8) dot += reduce_partner<4>(dot);
-            if constexpr (G >= 16) dot += reduce_partner<8>(dot);
-            if constexpr (G >= 32) dot += reduce_partner<16>(dot);
-            if constexpr (G >= 64) dot += reduce_partner<32>(dot);
+                for (int k = 0; k < VE; ++k) dot += v[j][k] * c[j][k];
+            dot = group_sum<G>(dot);
 #pragma unroll
             for (int j = 0; j < NV; ++j)
 #pragma unroll

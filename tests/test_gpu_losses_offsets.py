@@ -101,3 +101,32 @@ def test_distillation_gradient_without_pairs(cuda):
     within(a, want, bound + 2.0 ** -18 * want.abs().amax(1, keepdim=True), "without")
     with pytest.raises(RuntimeError, match="pairs must be"):
         ext.topk_distillation_backward(up, s, t, i, lse, tlse, norm, 2.0, pairs=pairs[:3])
+
+
+@pytest.mark.parametrize("offset", [0.0, 100.0, -1000.0, 2000.0])
+@pytest.mark.parametrize("tokens,e,k", [(300, 8, 2), (1000, 60, 4), (700, 256, 8), (5000, 384, 6), (400, 1000, 2)])
+def test_router_balance_of_shifted_logits(cuda, tokens, e, k, offset):
+    print(f"case router offset {tokens} {e} {k} {offset}", flush=True)
+    x = spread(cuda, (tokens, e), offset, e)
+    index = x.topk(k, 1).indices
+    x.requires_grad_(True)
+    out = fuselse_amd.router_balance(x, index)
+    (gx,) = torch.autograd.grad(out.balance_loss, x)
+    xd = x.detach().double()
+    xd = xd - xd.amax(1, keepdim=True)
+    p = torch.softmax(xd, 1)
+    f = torch.bincount(index.reshape(-1), minlength=e).double() / (tokens * k)
+    balance = e * (f * p.mean(0)).sum()
+    dot = (p * f).sum(1, keepdim=True)
+    want = p * (e / tokens * (f - dot))
+    # an exponent is off by three roundings of its size, a sum by the mean of that
+    # and by its additions: 16 a lane, and 64 for the merges
+    rel = xd.abs() * 2.0 ** -22
+    rel = rel + (p * rel).sum(1, keepdim=True) + (e / 64 + 80) * E23
+    # a lane adds its tokens' probabilities one after another
+    bal_b = e * (f * (p * rel).mean(0)).sum() + balance * (tokens / 256 + 64) * E23
+    within(out.balance_loss, balance, bal_b, "balance")
+    size = p * (e / tokens * (f + dot))
+    bound = size * (rel + 2.0 ** -21) + p * (e / tokens) * (p * f * (rel + (e / 64 + 16) * E23)).sum(1, keepdim=True) \
+        + 2.0 ** -126
+    within(gx, want, bound + u(torch.float32) * want.abs(), "dlogits")

@@ -76,18 +76,24 @@ def _on_device(t: torch.Tensor):
 _ws_cache = {}
 
 
+def _remembered(key, query: str, *args) -> int:
+    """The size that the library's `query` gives for args, asked once a key and
+    kept for the last few thousand keys: calls of ever new sizes do not make
+    the table grow without end."""
+    nbytes = _ws_cache.get(key)
+    if nbytes is None:
+        if len(_ws_cache) >= 4096:
+            _ws_cache.clear()
+        nbytes = _ws_cache[key] = getattr(_lib.load(), query)(*args)
+    return nbytes
+
+
 def _workspace_bytes(B: int, N: int, elem_bytes: int) -> int:
     """Bytes of split-row workspace the library's plan asks for at (B, N)
     (0: the one-pass kernels).  The plan is a fixed function of the shape, so
     each shape is asked once: the query is a second foreign call, about as
     long as the launch itself."""
-    key = (B, N, elem_bytes)
-    nbytes = _ws_cache.get(key)
-    if nbytes is None:
-        if len(_ws_cache) >= 4096:
-            _ws_cache.clear()
-        nbytes = _ws_cache[key] = _lib.load().fl_lse_fwd_workspace_bytes(B, N, elem_bytes)
-    return nbytes
+    return _remembered((B, N, elem_bytes), "fl_lse_fwd_workspace_bytes", B, N, elem_bytes)
 
 
 def _launch_fwd(entry: str, x: torch.Tensor, out: torch.Tensor, elem_bytes: int, robust: bool,
@@ -908,12 +914,8 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
 
 
 def _linear_workspace(N, V, D, dt, which, w_ptr, ldw, device):
-    key = (N, V, D, dt, which, w_ptr & 15, ldw)
-    nbytes = _ws_cache.get(key)
-    if nbytes is None:
-        if len(_ws_cache) >= 4096:
-            _ws_cache.clear()
-        nbytes = _ws_cache[key] = _lib.load().fl_linear_ce_workspace_bytes(N, V, D, dt, which, w_ptr, ldw)
+    nbytes = _remembered((N, V, D, dt, which, w_ptr & 15, ldw), "fl_linear_ce_workspace_bytes", N, V, D, dt, which,
+                         w_ptr, ldw)
     return torch.empty(nbytes, dtype=torch.uint8, device=device)
 
 
@@ -1030,10 +1032,7 @@ def _distill_fwd(logits, teacher, index, temperature, red, with_pairs):
     if rows == 0:
         return loss.zero_(), lse, tlse, norm, pairs
     dt = _DTYPE_CODE[logits.dtype]
-    key = (rows, V, dt)
-    nbytes = _ws_cache.get(key + ("distill",))
-    if nbytes is None:
-        nbytes = _ws_cache[key + ("distill",)] = _lib.load().fl_distill_workspace_bytes(rows, V, dt)
+    nbytes = _remembered(("distill", rows, V, dt), "fl_distill_workspace_bytes", rows, V, dt)
     at = stats.data_ptr()
     with _on_device(logits):
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
@@ -1118,10 +1117,7 @@ def _router_fwd(logits, index, mask):
     counts = torch.empty((E,), dtype=torch.int64, device=dev)
     stats = torch.empty((T + E + 1,), dtype=torch.float32, device=dev)
     dt = _DTYPE_CODE[logits.dtype]
-    key = ("router", T, E, dt)
-    nbytes = _ws_cache.get(key)
-    if nbytes is None:
-        nbytes = _ws_cache[key] = _lib.load().fl_router_workspace_bytes(T, E, dt)
+    nbytes = _remembered(("router", T, E, dt), "fl_router_workspace_bytes", T, E, dt)
     at = stats.data_ptr()
     with _on_device(logits):
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)

@@ -3,8 +3,9 @@
 import ctypes
 
 import pytest
+import torch
 
-from fuselse_amd import _lib
+from fuselse_amd import _lib, ext
 
 
 @pytest.mark.parametrize("dtype", [0, 1, 2])
@@ -37,3 +38,23 @@ def test_distillation_pairs_refusals():
         assert call(None) == 1 and "NULL" in lib.fl_last_error().decode()
         assert call(ctypes.c_void_p(4104)) == 1 and "16-byte" in lib.fl_last_error().decode()
     assert bwd(None, rows=0) == 0
+
+
+def test_remembered_workspace_sizes_stay_few(monkeypatch):
+    """Calls of ever new numbers of rows do not make the host's table grow
+    without end, whichever operator they call."""
+    monkeypatch.setattr(ext._lib, "call", lambda *a: None)
+    monkeypatch.setattr(ext, "_stream", lambda t: 0)
+    monkeypatch.setattr(ext, "_ws_cache", {})
+    x, i = torch.zeros(5000, 2), torch.zeros(5000, 1, dtype=torch.int64)
+    for n in range(1, 5000):
+        ext._distill_fwd(x[:n], x[:n, :1].contiguous(), i[:n], 1.0, 0, False)
+    assert len(ext._ws_cache) <= 4096
+    ext._ws_cache.clear()
+    for n in range(1, 5000):
+        ext._router_fwd(x[:n], i[:n], None)
+    assert len(ext._ws_cache) <= 4096
+    ext._ws_cache.clear()
+    for n in range(1, 5000):
+        ext._linear_fwd(x[:n], x[:3], i[:n, 0], -100, 0, 0.0, False)
+    assert len(ext._ws_cache) <= 4096

@@ -36,6 +36,15 @@ def _integers(t: torch.Tensor, name: str) -> torch.Tensor:
     return t.to(torch.int64)
 
 
+def _one_type(a: torch.Tensor, b: torch.Tensor):
+    """In an autocast region two tensors of different types brought to the
+    region's, as its matrix products take them; else the tensors themselves."""
+    if a.dtype != b.dtype and torch.is_autocast_enabled("cuda"):
+        to = torch.get_autocast_dtype("cuda")
+        a, b = (t.to(to) if t.dtype in ext._DTYPE_CODE else t for t in (a, b))
+    return a, b
+
+
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, target, ignore_index, reduction, z_loss):
@@ -66,12 +75,16 @@ def linear_cross_entropy(input: torch.Tensor, weight: torch.Tensor, target: torc
     the gradients.  reduction: "none" (a loss per token, target's shape), "sum",
     or "mean" over the tokens that are not ignored (0 where all are).
 
+    input and weight are of one type; in a torch.autocast region they may differ
+    and are then both cast to the region's.
+
     Gradients reach input and weight.  The backward makes the logits again in
     pieces of the vocabulary; its workspace, and the forward's, grow with
     N * D and with N and D times one piece, not with N * V.
     """
     ext._check(input.dim() >= 1 and tuple(input.shape[:-1]) == tuple(target.shape),
                "target must have input's shape without its last dimension")
+    input, weight = _one_type(input, weight)
     x, w = _rows(input), _rows(weight) if weight.dim() == 2 else weight
     t = _integers(target, "target").reshape(-1).contiguous()
     ext._check_linear(x, w, t)

@@ -324,6 +324,7 @@ struct PackArgs {
     const Head* head;
     int64_t d, ldp;
     int lanes;         // fp32: of a row
+    int64_t block0;    // fp16, bf16: blocks of the launches before
 };
 
 template <typename T>
@@ -357,7 +358,7 @@ template <int DT>
 __global__ __launch_bounds__(256) void pack(PackArgs p) {
     typedef typename Io<DT>::T T;
     const int64_t chunks = p.ldp / 8;
-    int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    int64_t i = (p.block0 + blockIdx.x) * 256 + threadIdx.x;
     const bool is_x = i < p.x.n * chunks;
     const PackSide& s = is_x ? p.x : p.w;
     if (!is_x) i -= p.x.n * chunks;
@@ -1381,7 +1382,10 @@ void operands(const Call& c, const Layout& l, int64_t v0, int64_t rows, bool dx,
         if (l.ldx <= 512) pack_f32<1><<<grid, 256, 0, c.s>>>(p);
         else pack_f32<2><<<grid, 256, 0, c.s>>>(p);
     } else {
-        pack<DT><<<dim3((unsigned)div_up(packed * (l.ldx / 8), 256)), 256, 0, c.s>>>(p);
+        for_grid_chunks(div_up(packed * (l.ldx / 8), 256), 256, [&](int64_t first, int64_t count) {
+            p.block0 = first;
+            pack<DT><<<dim3((unsigned)count), 256, 0, c.s>>>(p);
+        });
     }
 }
 

@@ -266,3 +266,28 @@ def test_pairs_joined_piece_by_piece(cuda, dtype, n, d, v):
     # a row's loss does not depend on the rows beside it, nor on the pieces
     few = fuselse_amd.linear_cross_entropy(x[some], w, t[some], reduction="none")
     within(few, want, bound, "loss of some rows")
+
+
+# ---------------------------------------------------------------------------
+# More elements of x than one launch has threads
+# ---------------------------------------------------------------------------
+def test_more_rows_than_one_packing_launch_covers(cuda):
+    """2^23 rows of 4096 columns are 2^32 threads of 8 elements; all but a few
+    are ignored, and hold whatever the memory held."""
+    print("case linear long", flush=True)
+    n, d, v = 1 << 23, 4096, 300
+    torch.cuda.empty_cache()
+    g = torch.Generator(device=cuda).manual_seed(51)
+    x = torch.empty(n, d, dtype=torch.bfloat16, device=cuda)
+    w = (torch.randn(v, d, device=cuda, generator=g) / 32).to(torch.bfloat16)
+    at = torch.tensor([0, 1, 4097, n // 2, n - 3, n - 1], device=cuda)
+    t = torch.full((n,), -100, device=cuda)
+    t[at] = torch.randint(0, v, (len(at),), device=cuda, generator=g)
+    x[at] = torch.randn(len(at), d, device=cuda, generator=g).to(torch.bfloat16)
+    loss = fuselse_amd.linear_cross_entropy(x, w, t, reduction="none")
+    xs = x[at].clone()
+    del x
+    torch.cuda.empty_cache()
+    want, _, _, b, _, _, _ = live_reference(xs, w, t[at], torch.ones(len(at), device=cuda), logit_error(xs, w))
+    within(loss[at], want, b, "loss")
+    assert int((loss != 0).sum()) == len(at)

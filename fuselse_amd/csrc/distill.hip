@@ -489,8 +489,10 @@ int check(const char* name, int64_t rows, int64_t n1, int64_t v, int64_t k, int 
     FL_CHECK(rows >= 0 && v >= 1 && k >= 0 && n1 >= 1, "%s: bad shape (rows=%lld, V=%lld, K=%lld)", name,
              (long long)rows, (long long)v, (long long)k);
     FL_CHECK(dtype >= 0 && dtype <= 2 && tdtype >= 0 && tdtype <= 2, "%s: dtype %d, %d", name, dtype, tdtype);
-    FL_CHECK(temp > 0.0f && __builtin_isfinite(temp) && __builtin_isfinite(1.0f / temp),
-             "%s: temperature must be positive and finite, and so its inverse", name);
+    // the loss carries the square
+    const float square = temp * temp;
+    FL_CHECK(temp > 0.0f && __builtin_isnormal(square) && __builtin_isnormal(1.0f / square),
+             "%s: temperature must be positive, its square and the square's inverse normal fp32 numbers", name);
     if (k > kMaxTop) return set_error(FL_ERANGE, "%s: at most %d teacher logits a row", name, kMaxTop);
     if (rows > (1 << 22) || v > (1 << 28)) return set_error(FL_ERANGE, "%s: at most 2^22 rows of 2^28 columns", name);
     return ok();

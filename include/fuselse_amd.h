@@ -399,6 +399,7 @@ int fl_linear_ce_bwd(const float* grad, const void* x, int64_t ldx, const void* 
  *   [rows, 4] (16-byte aligned), both sides' maxima and logs of the sums of
  *   exponentials of the differences from them over T.  A backward from them
  *   loses nothing to a value the logits have in common.
+ * T^2 and its inverse have to be normal fp32 numbers (about 1.1e-19 to 9e18).
  * At most 2^22 rows of 2^28 columns, K <= 1024 (FL_ERANGE).  With rows == 0
  * nothing is written.
  * ------------------------------------------------------------------------- */

@@ -58,3 +58,21 @@ def test_remembered_workspace_sizes_stay_few(monkeypatch):
     for n in range(1, 5000):
         ext._linear_fwd(x[:n], x[:3], i[:n, 0], -100, 0, 0.0, False)
     assert len(ext._ws_cache) <= 4096
+
+
+@pytest.mark.parametrize("call", ["fl_distill_fwd", "fl_distill_bwd"])
+def test_distillation_temperatures_whose_square_leaves_the_type(call):
+    """The loss carries T^2: where that or its inverse is no normal fp32 number
+    the call is refused rather than answered with 0, infinity or NaN."""
+    lib = _lib.load()
+    vp = ctypes.c_void_p(4096)
+
+    def code(temp):
+        if call == "fl_distill_fwd":
+            return lib.fl_distill_fwd(vp, 0, 2, 8, 8, 8, 0, vp, 0, vp, 2, temp, 0, vp, vp, vp, None, vp, 1 << 30, None)
+        return lib.fl_distill_bwd(vp, 1, None, vp, 0, 2, 8, 8, 8, 0, vp, 0, vp, 2, temp, vp, vp, vp, None)
+
+    for temp in (1e-25, 1e-20, 2e19, 1e30, -1.0):
+        assert code(temp) == 1 and "temperature" in lib.fl_last_error().decode(), temp
+    for temp in (2e-19, 1e-6, 1.0, 1e6, 5e18):
+        assert code(temp) == 0, temp

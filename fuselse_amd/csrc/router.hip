@@ -336,7 +336,7 @@ void shape(int experts, int dtype, int& g, int& nv) {
 }
 
 // Elements one block takes by itself, results and all, rather than a second
-// launch: (256, 64) 7.5 us for 11.0, but (1024, 64) 14.8 for 11.2.
+// launch: (256, 64) 6.1 us for 9.2, but (1024, 64) 13.2 for 9.6.
 constexpr int64_t kAlone = 16384;
 
 int block_count(int64_t tokens, int experts, int dtype) {
@@ -344,8 +344,8 @@ int block_count(int64_t tokens, int experts, int dtype) {
     shape(experts, dtype, g, nv);
     const int groups = kThreads / g;
     if (tokens * experts <= kAlone) return 1;
-    // one block a CU: (131072, 256) 38.2 us in all, with half as many 55.5, with
-    // twice as many, whose parts take longer to join, 39.0
+    // one block a CU: (131072, 256) 34.0 us in all, with half as many 44.0, with
+    // twice as many, whose parts take longer to join, 37.2
     const int64_t want = (tokens + groups - 1) / groups;
     return (int)(want < 256 ? (want < 1 ? 1 : want) : 256);
 }

@@ -369,22 +369,22 @@ __global__ __launch_bounds__(256) void pack(PackArgs p) {
     store_parts<DT, 1>(v, 1.0f, s.logits + r * p.ldp + c, s.logits_part);
 }
 
-// fp32: a group of lanes takes a row's largest finite magnitude, and with it the
-// row's scale, then writes the row for the logits and, where `grads` is not
-// NULL, for dx and dw.  The first C of a lane's chunks stay in registers; what a
-// row has beyond is read twice, the second time from the caches.  C of 1 / 2,
-// whole forwards, us: (513, 64, 32000) 40.6 / 41.3, (500, 768, 50257) 192 / 188,
-// (500, 2048, 32000) 325 / 316: 2 where a row has more than 64 chunks.
-template <int C>
+// fp32: a group of lanes, of a wave or (BLOCK) the whole block, takes a row's largest
+// finite magnitude, and with it the row's scale, then writes the row for the
+// logits and, where `grads` is not NULL, for dx and dw.  The first C of a lane's
+// chunks stay in registers; what a row has beyond is read twice, the second time
+// from the caches.
+template <int C, bool BLOCK>
 __global__ __launch_bounds__(256) void pack_f32(PackArgs p) {
-    const int sub = (int)threadIdx.x % p.lanes;
-    int64_t r = (int64_t)blockIdx.x * (256 / p.lanes) + (int)threadIdx.x / p.lanes;
+    const int lanes = BLOCK ? 256 : p.lanes;
+    const int sub = (int)threadIdx.x % lanes;
+    int64_t r = (int64_t)blockIdx.x * (256 / lanes) + (int)threadIdx.x / lanes;
     const bool is_x = r < p.x.n;
     const PackSide& s = is_x ? p.x : p.w;
     if (!is_x) r -= p.x.n;
     if (r >= (is_x ? (int64_t)p.head->live : s.n)) return;  // whole groups
     const float* src = static_cast<const float*>(s.src) + (s.rows ? (int64_t)s.rows[r] : r) * s.ld;
-    const int64_t first = sub * 8, step = p.lanes * 8;
+    const int64_t first = sub * 8, step = lanes * 8;
     float kept[C][8], big = 0.0f;
     auto take = [&](const float (&v)[8]) {
 #pragma unroll
@@ -402,7 +402,12 @@ __global__ __launch_bounds__(256) void pack_f32(PackArgs p) {
         load8(src + c, p.d - c, v);
         take(v);
     }
-    for (int d = 1; d < p.lanes; d *= 2) big = fmaxf(big, __shfl_xor(big, d, 64));
+    if constexpr (BLOCK) {
+        __shared__ float sh[4];
+        big = block_max<256>(big, sh);
+    } else {
+        for (int d = 1; d < lanes; d *= 2) big = fmaxf(big, __shfl_xor(big, d, 64));
+    }
     const int e = scale_exp(big, 15);
     const float scale = __builtin_ldexpf(1.0f, e);
     if (sub == 0) s.undo[r] = (int8_t)-e;
@@ -1378,11 +1383,18 @@ void operands(const Call& c, const Layout& l, int64_t v0, int64_t rows, bool dx,
     const int64_t packed = p.x.n + p.w.n;
     if (packed == 0) return;
     if constexpr (DT == kF32) {
+        // By a wave / a block a row, us: (2921, 3776) for the logits alone 21.0 / 17.1,
+        // with the gradients' parts 30.7 / 24.4.  One / two chunks a lane, whole
+        // forwards: (513, 64, 32000) 40.6 / 41.3, (500, 768, 50257) 192 / 188.
+        if (l.ldx > 1024) {
+            pack_f32<2, true><<<dim3((unsigned)packed), 256, 0, c.s>>>(p);
+            return;
+        }
         p.lanes = 8;  // a row is 64 elements at least
         while (p.lanes < 64 && p.lanes * 8 < l.ldx) p.lanes *= 2;
         const dim3 grid((unsigned)div_up(packed * p.lanes, 256));
-        if (l.ldx <= 512) pack_f32<1><<<grid, 256, 0, c.s>>>(p);
-        else pack_f32<2><<<grid, 256, 0, c.s>>>(p);
+        if (l.ldx <= 512) pack_f32<1, false><<<grid, 256, 0, c.s>>>(p);
+        else pack_f32<2, false><<<grid, 256, 0, c.s>>>(p);
     } else {
         for_grid_chunks(div_up(packed * (l.ldx / 8), 256), 256, [&](int64_t first, int64_t count) {
             p.block0 = first;

@@ -8,8 +8,8 @@
 // Forward: one pass over the student's row (running maximum and sum), K
 // gathers.  Backward: one read and one write of the row.  Both are bound by
 // memory; no product, no matrix cores.  (4092, 128256) in bf16 with 64 entries:
-// forward 171 us, 6.2 TB/s, backward 313 us, 6.7 TB/s; (1536, 50257) in fp32 with
-// 20: 53 us, 5.9 TB/s, and 97 us, 6.4 TB/s (a copy: 6.8).
+// forward 169 us, 6.2 TB/s, backward 314 us, 6.7 TB/s; (1533, 50257) in fp32 with
+// 20: 53 us, 5.9 TB/s, and 99 us, 6.2 TB/s (a copy: 6.8).
 //
 // Entries whose teacher logit is -inf are unused, whatever their index; a row
 // without any other has loss and gradient 0.  A used index outside [0, V) makes

@@ -12,7 +12,7 @@
 // (4096, 2048, 128256) in bf16 with 2867 live rows: forward 1.2 ms, backward 4.1 ms,
 // of which G 1.3, dx 1.4 and dw 1.35, 5.3 ms in all for 4.65 of four large library
 // products; (8, 2048, 128256) forward 95 us, w's 525 MB at the copy rate 77.
-// (2048, 1024, 32000) in fp32, both directions: 2.1 ms, for 3.0 of three products
+// (2048, 1024, 32000) in fp32, both directions: 2.2 ms, for 3.0 of three products
 // on the fp32 matrix pipe.
 #include <hip/hip_runtime.h>
 #include <stdint.h>

@@ -31,10 +31,10 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 // products, the one left out below 2^-22 of the product.  A scale a row, so that
 // no row's result depends on another row's size.
 //
-// dx and dw: three bf16 parts of 8 bits, to nearest: exact at any magnitude,
-// which G, whose entries reach from 1 down to nothing, needs and fp16's
-// exponents do not give (values within 2^-9 of the largest fp32 count as
-// infinite, and infinite ones make NaN).  Six partial products; those left out
+// dx and dw: three bf16 parts of 8 bits, to nearest: exact down to 2^-126, which
+// G, whose entries reach from 1 down to nothing, needs and fp16's exponents do
+// not give (values within 2^-9 of the largest fp32 count as infinite, and
+// infinite ones make NaN).  Six partial products; those left out
 // are below 2^-24 of the product together.
 //
 // The 16-bit matrix rate is 16 times the fp32 one, so three products cost 0.19

@@ -9,8 +9,8 @@
 // others come through ds_read_b64_tr_b16, which hands each lane four
 // consecutive K entries of its column.  The 16-byte chunks of an LDS row are
 // permuted by an exclusive or with bits of the row number, so that the lanes
-// that one cycle of a read serves meet different banks (measured: no bank
-// conflicts in either kind of read); the loads' lane addresses apply the
+// that one cycle of a read serves meet different banks (counted: no conflict
+// cycle in either kind of read); the loads' lane addresses apply the
 // permutation, since a direct-to-LDS load writes its lanes' data in lane order.
 //
 // A block takes one tile after another, and its loads run ahead of its products
@@ -23,10 +23,9 @@
 // phase that first reads the next buffer.
 //
 // Measured at 8192^3 in bf16: 830 us, 1324 TFLOP/s (the library's product:
-// 849 us), the matrix pipe busy 73% of cycles at the 1.73 GHz the card then
-// holds; with all of a step's loads issued at its start 870 us at 1.96 GHz and
-// 62%.  v_mfma 32x32x16 in place of 16x16x32 took 3% fewer cycles and 7% more
-// time: the clock falls further.
+// 849 us); with all of a step's loads issued at its start 870 us, with v_mfma
+// 32x32x16 in place of 16x16x32 7% more.  In the logits of (4096, 4096, 32000) the
+// matrix pipes are busy 72% of cycles.
 #pragma once
 
 #include <type_traits>

@@ -81,6 +81,13 @@ def linear_cross_entropy(input: torch.Tensor, weight: torch.Tensor, target: torc
     Gradients reach input and weight.  The backward makes the logits again in
     pieces of the vocabulary; its workspace, and the forward's, grow with
     N * D and with N and D times one piece, not with N * V.
+
+    Sums are fp32, and fp32 products good to 2^-21; an fp32 element's digits
+    below 2^-39 of the largest magnitude in its row do not enter the logits,
+    and magnitudes above 2^116 may overflow in the gradients.  In fp16 and bf16
+    the gradient of the logits is rounded to the type before its products; in
+    fp16 what lies below 2^-39 of the largest row's is lost.  At most 2^23
+    tokens, 2^28 vocabulary entries and 2^20 columns.
     """
     ext._check(input.dim() >= 1 and tuple(input.shape[:-1]) == tuple(target.shape),
                "target must have input's shape without its last dimension")
@@ -127,6 +134,9 @@ def topk_distillation(logits: torch.Tensor, teacher_logits: torch.Tensor, teache
     outside [0, V) makes the row's loss and gradient NaN; an index that comes
     several times takes the sum of its probabilities.  reduction: "none",
     "sum", or "mean" over the rows that have a teacher (0 where none has).
+
+    At most 2^22 rows of 2^28 columns and 1024 teacher entries a row; the
+    temperature's square and its inverse have to be normal fp32 numbers.
 
     The gradient reaches logits, in their type; the teacher gets none.  3-D
     logits whose last dimension is contiguous are read where they are
@@ -188,7 +198,8 @@ def router_balance(logits: torch.Tensor, index: torch.Tensor, mask: Optional[tor
     experts * sum_e counts[e] / (n * top) * mean of softmax(logits)[e], z_loss =
     mean of logsumexp(logits)^2, both fp32 and 0 where n is 0.  Choices outside
     [0, experts) count for no expert.  Gradients of both losses reach logits;
-    the counts are constants.
+    the counts are constants.  At most 1024 experts, 1024 choices a token and
+    2^31 - 1 choices.
     """
     ext._check(logits.dim() >= 1 and tuple(logits.shape[:-1]) == tuple(index.shape[:-1]) and index.dim() >= 1,
                "index must be (..., top) with the tokens of logits")

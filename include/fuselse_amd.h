@@ -347,10 +347,18 @@ int fl_sparse_blocked_grad(const float* node_flows, const float* node_mars, cons
  * count in the mean, and their x is not read (it may hold anything).  Any
  * other target outside [0, V) makes the row's loss NaN, and with it the
  * gradients it takes part in.  Products of fp16 and bf16 are exact, of fp32
- * to about 2^-21 (an element's digits below 2^-39 of the largest magnitude
- * in its row do not enter the logits; one that is not finite, or within
- * 2^-9 of the type's largest, makes NaN of the gradients it enters); sums are
- * fp32.
+ * to about 2^-21; sums are fp32.
+ * Ranges.  fp32: an element's digits below 2^-39 of the largest magnitude in
+ * its row do not enter the logits.  The gradients, and the losses of a
+ * forward without lse over at most 64 rows, take three bf16 parts of each
+ * element instead: digits below 2^-126 may be lost, and elements within 2^-9
+ * of the type's largest count as infinite.  An element that is not finite
+ * makes infinities or NaN of the losses and gradients it enters, and leaves
+ * the other rows' as they are.  fp32 and bf16: with magnitudes
+ * above 2^116 the gradients' sums may overflow before the upstream gradient's
+ * scale brings them down.  fp16: what the softmax gradient holds below 2^-39
+ * of the largest row's grad (1 + 2 z_loss lse) is lost; in rows whose upstream
+ * gradient is below about 2^-20 of the largest that can be part of them.
  *
  * fl_linear_ce_fwd: loss fp32 [N] (reduction 0) or [1]; lse fp32
  *   [N + 2], the rows' log-sum-exps (0 for ignored ones) and two zeros, or

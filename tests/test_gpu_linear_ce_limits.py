@@ -169,7 +169,7 @@ def rounded(G, dtype):
     (513, 64, 9000, "each"),        # a target of its own for nearly every row
     (2469, 64, 125, "weighted"),    # many rows a group: its targets in several waves
     (65536, 64, 16389, "ignored"),  # several pieces
-    (1500, 320, 9000, "few"),       # dw in whole sums
+    (1500, 320, 40000, "few"),      # dw in whole sums, tiles of 256
 ])
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 def test_the_rounding_of_a_targets_entry_is_given_back(cuda, n, d, v, kind, dtype):

@@ -3,17 +3,19 @@
 ``fuselse_amd.ext`` is the extension object carrying the reference's function
 names; ``make_fuselse_logsumexp(fuselse_amd.ext, robust=True)`` builds the
 torch.logsumexp drop-in.  ``losses`` holds the training losses built on row
-log-sum-exps.  The kernels live in ``libfuselse_amd.so`` behind the
+log-sum-exps, ``layers`` the layers of a training step around them.  The kernels live in ``libfuselse_amd.so`` behind the
 C ABI declared in ``include/fuselse_amd.h``.
 """
 
 from . import ext
 from .autograd import make_fuselse_logsumexp
+from .layers import ExpertOrder, embedding, expert_combine, expert_dispatch, expert_order, layer_norm
 from .losses import RouterBalance, linear_cross_entropy, router_balance, topk_distillation
 from .selective import make_selective_log_softmax
 
 __all__ = ["ext", "make_fuselse_logsumexp", "make_selective_log_softmax", "logsumexp", "selective_log_softmax",
-           "linear_cross_entropy", "topk_distillation", "router_balance", "RouterBalance"]
+           "linear_cross_entropy", "topk_distillation", "router_balance", "RouterBalance", "embedding", "layer_norm", "expert_order",
+           "expert_dispatch", "expert_combine", "ExpertOrder"]
 
 
 _default = None

@@ -82,6 +82,18 @@ SIGNATURES = {
     "fl_router_balance_fwd": (_int, [_vp, _i64, _i64, _i64, _int, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
                                      ctypes.c_size_t, _vp]),
     "fl_router_balance_bwd": (_int, [_vp, _vp, _vp, _i64, _i64, _i64, _int, _vp, _vp, _vp, _vp, _vp]),
+    "fl_embedding_fwd": (_int, [_vp, _i64, _i64, _i64, _int, _vp, _i64, _float, _vp, _vp]),
+    "fl_embedding_bwd_workspace_bytes": (ctypes.c_size_t, [_i64, _i64, _i64]),
+    "fl_embedding_bwd": (_int, [_vp, _i64, _vp, _i64, _i64, _i64, _int, _float, _i64, _vp, _vp, ctypes.c_size_t, _vp]),
+    "fl_layer_norm_fwd": (_int, [_vp, _i64, _i64, _i64, _int, _vp, _vp, _int, _float, _vp, _vp, _vp]),
+    "fl_layer_norm_bwd_workspace_bytes": (ctypes.c_size_t, [_i64, _i64, _int]),
+    "fl_layer_norm_bwd": (_int, [_vp, _i64, _vp, _i64, _i64, _i64, _int, _vp, _int, _vp, _vp, _vp, _vp, _vp,
+                                 ctypes.c_size_t, _vp]),
+    "fl_expert_order_workspace_bytes": (ctypes.c_size_t, [_i64, _i64, _i64]),
+    "fl_expert_order": (_int, [_vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, ctypes.c_size_t, _vp]),
+    "fl_expert_dispatch": (_int, [_vp, _i64, _i64, _i64, _int, _vp, _i64, _vp, _vp]),
+    "fl_expert_combine": (_int, [_vp, _i64, _i64, _i64, _int, _vp, _i64, _vp, _int, _vp, _vp]),
+    "fl_expert_combine_bwd": (_int, [_vp, _i64, _vp, _i64, _i64, _i64, _int, _vp, _i64, _vp, _int, _vp, _vp, _vp]),
 }
 
 # the measurement library (include/fuselse_amd_diag.h)

@@ -1,0 +1,454 @@
+// Tokens in their experts' order and back, on gfx950.
+//
+//   order:    entries (t, k) sorted by expert, tokens in order within one; entries
+//             of masked tokens and of no expert behind all others.
+//   dispatch: rows[pos(t, k)] = x[t], 0 for entries that are dropped
+//   combine:  y[t] = sum_k w_tk rows[pos(t, k)]           (w = 1: dispatch's gradient)
+//   gradient: drows[pos(t, k)] = w_tk dy[t], dw_tk = dy[t] . rows[pos(t, k)]
+//
+// All run from the token's side, which knows its rows: x and dy are then read
+// once and no row is found by a search.  Nothing is added by atomics, so results
+// do not depend on the order of blocks.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <type_traits>
+
+#include "../../include/fuselse_amd.h"
+#include "fl_status.hpp"
+#include "key_sort.hpp"
+#include "row_vec.hpp"
+
+namespace fl {
+namespace experts {
+namespace {
+
+constexpr int kMaxExperts = 1024;
+constexpr int kThreads = 256;
+
+// ---------------------------------------------------------------------------
+// The order
+// ---------------------------------------------------------------------------
+struct Key {
+    const int64_t* index;
+    const uint8_t* mask;  // NULL: every token takes part
+    uint32_t top;
+    int experts;
+    // an entry's expert, or `experts` where it has none
+    __device__ __forceinline__ int operator()(int64_t i) const {
+        if (mask && !mask[(uint32_t)i / top]) return experts;
+        const int64_t e = index[i];
+        return e >= 0 && e < experts ? (int)e : experts;
+    }
+};
+
+struct OrderArgs {
+    Key key;
+    int64_t n;
+    int bits;
+    int32_t* position;
+    int64_t* counts;
+    int32_t* offsets;
+    // more than one block
+    int* hist;
+    int* total;
+    int64_t blocks;
+};
+
+__device__ __forceinline__ void write_counts(const OrderArgs& p, const int (&total)[2], const int (&start)[2]) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int b = (int)threadIdx.x + j * key_sort::kThreads;
+        if (b < p.key.experts) p.counts[b] = total[j];
+        if (b <= p.key.experts) p.offsets[b] = start[j];
+    }
+}
+
+template <bool ALONE>
+__global__ __launch_bounds__(key_sort::kThreads) void place_kernel(OrderArgs p) {
+    __shared__ key_sort::Shared sh;
+    const int64_t first = (int64_t)blockIdx.x * key_sort::kChunk;
+    const int m = (int)(p.n - first < key_sort::kChunk ? p.n - first : key_sort::kChunk);
+    const int bins = p.key.experts + 1;
+    int key[key_sort::kRounds], place[key_sort::kRounds], total[2], start[2];
+#pragma unroll
+    for (int j = 0; j < key_sort::kRounds; ++j)
+        key[j] = key_sort::entry(j) < m ? p.key(first + key_sort::entry(j)) : 0;
+    key_sort::rank(sh, key, m, bins, p.bits, place, total);
+    if constexpr (ALONE) {
+        key_sort::starts(sh, total, bins, start);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int b = (int)threadIdx.x + j * key_sort::kThreads;
+            if (b < bins) sh.start[b] = start[j];
+        }
+        __syncthreads();
+    } else {
+        key_sort::block_starts(sh, p.hist, p.total, p.blocks, bins, total, start);
+    }
+    if (blockIdx.x == 0) write_counts(p, total, start);
+#pragma unroll
+    for (int j = 0; j < key_sort::kRounds; ++j)
+        if (key_sort::entry(j) < m) {
+            const int at = key_sort::placed(sh, key[j], place[j], bins);
+            p.position[first + key_sort::entry(j)] = key[j] == p.key.experts ? ~at : at;
+        }
+}
+
+// ---------------------------------------------------------------------------
+// Rows
+// ---------------------------------------------------------------------------
+struct RowArgs {
+    const void* in;  // x, rows, or dy
+    int64_t ldi;
+    int64_t tokens, D, n;  // n = tokens * top rows
+    const int32_t* position;
+    int top;
+    const void* weights;  // [tokens, top], NULL: 1
+    bool weights_f32;
+    void* out;  // rows, y, or drows
+    const void* rows;  // gradient: the experts' rows
+    int64_t ldr;
+    void* dweights;
+    int lanes, steps;
+    int64_t items;
+    bool ragged;  // rows are no whole vectors
+};
+
+template <typename T>
+__device__ __forceinline__ float weight_of(const RowArgs& p, int64_t i) {
+    if (!p.weights) return 1.0f;
+    return p.weights_f32 ? static_cast<const float*>(p.weights)[i] : Elem<T>::scalar(static_cast<const T*>(p.weights) + i);
+}
+
+// Item of this thread's lanes and its lane among them.
+__device__ __forceinline__ int64_t first_item(const RowArgs& p, int& sub) {
+    const int group = (int)threadIdx.x / p.lanes;
+    sub = (int)threadIdx.x % p.lanes;
+    return (int64_t)blockIdx.x * (kThreads / p.lanes) + group;
+}
+__device__ __forceinline__ int64_t item_stride(const RowArgs& p) {
+    return (int64_t)gridDim.x * (kThreads / p.lanes);
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void dispatch_kernel(RowArgs p) {
+    const int nvec = row_vectors<T>(p.D);
+    int sub;
+    for (int64_t it = first_item(p, sub); it < p.items; it += item_stride(p)) {
+        const int64_t t = it / p.steps;
+        const int v = (int)(it % p.steps) * 64 + sub;
+        if (v >= nvec) continue;
+        const u32x4 x = row_load(static_cast<const T*>(p.in) + t * p.ldi, p.D, v);
+        for (int k = 0; k < p.top; ++k) {
+            const int at = p.position[t * p.top + k];
+            const int row = at < 0 ? ~at : at;
+            if (row >= p.n) continue;
+            u32x4 r = x;
+            if (at < 0) r = u32x4{0, 0, 0, 0};
+            row_store(static_cast<T*>(p.out) + row * p.D, p.D, v, r);
+        }
+    }
+}
+
+constexpr int kAhead = 8;  // rows whose loads are in flight
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void combine_kernel(RowArgs p) {
+    constexpr int VE = Elem<T>::kVec;
+    const int nvec = row_vectors<T>(p.D);
+    int sub;
+    for (int64_t it = first_item(p, sub); it < p.items; it += item_stride(p)) {
+        const int64_t t = it / p.steps;
+        const int v = (int)(it % p.steps) * 64 + sub;
+        if (v >= nvec) continue;
+        float acc[VE] = {};
+        for (int k0 = 0; k0 < p.top; k0 += kAhead) {
+            u32x4 raw[kAhead];
+            float w[kAhead];
+            bool on[kAhead];
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                const int64_t i = t * p.top + k0 + u;
+                const int at = k0 + u < p.top ? p.position[i] : -1;
+                on[u] = at >= 0 && at < p.n;
+                if (on[u]) {
+                    w[u] = weight_of<T>(p, i);
+                    raw[u] = row_load(static_cast<const T*>(p.in) + at * p.ldi, p.D, v);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u)
+                if (on[u]) {
+                    float r[VE];
+                    Elem<T>::cvt(raw[u], r);
+#pragma unroll
+                    for (int k = 0; k < VE; ++k) acc[k] = __builtin_fmaf(w[u], r[k], acc[k]);
+                }
+        }
+        row_store(static_cast<T*>(p.out) + t * p.D, p.D, v, pack_vec<T>(acc));
+    }
+}
+
+// The gradient of a combination, a token by its lanes (steps == 1) or by the
+// block: dy is read once for eight rows.
+template <typename T, bool BLOCK>
+__global__ __launch_bounds__(kThreads) void combine_bwd_kernel(RowArgs p) {
+    constexpr int VE = Elem<T>::kVec;
+    __shared__ float sh[kThreads / 64][kAhead];
+    const int nvec = row_vectors<T>(p.D);
+    int sub = (int)threadIdx.x;
+    const int team = BLOCK ? kThreads : p.lanes;
+    int64_t t = blockIdx.x, stride = gridDim.x;
+    if constexpr (!BLOCK) {
+        t = first_item(p, sub);
+        stride = item_stride(p);
+    }
+    for (; t < p.tokens; t += stride) {
+        const T* dy = static_cast<const T*>(p.in) + t * p.ldi;
+        for (int k0 = 0; k0 < p.top; k0 += kAhead) {
+            float dot[kAhead] = {};
+            for (int v = sub; v < nvec; v += team) {
+                float g[VE];
+                Elem<T>::cvt(row_load(dy, p.D, v), g);
+                const int skip = p.ragged && p.D >= VE ? (int)((int64_t)v * VE - row_vec_at<T>(p.D, v)) : 0;
+#pragma unroll
+                for (int u = 0; u < kAhead; ++u) {
+                    if (k0 + u >= p.top) break;
+                    const int64_t i = t * p.top + k0 + u;
+                    const int at = p.position[i];
+                    const int row = at < 0 ? ~at : at;
+                    if (row >= p.n) continue;
+                    float d[VE] = {};
+                    if (at >= 0) {
+                        if (p.dweights) {
+                            float r[VE];
+                            Elem<T>::cvt(row_load(static_cast<const T*>(p.rows) + row * p.ldr, p.D, v), r);
+#pragma unroll
+                            for (int k = 0; k < VE; ++k) dot[u] += k < skip ? 0.0f : g[k] * r[k];
+                        }
+                        const float w = weight_of<T>(p, i);
+#pragma unroll
+                        for (int k = 0; k < VE; ++k) d[k] = w * g[k];
+                    }
+                    if (p.out) row_store(static_cast<T*>(p.out) + row * p.D, p.D, v, pack_vec<T>(d));
+                }
+            }
+            if (!p.dweights) continue;
+            for (int d = 1; d < (BLOCK ? 64 : p.lanes); d *= 2)
+#pragma unroll
+                for (int u = 0; u < kAhead; ++u) dot[u] += __shfl_xor(dot[u], d, 64);
+            if constexpr (BLOCK) {
+                __syncthreads();
+                if ((threadIdx.x & 63) == 0)
+#pragma unroll
+                    for (int u = 0; u < kAhead; ++u) sh[threadIdx.x >> 6][u] = dot[u];
+                __syncthreads();
+            }
+            if constexpr (BLOCK) {
+                if (sub < kAhead && k0 + sub < p.top) {
+                    float s = 0.0f;
+#pragma unroll
+                    for (int w = 0; w < kThreads / 64; ++w) s += sh[w][sub];
+                    const int64_t i = t * p.top + k0 + sub;
+                    if (p.weights_f32) static_cast<float*>(p.dweights)[i] = s;
+                    else Elem<T>::put(static_cast<T*>(p.dweights) + i, s);
+                }
+            } else if (sub == 0) {
+#pragma unroll
+                for (int u = 0; u < kAhead; ++u) {
+                    if (k0 + u >= p.top) break;
+                    const int64_t i = t * p.top + k0 + u;
+                    if (p.weights_f32) static_cast<float*>(p.dweights)[i] = dot[u];
+                    else Elem<T>::put(static_cast<T*>(p.dweights) + i, dot[u]);
+                }
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+int check_sizes(const char* name, int64_t tokens, int64_t top) {
+    FL_CHECK(tokens >= 0 && top >= 1, "%s: bad shape (tokens=%lld, top=%lld)", name, (long long)tokens,
+             (long long)top);
+    if (top > 1024 || tokens > (1 << 30) || tokens * top >= ((int64_t)1 << 31))
+        return set_error(FL_ERANGE, "%s: at most 2^30 tokens, 1024 choices each and 2^31 - 1 choices", name);
+    return ok();
+}
+
+int check_rows(const char* name, int64_t tokens, int64_t D, int dtype, int64_t top) {
+    const int rc = check_sizes(name, tokens, top);
+    if (rc != FL_OK) return rc;
+    FL_CHECK(D >= 1, "%s: bad shape (D=%lld)", name, (long long)D);
+    FL_CHECK(dtype >= 0 && dtype <= 2, "%s: dtype %d", name, dtype);
+    if (D > (1 << 24)) return set_error(FL_ERANGE, "%s: at most 2^24 columns", name);
+    return ok();
+}
+
+bool aligned(const void* p, int dtype) { return (reinterpret_cast<uintptr_t>(p) & (dtype == 0 ? 3u : 1u)) == 0; }
+
+template <typename F>
+void by_type(int dtype, F f) {
+    if (dtype == 0) f(float{});
+    else if (dtype == 1) f(_Float16{});
+    else f(bf16_t{});
+}
+
+int vectors(int64_t D, int dtype) { return dtype == 0 ? row_vectors<float>(D) : row_vectors<_Float16>(D); }
+
+void split_rows(RowArgs& a, int dtype) {
+    const int nvec = vectors(a.D, dtype);
+    a.lanes = row_lanes(nvec);
+    a.steps = row_steps(nvec);
+    a.items = a.tokens * a.steps;
+    a.ragged = a.D % (dtype == 0 ? 4 : 8) != 0;
+}
+
+unsigned grid_of(int64_t items, int per_block) {
+    const int64_t want = (items + per_block - 1) / per_block;
+    return (unsigned)(want < (1 << 22) ? want : (1 << 22));
+}
+
+}  // namespace
+}  // namespace experts
+}  // namespace fl
+
+using namespace fl;
+using namespace fl::experts;
+
+extern "C" size_t fl_expert_order_workspace_bytes(int64_t tokens, int64_t top, int64_t experts) {
+    if (tokens < 0 || top < 1 || experts < 1 || experts > kMaxExperts || tokens > (1 << 30) || top > 1024) return 0;
+    const int64_t blocks = key_sort::chunks(tokens * top);
+    return blocks <= 1 ? 0 : (size_t)(4 * (blocks + 1) * (experts + 1));
+}
+
+extern "C" int fl_expert_order(const int64_t* index, int64_t tokens, int64_t top, int64_t experts, const uint8_t* mask,
+                               int32_t* position, int64_t* counts, int32_t* offsets, void* workspace,
+                               size_t workspace_bytes, void* stream) {
+    const char* name = "fl_expert_order";
+    FL_CHECK(experts >= 1, "%s: bad shape (experts=%lld)", name, (long long)experts);
+    const int rc = check_sizes(name, tokens, top);
+    if (rc != FL_OK) return rc;
+    if (experts > kMaxExperts) return set_error(FL_ERANGE, "%s: at most %d experts", name, kMaxExperts);
+    FL_CHECK(counts && offsets && (tokens == 0 || (index && position)), "%s: NULL pointer argument", name);
+    const size_t need = fl_expert_order_workspace_bytes(tokens, top, experts);
+    FL_CHECK(workspace_bytes >= need, "%s: workspace of %llu bytes, %llu needed", name,
+             (unsigned long long)workspace_bytes, (unsigned long long)need);
+    FL_CHECK(need == 0 || (workspace && (reinterpret_cast<uintptr_t>(workspace) & 3u) == 0),
+             "%s: workspace is not 4-byte aligned", name);
+    OrderArgs a{};
+    a.key = Key{index, mask, (uint32_t)top, (int)experts};
+    a.n = tokens * top;
+    a.bits = key_sort::bits_of((int)experts + 1);
+    a.position = position;
+    a.counts = counts;
+    a.offsets = offsets;
+    a.blocks = key_sort::chunks(a.n);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (a.blocks <= 1) {
+        place_kernel<true><<<1, key_sort::kThreads, 0, s>>>(a);
+        return launch_status(name);
+    }
+    const int bins = (int)experts + 1;
+    a.total = static_cast<int*>(workspace);
+    a.hist = a.total + bins;
+    const unsigned blocks = (unsigned)a.blocks;
+    key_sort::count_kernel<<<blocks, key_sort::kThreads, 0, s>>>(a.key, a.n, bins, a.hist);
+    key_sort::sum_kernel<<<(unsigned)((bins + 3) / 4), 256, 0, s>>>(a.hist, a.blocks, bins, a.total);
+    place_kernel<false><<<blocks, key_sort::kThreads, 0, s>>>(a);
+    return launch_status(name);
+}
+
+extern "C" int fl_expert_dispatch(const void* x, int64_t row_stride, int64_t tokens, int64_t D, int dtype,
+                                  const int32_t* position, int64_t top, void* rows, void* stream) {
+    const char* name = "fl_expert_dispatch";
+    const int rc = check_rows(name, tokens, D, dtype, top);
+    if (rc != FL_OK || tokens == 0) return rc;
+    FL_CHECK(row_stride >= D, "%s: rows of x overlap", name);
+    FL_CHECK(x && position && rows, "%s: NULL pointer argument", name);
+    FL_CHECK(aligned(x, dtype) && aligned(rows, dtype), "%s: pointers are not element-aligned", name);
+    RowArgs a{};
+    a.in = x;
+    a.ldi = row_stride;
+    a.tokens = tokens;
+    a.D = D;
+    a.n = tokens * top;
+    a.position = position;
+    a.top = (int)top;
+    a.out = rows;
+    split_rows(a, dtype);
+    by_type(dtype, [&](auto t) {
+        dispatch_kernel<decltype(t)><<<grid_of(a.items, kThreads / a.lanes), kThreads, 0, static_cast<hipStream_t>(stream)>>>(a);
+    });
+    return launch_status(name);
+}
+
+extern "C" int fl_expert_combine(const void* rows, int64_t row_stride, int64_t tokens, int64_t D, int dtype,
+                                 const int32_t* position, int64_t top, const void* weights, int weights_dtype,
+                                 void* out, void* stream) {
+    const char* name = "fl_expert_combine";
+    const int rc = check_rows(name, tokens, D, dtype, top);
+    if (rc != FL_OK || tokens == 0) return rc;
+    FL_CHECK(row_stride >= D, "%s: the experts' rows overlap", name);
+    FL_CHECK(!weights || weights_dtype == 0 || weights_dtype == dtype, "%s: weights' dtype %d", name, weights_dtype);
+    FL_CHECK(rows && position && out, "%s: NULL pointer argument", name);
+    FL_CHECK(aligned(rows, dtype) && aligned(out, dtype) && aligned(weights, weights_dtype),
+             "%s: pointers are not element-aligned", name);
+    RowArgs a{};
+    a.in = rows;
+    a.ldi = row_stride;
+    a.tokens = tokens;
+    a.D = D;
+    a.n = tokens * top;
+    a.position = position;
+    a.top = (int)top;
+    a.weights = weights;
+    a.weights_f32 = weights_dtype == 0;
+    a.out = out;
+    split_rows(a, dtype);
+    by_type(dtype, [&](auto t) {
+        combine_kernel<decltype(t)><<<grid_of(a.items, kThreads / a.lanes), kThreads, 0, static_cast<hipStream_t>(stream)>>>(a);
+    });
+    return launch_status(name);
+}
+
+extern "C" int fl_expert_combine_bwd(const void* grad, int64_t grad_stride, const void* rows, int64_t row_stride,
+                                     int64_t tokens, int64_t D, int dtype, const int32_t* position, int64_t top,
+                                     const void* weights, int weights_dtype, void* grad_rows, void* grad_weights,
+                                     void* stream) {
+    const char* name = "fl_expert_combine_bwd";
+    const int rc = check_rows(name, tokens, D, dtype, top);
+    if (rc != FL_OK || tokens == 0) return rc;
+    FL_CHECK(grad_stride >= D && (!grad_weights || row_stride >= D), "%s: rows overlap", name);
+    FL_CHECK(weights_dtype == 0 || weights_dtype == dtype, "%s: weights' dtype %d", name, weights_dtype);
+    FL_CHECK(grad && position && weights && (rows || !grad_weights), "%s: NULL pointer argument", name);
+    FL_CHECK(aligned(grad, dtype) && aligned(rows, dtype) && aligned(grad_rows, dtype) &&
+                 aligned(weights, weights_dtype) && aligned(grad_weights, weights_dtype),
+             "%s: pointers are not element-aligned", name);
+    if (!grad_rows && !grad_weights) return ok();
+    RowArgs a{};
+    a.in = grad;
+    a.ldi = grad_stride;
+    a.tokens = tokens;
+    a.D = D;
+    a.n = tokens * top;
+    a.position = position;
+    a.top = (int)top;
+    a.weights = weights;
+    a.weights_f32 = weights_dtype == 0;
+    a.out = grad_rows;
+    a.rows = rows;
+    a.ldr = row_stride;
+    a.dweights = grad_weights;
+    split_rows(a, dtype);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    by_type(dtype, [&](auto t) {
+        if (a.steps > 1)
+            combine_bwd_kernel<decltype(t), true><<<grid_of(tokens, 1), kThreads, 0, s>>>(a);
+        else
+            combine_bwd_kernel<decltype(t), false><<<grid_of(tokens, kThreads / a.lanes), kThreads, 0, s>>>(a);
+    });
+    return launch_status(name);
+}

@@ -1151,3 +1151,270 @@ def router_balance_backward(grad_balance, grad_z, logits: torch.Tensor, mask, ls
                and t.is_contiguous() and t.numel() == n), f"{nm} must be contiguous CUDA float32 of {n}")
     _check_device(logits, "logits", grad_balance=grad_balance, grad_z=grad_z, lse=lse, coef=coef)
     return _router_bwd(grad_balance, grad_z, logits, mask, lse, coef)
+
+
+# ---------------------------------------------------------------------------
+# Layers around the losses (no reference counterpart)
+# ---------------------------------------------------------------------------
+def _check_rows(t, name):
+    """t is 2D with contiguous rows that do not overlap, of a type the kernels
+    take; a tensor of one row may carry any row stride."""
+    _check(t.is_cuda, f"{name} must be CUDA")
+    _check(t.dtype in _DTYPE_CODE, f"{name} must be float32, float16 or bfloat16")
+    _check(t.dim() == 2 and t.shape[1] >= 1, f"{name} must be 2D with at least one column")
+    _check((t.stride(1) == 1 or t.shape[1] == 1) and (t.stride(0) >= t.shape[1] or t.shape[0] <= 1),
+           f"{name} must have contiguous rows that do not overlap")
+
+
+def _check_vector(t, name, n, dtypes):
+    _check(t.is_cuda and t.is_contiguous() and t.dim() == 1 and t.shape[0] == n and t.dtype in dtypes,
+           f"{name} must be a contiguous CUDA tensor ({n},) of {' or '.join(str(d) for d in dtypes)}")
+
+
+def _ptr(t):
+    return t.data_ptr() if t is not None else None
+
+
+def _check_embedding(weight, index):
+    _check_rows(weight, "weight")
+    _check(weight.shape[0] >= 1, "weight must not be empty")
+    _check(index.is_cuda, "index must be CUDA")
+    _check(index.dtype == torch.int64 and index.dim() == 1 and index.is_contiguous(),
+           "index must be a contiguous int64 tensor (N,)")
+    _check_device(weight, "weight", index=index)
+
+
+def embedding(weight: torch.Tensor, index: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
+    """scale * weight[index], (N, D) of weight's type: weight (V, D) fp32, fp16
+    or bf16 with contiguous rows, index int64 (N,).  An index outside [0, V)
+    gives a row of NaN."""
+    _check_embedding(weight, index)
+    return _embedding_fwd(weight, index, scale)
+
+
+def _embedding_fwd(weight, index, scale):
+    V, D = weight.shape
+    N = index.shape[0]
+    out = torch.empty((N, D), dtype=weight.dtype, device=weight.device)
+    if N:
+        with _on_device(weight):
+            _lib.call("fl_embedding_fwd", weight.data_ptr(), _row_stride(weight), V, D, _DTYPE_CODE[weight.dtype],
+                      index.data_ptr(), N, scale, out.data_ptr(), _stream(weight))
+    return out
+
+
+def _embedding_bwd(grad, index, V, scale, padding):
+    N, D = grad.shape
+    dev = grad.device
+    out = torch.empty((V, D), dtype=grad.dtype, device=dev)
+    nbytes = _remembered(("embedding", N, V, D), "fl_embedding_bwd_workspace_bytes", N, V, D)
+    with _on_device(grad):
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        _lib.call("fl_embedding_bwd", grad.data_ptr(), _row_stride(grad), index.data_ptr(), N, V, D,
+                  _DTYPE_CODE[grad.dtype], scale, padding, out.data_ptr(), ws.data_ptr(), nbytes, _stream(grad))
+    return out
+
+
+def embedding_backward(grad_output: torch.Tensor, index: torch.Tensor, num_embeddings: int, scale: float = 1.0,
+                       padding_idx: int = -1) -> torch.Tensor:
+    """Gradient (num_embeddings, D) of embedding's weight, of grad_output's
+    type; grad_output (N, D) with contiguous rows.  Tokens of padding_idx (one
+    outside [0, num_embeddings): none) and of indexes outside the matrix give
+    nothing."""
+    _check_rows(grad_output, "grad_output")
+    _check(num_embeddings >= 1, "num_embeddings must be at least 1")
+    _check(index.is_cuda and index.dtype == torch.int64 and index.dim() == 1 and index.is_contiguous()
+           and index.shape[0] == grad_output.shape[0], "index must be a contiguous CUDA int64 tensor (N,)")
+    _check_device(grad_output, "grad_output", index=index)
+    return _embedding_bwd(grad_output, index, num_embeddings, scale, padding_idx)
+
+
+def _check_norm(x, weight, bias):
+    _check_rows(x, "x")
+    of = (x.dtype, torch.float32) if x.dtype != torch.float32 else (torch.float32,)
+    for t, nm in ((weight, "weight"), (bias, "bias")):
+        if t is not None:
+            _check_vector(t, nm, x.shape[1], of)
+    _check(weight is None or bias is None or weight.dtype == bias.dtype, "weight and bias must be of one type")
+    _check_device(x, "x", weight=weight, bias=bias)
+
+
+def _params_code(x, weight, bias):
+    t = weight if weight is not None else bias
+    return _DTYPE_CODE[t.dtype] if t is not None else 0
+
+
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+               eps: float = 1e-5, with_stats: bool = True):
+    """Layer norm of the rows of x (N, D), fp32, fp16 or bf16: (y, stats), stats
+    (N, 4) fp32 for the backward or None.  weight and bias (D,) of x's type or
+    fp32, or None."""
+    _check_norm(x, weight, bias)
+    return _norm_fwd(x, weight, bias, eps, with_stats)
+
+
+def _norm_fwd(x, weight, bias, eps, with_stats):
+    N, D = x.shape
+    y = torch.empty((N, D), dtype=x.dtype, device=x.device)
+    stats = torch.empty((N, 4), dtype=torch.float32, device=x.device) if with_stats else None
+    _check(eps >= 0, "eps must be at least 0")
+    if N:
+        with _on_device(x):
+            _lib.call("fl_layer_norm_fwd", x.data_ptr(), _row_stride(x), N, D, _DTYPE_CODE[x.dtype], _ptr(weight),
+                      _ptr(bias), _params_code(x, weight, bias), eps, y.data_ptr(), _ptr(stats), _stream(x))
+    return y, stats
+
+
+def _norm_bwd(grad, x, weight, bias, stats, need_x, need_weight, need_bias):
+    N, D = x.shape
+    dev = x.device
+    dx = torch.empty((N, D), dtype=x.dtype, device=dev) if need_x else None
+    dw = torch.empty_like(weight) if need_weight else None
+    db = torch.empty_like(bias) if need_bias else None
+    dt = _DTYPE_CODE[x.dtype]
+    nbytes = 0
+    if need_weight or need_bias:
+        nbytes = _remembered(("norm", N, D, dt), "fl_layer_norm_bwd_workspace_bytes", N, D, dt)
+    with _on_device(x):
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        _lib.call("fl_layer_norm_bwd", grad.data_ptr(), _row_stride(grad), x.data_ptr(), _row_stride(x), N, D, dt,
+                  _ptr(weight), _params_code(x, weight, bias), stats.data_ptr(), _ptr(dx), _ptr(dw), _ptr(db),
+                  ws.data_ptr(), nbytes, _stream(x))
+    return dx, dw, db
+
+
+def layer_norm_backward(grad_output: torch.Tensor, x: torch.Tensor, weight, bias, stats: torch.Tensor,
+                        need_x: bool = True, need_weight: bool = True, need_bias: bool = True):
+    """Gradients (of x, of weight, of bias) of layer_norm, None for one that is
+    not needed or not there; stats as the forward returned them."""
+    _check_norm(x, weight, bias)
+    _check_rows(grad_output, "grad_output")
+    _check(grad_output.shape == x.shape and grad_output.dtype == x.dtype, "grad_output must have x's shape and type")
+    _check(stats.is_cuda and stats.dtype == torch.float32 and stats.is_contiguous()
+           and tuple(stats.shape) == (x.shape[0], 4), "stats must be contiguous CUDA float32 (N, 4)")
+    _check_device(x, "x", grad_output=grad_output, stats=stats)
+    return _norm_bwd(grad_output, x, weight, bias, stats, need_x, need_weight and weight is not None,
+                     need_bias and bias is not None)
+
+
+def _check_order(index, experts, mask):
+    _check(index.is_cuda, "index must be CUDA")
+    _check(index.dtype == torch.int64 and index.dim() == 2 and index.is_contiguous() and index.shape[1] >= 1,
+           "index must be a contiguous int64 tensor (tokens, top)")
+    _check(experts >= 1, "num_experts must be at least 1")
+    if mask is not None:
+        _check(mask.is_cuda and mask.dtype == torch.bool and mask.is_contiguous() and mask.dim() == 1
+               and mask.shape[0] == index.shape[0], "mask must be a contiguous CUDA bool tensor (tokens,)")
+    _check_device(index, "index", mask=mask)
+
+
+def expert_order(index: torch.Tensor, num_experts: int, mask: Optional[torch.Tensor] = None):
+    """The order of the entries of index (tokens, top) int64 by expert:
+    (position int32 (tokens, top), counts int64 (experts,), offsets int32
+    (experts + 1,)).  position is an entry's place p, or -1 - p where it is
+    dropped (masked tokens, experts outside [0, num_experts)), which come
+    last."""
+    _check_order(index, num_experts, mask)
+    return _order(index, num_experts, mask)
+
+
+def _order(index, experts, mask):
+    T, K = index.shape
+    dev = index.device
+    position = torch.empty((T, K), dtype=torch.int32, device=dev)
+    counts = torch.empty((experts,), dtype=torch.int64, device=dev)
+    offsets = torch.empty((experts + 1,), dtype=torch.int32, device=dev)
+    nbytes = _remembered(("order", T, K, experts), "fl_expert_order_workspace_bytes", T, K, experts)
+    with _on_device(index):
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        _lib.call("fl_expert_order", index.data_ptr(), T, K, experts, _ptr(mask), position.data_ptr(),
+                  counts.data_ptr(), offsets.data_ptr(), _ptr(ws), nbytes, _stream(index))
+    return position, counts, offsets
+
+
+def _check_position(ref, ref_name, position):
+    _check(position.is_cuda and position.dtype == torch.int32 and position.dim() == 2 and position.is_contiguous()
+           and position.shape[1] >= 1, "position must be a contiguous CUDA int32 tensor (tokens, top)")
+    _check_device(ref, ref_name, position=position)
+
+
+def _check_dispatch(x, position):
+    _check_rows(x, "x")
+    _check_position(x, "x", position)
+    _check(x.shape[0] == position.shape[0], "x must be (tokens, D) with the tokens of position")
+
+
+def expert_dispatch(x: torch.Tensor, position: torch.Tensor) -> torch.Tensor:
+    """The rows of x (tokens, D) at their entries' places: (tokens * top, D),
+    zeros at the places of dropped entries.  position as expert_order gives
+    it."""
+    _check_dispatch(x, position)
+    return _dispatch(x, position)
+
+
+def _dispatch(x, position):
+    T, D = x.shape
+    K = position.shape[1]
+    rows = torch.empty((T * K, D), dtype=x.dtype, device=x.device)
+    if T:
+        with _on_device(x):
+            _lib.call("fl_expert_dispatch", x.data_ptr(), _row_stride(x), T, D, _DTYPE_CODE[x.dtype],
+                      position.data_ptr(), K, rows.data_ptr(), _stream(x))
+    return rows
+
+
+def _check_combine(rows, weights, position):
+    _check_rows(rows, "rows")
+    _check_position(rows, "rows", position)
+    T, K = position.shape
+    _check(rows.shape[0] == T * K, "rows must be (tokens * top, D)")
+    if weights is not None:
+        _check(weights.is_cuda and weights.is_contiguous() and tuple(weights.shape) == (T, K)
+               and weights.dtype in (rows.dtype, torch.float32),
+               "weights must be a contiguous CUDA tensor (tokens, top) of rows' type or float32")
+    _check_device(rows, "rows", weights=weights)
+
+
+def expert_combine(rows: torch.Tensor, weights: Optional[torch.Tensor], position: torch.Tensor) -> torch.Tensor:
+    """(tokens, D), each token's sum of its entries' rows times their weights
+    (None: 1, the gradient of expert_dispatch).  Dropped entries give nothing and
+    what belongs to them is not read."""
+    _check_combine(rows, weights, position)
+    return _combine(rows, weights, position)
+
+
+def _combine(rows, weights, position):
+    T, K = position.shape
+    D = rows.shape[1]
+    out = torch.empty((T, D), dtype=rows.dtype, device=rows.device)
+    if T:
+        with _on_device(rows):
+            _lib.call("fl_expert_combine", rows.data_ptr(), _row_stride(rows), T, D, _DTYPE_CODE[rows.dtype],
+                      position.data_ptr(), K, _ptr(weights), _DTYPE_CODE[weights.dtype] if weights is not None else 0,
+                      out.data_ptr(), _stream(rows))
+    return out
+
+
+def _combine_bwd(grad, rows, weights, position, need_rows, need_weights):
+    T, K = position.shape
+    D = rows.shape[1]
+    d_rows = torch.empty((T * K, D), dtype=rows.dtype, device=rows.device) if need_rows else None
+    d_weights = torch.empty_like(weights) if need_weights else None
+    if T:
+        with _on_device(rows):
+            _lib.call("fl_expert_combine_bwd", grad.data_ptr(), _row_stride(grad), rows.data_ptr(), _row_stride(rows),
+                      T, D, _DTYPE_CODE[rows.dtype], position.data_ptr(), K, weights.data_ptr(),
+                      _DTYPE_CODE[weights.dtype], _ptr(d_rows), _ptr(d_weights), _stream(rows))
+    return d_rows, d_weights
+
+
+def expert_combine_backward(grad_output: torch.Tensor, rows: torch.Tensor, weights: torch.Tensor,
+                            position: torch.Tensor, need_rows: bool = True, need_weights: bool = True):
+    """Gradients (of rows, of weights) of expert_combine, None for one that is
+    not needed, 0 for dropped entries."""
+    _check_combine(rows, weights, position)
+    _check_rows(grad_output, "grad_output")
+    _check(tuple(grad_output.shape) == (position.shape[0], rows.shape[1]) and grad_output.dtype == rows.dtype,
+           "grad_output must be (tokens, D) of rows' type")
+    _check_device(rows, "rows", grad_output=grad_output)
+    return _combine_bwd(grad_output, rows, weights, position, need_rows, need_weights)

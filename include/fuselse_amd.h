@@ -457,6 +457,89 @@ int fl_router_balance_bwd(const float* grad_balance, const float* grad_z, const 
                           int64_t tokens, int64_t experts, int dtype, const uint8_t* mask, const float* lse,
                           const float* coef, void* grad_logits, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Layers of a language model's training step around those losses.  dtype: 0
+ * fp32, 1 fp16, 2 bf16.  Sums are fp32, results are rounded once; no result
+ * depends on the order of atomics.  Workspaces as above.
+ * ------------------------------------------------------------------------- */
+
+/* ---------------------------------------------------------------------------
+ * Embedding lookup: out[i] = scale * weight[index[i]], weight [V, D], rows
+ * row_stride elements apart; index int64 [N]; out [N, D] contiguous, of weight's
+ * type (exact copies where scale is 1).  An index outside [0, V) gives a row of
+ * NaN.
+ * fl_embedding_bwd: grad_weight [V, D] contiguous, written in full,
+ *   grad_weight[v] = scale * sum of grad[i] over the i of index v, in their
+ *   order; 0 for v without any.  Tokens of index `padding` and of indexes
+ *   outside [0, V) give nothing (a padding outside [0, V): none).  workspace
+ *   256-byte aligned.
+ * At most 2^30 tokens and vocabulary entries and 2^20 columns (FL_ERANGE).
+ * ------------------------------------------------------------------------- */
+int fl_embedding_fwd(const void* weight, int64_t row_stride, int64_t V, int64_t D, int dtype, const int64_t* index,
+                     int64_t N, float scale, void* out, void* stream);
+size_t fl_embedding_bwd_workspace_bytes(int64_t N, int64_t V, int64_t D);
+int fl_embedding_bwd(const void* grad, int64_t grad_stride, const int64_t* index, int64_t N, int64_t V, int64_t D,
+                     int dtype, float scale, int64_t padding, void* grad_weight, void* workspace,
+                     size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Layer norm over rows of D elements, row_stride apart:
+ *   y = (x - mean) / sqrt(variance + eps) * weight + bias
+ * with the variance over D.  weight and bias [D] of params_dtype (0 or dtype),
+ * either may be NULL; y [rows, D] contiguous, of x's type.  Squares of
+ * differences from the mean are held in fp32: rows that spread over more than
+ * about 2^63 overflow.
+ * fl_layer_norm_fwd: stats fp32 [rows, 4] (16-byte aligned) for the backward,
+ *   or NULL.
+ * fl_layer_norm_bwd: dx [rows, D] contiguous, of x's type; dweight and dbias
+ *   [D] of params_dtype; any of the three may be NULL.  The workspace is needed
+ *   for the last two.
+ * At most 2^31 - 1 rows and 2^24 columns (FL_ERANGE).
+ * ------------------------------------------------------------------------- */
+int fl_layer_norm_fwd(const void* x, int64_t row_stride, int64_t rows, int64_t D, int dtype, const void* weight,
+                      const void* bias, int params_dtype, float eps, void* y, float* stats, void* stream);
+size_t fl_layer_norm_bwd_workspace_bytes(int64_t rows, int64_t D, int dtype);
+int fl_layer_norm_bwd(const void* grad, int64_t grad_stride, const void* x, int64_t row_stride, int64_t rows,
+                      int64_t D, int dtype, const void* weight, int params_dtype, const float* stats, void* dx,
+                      void* dweight, void* dbias, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Tokens in their experts' order, and back.
+ *
+ * fl_expert_order: index int64 [tokens, top], mask as for the router.  The
+ *   tokens * top entries are put in the order of their experts, entries of one
+ *   expert in the order of index; entries of masked tokens and of experts
+ *   outside [0, experts) are dropped and come last.  position int32
+ *   [tokens, top]: an entry's place p, or -1 - p where it is dropped; counts
+ *   int64 [experts]; offsets int32 [experts + 1]: expert e has the places
+ *   [offsets[e], offsets[e + 1]).  At most 1024 experts, 1024 choices a token,
+ *   2^30 tokens and 2^31 - 1 choices (FL_ERANGE).
+ * fl_expert_dispatch: rows[position[t, k]] = x[t], rows of dropped entries 0: x
+ *   [tokens, D], rows row_stride apart; rows [tokens * top, D] contiguous.
+ * fl_expert_combine: out[t] = sum_k weights[t, k] * rows[position[t, k]] over the
+ *   entries that are not dropped, rows row_stride apart, out [tokens, D]
+ *   contiguous; weights [tokens, top] contiguous of weights_dtype (0 or dtype),
+ *   or NULL: 1 (the gradient of a dispatch).  What belongs to a dropped entry is
+ *   not read.
+ * fl_expert_combine_bwd: grad [tokens, D] of out; grad_rows [tokens * top, D]
+ *   contiguous (0 where dropped) and grad_weights [tokens, top] of
+ *   weights_dtype (0 where dropped); either may be NULL.
+ * Places outside [0, tokens * top) are taken as dropped, without a row.
+ * At most 2^24 columns.
+ * ------------------------------------------------------------------------- */
+size_t fl_expert_order_workspace_bytes(int64_t tokens, int64_t top, int64_t experts);
+int fl_expert_order(const int64_t* index, int64_t tokens, int64_t top, int64_t experts, const uint8_t* mask,
+                    int32_t* position, int64_t* counts, int32_t* offsets, void* workspace, size_t workspace_bytes,
+                    void* stream);
+int fl_expert_dispatch(const void* x, int64_t row_stride, int64_t tokens, int64_t D, int dtype,
+                       const int32_t* position, int64_t top, void* rows, void* stream);
+int fl_expert_combine(const void* rows, int64_t row_stride, int64_t tokens, int64_t D, int dtype,
+                      const int32_t* position, int64_t top, const void* weights, int weights_dtype, void* out,
+                      void* stream);
+int fl_expert_combine_bwd(const void* grad, int64_t grad_stride, const void* rows, int64_t row_stride, int64_t tokens,
+                          int64_t D, int dtype, const int32_t* position, int64_t top, const void* weights,
+                          int weights_dtype, void* grad_rows, void* grad_weights, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -112,7 +112,8 @@ struct RowArgs {
     void* dweights;
     int lanes, steps;
     int64_t items;
-    bool ragged;  // rows are no whole vectors
+    bool ragged;   // rows are no whole vectors
+    bool through;  // rows of out are whole, aligned vectors
 };
 
 template <typename T>
@@ -121,65 +122,95 @@ __device__ __forceinline__ float weight_of(const RowArgs& p, int64_t i) {
     return p.weights_f32 ? static_cast<const float*>(p.weights)[i] : Elem<T>::scalar(static_cast<const T*>(p.weights) + i);
 }
 
-// Item of this thread's lanes and its lane among them.
+// Item of this thread's lanes and its lane among them.  With WAVE a wave has one
+// item, and what belongs to it is read by scalar loads.
+template <bool WAVE>
 __device__ __forceinline__ int64_t first_item(const RowArgs& p, int& sub) {
-    const int group = (int)threadIdx.x / p.lanes;
-    sub = (int)threadIdx.x % p.lanes;
-    return (int64_t)blockIdx.x * (kThreads / p.lanes) + group;
-}
-__device__ __forceinline__ int64_t item_stride(const RowArgs& p) {
-    return (int64_t)gridDim.x * (kThreads / p.lanes);
-}
-
-template <typename T>
-__global__ __launch_bounds__(kThreads) void dispatch_kernel(RowArgs p) {
-    const int nvec = row_vectors<T>(p.D);
-    int sub;
-    for (int64_t it = first_item(p, sub); it < p.items; it += item_stride(p)) {
-        const int64_t t = it / p.steps;
-        const int v = (int)(it % p.steps) * 64 + sub;
-        if (v >= nvec) continue;
-        const u32x4 x = row_load(static_cast<const T*>(p.in) + t * p.ldi, p.D, v);
-        for (int k = 0; k < p.top; ++k) {
-            const int at = p.position[t * p.top + k];
-            const int row = at < 0 ? ~at : at;
-            if (row >= p.n) continue;
-            u32x4 r = x;
-            if (at < 0) r = u32x4{0, 0, 0, 0};
-            row_store(static_cast<T*>(p.out) + row * p.D, p.D, v, r);
-        }
+    if constexpr (WAVE) {
+        sub = (int)threadIdx.x & 63;
+        return (int64_t)blockIdx.x * (kThreads / 64) + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    } else {
+        sub = (int)threadIdx.x % p.lanes;
+        return (int64_t)blockIdx.x * (kThreads / p.lanes) + (int)threadIdx.x / p.lanes;
     }
+}
+template <bool WAVE>
+__device__ __forceinline__ int64_t item_stride(const RowArgs& p) {
+    return (int64_t)gridDim.x * (kThreads / (WAVE ? 64 : p.lanes));
 }
 
 constexpr int kAhead = 8;  // rows whose loads are in flight
 
-template <typename T>
+// Places of the token's entries k0 .. k0 + 7; INT_MAX, outside all rows, past
+// the last.
+__device__ __forceinline__ void load_places(const RowArgs& p, int64_t t, int k0, int (&at)[kAhead]) {
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) at[u] = k0 + u < p.top ? p.position[t * p.top + k0 + u] : 0x7FFFFFFF;
+}
+
+// x is read with plain loads, since what made it has often left it in the caches
+// (with the nontemporal hint (16383, 2048) in bf16 to 6 experts each takes 98 us
+// for 80), and a wave's rows are written through to memory (77).
+template <typename T, bool WAVE>
+__global__ __launch_bounds__(kThreads) void dispatch_kernel(RowArgs p) {
+    const int nvec = row_vectors<T>(p.D);
+    int sub;
+    for (int64_t it = first_item<WAVE>(p, sub); it < p.items; it += item_stride<WAVE>(p)) {
+        const int64_t t = p.steps == 1 ? it : it / p.steps;
+        const int v = (int)(it - t * p.steps) * 64 + sub;
+        if (v >= nvec) continue;
+        const u32x4 x = row_load(static_cast<const T*>(p.in) + t * p.ldi, p.D, v);
+        for (int k0 = 0; k0 < p.top; k0 += kAhead) {
+            int at[kAhead];
+            load_places(p, t, k0, at);
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                const int row = at[u] < 0 ? ~at[u] : at[u];
+                if (row >= p.n) continue;
+                T* to = static_cast<T*>(p.out) + row * p.D;
+                u32x4 r = x;
+                if (at[u] < 0) r = u32x4{0, 0, 0, 0};
+                if (WAVE && p.through) {  // a row of 64 MB at most
+                    const __amdgpu_buffer_rsrc_t rsrc =
+                        __builtin_amdgcn_make_buffer_rsrc(to, 0, (int)(p.D * sizeof(T)), 0x00020000);
+                    __builtin_amdgcn_raw_buffer_store_b128(r, rsrc, (int)(row_vec_at<T>(p.D, v) * sizeof(T)), 0,
+                                                           kStoreStreamAux);
+                } else {
+                    row_store(to, p.D, v, r);
+                }
+            }
+        }
+    }
+}
+
+// The experts' rows are read once, with the nontemporal hint: (131072, 512) in
+// bf16 from 8 experts each 200 us (6.0 TB/s), without it 217.  More vectors a
+// lane with fewer rows in flight take longer (two of four rows 205, four of two
+// 240).
+template <typename T, bool WAVE>
 __global__ __launch_bounds__(kThreads) void combine_kernel(RowArgs p) {
     constexpr int VE = Elem<T>::kVec;
     const int nvec = row_vectors<T>(p.D);
     int sub;
-    for (int64_t it = first_item(p, sub); it < p.items; it += item_stride(p)) {
-        const int64_t t = it / p.steps;
-        const int v = (int)(it % p.steps) * 64 + sub;
+    for (int64_t it = first_item<WAVE>(p, sub); it < p.items; it += item_stride<WAVE>(p)) {
+        const int64_t t = p.steps == 1 ? it : it / p.steps;
+        const int v = (int)(it - t * p.steps) * 64 + sub;
         if (v >= nvec) continue;
         float acc[VE] = {};
         for (int k0 = 0; k0 < p.top; k0 += kAhead) {
+            int at[kAhead];
             u32x4 raw[kAhead];
             float w[kAhead];
-            bool on[kAhead];
+            load_places(p, t, k0, at);
 #pragma unroll
-            for (int u = 0; u < kAhead; ++u) {
-                const int64_t i = t * p.top + k0 + u;
-                const int at = k0 + u < p.top ? p.position[i] : -1;
-                on[u] = at >= 0 && at < p.n;
-                if (on[u]) {
-                    w[u] = weight_of<T>(p, i);
-                    raw[u] = row_load(static_cast<const T*>(p.in) + at * p.ldi, p.D, v);
-                }
-            }
+            for (int u = 0; u < kAhead; ++u) w[u] = k0 + u < p.top ? weight_of<T>(p, t * p.top + k0 + u) : 0.0f;
 #pragma unroll
             for (int u = 0; u < kAhead; ++u)
-                if (on[u]) {
+                if (at[u] >= 0 && at[u] < p.n)
+                    raw[u] = row_load<true>(static_cast<const T*>(p.in) + at[u] * p.ldi, p.D, v);
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u)
+                if (at[u] >= 0 && at[u] < p.n) {
                     float r[VE];
                     Elem<T>::cvt(raw[u], r);
 #pragma unroll
@@ -190,78 +221,111 @@ __global__ __launch_bounds__(kThreads) void combine_kernel(RowArgs p) {
     }
 }
 
-// The gradient of a combination, a token by its lanes (steps == 1) or by the
-// block: dy is read once for eight rows.
-template <typename T, bool BLOCK>
+// Sums of eight values over lanes that share a token (8, 16, 32 or 64): three
+// exchanges halve the values a lane holds, the rest add one value, so that lane
+// l ends with value 4 (l & 1) + (l & 2) + (l >> 2 & 1) of its lanes' eight.
+__device__ __forceinline__ float sum_eight(const float (&v)[8], int lanes) {
+    const int lane = (int)threadIdx.x & 63;
+    float a[4], b[2], c;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        const float give = lane & 1 ? v[u] : v[u + 4], keep = lane & 1 ? v[u + 4] : v[u];
+        a[u] = keep + reduce_partner<1>(give);
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        const float give = lane & 2 ? a[u] : a[u + 2], keep = lane & 2 ? a[u + 2] : a[u];
+        b[u] = keep + reduce_partner<2>(give);
+    }
+    {
+        const float give = lane & 4 ? b[0] : b[1], keep = lane & 4 ? b[1] : b[0];
+        c = keep + exact_xor<4>(give);
+    }
+    if (lanes >= 16) c += exact_xor<8>(c);
+    if (lanes >= 32) c += exact_xor<16>(c);
+    if (lanes >= 64) c += exact_xor<32>(c);
+    return c;
+}
+__device__ __forceinline__ int eighth(int sub) { return 4 * (sub & 1) + (sub & 2) + ((sub >> 2) & 1); }
+
+// The gradient of a combination, a token by its lanes or by the block: dy is
+// read once for eight rows, whose loads are in flight together.
+template <typename T, int TEAM>  // 0: p.lanes, 1: a wave, 2: the block
 __global__ __launch_bounds__(kThreads) void combine_bwd_kernel(RowArgs p) {
     constexpr int VE = Elem<T>::kVec;
-    __shared__ float sh[kThreads / 64][kAhead];
+    constexpr bool BLOCK = TEAM == 2;
+    __shared__ float sh[2][kThreads / 64][kAhead];
     const int nvec = row_vectors<T>(p.D);
-    int sub = (int)threadIdx.x;
-    const int team = BLOCK ? kThreads : p.lanes;
+    int sub = (int)threadIdx.x, turn = 0;
+    const int team = BLOCK ? kThreads : TEAM == 1 ? 64 : p.lanes;
     int64_t t = blockIdx.x, stride = gridDim.x;
     if constexpr (!BLOCK) {
-        t = first_item(p, sub);
-        stride = item_stride(p);
+        t = first_item<TEAM == 1>(p, sub);
+        stride = item_stride<TEAM == 1>(p);
     }
     for (; t < p.tokens; t += stride) {
         const T* dy = static_cast<const T*>(p.in) + t * p.ldi;
-        for (int k0 = 0; k0 < p.top; k0 += kAhead) {
+        for (int k0 = 0; k0 < p.top; k0 += kAhead, turn ^= 1) {
             float dot[kAhead] = {};
+            int at[kAhead];
+            load_places(p, t, k0, at);
             for (int v = sub; v < nvec; v += team) {
+                u32x4 raw[kAhead];
+                const u32x4 gr = row_load(dy, p.D, v);
+                if (p.dweights)
+#pragma unroll
+                    for (int u = 0; u < kAhead; ++u)
+                        if (at[u] >= 0 && at[u] < p.n)
+                            raw[u] = row_load<true>(static_cast<const T*>(p.rows) + at[u] * p.ldr, p.D, v);
                 float g[VE];
-                Elem<T>::cvt(row_load(dy, p.D, v), g);
+                Elem<T>::cvt(gr, g);
+                if (p.out)
+#pragma unroll
+                    for (int u = 0; u < kAhead; ++u) {
+                        const int row = at[u] < 0 ? ~at[u] : at[u];
+                        if (row >= p.n) continue;
+                        u32x4 r{0, 0, 0, 0};
+                        if (at[u] >= 0) {
+                            const float w = weight_of<T>(p, t * p.top + k0 + u);
+                            float d[VE];
+#pragma unroll
+                            for (int k = 0; k < VE; ++k) d[k] = w * g[k];
+                            r = pack_vec<T>(d);
+                        }
+                        row_store(static_cast<T*>(p.out) + row * p.D, p.D, v, r);
+                    }
+                if (!p.dweights) continue;
+                // elements that the vector before has too
                 const int skip = p.ragged && p.D >= VE ? (int)((int64_t)v * VE - row_vec_at<T>(p.D, v)) : 0;
 #pragma unroll
-                for (int u = 0; u < kAhead; ++u) {
-                    if (k0 + u >= p.top) break;
-                    const int64_t i = t * p.top + k0 + u;
-                    const int at = p.position[i];
-                    const int row = at < 0 ? ~at : at;
-                    if (row >= p.n) continue;
-                    float d[VE] = {};
-                    if (at >= 0) {
-                        if (p.dweights) {
-                            float r[VE];
-                            Elem<T>::cvt(row_load(static_cast<const T*>(p.rows) + row * p.ldr, p.D, v), r);
+                for (int u = 0; u < kAhead; ++u)
+                    if (at[u] >= 0 && at[u] < p.n) {
+                        float r[VE];
+                        Elem<T>::cvt(raw[u], r);
 #pragma unroll
-                            for (int k = 0; k < VE; ++k) dot[u] += k < skip ? 0.0f : g[k] * r[k];
-                        }
-                        const float w = weight_of<T>(p, i);
-#pragma unroll
-                        for (int k = 0; k < VE; ++k) d[k] = w * g[k];
+                        for (int k = 0; k < VE; ++k)
+                            if (k >= skip) dot[u] = __builtin_fmaf(g[k], r[k], dot[u]);
                     }
-                    if (p.out) row_store(static_cast<T*>(p.out) + row * p.D, p.D, v, pack_vec<T>(d));
-                }
             }
             if (!p.dweights) continue;
-            for (int d = 1; d < (BLOCK ? 64 : p.lanes); d *= 2)
-#pragma unroll
-                for (int u = 0; u < kAhead; ++u) dot[u] += __shfl_xor(dot[u], d, 64);
+            float s = sum_eight(dot, BLOCK ? 64 : team);
+            int u = eighth(sub);
+            bool mine = sub < kAhead;
             if constexpr (BLOCK) {
+                // two turns' values, so that one barrier a turn is enough
+                if (((int)threadIdx.x & 63) < kAhead) sh[turn][threadIdx.x >> 6][u] = s;
                 __syncthreads();
-                if ((threadIdx.x & 63) == 0)
+                u = sub;
+                if (mine) {
+                    s = sh[turn][0][u];
 #pragma unroll
-                    for (int u = 0; u < kAhead; ++u) sh[threadIdx.x >> 6][u] = dot[u];
-                __syncthreads();
+                    for (int w = 1; w < kThreads / 64; ++w) s += sh[turn][w][u];
+                }
             }
-            if constexpr (BLOCK) {
-                if (sub < kAhead && k0 + sub < p.top) {
-                    float s = 0.0f;
-#pragma unroll
-                    for (int w = 0; w < kThreads / 64; ++w) s += sh[w][sub];
-                    const int64_t i = t * p.top + k0 + sub;
-                    if (p.weights_f32) static_cast<float*>(p.dweights)[i] = s;
-                    else Elem<T>::put(static_cast<T*>(p.dweights) + i, s);
-                }
-            } else if (sub == 0) {
-#pragma unroll
-                for (int u = 0; u < kAhead; ++u) {
-                    if (k0 + u >= p.top) break;
-                    const int64_t i = t * p.top + k0 + u;
-                    if (p.weights_f32) static_cast<float*>(p.dweights)[i] = dot[u];
-                    else Elem<T>::put(static_cast<T*>(p.dweights) + i, dot[u]);
-                }
+            if (mine && k0 + u < p.top) {
+                const int64_t i = t * p.top + k0 + u;
+                if (p.weights_f32) static_cast<float*>(p.dweights)[i] = s;
+                else Elem<T>::put(static_cast<T*>(p.dweights) + i, s);
             }
         }
     }
@@ -304,6 +368,7 @@ void split_rows(RowArgs& a, int dtype) {
     a.steps = row_steps(nvec);
     a.items = a.tokens * a.steps;
     a.ragged = a.D % (dtype == 0 ? 4 : 8) != 0;
+    a.through = !a.ragged && (reinterpret_cast<uintptr_t>(a.out) & 15u) == 0;
 }
 
 unsigned grid_of(int64_t items, int per_block) {
@@ -379,8 +444,11 @@ extern "C" int fl_expert_dispatch(const void* x, int64_t row_stride, int64_t tok
     a.top = (int)top;
     a.out = rows;
     split_rows(a, dtype);
+    hipStream_t s = static_cast<hipStream_t>(stream);
     by_type(dtype, [&](auto t) {
-        dispatch_kernel<decltype(t)><<<grid_of(a.items, kThreads / a.lanes), kThreads, 0, static_cast<hipStream_t>(stream)>>>(a);
+        const unsigned grid = grid_of(a.items, kThreads / a.lanes);
+        if (a.lanes == 64) dispatch_kernel<decltype(t), true><<<grid, kThreads, 0, s>>>(a);
+        else dispatch_kernel<decltype(t), false><<<grid, kThreads, 0, s>>>(a);
     });
     return launch_status(name);
 }
@@ -408,8 +476,11 @@ extern "C" int fl_expert_combine(const void* rows, int64_t row_stride, int64_t t
     a.weights_f32 = weights_dtype == 0;
     a.out = out;
     split_rows(a, dtype);
+    hipStream_t s = static_cast<hipStream_t>(stream);
     by_type(dtype, [&](auto t) {
-        combine_kernel<decltype(t)><<<grid_of(a.items, kThreads / a.lanes), kThreads, 0, static_cast<hipStream_t>(stream)>>>(a);
+        const unsigned grid = grid_of(a.items, kThreads / a.lanes);
+        if (a.lanes == 64) combine_kernel<decltype(t), true><<<grid, kThreads, 0, s>>>(a);
+        else combine_kernel<decltype(t), false><<<grid, kThreads, 0, s>>>(a);
     });
     return launch_status(name);
 }
@@ -445,10 +516,12 @@ extern "C" int fl_expert_combine_bwd(const void* grad, int64_t grad_stride, cons
     split_rows(a, dtype);
     hipStream_t s = static_cast<hipStream_t>(stream);
     by_type(dtype, [&](auto t) {
-        if (a.steps > 1)
-            combine_bwd_kernel<decltype(t), true><<<grid_of(tokens, 1), kThreads, 0, s>>>(a);
-        else
-            combine_bwd_kernel<decltype(t), false><<<grid_of(tokens, kThreads / a.lanes), kThreads, 0, s>>>(a);
+        // from 193 vectors on a block shares a token: (16383, 2048) in bf16 162 us for
+        // 186 by a wave, but (60000, 999) 338 for 312
+        if (a.steps > 3) combine_bwd_kernel<decltype(t), 2><<<grid_of(tokens, 1), kThreads, 0, s>>>(a);
+        else if (a.lanes == 64)
+            combine_bwd_kernel<decltype(t), 1><<<grid_of(tokens, kThreads / 64), kThreads, 0, s>>>(a);
+        else combine_bwd_kernel<decltype(t), 0><<<grid_of(tokens, kThreads / a.lanes), kThreads, 0, s>>>(a);
     });
     return launch_status(name);
 }

@@ -20,9 +20,14 @@ __device__ __forceinline__ int64_t row_vec_at(int64_t D, int v) {
     return e < last ? e : last;
 }
 
-template <typename T>
+// STREAM: with the nontemporal hint, for rows that are read once.
+template <bool STREAM = false, typename T>
 __device__ __forceinline__ u32x4 row_load(const T* row, int64_t D, int v) {
-    if (D >= Elem<T>::kVec) return *reinterpret_cast<const u32x4_any*>(row + row_vec_at<T>(D, v));
+    if (D >= Elem<T>::kVec) {
+        const T* at = row + row_vec_at<T>(D, v);
+        if constexpr (STREAM) return load_raw_stream(at);
+        else return *reinterpret_cast<const u32x4_any*>(at);
+    }
     T part[Elem<T>::kVec];
 #pragma unroll
     for (int k = 0; k < Elem<T>::kVec; ++k) part[k] = k < D ? row[k] : T{};
@@ -61,10 +66,10 @@ __device__ __forceinline__ u32x4 pack_vec(const float (&v)[Elem<T>::kVec]) {
     return r;
 }
 
-// Lanes that share a row of nvec vectors (a power of two up to a wave) and the
-// steps of 64 vectors that longer rows take.
+// Lanes that share a row of nvec vectors (a power of two from 8 up to a wave) and
+// the steps of 64 vectors that longer rows take.
 inline int row_lanes(int nvec) {
-    int lanes = 1;
+    int lanes = 8;
     while (lanes < nvec && lanes < 64) lanes *= 2;
     return lanes;
 }

@@ -3,8 +3,10 @@
 //   m = mean x, r = 1 / sqrt(mean (x - m)^2 + eps), h = (x - m) r, y = h w + b
 //   dx = r (a - mean a - h mean(a h)) with a = g w;  dw = sum_rows g h, db = sum_rows g
 //
-// A row is held in registers by some lanes of a wave, a block, or, past 4096
-// vectors, read again from the caches, so memory sees each operand once.  The
+// A row is held in registers by some lanes of a wave or a block, or read again from
+// the caches, so that memory sees each operand once; only the backward of rows of
+// more than 1024 vectors reads x and g twice, since a block's registers do not hold
+// sums for as many columns.  The
 // mean is kept as two numbers: m0, the rounded sum over D, and m1, the mean of
 // the differences to it.  x - m0 - m1 then keeps its digits when the row has a
 // large value in common, which one fp32 mean would take from it.  Lanes meet the
@@ -36,16 +38,27 @@ struct Args {
     bool params_f32;
     float eps;
     void* y;       // forward: y; backward: dx (NULL: not wanted)
-    f32x4* stats;  // [rows]: m0, m1, r
+    f32x4* stats;  // [rows]: m0, -m1 r, r
     const void* g;
     int64_t ldg;
     float* part;  // [blocks][2][D]: sums of g h and of g
     int blocks;
 };
 
+// Columns c, c + 1, .. of a parameter, widened.
 template <typename T>
-__device__ __forceinline__ float param(const Args& p, const void* a, int64_t c) {
-    return p.params_f32 ? static_cast<const float*>(a)[c] : Elem<T>::scalar(static_cast<const T*>(a) + c);
+__device__ __forceinline__ void load_param_at(const Args& p, const void* a, int64_t c, float (&v)[Elem<T>::kVec]) {
+    if (p.params_f32) {
+#pragma unroll
+        for (int k = 0; k < Elem<T>::kVec; k += 4) {
+            float f[4];
+            load_vec_any<float>(static_cast<const float*>(a) + c + k, f);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[k + i] = f[i];
+        }
+    } else {
+        load_vec_any<T>(static_cast<const T*>(a) + c, v);
+    }
 }
 
 // Sums over a row's lanes: LANES up to a wave within it, more across the block.
@@ -76,6 +89,14 @@ __device__ __forceinline__ void row_sum(float (&v)[N], float (*sh)[N]) {
     }
 }
 
+// What the backward needs of a row: m0, -m1 r and r, so that h is two operations:
+// (x - m0) r - m1 r.
+__device__ __forceinline__ f32x4 row_stats(float m0, float m1, float mean_square, float eps) {
+    const float var = mean_square - m1 * m1;
+    const float rstd = 1.0f / sqrtf((var < 0.0f ? 0.0f : var) + eps);
+    return f32x4{m0, -m1 * rstd, rstd, 0.0f};
+}
+
 // How a block is laid out for rows of LANES * NV vectors at most.
 template <int LANES>
 struct Shape {
@@ -83,70 +104,102 @@ struct Shape {
     static constexpr int kRows = kThreads / LANES;
 };
 
-// Lane `sub` holds vectors sub, sub + LANES, ..; elements past the row are 0.
+// Lane `sub` holds vectors sub, sub + LANES, .. of a row.  Where rows are no whole
+// vectors (!WHOLE) the last vector is moved back to end with the row, so that all
+// loads and stores are whole; the elements that it shares with the one before
+// count once, there.
 template <typename T, int LANES, int NV, bool WHOLE>
-__device__ __forceinline__ void load_row(const T* row, int D, int sub, float (&v)[NV][Elem<T>::kVec]) {
-    constexpr int VE = Elem<T>::kVec;
+struct Columns {
+    using Type = T;
+    static constexpr int VE = Elem<T>::kVec;
+    int at[NV];    // the vector's first column
+    int skip[NV];  // its elements that do not count: VE, or those shared
+    __device__ __forceinline__ Columns(int D, int sub) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        const int c = (sub + j * LANES) * VE;
-        if constexpr (WHOLE) {
-            u32x4 r{0, 0, 0, 0};
-            if (c < D) r = load_raw_stream(row + c);
-            Elem<T>::cvt(r, v[j]);
-        } else {
-            load_vec_part<T>(row + c, D - c, 0.0f, v[j]);
+        for (int j = 0; j < NV; ++j) {
+            const int c = (sub + j * LANES) * VE;
+            at[j] = WHOLE ? c : c < D - VE ? c : D - VE;
+            skip[j] = c >= D ? VE : WHOLE ? 0 : c - at[j];
         }
+    }
+    __device__ __forceinline__ bool any(int j) const { return skip[j] < VE; }
+    __device__ __forceinline__ bool counts(int j, int k) const { return WHOLE ? skip[j] == 0 : k >= skip[j]; }
+};
+
+template <typename T, int NV, typename C>
+__device__ __forceinline__ void load_row(const C& col, const T* row, u32x4 (&v)[NV]) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) v[j] = col.any(j) ? load_raw_stream(row + col.at[j]) : u32x4{0, 0, 0, 0};
+}
+
+// Vector j's columns of a parameter, or `fill` where there is none.
+template <typename C, int VE>
+__device__ __forceinline__ void load_param(const Args& p, const C& col, int j, const void* a, float fill,
+                                           float (&v)[VE]) {
+#pragma unroll
+    for (int k = 0; k < VE; ++k) v[k] = fill;
+    if (a && col.any(j)) load_param_at<typename C::Type>(p, a, col.at[j], v);
+}
+
+template <typename T, typename C>
+__device__ __forceinline__ void store_vec(const C& col, int j, T* row, const float (&v)[Elem<T>::kVec]) {
+    if (col.any(j)) __builtin_nontemporal_store(pack_vec<T>(v), reinterpret_cast<u32x4_any*>(row + col.at[j]));
+}
+
+// Adds a vector's elements to s, two an instruction where they are 16-bit.
+template <typename T>
+__device__ __forceinline__ void add_vec(u32x4 r, float& s) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const uint32_t e = r[k];
+        if constexpr (sizeof(T) == 4) s += __builtin_bit_cast(float, e);
+        else if constexpr (__is_same(T, _Float16))
+            s = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, e), f16x2{(_Float16)1.0f, (_Float16)1.0f}, s, false);
+        else
+            s = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, e), bf16x2{(__bf16)1.0f, (__bf16)1.0f}, s,
+                                                false);
     }
 }
 
-template <typename T, int LANES, int NV>
-__device__ __forceinline__ void load_params(const Args& p, const void* a, float fill, int sub,
-                                            float (&v)[NV][Elem<T>::kVec]) {
-    constexpr int VE = Elem<T>::kVec;
-#pragma unroll
-    for (int j = 0; j < NV; ++j)
-#pragma unroll
-        for (int k = 0; k < VE; ++k) {
-            const int c = (sub + j * LANES) * VE + k;
-            v[j][k] = a && c < p.D ? param<T>(p, a, c) : fill;
-        }
-}
-
-template <typename T, int LANES, int NV, bool WHOLE>
-__device__ __forceinline__ void store_row(T* row, int D, int sub, const float (&v)[NV][Elem<T>::kVec]) {
-    constexpr int VE = Elem<T>::kVec;
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        const int c = (sub + j * LANES) * VE;
-        if (WHOLE ? c < D : c + VE <= D) {
-            __builtin_nontemporal_store(pack_vec<T>(v[j]), reinterpret_cast<u32x4_any*>(row + c));
-        } else if constexpr (!WHOLE) {
-#pragma unroll
-            for (int k = 0; k < VE; ++k)
-                if (c + k < D) Elem<T>::put(row + c + k, v[j][k]);
-        }
-    }
-}
-
+// A row's loads are issued before the row before it is reduced, and the parameters
+// stay in registers, but for rows of more than 2048 vectors, whose block is alone on
+// its CU and has too few.
 template <typename T, int LANES, int NV, bool WHOLE>
 __global__ __launch_bounds__(Shape<LANES>::kThreads) void fwd_kernel(Args p) {
     constexpr int VE = Elem<T>::kVec;
     __shared__ float sh1[Shape<LANES>::kThreads / 64][1], sh2[Shape<LANES>::kThreads / 64][2];
-    const int sub = (int)threadIdx.x % LANES, D = (int)p.D;
-    const float inv = 1.0f / (float)D;
-    float w[NV][VE], b[NV][VE];
-    load_params<T, LANES, NV>(p, p.w, 1.0f, sub, w);
-    load_params<T, LANES, NV>(p, p.b, 0.0f, sub, b);
-    for (int64_t r = (int64_t)blockIdx.x * Shape<LANES>::kRows + (int)threadIdx.x / LANES; r < p.rows;
-         r += (int64_t)p.blocks * Shape<LANES>::kRows) {
+    const int sub = (int)threadIdx.x % LANES;
+    const Columns<T, LANES, NV, WHOLE> col((int)p.D, sub);
+    const float inv = 1.0f / (float)p.D;
+    const int64_t step = (int64_t)p.blocks * Shape<LANES>::kRows;
+    int64_t r = (int64_t)blockIdx.x * Shape<LANES>::kRows + (int)threadIdx.x / LANES;
+    constexpr bool HOLD = LANES <= 256 || NV <= 2;
+    u32x4 next[NV];
+    if (r < p.rows) load_row<T>(col, static_cast<const T*>(p.x) + r * p.ldx, next);
+    float w[HOLD ? NV : 1][VE], b[HOLD ? NV : 1][VE];
+    if constexpr (HOLD) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            load_param(p, col, j, p.w, 1.0f, w[j]);
+            load_param(p, col, j, p.b, 0.0f, b[j]);
+        }
+    }
+    for (; r < p.rows; r += step) {
         float x[NV][VE];
-        load_row<T, LANES, NV, WHOLE>(static_cast<const T*>(p.x) + r * p.ldx, D, sub, x);
         float s[1] = {};
 #pragma unroll
-        for (int j = 0; j < NV; ++j)
+        for (int j = 0; j < NV; ++j) {
+            Elem<T>::cvt(next[j], x[j]);
+            if constexpr (WHOLE) {
+                add_vec<T>(next[j], s[0]);
+            } else {
 #pragma unroll
-            for (int k = 0; k < VE; ++k) s[0] += x[j][k];
+                for (int k = 0; k < VE; ++k)
+                    if (col.counts(j, k)) s[0] += x[j][k];
+            }
+        }
+        if (r + step < p.rows) load_row<T>(col, static_cast<const T*>(p.x) + (r + step) * p.ldx, next);
         row_sum<LANES>(s, sh1);
         const float m0 = s[0] * inv;
         float d[2] = {};
@@ -155,78 +208,108 @@ __global__ __launch_bounds__(Shape<LANES>::kThreads) void fwd_kernel(Args p) {
 #pragma unroll
             for (int k = 0; k < VE; ++k) {
                 x[j][k] -= m0;
-                if ((sub + j * LANES) * VE + (WHOLE ? 0 : k) < D) {
+                if (col.counts(j, k)) {
                     d[0] += x[j][k];
                     d[1] = __builtin_fmaf(x[j][k], x[j][k], d[1]);
                 }
             }
         row_sum<LANES>(d, sh2);
-        const float m1 = d[0] * inv;
-        const float var = d[1] * inv - m1 * m1;
-        const float rstd = 1.0f / sqrtf((var < 0.0f ? 0.0f : var) + p.eps);
-        if (p.stats && sub == 0) p.stats[r] = f32x4{m0, m1, rstd, 0.0f};
+        const f32x4 st = row_stats(m0, d[0] * inv, d[1] * inv, p.eps);
+        if (p.stats && sub == 0) p.stats[r] = st;
+        T* y = static_cast<T*>(p.y) + r * p.D;
 #pragma unroll
-        for (int j = 0; j < NV; ++j)
+        for (int j = 0; j < NV; ++j) {
+            constexpr int ONE = HOLD ? 1 : 0;
+            if constexpr (!HOLD) {
+                load_param(p, col, j, p.w, 1.0f, w[0]);
+                load_param(p, col, j, p.b, 0.0f, b[0]);
+            }
 #pragma unroll
-            for (int k = 0; k < VE; ++k) x[j][k] = __builtin_fmaf((x[j][k] - m1) * rstd, w[j][k], b[j][k]);
-        store_row<T, LANES, NV, WHOLE>(static_cast<T*>(p.y) + r * p.D, D, sub, x);
+            for (int k = 0; k < VE; ++k)
+                x[j][k] = __builtin_fmaf(__builtin_fmaf(x[j][k], st[2], st[1]), w[j * ONE][k], b[j * ONE][k]);
+            store_vec<T>(col, j, y, x[j]);
+        }
     }
 }
 
+// With more than 256 lanes a row it gives dx alone.
 template <typename T, int LANES, int NV, bool WHOLE>
 __global__ __launch_bounds__(Shape<LANES>::kThreads) void bwd_kernel(Args p) {
     constexpr int VE = Elem<T>::kVec;
     constexpr int ROWS = Shape<LANES>::kRows;
-    __shared__ float sh2[Shape<LANES>::kThreads / 64][2];
-    const int sub = (int)threadIdx.x % LANES, D = (int)p.D;
-    const float inv = 1.0f / (float)D;
-    float w[NV][VE], dw[NV][VE] = {}, db[NV][VE] = {};
-    load_params<T, LANES, NV>(p, p.w, 1.0f, sub, w);
-    for (int64_t r = (int64_t)blockIdx.x * ROWS + (int)threadIdx.x / LANES; r < p.rows;
-         r += (int64_t)p.blocks * ROWS) {
-        float x[NV][VE], g[NV][VE];
-        load_row<T, LANES, NV, WHOLE>(static_cast<const T*>(p.x) + r * p.ldx, D, sub, x);
-        load_row<T, LANES, NV, WHOLE>(static_cast<const T*>(p.g) + r * p.ldg, D, sub, g);
-        const f32x4 st = p.stats[r];
-        const float m0 = st[0], m1 = st[1], rstd = st[2];
+    __shared__ float sh2[2][Shape<LANES>::kThreads / 64][2];
+    const int sub = (int)threadIdx.x % LANES;
+    const Columns<T, LANES, NV, WHOLE> col((int)p.D, sub);
+    const float inv = 1.0f / (float)p.D;
+    const int64_t step = (int64_t)p.blocks * ROWS;
+    int64_t r = (int64_t)blockIdx.x * ROWS + (int)threadIdx.x / LANES;
+    u32x4 next_x[NV], next_g[NV];
+    f32x4 next_st{0, 0, 0, 0};
+    if (r < p.rows) {
+        load_row<T>(col, static_cast<const T*>(p.x) + r * p.ldx, next_x);
+        load_row<T>(col, static_cast<const T*>(p.g) + r * p.ldg, next_g);
+        next_st = p.stats[r];
+    }
+    constexpr bool SUMS = LANES <= 256, HOLD = SUMS || NV <= 2;
+    constexpr int ONE = HOLD ? 1 : 0;
+    float w[HOLD ? NV : 1][VE], dw[SUMS ? NV : 1][VE] = {}, db[SUMS ? NV : 1][VE] = {};
+    if constexpr (HOLD) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) load_param(p, col, j, p.w, 1.0f, w[j]);
+    }
+    for (int turn = 0; r < p.rows; r += step, turn ^= 1) {
+        const float m0 = next_st[0], shift = next_st[1], rstd = next_st[2];
+        float h[NV][VE], g[NV][VE];
         float s[2] = {};
 #pragma unroll
-        for (int j = 0; j < NV; ++j)
+        for (int j = 0; j < NV; ++j) {
+            Elem<T>::cvt(next_x[j], h[j]);
+            Elem<T>::cvt(next_g[j], g[j]);
+            if constexpr (!HOLD) load_param(p, col, j, p.w, 1.0f, w[0]);
 #pragma unroll
             for (int k = 0; k < VE; ++k) {
-                const float h = (x[j][k] - m0 - m1) * rstd;
-                x[j][k] = h;
-                if ((sub + j * LANES) * VE + (WHOLE ? 0 : k) < D) {
-                    dw[j][k] = __builtin_fmaf(g[j][k], h, dw[j][k]);
+                h[j][k] = __builtin_fmaf(h[j][k] - m0, rstd, shift);
+                if constexpr (SUMS) {
+                    dw[j][k] = __builtin_fmaf(g[j][k], h[j][k], dw[j][k]);
                     db[j][k] += g[j][k];
-                    g[j][k] *= w[j][k];
+                }
+                g[j][k] *= w[j * ONE][k];
+                if (col.counts(j, k)) {
                     s[0] += g[j][k];
-                    s[1] = __builtin_fmaf(g[j][k], h, s[1]);
+                    s[1] = __builtin_fmaf(g[j][k], h[j][k], s[1]);
                 }
             }
+        }
+        if (r + step < p.rows) {
+            load_row<T>(col, static_cast<const T*>(p.x) + (r + step) * p.ldx, next_x);
+            load_row<T>(col, static_cast<const T*>(p.g) + (r + step) * p.ldg, next_g);
+            next_st = p.stats[r + step];
+        }
         if (!p.y) continue;
-        row_sum<LANES>(s, sh2);
-        const float c0 = s[0] * inv, c1 = s[1] * inv;
+        row_sum<LANES>(s, sh2[turn]);
+        const float c0 = -rstd * (s[0] * inv), c1 = -rstd * (s[1] * inv);
+        T* dx = static_cast<T*>(p.y) + r * p.D;
 #pragma unroll
-        for (int j = 0; j < NV; ++j)
+        for (int j = 0; j < NV; ++j) {
 #pragma unroll
-            for (int k = 0; k < VE; ++k) g[j][k] = rstd * (g[j][k] - c0 - x[j][k] * c1);
-        store_row<T, LANES, NV, WHOLE>(static_cast<T*>(p.y) + r * p.D, D, sub, g);
+            for (int k = 0; k < VE; ++k)
+                g[j][k] = __builtin_fmaf(h[j][k], c1, __builtin_fmaf(g[j][k], rstd, c0));
+            store_vec<T>(col, j, dx, g[j]);
+        }
     }
-    if (!p.part) return;
+    if (!SUMS || !p.part) return;
     // the block's rows, joined over its groups of lanes in their order
     float* part = p.part + (int64_t)blockIdx.x * 2 * p.D;
-    if constexpr (ROWS == 1) {
+    if constexpr (!SUMS) {
+    } else if constexpr (ROWS == 1) {
 #pragma unroll
         for (int j = 0; j < NV; ++j)
 #pragma unroll
-            for (int k = 0; k < VE; ++k) {
-                const int c = (sub + j * LANES) * VE + k;
-                if (c < D) {
-                    part[c] = dw[j][k];
-                    part[p.D + c] = db[j][k];
+            for (int k = 0; k < VE; ++k)
+                if (col.counts(j, k)) {
+                    part[col.at[j] + k] = dw[j][k];
+                    part[p.D + col.at[j] + k] = db[j][k];
                 }
-            }
     } else {
         constexpr int W = LANES * NV * VE;
         __shared__ float sum[2][W];
@@ -235,82 +318,181 @@ __global__ __launch_bounds__(Shape<LANES>::kThreads) void bwd_kernel(Args p) {
 #pragma unroll
                 for (int j = 0; j < NV; ++j)
 #pragma unroll
-                    for (int k = 0; k < VE; ++k) {
-                        const int c = (sub + j * LANES) * VE + k;
-                        sum[0][c] = q ? sum[0][c] + dw[j][k] : dw[j][k];
-                        sum[1][c] = q ? sum[1][c] + db[j][k] : db[j][k];
-                    }
+                    for (int k = 0; k < VE; ++k)
+                        if (col.counts(j, k)) {
+                            const int c = col.at[j] + k;
+                            sum[0][c] = q ? sum[0][c] + dw[j][k] : dw[j][k];
+                            sum[1][c] = q ? sum[1][c] + db[j][k] : db[j][k];
+                        }
             }
             __syncthreads();
         }
-        for (int c = threadIdx.x; c < D; c += Shape<LANES>::kThreads) {
+        for (int c = threadIdx.x; c < (int)p.D; c += Shape<LANES>::kThreads) {
             part[c] = sum[0][c];
             part[p.D + c] = sum[1][c];
         }
     }
 }
 
-// Rows too long for a block's registers: a block reads the row again from the
-// caches for each step.
+// Any row, by a block that reads it again from the caches for each step: rows too
+// long for registers, and rows shorter than a vector.
 constexpr int kLong = 1024;
+
+// Vector v of a row, the elements that another vector has too marked by skip.
+template <typename T>
+struct LongVec {
+    int64_t at;
+    int skip;
+    __device__ __forceinline__ LongVec(int64_t D, int v) {
+        at = D >= Elem<T>::kVec ? row_vec_at<T>(D, v) : 0;
+        skip = (int)((int64_t)v * Elem<T>::kVec - at);
+    }
+    // elements of the vector that count, of a row of D
+    __device__ __forceinline__ bool counts(int64_t D, int k) const { return k >= skip && k < D; }
+};
+template <typename T>
+__device__ __forceinline__ void load_long(const T* row, int64_t D, int v, float (&x)[Elem<T>::kVec]) {
+    Elem<T>::cvt(row_load(row, D, v), x);
+}
+template <typename T>
+__device__ __forceinline__ void load_param_long(const Args& p, const void* a, float fill, int64_t at,
+                                                float (&v)[Elem<T>::kVec]) {
+#pragma unroll
+    for (int k = 0; k < Elem<T>::kVec; ++k) v[k] = fill;
+    if (!a) return;
+    if (p.D >= Elem<T>::kVec) {
+        load_param_at<T>(p, a, at, v);
+        return;
+    }
+#pragma unroll
+    for (int k = 0; k < Elem<T>::kVec; ++k)
+        if (k < p.D)
+            v[k] = p.params_f32 ? static_cast<const float*>(a)[k] : Elem<T>::scalar(static_cast<const T*>(a) + k);
+}
+
 template <typename T>
 __global__ __launch_bounds__(kLong) void fwd_long(Args p) {
+    constexpr int VE = Elem<T>::kVec;
     __shared__ float sh1[kLong / 64][1], sh2[kLong / 64][2];
     const float inv = 1.0f / (float)p.D;
+    const int nvec = row_vectors<T>(p.D);
     for (int64_t r = blockIdx.x; r < p.rows; r += p.blocks) {
-        const T* x = static_cast<const T*>(p.x) + r * p.ldx;
-        T* y = static_cast<T*>(p.y) + r * p.D;
-        float s[1] = {}, d[2] = {};
-        for (int64_t c = threadIdx.x; c < p.D; c += kLong) s[0] += Elem<T>::scalar(x + c);
+        const T* row = static_cast<const T*>(p.x) + r * p.ldx;
+        float s[1] = {}, d[2] = {}, x[VE], w[VE], b[VE];
+        for (int v = threadIdx.x; v < nvec; v += kLong) {
+            const LongVec<T> at(p.D, v);
+            load_long(row, p.D, v, x);
+#pragma unroll
+            for (int k = 0; k < VE; ++k)
+                if (at.counts(p.D, k)) s[0] += x[k];
+        }
         row_sum<kLong>(s, sh1);
         const float m0 = s[0] * inv;
-        for (int64_t c = threadIdx.x; c < p.D; c += kLong) {
-            const float v = Elem<T>::scalar(x + c) - m0;
-            d[0] += v;
-            d[1] = __builtin_fmaf(v, v, d[1]);
+        for (int v = threadIdx.x; v < nvec; v += kLong) {
+            const LongVec<T> at(p.D, v);
+            load_long(row, p.D, v, x);
+#pragma unroll
+            for (int k = 0; k < VE; ++k)
+                if (at.counts(p.D, k)) {
+                    const float c = x[k] - m0;
+                    d[0] += c;
+                    d[1] = __builtin_fmaf(c, c, d[1]);
+                }
         }
         row_sum<kLong>(d, sh2);
-        const float m1 = d[0] * inv;
-        const float var = d[1] * inv - m1 * m1;
-        const float rstd = 1.0f / sqrtf((var < 0.0f ? 0.0f : var) + p.eps);
-        if (p.stats && threadIdx.x == 0) p.stats[r] = f32x4{m0, m1, rstd, 0.0f};
-        for (int64_t c = threadIdx.x; c < p.D; c += kLong) {
-            const float w = p.w ? param<T>(p, p.w, c) : 1.0f, b = p.b ? param<T>(p, p.b, c) : 0.0f;
-            Elem<T>::put(y + c, __builtin_fmaf((Elem<T>::scalar(x + c) - m0 - m1) * rstd, w, b));
+        const f32x4 st = row_stats(m0, d[0] * inv, d[1] * inv, p.eps);
+        if (p.stats && threadIdx.x == 0) p.stats[r] = st;
+        for (int v = threadIdx.x; v < nvec; v += kLong) {
+            const LongVec<T> at(p.D, v);
+            load_long(row, p.D, v, x);
+            load_param_long<T>(p, p.w, 1.0f, at.at, w);
+            load_param_long<T>(p, p.b, 0.0f, at.at, b);
+#pragma unroll
+            for (int k = 0; k < VE; ++k) x[k] = __builtin_fmaf(__builtin_fmaf(x[k] - m0, st[2], st[1]), w[k], b[k]);
+            row_store(static_cast<T*>(p.y) + r * p.D, p.D, v, pack_vec<T>(x));
         }
     }
 }
+
+// dx of such rows; their dw and db take another kernel, columns at a time.
 template <typename T>
-__global__ __launch_bounds__(kLong) void bwd_long(Args p) {
+__global__ __launch_bounds__(kLong) void dx_long(Args p) {
+    constexpr int VE = Elem<T>::kVec;
     __shared__ float sh2[kLong / 64][2];
     const float inv = 1.0f / (float)p.D;
-    float* part = p.part ? p.part + (int64_t)blockIdx.x * 2 * p.D : nullptr;
-    bool first = true;
-    for (int64_t r = blockIdx.x; r < p.rows; r += p.blocks, first = false) {
+    const int nvec = row_vectors<T>(p.D);
+    for (int64_t r = blockIdx.x; r < p.rows; r += p.blocks) {
         const T* x = static_cast<const T*>(p.x) + r * p.ldx;
         const T* g = static_cast<const T*>(p.g) + r * p.ldg;
         const f32x4 st = p.stats[r];
-        const float m0 = st[0], m1 = st[1], rstd = st[2];
-        float s[2] = {};
-        for (int64_t c = threadIdx.x; c < p.D; c += kLong) {
-            const float h = (Elem<T>::scalar(x + c) - m0 - m1) * rstd, gv = Elem<T>::scalar(g + c);
-            if (part) {  // this thread alone meets column c
-                part[c] = first ? gv * h : __builtin_fmaf(gv, h, part[c]);
-                part[p.D + c] = first ? gv : part[p.D + c] + gv;
-            }
-            const float a = gv * (p.w ? param<T>(p, p.w, c) : 1.0f);
-            s[0] += a;
-            s[1] = __builtin_fmaf(a, h, s[1]);
+        float s[2] = {}, h[VE], a[VE], w[VE];
+        for (int v = threadIdx.x; v < nvec; v += kLong) {
+            const LongVec<T> at(p.D, v);
+            load_long(x, p.D, v, h);
+            load_long(g, p.D, v, a);
+            load_param_long<T>(p, p.w, 1.0f, at.at, w);
+#pragma unroll
+            for (int k = 0; k < VE; ++k)
+                if (at.counts(p.D, k)) {
+                    s[0] = __builtin_fmaf(a[k], w[k], s[0]);
+                    s[1] = __builtin_fmaf(a[k] * w[k], __builtin_fmaf(h[k] - st[0], st[2], st[1]), s[1]);
+                }
         }
-        if (!p.y) continue;
         row_sum<kLong>(s, sh2);
-        const float c0 = s[0] * inv, c1 = s[1] * inv;
-        T* dx = static_cast<T*>(p.y) + r * p.D;
-        for (int64_t c = threadIdx.x; c < p.D; c += kLong) {
-            const float h = (Elem<T>::scalar(x + c) - m0 - m1) * rstd;
-            const float a = Elem<T>::scalar(g + c) * (p.w ? param<T>(p, p.w, c) : 1.0f);
-            Elem<T>::put(dx + c, rstd * (a - c0 - h * c1));
+        const float c0 = -st[2] * (s[0] * inv), c1 = -st[2] * (s[1] * inv);
+        for (int v = threadIdx.x; v < nvec; v += kLong) {
+            const LongVec<T> at(p.D, v);
+            load_long(x, p.D, v, h);
+            load_long(g, p.D, v, a);
+            load_param_long<T>(p, p.w, 1.0f, at.at, w);
+#pragma unroll
+            for (int k = 0; k < VE; ++k)
+                a[k] = __builtin_fmaf(__builtin_fmaf(h[k] - st[0], st[2], st[1]), c1,
+                                      __builtin_fmaf(a[k] * w[k], st[2], c0));
+            row_store(static_cast<T*>(p.y) + r * p.D, p.D, v, pack_vec<T>(a));
         }
+    }
+}
+
+// A group's rows of 64 vectors of columns: sums of g h and of g, over the waves and
+// then over the groups in their order.
+template <typename T>
+__global__ __launch_bounds__(256) void columns_long(Args p) {
+    constexpr int VE = Elem<T>::kVec;
+    __shared__ float sh[2][4][64 * VE];
+    const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+    const int v = (int)blockIdx.x * 64 + lane;
+    const bool live = v < row_vectors<T>(p.D);
+    const LongVec<T> at(p.D, live ? v : 0);
+    float dw[VE] = {}, db[VE] = {};
+    if (live) {
+#pragma unroll 4
+        for (int64_t r = (int64_t)blockIdx.y * 4 + wave; r < p.rows; r += (int64_t)gridDim.y * 4) {
+            float x[VE], g[VE];
+            load_long(static_cast<const T*>(p.x) + r * p.ldx, p.D, v, x);
+            load_long(static_cast<const T*>(p.g) + r * p.ldg, p.D, v, g);
+            const f32x4 st = p.stats[r];
+#pragma unroll
+            for (int k = 0; k < VE; ++k) {
+                dw[k] = __builtin_fmaf(g[k], __builtin_fmaf(x[k] - st[0], st[2], st[1]), dw[k]);
+                db[k] += g[k];
+            }
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < VE; ++k) {
+        sh[0][wave][lane * VE + k] = dw[k];
+        sh[1][wave][lane * VE + k] = db[k];
+    }
+    __syncthreads();
+    if (wave > 1 || !live) return;
+    float* part = p.part + ((int64_t)blockIdx.y * 2 + wave) * p.D + at.at;
+#pragma unroll
+    for (int k = 0; k < VE; ++k) {
+        float s = sh[wave][0][lane * VE + k];
+#pragma unroll
+        for (int q = 1; q < 4; ++q) s += sh[wave][q][lane * VE + k];
+        if (at.counts(p.D, k)) part[k] = s;
     }
 }
 
@@ -326,6 +508,7 @@ __global__ __launch_bounds__(kJoinCols * kJoinRuns) void join_kernel(const float
     if (!out) return;
     float s = 0.0f;
     if (c < D)
+#pragma unroll 8
         for (int b = run; b < blocks; b += kJoinRuns) s += part[((int64_t)b * 2 + blockIdx.y) * D + c];
     sh[run][col] = s;
     __syncthreads();
@@ -358,7 +541,10 @@ struct Plan {
 };
 Plan plan(int64_t D, int dtype) {
     const int64_t vecs = (D * elem_size(dtype) + 15) / 16;
+    if (D * elem_size(dtype) < 16) return {0, 0, 1};
+    if (vecs <= 8) return {8, 1, 32};
     if (vecs <= 16) return {16, 1, 16};
+    if (vecs <= 32) return {32, 1, 8};
     if (vecs <= 64) return {64, 1, 4};
     if (vecs <= 128) return {64, 2, 4};
     if (vecs <= 256) return {64, 4, 4};
@@ -372,15 +558,37 @@ int block_count(int64_t rows, const Plan& q, int most) {
     const int64_t want = (rows + q.rows - 1) / q.rows;
     return (int)(want < most ? want : most);
 }
-int fwd_blocks(int64_t rows, const Plan& q) { return block_count(rows, q, 2048); }
-int bwd_blocks(int64_t rows, const Plan& q) { return block_count(rows, q, 512); }
+// Blocks of a forward: with ever more, short-lived ones memory is walked in order,
+// which takes less time until a block's parameters cost as much as its rows: (65536,
+// 4096) in bf16 209 us with 1024 blocks, 190 with 8192, 246 with one a row.
+int fwd_blocks(int64_t rows, const Plan& q) { return block_count(rows, q, q.lanes > 256 ? 1024 : 8192); }
+// Blocks of a backward, each with its sums to join: as many as are at work at
+// once.  With four vectors a lane that is one a CU: (32768, 4096) in fp32 269 us for
+// 276 with two, but (65536, 4096) in bf16, two vectors, 314 for 281.
+int bwd_blocks(int64_t rows, const Plan& q) { return block_count(rows, q, q.nv >= 4 ? 256 : 512); }
+
+// Rows too long for the backward's registers: groups of rows whose columns a block
+// sums, about four blocks a CU in all.
+int column_tiles(int64_t D, int dtype) { return (int)((D * elem_size(dtype) + 1023) / 1024); }
+int row_groups(int64_t rows, int64_t D, int dtype) {
+    const int64_t most = (rows + 15) / 16, want = (1024 + column_tiles(D, dtype) - 1) / column_tiles(D, dtype);
+    return (int)(want < most ? want : most);
+}
+// Rows of more than 256 lanes: a block of 1024 threads holds no sums beside them
+// ((16384, 16384) in bf16 950 us, spilling, for 481), and past 16 columns a lane not
+// even the rows ((8192, 20000) 375 us for dx, 290 where they are read again).
+bool bwd_long_rows(const Plan& q) { return q.lanes == 0 || q.lanes > 256; }
+constexpr int kBwdColumns = 16384;
+int bwd_columns(const Plan& q, int dtype) { return q.lanes * q.nv * 16 / elem_size(dtype); }
 
 template <typename T, bool WHOLE, typename F>
 void by_plan(const Plan& q, F f) {
 #define FL_CASE(L, N) \
     if (q.lanes == L && q.nv == N) \
     return f(T{}, std::integral_constant<int, L>{}, std::integral_constant<int, N>{}, std::bool_constant<WHOLE>{})
+    FL_CASE(8, 1);
     FL_CASE(16, 1);
+    FL_CASE(32, 1);
     FL_CASE(64, 1);
     FL_CASE(64, 2);
     FL_CASE(64, 4);
@@ -451,7 +659,8 @@ extern "C" int fl_layer_norm_fwd(const void* x, int64_t row_stride, int64_t rows
 
 extern "C" size_t fl_layer_norm_bwd_workspace_bytes(int64_t rows, int64_t D, int dtype) {
     if (rows < 0 || D < 1 || D > (1 << 24) || dtype < 0 || dtype > 2) return 0;
-    return (size_t)bwd_blocks(rows, plan(D, dtype)) * 2 * (size_t)D * 4;
+    const Plan q = plan(D, dtype);
+    return (size_t)(bwd_long_rows(q) ? row_groups(rows, D, dtype) : bwd_blocks(rows, q)) * 2 * (size_t)D * 4;
 }
 
 extern "C" int fl_layer_norm_bwd(const void* grad, int64_t grad_stride, const void* x, int64_t row_stride, int64_t rows,
@@ -487,23 +696,28 @@ extern "C" int fl_layer_norm_bwd(const void* grad, int64_t grad_stride, const vo
     a.g = grad;
     a.ldg = grad_stride;
     a.part = params ? static_cast<float*>(workspace) : nullptr;
-    a.blocks = bwd_blocks(rows, q);
+    const bool lng = bwd_long_rows(q);
+    const int groups = row_groups(rows, D, dtype);
+    a.blocks = lng ? block_count(rows, q, 1024) : bwd_blocks(rows, q);
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (rows > 0) {
-        if (q.lanes == 0) {
-            by_type(dtype, [&](auto t) { bwd_long<decltype(t)><<<(unsigned)a.blocks, kLong, 0, s>>>(a); });
-        } else {
-            by_shape(q, D, dtype, [&](auto t, auto lanes, auto nv, auto whole) {
-                constexpr int L = decltype(lanes)::value;
-                bwd_kernel<decltype(t), L, decltype(nv)::value, decltype(whole)::value>
+    if (rows > 0 && (q.lanes == 0 || bwd_columns(q, dtype) > kBwdColumns)) {
+        if (dx) by_type(dtype, [&](auto t) { dx_long<decltype(t)><<<(unsigned)a.blocks, kLong, 0, s>>>(a); });
+    } else if (rows > 0 && (dx || !lng)) {
+        by_shape(q, D, dtype, [&](auto t, auto lanes, auto nv, auto whole) {
+            constexpr int L = decltype(lanes)::value, NV = decltype(nv)::value;
+            if constexpr (L * NV * Elem<decltype(t)>::kVec <= kBwdColumns)
+                bwd_kernel<decltype(t), L, NV, decltype(whole)::value>
                     <<<(unsigned)a.blocks, Shape<L>::kThreads, 0, s>>>(a);
-            });
-        }
+        });
     }
+    if (rows > 0 && lng && params)
+        by_type(dtype, [&](auto t) {
+            columns_long<decltype(t)><<<dim3((unsigned)column_tiles(D, dtype), (unsigned)groups), 256, 0, s>>>(a);
+        });
     if (params)
         by_type(dtype, [&](auto t) {
             join_kernel<decltype(t)><<<dim3((unsigned)((D + kJoinCols - 1) / kJoinCols), 2), kJoinCols * kJoinRuns, 0, s>>>(
-                a.part, a.blocks, D, dweight, dbias, a.params_f32);
+                a.part, lng ? groups : a.blocks, D, dweight, dbias, a.params_f32);
         });
     return launch_status(name);
 }

@@ -5,7 +5,7 @@
 // The lookup copies rows and is bound by memory.  The gradient sorts the token
 // ids (stably, so sums always run in the tokens' order and take no atomics), sums
 // runs of equal ids in fp32 and rounds a row once.  A sorted run is cut where it
-// crosses a border of 32 entries, so a token that comes often is summed by many
+// crosses a border of 16 or 64 entries, so a token that comes often is summed by many
 // waves; the pieces are joined in their order.  Rows that no token takes are
 // zeroed by other blocks of the same launch: most of the gradient's time, where
 // the vocabulary is large, is writing them.
@@ -32,6 +32,7 @@ struct LookupArgs {
     void* out;
     int lanes, steps;
     int64_t items;
+    bool through;  // a wave an item, rows of out whole, aligned vectors
 };
 
 template <typename T>
@@ -41,8 +42,8 @@ __global__ __launch_bounds__(kThreads) void lookup_kernel(LookupArgs p) {
     const int sub = (int)threadIdx.x % p.lanes, per = kThreads / p.lanes;
     for (int64_t it = (int64_t)blockIdx.x * per + (int)threadIdx.x / p.lanes; it < p.items;
          it += (int64_t)gridDim.x * per) {
-        const int64_t i = it / p.steps;
-        const int v = (int)(it % p.steps) * 64 + sub;
+        const int64_t i = p.steps == 1 ? it : it / p.steps;
+        const int v = (int)(it - i * p.steps) * 64 + sub;
         if (v >= nvec) continue;
         const int64_t id = p.index[i];
         const bool inside = id >= 0 && id < p.V;
@@ -54,7 +55,8 @@ __global__ __launch_bounds__(kThreads) void lookup_kernel(LookupArgs p) {
             for (int k = 0; k < VE; ++k) f[k] = inside ? f[k] * p.scale : __builtin_nanf("");
             r = pack_vec<T>(f);
         }
-        row_store(static_cast<T*>(p.out) + i * p.D, p.D, v, r);
+        if (p.through) row_store_through(static_cast<T*>(p.out) + i * p.D, p.D, v, r);
+        else row_store(static_cast<T*>(p.out) + i * p.D, p.D, v, r);
     }
 }
 
@@ -85,58 +87,98 @@ struct NextKey {
     __device__ __forceinline__ int operator()(int64_t i) const { return (int)(e[i].id >> shift) & mask; }
 };
 
+// Zeros over a launch's share of dW, and in the list's length: two blocks a CU, which
+// walk the share together, 128 KB at a time each, written through to memory: 525 MB
+// in 83 us, 95 with the nontemporal hint alone, 106 in steps of 16 KB.
+struct Zeros {
+    char* at;
+    int64_t bytes;
+    int* joins;  // cleared too, by the first block
+    static constexpr int kBlocks = 511, kSteps = 8, kBytes = 16 * kSteps * key_sort::kThreads;
+    __device__ __forceinline__ void operator()(int64_t block) const {
+        if (block == 0 && threadIdx.x == 0) *joins = 0;
+        int64_t first = block * kBytes;
+        for (; first + kBytes <= bytes; first += (int64_t)kBlocks * kBytes) {
+            const bool aligned = (reinterpret_cast<uintptr_t>(at) & 15u) == 0;
+            const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(at + first, 0, kBytes, 0x00020000);
+#pragma unroll
+            for (int j = 0; j < kSteps; ++j) {
+                const int k = 16 * (j * key_sort::kThreads + (int)threadIdx.x);
+                if (aligned) __builtin_amdgcn_raw_buffer_store_b128(u32x4{0, 0, 0, 0}, rsrc, k, 0, kStoreStreamAux);
+                else *reinterpret_cast<u32x4_any*>(at + first + k) = u32x4{0, 0, 0, 0};
+            }
+        }
+        if (first < bytes)  // the share's end: whole elements, of two bytes at least
+            for (int64_t k = first + 2 * (int)threadIdx.x; k < bytes; k += 2 * key_sort::kThreads)
+                *reinterpret_cast<uint16_t*>(at + k) = 0;
+    }
+    unsigned blocks() const {
+        const int64_t want = (bytes + kBytes - 1) / kBytes;
+        return (unsigned)(want < 1 ? 1 : want < kBlocks ? want : kBlocks);
+    }
+};
+
 template <typename Key>
-__global__ __launch_bounds__(key_sort::kThreads) void place_kernel(Key key, int64_t n, int bits, const int* hist,
-                                                                   const int* total, Entry* to) {
-    __shared__ key_sort::Shared sh;
+__global__ __launch_bounds__(key_sort::kThreads) void place_kernel(Key key, int64_t n, int bits, int blocks,
+                                                                   const int* hist, const int* total, Entry* to,
+                                                                   Zeros zeros) {
+    __shared__ key_sort::Shared<1024> sh;
+    if ((int)blockIdx.x >= blocks) return zeros((int)blockIdx.x - blocks);
     const int64_t first = (int64_t)blockIdx.x * key_sort::kChunk;
     const int m = (int)(n - first < key_sort::kChunk ? n - first : key_sort::kChunk);
     const int bins = 1 << bits;
-    int k[key_sort::kRounds], place[key_sort::kRounds], all[2], start[2];
+    int k[key_sort::kRounds], place[key_sort::kRounds], all[2], before[2], own[2], start[2];
 #pragma unroll
     for (int j = 0; j < key_sort::kRounds; ++j)
         k[j] = key_sort::entry(j) < m ? key(first + key_sort::entry(j)) : 0;
-    key_sort::rank(sh, k, m, bins, bits, place, all);
-    key_sort::block_starts(sh, hist, total, gridDim.x, bins, all, start);
+    key_sort::load_counts(hist, total, blocks, bins, all, before);
+    key_sort::rank(sh, k, m, bins, bits, place, own);
+    key_sort::block_starts(sh, all, before, bins, start);
 #pragma unroll
     for (int j = 0; j < key_sort::kRounds; ++j)
         if (key_sort::entry(j) < m)
             to[key_sort::placed(sh, k[j], place[j], bins)] = key.entry(first + key_sort::entry(j));
 }
 
-// Up to 4096 entries: one block sorts them by all digits, in shared memory.
-__global__ __launch_bounds__(key_sort::kThreads) void sort_alone(FirstKey src, int n, int bits, int passes, Entry* to) {
-    __shared__ key_sort::Shared sh;
-    __shared__ Entry e[key_sort::kChunk];
-    Entry mine[key_sort::kRounds];
+// Up to 8192 entries: one block sorts them by all digits, in shared memory, of which
+// short digits leave enough for two blocks a CU, as the zeros' blocks need.
+constexpr int kAloneBits = 6, kAloneRounds = 8, kAlone = kAloneRounds * key_sort::kThreads;
+__global__ __launch_bounds__(key_sort::kThreads) void sort_alone(FirstKey src, int n, int bits, int passes, Entry* to,
+                                                                 Zeros zeros) {
+    constexpr int R = kAloneRounds;
+    __shared__ key_sort::Shared<1 << kAloneBits> sh;
+    __shared__ Entry e[kAlone];
+    if (blockIdx.x > 0) return zeros((int64_t)blockIdx.x - 1);
+    Entry mine[R];
 #pragma unroll
-    for (int j = 0; j < key_sort::kRounds; ++j)
-        mine[j] = key_sort::entry(j) < n ? src.entry(key_sort::entry(j)) : Entry{0, 0};
+    for (int j = 0; j < R; ++j) {
+        const int i = key_sort::entry<R>(j);
+        mine[j] = i < n ? src.entry(i) : Entry{0, 0};
+    }
     const int bins = 1 << bits;
     for (int pass = 0; pass < passes; ++pass) {
-        int k[key_sort::kRounds], place[key_sort::kRounds], total[2], start[2];
+        int k[R], place[R], total[2], start[2];
 #pragma unroll
-        for (int j = 0; j < key_sort::kRounds; ++j) k[j] = (int)(mine[j].id >> (pass * bits)) & (bins - 1);
+        for (int j = 0; j < R; ++j) k[j] = (int)(mine[j].id >> (pass * bits)) & (bins - 1);
         key_sort::rank(sh, k, n, bins, bits, place, total);
         key_sort::starts(sh, total, bins, start);
         if ((int)threadIdx.x < bins) sh.start[threadIdx.x] = start[0];
         __syncthreads();
 #pragma unroll
-        for (int j = 0; j < key_sort::kRounds; ++j)
-            if (key_sort::entry(j) < n) e[key_sort::placed(sh, k[j], place[j], bins)] = mine[j];
+        for (int j = 0; j < R; ++j)
+            if (key_sort::entry<R>(j) < n) e[key_sort::placed(sh, k[j], place[j], bins)] = mine[j];
         __syncthreads();
 #pragma unroll
-        for (int j = 0; j < key_sort::kRounds; ++j)
-            if (key_sort::entry(j) < n) mine[j] = e[key_sort::entry(j)];
+        for (int j = 0; j < R; ++j)
+            if (key_sort::entry<R>(j) < n) mine[j] = e[key_sort::entry<R>(j)];
     }
 #pragma unroll
-    for (int j = 0; j < key_sort::kRounds; ++j)
-        if (key_sort::entry(j) < n) to[key_sort::entry(j)] = mine[j];
+    for (int j = 0; j < R; ++j)
+        if (key_sort::entry<R>(j) < n) to[key_sort::entry<R>(j)] = mine[j];
 }
 
-constexpr int kRun = 32;       // sorted entries a wave sums
-constexpr int kAhead = 8;      // rows whose loads are in flight
-constexpr int kFillRows = 64;  // rows of dW that a block looks through
+constexpr int kAhead = 16;  // sorted entries whose rows' loads are in flight
+constexpr int kPieces = 8;  // pieces of a row whose loads are in flight
 
 struct GradArgs {
     const void* g;
@@ -146,159 +188,145 @@ struct GradArgs {
     float scale;
     void* dw;
     float* part;  // [runs][2][D]: a run's first and last pieces where they go on beyond it
+    int run;  // entries of a run
     int64_t runs;
     int steps;
-    int64_t sum_blocks;
+    int* joins;  // number of rows of several pieces
+    int* list;   // [runs]: the runs they begin in
 };
 
-// Sums of the sorted entries [32 run, 32 run + 32) of equal ids, 64 vectors of
+// Sums of the sorted entries [run RUN, (run + 1) RUN) of equal ids, 64 vectors of
 // columns a wave.
-template <typename T>
+template <typename T, int RUN>
 __device__ __forceinline__ void sum_run(const GradArgs& p, int64_t run, int step) {
     constexpr int VE = Elem<T>::kVec;
     const int lane = (int)threadIdx.x & 63, v = step * 64 + lane;
-    const int nvec = row_vectors<T>(p.D);
-    const int64_t first = run * kRun;
-    const int m = (int)(p.n - first < kRun ? p.n - first : kRun);
-    // lane l: entry l of the run; lane 32 the one behind it, lane 33 the one before
-    Entry mine{0xFFFFFFFFu, 0};
-    if (lane < m || (lane == kRun && first + m < p.n)) mine = p.e[first + (lane < m ? lane : m)];
-    if (lane == kRun + 1 && run > 0) mine = p.e[first - 1];
-    const uint32_t behind = (uint32_t)__builtin_amdgcn_readlane((int)mine.id, kRun);
-    const uint32_t ahead = (uint32_t)__builtin_amdgcn_readlane((int)mine.id, kRun + 1);
+    const bool live = v < row_vectors<T>(p.D);
+    const int64_t first = run * RUN;
+    const int m = (int)(p.n - first < RUN ? p.n - first : RUN);
+    Entry mine{0xFFFFFFFFu, 0};  // entry `lane` of the run
+    if (lane < m) mine = p.e[first + lane];
+    const uint32_t behind = first + m < p.n ? p.e[first + m].id : 0xFFFFFFFFu;
+    const uint32_t ahead = run > 0 ? p.e[first - 1].id : 0xFFFFFFFFu;
+    const auto id_of = [&](int i) { return (uint32_t)__builtin_amdgcn_readlane((int)mine.id, i); };
     float acc[VE] = {};
-    bool head = (uint32_t)__builtin_amdgcn_readfirstlane((int)mine.id) == ahead;  // the piece began before
+    bool head = id_of(0) == ahead;  // the piece began before
     for (int i0 = 0; i0 < m; i0 += kAhead) {
         u32x4 raw[kAhead];
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
-            const int i = i0 + u;
-            const uint32_t id = (uint32_t)__builtin_amdgcn_readlane((int)mine.id, i);
-            const uint32_t at = (uint32_t)__builtin_amdgcn_readlane((int)mine.at, i);
-            if (i < m && id < p.V && v < nvec) raw[u] = row_load(static_cast<const T*>(p.g) + at * p.ldg, p.D, v);
+            const uint32_t at = (uint32_t)__builtin_amdgcn_readlane((int)mine.at, i0 + u);
+            if (id_of(i0 + u) < p.V && live) raw[u] = row_load<true>(static_cast<const T*>(p.g) + at * p.ldg, p.D, v);
         }
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
             const int i = i0 + u;
-            if (i >= m) break;
-            const uint32_t id = (uint32_t)__builtin_amdgcn_readlane((int)mine.id, i);
-            if (id >= p.V) return;  // nothing but such tokens from here on
-            const uint32_t next = i + 1 < m ? (uint32_t)__builtin_amdgcn_readlane((int)mine.id, i + 1) : behind;
-            if (v < nvec) {
-                float f[VE];
-                Elem<T>::cvt(raw[u], f);
+            const uint32_t id = id_of(i);
+            if (id >= p.V) return;  // nothing but such entries, or none, from here on
+            const uint32_t next = i + 1 < m ? id_of(i + 1) : behind;
+            float f[VE];
+            Elem<T>::cvt(raw[u], f);
 #pragma unroll
-                for (int k = 0; k < VE; ++k) acc[k] += f[k];
-            }
-            if (next != id || i + 1 == m) {
-                const bool tail = next == id;  // the piece goes on behind the run
-                if (v < nvec) {
-                    if (head || tail) {
-                        float* to = p.part + (run * 2 + (head ? 0 : 1)) * p.D;
+            for (int k = 0; k < VE; ++k) acc[k] += f[k];
+            if (next == id && i + 1 < m) continue;
+            const bool tail = next == id;  // the piece goes on behind the run
+            if (live && (head || tail)) {
+                float* to = p.part + (run * 2 + (head ? 0 : 1)) * p.D;
 #pragma unroll
-                        for (int k = 0; k < VE; k += 4) {
-                            float q[4] = {acc[k], acc[k + 1], acc[k + 2], acc[k + 3]};
-                            if (p.D >= VE) {
-                                __builtin_memcpy(to + row_vec_at<T>(p.D, v) + k, q, 16);
-                            } else {
-#pragma unroll
-                                for (int j = 0; j < 4; ++j)
-                                    if (k + j < p.D) to[k + j] = q[j];
-                            }
-                        }
+                for (int k = 0; k < VE; k += 4) {
+                    float q[4] = {acc[k], acc[k + 1], acc[k + 2], acc[k + 3]};
+                    if (p.D >= VE) {
+                        __builtin_memcpy(to + row_vec_at<T>(p.D, v) + k, q, 16);
                     } else {
 #pragma unroll
-                        for (int k = 0; k < VE; ++k) acc[k] *= p.scale;
-                        row_store(static_cast<T*>(p.dw) + id * p.D, p.D, v, pack_vec<T>(acc));
+                        for (int j = 0; j < 4; ++j)
+                            if (k + j < p.D) to[k + j] = q[j];
                     }
                 }
+            } else if (live) {
 #pragma unroll
-                for (int k = 0; k < VE; ++k) acc[k] = 0.0f;
-                head = false;
+                for (int k = 0; k < VE; ++k) acc[k] *= p.scale;
+                row_store(static_cast<T*>(p.dw) + id * p.D, p.D, v, pack_vec<T>(acc));
             }
+            // the list of runs in which a row of several pieces begins, in any order
+            if (tail && !head && step == 0 && lane == 0) p.list[atomicAdd(p.joins, 1)] = (int)run;
+#pragma unroll
+            for (int k = 0; k < VE; ++k) acc[k] = 0.0f;
+            head = false;
         }
     }
 }
 
-// Zeros in those of the block's rows that no token takes: a lane a row searches
-// the sorted ids for it.
-template <typename T>
-__device__ __forceinline__ void fill_rows(const GradArgs& p, int64_t block) {
-    __shared__ int taken[kFillRows];
-    const int64_t first = block * kFillRows;
-    if (threadIdx.x < kFillRows) {
-        const int64_t id = first + threadIdx.x;
-        int64_t lo = 0, hi = p.n;  // the first entry that is not below id
-        while (lo < hi) {
-            const int64_t mid = (lo + hi) / 2;
-            if ((int64_t)p.e[mid].id < id) lo = mid + 1;
-            else hi = mid;
-        }
-        taken[threadIdx.x] = id >= p.V || (lo < p.n && (int64_t)p.e[lo].id == id);
-    }
-    __syncthreads();
-    const int nvec = row_vectors<T>(p.D);
-    for (int r = 0; r < kFillRows; ++r) {
-        if (taken[r]) continue;
-        T* row = static_cast<T*>(p.dw) + (first + r) * p.D;
-        for (int v = threadIdx.x; v < nvec; v += kThreads) row_store(row, p.D, v, u32x4{0, 0, 0, 0});
-    }
+template <typename T, int RUN>
+__global__ __launch_bounds__(kThreads) void sum_kernel(GradArgs p) {
+    const int64_t it = (int64_t)blockIdx.x * (kThreads / 64) + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    if (it < p.runs * p.steps) sum_run<T, RUN>(p, it / p.steps, (int)(it % p.steps));
 }
 
+// Rows of several pieces: a block adds them for 64 vectors of columns, a wave each
+// fourth of them, eight at a time.
+constexpr int kJoinBlocks = 2048;
 template <typename T>
-__global__ __launch_bounds__(kThreads) void grad_kernel(GradArgs p) {
-    if ((int64_t)blockIdx.x >= p.sum_blocks) {
-        fill_rows<T>(p, (int64_t)blockIdx.x - p.sum_blocks);
-        return;
-    }
-    const int64_t it = (int64_t)blockIdx.x * (kThreads / 64) + (int)(threadIdx.x >> 6);
-    if (it < p.runs * p.steps) sum_run<T>(p, it / p.steps, (int)(it % p.steps));
-}
-
-// Rows whose entries lie in several runs: the run they begin in finds their end
-// and adds the pieces, a wave each 16th of them.
-constexpr int kJoin = 1024;
-template <typename T>
-__global__ __launch_bounds__(kJoin) void join_kernel(GradArgs p) {
-    constexpr int VE = Elem<T>::kVec, WAVES = kJoin / 64;
+__global__ __launch_bounds__(kThreads) void join_kernel(GradArgs p) {
+    constexpr int VE = Elem<T>::kVec, WAVES = kThreads / 64;
     __shared__ float sh[WAVES][64 * VE];
-    const int64_t run = (int64_t)blockIdx.x / p.steps;
     const int wave = (int)threadIdx.x >> 6, lane = (int)threadIdx.x & 63;
-    const int v = (int)((int64_t)blockIdx.x % p.steps) * 64 + lane;
-    const int64_t last = run * kRun + kRun - 1;
-    if (last + 1 >= p.n) return;
-    const uint32_t id = p.e[last].id;
-    if (id >= p.V || p.e[last + 1].id != id) return;
-    if (p.e[run * kRun].id == id && run > 0 && p.e[run * kRun - 1].id == id) return;  // began before
-    int64_t lo = last + 1, hi = p.n;  // the first entry past the row's
-    while (lo < hi) {
-        const int64_t mid = (lo + hi) / 2;
-        if (p.e[mid].id <= id) lo = mid + 1;
-        else hi = mid;
-    }
-    const int64_t pieces = (lo - 1) / kRun - run + 1;
-    const int nvec = row_vectors<T>(p.D);
-    float acc[VE] = {};
-    if (v < nvec) {
-        const int64_t at = p.D >= VE ? row_vec_at<T>(p.D, v) : 0;
-        const int n = p.D >= VE ? VE : (int)p.D;
-        for (int64_t k = wave; k < pieces; k += WAVES) {
-            const float* from = p.part + ((run + k) * 2 + (k == 0 ? 1 : 0)) * p.D + at;
-#pragma unroll
-            for (int j = 0; j < VE; ++j)
-                if (j < n) acc[j] += from[j];
+    const int64_t items = (int64_t)*p.joins * p.steps;
+    for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
+        const int64_t run = p.list[it / p.steps];
+        const int v = (int)(it % p.steps) * 64 + lane;
+        const uint32_t id = p.e[run * p.run + p.run - 1].id;
+        // the row has a piece in each following run that begins with it
+        int64_t pieces = 1;
+        for (bool on = true; on;) {
+            const int64_t r = run + pieces + lane;
+            const uint64_t not_its = __ballot(r >= p.runs || p.e[r * p.run].id != id);
+            pieces += not_its ? __builtin_ctzll(not_its) : 64;
+            on = not_its == 0;
         }
-    }
+        const bool live = v < row_vectors<T>(p.D);
+        const int64_t at = live && p.D >= VE ? row_vec_at<T>(p.D, v) : 0;
+        const int n = p.D >= VE ? VE : (int)p.D;
+        float acc[VE] = {};
+        for (int64_t k0 = wave; k0 < pieces; k0 += WAVES * kPieces) {
+            float f[kPieces][VE];
 #pragma unroll
-    for (int j = 0; j < VE; ++j) sh[wave][lane * VE + j] = acc[j];
-    __syncthreads();
-    if (wave == 0 && v < nvec) {
-        for (int w = 1; w < WAVES; ++w)
+            for (int u = 0; u < kPieces; ++u) {
+                const int64_t k = k0 + u * WAVES;
+                const float* from = p.part + ((run + k) * 2 + (k == 0 ? 1 : 0)) * p.D + at;
+                const bool on = live && k < pieces;
 #pragma unroll
-            for (int j = 0; j < VE; ++j) acc[j] += sh[w][lane * VE + j];
+                for (int j = 0; j < VE; j += 4) {
+                    f32x4 q{0, 0, 0, 0};
+                    if (on && n == VE) {
+                        __builtin_memcpy(&q, from + j, 16);
+                    } else if (on) {
 #pragma unroll
-        for (int j = 0; j < VE; ++j) acc[j] *= p.scale;
-        row_store(static_cast<T*>(p.dw) + id * p.D, p.D, v, pack_vec<T>(acc));
+                        for (int i = 0; i < 4; ++i)
+                            if (j + i < n) q[i] = from[j + i];
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) f[u][j + i] = q[i];
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < kPieces; ++u)
+#pragma unroll
+                for (int j = 0; j < VE; ++j) acc[j] += f[u][j];
+        }
+        __syncthreads();  // the item before is done with sh
+#pragma unroll
+        for (int j = 0; j < VE; ++j) sh[wave][lane * VE + j] = acc[j];
+        __syncthreads();
+        if (wave == 0 && live) {
+#pragma unroll
+            for (int w = 1; w < WAVES; ++w)
+#pragma unroll
+                for (int j = 0; j < VE; ++j) acc[j] += sh[w][lane * VE + j];
+#pragma unroll
+            for (int j = 0; j < VE; ++j) acc[j] *= p.scale;
+            row_store(static_cast<T*>(p.dw) + id * p.D, p.D, v, pack_vec<T>(acc));
+        }
     }
 }
 
@@ -325,30 +353,39 @@ void by_type(int dtype, F f) {
 
 int vectors(int64_t D, int dtype) { return dtype == 0 ? row_vectors<float>(D) : row_vectors<_Float16>(D); }
 
-// Digits that the ids 0 .. V (V: no gradient) are sorted by, of ten bits at most.
-void digits(int64_t V, int& passes, int& bits) {
+// Digits that the ids 0 .. V (V: no gradient) are sorted by, of ten bits at most, of six where one block sorts.
+void digits(int64_t n, int64_t V, int& passes, int& bits) {
+    const int most = n <= kAlone ? kAloneBits : 10;
     int all = 1;
     while (((int64_t)1 << all) <= V) ++all;
-    passes = (all + 9) / 10;
+    passes = (all + most - 1) / most;
     bits = (all + passes - 1) / passes;
 }
 
 int64_t align256(int64_t v) { return (v + 255) & ~(int64_t)255; }
 
+// Entries of a run: as many as a wave has loads in flight, or 64, which leave fewer
+// pieces to join, where that many waves keep the memory busy: (65536, 2048), all of
+// one token, 137 us for 253, but (32768, 1024) 90 for 69.
+int run_of(int64_t n, int64_t D) { return n * D >= (1 << 26) ? 64 : kAhead; }
+int64_t runs_of(int64_t n, int64_t D) { return (n + run_of(n, D) - 1) / run_of(n, D); }
+
 struct Ws {
-    int64_t a, b, hist, total, part, bytes;
+    int64_t joins, list, a, b, hist, total, part, bytes;
 };
 Ws ws_layout(int64_t n, int64_t V, int64_t D) {
     int passes, bits;
-    digits(V, passes, bits);
+    digits(n, V, passes, bits);
     Ws w{};
-    const bool alone = n <= key_sort::kChunk;
-    w.a = 0;
-    w.b = align256(8 * n);
+    const bool alone = n <= kAlone;
+    w.joins = 0;
+    w.list = 256;
+    w.a = w.list + align256(4 * runs_of(n, D));
+    w.b = w.a + align256(8 * n);
     w.hist = w.b + (alone || passes == 1 ? 0 : align256(8 * n));
     w.total = w.hist + (alone ? 0 : align256(4 * (key_sort::chunks(n) << bits)));
     w.part = w.total + (alone ? 0 : align256((int64_t)4 << bits));
-    w.bytes = w.part + (n <= kRun ? 0 : 8 * D * ((n + kRun - 1) / kRun));
+    w.bytes = w.part + (n <= kAhead ? 0 : 8 * D * runs_of(n, D));
     return w;
 }
 
@@ -367,11 +404,12 @@ extern "C" int fl_embedding_fwd(const void* weight, int64_t row_stride, int64_t 
     FL_CHECK(row_stride >= D, "%s: rows of the matrix overlap", name);
     FL_CHECK(weight && index && out, "%s: NULL pointer argument", name);
     FL_CHECK(aligned(weight, dtype) && aligned(out, dtype), "%s: pointers are not element-aligned", name);
-    LookupArgs a{weight, row_stride, V, D, index, N, scale, out, 0, 0, 0};
+    LookupArgs a{weight, row_stride, V, D, index, N, scale, out, 0, 0, 0, false};
     const int nvec = vectors(D, dtype);
     a.lanes = row_lanes(nvec);
     a.steps = row_steps(nvec);
     a.items = N * a.steps;
+    a.through = a.lanes == 64 && D % (dtype == 0 ? 4 : 8) == 0 && (reinterpret_cast<uintptr_t>(out) & 15u) == 0;
     const int per = kThreads / a.lanes;
     const int64_t want = (a.items + per - 1) / per;
     const unsigned blocks = (unsigned)(want < (1 << 22) ? want : (1 << 22));
@@ -398,17 +436,35 @@ extern "C" int fl_embedding_bwd(const void* grad, int64_t grad_stride, const int
     const Ws w = ws_layout(N, V, D);
     FL_CHECK((int64_t)workspace_bytes >= w.bytes, "%s: workspace of %llu bytes, %lld needed", name,
              (unsigned long long)workspace_bytes, (long long)w.bytes);
-    FL_CHECK(w.bytes == 0 || (workspace && (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0),
+    FL_CHECK((workspace && (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0),
              "%s: workspace is not 256-byte aligned", name);
+    if ((N + kAhead - 1) / kAhead * row_steps(vectors(D, dtype)) > max_grid_blocks(kThreads))
+        return set_error(FL_ERANGE, "%s: N=%lld, V=%lld, D=%lld are too many for a launch", name, (long long)N,
+                         (long long)V, (long long)D);
     char* ws = static_cast<char*>(workspace);
     hipStream_t s = static_cast<hipStream_t>(stream);
     int passes, bits;
-    digits(V, passes, bits);
+    digits(N, V, passes, bits);
     Entry* sorted = reinterpret_cast<Entry*>(ws + w.a);
     const FirstKey first{index, V, padding, (1 << bits) - 1};
-    if (N > 0 && N <= key_sort::kChunk) {
-        sort_alone<<<1, key_sort::kThreads, 0, s>>>(first, (int)N, bits, passes, sorted);
-    } else if (N > 0) {
+    int* joins = reinterpret_cast<int*>(ws + w.joins);
+    // dW's zeros in `shares` parts, of which each launch takes the next ones
+    char* dw = static_cast<char*>(grad_weight);
+    const int64_t dw_bytes = V * D * (dtype == 0 ? 4 : 2);
+    const bool alone = N <= kAlone;
+    const int shares = alone ? 1 : 3 * passes;
+    const int64_t per = align256(dw_bytes / shares + 1);
+    int64_t done = 0;
+    const auto zeros = [&](int parts) {
+        int64_t bytes = per * parts < dw_bytes - done ? per * parts : dw_bytes - done;
+        const Zeros z{dw + done, bytes, joins};
+        done += bytes;
+        return z;
+    };
+    if (alone) {
+        const Zeros z = zeros(1);
+        sort_alone<<<1 + z.blocks(), key_sort::kThreads, 0, s>>>(first, (int)N, bits, passes, sorted, z);
+    } else {
         int* hist = reinterpret_cast<int*>(ws + w.hist);
         int* total = reinterpret_cast<int*>(ws + w.total);
         const unsigned blocks = (unsigned)key_sort::chunks(N);
@@ -419,11 +475,17 @@ extern "C" int fl_embedding_bwd(const void* grad, int64_t grad_stride, const int
         for (int pass = 0; pass < passes; ++pass) {
             Entry* from = to == sorted ? other : sorted;
             const NextKey next{from, pass * bits, bins - 1};
-            if (pass == 0) key_sort::count_kernel<<<blocks, key_sort::kThreads, 0, s>>>(first, N, bins, hist);
-            else key_sort::count_kernel<<<blocks, key_sort::kThreads, 0, s>>>(next, N, bins, hist);
-            key_sort::sum_kernel<<<(unsigned)((bins + 3) / 4), 256, 0, s>>>(hist, blocks, bins, total);
-            if (pass == 0) place_kernel<<<blocks, key_sort::kThreads, 0, s>>>(first, N, bits, hist, total, to);
-            else place_kernel<<<blocks, key_sort::kThreads, 0, s>>>(next, N, bits, hist, total, to);
+            const auto go = [&](auto key) {
+                const Zeros z1 = zeros(1), z2 = zeros(2);
+                key_sort::count_kernel<<<blocks + z1.blocks(), key_sort::kThreads, 0, s>>>(key, N, bins, hist, z1);
+                if (blocks > (unsigned)key_sort::kFewBlocks)
+                    key_sort::sum_kernel<<<(unsigned)((bins + 63) / 64), key_sort::kThreads, 0, s>>>(hist, (int)blocks,
+                                                                                                    bins, total);
+                place_kernel<<<blocks + z2.blocks(), key_sort::kThreads, 0, s>>>(key, N, bits, (int)blocks, hist, total,
+                                                                                 to, z2);
+            };
+            if (pass == 0) go(first);
+            else go(next);
             to = from;
         }
     }
@@ -437,16 +499,19 @@ extern "C" int fl_embedding_bwd(const void* grad, int64_t grad_stride, const int
     a.scale = scale;
     a.dw = grad_weight;
     a.part = reinterpret_cast<float*>(ws + w.part);
-    a.runs = (N + kRun - 1) / kRun;
+    a.run = run_of(N, D);
+    a.runs = runs_of(N, D);
     a.steps = row_steps(vectors(D, dtype));
-    a.sum_blocks = (a.runs * a.steps + kThreads / 64 - 1) / (kThreads / 64);
-    const int64_t fill = (V + kFillRows - 1) / kFillRows;
-    const int64_t joins = a.runs > 1 ? (a.runs - 1) * a.steps : 0;
-    if (a.sum_blocks + fill > max_grid_blocks(kThreads) || joins > max_grid_blocks(kJoin))
-        return set_error(FL_ERANGE, "%s: too many tokens for rows of %lld columns", name, (long long)D);
+    a.joins = joins;
+    a.list = reinterpret_cast<int*>(ws + w.list);
+    if (N == 0) return launch_status(name);
+    const int64_t sums = (a.runs * a.steps + kThreads / 64 - 1) / (kThreads / 64);
+    const int64_t most = (a.runs - 1) * a.steps;
+    const unsigned blocks = (unsigned)(most < kJoinBlocks ? most : kJoinBlocks);
     by_type(dtype, [&](auto t) {
-        grad_kernel<decltype(t)><<<(unsigned)(a.sum_blocks + fill), kThreads, 0, s>>>(a);
-        if (joins) join_kernel<decltype(t)><<<(unsigned)joins, kJoin, 0, s>>>(a);
+        if (a.run == 64) sum_kernel<decltype(t), 64><<<(unsigned)sums, kThreads, 0, s>>>(a);
+        else sum_kernel<decltype(t), kAhead><<<(unsigned)sums, kThreads, 0, s>>>(a);
+        if (blocks) join_kernel<decltype(t)><<<blocks, kThreads, 0, s>>>(a);
     });
     return launch_status(name);
 }

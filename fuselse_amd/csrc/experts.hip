@@ -66,26 +66,21 @@ __device__ __forceinline__ void write_counts(const OrderArgs& p, const int (&tot
 
 template <bool ALONE>
 __global__ __launch_bounds__(key_sort::kThreads) void place_kernel(OrderArgs p) {
-    __shared__ key_sort::Shared sh;
+    __shared__ key_sort::Shared<> sh;
     const int64_t first = (int64_t)blockIdx.x * key_sort::kChunk;
     const int m = (int)(p.n - first < key_sort::kChunk ? p.n - first : key_sort::kChunk);
     const int bins = p.key.experts + 1;
-    int key[key_sort::kRounds], place[key_sort::kRounds], total[2], start[2];
+    int key[key_sort::kRounds], place[key_sort::kRounds], total[2], start[2], before[2] = {}, own[2];
 #pragma unroll
     for (int j = 0; j < key_sort::kRounds; ++j)
         key[j] = key_sort::entry(j) < m ? p.key(first + key_sort::entry(j)) : 0;
-    key_sort::rank(sh, key, m, bins, p.bits, place, total);
+    if constexpr (!ALONE) key_sort::load_counts(p.hist, p.total, (int)p.blocks, bins, total, before);
+    key_sort::rank(sh, key, m, bins, p.bits, place, own);
     if constexpr (ALONE) {
-        key_sort::starts(sh, total, bins, start);
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const int b = (int)threadIdx.x + j * key_sort::kThreads;
-            if (b < bins) sh.start[b] = start[j];
-        }
-        __syncthreads();
-    } else {
-        key_sort::block_starts(sh, p.hist, p.total, p.blocks, bins, total, start);
+        total[0] = own[0];
+        total[1] = own[1];
     }
+    key_sort::block_starts(sh, total, before, bins, start);
     if (blockIdx.x == 0) write_counts(p, total, start);
 #pragma unroll
     for (int j = 0; j < key_sort::kRounds; ++j)
@@ -170,14 +165,8 @@ __global__ __launch_bounds__(kThreads) void dispatch_kernel(RowArgs p) {
                 T* to = static_cast<T*>(p.out) + row * p.D;
                 u32x4 r = x;
                 if (at[u] < 0) r = u32x4{0, 0, 0, 0};
-                if (WAVE && p.through) {  // a row of 64 MB at most
-                    const __amdgpu_buffer_rsrc_t rsrc =
-                        __builtin_amdgcn_make_buffer_rsrc(to, 0, (int)(p.D * sizeof(T)), 0x00020000);
-                    __builtin_amdgcn_raw_buffer_store_b128(r, rsrc, (int)(row_vec_at<T>(p.D, v) * sizeof(T)), 0,
-                                                           kStoreStreamAux);
-                } else {
-                    row_store(to, p.D, v, r);
-                }
+                if (WAVE && p.through) row_store_through(to, p.D, v, r);
+                else row_store(to, p.D, v, r);
             }
         }
     }
@@ -420,8 +409,10 @@ extern "C" int fl_expert_order(const int64_t* index, int64_t tokens, int64_t top
     a.total = static_cast<int*>(workspace);
     a.hist = a.total + bins;
     const unsigned blocks = (unsigned)a.blocks;
-    key_sort::count_kernel<<<blocks, key_sort::kThreads, 0, s>>>(a.key, a.n, bins, a.hist);
-    key_sort::sum_kernel<<<(unsigned)((bins + 3) / 4), 256, 0, s>>>(a.hist, a.blocks, bins, a.total);
+    key_sort::count_kernel<<<blocks, key_sort::kThreads, 0, s>>>(a.key, a.n, bins, a.hist, key_sort::NoWork{});
+    if (a.blocks > key_sort::kFewBlocks)
+        key_sort::sum_kernel<<<(unsigned)((bins + 63) / 64), key_sort::kThreads, 0, s>>>(a.hist, (int)a.blocks, bins,
+                                                                                        a.total);
     place_kernel<false><<<blocks, key_sort::kThreads, 0, s>>>(a);
     return launch_status(name);
 }

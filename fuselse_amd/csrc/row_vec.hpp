@@ -49,6 +49,18 @@ __device__ __forceinline__ void row_store(T* row, int64_t D, int v, u32x4 r) {
         if (k < D) row[k] = part[k];
 }
 
+// The same written through to memory, for a row that all of a wave has and that is
+// whole, aligned vectors, of 64 MB at most.
+template <typename T>
+__device__ __forceinline__ void row_store_through(T* row, int64_t D, int v, u32x4 r) {
+    const uint64_t a = reinterpret_cast<uint64_t>(row);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)a);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(a >> 32));
+    const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
+        reinterpret_cast<void*>((uint64_t)hi << 32 | lo), 0, (int)(D * sizeof(T)), 0x00020000);
+    __builtin_amdgcn_raw_buffer_store_b128(r, rsrc, (int)(row_vec_at<T>(D, v) * sizeof(T)), 0, kStoreStreamAux);
+}
+
 // fp32 values rounded to the type, once.
 template <typename T>
 __device__ __forceinline__ u32x4 pack_vec(const float (&v)[Elem<T>::kVec]) {

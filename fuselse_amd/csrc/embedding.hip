@@ -98,15 +98,22 @@ struct Zeros {
     __device__ __forceinline__ void operator()(int64_t block) const {
         if (block == 0 && threadIdx.x == 0) *joins = 0;
         int64_t first = block * kBytes;
-        for (; first + kBytes <= bytes; first += (int64_t)kBlocks * kBytes) {
-            const bool aligned = (reinterpret_cast<uintptr_t>(at) & 15u) == 0;
-            const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(at + first, 0, kBytes, 0x00020000);
+        if ((reinterpret_cast<uintptr_t>(at) & 15u) == 0) {
+            for (; first + kBytes <= bytes; first += (int64_t)kBlocks * kBytes) {
+                const __amdgpu_buffer_rsrc_t rsrc =
+                    __builtin_amdgcn_make_buffer_rsrc(at + first, 0, kBytes, 0x00020000);
 #pragma unroll
-            for (int j = 0; j < kSteps; ++j) {
-                const int k = 16 * (j * key_sort::kThreads + (int)threadIdx.x);
-                if (aligned) __builtin_amdgcn_raw_buffer_store_b128(u32x4{0, 0, 0, 0}, rsrc, k, 0, kStoreStreamAux);
-                else *reinterpret_cast<u32x4_any*>(at + first + k) = u32x4{0, 0, 0, 0};
+                for (int j = 0; j < kSteps; ++j)
+                    __builtin_amdgcn_raw_buffer_store_b128(u32x4{0, 0, 0, 0}, rsrc,
+                                                           16 * (j * key_sort::kThreads + (int)threadIdx.x), 0,
+                                                           kStoreStreamAux);
             }
+        } else {
+            for (; first + kBytes <= bytes; first += (int64_t)kBlocks * kBytes)
+#pragma unroll
+                for (int j = 0; j < kSteps; ++j)
+                    *(reinterpret_cast<u32x4_any*>(at + first) + j * key_sort::kThreads + (int)threadIdx.x) =
+                        u32x4{0, 0, 0, 0};
         }
         if (first < bytes)  // the share's end: whole elements, of two bytes at least
             for (int64_t k = first + 2 * (int)threadIdx.x; k < bytes; k += 2 * key_sort::kThreads)

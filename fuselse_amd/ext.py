@@ -1154,8 +1154,31 @@ def router_balance_backward(grad_balance, grad_z, logits: torch.Tensor, mask, ls
 
 
 # ---------------------------------------------------------------------------
-# Layers around the losses (no reference counterpart)
+# Layers around the losses (no reference counterpart).  Most of a small call's
+# time is the host's, so each first asks in one expression whether its tensors
+# are as most callers have them, and checks them one by one only if not.
 # ---------------------------------------------------------------------------
+def _launch(t, name, *args):
+    """Entry point `name` with args on t's device and its current stream."""
+    idx = t.device.index
+    if _raw_stream is not None and idx == _current_device():
+        _lib.call(name, *args, _raw_stream(idx))
+    else:
+        with _on_device(t):
+            _lib.call(name, *args, _stream(t))
+
+
+def _plain(t, dim):
+    """t is a contiguous CUDA tensor of `dim` dimensions of a type the kernels
+    take, and not empty."""
+    return t.is_cuda and t.dtype in _DTYPE_CODE and t.dim() == dim and t.is_contiguous() and t.numel() > 0
+
+
+def _rows_like(t):
+    """An uninitialised contiguous tensor of t's shape, type and device."""
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+
+
 def _check_rows(t, name):
     """t is 2D with contiguous rows that do not overlap, of a type the kernels
     take; a tensor of one row may carry any row stride."""
@@ -1176,6 +1199,9 @@ def _ptr(t):
 
 
 def _check_embedding(weight, index):
+    if (_plain(weight, 2) and index.dtype == torch.int64 and index.dim() == 1 and index.device == weight.device
+            and index.is_contiguous()):
+        return
     _check_rows(weight, "weight")
     _check(weight.shape[0] >= 1, "weight must not be empty")
     _check(index.is_cuda, "index must be CUDA")
@@ -1195,23 +1221,20 @@ def embedding(weight: torch.Tensor, index: torch.Tensor, scale: float = 1.0) -> 
 def _embedding_fwd(weight, index, scale):
     V, D = weight.shape
     N = index.shape[0]
-    out = torch.empty((N, D), dtype=weight.dtype, device=weight.device)
+    out = weight.new_empty((N, D))
     if N:
-        with _on_device(weight):
-            _lib.call("fl_embedding_fwd", weight.data_ptr(), _row_stride(weight), V, D, _DTYPE_CODE[weight.dtype],
-                      index.data_ptr(), N, scale, out.data_ptr(), _stream(weight))
+        _launch(weight, "fl_embedding_fwd", weight.data_ptr(), _row_stride(weight), V, D, _DTYPE_CODE[weight.dtype],
+                index.data_ptr(), N, scale, out.data_ptr())
     return out
 
 
 def _embedding_bwd(grad, index, V, scale, padding):
     N, D = grad.shape
-    dev = grad.device
-    out = torch.empty((V, D), dtype=grad.dtype, device=dev)
+    out = grad.new_empty((V, D))
     nbytes = _remembered(("embedding", N, V, D), "fl_embedding_bwd_workspace_bytes", N, V, D)
-    with _on_device(grad):
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        _lib.call("fl_embedding_bwd", grad.data_ptr(), _row_stride(grad), index.data_ptr(), N, V, D,
-                  _DTYPE_CODE[grad.dtype], scale, padding, out.data_ptr(), ws.data_ptr(), nbytes, _stream(grad))
+    ws = grad.new_empty((nbytes,), dtype=torch.uint8)
+    _launch(grad, "fl_embedding_bwd", grad.data_ptr(), _row_stride(grad), index.data_ptr(), N, V, D,
+            _DTYPE_CODE[grad.dtype], scale, padding, out.data_ptr(), ws.data_ptr(), nbytes)
     return out
 
 
@@ -1229,7 +1252,15 @@ def embedding_backward(grad_output: torch.Tensor, index: torch.Tensor, num_embed
     return _embedding_bwd(grad_output, index, num_embeddings, scale, padding_idx)
 
 
+def _plain_param(t, x):
+    return t is None or (t.dim() == 1 and t.shape[0] == x.shape[1] and t.device == x.device and t.is_contiguous()
+                         and (t.dtype == x.dtype or t.dtype == torch.float32))
+
+
 def _check_norm(x, weight, bias):
+    if (_plain(x, 2) and _plain_param(weight, x) and _plain_param(bias, x)
+            and (weight is None or bias is None or weight.dtype == bias.dtype)):
+        return
     _check_rows(x, "x")
     of = (x.dtype, torch.float32) if x.dtype != torch.float32 else (torch.float32,)
     for t, nm in ((weight, "weight"), (bias, "bias")):
@@ -1237,11 +1268,6 @@ def _check_norm(x, weight, bias):
             _check_vector(t, nm, x.shape[1], of)
     _check(weight is None or bias is None or weight.dtype == bias.dtype, "weight and bias must be of one type")
     _check_device(x, "x", weight=weight, bias=bias)
-
-
-def _params_code(x, weight, bias):
-    t = weight if weight is not None else bias
-    return _DTYPE_CODE[t.dtype] if t is not None else 0
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
@@ -1253,33 +1279,37 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     return _norm_fwd(x, weight, bias, eps, with_stats)
 
 
+def _params_code(weight, bias):
+    t = weight if weight is not None else bias
+    return _DTYPE_CODE[t.dtype] if t is not None else 0
+
+
 def _norm_fwd(x, weight, bias, eps, with_stats):
-    N, D = x.shape
-    y = torch.empty((N, D), dtype=x.dtype, device=x.device)
-    stats = torch.empty((N, 4), dtype=torch.float32, device=x.device) if with_stats else None
     _check(eps >= 0, "eps must be at least 0")
+    N, D = x.shape
+    y = _rows_like(x)
+    stats = x.new_empty((N, 4), dtype=torch.float32) if with_stats else None
     if N:
-        with _on_device(x):
-            _lib.call("fl_layer_norm_fwd", x.data_ptr(), _row_stride(x), N, D, _DTYPE_CODE[x.dtype], _ptr(weight),
-                      _ptr(bias), _params_code(x, weight, bias), eps, y.data_ptr(), _ptr(stats), _stream(x))
+        _launch(x, "fl_layer_norm_fwd", x.data_ptr(), _row_stride(x), N, D, _DTYPE_CODE[x.dtype], _ptr(weight),
+                _ptr(bias), _params_code(weight, bias), eps, y.data_ptr(), _ptr(stats))
     return y, stats
 
 
-def _norm_bwd(grad, x, weight, bias, stats, need_x, need_weight, need_bias):
+def _norm_bwd(grad, x, weight, params_dtype, stats, need_x, need_weight, need_bias):
+    """Gradients of those that are needed; the parameters' are of params_dtype
+    (of neither: None)."""
     N, D = x.shape
-    dev = x.device
-    dx = torch.empty((N, D), dtype=x.dtype, device=dev) if need_x else None
-    dw = torch.empty_like(weight) if need_weight else None
-    db = torch.empty_like(bias) if need_bias else None
+    dx = _rows_like(x) if need_x else None
+    dw = x.new_empty((D,), dtype=params_dtype) if need_weight else None
+    db = x.new_empty((D,), dtype=params_dtype) if need_bias else None
     dt = _DTYPE_CODE[x.dtype]
-    nbytes = 0
+    nbytes, ws = 0, None
     if need_weight or need_bias:
         nbytes = _remembered(("norm", N, D, dt), "fl_layer_norm_bwd_workspace_bytes", N, D, dt)
-    with _on_device(x):
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        _lib.call("fl_layer_norm_bwd", grad.data_ptr(), _row_stride(grad), x.data_ptr(), _row_stride(x), N, D, dt,
-                  _ptr(weight), _params_code(x, weight, bias), stats.data_ptr(), _ptr(dx), _ptr(dw), _ptr(db),
-                  ws.data_ptr(), nbytes, _stream(x))
+        ws = x.new_empty((nbytes,), dtype=torch.uint8)
+    _launch(x, "fl_layer_norm_bwd", grad.data_ptr(), _row_stride(grad), x.data_ptr(), _row_stride(x), N, D, dt,
+            _ptr(weight), _DTYPE_CODE.get(params_dtype, 0), stats.data_ptr(), _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws),
+            nbytes)
     return dx, dw, db
 
 
@@ -1293,8 +1323,9 @@ def layer_norm_backward(grad_output: torch.Tensor, x: torch.Tensor, weight, bias
     _check(stats.is_cuda and stats.dtype == torch.float32 and stats.is_contiguous()
            and tuple(stats.shape) == (x.shape[0], 4), "stats must be contiguous CUDA float32 (N, 4)")
     _check_device(x, "x", grad_output=grad_output, stats=stats)
-    return _norm_bwd(grad_output, x, weight, bias, stats, need_x, need_weight and weight is not None,
-                     need_bias and bias is not None)
+    of = weight if weight is not None else bias
+    return _norm_bwd(grad_output, x, weight, of.dtype if of is not None else None, stats, need_x,
+                     need_weight and weight is not None, need_bias and bias is not None)
 
 
 def _check_order(index, experts, mask):
@@ -1305,7 +1336,7 @@ def _check_order(index, experts, mask):
     if mask is not None:
         _check(mask.is_cuda and mask.dtype == torch.bool and mask.is_contiguous() and mask.dim() == 1
                and mask.shape[0] == index.shape[0], "mask must be a contiguous CUDA bool tensor (tokens,)")
-    _check_device(index, "index", mask=mask)
+        _check_device(index, "index", mask=mask)
 
 
 def expert_order(index: torch.Tensor, num_experts: int, mask: Optional[torch.Tensor] = None):
@@ -1320,26 +1351,28 @@ def expert_order(index: torch.Tensor, num_experts: int, mask: Optional[torch.Ten
 
 def _order(index, experts, mask):
     T, K = index.shape
-    dev = index.device
-    position = torch.empty((T, K), dtype=torch.int32, device=dev)
-    counts = torch.empty((experts,), dtype=torch.int64, device=dev)
-    offsets = torch.empty((experts + 1,), dtype=torch.int32, device=dev)
+    position = index.new_empty((T, K), dtype=torch.int32)
+    counts = index.new_empty((experts,))
+    offsets = index.new_empty((experts + 1,), dtype=torch.int32)
     nbytes = _remembered(("order", T, K, experts), "fl_expert_order_workspace_bytes", T, K, experts)
-    with _on_device(index):
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-        _lib.call("fl_expert_order", index.data_ptr(), T, K, experts, _ptr(mask), position.data_ptr(),
-                  counts.data_ptr(), offsets.data_ptr(), _ptr(ws), nbytes, _stream(index))
+    ws = index.new_empty((nbytes,), dtype=torch.uint8) if nbytes else None
+    _launch(index, "fl_expert_order", index.data_ptr(), T, K, experts, _ptr(mask), position.data_ptr(),
+            counts.data_ptr(), offsets.data_ptr(), _ptr(ws), nbytes)
     return position, counts, offsets
 
 
 def _check_position(ref, ref_name, position):
+    if (position.dtype == torch.int32 and position.dim() == 2 and position.is_contiguous()
+            and position.device == ref.device and position.shape[1] >= 1 and ref.is_cuda):
+        return
     _check(position.is_cuda and position.dtype == torch.int32 and position.dim() == 2 and position.is_contiguous()
            and position.shape[1] >= 1, "position must be a contiguous CUDA int32 tensor (tokens, top)")
     _check_device(ref, ref_name, position=position)
 
 
 def _check_dispatch(x, position):
-    _check_rows(x, "x")
+    if not _plain(x, 2):
+        _check_rows(x, "x")
     _check_position(x, "x", position)
     _check(x.shape[0] == position.shape[0], "x must be (tokens, D) with the tokens of position")
 
@@ -1355,24 +1388,24 @@ def expert_dispatch(x: torch.Tensor, position: torch.Tensor) -> torch.Tensor:
 def _dispatch(x, position):
     T, D = x.shape
     K = position.shape[1]
-    rows = torch.empty((T * K, D), dtype=x.dtype, device=x.device)
+    rows = x.new_empty((T * K, D))
     if T:
-        with _on_device(x):
-            _lib.call("fl_expert_dispatch", x.data_ptr(), _row_stride(x), T, D, _DTYPE_CODE[x.dtype],
-                      position.data_ptr(), K, rows.data_ptr(), _stream(x))
+        _launch(x, "fl_expert_dispatch", x.data_ptr(), _row_stride(x), T, D, _DTYPE_CODE[x.dtype],
+                position.data_ptr(), K, rows.data_ptr())
     return rows
 
 
 def _check_combine(rows, weights, position):
-    _check_rows(rows, "rows")
+    if not _plain(rows, 2):
+        _check_rows(rows, "rows")
     _check_position(rows, "rows", position)
     T, K = position.shape
     _check(rows.shape[0] == T * K, "rows must be (tokens * top, D)")
     if weights is not None:
-        _check(weights.is_cuda and weights.is_contiguous() and tuple(weights.shape) == (T, K)
-               and weights.dtype in (rows.dtype, torch.float32),
+        _check(weights.is_cuda and weights.is_contiguous() and weights.shape == position.shape
+               and (weights.dtype == rows.dtype or weights.dtype == torch.float32),
                "weights must be a contiguous CUDA tensor (tokens, top) of rows' type or float32")
-    _check_device(rows, "rows", weights=weights)
+        _check(weights.device == rows.device, "weights must be on the same device as rows")
 
 
 def expert_combine(rows: torch.Tensor, weights: Optional[torch.Tensor], position: torch.Tensor) -> torch.Tensor:
@@ -1386,25 +1419,22 @@ def expert_combine(rows: torch.Tensor, weights: Optional[torch.Tensor], position
 def _combine(rows, weights, position):
     T, K = position.shape
     D = rows.shape[1]
-    out = torch.empty((T, D), dtype=rows.dtype, device=rows.device)
+    out = rows.new_empty((T, D))
     if T:
-        with _on_device(rows):
-            _lib.call("fl_expert_combine", rows.data_ptr(), _row_stride(rows), T, D, _DTYPE_CODE[rows.dtype],
-                      position.data_ptr(), K, _ptr(weights), _DTYPE_CODE[weights.dtype] if weights is not None else 0,
-                      out.data_ptr(), _stream(rows))
+        _launch(rows, "fl_expert_combine", rows.data_ptr(), _row_stride(rows), T, D, _DTYPE_CODE[rows.dtype],
+                position.data_ptr(), K, _ptr(weights), _DTYPE_CODE[weights.dtype] if weights is not None else 0,
+                out.data_ptr())
     return out
 
 
 def _combine_bwd(grad, rows, weights, position, need_rows, need_weights):
     T, K = position.shape
-    D = rows.shape[1]
-    d_rows = torch.empty((T * K, D), dtype=rows.dtype, device=rows.device) if need_rows else None
+    d_rows = _rows_like(rows) if need_rows else None
     d_weights = torch.empty_like(weights) if need_weights else None
     if T:
-        with _on_device(rows):
-            _lib.call("fl_expert_combine_bwd", grad.data_ptr(), _row_stride(grad), rows.data_ptr(), _row_stride(rows),
-                      T, D, _DTYPE_CODE[rows.dtype], position.data_ptr(), K, weights.data_ptr(),
-                      _DTYPE_CODE[weights.dtype], _ptr(d_rows), _ptr(d_weights), _stream(rows))
+        _launch(rows, "fl_expert_combine_bwd", grad.data_ptr(), _row_stride(grad), rows.data_ptr(), _row_stride(rows),
+                T, rows.shape[1], _DTYPE_CODE[rows.dtype], position.data_ptr(), K, weights.data_ptr(),
+                _DTYPE_CODE[weights.dtype], _ptr(d_rows), _ptr(d_weights))
     return d_rows, d_weights
 
 

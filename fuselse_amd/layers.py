@@ -21,6 +21,22 @@ from . import ext
 from .losses import _integers, _rows
 
 
+def _once(backward):
+    """once_differentiable, but for the common call outside create_graph, which
+    has no graph to keep from being made."""
+    guarded = once_differentiable(backward)
+
+    def run(ctx, grad):
+        return guarded(ctx, grad) if torch.is_grad_enabled() else backward(ctx, grad)
+
+    return staticmethod(run)
+
+
+def _flat(t: torch.Tensor) -> torch.Tensor:
+    """t in rows, as the kernels take them."""
+    return t if t.dim() == 2 and t.is_contiguous() else _rows(t)
+
+
 class _Embedding(torch.autograd.Function):
     @staticmethod
     def forward(ctx, weight, index, scale, padding):
@@ -28,11 +44,10 @@ class _Embedding(torch.autograd.Function):
         ctx.args = (weight.shape[0], scale, padding)
         return ext._embedding_fwd(weight, index, scale)
 
-    @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, grad):
         (index,) = ctx.saved_tensors
-        return ext._embedding_bwd(_rows(grad), index, *ctx.args), None, None, None
+        return ext._embedding_bwd(_flat(grad), index, *ctx.args), None, None, None
 
 
 def embedding(index: torch.Tensor, weight: torch.Tensor, scale: float = 1.0,
@@ -48,34 +63,39 @@ def embedding(index: torch.Tensor, weight: torch.Tensor, scale: float = 1.0,
     from the end) give none.  At most 2^30 tokens and vocabulary entries and
     2^20 columns.
     """
-    w = _rows(weight) if weight.dim() == 2 else weight
-    i = _integers(index, "index").reshape(-1).contiguous()
+    i = index
+    if i.dtype != torch.int64 or i.dim() != 1 or not i.is_contiguous():
+        i = _integers(i, "index").reshape(-1).contiguous()
+    w = _flat(weight) if weight.dim() == 2 else weight
     ext._check_embedding(w, i)
-    V, D = w.shape
     padding = -1
     if padding_idx is not None:
+        V = w.shape[0]
         ext._check(-V <= padding_idx < V, "padding_idx must be within the rows of weight")
         padding = padding_idx % V
-    if torch.is_grad_enabled() and weight.requires_grad:
+    if weight.requires_grad and torch.is_grad_enabled():
         out = _Embedding.apply(w, i, scale, padding)
     else:
         out = ext._embedding_fwd(w, i, scale)
-    return out if index.dim() == 1 else out.reshape(*index.shape, D)
+    return out if index.dim() == 1 else out.reshape(*index.shape, w.shape[1])
 
 
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
         y, stats = ext._norm_fwd(x, weight, bias, eps, True)
-        ctx.save_for_backward(x, weight, bias, stats)
+        ctx.save_for_backward(x, weight, stats)
+        of = weight if weight is not None else bias
+        ctx.params_dtype = of.dtype if of is not None else None
         return y
 
-    @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, grad):
-        x, weight, bias, stats = ctx.saved_tensors
+        x, weight, stats = ctx.saved_tensors
+        need = ctx.needs_input_grad
         # in rows again, which a saved-tensor hook may have changed
-        return *ext._norm_bwd(_rows(grad), _rows(x), weight, bias, stats, *ctx.needs_input_grad[:3]), None
+        dx, dw, db = ext._norm_bwd(_flat(grad), _flat(x), weight, ctx.params_dtype, stats, need[0], need[1], need[2])
+        return dx, dw, db, None
 
 
 def layer_norm(input: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
@@ -91,13 +111,15 @@ def layer_norm(input: torch.Tensor, weight: Optional[torch.Tensor] = None, bias:
     columns.
     """
     ext._check(input.dim() >= 1, "input must have a last dimension")
-    x = _rows(input)
-    params = [t for t in (weight, bias) if t is not None]
-    if params and not all(t.dtype == x.dtype for t in params):
-        weight, bias = (t.float() if t is not None and t.dtype in ext._DTYPE_CODE else t for t in (weight, bias))
-    weight, bias = (t.contiguous() if t is not None else None for t in (weight, bias))
+    x = _flat(input)
+    needs = input.requires_grad
+    if weight is not None or bias is not None:
+        needs = needs or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)
+        if any(t is not None and t.dtype != x.dtype for t in (weight, bias)):
+            weight, bias = (t.float() if t is not None and t.dtype in ext._DTYPE_CODE else t for t in (weight, bias))
+        weight, bias = (t.contiguous() if t is not None else None for t in (weight, bias))
     ext._check_norm(x, weight, bias)
-    if torch.is_grad_enabled() and (input.requires_grad or any(t.requires_grad for t in params)):
+    if needs and torch.is_grad_enabled():
         y = _LayerNorm.apply(x, weight, bias, eps)
     else:
         y = ext._norm_fwd(x, weight, bias, eps, False)[0]
@@ -126,23 +148,17 @@ def expert_order(index: torch.Tensor, num_experts: int, mask: Optional[torch.Ten
     takes.  At most 1024 experts, 1024 choices a token, 2^30 tokens and 2^31 - 1
     choices.
     """
-    ext._check(index.dim() >= 1, "index must be (..., top)")
-    ext._check(mask is None or tuple(mask.shape) == tuple(index.shape[:-1]),
-               "mask must have the shape of index's tokens")
-    i = _integers(index, "index")
-    i = i.reshape(i.shape[:-1].numel(), i.shape[-1]) if i.dim() != 2 else i
-    i = i.contiguous()
-    m = mask.reshape(-1).contiguous() if mask is not None else None
+    i, m = index, mask
+    if i.dtype != torch.int64 or i.dim() != 2 or not i.is_contiguous():
+        ext._check(i.dim() >= 1, "index must be (..., top)")
+        i = _integers(i, "index")
+        i = i.reshape(i.shape[:-1].numel(), i.shape[-1]).contiguous()
+    if m is not None:
+        ext._check(m.shape == index.shape[:-1], "mask must have the shape of index's tokens")
+        m = m.reshape(-1).contiguous()
     ext._check_order(i, num_experts, m)
     position, counts, offsets = ext._order(i, num_experts, m)
     return ExpertOrder(position if index.dim() == 2 else position.reshape(index.shape), counts, offsets)
-
-
-def _position(order: ExpertOrder) -> torch.Tensor:
-    p = order.position
-    if p.dim() != 2:
-        p = p.reshape(p.shape[:-1].numel(), p.shape[-1])
-    return p.contiguous()
 
 
 class _Dispatch(torch.autograd.Function):
@@ -151,11 +167,10 @@ class _Dispatch(torch.autograd.Function):
         ctx.save_for_backward(position)
         return ext._dispatch(x, position)
 
-    @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, grad):
         (position,) = ctx.saved_tensors
-        return ext._combine(_rows(grad), None, position), None
+        return ext._combine(_flat(grad), None, position), None
 
 
 def expert_dispatch(input: torch.Tensor, order: ExpertOrder) -> torch.Tensor:
@@ -167,11 +182,11 @@ def expert_dispatch(input: torch.Tensor, order: ExpertOrder) -> torch.Tensor:
     order was made of.  The gradient reaches input: a token's is the sum of its
     rows', in the order of its choices.  At most 2^24 columns.
     """
-    ext._check(input.dim() >= 1 and tuple(input.shape[:-1]) == tuple(order.position.shape[:-1]),
+    ext._check(input.dim() >= 1 and input.shape[:-1] == order.position.shape[:-1],
                "input must be (..., D) with the tokens of order")
-    x, position = _rows(input), _position(order)
+    x, position = _flat(input), _flat(order.position)
     ext._check_dispatch(x, position)
-    if torch.is_grad_enabled() and input.requires_grad:
+    if input.requires_grad and torch.is_grad_enabled():
         return _Dispatch.apply(x, position)
     return ext._dispatch(x, position)
 
@@ -182,11 +197,12 @@ class _Combine(torch.autograd.Function):
         ctx.save_for_backward(rows, weights, position)
         return ext._combine(rows, weights, position)
 
-    @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, grad):
         rows, weights, position = ctx.saved_tensors
-        return *ext._combine_bwd(_rows(grad), _rows(rows), weights, position, *ctx.needs_input_grad[:2]), None
+        need = ctx.needs_input_grad
+        d_rows, d_weights = ext._combine_bwd(_flat(grad), _flat(rows), weights, position, need[0], need[1])
+        return d_rows, d_weights, None
 
 
 def expert_combine(rows: torch.Tensor, weights: torch.Tensor, order: ExpertOrder) -> torch.Tensor:
@@ -200,13 +216,14 @@ def expert_combine(rows: torch.Tensor, weights: torch.Tensor, order: ExpertOrder
     reach rows and weights.  At most 2^24 columns.
     """
     ext._check(weights.shape == order.position.shape, "weights must have the shape of order's index")
-    if weights.dtype != rows.dtype and weights.dtype in ext._DTYPE_CODE:
-        weights = weights.float()
-    r, position = _rows(rows) if rows.dim() == 2 else rows, _position(order)
-    w = weights.reshape(position.shape).contiguous()
+    needs = rows.requires_grad or weights.requires_grad
+    w = weights
+    if w.dtype != rows.dtype and w.dtype in ext._DTYPE_CODE:
+        w = w.float()
+    r, w, position = _flat(rows) if rows.dim() == 2 else rows, _flat(w).contiguous(), _flat(order.position)
     ext._check_combine(r, w, position)
-    if torch.is_grad_enabled() and (rows.requires_grad or weights.requires_grad):
+    if needs and torch.is_grad_enabled():
         out = _Combine.apply(r, w, position)
     else:
         out = ext._combine(r, w, position)
-    return out if weights.dim() == 2 else out.reshape(*weights.shape[:-1], rows.shape[1])
+    return out if weights.dim() == 2 else out.reshape(*weights.shape[:-1], r.shape[1])

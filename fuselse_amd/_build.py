@@ -8,6 +8,9 @@
 * ``fuselse_amd/libfuselse_amd_diag.so``: the measurement kernels under
   ``fuselse_amd/csrc/diag`` (``include/fuselse_amd_diag.h``), linked against
   the first library, whose status and error functions it uses.
+* ``fuselse_amd/_layers.so``: the layers' common calls over torch's C++ API
+  (``fuselse_amd/csrc/torch``), compiled with the host compiler against the
+  headers of the torch that imports it and linked against the first library.
 """
 
 from __future__ import annotations
@@ -25,6 +28,8 @@ OBJ_DIR = os.path.join(PKG_DIR, "_obj")
 LIB_PATH = os.path.join(PKG_DIR, "libfuselse_amd.so")
 DIAG_DIR = os.path.join(CSRC, "diag")
 DIAG_LIB_PATH = os.path.join(PKG_DIR, "libfuselse_amd_diag.so")
+TORCH_DIR = os.path.join(CSRC, "torch")
+LAYERS_PATH = os.path.join(PKG_DIR, "_layers.so")
 ARCH = os.environ.get("FUSELSE_AMD_ARCH", "gfx950")
 
 COMMON_FLAGS = [
@@ -73,6 +78,42 @@ def _compile(src: str, verbose: bool) -> str:
     return obj
 
 
+def _compile_torch(src: str, verbose: bool) -> str:
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    obj = os.path.join(OBJ_DIR, "torch_" + os.path.basename(src) + ".o")
+    include = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"], "/opt/rocm/include"]
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-Wall", "-D__HIP_PLATFORM_AMD__",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *(f for d in include for f in ("-isystem", d)), "-c", src, "-o", obj]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for {src}:\n" + r.stdout + r.stderr)
+    if verbose and r.stderr:
+        print(r.stderr, file=sys.stderr)
+    return obj
+
+
+def _link_torch(objs, verbose: bool) -> None:
+    import torch
+
+    lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    tmp = LAYERS_PATH + ".tmp"
+    cmd = ["g++", "-shared", "-fPIC", *objs, f"-L{PKG_DIR}", "-lfuselse_amd", "-Wl,-rpath,$ORIGIN", f"-L{lib}",
+           "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip", "-ltorch_python", "-ltorch", "-o", tmp]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError("link failed:\n" + r.stdout + r.stderr)
+    os.replace(tmp, LAYERS_PATH)
+
+
 def _link(objs, out_path, extra, verbose):
     tmp = out_path + ".tmp"
     cmd = [_hipcc(), f"--offload-arch={ARCH}", "-shared", "-fPIC", *objs, *extra, "-o", tmp]
@@ -85,15 +126,19 @@ def _link(objs, out_path, extra, verbose):
 
 
 def build(verbose: bool = False, jobs: int = 8) -> str:
-    """Compile every source, link libfuselse_amd.so and libfuselse_amd_diag.so;
-    returns the first library's path."""
+    """Compile every source, link libfuselse_amd.so, libfuselse_amd_diag.so and
+    _layers.so; returns the first library's path."""
     os.makedirs(OBJ_DIR, exist_ok=True)
     srcs = sources()
     diag_srcs = sources(DIAG_DIR)
-    with cf.ThreadPoolExecutor(max_workers=max(1, min(jobs, len(srcs) + len(diag_srcs)))) as ex:
+    torch_srcs = sources(TORCH_DIR)
+    with cf.ThreadPoolExecutor(max_workers=max(1, min(jobs, len(srcs) + len(diag_srcs) + len(torch_srcs)))) as ex:
+        torch_objs = [ex.submit(_compile_torch, s, verbose) for s in torch_srcs]
         objs = list(ex.map(lambda s: _compile(s, verbose), srcs + diag_srcs))
+        torch_objs = [f.result() for f in torch_objs]
     _link(objs[:len(srcs)], LIB_PATH, [], verbose)
     _link(objs[len(srcs):], DIAG_LIB_PATH, [f"-L{PKG_DIR}", "-lfuselse_amd", "-Wl,-rpath,$ORIGIN"], verbose)
+    _link_torch(torch_objs, verbose)
     return LIB_PATH
 
 

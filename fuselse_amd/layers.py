@@ -8,6 +8,10 @@ holds no state: its workspace comes from torch's allocator on the current
 stream, so calls may run on several streams and be captured into graphs.
 Sums are fp32 and results are rounded once, to the input's type, in autocast
 regions too.
+
+A call on contiguous tensors of the current device that need no conversion is
+made by compiled code (``_layers.so``), autograd and all, since the host's part
+is most of a small call; what follows here is every other call, and what refuses.
 """
 
 from __future__ import annotations
@@ -17,8 +21,24 @@ from typing import NamedTuple, Optional
 import torch
 from torch.autograd.function import once_differentiable
 
-from . import ext
+from . import _lib, ext
 from .losses import _integers, _rows
+
+_common = None
+
+
+def _bind():
+    """The compiled calls, which need the library and torch loaded first."""
+    global _common
+    _lib.load()
+    try:
+        from . import _layers
+    except ImportError as e:
+        raise _lib.NativeLibraryMissing(
+            f"fuselse_amd: cannot load fuselse_amd/_layers.so ({e}); run "
+            "`python -c 'import __graft_entry__ as g; g.build()'`") from e
+    _common = _layers
+    return _layers
 
 
 def _once(backward):
@@ -63,16 +83,17 @@ def embedding(index: torch.Tensor, weight: torch.Tensor, scale: float = 1.0,
     from the end) give none.  At most 2^30 tokens and vocabulary entries and
     2^20 columns.
     """
-    i = index
-    if i.dtype != torch.int64 or i.dim() != 1 or not i.is_contiguous():
-        i = _integers(i, "index").reshape(-1).contiguous()
-    w = _flat(weight) if weight.dim() == 2 else weight
-    ext._check_embedding(w, i)
     padding = -1
     if padding_idx is not None:
-        V = w.shape[0]
+        V = weight.shape[0] if weight.dim() else 0
         ext._check(-V <= padding_idx < V, "padding_idx must be within the rows of weight")
         padding = padding_idx % V
+    out = (_common or _bind()).embedding(index, weight, scale, padding)
+    if out is not None:
+        return out
+    i = _integers(index, "index").reshape(-1).contiguous()
+    w = _flat(weight) if weight.dim() == 2 else weight
+    ext._check_embedding(w, i)
     if weight.requires_grad and torch.is_grad_enabled():
         out = _Embedding.apply(w, i, scale, padding)
     else:
@@ -110,6 +131,9 @@ def layer_norm(input: torch.Tensor, weight: Optional[torch.Tensor] = None, bias:
     overflow.  Gradients reach all three.  At most 2^31 - 1 rows and 2^24
     columns.
     """
+    out = (_common or _bind()).layer_norm(input, weight, bias, eps)
+    if out is not None:
+        return out
     ext._check(input.dim() >= 1, "input must have a last dimension")
     x = _flat(input)
     needs = input.requires_grad
@@ -148,11 +172,12 @@ def expert_order(index: torch.Tensor, num_experts: int, mask: Optional[torch.Ten
     takes.  At most 1024 experts, 1024 choices a token, 2^30 tokens and 2^31 - 1
     choices.
     """
-    i, m = index, mask
-    if i.dtype != torch.int64 or i.dim() != 2 or not i.is_contiguous():
-        ext._check(i.dim() >= 1, "index must be (..., top)")
-        i = _integers(i, "index")
-        i = i.reshape(i.shape[:-1].numel(), i.shape[-1]).contiguous()
+    out = (_common or _bind()).expert_order(index, num_experts, mask)
+    if out is not None:
+        return ExpertOrder._make(out)
+    ext._check(index.dim() >= 1, "index must be (..., top)")
+    i, m = _integers(index, "index"), mask
+    i = i.reshape(i.shape[:-1].numel(), i.shape[-1]).contiguous()
     if m is not None:
         ext._check(m.shape == index.shape[:-1], "mask must have the shape of index's tokens")
         m = m.reshape(-1).contiguous()
@@ -182,6 +207,9 @@ def expert_dispatch(input: torch.Tensor, order: ExpertOrder) -> torch.Tensor:
     order was made of.  The gradient reaches input: a token's is the sum of its
     rows', in the order of its choices.  At most 2^24 columns.
     """
+    out = (_common or _bind()).expert_dispatch(input, order.position)
+    if out is not None:
+        return out
     ext._check(input.dim() >= 1 and input.shape[:-1] == order.position.shape[:-1],
                "input must be (..., D) with the tokens of order")
     x, position = _flat(input), _flat(order.position)
@@ -215,6 +243,9 @@ def expert_combine(rows: torch.Tensor, weights: torch.Tensor, order: ExpertOrder
     are not read and may hold anything, and their gradients are 0.  Gradients
     reach rows and weights.  At most 2^24 columns.
     """
+    out = (_common or _bind()).expert_combine(rows, weights, order.position)
+    if out is not None:
+        return out
     ext._check(weights.shape == order.position.shape, "weights must have the shape of order's index")
     needs = rows.requires_grad or weights.requires_grad
     w = weights

@@ -219,11 +219,13 @@ __device__ __forceinline__ void sum_run(const GradArgs& p, int64_t run, int step
     float acc[VE] = {};
     bool head = id_of(0) == ahead;  // the piece began before
     for (int i0 = 0; i0 < m; i0 += kAhead) {
+        if (id_of(i0) >= p.V) return;
+        // loads without conditions, all in flight: entries that are not there have row 0
         u32x4 raw[kAhead];
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
             const uint32_t at = (uint32_t)__builtin_amdgcn_readlane((int)mine.at, i0 + u);
-            if (id_of(i0 + u) < p.V && live) raw[u] = row_load<true>(static_cast<const T*>(p.g) + at * p.ldg, p.D, v);
+            raw[u] = row_load<true>(static_cast<const T*>(p.g) + at * p.ldg, p.D, live ? v : 0);
         }
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
@@ -293,33 +295,26 @@ __global__ __launch_bounds__(kThreads) void join_kernel(GradArgs p) {
         }
         const bool live = v < row_vectors<T>(p.D);
         const int64_t at = live && p.D >= VE ? row_vec_at<T>(p.D, v) : 0;
-        const int n = p.D >= VE ? VE : (int)p.D;
         float acc[VE] = {};
         for (int64_t k0 = wave; k0 < pieces; k0 += WAVES * kPieces) {
+            // loads at places that are there in any case, all in flight; what is too much
+            // is not added
             float f[kPieces][VE];
 #pragma unroll
             for (int u = 0; u < kPieces; ++u) {
-                const int64_t k = k0 + u * WAVES;
+                const int64_t k = k0 + u * WAVES < pieces ? k0 + u * WAVES : pieces - 1;
                 const float* from = p.part + ((run + k) * 2 + (k == 0 ? 1 : 0)) * p.D + at;
-                const bool on = live && k < pieces;
+                if (p.D >= VE) {
+                    __builtin_memcpy(f[u], from, 4 * VE);
+                } else {
 #pragma unroll
-                for (int j = 0; j < VE; j += 4) {
-                    f32x4 q{0, 0, 0, 0};
-                    if (on && n == VE) {
-                        __builtin_memcpy(&q, from + j, 16);
-                    } else if (on) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if (j + i < n) q[i] = from[j + i];
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) f[u][j + i] = q[i];
+                    for (int j = 0; j < VE; ++j) f[u][j] = j < p.D ? from[j] : 0.0f;
                 }
             }
 #pragma unroll
             for (int u = 0; u < kPieces; ++u)
 #pragma unroll
-                for (int j = 0; j < VE; ++j) acc[j] += f[u][j];
+                for (int j = 0; j < VE; ++j) acc[j] += k0 + u * WAVES < pieces ? f[u][j] : 0.0f;
         }
         __syncthreads();  // the item before is done with sh
 #pragma unroll
@@ -373,7 +368,7 @@ int64_t align256(int64_t v) { return (v + 255) & ~(int64_t)255; }
 
 // Entries of a run: as many as a wave has loads in flight, or 64, which leave fewer
 // pieces to join, where that many waves keep the memory busy: (65536, 2048), all of
-// one token, 137 us for 253, but (32768, 1024) 90 for 69.
+// one token, 136 us for 266, (65536, 4096) 201 for 226, but (32768, 1024) 90 for 69.
 int run_of(int64_t n, int64_t D) { return n * D >= (1 << 26) ? 64 : kAhead; }
 int64_t runs_of(int64_t n, int64_t D) { return (n + run_of(n, D) - 1) / run_of(n, D); }
 

@@ -159,7 +159,8 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const auto saved = ctx->get_saved_variables();
-        const Tensor g = grads[0].contiguous(), x = saved[0].contiguous(), w = saved[1], st = saved[2];
+        const Tensor g = grads[0].contiguous(), x = saved[0].contiguous(), st = saved[2].contiguous();
+        const Tensor w = saved[1].defined() ? saved[1].contiguous() : saved[1];
         const c10::DeviceGuard guard(g.device());
         const int64_t N = lead(x), D = last(x);
         const auto type = (at::ScalarType)ctx->saved_data["type"].toInt();

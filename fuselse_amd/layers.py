@@ -67,7 +67,7 @@ class _Embedding(torch.autograd.Function):
     @_once
     def backward(ctx, grad):
         (index,) = ctx.saved_tensors
-        return ext._embedding_bwd(_flat(grad), index, *ctx.args), None, None, None
+        return ext._embedding_bwd(_flat(grad), index.contiguous(), *ctx.args), None, None, None
 
 
 def embedding(index: torch.Tensor, weight: torch.Tensor, scale: float = 1.0,
@@ -114,8 +114,9 @@ class _LayerNorm(torch.autograd.Function):
     def backward(ctx, grad):
         x, weight, stats = ctx.saved_tensors
         need = ctx.needs_input_grad
-        # in rows again, which a saved-tensor hook may have changed
-        dx, dw, db = ext._norm_bwd(_flat(grad), _flat(x), weight, ctx.params_dtype, stats, need[0], need[1], need[2])
+        # as they were saved, which a saved-tensor hook may have changed
+        weight = weight.contiguous() if weight is not None else None
+        dx, dw, db = ext._norm_bwd(_flat(grad), _flat(x), weight, ctx.params_dtype, stats.contiguous(), *need[:3])
         return dx, dw, db, None
 
 
@@ -195,7 +196,7 @@ class _Dispatch(torch.autograd.Function):
     @_once
     def backward(ctx, grad):
         (position,) = ctx.saved_tensors
-        return ext._combine(_flat(grad), None, position), None
+        return ext._combine(_flat(grad), None, position.contiguous()), None
 
 
 def expert_dispatch(input: torch.Tensor, order: ExpertOrder) -> torch.Tensor:
@@ -229,7 +230,8 @@ class _Combine(torch.autograd.Function):
     def backward(ctx, grad):
         rows, weights, position = ctx.saved_tensors
         need = ctx.needs_input_grad
-        d_rows, d_weights = ext._combine_bwd(_flat(grad), _flat(rows), weights, position, need[0], need[1])
+        d_rows, d_weights = ext._combine_bwd(_flat(grad), _flat(rows), weights.contiguous(), position.contiguous(),
+                                             need[0], need[1])
         return d_rows, d_weights, None
 
 

@@ -440,7 +440,9 @@ extern "C" int fl_embedding_bwd(const void* grad, int64_t grad_stride, const int
              (unsigned long long)workspace_bytes, (long long)w.bytes);
     FL_CHECK((workspace && (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0),
              "%s: workspace is not 256-byte aligned", name);
-    if ((N + kAhead - 1) / kAhead * row_steps(vectors(D, dtype)) > max_grid_blocks(kThreads))
+    const int steps = row_steps(vectors(D, dtype));
+    const int64_t sums = (runs_of(N, D) * steps + kThreads / 64 - 1) / (kThreads / 64);
+    if (sums > max_grid_blocks(kThreads))
         return set_error(FL_ERANGE, "%s: N=%lld, V=%lld, D=%lld are too many for a launch", name, (long long)N,
                          (long long)V, (long long)D);
     char* ws = static_cast<char*>(workspace);
@@ -503,11 +505,10 @@ extern "C" int fl_embedding_bwd(const void* grad, int64_t grad_stride, const int
     a.part = reinterpret_cast<float*>(ws + w.part);
     a.run = run_of(N, D);
     a.runs = runs_of(N, D);
-    a.steps = row_steps(vectors(D, dtype));
+    a.steps = steps;
     a.joins = joins;
     a.list = reinterpret_cast<int*>(ws + w.list);
     if (N == 0) return launch_status(name);
-    const int64_t sums = (a.runs * a.steps + kThreads / 64 - 1) / (kThreads / 64);
     const int64_t most = (a.runs - 1) * a.steps;
     const unsigned blocks = (unsigned)(most < kJoinBlocks ? most : kJoinBlocks);
     by_type(dtype, [&](auto t) {

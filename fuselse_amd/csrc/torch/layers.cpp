@@ -52,11 +52,14 @@ void* mut(const Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr
 bool plain(PyObject* o, Tensor& t) {
     if (!THPVariable_CheckExact(o)) return false;
     t = THPVariable_Unpack(o);
-    return t.is_cuda() && t.layout() == at::kStrided && t.is_contiguous() && t.numel() > 0 &&
+    return t.is_cuda() && t.layout() == at::kStrided && !t.is_neg() && t.is_contiguous() && t.numel() > 0 &&
            t.device().index() == c10::hip::current_device();
 }
 bool floating(PyObject* o, Tensor& t) { return plain(o, t) && t.dim() >= 1 && code_of(t) >= 0; }
 bool absent(PyObject* o) { return o == Py_None; }
+
+// A gradient as the kernels read it.
+Tensor in_memory(const Tensor& g) { return g.resolve_neg().contiguous(); }
 
 // Size of t's leading dimensions, its last, and whether both have these leading ones.
 int64_t last(const Tensor& t) { return t.size(-1); }
@@ -105,7 +108,7 @@ struct Embedding : torch::autograd::Function<Embedding> {
         return embedding_fwd(weight, index, scale);
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
-        const Tensor index = ctx->get_saved_variables()[0].contiguous(), g = grads[0].contiguous();
+        const Tensor index = ctx->get_saved_variables()[0].contiguous(), g = in_memory(grads[0]);
         const c10::DeviceGuard guard(g.device());
         const int64_t V = ctx->saved_data["rows"].toInt(), D = last(g), N = index.numel();
         Tensor dw = make(g, {V, D});
@@ -159,7 +162,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const auto saved = ctx->get_saved_variables();
-        const Tensor g = grads[0].contiguous(), x = saved[0].contiguous(), st = saved[2].contiguous();
+        const Tensor g = in_memory(grads[0]), x = saved[0].contiguous(), st = saved[2].contiguous();
         const Tensor w = saved[1].defined() ? saved[1].contiguous() : saved[1];
         const c10::DeviceGuard guard(g.device());
         const int64_t N = lead(x), D = last(x);
@@ -256,7 +259,7 @@ struct Dispatch : torch::autograd::Function<Dispatch> {
         return dispatch(x, position);
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
-        const Tensor position = ctx->get_saved_variables()[0].contiguous(), g = grads[0].contiguous();
+        const Tensor position = ctx->get_saved_variables()[0].contiguous(), g = in_memory(grads[0]);
         const c10::DeviceGuard guard(g.device());
         return once({combine(g, Tensor(), position), Tensor()}, grads);
     }
@@ -269,7 +272,7 @@ struct Combine : torch::autograd::Function<Combine> {
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const auto saved = ctx->get_saved_variables();
-        const Tensor g = grads[0].contiguous(), rows = saved[0].contiguous(), weights = saved[1].contiguous();
+        const Tensor g = in_memory(grads[0]), rows = saved[0].contiguous(), weights = saved[1].contiguous();
         const Tensor position = saved[2].contiguous();
         const c10::DeviceGuard guard(g.device());
         const int64_t T = lead(position), K = last(position), D = rows.size(1);

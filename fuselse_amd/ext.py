@@ -1410,8 +1410,8 @@ def _check_combine(rows, weights, position):
 
 def expert_combine(rows: torch.Tensor, weights: Optional[torch.Tensor], position: torch.Tensor) -> torch.Tensor:
     """(tokens, D), each token's sum of its entries' rows times their weights
-    (None: 1, the gradient of expert_dispatch).  Dropped entries give nothing and
-    what belongs to them is not read."""
+    (None: 1, the gradient of expert_dispatch).  Dropped entries give nothing,
+    whatever their rows and weights hold."""
     _check_combine(rows, weights, position)
     return _combine(rows, weights, position)
 

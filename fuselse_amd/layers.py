@@ -54,6 +54,7 @@ def _once(backward):
 
 def _flat(t: torch.Tensor) -> torch.Tensor:
     """t in rows, as the kernels take them."""
+    t = t.resolve_neg()
     return t if t.dim() == 2 and t.is_contiguous() else _rows(t)
 
 
@@ -142,7 +143,7 @@ def layer_norm(input: torch.Tensor, weight: Optional[torch.Tensor] = None, bias:
         needs = needs or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)
         if any(t is not None and t.dtype != x.dtype for t in (weight, bias)):
             weight, bias = (t.float() if t is not None and t.dtype in ext._DTYPE_CODE else t for t in (weight, bias))
-        weight, bias = (t.contiguous() if t is not None else None for t in (weight, bias))
+        weight, bias = (t.resolve_neg().contiguous() if t is not None else None for t in (weight, bias))
     ext._check_norm(x, weight, bias)
     if needs and torch.is_grad_enabled():
         y = _LayerNorm.apply(x, weight, bias, eps)
@@ -242,7 +243,7 @@ def expert_combine(rows: torch.Tensor, weights: torch.Tensor, order: ExpertOrder
     rows (entries, D) in fp32, fp16 or bf16, in the order that expert_dispatch
     gives; weights (..., top), order's index's shape, taken in fp32 where they
     are not of rows' type.  Dropped entries give nothing: their rows and weights
-    are not read and may hold anything, and their gradients are 0.  Gradients
+    may hold anything, and their gradients are 0.  Gradients
     reach rows and weights.  At most 2^24 columns.
     """
     out = (_common or _bind()).expert_combine(rows, weights, order.position)

@@ -519,8 +519,8 @@ int fl_layer_norm_bwd(const void* grad, int64_t grad_stride, const void* x, int6
  * fl_expert_combine: out[t] = sum_k weights[t, k] * rows[position[t, k]] over the
  *   entries that are not dropped, rows row_stride apart, out [tokens, D]
  *   contiguous; weights [tokens, top] contiguous of weights_dtype (0 or dtype),
- *   or NULL: 1 (the gradient of a dispatch).  What belongs to a dropped entry is
- *   not read.
+ *   or NULL: 1 (the gradient of a dispatch).  A dropped entry's row is not read,
+ *   its weight may hold anything.
  * fl_expert_combine_bwd: grad [tokens, D] of out; grad_rows [tokens * top, D]
  *   contiguous (0 where dropped) and grad_weights [tokens, top] of
  *   weights_dtype (0 where dropped); either may be NULL.

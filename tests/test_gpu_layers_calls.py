@@ -451,3 +451,21 @@ def test_gradients_against_differences(cuda):
         size = (y.detach().abs().double() * up.abs().double()).sum() * E23 / step
         size = size + 2.0 ** -9 * (g.abs().double() * way.abs().double()).sum()
         assert abs(float(change - (g.double() * way.double()).sum())) <= float(size), name
+
+
+def test_tensors_that_are_negated_lazily(cuda):
+    """A view whose memory holds the negated values (the imaginary part of a
+    conjugate) is taken for what it stands for."""
+    d = 24
+    view = torch.complex(randn(cuda, 6, d), randn(cuda, 6, d, seed=1)).conj().imag
+    assert view.is_neg()
+    x = view.clone()
+    order = fuselse_amd.expert_order(randint(cuda, 3, 6, 2), 3)
+    w = torch.rand(6, 2, device=cuda)
+    ids = randint(cuda, 6, 5)
+    assert torch.equal(fuselse_amd.layer_norm(view), fuselse_amd.layer_norm(x))
+    assert torch.equal(fuselse_amd.embedding(ids, view), fuselse_amd.embedding(ids, x))
+    assert torch.equal(fuselse_amd.expert_dispatch(view, order), fuselse_amd.expert_dispatch(x, order))
+    rows = torch.cat([x, x]).requires_grad_(True)
+    y = fuselse_amd.expert_combine(rows, w, order)
+    assert torch.equal(torch.autograd.grad(y, rows, view, retain_graph=True)[0], torch.autograd.grad(y, rows, x)[0])

@@ -35,7 +35,10 @@ struct LookupArgs {
     bool through;  // a wave an item, rows of out whole, aligned vectors
 };
 
-template <typename T>
+// Lanes share a token's row, or a wave takes U times 64 vectors of it: a row's loads
+// wait for its index, and two of them in flight a lane take (65536, 4096) in bf16 from
+// 174 to 141 us (5.8 TB/s), four to 137 to 164 by the tokens' order.
+template <typename T, int U>
 __global__ __launch_bounds__(kThreads) void lookup_kernel(LookupArgs p) {
     constexpr int VE = Elem<T>::kVec;
     const int nvec = row_vectors<T>(p.D);
@@ -43,20 +46,28 @@ __global__ __launch_bounds__(kThreads) void lookup_kernel(LookupArgs p) {
     for (int64_t it = (int64_t)blockIdx.x * per + (int)threadIdx.x / p.lanes; it < p.items;
          it += (int64_t)gridDim.x * per) {
         const int64_t i = p.steps == 1 ? it : it / p.steps;
-        const int v = (int)(it - i * p.steps) * 64 + sub;
-        if (v >= nvec) continue;
+        const int v = (int)(it - i * p.steps) * 64 * U + sub;
         const int64_t id = p.index[i];
         const bool inside = id >= 0 && id < p.V;
-        u32x4 r = row_load(static_cast<const T*>(p.w) + (inside ? id : 0) * p.ldw, p.D, v);
-        if (!inside || p.scale != 1.0f) {
-            float f[VE];
-            Elem<T>::cvt(r, f);
+        const T* row = static_cast<const T*>(p.w) + (inside ? id : 0) * p.ldw;
+        T* out = static_cast<T*>(p.out) + i * p.D;
+        u32x4 r[U];
 #pragma unroll
-            for (int k = 0; k < VE; ++k) f[k] = inside ? f[k] * p.scale : __builtin_nanf("");
-            r = pack_vec<T>(f);
+        for (int u = 0; u < U; ++u)
+            if (v + 64 * u < nvec) r[u] = row_load(row, p.D, v + 64 * u);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (v + 64 * u >= nvec) continue;
+            if (!inside || p.scale != 1.0f) {
+                float f[VE];
+                Elem<T>::cvt(r[u], f);
+#pragma unroll
+                for (int k = 0; k < VE; ++k) f[k] = inside ? f[k] * p.scale : __builtin_nanf("");
+                r[u] = pack_vec<T>(f);
+            }
+            if (p.through) row_store_through(out, p.D, v + 64 * u, r[u]);
+            else row_store(out, p.D, v + 64 * u, r[u]);
         }
-        if (p.through) row_store_through(static_cast<T*>(p.out) + i * p.D, p.D, v, r);
-        else row_store(static_cast<T*>(p.out) + i * p.D, p.D, v, r);
     }
 }
 
@@ -410,13 +421,16 @@ extern "C" int fl_embedding_fwd(const void* weight, int64_t row_stride, int64_t 
     const int nvec = vectors(D, dtype);
     a.lanes = row_lanes(nvec);
     a.steps = row_steps(nvec);
+    const bool more = a.steps > 1 && N * a.steps >= 1024;  // fewer waves would not fill the chip
+    if (more) a.steps = (a.steps + 1) / 2;
     a.items = N * a.steps;
     a.through = a.lanes == 64 && D % (dtype == 0 ? 4 : 8) == 0 && (reinterpret_cast<uintptr_t>(out) & 15u) == 0;
     const int per = kThreads / a.lanes;
     const int64_t want = (a.items + per - 1) / per;
     const unsigned blocks = (unsigned)(want < (1 << 22) ? want : (1 << 22));
     by_type(dtype, [&](auto t) {
-        lookup_kernel<decltype(t)><<<blocks, kThreads, 0, static_cast<hipStream_t>(stream)>>>(a);
+        if (more) lookup_kernel<decltype(t), 2><<<blocks, kThreads, 0, static_cast<hipStream_t>(stream)>>>(a);
+        else lookup_kernel<decltype(t), 1><<<blocks, kThreads, 0, static_cast<hipStream_t>(stream)>>>(a);
     });
     return launch_status(name);
 }

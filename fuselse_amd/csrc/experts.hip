@@ -136,11 +136,12 @@ __device__ __forceinline__ int64_t item_stride(const RowArgs& p) {
 
 constexpr int kAhead = 8;  // rows whose loads are in flight
 
-// Places of the token's entries k0 .. k0 + 7; INT_MAX, outside all rows, past
+// Places of the token's entries k0, k0 + 1, ..; INT_MAX, outside all rows, past
 // the last.
-__device__ __forceinline__ void load_places(const RowArgs& p, int64_t t, int k0, int (&at)[kAhead]) {
+template <int A>
+__device__ __forceinline__ void load_places(const RowArgs& p, int64_t t, int k0, int (&at)[A]) {
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) at[u] = k0 + u < p.top ? p.position[t * p.top + k0 + u] : 0x7FFFFFFF;
+    for (int u = 0; u < A; ++u) at[u] = k0 + u < p.top ? p.position[t * p.top + k0 + u] : 0x7FFFFFFF;
 }
 
 // x is read with plain loads, since what made it has often left it in the caches
@@ -173,40 +174,48 @@ __global__ __launch_bounds__(kThreads) void dispatch_kernel(RowArgs p) {
 }
 
 // The experts' rows are read once, with the nontemporal hint: (131072, 512) in
-// bf16 from 8 experts each 200 us (6.0 TB/s), without it 217.  More vectors a
-// lane with fewer rows in flight take longer (two of four rows 205, four of two
-// 240).
-template <typename T, bool WAVE>
+// bf16 from 8 experts each 200 us (6.0 TB/s), without it 217.  A wave takes A rows'
+// loads and U times 64 vectors of them together: eight rows of one, or, where rows
+// are longer than that, up to four of two ((60000, 4096) from one expert each 225 us
+// with one vector a lane, 156 with two; (60000, 999) from 5 141 and 130).
+template <typename T, bool WAVE, int A, int U>
 __global__ __launch_bounds__(kThreads) void combine_kernel(RowArgs p) {
     constexpr int VE = Elem<T>::kVec;
     const int nvec = row_vectors<T>(p.D);
     int sub;
     for (int64_t it = first_item<WAVE>(p, sub); it < p.items; it += item_stride<WAVE>(p)) {
         const int64_t t = p.steps == 1 ? it : it / p.steps;
-        const int v = (int)(it - t * p.steps) * 64 + sub;
+        const int v = (int)(it - t * p.steps) * 64 * U + sub;
         if (v >= nvec) continue;
-        float acc[VE] = {};
-        for (int k0 = 0; k0 < p.top; k0 += kAhead) {
-            int at[kAhead];
-            u32x4 raw[kAhead];
-            float w[kAhead];
+        float acc[U][VE] = {};
+        for (int k0 = 0; k0 < p.top; k0 += A) {
+            int at[A];
+            u32x4 raw[A][U];
+            float w[A];
             load_places(p, t, k0, at);
 #pragma unroll
-            for (int u = 0; u < kAhead; ++u) w[u] = k0 + u < p.top ? weight_of<T>(p, t * p.top + k0 + u) : 0.0f;
+            for (int u = 0; u < A; ++u) w[u] = k0 + u < p.top ? weight_of<T>(p, t * p.top + k0 + u) : 0.0f;
 #pragma unroll
-            for (int u = 0; u < kAhead; ++u)
+            for (int u = 0; u < A; ++u)
                 if (at[u] >= 0 && at[u] < p.n)
-                    raw[u] = row_load<true>(static_cast<const T*>(p.in) + at[u] * p.ldi, p.D, v);
 #pragma unroll
-            for (int u = 0; u < kAhead; ++u)
-                if (at[u] >= 0 && at[u] < p.n) {
-                    float r[VE];
-                    Elem<T>::cvt(raw[u], r);
+                    for (int j = 0; j < U; ++j)
+                        raw[u][j] = row_load<true>(static_cast<const T*>(p.in) + at[u] * p.ldi, p.D,
+                                                   v + 64 * j < nvec ? v + 64 * j : v);
 #pragma unroll
-                    for (int k = 0; k < VE; ++k) acc[k] = __builtin_fmaf(w[u], r[k], acc[k]);
-                }
+            for (int u = 0; u < A; ++u)
+                if (at[u] >= 0 && at[u] < p.n)
+#pragma unroll
+                    for (int j = 0; j < U; ++j) {
+                        float r[VE];
+                        Elem<T>::cvt(raw[u][j], r);
+#pragma unroll
+                        for (int k = 0; k < VE; ++k) acc[j][k] = __builtin_fmaf(w[u], r[k], acc[j][k]);
+                    }
         }
-        row_store(static_cast<T*>(p.out) + t * p.D, p.D, v, pack_vec<T>(acc));
+#pragma unroll
+        for (int j = 0; j < U; ++j)
+            if (v + 64 * j < nvec) row_store(static_cast<T*>(p.out) + t * p.D, p.D, v + 64 * j, pack_vec<T>(acc[j]));
     }
 }
 
@@ -467,11 +476,20 @@ extern "C" int fl_expert_combine(const void* rows, int64_t row_stride, int64_t t
     a.weights_f32 = weights_dtype == 0;
     a.out = out;
     split_rows(a, dtype);
+    const bool two = a.steps > 1 && a.items >= 1024;  // fewer waves would not fill the chip
+    if (two) {
+        a.steps = (a.steps + 1) / 2;
+        a.items = tokens * a.steps;
+    }
     hipStream_t s = static_cast<hipStream_t>(stream);
     by_type(dtype, [&](auto t) {
+        using T = decltype(t);
         const unsigned grid = grid_of(a.items, kThreads / a.lanes);
-        if (a.lanes == 64) combine_kernel<decltype(t), true><<<grid, kThreads, 0, s>>>(a);
-        else combine_kernel<decltype(t), false><<<grid, kThreads, 0, s>>>(a);
+        if (a.lanes < 64) combine_kernel<T, false, 8, 1><<<grid, kThreads, 0, s>>>(a);
+        else if (!two) combine_kernel<T, true, 8, 1><<<grid, kThreads, 0, s>>>(a);
+        else if (top == 1) combine_kernel<T, true, 1, 2><<<grid, kThreads, 0, s>>>(a);
+        else if (top == 2) combine_kernel<T, true, 2, 2><<<grid, kThreads, 0, s>>>(a);
+        else combine_kernel<T, true, 4, 2><<<grid, kThreads, 0, s>>>(a);
     });
     return launch_status(name);
 }

@@ -423,7 +423,7 @@ def check_rows(t, k, e, d, dtype, wdtype, mask=None, index=None, view=lambda a: 
 
 ROWS = [(1, 1, 1, 1), (1, 8, 256, 2048), (3, 2, 4, 3), (7, 3, 5, 7), (5, 2, 3, 8), (33, 6, 8, 9), (8, 9, 16, 65),
         (100, 8, 64, 128), (64, 17, 24, 136), (20, 2, 8, 511), (20, 2, 8, 512), (31, 4, 8, 513), (9, 8, 16, 1100),
-        (512, 2, 8, 768), (3, 40, 64, 4104), (1000, 6, 60, 200)]
+        (512, 2, 8, 768), (3, 40, 64, 4104), (1000, 6, 60, 200), (600, 1, 4, 1030), (700, 2, 8, 1041), (520, 5, 8, 1544)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)

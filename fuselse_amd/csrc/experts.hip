@@ -246,9 +246,10 @@ __device__ __forceinline__ float sum_eight(const float (&v)[8], int lanes) {
 }
 __device__ __forceinline__ int eighth(int sub) { return 4 * (sub & 1) + (sub & 2) + ((sub >> 2) & 1); }
 
-// The gradient of a combination, a token by its lanes or by the block: dy is
-// read once for eight rows, whose loads are in flight together.
-template <typename T, int TEAM>  // 0: p.lanes, 1: a wave, 2: the block
+// The gradient of a combination, a token by its lanes or by the block: dy is read
+// once for A rows, and the loads of U vectors a lane of all of them are in flight
+// together, ahead of the stores, whose end a later load would wait for.
+template <typename T, int TEAM, int A, int U>  // TEAM 0: p.lanes, 1: a wave, 2: the block
 __global__ __launch_bounds__(kThreads) void combine_bwd_kernel(RowArgs p) {
     constexpr int VE = Elem<T>::kVec;
     constexpr bool BLOCK = TEAM == 2;
@@ -263,47 +264,61 @@ __global__ __launch_bounds__(kThreads) void combine_bwd_kernel(RowArgs p) {
     }
     for (; t < p.tokens; t += stride) {
         const T* dy = static_cast<const T*>(p.in) + t * p.ldi;
-        for (int k0 = 0; k0 < p.top; k0 += kAhead, turn ^= 1) {
+        for (int k0 = 0; k0 < p.top; k0 += A, turn ^= 1) {
             float dot[kAhead] = {};
-            int at[kAhead];
+            int at[A];
             load_places(p, t, k0, at);
-            for (int v = sub; v < nvec; v += team) {
-                u32x4 raw[kAhead];
-                const u32x4 gr = row_load(dy, p.D, v);
+            for (int v0 = sub; v0 < nvec; v0 += team * U) {
+                u32x4 raw[A][U], gr[U];
+#pragma unroll
+                for (int j = 0; j < U; ++j) {
+                    const int v = v0 + j * team;
+                    gr[j] = row_load(dy, p.D, v < nvec ? v : v0);
+                }
                 if (p.dweights)
 #pragma unroll
-                    for (int u = 0; u < kAhead; ++u)
+                    for (int u = 0; u < A; ++u)
                         if (at[u] >= 0 && at[u] < p.n)
-                            raw[u] = row_load<true>(static_cast<const T*>(p.rows) + at[u] * p.ldr, p.D, v);
-                float g[VE];
-                Elem<T>::cvt(gr, g);
-                if (p.out)
 #pragma unroll
-                    for (int u = 0; u < kAhead; ++u) {
-                        const int row = at[u] < 0 ? ~at[u] : at[u];
-                        if (row >= p.n) continue;
-                        u32x4 r{0, 0, 0, 0};
-                        if (at[u] >= 0) {
-                            const float w = weight_of<T>(p, t * p.top + k0 + u);
-                            float d[VE];
+                            for (int j = 0; j < U; ++j) {
+                                const int v = v0 + j * team;
+                                raw[u][j] = row_load<true>(static_cast<const T*>(p.rows) + at[u] * p.ldr, p.D,
+                                                           v < nvec ? v : v0);
+                            }
 #pragma unroll
-                            for (int k = 0; k < VE; ++k) d[k] = w * g[k];
-                            r = pack_vec<T>(d);
+                for (int j = 0; j < U; ++j) {
+                    const int v = v0 + j * team;
+                    if (v >= nvec) continue;
+                    float g[VE];
+                    Elem<T>::cvt(gr[j], g);
+                    if (p.out)
+#pragma unroll
+                        for (int u = 0; u < A; ++u) {
+                            const int row = at[u] < 0 ? ~at[u] : at[u];
+                            if (row >= p.n) continue;
+                            u32x4 r{0, 0, 0, 0};
+                            if (at[u] >= 0) {
+                                const float w = weight_of<T>(p, t * p.top + k0 + u);
+                                float d[VE];
+#pragma unroll
+                                for (int k = 0; k < VE; ++k) d[k] = w * g[k];
+                                r = pack_vec<T>(d);
+                            }
+                            row_store(static_cast<T*>(p.out) + row * p.D, p.D, v, r);
                         }
-                        row_store(static_cast<T*>(p.out) + row * p.D, p.D, v, r);
-                    }
-                if (!p.dweights) continue;
-                // elements that the vector before has too
-                const int skip = p.ragged && p.D >= VE ? (int)((int64_t)v * VE - row_vec_at<T>(p.D, v)) : 0;
+                    if (!p.dweights) continue;
+                    // elements that the vector before has too
+                    const int skip = p.ragged && p.D >= VE ? (int)((int64_t)v * VE - row_vec_at<T>(p.D, v)) : 0;
 #pragma unroll
-                for (int u = 0; u < kAhead; ++u)
-                    if (at[u] >= 0 && at[u] < p.n) {
-                        float r[VE];
-                        Elem<T>::cvt(raw[u], r);
+                    for (int u = 0; u < A; ++u)
+                        if (at[u] >= 0 && at[u] < p.n) {
+                            float r[VE];
+                            Elem<T>::cvt(raw[u][j], r);
 #pragma unroll
-                        for (int k = 0; k < VE; ++k)
-                            if (k >= skip) dot[u] = __builtin_fmaf(g[k], r[k], dot[u]);
-                    }
+                            for (int k = 0; k < VE; ++k)
+                                if (k >= skip) dot[u] = __builtin_fmaf(g[k], r[k], dot[u]);
+                        }
+                }
             }
             if (!p.dweights) continue;
             float s = sum_eight(dot, BLOCK ? 64 : team);
@@ -320,7 +335,7 @@ __global__ __launch_bounds__(kThreads) void combine_bwd_kernel(RowArgs p) {
                     for (int w = 1; w < kThreads / 64; ++w) s += sh[turn][w][u];
                 }
             }
-            if (mine && k0 + u < p.top) {
+            if (mine && u < A && k0 + u < p.top) {
                 const int64_t i = t * p.top + k0 + u;
                 if (p.weights_f32) static_cast<float*>(p.dweights)[i] = s;
                 else Elem<T>::put(static_cast<T*>(p.dweights) + i, s);
@@ -525,12 +540,23 @@ extern "C" int fl_expert_combine_bwd(const void* grad, int64_t grad_stride, cons
     split_rows(a, dtype);
     hipStream_t s = static_cast<hipStream_t>(stream);
     by_type(dtype, [&](auto t) {
-        // from 193 vectors on a block shares a token: (16383, 2048) in bf16 162 us for
-        // 186 by a wave, but (60000, 999) 338 for 312
-        if (a.steps > 3) combine_bwd_kernel<decltype(t), 2><<<grid_of(tokens, 1), kThreads, 0, s>>>(a);
-        else if (a.lanes == 64)
-            combine_bwd_kernel<decltype(t), 1><<<grid_of(tokens, kThreads / 64), kThreads, 0, s>>>(a);
-        else combine_bwd_kernel<decltype(t), 0><<<grid_of(tokens, kThreads / a.lanes), kThreads, 0, s>>>(a);
+        using T = decltype(t);
+        const unsigned by_wave = grid_of(tokens, kThreads / 64);
+        // Steps of a wave over a row.  With one or two rows a token a wave takes up to
+        // eight loads a lane of them in one step ((60000, 4096) from one expert each, bf16:
+        // 260 us, 284 by a block; (40000, 2048) from two 147 and 167).  With more, a block
+        // shares a token from 193 vectors on: (16383, 2048) from six 162 us for 186 by a
+        // wave, but (60000, 999) 338 for 312.
+        const int u = a.steps;
+        if (a.lanes < 64) combine_bwd_kernel<T, 0, 8, 1><<<grid_of(tokens, kThreads / a.lanes), kThreads, 0, s>>>(a);
+        else if (u == 1) combine_bwd_kernel<T, 1, 8, 1><<<by_wave, kThreads, 0, s>>>(a);
+        else if (top == 1 && u <= 2) combine_bwd_kernel<T, 1, 1, 2><<<by_wave, kThreads, 0, s>>>(a);
+        else if (top == 1 && u <= 4) combine_bwd_kernel<T, 1, 1, 4><<<by_wave, kThreads, 0, s>>>(a);
+        else if (top == 1 && u <= 8) combine_bwd_kernel<T, 1, 1, 8><<<by_wave, kThreads, 0, s>>>(a);
+        else if (top == 2 && u <= 2) combine_bwd_kernel<T, 1, 2, 2><<<by_wave, kThreads, 0, s>>>(a);
+        else if (top == 2 && u <= 4) combine_bwd_kernel<T, 1, 2, 4><<<by_wave, kThreads, 0, s>>>(a);
+        else if (u > 3) combine_bwd_kernel<T, 2, 8, 1><<<grid_of(tokens, 1), kThreads, 0, s>>>(a);
+        else combine_bwd_kernel<T, 1, 8, 1><<<by_wave, kThreads, 0, s>>>(a);
     });
     return launch_status(name);
 }

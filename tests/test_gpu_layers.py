@@ -68,7 +68,8 @@ def check_embedding(index, w, scale=1.0, padding=None, grad=None, seed=0):
 
 EMBEDDING = [(1, 1, 1), (3, 5, 7), (2, 3, 2), (31, 4, 8), (33, 4, 9), (129, 1031, 200), (1000, 1023, 64),
              (1000, 1024, 24), (4095, 50257, 65), (4096, 50257, 64), (4097, 1000, 40), (8191, 50257, 24),
-             (8192, 300, 513), (20000, 37, 33), (5000, (1 << 20) - 1, 4), (5000, 1 << 20, 4), (300, (1 << 20) + 5, 3)]
+             (8192, 300, 513), (20000, 37, 33), (5000, (1 << 20) - 1, 4), (5000, 1 << 20, 4), (300, (1 << 20) + 5, 3),
+             (9000, (1 << 20) + 5, 3), (9000, 1 << 20, 2), (8193, 5, 7)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -423,7 +424,8 @@ def check_rows(t, k, e, d, dtype, wdtype, mask=None, index=None, view=lambda a: 
 
 ROWS = [(1, 1, 1, 1), (1, 8, 256, 2048), (3, 2, 4, 3), (7, 3, 5, 7), (5, 2, 3, 8), (33, 6, 8, 9), (8, 9, 16, 65),
         (100, 8, 64, 128), (64, 17, 24, 136), (20, 2, 8, 511), (20, 2, 8, 512), (31, 4, 8, 513), (9, 8, 16, 1100),
-        (512, 2, 8, 768), (3, 40, 64, 4104), (1000, 6, 60, 200), (600, 1, 4, 1030), (700, 2, 8, 1041), (520, 5, 8, 1544)]
+        (512, 2, 8, 768), (3, 40, 64, 4104), (1000, 6, 60, 200), (600, 1, 4, 1030), (700, 2, 8, 1041), (520, 5, 8, 1544), (30, 1, 4, 3001), (30, 2, 4, 1900), (30, 2, 4, 700), (30, 1, 4, 600),
+        (9, 1, 4, 5000), (9, 2, 4, 5001)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)

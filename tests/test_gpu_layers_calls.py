@@ -295,6 +295,24 @@ def test_large_embedding(cuda):
         assert torch.equal(dw[:, c].float(), want.bfloat16().float())
 
 
+@pytest.mark.parametrize("n", [5000, 9000])
+def test_embedding_of_the_largest_vocabulary(cuda, n):
+    """Ids of 31 bits, sorted by as many digits as they take."""
+    from fuselse_amd import ext
+
+    v = 1 << 30
+    table = torch.zeros(v, 1, dtype=torch.float16, device=cuda)
+    ids = torch.cat([randint(cuda, v, n - 4), torch.tensor([0, v - 1, v - 1, v // 2], device=cuda)])
+    table[ids, 0] = (ids % 1000).half()
+    assert torch.equal(fuselse_amd.embedding(ids, table)[:, 0], (ids % 1000).half())
+    dw = ext.embedding_backward(torch.ones(n, 1, dtype=torch.float16, device=cuda), ids, v)
+    unique, counts = ids.unique(return_counts=True)
+    assert torch.equal(dw[unique, 0], counts.half())
+    assert int(torch.count_nonzero(dw)) == unique.numel()
+    with pytest.raises(RuntimeError, match="2\\^30"):
+        ext.embedding_backward(torch.ones(1, 1, dtype=torch.float16, device=cuda), ids[:1], v + 1)
+
+
 def test_large_layer_norm(cuda):
     n, d = 530000, 4096
     x = torch.empty(n, d, dtype=torch.bfloat16, device=cuda)

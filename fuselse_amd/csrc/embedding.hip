@@ -6,9 +6,10 @@
 // ids (stably, so sums always run in the tokens' order and take no atomics), sums
 // runs of equal ids in fp32 and rounds a row once.  A sorted run is cut where it
 // crosses a border of 16 or 64 entries, so a token that comes often is summed by many
-// waves; the pieces are joined in their order.  Rows that no token takes are
-// zeroed by other blocks of the same launch: most of the gradient's time, where
-// the vocabulary is large, is writing them.
+// waves; the pieces are joined in their order.  All of dW is zeroed by further
+// blocks of the sort's launches, which leave most of the chip idle: rows that no
+// token takes, most of them where the vocabulary is large, need nothing more, and
+// the time the sort takes is hidden.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -126,9 +127,11 @@ struct Zeros {
                     *(reinterpret_cast<u32x4_any*>(at + first) + j * key_sort::kThreads + (int)threadIdx.x) =
                         u32x4{0, 0, 0, 0};
         }
-        if (first < bytes)  // the share's end: whole elements, of two bytes at least
-            for (int64_t k = first + 2 * (int)threadIdx.x; k < bytes; k += 2 * key_sort::kThreads)
-                *reinterpret_cast<uint16_t*>(at + k) = 0;
+        if (first >= bytes) return;
+        // the share's end, to whole elements, of two bytes at least
+        int64_t k = first + 16 * (int)threadIdx.x;
+        for (; k + 16 <= bytes; k += 16 * key_sort::kThreads) *reinterpret_cast<u32x4_any*>(at + k) = u32x4{0, 0, 0, 0};
+        for (; k < bytes; k += 2) *reinterpret_cast<uint16_t*>(at + k) = 0;
     }
     unsigned blocks() const {
         const int64_t want = (bytes + kBytes - 1) / kBytes;

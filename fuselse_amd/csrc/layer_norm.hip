@@ -6,12 +6,11 @@
 // A row is held in registers by some lanes of a wave or a block, or read again from
 // the caches, so that memory sees each operand once; only the backward of rows of
 // more than 1024 vectors reads x and g twice, since a block's registers do not hold
-// sums for as many columns.  The
-// mean is kept as two numbers: m0, the rounded sum over D, and m1, the mean of
-// the differences to it.  x - m0 - m1 then keeps its digits when the row has a
-// large value in common, which one fp32 mean would take from it.  Lanes meet the
-// same columns in every row and sum dw and db in registers; the blocks' sums are
-// joined in their order.
+// sums for as many columns.  The mean is kept as two numbers: m0, the rounded sum
+// over D, and m1, the mean of the differences to it.  x - m0 - m1 then keeps its
+// digits when the row has a large value in common, which one fp32 mean would take
+// from it.  Lanes meet the same columns in every row and sum dw and db in registers;
+// the blocks' sums are joined in their order.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -535,7 +534,8 @@ int check(const char* name, int64_t rows, int64_t D, int64_t ldx, int dtype) {
 bool aligned(const void* p, int size) { return (reinterpret_cast<uintptr_t>(p) & (unsigned)(size - 1)) == 0; }
 int elem_size(int dtype) { return dtype == 0 ? 4 : 2; }
 
-// Lanes a row and vectors a lane; lanes 0: the row is longer than a block holds.
+// Lanes a row and vectors a lane, the fewest lanes that hold it in four vectors each;
+// lanes 0: the row is longer than a block holds, or shorter than a vector.
 struct Plan {
     int lanes, nv, rows;  // rows a block at once
 };

@@ -232,6 +232,17 @@ def test_layer_norm_many_rows(cuda, n, d):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", range(1, 10))
+def test_layer_norm_short_rows(cuda, d, dtype):
+    print(f"case norm short {d} {dtype}", flush=True)
+    for n, pdtype in ((255, torch.float32), (257, dtype), (200001, torch.float32)):
+        x, w, b = norm_inputs(cuda, n, d, dtype, pdtype)
+        check_norm(x, w, b)
+    check_norm(x.detach()[:1000], None, None)
+    check_norm(randn(cuda, 300, d + 3).to(dtype)[:, 2:2 + d], w.detach(), None)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("has", ["w", "b", ""])
 def test_layer_norm_parameters(cuda, dtype, has):
     print(f"case norm parameters {has} {dtype}", flush=True)

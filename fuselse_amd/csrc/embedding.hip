@@ -33,7 +33,7 @@ struct LookupArgs {
     void* out;
     int lanes, steps;
     int64_t items;
-    bool through;  // a wave an item, rows of out whole, aligned vectors
+    bool through;  // a wave an item, rows of out that are written through
 };
 
 // Lanes share a token's row, or a wave takes U times 64 vectors of it: a row's loads
@@ -437,7 +437,7 @@ extern "C" int fl_embedding_fwd(const void* weight, int64_t row_stride, int64_t 
     const bool more = a.steps > 1 && N * a.steps >= 1024;  // fewer waves would not fill the chip
     if (more) a.steps = (a.steps + 1) / 2;
     a.items = N * a.steps;
-    a.through = a.lanes == 64 && D % (dtype == 0 ? 4 : 8) == 0 && (reinterpret_cast<uintptr_t>(out) & 15u) == 0;
+    a.through = a.lanes == 64 && row_through(out, D * (dtype == 0 ? 4 : 2));
     const int per = kThreads / a.lanes;
     const int64_t want = (a.items + per - 1) / per;
     const unsigned blocks = (unsigned)(want < (1 << 22) ? want : (1 << 22));

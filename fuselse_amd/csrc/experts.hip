@@ -108,7 +108,7 @@ struct RowArgs {
     int lanes, steps;
     int64_t items;
     bool ragged;   // rows are no whole vectors
-    bool through;  // rows of out are whole, aligned vectors
+    bool through;  // rows of out are written through
 };
 
 template <typename T>
@@ -248,7 +248,8 @@ __device__ __forceinline__ int eighth(int sub) { return 4 * (sub & 1) + (sub & 2
 
 // The gradient of a combination, a token by its lanes or by the block: dy is read
 // once for A rows, and the loads of U vectors a lane of all of them are in flight
-// together, ahead of the stores, whose end a later load would wait for.
+// together, ahead of the stores, whose end a later load would wait for.  A wave's
+// rows are written through: (131072, 512) in bf16 from 8 experts each 434 us for 441.
 template <typename T, int TEAM, int A, int U>  // TEAM 0: p.lanes, 1: a wave, 2: the block
 __global__ __launch_bounds__(kThreads) void combine_bwd_kernel(RowArgs p) {
     constexpr int VE = Elem<T>::kVec;
@@ -304,7 +305,9 @@ __global__ __launch_bounds__(kThreads) void combine_bwd_kernel(RowArgs p) {
                                 for (int k = 0; k < VE; ++k) d[k] = w * g[k];
                                 r = pack_vec<T>(d);
                             }
-                            row_store(static_cast<T*>(p.out) + row * p.D, p.D, v, r);
+                            T* to = static_cast<T*>(p.out) + row * p.D;
+                            if (TEAM == 1 && p.through) row_store_through(to, p.D, v, r);
+                            else row_store(to, p.D, v, r);
                         }
                     if (!p.dweights) continue;
                     // elements that the vector before has too
@@ -381,7 +384,7 @@ void split_rows(RowArgs& a, int dtype) {
     a.steps = row_steps(nvec);
     a.items = a.tokens * a.steps;
     a.ragged = a.D % (dtype == 0 ? 4 : 8) != 0;
-    a.through = !a.ragged && (reinterpret_cast<uintptr_t>(a.out) & 15u) == 0;
+    a.through = row_through(a.out, a.D * (dtype == 0 ? 4 : 2));
 }
 
 unsigned grid_of(int64_t items, int per_block) {

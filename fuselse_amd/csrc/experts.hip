@@ -105,7 +105,7 @@ struct RowArgs {
     const void* rows;  // gradient: the experts' rows
     int64_t ldr;
     void* dweights;
-    int lanes, steps;
+    int lanes, steps, groups;  // groups of a token's rows
     int64_t items;
     bool ragged;   // rows are no whole vectors
     bool through;  // rows of out are written through
@@ -136,6 +136,17 @@ __device__ __forceinline__ int64_t item_stride(const RowArgs& p) {
 
 constexpr int kAhead = 8;  // rows whose loads are in flight
 
+// Token of item `it` of a group of A of its rows, and the first of them.  Groups are
+// items of their own, so that few tokens of many rows fill the chip too: 4 tokens of
+// 1024 rows of 512 in fp32 7 us to dispatch and 13 for the gradient, 166 and 1313 by
+// a loop over a token's; (8192, 2048) in bf16 of 16 rows each 100 for 104, 211 for 219.
+template <int A>
+__device__ __forceinline__ int64_t token_of(const RowArgs& p, int64_t it, int& k0) {
+    const int64_t t = p.groups == 1 ? it : it / p.groups;
+    k0 = (int)(it - t * p.groups) * A;
+    return t;
+}
+
 // Places of the token's entries k0, k0 + 1, ..; INT_MAX, outside all rows, past
 // the last.
 template <int A>
@@ -146,29 +157,31 @@ __device__ __forceinline__ void load_places(const RowArgs& p, int64_t t, int k0,
 
 // x is read with plain loads, since what made it has often left it in the caches
 // (with the nontemporal hint (16383, 2048) in bf16 to 6 experts each takes 98 us
-// for 80), and a wave's rows are written through to memory (77).
-template <typename T, bool WAVE>
+// for 80), and a wave's rows are written through to memory (77).  MANY: tokens may have
+// more rows than a group; whoever has one group is spared the division, for which the
+// load of x would wait ((60000, 4096) in bf16 to one expert each 158 us for 163).
+template <typename T, bool WAVE, bool MANY>
 __global__ __launch_bounds__(kThreads) void dispatch_kernel(RowArgs p) {
     const int nvec = row_vectors<T>(p.D);
     int sub;
     for (int64_t it = first_item<WAVE>(p, sub); it < p.items; it += item_stride<WAVE>(p)) {
-        const int64_t t = p.steps == 1 ? it : it / p.steps;
-        const int v = (int)(it - t * p.steps) * 64 + sub;
+        const int64_t group = p.steps == 1 ? it : it / p.steps;
+        const int v = (int)(it - group * p.steps) * 64 + sub;
         if (v >= nvec) continue;
+        int k0 = 0, at[kAhead];
+        int64_t t = group;
+        if constexpr (MANY) t = token_of<kAhead>(p, group, k0);
         const u32x4 x = row_load(static_cast<const T*>(p.in) + t * p.ldi, p.D, v);
-        for (int k0 = 0; k0 < p.top; k0 += kAhead) {
-            int at[kAhead];
-            load_places(p, t, k0, at);
+        load_places(p, t, k0, at);
 #pragma unroll
-            for (int u = 0; u < kAhead; ++u) {
-                const int row = at[u] < 0 ? ~at[u] : at[u];
-                if (row >= p.n) continue;
-                T* to = static_cast<T*>(p.out) + row * p.D;
-                u32x4 r = x;
-                if (at[u] < 0) r = u32x4{0, 0, 0, 0};
-                if (WAVE && p.through) row_store_through(to, p.D, v, r);
-                else row_store(to, p.D, v, r);
-            }
+        for (int u = 0; u < kAhead; ++u) {
+            const int row = at[u] < 0 ? ~at[u] : at[u];
+            if (row >= p.n) continue;
+            T* to = static_cast<T*>(p.out) + row * p.D;
+            u32x4 r = x;
+            if (at[u] < 0) r = u32x4{0, 0, 0, 0};
+            if (WAVE && p.through) row_store_through(to, p.D, v, r);
+            else row_store(to, p.D, v, r);
         }
     }
 }
@@ -258,91 +271,91 @@ __global__ __launch_bounds__(kThreads) void combine_bwd_kernel(RowArgs p) {
     const int nvec = row_vectors<T>(p.D);
     int sub = (int)threadIdx.x, turn = 0;
     const int team = BLOCK ? kThreads : TEAM == 1 ? 64 : p.lanes;
-    int64_t t = blockIdx.x, stride = gridDim.x;
+    int64_t it = blockIdx.x, stride = gridDim.x;
     if constexpr (!BLOCK) {
-        t = first_item<TEAM == 1>(p, sub);
+        it = first_item<TEAM == 1>(p, sub);
         stride = item_stride<TEAM == 1>(p);
     }
-    for (; t < p.tokens; t += stride) {
+    for (; it < p.items; it += stride, turn ^= 1) {
+        int k0;
+        const int64_t t = token_of<A>(p, it, k0);
         const T* dy = static_cast<const T*>(p.in) + t * p.ldi;
-        for (int k0 = 0; k0 < p.top; k0 += A, turn ^= 1) {
-            float dot[kAhead] = {};
-            int at[A];
-            load_places(p, t, k0, at);
-            for (int v0 = sub; v0 < nvec; v0 += team * U) {
-                u32x4 raw[A][U], gr[U];
+        float dot[kAhead] = {};
+        int at[A];
+        load_places(p, t, k0, at);
+        for (int v0 = sub; v0 < nvec; v0 += team * U) {
+            u32x4 raw[A][U], gr[U];
 #pragma unroll
-                for (int j = 0; j < U; ++j) {
-                    const int v = v0 + j * team;
-                    gr[j] = row_load(dy, p.D, v < nvec ? v : v0);
-                }
-                if (p.dweights)
+            for (int j = 0; j < U; ++j) {
+                const int v = v0 + j * team;
+                gr[j] = row_load(dy, p.D, v < nvec ? v : v0);
+            }
+            if (p.dweights)
 #pragma unroll
-                    for (int u = 0; u < A; ++u)
-                        if (at[u] >= 0 && at[u] < p.n)
+                for (int u = 0; u < A; ++u)
+                    if (at[u] >= 0 && at[u] < p.n)
 #pragma unroll
-                            for (int j = 0; j < U; ++j) {
-                                const int v = v0 + j * team;
-                                raw[u][j] = row_load<true>(static_cast<const T*>(p.rows) + at[u] * p.ldr, p.D,
-                                                           v < nvec ? v : v0);
-                            }
-#pragma unroll
-                for (int j = 0; j < U; ++j) {
-                    const int v = v0 + j * team;
-                    if (v >= nvec) continue;
-                    float g[VE];
-                    Elem<T>::cvt(gr[j], g);
-                    if (p.out)
-#pragma unroll
-                        for (int u = 0; u < A; ++u) {
-                            const int row = at[u] < 0 ? ~at[u] : at[u];
-                            if (row >= p.n) continue;
-                            u32x4 r{0, 0, 0, 0};
-                            if (at[u] >= 0) {
-                                const float w = weight_of<T>(p, t * p.top + k0 + u);
-                                float d[VE];
-#pragma unroll
-                                for (int k = 0; k < VE; ++k) d[k] = w * g[k];
-                                r = pack_vec<T>(d);
-                            }
-                            T* to = static_cast<T*>(p.out) + row * p.D;
-                            if (TEAM == 1 && p.through) row_store_through(to, p.D, v, r);
-                            else row_store(to, p.D, v, r);
+                        for (int j = 0; j < U; ++j) {
+                            const int v = v0 + j * team;
+                            raw[u][j] = row_load<true>(static_cast<const T*>(p.rows) + at[u] * p.ldr, p.D,
+                                                       v < nvec ? v : v0);
                         }
-                    if (!p.dweights) continue;
-                    // elements that the vector before has too
-                    const int skip = p.ragged && p.D >= VE ? (int)((int64_t)v * VE - row_vec_at<T>(p.D, v)) : 0;
 #pragma unroll
-                    for (int u = 0; u < A; ++u)
-                        if (at[u] >= 0 && at[u] < p.n) {
-                            float r[VE];
-                            Elem<T>::cvt(raw[u][j], r);
+            for (int j = 0; j < U; ++j) {
+                const int v = v0 + j * team;
+                if (v >= nvec) continue;
+                float g[VE];
+                Elem<T>::cvt(gr[j], g);
+                if (p.out)
 #pragma unroll
-                            for (int k = 0; k < VE; ++k)
-                                if (k >= skip) dot[u] = __builtin_fmaf(g[k], r[k], dot[u]);
+                    for (int u = 0; u < A; ++u) {
+                        const int row = at[u] < 0 ? ~at[u] : at[u];
+                        if (row >= p.n) continue;
+                        u32x4 r{0, 0, 0, 0};
+                        if (at[u] >= 0) {
+                            const float w = weight_of<T>(p, t * p.top + k0 + u);
+                            float d[VE];
+#pragma unroll
+                            for (int k = 0; k < VE; ++k) d[k] = w * g[k];
+                            r = pack_vec<T>(d);
                         }
-                }
-            }
-            if (!p.dweights) continue;
-            float s = sum_eight(dot, BLOCK ? 64 : team);
-            int u = eighth(sub);
-            bool mine = sub < kAhead;
-            if constexpr (BLOCK) {
-                // two turns' values, so that one barrier a turn is enough
-                if (((int)threadIdx.x & 63) < kAhead) sh[turn][threadIdx.x >> 6][u] = s;
-                __syncthreads();
-                u = sub;
-                if (mine) {
-                    s = sh[turn][0][u];
+                        T* to = static_cast<T*>(p.out) + row * p.D;
+                        if (TEAM == 1 && p.through) row_store_through(to, p.D, v, r);
+                        else row_store(to, p.D, v, r);
+                    }
+                if (!p.dweights) continue;
+                // elements that the vector before has too
+                const int skip = p.ragged && p.D >= VE ? (int)((int64_t)v * VE - row_vec_at<T>(p.D, v)) : 0;
 #pragma unroll
-                    for (int w = 1; w < kThreads / 64; ++w) s += sh[turn][w][u];
-                }
+                for (int u = 0; u < A; ++u)
+                    if (at[u] >= 0 && at[u] < p.n) {
+                        float r[VE];
+                        Elem<T>::cvt(raw[u][j], r);
+#pragma unroll
+                        for (int k = 0; k < VE; ++k)
+                            if (k >= skip) dot[u] = __builtin_fmaf(g[k], r[k], dot[u]);
+                    }
             }
-            if (mine && u < A && k0 + u < p.top) {
-                const int64_t i = t * p.top + k0 + u;
-                if (p.weights_f32) static_cast<float*>(p.dweights)[i] = s;
-                else Elem<T>::put(static_cast<T*>(p.dweights) + i, s);
+        }
+        if (!p.dweights) continue;
+        float s = sum_eight(dot, BLOCK ? 64 : team);
+        int u = eighth(sub);
+        bool mine = sub < kAhead;
+        if constexpr (BLOCK) {
+            // two turns' values, so that one barrier a turn is enough
+            if (((int)threadIdx.x & 63) < kAhead) sh[turn][threadIdx.x >> 6][u] = s;
+            __syncthreads();
+            u = sub;
+            if (mine) {
+                s = sh[turn][0][u];
+#pragma unroll
+                for (int w = 1; w < kThreads / 64; ++w) s += sh[turn][w][u];
             }
+        }
+        if (mine && u < A && k0 + u < p.top) {
+            const int64_t i = t * p.top + k0 + u;
+            if (p.weights_f32) static_cast<float*>(p.dweights)[i] = s;
+            else Elem<T>::put(static_cast<T*>(p.dweights) + i, s);
         }
     }
 }
@@ -382,7 +395,7 @@ void split_rows(RowArgs& a, int dtype) {
     const int nvec = vectors(a.D, dtype);
     a.lanes = row_lanes(nvec);
     a.steps = row_steps(nvec);
-    a.items = a.tokens * a.steps;
+    a.groups = (a.top + kAhead - 1) / kAhead;
     a.ragged = a.D % (dtype == 0 ? 4 : 8) != 0;
     a.through = row_through(a.out, a.D * (dtype == 0 ? 4 : 2));
 }
@@ -462,11 +475,13 @@ extern "C" int fl_expert_dispatch(const void* x, int64_t row_stride, int64_t tok
     a.top = (int)top;
     a.out = rows;
     split_rows(a, dtype);
+    a.items = tokens * a.groups * a.steps;
     hipStream_t s = static_cast<hipStream_t>(stream);
     by_type(dtype, [&](auto t) {
         const unsigned grid = grid_of(a.items, kThreads / a.lanes);
-        if (a.lanes == 64) dispatch_kernel<decltype(t), true><<<grid, kThreads, 0, s>>>(a);
-        else dispatch_kernel<decltype(t), false><<<grid, kThreads, 0, s>>>(a);
+        if (a.lanes < 64) dispatch_kernel<decltype(t), false, true><<<grid, kThreads, 0, s>>>(a);
+        else if (a.groups > 1) dispatch_kernel<decltype(t), true, true><<<grid, kThreads, 0, s>>>(a);
+        else dispatch_kernel<decltype(t), true, false><<<grid, kThreads, 0, s>>>(a);
     });
     return launch_status(name);
 }
@@ -494,11 +509,9 @@ extern "C" int fl_expert_combine(const void* rows, int64_t row_stride, int64_t t
     a.weights_f32 = weights_dtype == 0;
     a.out = out;
     split_rows(a, dtype);
-    const bool two = a.steps > 1 && a.items >= 1024;  // fewer waves would not fill the chip
-    if (two) {
-        a.steps = (a.steps + 1) / 2;
-        a.items = tokens * a.steps;
-    }
+    const bool two = a.steps > 1 && tokens * a.steps >= 1024;  // fewer waves would not fill the chip
+    if (two) a.steps = (a.steps + 1) / 2;
+    a.items = tokens * a.steps;
     hipStream_t s = static_cast<hipStream_t>(stream);
     by_type(dtype, [&](auto t) {
         using T = decltype(t);
@@ -541,24 +554,25 @@ extern "C" int fl_expert_combine_bwd(const void* grad, int64_t grad_stride, cons
     a.ldr = row_stride;
     a.dweights = grad_weights;
     split_rows(a, dtype);
+    a.items = tokens * a.groups;
     hipStream_t s = static_cast<hipStream_t>(stream);
     by_type(dtype, [&](auto t) {
         using T = decltype(t);
-        const unsigned by_wave = grid_of(tokens, kThreads / 64);
+        const unsigned by_wave = grid_of(a.items, kThreads / 64);
         // Steps of a wave over a row.  With one or two rows a token a wave takes up to
         // eight loads a lane of them in one step ((60000, 4096) from one expert each, bf16:
         // 260 us, 284 by a block; (40000, 2048) from two 147 and 167).  With more, a block
         // shares a token from 193 vectors on: (16383, 2048) from six 162 us for 186 by a
         // wave, but (60000, 999) 338 for 312.
         const int u = a.steps;
-        if (a.lanes < 64) combine_bwd_kernel<T, 0, 8, 1><<<grid_of(tokens, kThreads / a.lanes), kThreads, 0, s>>>(a);
+        if (a.lanes < 64) combine_bwd_kernel<T, 0, 8, 1><<<grid_of(a.items, kThreads / a.lanes), kThreads, 0, s>>>(a);
         else if (u == 1) combine_bwd_kernel<T, 1, 8, 1><<<by_wave, kThreads, 0, s>>>(a);
         else if (top == 1 && u <= 2) combine_bwd_kernel<T, 1, 1, 2><<<by_wave, kThreads, 0, s>>>(a);
         else if (top == 1 && u <= 4) combine_bwd_kernel<T, 1, 1, 4><<<by_wave, kThreads, 0, s>>>(a);
         else if (top == 1 && u <= 8) combine_bwd_kernel<T, 1, 1, 8><<<by_wave, kThreads, 0, s>>>(a);
         else if (top == 2 && u <= 2) combine_bwd_kernel<T, 1, 2, 2><<<by_wave, kThreads, 0, s>>>(a);
         else if (top == 2 && u <= 4) combine_bwd_kernel<T, 1, 2, 4><<<by_wave, kThreads, 0, s>>>(a);
-        else if (u > 3) combine_bwd_kernel<T, 2, 8, 1><<<grid_of(tokens, 1), kThreads, 0, s>>>(a);
+        else if (u > 3) combine_bwd_kernel<T, 2, 8, 1><<<grid_of(a.items, 1), kThreads, 0, s>>>(a);
         else combine_bwd_kernel<T, 1, 8, 1><<<by_wave, kThreads, 0, s>>>(a);
     });
     return launch_status(name);

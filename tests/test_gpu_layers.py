@@ -95,6 +95,18 @@ def test_embedding_one_token_many_times(cuda, n, d):
     check_embedding((torch.arange(n, device=cuda) // 32) % 77, w.detach())
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,v,d", [(131071, 3000, 8), (131072, 3000, 3), (131073, 5, 65), (200001, 70000, 24),
+                                   (65536, 4000, 520)])
+def test_embedding_many_tokens_of_short_rows(cuda, n, v, d, dtype):
+    print(f"case embedding many tokens {n} {v} {d} {dtype}", flush=True)
+    w = randn(cuda, v, d).to(dtype)
+    check_embedding(randint(cuda, v, n, seed=3), w)
+    # runs that end at and around the borders of 64 entries
+    for run in (63, 64, 65):
+        check_embedding((torch.arange(n, device=cuda) // run) % v, w.detach(), padding=0)
+
+
 @pytest.mark.parametrize("n", [0, 1, 40, 5000])
 def test_embedding_indexes_outside_and_padding(cuda, n):
     print(f"case embedding outside {n}", flush=True)
@@ -500,6 +512,14 @@ def test_expert_refusals(cuda):
         fuselse_amd.expert_combine(randn(cuda, 12, 8), w.double(), order)
     with pytest.raises(RuntimeError, match="position must be"):
         fuselse_amd.expert_dispatch(x, order._replace(position=order.position.long()))
+
+
+@pytest.mark.parametrize("t,k,d", [(3, 1024, 40), (5, 100, 520), (2, 1000, 2100), (70, 25, 9), (11, 16, 1024)])
+def test_expert_rows_of_many_choices(cuda, t, k, d):
+    print(f"case rows of many choices {t} {k} {d}", flush=True)
+    check_rows(t, k, 64, d, torch.bfloat16, torch.float32)
+    check_rows(t, k, 64, d, torch.float32, torch.float32, mask=randint(cuda, 2, t, seed=8) > 0)
+    check_rows(t, k, 64, d, torch.float16, torch.float16, index=randint(cuda, 70, t, k, seed=9) - 3)
 
 
 def test_places_outside_the_rows_are_dropped(cuda):

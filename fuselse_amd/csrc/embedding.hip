@@ -391,9 +391,10 @@ void digits(int64_t n, int64_t V, int& passes, int& bits) {
 int64_t align256(int64_t v) { return (v + 255) & ~(int64_t)255; }
 
 // Entries of a run: as many as a wave has loads in flight, or 64, which leave fewer
-// pieces to join, where that many waves keep the memory busy: (65536, 2048), all of
-// one token, 136 us for 266, (65536, 4096) 188 for 226, but (32768, 1024) 90 for 69.
-int run_of(int64_t n, int64_t D) { return n * D >= (1 << 26) ? 64 : kAhead; }
+// pieces to join, where that many waves keep the memory busy (steps of 512 columns):
+// (65536, 2048), all of one token, 136 us for 266, (65536, 4096) 188 for 226, (2^20, 4)
+// of 100000 rows in fp32 180 for 370, but (32768, 1024) 90 for 69.
+int run_of(int64_t n, int64_t D) { return n * ((D + 511) / 512) >= (1 << 17) ? 64 : kAhead; }
 int64_t runs_of(int64_t n, int64_t D) { return (n + run_of(n, D) - 1) / run_of(n, D); }
 
 struct Ws {

@@ -117,8 +117,7 @@ __device__ __forceinline__ float weight_of(const RowArgs& p, int64_t i) {
     return p.weights_f32 ? static_cast<const float*>(p.weights)[i] : Elem<T>::scalar(static_cast<const T*>(p.weights) + i);
 }
 
-// Item of this thread's lanes and its lane among them.  With WAVE a wave has one
-// item, and what belongs to it is read by scalar loads.
+// Item of this thread's lanes and its lane among them.  With WAVE a wave has one item.
 template <bool WAVE>
 __device__ __forceinline__ int64_t first_item(const RowArgs& p, int& sub) {
     if constexpr (WAVE) {
@@ -148,33 +147,65 @@ __device__ __forceinline__ int64_t token_of(const RowArgs& p, int64_t it, int& k
 }
 
 // Places of the token's entries k0, k0 + 1, ..; INT_MAX, outside all rows, past
-// the last.
+// the last.  A load each, which a wave waits for one by one.  All at once, as below, are
+// there sooner: 100 tokens of 2048 in bf16 from 32 experts each 9.4 us for 11.0, the
+// gradient of (40000, 2048) from two 141 for 147.  But the rows' loads then come in
+// bursts, and those of (131072, 512) from 8 take 211 us for 200.
 template <int A>
 __device__ __forceinline__ void load_places(const RowArgs& p, int64_t t, int k0, int (&at)[A]) {
 #pragma unroll
     for (int u = 0; u < A; ++u) at[u] = k0 + u < p.top ? p.position[t * p.top + k0 + u] : 0x7FFFFFFF;
 }
 
+// The same with their weights, by one load a wave, a lane an entry, for which all of it
+// has to be there.
+template <typename T, bool WAVE, int A>
+__device__ __forceinline__ void load_entries(const RowArgs& p, int64_t t, int k0, int (&at)[A], float (&w)[A]) {
+    const auto load = [&](int k, int& place, float& weight) {
+        const int64_t i = t * p.top + (k < p.top ? k : p.top - 1);
+        place = p.position[i];
+        weight = weight_of<T>(p, i);
+    };
+    if constexpr (WAVE) {
+        int place;
+        float weight;
+        load(k0 + (int)threadIdx.x % A, place, weight);
+#pragma unroll
+        for (int u = 0; u < A; ++u) {
+            at[u] = __builtin_amdgcn_readlane(place, u);
+            w[u] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, weight), u));
+        }
+    } else {
+#pragma unroll
+        for (int u = 0; u < A; ++u) load(k0 + u, at[u], w[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < A; ++u) at[u] = k0 + u < p.top ? at[u] : 0x7FFFFFFF;
+}
+
 // x is read with plain loads, since what made it has often left it in the caches
 // (with the nontemporal hint (16383, 2048) in bf16 to 6 experts each takes 98 us
 // for 80), and a wave's rows are written through to memory (77).  MANY: tokens may have
 // more rows than a group; whoever has one group is spared the division, for which the
-// load of x would wait ((60000, 4096) in bf16 to one expert each 158 us for 163).
-template <typename T, bool WAVE, bool MANY>
+// load of x would wait ((60000, 4096) in bf16 to one expert each 158 us for 163).  A is 1
+// where tokens are few: 8 of 2048 in bf16 to 8 experts each 3.1 us, 5.6 with all of a
+// token's rows by a wave.
+template <typename T, bool WAVE, int A, bool MANY>
 __global__ __launch_bounds__(kThreads) void dispatch_kernel(RowArgs p) {
+    if constexpr (WAVE) __builtin_assume(p.D >= Elem<T>::kVec);  // more than 32 vectors
     const int nvec = row_vectors<T>(p.D);
     int sub;
     for (int64_t it = first_item<WAVE>(p, sub); it < p.items; it += item_stride<WAVE>(p)) {
         const int64_t group = p.steps == 1 ? it : it / p.steps;
         const int v = (int)(it - group * p.steps) * 64 + sub;
         if (v >= nvec) continue;
-        int k0 = 0, at[kAhead];
+        int k0 = 0, at[A];
         int64_t t = group;
-        if constexpr (MANY) t = token_of<kAhead>(p, group, k0);
+        if constexpr (MANY) t = token_of<A>(p, group, k0);
         const u32x4 x = row_load(static_cast<const T*>(p.in) + t * p.ldi, p.D, v);
         load_places(p, t, k0, at);
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
+        for (int u = 0; u < A; ++u) {
             const int row = at[u] < 0 ? ~at[u] : at[u];
             if (row >= p.n) continue;
             T* to = static_cast<T*>(p.out) + row * p.D;
@@ -191,23 +222,28 @@ __global__ __launch_bounds__(kThreads) void dispatch_kernel(RowArgs p) {
 // loads and U times 64 vectors of them together: eight rows of one, or, where rows
 // are longer than that, up to four of two ((60000, 4096) from one expert each 225 us
 // with one vector a lane, 156 with two; (60000, 999) from 5 141 and 130).
-template <typename T, bool WAVE, int A, int U>
+template <typename T, bool WAVE, int A, int U, bool FEW = false>
 __global__ __launch_bounds__(kThreads) void combine_kernel(RowArgs p) {
     constexpr int VE = Elem<T>::kVec;
+    if constexpr (WAVE) __builtin_assume(p.D >= Elem<T>::kVec);  // more than 32 vectors
     const int nvec = row_vectors<T>(p.D);
     int sub;
     for (int64_t it = first_item<WAVE>(p, sub); it < p.items; it += item_stride<WAVE>(p)) {
         const int64_t t = p.steps == 1 ? it : it / p.steps;
-        const int v = (int)(it - t * p.steps) * 64 * U + sub;
-        if (v >= nvec) continue;
+        const int first = (int)(it - t * p.steps) * 64 * U + sub;
+        const int v = first < nvec ? first : nvec - 1;  // lanes behind the row load places too
         float acc[U][VE] = {};
         for (int k0 = 0; k0 < p.top; k0 += A) {
             int at[A];
             u32x4 raw[A][U];
             float w[A];
-            load_places(p, t, k0, at);
+            if constexpr (FEW) {
+                load_entries<T, WAVE>(p, t, k0, at, w);
+            } else {
+                load_places(p, t, k0, at);
 #pragma unroll
-            for (int u = 0; u < A; ++u) w[u] = k0 + u < p.top ? weight_of<T>(p, t * p.top + k0 + u) : 0.0f;
+                for (int u = 0; u < A; ++u) w[u] = k0 + u < p.top ? weight_of<T>(p, t * p.top + k0 + u) : 0.0f;
+            }
 #pragma unroll
             for (int u = 0; u < A; ++u)
                 if (at[u] >= 0 && at[u] < p.n)
@@ -228,7 +264,7 @@ __global__ __launch_bounds__(kThreads) void combine_kernel(RowArgs p) {
         }
 #pragma unroll
         for (int j = 0; j < U; ++j)
-            if (v + 64 * j < nvec) row_store(static_cast<T*>(p.out) + t * p.D, p.D, v + 64 * j, pack_vec<T>(acc[j]));
+            if (first + 64 * j < nvec) row_store(static_cast<T*>(p.out) + t * p.D, p.D, v + 64 * j, pack_vec<T>(acc[j]));
     }
 }
 
@@ -268,6 +304,7 @@ __global__ __launch_bounds__(kThreads) void combine_bwd_kernel(RowArgs p) {
     constexpr int VE = Elem<T>::kVec;
     constexpr bool BLOCK = TEAM == 2;
     __shared__ float sh[2][kThreads / 64][kAhead];
+    if constexpr (TEAM > 0) __builtin_assume(p.D >= VE);  // more than 32 vectors
     const int nvec = row_vectors<T>(p.D);
     int sub = (int)threadIdx.x, turn = 0;
     const int team = BLOCK ? kThreads : TEAM == 1 ? 64 : p.lanes;
@@ -282,7 +319,8 @@ __global__ __launch_bounds__(kThreads) void combine_bwd_kernel(RowArgs p) {
         const T* dy = static_cast<const T*>(p.in) + t * p.ldi;
         float dot[kAhead] = {};
         int at[A];
-        load_places(p, t, k0, at);
+        float w[A];
+        load_entries<T, (TEAM > 0)>(p, t, k0, at, w);
         for (int v0 = sub; v0 < nvec; v0 += team * U) {
             u32x4 raw[A][U], gr[U];
 #pragma unroll
@@ -313,10 +351,9 @@ __global__ __launch_bounds__(kThreads) void combine_bwd_kernel(RowArgs p) {
                         if (row >= p.n) continue;
                         u32x4 r{0, 0, 0, 0};
                         if (at[u] >= 0) {
-                            const float w = weight_of<T>(p, t * p.top + k0 + u);
                             float d[VE];
 #pragma unroll
-                            for (int k = 0; k < VE; ++k) d[k] = w * g[k];
+                            for (int k = 0; k < VE; ++k) d[k] = w[u] * g[k];
                             r = pack_vec<T>(d);
                         }
                         T* to = static_cast<T*>(p.out) + row * p.D;
@@ -475,13 +512,16 @@ extern "C" int fl_expert_dispatch(const void* x, int64_t row_stride, int64_t tok
     a.top = (int)top;
     a.out = rows;
     split_rows(a, dtype);
+    const bool few = a.lanes == 64 && tokens * a.groups * a.steps < 1024;  // so few waves do not fill the chip
+    if (few) a.groups = a.top;
     a.items = tokens * a.groups * a.steps;
     hipStream_t s = static_cast<hipStream_t>(stream);
     by_type(dtype, [&](auto t) {
         const unsigned grid = grid_of(a.items, kThreads / a.lanes);
-        if (a.lanes < 64) dispatch_kernel<decltype(t), false, true><<<grid, kThreads, 0, s>>>(a);
-        else if (a.groups > 1) dispatch_kernel<decltype(t), true, true><<<grid, kThreads, 0, s>>>(a);
-        else dispatch_kernel<decltype(t), true, false><<<grid, kThreads, 0, s>>>(a);
+        if (a.lanes < 64) dispatch_kernel<decltype(t), false, kAhead, true><<<grid, kThreads, 0, s>>>(a);
+        else if (few) dispatch_kernel<decltype(t), true, 1, true><<<grid, kThreads, 0, s>>>(a);
+        else if (a.groups > 1) dispatch_kernel<decltype(t), true, kAhead, true><<<grid, kThreads, 0, s>>>(a);
+        else dispatch_kernel<decltype(t), true, kAhead, false><<<grid, kThreads, 0, s>>>(a);
     });
     return launch_status(name);
 }
@@ -509,7 +549,7 @@ extern "C" int fl_expert_combine(const void* rows, int64_t row_stride, int64_t t
     a.weights_f32 = weights_dtype == 0;
     a.out = out;
     split_rows(a, dtype);
-    const bool two = a.steps > 1 && tokens * a.steps >= 1024;  // fewer waves would not fill the chip
+    const bool few = tokens * a.steps < 1024, two = a.steps > 1 && !few;  // so few waves do not fill the chip
     if (two) a.steps = (a.steps + 1) / 2;
     a.items = tokens * a.steps;
     hipStream_t s = static_cast<hipStream_t>(stream);
@@ -517,6 +557,7 @@ extern "C" int fl_expert_combine(const void* rows, int64_t row_stride, int64_t t
         using T = decltype(t);
         const unsigned grid = grid_of(a.items, kThreads / a.lanes);
         if (a.lanes < 64) combine_kernel<T, false, 8, 1><<<grid, kThreads, 0, s>>>(a);
+        else if (few) combine_kernel<T, true, 8, 1, true><<<grid, kThreads, 0, s>>>(a);
         else if (!two) combine_kernel<T, true, 8, 1><<<grid, kThreads, 0, s>>>(a);
         else if (top == 1) combine_kernel<T, true, 1, 2><<<grid, kThreads, 0, s>>>(a);
         else if (top == 2) combine_kernel<T, true, 2, 2><<<grid, kThreads, 0, s>>>(a);

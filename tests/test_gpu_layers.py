@@ -514,6 +514,14 @@ def test_expert_refusals(cuda):
         fuselse_amd.expert_dispatch(x, order._replace(position=order.position.long()))
 
 
+@pytest.mark.parametrize("t,k,d", [(1, 1, 520), (1023, 1, 512), (1024, 1, 512), (127, 8, 516), (128, 9, 2048),
+                                   (250, 3, 2052), (256, 3, 2050), (60, 16, 8200)])
+def test_expert_rows_around_the_fewest_waves(cuda, t, k, d):
+    print(f"case rows of few waves {t} {k} {d}", flush=True)
+    check_rows(t, k, 32, d, torch.bfloat16, torch.bfloat16, index=randint(cuda, 33, t, k, seed=9))
+    check_rows(t, k, 32, d, torch.float32, torch.float32, mask=randint(cuda, 2, t, seed=8) > 0)
+
+
 @pytest.mark.parametrize("t,k,d", [(3, 1024, 40), (5, 100, 520), (2, 1000, 2100), (70, 25, 9), (11, 16, 1024)])
 def test_expert_rows_of_many_choices(cuda, t, k, d):
     print(f"case rows of many choices {t} {k} {d}", flush=True)

@@ -454,6 +454,7 @@ __device__ __forceinline__ void load_param_long(const Args& p, const void* a, fl
 template <typename T>
 __global__ __launch_bounds__(kLong) void fwd_long(Args p) {
     constexpr int VE = Elem<T>::kVec;
+    __builtin_assume(p.D >= VE);  // more than 1024 vectors
     __shared__ float sh1[kLong / 64][1], sh2[kLong / 64][2];
     const float inv = 1.0f / (float)p.D;
     const int nvec = row_vectors<T>(p.D);
@@ -499,6 +500,7 @@ __global__ __launch_bounds__(kLong) void fwd_long(Args p) {
 template <typename T>
 __global__ __launch_bounds__(kLong) void dx_long(Args p) {
     constexpr int VE = Elem<T>::kVec;
+    __builtin_assume(p.D >= VE);  // more than 1024 vectors
     __shared__ float sh2[kLong / 64][2];
     const float inv = 1.0f / (float)p.D;
     const int nvec = row_vectors<T>(p.D);
@@ -536,10 +538,12 @@ __global__ __launch_bounds__(kLong) void dx_long(Args p) {
 }
 
 // A group's rows of 64 vectors of columns: sums of g h and of g, over the waves and
-// then over the groups in their order.
+// then over the groups in their order.  A wave has one row's loads in flight, as the
+// others fill the memory: (16384, 16384) in bf16 184 us, 218 with two or more.
 template <typename T>
 __global__ __launch_bounds__(256) void columns_long(Args p) {
     constexpr int VE = Elem<T>::kVec;
+    __builtin_assume(p.D >= VE);  // more than 1024 vectors
     __shared__ float sh[2][4][64 * VE];
     const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
     const int v = (int)blockIdx.x * 64 + lane;
@@ -547,7 +551,7 @@ __global__ __launch_bounds__(256) void columns_long(Args p) {
     const LongVec<T> at(p.D, live ? v : 0);
     float dw[VE] = {}, db[VE] = {};
     if (live) {
-#pragma unroll 4
+#pragma unroll 1
         for (int64_t r = (int64_t)blockIdx.y * 4 + wave; r < p.rows; r += (int64_t)gridDim.y * 4) {
             float x[VE], g[VE];
             load_long(static_cast<const T*>(p.x) + r * p.ldx, p.D, v, x);
@@ -657,8 +661,8 @@ int row_groups(int64_t rows, int64_t D, int dtype) {
     return (int)(want < most ? want : most);
 }
 // Rows of more than 256 lanes: a block of 1024 threads holds no sums beside them
-// ((16384, 16384) in bf16 950 us, spilling, for 481), and past 16 columns a lane not
-// even the rows ((8192, 20000) 375 us for dx, 290 where they are read again).
+// ((16384, 16384) in bf16 950 us, spilling, for 448), and past 16 columns a lane not
+// even the rows ((8192, 20000) 375 us for dx, 233 where they are read again).
 bool bwd_long_rows(const Plan& q) { return q.lanes == 0 || q.lanes > 256; }
 constexpr int kBwdColumns = 16384;
 int bwd_columns(const Plan& q, int dtype) { return q.lanes * q.nv * 16 / elem_size(dtype); }

@@ -7,9 +7,9 @@ contract (fuselse/gpu/autograd.py:6-61):
   ``robust`` is False) and ``ext.onepass_lse_float_backward``;
 * the returned ``logsumexp(input, dim=-1, keepdim=False)`` runs the kernel only
   for a CUDA fp32 tensor reduced over its last dimension with at least two
-  elements there, and calls ``torch.logsumexp`` (captured at factory time, so a
-  later ``torch.logsumexp = logsumexp`` patch does not recurse) for everything
-  else;
+  elements there and no forward-mode derivative, and calls ``torch.logsumexp``
+  (captured at factory time, so a later ``torch.logsumexp = logsumexp`` patch
+  does not recurse) for everything else;
 * with grad enabled and ``input.requires_grad`` it goes through an autograd
   Function whose backward is the fused ``grad * exp(x - lse)`` kernel (no
   double backward); its forward is the same kernel as without grad, as in the
@@ -35,6 +35,8 @@ of a training step does.
 from __future__ import annotations
 
 import torch
+
+from .ext import _has_tangent
 
 
 def make_fuselse_logsumexp(ext, robust: bool = True, half_inputs: bool = False, keep: bool = False):
@@ -111,7 +113,8 @@ def make_fuselse_logsumexp(ext, robust: bool = True, half_inputs: bool = False, 
         d = dim if dim >= 0 else nd + dim
         dtype = input.dtype
         half = dtype in half_fwd
-        if not (input.is_cuda and (dtype == torch.float32 or half) and d == nd - 1 and input.shape[-1] >= 2):
+        if not (input.is_cuda and (dtype == torch.float32 or half) and d == nd - 1 and input.shape[-1] >= 2
+                and not _has_tangent(input)):
             return torch_logsumexp(input, dim=dim, keepdim=keepdim)
         if torch.is_grad_enabled() and input.requires_grad:
             out = (_HalfRowLSE if half else _RowLSE).apply(input)

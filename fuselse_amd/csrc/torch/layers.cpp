@@ -10,12 +10,14 @@
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include "../../../include/fuselse_amd.h"
 
@@ -48,14 +50,17 @@ Tensor workspace(const Tensor& like, size_t bytes) { return make(like, {(int64_t
 const void* ptr(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 void* mut(const Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
 
-// A plain tensor or parameter, not empty, contiguous, on the current device.
+// A plain tensor or parameter, not empty, contiguous, on the current device, without a
+// forward-mode derivative.
 bool plain(PyObject* o, Tensor& t) {
     if (!THPVariable_CheckExact(o)) return false;
     t = THPVariable_Unpack(o);
     return t.is_cuda() && t.layout() == at::kStrided && !t.is_neg() && t.is_contiguous() && t.numel() > 0 &&
-           t.device().index() == c10::hip::current_device();
+           t.device().index() == c10::hip::current_device() && !t._fw_grad(0).defined();
 }
 bool floating(PyObject* o, Tensor& t) { return plain(o, t) && t.dim() >= 1 && code_of(t) >= 0; }
+// Whether torch may follow calls by more than autograd's nodes.
+bool followed() { return c10::impl::TorchDispatchModeTLS::any_modes_set() || torch::jit::tracer::isTracing(); }
 bool absent(PyObject* o) { return o == Py_None; }
 
 // A gradient as the kernels read it.
@@ -124,7 +129,7 @@ struct Embedding : torch::autograd::Function<Embedding> {
 PyObject* embedding(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     Tensor index, weight;
-    if (n != 4 || !plain(a[0], index) || index.scalar_type() != at::kLong || !floating(a[1], weight) ||
+    if (n != 4 || followed() || !plain(a[0], index) || index.scalar_type() != at::kLong || !floating(a[1], weight) ||
         weight.dim() != 2)
         Py_RETURN_NONE;
     const double scale = PyFloat_AsDouble(a[2]);
@@ -184,7 +189,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 PyObject* layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     Tensor x, w, b;
-    if (n != 4 || !floating(a[0], x)) Py_RETURN_NONE;
+    if (n != 4 || followed() || !floating(a[0], x)) Py_RETURN_NONE;
     for (int i = 1; i < 3; ++i) {
         Tensor& t = i == 1 ? w : b;
         if (absent(a[i])) continue;
@@ -209,7 +214,8 @@ PyObject* layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* expert_order(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     Tensor index, mask;
-    if (n != 3 || !plain(a[0], index) || index.scalar_type() != at::kLong || index.dim() < 1) Py_RETURN_NONE;
+    if (n != 3 || followed() || !plain(a[0], index) || index.scalar_type() != at::kLong || index.dim() < 1)
+        Py_RETURN_NONE;
     if (!absent(a[2]) && (!plain(a[2], mask) || mask.scalar_type() != at::kBool ||
                           mask.sizes() != index.sizes().slice(0, index.dim() - 1)))
         Py_RETURN_NONE;
@@ -289,7 +295,8 @@ struct Combine : torch::autograd::Function<Combine> {
 PyObject* expert_dispatch(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     Tensor x, position;
-    if (n != 2 || !floating(a[0], x) || !places(a[1], position) || !same_lead(x, position)) Py_RETURN_NONE;
+    if (n != 2 || followed() || !floating(a[0], x) || !places(a[1], position) || !same_lead(x, position))
+        Py_RETURN_NONE;
     if (x.requires_grad() && at::GradMode::is_enabled()) return THPVariable_Wrap(Dispatch::apply(x, position));
     return THPVariable_Wrap(dispatch(x, position));
     END_HANDLE_TH_ERRORS
@@ -299,8 +306,9 @@ PyObject* expert_dispatch(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* expert_combine(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     Tensor rows, weights, position;
-    if (n != 3 || !floating(a[0], rows) || rows.dim() != 2 || !floating(a[1], weights) || !places(a[2], position) ||
-        weights.sizes() != position.sizes() || rows.size(0) != position.numel() ||
+    if (n != 3 || followed() || !floating(a[0], rows) || rows.dim() != 2 || !floating(a[1], weights) ||
+        !places(a[2], position) || weights.sizes() != position.sizes() ||
+        rows.size(0) != position.numel() ||
         (weights.scalar_type() != rows.scalar_type() && weights.scalar_type() != at::kFloat))
         Py_RETURN_NONE;
     if ((rows.requires_grad() || weights.requires_grad()) && at::GradMode::is_enabled())

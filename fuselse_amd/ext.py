@@ -12,6 +12,7 @@ from __future__ import annotations
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -28,6 +29,24 @@ def _check_device(ref: torch.Tensor, ref_name: str, **others) -> None:
     for name, t in others.items():
         if t is not None:
             _check(t.device == ref.device, f"{name} must be on the same device as {ref_name}")
+
+
+def _has_tangent(*tensors) -> bool:
+    """Whether one of `tensors` (None is skipped) carries a forward-mode
+    derivative, which a kernel's result would lose without a word."""
+    return forward_ad._current_level >= 0 and any(
+        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
+def _check_eager(*tensors) -> None:
+    """Refuses a call that torch would have to follow: of tensors with a
+    forward-mode derivative, or while a graph is traced, into which the
+    allocation of a result would go and the kernel that writes it would not."""
+    _check(not _has_tangent(*tensors), "forward-mode derivatives are not supported")
+    _check(not torch._C._is_tracing() and not (
+        torch._C._len_torch_dispatch_stack()
+        and torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None),
+        "calls cannot be traced into a graph")
 
 
 # torch's raw current-stream query (what its own compiled kernels use) costs

@@ -3,11 +3,11 @@ autograd: the embedding lookup, layer norm, and tokens brought into their
 experts' order and back.  No counterpart in the reference.
 
 All take CUDA tensors only and raise RuntimeError for anything the kernels do
-not take; there is no CPU fallback.  They are differentiable once.  A call
-holds no state: its workspace comes from torch's allocator on the current
-stream, so calls may run on several streams and be captured into graphs.
-Sums are fp32 and results are rounded once, to the input's type, in autocast
-regions too.
+not take; there is no CPU fallback.  They are differentiable once, backward,
+and cannot be traced into a graph (torch.jit.trace, make_fx).  A call holds no
+state: its workspace comes from torch's allocator on the current stream, so
+calls may run on several streams and be captured into graphs.  Sums are fp32
+and results are rounded once, to the input's type, in autocast regions too.
 
 A call on contiguous tensors of the current device that need no conversion is
 made by compiled code (``_layers.so``), autograd and all, since the host's part
@@ -92,6 +92,7 @@ def embedding(index: torch.Tensor, weight: torch.Tensor, scale: float = 1.0,
     out = (_common or _bind()).embedding(index, weight, scale, padding)
     if out is not None:
         return out
+    ext._check_eager(weight)
     i = _integers(index, "index").reshape(-1).contiguous()
     w = _flat(weight) if weight.dim() == 2 else weight
     ext._check_embedding(w, i)
@@ -136,6 +137,7 @@ def layer_norm(input: torch.Tensor, weight: Optional[torch.Tensor] = None, bias:
     out = (_common or _bind()).layer_norm(input, weight, bias, eps)
     if out is not None:
         return out
+    ext._check_eager(input, weight, bias)
     ext._check(input.dim() >= 1, "input must have a last dimension")
     x = _flat(input)
     needs = input.requires_grad
@@ -177,6 +179,7 @@ def expert_order(index: torch.Tensor, num_experts: int, mask: Optional[torch.Ten
     out = (_common or _bind()).expert_order(index, num_experts, mask)
     if out is not None:
         return ExpertOrder._make(out)
+    ext._check_eager()
     ext._check(index.dim() >= 1, "index must be (..., top)")
     i, m = _integers(index, "index"), mask
     i = i.reshape(i.shape[:-1].numel(), i.shape[-1]).contiguous()
@@ -212,6 +215,7 @@ def expert_dispatch(input: torch.Tensor, order: ExpertOrder) -> torch.Tensor:
     out = (_common or _bind()).expert_dispatch(input, order.position)
     if out is not None:
         return out
+    ext._check_eager(input)
     ext._check(input.dim() >= 1 and input.shape[:-1] == order.position.shape[:-1],
                "input must be (..., D) with the tokens of order")
     x, position = _flat(input), _flat(order.position)
@@ -249,6 +253,7 @@ def expert_combine(rows: torch.Tensor, weights: torch.Tensor, order: ExpertOrder
     out = (_common or _bind()).expert_combine(rows, weights, order.position)
     if out is not None:
         return out
+    ext._check_eager(rows, weights)
     ext._check(weights.shape == order.position.shape, "weights must have the shape of order's index")
     needs = rows.requires_grad or weights.requires_grad
     w = weights

@@ -4,9 +4,10 @@ distillation from a teacher's top logits, and the balance loss of a
 mixture-of-experts router.  No counterpart in the reference.
 
 All take CUDA tensors only and raise RuntimeError for anything the kernels do
-not take; there is no CPU fallback.  They are differentiable once.  A call
-holds no state: its workspace comes from torch's allocator on the current
-stream, so calls may run on several streams and be captured into graphs.
+not take; there is no CPU fallback.  They are differentiable once, backward,
+and cannot be traced into a graph (torch.jit.trace, make_fx).  A call holds no
+state: its workspace comes from torch's allocator on the current stream, so
+calls may run on several streams and be captured into graphs.
 """
 
 from __future__ import annotations
@@ -89,6 +90,7 @@ def linear_cross_entropy(input: torch.Tensor, weight: torch.Tensor, target: torc
     fp16 what lies below 2^-39 of the largest row's is lost.  At most 2^23
     tokens, 2^28 vocabulary entries and 2^20 columns.
     """
+    ext._check_eager(input, weight)
     ext._check(input.dim() >= 1 and tuple(input.shape[:-1]) == tuple(target.shape),
                "target must have input's shape without its last dimension")
     input, weight = _one_type(input, weight)
@@ -142,6 +144,7 @@ def topk_distillation(logits: torch.Tensor, teacher_logits: torch.Tensor, teache
     logits whose last dimension is contiguous are read where they are
     (logits[:, :-1] of a batch of sequences is not copied).
     """
+    ext._check_eager(logits, teacher_logits)
     ext._check(logits.dim() >= 1 and tuple(logits.shape[:-1]) == tuple(teacher_logits.shape[:-1])
                and teacher_logits.shape == teacher_index.shape,
                "teacher_logits and teacher_index must be (..., K) with the rows of logits")
@@ -201,6 +204,7 @@ def router_balance(logits: torch.Tensor, index: torch.Tensor, mask: Optional[tor
     the counts are constants.  At most 1024 experts, 1024 choices a token and
     2^31 - 1 choices.
     """
+    ext._check_eager(logits)
     ext._check(logits.dim() >= 1 and tuple(logits.shape[:-1]) == tuple(index.shape[:-1]) and index.dim() >= 1,
                "index must be (..., top) with the tokens of logits")
     ext._check(mask is None or tuple(mask.shape) == tuple(logits.shape[:-1]),

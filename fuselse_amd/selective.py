@@ -12,15 +12,18 @@ thing is one pass over the logits (forward) and one read + one write
 ``make_selective_log_softmax(ext, original=None, robust=True)`` returns
 ``selective_log_softmax(logits, index)`` with trl's signature: logits
 [..., V], index [...] (integer), result [...] fp32.  CUDA fp32 logits take
-the kernels, with autograd through the fused backward.  Other inputs go to
-``original`` (for instance trl's own function), or, when it is None, to
-trl's published algorithm in torch ops (``_trl_algorithm``).
+the kernels, with autograd through the fused backward.  Other inputs, and
+logits with a forward-mode derivative, go to ``original`` (for instance trl's
+own function), or, when it is None, to trl's published algorithm in torch ops
+(``_trl_algorithm``).
 """
 
 from __future__ import annotations
 
 import torch
 import torch.nn.functional as F
+
+from .ext import _has_tangent
 
 
 def _trl_algorithm(logits: torch.Tensor, index: torch.Tensor) -> torch.Tensor:
@@ -128,7 +131,8 @@ def make_selective_log_softmax(ext, original=None, robust: bool = True):
     def selective_log_softmax(logits, index):
         ok = (logits.is_cuda and logits.dtype == torch.float32 and logits.dim() >= 1
               and index.device == logits.device and not torch.is_floating_point(index)
-              and tuple(index.shape) == tuple(logits.shape[:-1]) and logits.shape[-1] >= 1)
+              and tuple(index.shape) == tuple(logits.shape[:-1]) and logits.shape[-1] >= 1
+              and not _has_tangent(logits))
         if not ok:
             return fallback(logits, index)
         if torch.is_grad_enabled() and logits.requires_grad:

@@ -78,18 +78,20 @@ std::vector<int64_t> with_last(const Tensor& t, int64_t n) {
     return s;
 }
 
-// Results of a backward are constants: with create_graph, what is differentiated
-// again says so.
-variable_list once(variable_list&& out, const variable_list& grads) {
+// Results of a backward are constants: with create_graph, those that depend on what
+// requires a gradient (the upstream one, or, where `saved` says so, saved tensors) are an
+// error where they are differentiated again.
+variable_list once(variable_list&& out, const variable_list& grads, std::initializer_list<bool> saved = {}) {
     if (!at::GradMode::is_enabled()) return std::move(out);
-    bool any = false;
-    for (const Tensor& g : grads) any = any || (g.defined() && g.requires_grad());
-    if (!any) return std::move(out);
-    for (Tensor& g : out)
-        if (g.defined()) g = g.detach().set_requires_grad(true);
-    const auto error = std::make_shared<torch::autograd::DelayedError>(
-        "trying to differentiate twice a function that is differentiable once", (int64_t)out.size());
-    return error->apply(std::move(out));
+    bool all = false;
+    for (const Tensor& g : grads) all = all || (g.defined() && g.requires_grad());
+    for (size_t i = 0; i < out.size(); ++i) {
+        if (!out[i].defined() || !(all || (i < saved.size() && saved.begin()[i]))) continue;
+        const auto error = std::make_shared<torch::autograd::DelayedError>(
+            "trying to differentiate twice a function that is differentiable once", 1);
+        out[i] = error->apply({out[i].detach().set_requires_grad(true)})[0];
+    }
+    return std::move(out);
 }
 
 // ---------------------------------------------------------------------------
@@ -159,6 +161,8 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
         const Tensor weight = w.value_or(Tensor()), bias = b.value_or(Tensor());
         Tensor y = norm_fwd(x, weight, bias, eps, &stats);
         ctx->save_for_backward({x, weight, stats});
+        ctx->saved_data["x_grad"] = x.requires_grad();
+        ctx->saved_data["w_grad"] = weight.defined() && weight.requires_grad();
         ctx->saved_data["weight"] = w.has_value();
         ctx->saved_data["bias"] = b.has_value();
         ctx->saved_data["type"] =
@@ -181,7 +185,8 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
         check(fl_layer_norm_bwd(ptr(g), D, ptr(x), D, N, D, code_of(x), ptr(w), code_of(type),
                                 st.const_data_ptr<float>(), mut(dx), mut(dw), mut(db), mut(ws),
                                 ws.defined() ? (size_t)ws.numel() : 0, stream_of(x)));
-        return once({dx, dw, db, Tensor()}, grads);
+        const bool of_x = ctx->saved_data["x_grad"].toBool(), of_w = ctx->saved_data["w_grad"].toBool();
+        return once({dx, dw, db, Tensor()}, grads, {of_x || of_w, of_x});
     }
 };
 
@@ -274,6 +279,8 @@ struct Dispatch : torch::autograd::Function<Dispatch> {
 struct Combine : torch::autograd::Function<Combine> {
     static Tensor forward(AutogradContext* ctx, const Tensor& rows, const Tensor& weights, const Tensor& position) {
         ctx->save_for_backward({rows, weights, position});
+        ctx->saved_data["rows_grad"] = rows.requires_grad();
+        ctx->saved_data["weights_grad"] = weights.requires_grad();
         return combine(rows, weights, position);
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -287,7 +294,8 @@ struct Combine : torch::autograd::Function<Combine> {
         if (ctx->needs_input_grad(1)) d_weights = at::empty_like(weights);
         check(fl_expert_combine_bwd(ptr(g), D, ptr(rows), D, T, D, code_of(rows), position.const_data_ptr<int32_t>(),
                                     K, ptr(weights), code_of(weights), mut(d_rows), mut(d_weights), stream_of(rows)));
-        return once({d_rows, d_weights, Tensor()}, grads);
+        return once({d_rows, d_weights, Tensor()}, grads,
+                    {ctx->saved_data["weights_grad"].toBool(), ctx->saved_data["rows_grad"].toBool()});
     }
 };
 

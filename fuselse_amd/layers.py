@@ -19,10 +19,9 @@ from __future__ import annotations
 from typing import NamedTuple, Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib, ext
-from .losses import _integers, _rows
+from .losses import _integers, _once, _rows
 
 _common = None
 
@@ -41,17 +40,6 @@ def _bind():
     return _layers
 
 
-def _once(backward):
-    """once_differentiable, but for the common call outside create_graph, which
-    has no graph to keep from being made."""
-    guarded = once_differentiable(backward)
-
-    def run(ctx, grad):
-        return guarded(ctx, grad) if torch.is_grad_enabled() else backward(ctx, grad)
-
-    return staticmethod(run)
-
-
 def _flat(t: torch.Tensor) -> torch.Tensor:
     """t in rows, as the kernels take them."""
     t = t.resolve_neg()
@@ -63,6 +51,7 @@ class _Embedding(torch.autograd.Function):
     def forward(ctx, weight, index, scale, padding):
         ctx.save_for_backward(index)
         ctx.args = (weight.shape[0], scale, padding)
+        ctx.saved = (False,) * 4
         return ext._embedding_fwd(weight, index, scale)
 
     @_once
@@ -110,6 +99,8 @@ class _LayerNorm(torch.autograd.Function):
         ctx.save_for_backward(x, weight, stats)
         of = weight if weight is not None else bias
         ctx.params_dtype = of.dtype if of is not None else None
+        of_x, of_weight = ctx.needs_input_grad[:2]
+        ctx.saved = (of_x or of_weight, of_x, False, False)
         return y
 
     @_once
@@ -195,6 +186,7 @@ class _Dispatch(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, position):
         ctx.save_for_backward(position)
+        ctx.saved = (False, False)
         return ext._dispatch(x, position)
 
     @_once
@@ -229,6 +221,7 @@ class _Combine(torch.autograd.Function):
     @staticmethod
     def forward(ctx, rows, weights, position):
         ctx.save_for_backward(rows, weights, position)
+        ctx.saved = (ctx.needs_input_grad[1], ctx.needs_input_grad[0], False)
         return ext._combine(rows, weights, position)
 
     @_once

@@ -15,7 +15,6 @@ from __future__ import annotations
 from typing import NamedTuple, Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import ext
 
@@ -46,16 +45,39 @@ def _one_type(a: torch.Tensor, b: torch.Tensor):
     return a, b
 
 
+def _once(backward):
+    """A backward whose results are constants: with create_graph, those that
+    depend on what requires a gradient (the upstream one, or, where ctx.saved
+    says so, saved tensors) are an error where they are differentiated again."""
+
+    def run(ctx, *grads):
+        if not torch.is_grad_enabled():
+            return backward(ctx, *grads)
+        with torch.no_grad():
+            out = backward(ctx, *grads)
+        out = out if isinstance(out, tuple) else (out,)
+        saved = (True,) * len(out) if any(g is not None and g.requires_grad for g in grads) else ctx.saved
+        return tuple(_constant(t) if t is not None and s else t for t, s in zip(out, saved))
+
+    return staticmethod(run)
+
+
+def _constant(t: torch.Tensor) -> torch.Tensor:
+    error = torch._C._functions.DelayedError(
+        b"trying to differentiate twice a function that is differentiable once", 1)
+    return error(t.detach().requires_grad_())
+
+
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, target, ignore_index, reduction, z_loss):
         loss, lse = ext._linear_fwd(x, weight, target, ignore_index, reduction, z_loss, True)
         ctx.save_for_backward(x, weight, target, lse)
         ctx.args = (ignore_index, reduction, z_loss)
+        ctx.saved = (True, True, False, False, False, False)
         return loss
 
-    @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, grad):
         x, weight, target, lse = ctx.saved_tensors
         need = ctx.needs_input_grad
@@ -111,10 +133,10 @@ class _TopkDistillation(torch.autograd.Function):
         loss, _, _, norm, pairs = ext._distill_fwd(logits, teacher, index, temperature, reduction, True)
         ctx.save_for_backward(logits, teacher, index, norm, pairs)
         ctx.temperature = temperature
+        ctx.saved = (True, False, False, False, False)
         return loss
 
-    @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, grad):
         logits, teacher, index, norm, pairs = ctx.saved_tensors
         if logits.stride(-1) != 1 and logits.shape[-1] != 1:  # as a saved-tensor hook may give it back
@@ -179,10 +201,10 @@ class _RouterBalance(torch.autograd.Function):
         ctx.save_for_backward(logits, mask, lse, coef)
         ctx.mark_non_differentiable(counts)
         ctx.set_materialize_grads(False)
+        ctx.saved = (True, False, False)
         return balance, z, counts
 
-    @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, grad_balance, grad_z, _):
         if grad_balance is None and grad_z is None:
             return None, None, None

@@ -89,11 +89,45 @@ __device__ __forceinline__ void row_sum(float (&v)[N], float (*sh)[N]) {
 }
 
 // What the backward needs of a row: m0, -m1 r and r, so that h is two operations:
-// (x - m0) r - m1 r.
-__device__ __forceinline__ f32x4 row_stats(float m0, float m1, float mean_square, float eps) {
+// (x - m0) r - m1 r.  m1 and the mean square are of the differences times f, a power of two.
+__device__ __forceinline__ f32x4 row_stats(float m0, float m1, float mean_square, float eps, float f = 1.0f) {
     const float var = mean_square - m1 * m1;
-    const float rstd = 1.0f / sqrtf((var < 0.0f ? 0.0f : var) + eps);
-    return f32x4{m0, -m1 * rstd, rstd, 0.0f};
+    const float rstd = 1.0f / sqrtf((var < 0.0f ? 0.0f : var) + eps * f * f);
+    return f32x4{m0, -m1 * rstd, rstd * f, 0.0f};
+}
+
+// Sums over a row may leave fp32 where its elements do not.  That of the elements is then
+// made of elements scaled down (row_mean_wide).  That of the squared differences to m0
+// may too, and where the elements are equal, or all but, these differences are m0's
+// rounding alone, of which no variance is left.  Such a row is summed again: m0 moves by
+// the differences' mean, so that equal elements come to differ by 0 exactly; unscaled
+// differences are then in range where only m0 was off; and scaled down they are whatever
+// they are.  sums(m0, f, d) gives d, the row's sums of f (x - m0) and of its squares, and
+// move(m0, to) what it keeps of x - m0.
+__device__ __forceinline__ bool finite(float v) { return __builtin_fabsf(v) < kInf; }
+constexpr float kDown = 0x1p-26f;  // of 2^24 elements
+template <typename Sum>
+__device__ __forceinline__ float row_mean_wide(float inv, Sum sum) {
+    return sum(kDown) * inv * (1.0f / kDown);
+}
+
+__device__ __forceinline__ bool row_stats_hold(const float (&d)[2], float inv) {
+    const float m1 = d[0] * inv, mean_square = d[1] * inv;
+    return mean_square < kInf && mean_square - m1 * m1 >= mean_square * 0x1p-10f;
+}
+constexpr float kWide = 0x1p-80f;  // squares of 2^24 elements that it scales down are in range
+template <typename Sums, typename Move>
+__device__ __forceinline__ f32x4 row_stats_wide(float m0, float inv, float eps, float (&d)[2], Sums sums, Move move) {
+    float f = finite(d[0]) ? 1.0f : kWide;
+    if (f != 1.0f) sums(m0, f, d);
+    const float to = m0 + d[0] * inv * (1.0f / f);
+    move(m0, to);
+#pragma unroll 1
+    for (f = 1.0f;; f = kWide) {
+        sums(to, f, d);
+        if (f != 1.0f || d[1] < kInf) break;
+    }
+    return row_stats(to, d[0] * inv, d[1] * inv, eps, f);
 }
 
 // How a block is laid out for rows of LANES * NV vectors at most.
@@ -200,7 +234,18 @@ __global__ __launch_bounds__(Shape<LANES>::kThreads) void fwd_kernel(Args p) {
         }
         if (r + step < p.rows) load_row<T>(col, static_cast<const T*>(p.x) + (r + step) * p.ldx, next);
         row_sum<LANES>(s, sh1);
-        const float m0 = s[0] * inv;
+        float m0 = s[0] * inv;
+        if (!finite(m0))
+            m0 = row_mean_wide(inv, [&](float f) {
+                float o[1] = {};
+#pragma unroll
+                for (int j = 0; j < NV; ++j)
+#pragma unroll
+                    for (int k = 0; k < VE; ++k)
+                        if (col.counts(j, k)) o[0] += x[j][k] * f;
+                row_sum<LANES>(o, sh1);
+                return o[0];
+            });
         float d[2] = {};
 #pragma unroll
         for (int j = 0; j < NV; ++j)
@@ -213,7 +258,29 @@ __global__ __launch_bounds__(Shape<LANES>::kThreads) void fwd_kernel(Args p) {
                 }
             }
         row_sum<LANES>(d, sh2);
-        const f32x4 st = row_stats(m0, d[0] * inv, d[1] * inv, p.eps);
+        f32x4 st = row_stats(m0, d[0] * inv, d[1] * inv, p.eps);
+        if (!row_stats_hold(d, inv))
+            st = row_stats_wide(
+                m0, inv, p.eps, d,
+                [&](float, float f, float (&o)[2]) {
+                    o[0] = o[1] = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < NV; ++j)
+#pragma unroll
+                        for (int k = 0; k < VE; ++k)
+                            if (col.counts(j, k)) {
+                                const float c = x[j][k] * f;
+                                o[0] += c;
+                                o[1] = __builtin_fmaf(c, c, o[1]);
+                            }
+                    row_sum<LANES>(o, sh2);
+                },
+                [&](float from, float to) {
+#pragma unroll
+                    for (int j = 0; j < NV; ++j)
+#pragma unroll
+                        for (int k = 0; k < VE; ++k) x[j][k] = x[j][k] + from - to;
+                });
         if (p.stats && sub == 0) p.stats[r] = st;
         T* y = static_cast<T*>(p.y) + r * p.D;
 #pragma unroll
@@ -361,21 +428,46 @@ __global__ __launch_bounds__(kShort) void fwd_short(Args p) {
     load_param_short<T>(p, p.w, 1.0f, w);
     load_param_short<T>(p, p.b, 0.0f, b);
     for (int64_t r = (int64_t)blockIdx.x * kShort + threadIdx.x; r < p.rows; r += (int64_t)p.blocks * kShort) {
-        float x[VE], s = 0.0f, d = 0.0f, sq = 0.0f;
+        float x[VE], s = 0.0f, d[2] = {};
         load_short(static_cast<const T*>(p.x) + r * p.ldx, p.D, x);
 #pragma unroll
         for (int k = 0; k < VE; ++k)
             if (k < p.D) s += x[k];
-        const float m0 = s * inv;
+        float m0 = s * inv;
+        if (!finite(m0))
+            m0 = row_mean_wide(inv, [&](float f) {
+                float o = 0.0f;
+#pragma unroll
+                for (int k = 0; k < VE; ++k)
+                    if (k < p.D) o += x[k] * f;
+                return o;
+            });
 #pragma unroll
         for (int k = 0; k < VE; ++k) {
             x[k] -= m0;
             if (k < p.D) {
-                d += x[k];
-                sq = __builtin_fmaf(x[k], x[k], sq);
+                d[0] += x[k];
+                d[1] = __builtin_fmaf(x[k], x[k], d[1]);
             }
         }
-        const f32x4 st = row_stats(m0, d * inv, sq * inv, p.eps);
+        f32x4 st = row_stats(m0, d[0] * inv, d[1] * inv, p.eps);
+        if (!row_stats_hold(d, inv))
+            st = row_stats_wide(
+                m0, inv, p.eps, d,
+                [&](float, float f, float (&o)[2]) {
+                    o[0] = o[1] = 0.0f;
+#pragma unroll
+                    for (int k = 0; k < VE; ++k)
+                        if (k < p.D) {
+                            const float c = x[k] * f;
+                            o[0] += c;
+                            o[1] = __builtin_fmaf(c, c, o[1]);
+                        }
+                },
+                [&](float from, float to) {
+#pragma unroll
+                    for (int k = 0; k < VE; ++k) x[k] = x[k] + from - to;
+                });
         if (p.stats) p.stats[r] = st;
 #pragma unroll
         for (int k = 0; k < VE; ++k) x[k] = __builtin_fmaf(__builtin_fmaf(x[k], st[2], st[1]), w[k], b[k]);
@@ -460,29 +552,39 @@ __global__ __launch_bounds__(kLong) void fwd_long(Args p) {
     const int nvec = row_vectors<T>(p.D);
     for (int64_t r = blockIdx.x; r < p.rows; r += p.blocks) {
         const T* row = static_cast<const T*>(p.x) + r * p.ldx;
-        float s[1] = {}, d[2] = {}, x[VE], w[VE], b[VE];
-        for (int v = threadIdx.x; v < nvec; v += kLong) {
-            const LongVec<T> at(p.D, v);
-            load_long(row, p.D, v, x);
+        float d[2], x[VE], w[VE], b[VE];
+        const auto sum = [&](float f) {
+            float o[1] = {};
+            for (int v = threadIdx.x; v < nvec; v += kLong) {
+                const LongVec<T> at(p.D, v);
+                load_long(row, p.D, v, x);
 #pragma unroll
-            for (int k = 0; k < VE; ++k)
-                if (at.counts(k)) s[0] += x[k];
-        }
-        row_sum<kLong>(s, sh1);
-        const float m0 = s[0] * inv;
-        for (int v = threadIdx.x; v < nvec; v += kLong) {
-            const LongVec<T> at(p.D, v);
-            load_long(row, p.D, v, x);
+                for (int k = 0; k < VE; ++k)
+                    if (at.counts(k)) o[0] += x[k] * f;
+            }
+            row_sum<kLong>(o, sh1);
+            return o[0];
+        };
+        const auto sums = [&](float m0, float f, float (&o)[2]) {
+            o[0] = o[1] = 0.0f;
+            for (int v = threadIdx.x; v < nvec; v += kLong) {
+                const LongVec<T> at(p.D, v);
+                load_long(row, p.D, v, x);
 #pragma unroll
-            for (int k = 0; k < VE; ++k)
-                if (at.counts(k)) {
-                    const float c = x[k] - m0;
-                    d[0] += c;
-                    d[1] = __builtin_fmaf(c, c, d[1]);
-                }
-        }
-        row_sum<kLong>(d, sh2);
-        const f32x4 st = row_stats(m0, d[0] * inv, d[1] * inv, p.eps);
+                for (int k = 0; k < VE; ++k)
+                    if (at.counts(k)) {
+                        const float c = (x[k] - m0) * f;
+                        o[0] += c;
+                        o[1] = __builtin_fmaf(c, c, o[1]);
+                    }
+            }
+            row_sum<kLong>(o, sh2);
+        };
+        float m0 = sum(1.0f) * inv;
+        if (!finite(m0)) m0 = row_mean_wide(inv, sum);
+        sums(m0, 1.0f, d);
+        f32x4 st = row_stats(m0, d[0] * inv, d[1] * inv, p.eps);
+        if (!row_stats_hold(d, inv)) st = row_stats_wide(m0, inv, p.eps, d, sums, [](float, float) {});
         if (p.stats && threadIdx.x == 0) p.stats[r] = st;
         for (int v = threadIdx.x; v < nvec; v += kLong) {
             const LongVec<T> at(p.D, v);
@@ -490,7 +592,7 @@ __global__ __launch_bounds__(kLong) void fwd_long(Args p) {
             load_param_long<T>(p, p.w, 1.0f, at.at, w);
             load_param_long<T>(p, p.b, 0.0f, at.at, b);
 #pragma unroll
-            for (int k = 0; k < VE; ++k) x[k] = __builtin_fmaf(__builtin_fmaf(x[k] - m0, st[2], st[1]), w[k], b[k]);
+            for (int k = 0; k < VE; ++k) x[k] = __builtin_fmaf(__builtin_fmaf(x[k] - st[0], st[2], st[1]), w[k], b[k]);
             row_store(static_cast<T*>(p.y) + r * p.D, p.D, v, pack_vec<T>(x));
         }
     }

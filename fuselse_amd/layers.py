@@ -121,9 +121,10 @@ def layer_norm(input: torch.Tensor, weight: Optional[torch.Tensor] = None, bias:
     None; they may be of any of these types and are taken in fp32 where they
     are not of input's.  y = (x - mean) / sqrt(variance + eps) * weight + bias
     in input's type, the variance over D; a value that a row's elements have in
-    common costs no digits.  Rows that spread over more than about 2^63
-    overflow.  Gradients reach all three.  At most 2^31 - 1 rows and 2^24
-    columns.
+    common costs no digits, and equal elements give the bias exactly.  Elements
+    may be of any size: only a row in which one differs from the mean by more
+    than fp32 holds is NaN.  Gradients reach all three.  At most 2^31 - 1 rows
+    and 2^24 columns.
     """
     out = (_common or _bind()).layer_norm(input, weight, bias, eps)
     if out is not None:

@@ -486,9 +486,9 @@ int fl_embedding_bwd(const void* grad, int64_t grad_stride, const int64_t* index
  * Layer norm over rows of D elements, row_stride apart:
  *   y = (x - mean) / sqrt(variance + eps) * weight + bias
  * with the variance over D.  weight and bias [D] of params_dtype (0 or dtype),
- * either may be NULL; y [rows, D] contiguous, of x's type.  Squares of
- * differences from the mean are held in fp32: rows that spread over more than
- * about 2^63 overflow.
+ * either may be NULL; y [rows, D] contiguous, of x's type.  A row's
+ * elements may be of any size: equal ones give the bias exactly, and only where
+ * one differs from the mean by more than fp32 holds is the row NaN.
  * fl_layer_norm_fwd: stats fp32 [rows, 4] (16-byte aligned) for the backward,
  *   or NULL.
  * fl_layer_norm_bwd: dx [rows, D] contiguous, of x's type; dweight and dbias

@@ -224,9 +224,10 @@ PyObject* expert_order(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!absent(a[2]) && (!plain(a[2], mask) || mask.scalar_type() != at::kBool ||
                           mask.sizes() != index.sizes().slice(0, index.dim() - 1)))
         Py_RETURN_NONE;
-    const int64_t experts = PyLong_AsLongLong(a[1]);
+    int overflow = 0;
+    const int64_t experts = PyLong_AsLongLongAndOverflow(a[1], &overflow);
     if (PyErr_Occurred()) return nullptr;
-    if (experts < 1) Py_RETURN_NONE;
+    if (overflow || experts < 1 || experts > 1024) Py_RETURN_NONE;  // before results of that size are made
     const int64_t T = lead(index), K = last(index);
     Tensor position = make(index, index.sizes(), at::kInt), counts = make(index, {experts});
     Tensor offsets = make(index, {experts + 1}, at::kInt), ws;

@@ -1352,6 +1352,7 @@ def _check_order(index, experts, mask):
     _check(index.dtype == torch.int64 and index.dim() == 2 and index.is_contiguous() and index.shape[1] >= 1,
            "index must be a contiguous int64 tensor (tokens, top)")
     _check(experts >= 1, "num_experts must be at least 1")
+    _check(experts <= 1024, "at most 1024 experts")
     if mask is not None:
         _check(mask.is_cuda and mask.dtype == torch.bool and mask.is_contiguous() and mask.dim() == 1
                and mask.shape[0] == index.shape[0], "mask must be a contiguous CUDA bool tensor (tokens,)")

@@ -135,10 +135,10 @@ def build(verbose: bool = False, jobs: int = 8) -> str:
     with cf.ThreadPoolExecutor(max_workers=max(1, min(jobs, len(srcs) + len(diag_srcs) + len(torch_srcs)))) as ex:
         torch_objs = [ex.submit(_compile_torch, s, verbose) for s in torch_srcs]
         objs = list(ex.map(lambda s: _compile(s, verbose), srcs + diag_srcs))
-        torch_objs = [f.result() for f in torch_objs]
-    _link(objs[:len(srcs)], LIB_PATH, [], verbose)
-    _link(objs[len(srcs):], DIAG_LIB_PATH, [f"-L{PKG_DIR}", "-lfuselse_amd", "-Wl,-rpath,$ORIGIN"], verbose)
-    _link_torch(torch_objs, verbose)
+        # first what needs neither torch nor the host compiler
+        _link(objs[:len(srcs)], LIB_PATH, [], verbose)
+        _link(objs[len(srcs):], DIAG_LIB_PATH, [f"-L{PKG_DIR}", "-lfuselse_amd", "-Wl,-rpath,$ORIGIN"], verbose)
+        _link_torch([f.result() for f in torch_objs], verbose)
     return LIB_PATH
 
 

@@ -3,10 +3,11 @@
 //   out[i] = scale W[id_i];   dW[v] = scale sum_{i: id_i = v} g_i
 //
 // The lookup copies rows and is bound by memory.  The gradient sorts the token
-// ids (stably, so sums always run in the tokens' order and take no atomics), sums
+// ids (stably, so a run's sum is in the tokens' order and takes no atomics), sums
 // runs of equal ids in fp32 and rounds a row once.  A sorted run is cut where it
 // crosses a border of 16 or 64 entries, so a token that comes often is summed by many
-// waves; the pieces are joined in their order.  All of dW is zeroed by further
+// waves; its pieces are joined in an order that their number alone decides (every
+// fourth by a wave, then the waves).  All of dW is zeroed by further
 // blocks of the sort's launches, which leave most of the chip idle: rows that no
 // token takes, most of them where the vocabulary is large, need nothing more, and
 // the time the sort takes is hidden.
@@ -30,7 +31,6 @@ struct LookupArgs {
     const void* w;
     int64_t ldw, V, D;
     const int64_t* index;
-    int64_t n;
     float scale;
     void* out;
     int lanes, steps;
@@ -437,7 +437,7 @@ extern "C" int fl_embedding_fwd(const void* weight, int64_t row_stride, int64_t 
     FL_CHECK(row_stride >= D, "%s: rows of the matrix overlap", name);
     FL_CHECK(weight && index && out, "%s: NULL pointer argument", name);
     FL_CHECK(aligned(weight, dtype) && aligned(out, dtype), "%s: pointers are not element-aligned", name);
-    LookupArgs a{weight, row_stride, V, D, index, N, scale, out, 0, 0, 0, false};
+    LookupArgs a{weight, row_stride, V, D, index, scale, out, 0, 0, 0, false};
     const int nvec = vectors(D, dtype);
     a.lanes = row_lanes(nvec);
     a.steps = row_steps(nvec);

@@ -96,7 +96,7 @@ __global__ __launch_bounds__(key_sort::kThreads) void place_kernel(OrderArgs p) 
 struct RowArgs {
     const void* in;  // x, rows, or dy
     int64_t ldi;
-    int64_t tokens, D, n;  // n = tokens * top rows
+    int64_t D, n;  // n rows, of all tokens' choices
     const int32_t* position;
     int top;
     const void* weights;  // [tokens, top], NULL: 1
@@ -505,7 +505,6 @@ extern "C" int fl_expert_dispatch(const void* x, int64_t row_stride, int64_t tok
     RowArgs a{};
     a.in = x;
     a.ldi = row_stride;
-    a.tokens = tokens;
     a.D = D;
     a.n = tokens * top;
     a.position = position;
@@ -540,7 +539,6 @@ extern "C" int fl_expert_combine(const void* rows, int64_t row_stride, int64_t t
     RowArgs a{};
     a.in = rows;
     a.ldi = row_stride;
-    a.tokens = tokens;
     a.D = D;
     a.n = tokens * top;
     a.position = position;
@@ -583,7 +581,6 @@ extern "C" int fl_expert_combine_bwd(const void* grad, int64_t grad_stride, cons
     RowArgs a{};
     a.in = grad;
     a.ldi = grad_stride;
-    a.tokens = tokens;
     a.D = D;
     a.n = tokens * top;
     a.position = position;

@@ -10,7 +10,7 @@
 // over D, and m1, the mean of the differences to it.  x - m0 - m1 then keeps its
 // digits when the row has a large value in common, which one fp32 mean would take
 // from it.  Lanes meet the same columns in every row and sum dw and db in registers;
-// the blocks' sums are joined in their order.
+// the blocks' sums are joined in an order that their number alone decides.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -639,8 +639,8 @@ __global__ __launch_bounds__(kLong) void dx_long(Args p) {
     }
 }
 
-// A group's rows of 64 vectors of columns: sums of g h and of g, over the waves and
-// then over the groups in their order.  A wave has one row's loads in flight, as the
+// A group's rows of 64 vectors of columns: sums of g h and of g, over the waves; the
+// groups' are joined as blocks' are.  A wave has one row's loads in flight, as the
 // others fill the memory: (16384, 16384) in bf16 184 us, 218 with two or more.
 template <typename T>
 __global__ __launch_bounds__(256) void columns_long(Args p) {

@@ -69,8 +69,8 @@ def embedding(index: torch.Tensor, weight: torch.Tensor, scale: float = 1.0,
     index outside [0, V) gives a row of NaN and no gradient.
 
     The gradient reaches weight, dense: each row the sum of its tokens'
-    gradients in their order, times scale; tokens of padding_idx (negative:
-    from the end) give none.  At most 2^30 tokens and vocabulary entries and
+    gradients, in an order that index alone decides, times scale; tokens of
+    padding_idx (negative: from the end) give none.  At most 2^30 tokens and vocabulary entries and
     2^20 columns.
     """
     padding = -1
@@ -121,10 +121,10 @@ def layer_norm(input: torch.Tensor, weight: Optional[torch.Tensor] = None, bias:
     None; they may be of any of these types and are taken in fp32 where they
     are not of input's.  y = (x - mean) / sqrt(variance + eps) * weight + bias
     in input's type, the variance over D; a value that a row's elements have in
-    common costs no digits, and equal elements give the bias exactly.  Elements
-    may be of any size: only a row in which one differs from the mean by more
-    than fp32 holds is NaN.  Gradients reach all three.  At most 2^31 - 1 rows
-    and 2^24 columns.
+    common costs no digits, and equal elements give the bias exactly (eps 0:
+    NaN).  Elements may be of any size: only a row in which one differs from
+    the mean by more than fp32 holds is NaN.  Gradients reach all three.  At
+    most 2^31 - 1 rows and 2^24 columns.
     """
     out = (_common or _bind()).layer_norm(input, weight, bias, eps)
     if out is not None:

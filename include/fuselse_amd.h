@@ -469,8 +469,8 @@ int fl_router_balance_bwd(const float* grad_balance, const float* grad_z, const 
  * type (exact copies where scale is 1).  An index outside [0, V) gives a row of
  * NaN.
  * fl_embedding_bwd: grad_weight [V, D] contiguous, written in full,
- *   grad_weight[v] = scale * sum of grad[i] over the i of index v, in their
- *   order; 0 for v without any.  Tokens of index `padding` and of indexes
+ *   grad_weight[v] = scale * sum of grad[i] over the i of index v, in an order
+ *   that index alone decides; 0 for v without any.  Tokens of index `padding` and of indexes
  *   outside [0, V) give nothing (a padding outside [0, V): none).  workspace
  *   256-byte aligned.
  * At most 2^30 tokens and vocabulary entries and 2^20 columns (FL_ERANGE).
@@ -487,8 +487,8 @@ int fl_embedding_bwd(const void* grad, int64_t grad_stride, const int64_t* index
  *   y = (x - mean) / sqrt(variance + eps) * weight + bias
  * with the variance over D.  weight and bias [D] of params_dtype (0 or dtype),
  * either may be NULL; y [rows, D] contiguous, of x's type.  A row's
- * elements may be of any size: equal ones give the bias exactly, and only where
- * one differs from the mean by more than fp32 holds is the row NaN.
+ * elements may be of any size: equal ones give the bias exactly (eps 0: NaN),
+ * and only where one differs from the mean by more than fp32 holds is the row NaN.
  * fl_layer_norm_fwd: stats fp32 [rows, 4] (16-byte aligned) for the backward,
  *   or NULL.
  * fl_layer_norm_bwd: dx [rows, D] contiguous, of x's type; dweight and dbias

@@ -17,8 +17,10 @@ Beside it, `step` holds the same pair in autograd's order (the backward on the
 batch its forward just read), with the nt forward and with the keeping
 forward, each also with 512 MB of other traffic between the two.
 
-Prints ONE JSON line on stdout; progress goes to stderr.
-    python bench.py [--gpus 1] [--steps K] [--warmup W] [--no-cpu]
+Prints ONE JSON line on stdout; progress goes to stderr.  Series of many points
+(SERIES) would be most of that line: they are left out of it, and written whole
+with --series.
+    python bench.py [--gpus 1] [--steps K] [--warmup W] [--no-cpu] [--series FILE]
 """
 
 from __future__ import annotations
@@ -37,6 +39,22 @@ BWD_BYTES = 8 * B * N + 8 * B  # read x, g, lse; write grad_x
 METRIC = "fwd+bwd ms/call & HBM GB/s (% peak), fp32 LSE at (512,128256), 1 MI355X"
 ROOT = os.path.dirname(os.path.abspath(__file__))
 TRAFFIC_FILE = os.path.join(ROOT, "profiles", "traffic_lse_f32_c2.json")
+
+
+# Records of other_configs that hold a value for each of many launches, shapes or steps.
+SERIES = ("chain_latency", "microbench_sweep_512xN_u100", "half_rows_cap", "blocktimes_c2", "intlse_phases")
+
+
+def split_series(configs):
+    """(what the line holds of other_configs, the series left out of it)."""
+    if configs is None:
+        return None, {}
+    line = {k: v for k, v in configs.items() if k not in SERIES}
+    sweep = configs.get("microbench_sweep_512xN_u100")
+    if sweep:
+        line["microbench_sweep_512xN_u100"] = {"B": sweep["B"], "data": sweep["data"],
+                                               "fuselse_us": {r["N"]: r["fuselse_us"] for r in sweep["rows"]}}
+    return line, {k: v for k, v in configs.items() if k in SERIES}
 
 
 def log(*a):
@@ -1026,6 +1044,7 @@ def main():
                          "blocktimes, phases, C5) to run alone, "
                          "without the C2 "
                          "step; for profiling passes over one group")
+    ap.add_argument("--series", default=None, metavar="FILE", help="write the series left out of the line here")
     ap.add_argument("--copy-calib", action="store_true",
                     help="also launch one plain 1 GiB device copy (counter calibration runs)")
     args = ap.parse_args()
@@ -1249,6 +1268,11 @@ def main():
     configs = None
     if not args.no_configs:
         configs = measure_configs(torch, ext, dev, stream)
+
+    configs, series = split_series(configs)
+    if args.series:
+        with open(args.series, "w") as f:
+            json.dump(series, f)
 
     cpu = None
     if not args.no_cpu:

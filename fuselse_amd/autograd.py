@@ -35,6 +35,7 @@ of a training step does.
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from .ext import _has_tangent
 
@@ -114,7 +115,7 @@ def make_fuselse_logsumexp(ext, robust: bool = True, half_inputs: bool = False, 
         dtype = input.dtype
         half = dtype in half_fwd
         if not (input.is_cuda and (dtype == torch.float32 or half) and d == nd - 1 and input.shape[-1] >= 2
-                and not _has_tangent(input)):
+                and (forward_ad._current_level < 0 or not _has_tangent(input))):
             return torch_logsumexp(input, dim=dim, keepdim=keepdim)
         if torch.is_grad_enabled() and input.requires_grad:
             out = (_HalfRowLSE if half else _RowLSE).apply(input)
